@@ -371,6 +371,72 @@ SO3LR_B200_API int so3lr_b200_neighbor_list_noalloc(void* stream, int n_atoms, c
                                                     float r_cutoff, int ordered, int32_t* idx_dev, int64_t capacity,
                                                     int64_t* count_dev, int* overflow_dev);
 
+/* ---- attention inside the structures of a packed batch -----------------------------------------------------------------
+ * Operators for a readout on the network's per-atom features (or any rows packed structure by structure): queries and keys
+ * normalised per head and rotated by angles linear in the row's position, and softmax attention over all rows of a
+ * structure.  No counterpart in the reference.  All memory is the caller's; calls enqueue on `stream` of the current device
+ * and keep nothing between calls, so they may overlap and be captured into graphs. */
+
+/* rows of one operand: element (row, head, i) at data + row * row_stride + head * head_stride + i (strides in elements); data
+ * and both strides are multiples of 16 bytes */
+typedef struct {
+  const void* data;
+  int64_t row_stride, head_stride;
+} so3lr_b200_rows;
+
+enum { SO3LR_B200_F32 = 0, SO3LR_B200_BF16 = 1, SO3LR_B200_F16 = 2 };
+
+typedef struct {
+  int n, d, heads_q, heads_k;      /* d: values of a head, a multiple of 16 up to 256; either count of heads may be 0 */
+  int type;                        /* of q, k, their cotangents and all results of their shape */
+  int axes;                        /* of the positions, up to 16; 0: no rotation */
+  int neighbors;                   /* pairs (2p, 2p + 1) instead of (p, p + d / 2) */
+  int norm, weights_f32;           /* weights: float32, or `type` */
+  int positions_f64;               /* positions: float64, or float32 */
+  float eps;
+  const void* positions;           /* (n, axes) contiguous, device */
+  const float* frequencies;        /* (axes, d / 2) contiguous, device */
+  const void *weight_q, *weight_k; /* (d), device */
+} so3lr_b200_norm_rotate_args;
+
+/* y = weight * x / sqrt(mean(x^2) + eps) (norm != 0), pairs of y rotated by theta_p = sum_a positions[a] frequencies[a][p].
+ * out_q (n, heads_q, d), out_k (n, heads_k, d) contiguous. */
+SO3LR_B200_API int so3lr_b200_norm_rotate(void* stream, const so3lr_b200_norm_rotate_args* args, const so3lr_b200_rows* q,
+                                          const so3lr_b200_rows* k, void* out_q, void* out_k);
+/* its transpose for cotangents g_q, g_k; d_positions, d_weight_q, d_weight_k may be NULL (the weights' need the workspace of
+ * so3lr_b200_norm_rotate_workspace(d) bytes).  Results do not depend on the order in which CTAs run. */
+SO3LR_B200_API int64_t so3lr_b200_norm_rotate_workspace(int d);
+SO3LR_B200_API int so3lr_b200_norm_rotate_vjp(void* stream, const so3lr_b200_norm_rotate_args* args, const so3lr_b200_rows* q,
+                                              const so3lr_b200_rows* k, const so3lr_b200_rows* g_q, const so3lr_b200_rows* g_k, void* d_q,
+                                              void* d_k, void* d_positions, void* d_weight_q, void* d_weight_k, void* workspace,
+                                              int64_t workspace_bytes);
+
+/* The layout of a batch: structure s holds rows [start[s], start[s + 1]) of the queries and of the keys (n_structures + 1
+ * ascending entries from 0, host memory).  packing_size returns the int32 words of its image (-1: not ascending, or more
+ * than 2^31 words), packing_build fills it; the caller keeps it on the host and a copy of it on the device.  causal: query i
+ * of lq sees key j of lk where j <= i + lk - lq. */
+SO3LR_B200_API int64_t so3lr_b200_packing_size(int n_structures, const int32_t* start_q, const int32_t* start_kv);
+SO3LR_B200_API int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int32_t* start_kv, int causal, int32_t* image,
+                                            int64_t capacity);
+
+typedef struct {
+  int type, heads_q, heads_kv, d;  /* heads_q a multiple of heads_kv: query head h reads key head h / (heads_q / heads_kv); d as above, to 128 */
+  int64_t rows_q, rows_kv;         /* rows of the arrays, at least those of the layout; rows behind the layout's last are not touched */
+  float scale;                     /* of the logits, positive */
+} so3lr_b200_attention_shape;
+
+/* out (rows_q, heads_q, d) contiguous; lse (heads_q, rows_q) float32 or NULL: logarithm of the sum of exponentials (-inf and
+ * out = 0 for a row without keys).  Values that are not finite spoil the rows of their own structure only. */
+SO3LR_B200_API int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* shape);
+SO3LR_B200_API int so3lr_b200_structure_attention(const int32_t* image, const int32_t* image_dev, void* stream,
+                                                  const so3lr_b200_attention_shape* shape, const so3lr_b200_rows* q, const so3lr_b200_rows* k,
+                                                  const so3lr_b200_rows* v, void* out, float* lse, void* workspace, int64_t workspace_bytes);
+/* gradients for the cotangent g of out; delta (heads_q, rows_q) float32 is scratch; d_q, d_k, d_v contiguous */
+SO3LR_B200_API int so3lr_b200_structure_attention_vjp(const int32_t* image, const int32_t* image_dev, void* stream,
+                                                      const so3lr_b200_attention_shape* shape, const so3lr_b200_rows* q,
+                                                      const so3lr_b200_rows* k, const so3lr_b200_rows* v, const void* out, const float* lse,
+                                                      const so3lr_b200_rows* g, float* delta, void* d_q, void* d_k, void* d_v);
+
 /* Host-callable pieces of the device math, exported for the CPU tests (no GPU needed). */
 /* 64-bit total of a device array of per-row pair counts, formed the way the list builder forms it ahead of its 32-bit
  * offset scan; returns SO3LR_B200_TOO_LARGE when the offsets of such a list would leave the int32 range (the builder then

@@ -24,6 +24,20 @@ class Options(C.Structure):
                 ("lr_list_cutoff", C.c_float)]
 
 
+class Rows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class NormRotateArgs(C.Structure):
+    _fields_ = [(k, C.c_int) for k in ("n", "d", "heads_q", "heads_k", "type", "axes", "neighbors", "norm", "weights_f32", "positions_f64")] + [
+        ("eps", C.c_float), ("positions", C.c_void_p), ("frequencies", C.c_void_p), ("weight_q", C.c_void_p), ("weight_k", C.c_void_p)]
+
+
+class AttentionShape(C.Structure):
+    _fields_ = [("type", C.c_int), ("heads_q", C.c_int), ("heads_kv", C.c_int), ("d", C.c_int), ("rows_q", C.c_int64), ("rows_kv", C.c_int64),
+                ("scale", C.c_float)]
+
+
 def _load():
     if not os.path.exists(LIB_PATH):
         raise ImportError(
@@ -83,6 +97,14 @@ def _load():
         "so3lr_b200_system_profile_read": (i32, [p, i32, p, p, p]),
         "so3lr_b200_neighbor_list_noalloc": (i32, [p, i32, p, p, f32, i32, p, i64, p, p]),
         "so3lr_b200_list_row_total": (i32, [p, p, i32, C.POINTER(i64)]),
+        "so3lr_b200_norm_rotate": (i32, [p, p, p, p, p, p]),
+        "so3lr_b200_norm_rotate_workspace": (i64, [i32]),
+        "so3lr_b200_norm_rotate_vjp": (i32, [p] * 12 + [i64]),
+        "so3lr_b200_packing_size": (i64, [i32, p, p]),
+        "so3lr_b200_packing_build": (i32, [i32, p, p, i32, p, i64]),
+        "so3lr_b200_structure_attention_workspace": (i64, [p, p]),
+        "so3lr_b200_structure_attention": (i32, [p] * 10 + [i64]),
+        "so3lr_b200_structure_attention_vjp": (i32, [p] * 14),
         "so3lr_b200_host_fail_allocation": (i64, [i64, i32]),
         "so3lr_b200_host_sph_harm": (None, [f32, f32, f32, p]),
         "so3lr_b200_host_sph_harm_vjp": (None, [f32, f32, f32, p, p]),

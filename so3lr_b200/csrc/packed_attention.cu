@@ -1,0 +1,227 @@
+// Attention inside the structures of a packed batch: the work items of a batch's layout, and which kernels a call runs.
+#include "packed_attention.h"
+
+#include "../../include/so3lr_b200.h"
+
+#include <algorithm>
+#include <cmath>
+#include <new>
+#include <vector>
+
+#include "kernels.h"
+
+namespace so3lr {
+namespace {
+
+// The image of a layout (int32): a header, the offsets of both sides, and tables of work items {structure, tile, first, last}.
+enum Head : int { kMagicAt, kN, kCausal, kRowsQ, kRowsKv, kMaxQ, kStartQ, kStartKv, kItemsQ, kNItemsQ, kItemsKv, kNItemsKv, kItemsSplit, kNItemsSplit,
+                  kSplitFirst, kCombine, kTotal, kHeadInts = 32 };
+constexpr int kMagic = 0x53334c50;
+
+int64_t align4(int64_t x) { return (x + 3) & ~3LL; }
+
+// Stretches of the keys in the form for few queries.  A stretch of 512 keys is long enough that its CTA's start costs little; with few
+// keys in all, shorter ones give every SM two.
+int split_length(int64_t keys) {
+  const int64_t want = (keys + 295) / 296;
+  return (int)std::min<int64_t>(512, std::max<int64_t>(64, (want + 63) / 64 * 64));
+}
+
+struct Counts { int64_t q = 0, kv = 0, split = 0, total = 0; };
+
+bool valid(int n, const int32_t* sq, const int32_t* sk) {
+  if (n < 0 || !sq || !sk || sq[0] != 0 || sk[0] != 0) return false;
+  for (int i = 0; i < n; ++i) if (sq[i + 1] < sq[i] || sk[i + 1] < sk[i]) return false;
+  return true;
+}
+
+Counts count(int n, const int32_t* sq, const int32_t* sk) {
+  Counts c;
+  const int chunk = split_length(sk[n]);
+  for (int i = 0; i < n; ++i) {
+    const int64_t lq = sq[i + 1] - sq[i], lk = sk[i + 1] - sk[i];
+    c.q += (lq + kPackTile - 1) / kPackTile;
+    c.kv += (lk + kPackTile - 1) / kPackTile;
+    if (lq > 0) c.split += std::max<int64_t>(1, (lk + chunk - 1) / chunk);
+  }
+  c.total = kHeadInts + 2 * align4(n + 1) + 4 * (c.q + c.kv + c.split) + align4(n + 1);
+  return c;
+}
+
+struct Item { int32_t s, tile, first, last; };
+
+void put(int32_t* at, std::vector<Item>& items) {
+  // the longest first, so that what is left at the end is short
+  std::stable_sort(items.begin(), items.end(), [](const Item& a, const Item& b) { return a.last - a.first > b.last - b.first; });
+  for (size_t i = 0; i < items.size(); ++i) { at[4 * i] = items[i].s; at[4 * i + 1] = items[i].tile; at[4 * i + 2] = items[i].first; at[4 * i + 3] = items[i].last; }
+}
+
+void build_image(int n, const int32_t* sq, const int32_t* sk, bool causal, int32_t* im) {
+  const Counts c = count(n, sq, sk);
+  std::fill(im, im + c.total, 0);
+  int max_q = 0;
+  im[kMagicAt] = kMagic; im[kN] = n; im[kCausal] = causal; im[kRowsQ] = sq[n]; im[kRowsKv] = sk[n];
+  im[kStartQ] = kHeadInts; im[kStartKv] = (int32_t)(kHeadInts + align4(n + 1));
+  im[kItemsQ] = (int32_t)(kHeadInts + 2 * align4(n + 1)); im[kNItemsQ] = (int32_t)c.q;
+  im[kItemsKv] = (int32_t)(im[kItemsQ] + 4 * c.q); im[kNItemsKv] = (int32_t)c.kv;
+  im[kItemsSplit] = (int32_t)(im[kItemsKv] + 4 * c.kv); im[kNItemsSplit] = (int32_t)c.split;
+  im[kSplitFirst] = (int32_t)(im[kItemsSplit] + 4 * c.split); im[kTotal] = (int32_t)c.total;
+  std::copy(sq, sq + n + 1, im + im[kStartQ]);
+  std::copy(sk, sk + n + 1, im + im[kStartKv]);
+  std::vector<Item> q, kv;
+  q.reserve(c.q); kv.reserve(c.kv);
+  const int chunk = split_length(sk[n]);
+  int32_t* split = im + im[kItemsSplit];
+  int at = 0, combine = 0;
+  for (int s = 0; s < n; ++s) {
+    const int lq = sq[s + 1] - sq[s], lk = sk[s + 1] - sk[s], off = lk - lq;
+    max_q = std::max(max_q, lq);
+    for (int t = 0; (int64_t)t * kPackTile < lq; ++t) {
+      const int64_t end = causal ? std::min<int64_t>(lk, std::max<int64_t>(0, std::min<int64_t>(lq, (t + 1LL) * kPackTile) + off)) : lk;
+      q.push_back({s, t, 0, (int32_t)end});
+    }
+    for (int t = 0; (int64_t)t * kPackTile < lk; ++t) {
+      const int64_t first = causal ? std::min<int64_t>(lq, std::max<int64_t>(0, (int64_t)t * kPackTile - off)) : 0;
+      kv.push_back({s, t, (int32_t)first, lq});
+    }
+    im[im[kSplitFirst] + s] = at;
+    if (lq > 0) {
+      const int pieces = std::max(1, (lk + chunk - 1) / chunk);
+      if (pieces > 1) combine = 1;
+      for (int p = 0; p < pieces; ++p, ++at) {
+        split[4 * at] = s; split[4 * at + 1] = pieces;
+        split[4 * at + 2] = p * chunk; split[4 * at + 3] = (int32_t)std::min<int64_t>(lk, (int64_t)(p + 1) * chunk);
+      }
+    }
+  }
+  im[im[kSplitFirst] + n] = at;
+  im[kMaxQ] = max_q; im[kCombine] = combine;
+  put(im + im[kItemsQ], q);
+  put(im + im[kItemsKv], kv);
+}
+
+bool rows_ok(const so3lr_b200_rows* r, int type) {
+  const long long unit = type == kF32 ? 4 : 8;
+  return r && r->data && reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride % unit == 0 && r->head_stride % unit == 0;
+}
+Rows rows_of(const so3lr_b200_rows* r) { return {r->data, r->row_stride, r->head_stride}; }
+
+bool shape_ok(const int32_t* im, const so3lr_b200_attention_shape* a) {
+  return im && im[kMagicAt] == kMagic && a && a->type >= 0 && a->type <= 2 && a->heads_q > 0 && a->heads_kv > 0 && a->heads_q % a->heads_kv == 0 &&
+         a->heads_q <= 65535 && a->d >= 16 && a->d <= 128 && a->d % 16 == 0 && a->rows_q >= im[kRowsQ] && a->rows_q < 0x7fffffff && a->rows_kv >= im[kRowsKv] &&
+         a->scale > 0.f && std::isfinite(a->scale);
+}
+
+PackedArgs common(const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a) {
+  PackedArgs p;
+  p.start_q = dev + im[kStartQ]; p.start_kv = dev + im[kStartKv]; p.split_first = dev + im[kSplitFirst];
+  p.nq = (int)a->rows_q; p.hq = a->heads_q; p.hk = a->heads_kv; p.group = a->heads_q / a->heads_kv; p.d = a->d; p.causal = im[kCausal];
+  p.scale = a->scale; p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
+  return p;
+}
+
+// Few queries: the heads of a group share one tile of rows with their token, and the keys are cut into stretches.  The keys are then
+// read once per group and not once per head.
+bool few_rows(const int32_t* im, const so3lr_b200_attention_shape* a) {
+  return (int64_t)im[kMaxQ] * (a->heads_q / a->heads_kv) <= kPackTile;
+}
+int64_t part_floats(const int32_t* im, const so3lr_b200_attention_shape* a) {
+  return (int64_t)im[kNItemsSplit] * a->heads_kv * im[kMaxQ] * (a->heads_q / a->heads_kv) * packed_padded(a->d);
+}
+
+template <typename T>
+void forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
+  if (few_rows(im, a)) {
+    p.items = reinterpret_cast<const int4*>(dev + im[kItemsSplit]);
+    p.part_rows = im[kMaxQ] * p.group;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + part_floats(im, a));
+    packed_forward_split<T>(st, p, im[kNItemsSplit], im[kN], im[kCombine]);
+    return;
+  }
+  p.items = reinterpret_cast<const int4*>(dev + im[kItemsQ]);
+  packed_forward_mma<T>(st, p, im[kNItemsQ]);
+}
+
+template <typename T>
+void reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev) {
+  packed_delta<T>(st, p, im[kRowsQ]);
+  p.items = reinterpret_cast<const int4*>(dev + im[kItemsQ]);
+  if (im[kNItemsQ]) packed_dq_mma<T>(st, p, im[kNItemsQ]);
+  p.items = reinterpret_cast<const int4*>(dev + im[kItemsKv]);
+  if (im[kNItemsKv]) packed_dkv_mma<T>(st, p, im[kNItemsKv]);
+}
+
+}  // namespace
+}  // namespace so3lr
+
+using namespace so3lr;
+
+extern "C" {
+
+int64_t so3lr_b200_packing_size(int n_structures, const int32_t* start_q, const int32_t* start_kv) {
+  if (!valid(n_structures, start_q, start_kv)) return -1;
+  const int64_t total = count(n_structures, start_q, start_kv).total;
+  return total < 0x7fffffff ? total : -1;
+}
+
+int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int32_t* start_kv, int causal, int32_t* image, int64_t capacity) {
+  const int64_t need = so3lr_b200_packing_size(n_structures, start_q, start_kv);
+  if (need < 0 || !image || capacity < need) return kInvalidArgument;
+  try {
+    build_image(n_structures, start_q, start_kv, causal != 0, image);
+  } catch (const std::bad_alloc&) {
+    return kTooLarge;
+  }
+  return kOk;
+}
+
+int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* a) {
+  if (!shape_ok(image, a)) return -1;
+  if (!few_rows(image, a) || !image[kCombine]) return 0;
+  return part_floats(image, a) * (int64_t)sizeof(float) + part_floats(image, a) / packed_padded(a->d) * (int64_t)sizeof(float2);
+}
+
+int so3lr_b200_structure_attention(const int32_t* image, const int32_t* image_dev, void* stream, const so3lr_b200_attention_shape* a,
+                                   const so3lr_b200_rows* q, const so3lr_b200_rows* k, const so3lr_b200_rows* v, void* out, float* lse,
+                                   void* workspace, int64_t workspace_bytes) {
+  if (!shape_ok(image, a) || !image_dev) return kInvalidArgument;
+  if (image[kRowsQ] == 0) return kOk;
+  if (!rows_ok(q, a->type) || (image[kRowsKv] && (!rows_ok(k, a->type) || !rows_ok(v, a->type))) || !out) return kInvalidArgument;
+  const int64_t need = so3lr_b200_structure_attention_workspace(image, a);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return kInvalidArgument;
+  PackedArgs p = common(image, image_dev, a);
+  p.q = rows_of(q);
+  if (image[kRowsKv]) { p.k = rows_of(k); p.v = rows_of(v); } else { p.k = p.v = p.q; }   // never read: no structure has keys
+  p.out = out; p.lse = lse;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->type == kBF16) forward<__nv_bfloat16>(st, p, image, image_dev, a, workspace);
+  else if (a->type == kF16) forward<__half>(st, p, image, image_dev, a, workspace);
+  else forward<float>(st, p, image, image_dev, a, workspace);
+  SO3LR_CUDA_CHECK(cudaGetLastError());
+  return kOk;
+}
+
+int so3lr_b200_structure_attention_vjp(const int32_t* image, const int32_t* image_dev, void* stream, const so3lr_b200_attention_shape* a,
+                                       const so3lr_b200_rows* q, const so3lr_b200_rows* k, const so3lr_b200_rows* v, const void* out,
+                                       const float* lse, const so3lr_b200_rows* g, float* delta, void* d_q, void* d_k, void* d_v) {
+  if (!shape_ok(image, a) || !image_dev) return kInvalidArgument;
+  if (image[kRowsQ] == 0 && image[kRowsKv] == 0) return kOk;
+  if ((image[kRowsQ] && (!rows_ok(q, a->type) || !rows_ok(g, a->type) || !out || !lse || !delta || !d_q)) ||
+      (image[kRowsKv] && (!rows_ok(k, a->type) || !rows_ok(v, a->type) || !d_k || !d_v)))
+    return kInvalidArgument;
+  PackedArgs p = common(image, image_dev, a);
+  if (image[kRowsQ]) { p.q = rows_of(q); p.g = rows_of(g); }
+  if (image[kRowsKv]) { p.k = rows_of(k); p.v = rows_of(v); }
+  if (!image[kRowsQ]) p.q = p.g = p.k;      // never read: one side has no rows
+  if (!image[kRowsKv]) p.k = p.v = p.q;
+  p.o.p = out; p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = d_q; p.dk = d_k; p.dv = d_v;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->type == kBF16) reverse<__nv_bfloat16>(st, p, image, image_dev);
+  else if (a->type == kF16) reverse<__half>(st, p, image, image_dev);
+  else reverse<float>(st, p, image, image_dev);
+  SO3LR_CUDA_CHECK(cudaGetLastError());
+  return kOk;
+}
+
+}  // extern "C"

@@ -1,0 +1,52 @@
+// Attention inside the structures of a packed batch: arguments shared by its kernels (packed_mma.cuh, packed_tc.cu) and its host side
+// (packed_attention.cu).
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "common.cuh"
+
+namespace so3lr {
+
+enum ValueType : int { kF32 = 0, kBF16 = 1, kF16 = 2 };
+
+// Rows of a strided operand: element (row, head, 0) lies at p + row * row_stride + head * head_stride (in elements), its d values
+// contiguous; p and both strides are multiples of 16 bytes.
+struct Rows {
+  const void* p = nullptr;
+  long long row = 0, head = 0;
+};
+
+struct PackedArgs {
+  Rows q, k, v, g, o;           // g: cotangent of the output; o: the output (reverse pass)
+  void* out = nullptr;          // (nq, hq, d) contiguous
+  float* lse = nullptr;         // (hq, nq) natural logarithm of the sum of exponentials; -inf for a row without keys
+  float* delta = nullptr;       // (hq, nq) sum over d of g * o
+  void *dq = nullptr, *dk = nullptr, *dv = nullptr;   // contiguous
+  const int *start_q = nullptr, *start_kv = nullptr;
+  // one work item per CTA and head: {structure, tile, first, last}; [first, last) are the rows of the other side that the tile meets
+  const int4* items = nullptr;
+  const int* split_first = nullptr;                   // items of structure s: [split_first[s], split_first[s + 1])
+  float* part_o = nullptr;      // (item, hk, part_rows, DP) of the split form
+  float2* part_ml = nullptr;    // (item, hk, part_rows): running maximum (in units of log2) and sum
+  int part_rows = 0;            // most rows of a structure: tokens times heads of a group
+  int nq = 0, hq = 0, hk = 0, group = 1, d = 0, causal = 0;
+  float scale = 0.f, scale_log2 = 0.f;                // scale * log2(e): the softmax runs on powers of two
+  int* err = nullptr;
+};
+
+constexpr int kPackTile = 64;   // rows of a tile of the mma kernels
+
+// kernels on the warp-level matrix instructions, one translation unit per type
+template <typename T> void packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> void packed_forward_split(cudaStream_t st, const PackedArgs& a, int n_items, int n_structures, bool combine);
+template <typename T> void packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> void packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> void packed_delta(cudaStream_t st, const PackedArgs& a, int rows);
+
+inline int packed_padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
+
+}  // namespace so3lr

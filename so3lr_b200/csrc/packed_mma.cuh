@@ -1,0 +1,583 @@
+// Attention inside the structures of a packed batch on the warp-level matrix instructions: forward, its form split over the keys, and the
+// two halves of the reverse pass, for float32, bfloat16 and float16 and up to 128 values a head.
+//
+//   s_ij = scale q_i . k_j,  o_i = sum_j exp(s_ij - lse_i) v_j            one pass over the keys with a running maximum m and sum l:
+//   a tile of keys raises m to m', o and l are scaled by exp(m - m') and the tile's share is added; o / l at the end.
+//   reverse: P_ij = exp(s_ij - lse_i), dP_ij = g_i . v_j, dS_ij = P_ij (dP_ij - delta_i), delta_i = g_i . o_i,
+//   dq_i = scale sum_j dS_ij k_j     (a CTA per tile of queries, walking over the keys)
+//   dk_j = scale sum_i dS_ij q_i,  dv_j = sum_i P_ij g_i   (a CTA per tile of keys, walking over the queries of all heads of its group)
+// Two kernels form the exponentials twice, but every sum has one owner: no atomics, results do not change from run to run, and the
+// gradients of shared keys need no second pass.
+//
+// A CTA has four warps with 16 rows each; the tile of the other side is double-buffered by 16-byte asynchronous copies that fill rows and
+// columns that are not there with zeros.  The accumulator fragment of one product is the A fragment of the next, so P and dS never leave
+// the registers (and are rounded to the inputs' type on the way into the second product: their error then is that of one rounding of an
+// input).  float32 runs as three products of operands split into two tf32 numbers each (hi hi + hi lo + lo hi): 2^-21 of the
+// product, where a single tf32 product has 2^-11.
+#pragma once
+#include <type_traits>
+
+#include "packed_attention.h"
+
+namespace so3lr {
+namespace packed {
+
+constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+// 16 bytes, or zeros where `ok` is false
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t* r) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, const uint32_t* b) {
+  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ void tf32_split(float x, uint32_t& hi, uint32_t& lo) {
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
+  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+}
+
+template <typename T> struct Half;
+// float16 keeps its 11 bits down to 2^-14 only, and a normalised probability over thousands of keys lies there: the reverse kernels form
+// 2^15 P (at most 2^15 < 65504, exact, no instruction more) and take the factor out of dv at the end and out of dP - delta.
+template <typename T> constexpr float prob_shift() { return std::is_same<T, __half>::value ? 15.f : 0.f; }
+template <typename T> constexpr float prob_unscale() { return std::is_same<T, __half>::value ? 1.f / 32768.f : 1.f; }
+template <> struct Half<__nv_bfloat16> {
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
+  static __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+  }
+};
+template <> struct Half<__half> {
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+  static __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+  }
+};
+
+// Tiles in shared memory: rows of DP values plus 16 bytes, which puts the 16-byte pieces of eight consecutive rows into different banks.
+template <typename T, int DP> struct Tile {
+  static constexpr int kStride = DP * (int)sizeof(T) + 16;   // bytes
+  static constexpr int kChunks = DP * (int)sizeof(T) / 16;
+  static constexpr int kPer = 16 / (int)sizeof(T);           // values of a chunk
+};
+
+// rows [r0, r0 + N) of one head into a tile; row r is there where r < r1
+template <typename T, int DP, int N>
+__device__ __forceinline__ void load_rows(uint32_t tile, const Rows& src, int head, long long base, int r0, int r1, int d, int tid) {
+  using L = Tile<T, DP>;
+  const T* p = static_cast<const T*>(src.p) + head * src.head;
+#pragma unroll
+  for (int i = tid; i < N * L::kChunks; i += 128) {
+    const int r = i / L::kChunks, c = i % L::kChunks;
+    const bool ok = r0 + r < r1 && c * L::kPer < d;
+    copy16(tile + r * L::kStride + c * 16, ok ? p + (base + r0 + r) * src.row + c * L::kPer : p, ok);
+  }
+}
+
+// ---- products of a warp's 16 rows -----------------------------------------------------------------------------------
+// acc[16 x 8 NT] += A[16 x DP] B[8 NT x DP]^T, A at `a` (the warp's first row), B at `b`
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void product_nt(float (&acc)[NT][4], uint32_t a, uint32_t b, int lane) {
+  using L = Tile<T, DP>;
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t al = a + (lane & 15) * L::kStride + (lane >> 4) * 16;
+    const uint32_t bl = b + ((lane & 7) + ((lane >> 4) << 3)) * L::kStride + ((lane >> 3) & 1) * 16;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) {
+      uint32_t fa[4];
+      ldsm4(al + ks * 32, fa);
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        uint32_t fb[4];
+        ldsm4(bl + n * 8 * L::kStride + ks * 32, fb);
+        Half<T>::mma(acc[n], fa, fb);
+        Half<T>::mma(acc[n + 1], fa, fb + 2);
+      }
+    }
+  } else {
+    const uint32_t al = a + (lane & 15) * L::kStride + (lane >> 4) * 16;
+    const uint32_t bl = b + ((lane & 7) + ((lane >> 4) << 3)) * L::kStride + ((lane >> 3) & 1) * 16;
+#pragma unroll 4
+    for (int ks = 0; ks < DP / 8; ++ks) {
+      uint32_t fa[4], ah[4], alo[4];
+      ldsm4(al + ks * 32, fa);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) tf32_split(__uint_as_float(fa[i]), ah[i], alo[i]);
+#pragma unroll
+      for (int n = 0; n < NT; n += 2) {
+        uint32_t fb[4], bh[4], blo[4];
+        ldsm4(bl + n * 8 * L::kStride + ks * 32, fb);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tf32_split(__uint_as_float(fb[i]), bh[i], blo[i]);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          mma_tf32(acc[n + h], alo, bh + 2 * h);
+          mma_tf32(acc[n + h], ah, blo + 2 * h);
+          mma_tf32(acc[n + h], ah, bh + 2 * h);
+        }
+      }
+    }
+  }
+}
+
+// acc[16 x DP] += A[16 x 8 NT] B[8 NT x DP], A the accumulator fragments of an earlier product
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void product_nn(float (&acc)[DP / 8][4], const float (&p)[NT][4], uint32_t b, int lane) {
+  using L = Tile<T, DP>;
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t bl = b + (lane & 15) * L::kStride + (lane >> 4) * 16;
+#pragma unroll
+    for (int j = 0; j < NT / 2; ++j) {
+      const uint32_t fa[4] = {Half<T>::pack(p[2 * j][0], p[2 * j][1]), Half<T>::pack(p[2 * j][2], p[2 * j][3]),
+                              Half<T>::pack(p[2 * j + 1][0], p[2 * j + 1][1]), Half<T>::pack(p[2 * j + 1][2], p[2 * j + 1][3])};
+#pragma unroll
+      for (int n = 0; n < DP / 8; n += 2) {
+        uint32_t fb[4];
+        ldsm4t(bl + j * 16 * L::kStride + n * 16, fb);
+        Half<T>::mma(acc[n], fa, fb);
+        Half<T>::mma(acc[n + 1], fa, fb + 2);
+      }
+    }
+  } else {
+    // the order of the contracted index is free: position t stands for column 2 t, position t + 4 for column 2 t + 1, which is how the
+    // accumulator fragment holds them; B follows (rows 2 t and 2 t + 1: banks 8 t + g, all different)
+    const uint32_t bl = b + 2 * (lane & 3) * L::kStride + (lane >> 2) * 4;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      uint32_t ah[4], alo[4];
+      tf32_split(p[j][0], ah[0], alo[0]); tf32_split(p[j][2], ah[1], alo[1]);
+      tf32_split(p[j][1], ah[2], alo[2]); tf32_split(p[j][3], ah[3], alo[3]);
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) {
+        float x, y;
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(bl + j * 8 * L::kStride + n * 32) : "memory");
+        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(bl + (j * 8 + 1) * L::kStride + n * 32) : "memory");
+        uint32_t bh[2], blo[2];
+        tf32_split(x, bh[0], blo[0]); tf32_split(y, bh[1], blo[1]);
+        mma_tf32(acc[n], alo, bh);
+        mma_tf32(acc[n], ah, blo);
+        mma_tf32(acc[n], ah, bh);
+      }
+    }
+  }
+}
+
+// the warp's accumulators (rows g and g + 8 of its 16, columns 8 n + 2 t, + 1) times `f` to a contiguous destination
+template <typename T>
+__device__ __forceinline__ void store2(T* p, float x, float y) {
+  if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(p) = Half<T>::pack(x, y);
+  else *reinterpret_cast<float2*>(p) = make_float2(x, y);
+}
+
+template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 4 && DP > 64 ? 32 : 64; }
+template <typename T, int DP> constexpr int forward_smem() { return (kPackTile + 4 * key_tile<T, DP>()) * Tile<T, DP>::kStride; }
+constexpr int kRevTile = 32;   // rows of the walked side in the reverse kernels: two accumulators of 16 x DP are held at the same time
+template <typename T, int DP> constexpr int reverse_smem() { return (2 * kPackTile + 4 * kRevTile) * Tile<T, DP>::kStride + 4 * kRevTile * 4; }
+
+// ---- forward --------------------------------------------------------------------------------------------------------
+// SPLIT: rows are (token, head of the group) of ONE key head, a structure has at most 64 of them, and the item is a stretch of the keys;
+// what it finds is joined by combine_kernel, or written where the structure has one stretch only.
+template <typename T, int DP, bool SPLIT>
+__global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
+  using L = Tile<T, DP>;
+  constexpr int BN = key_tile<T, DP>(), NT = BN / 8;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const uint32_t sq = smem_addr(smem), sk = sq + kPackTile * L::kStride, sv = sk + 2 * BN * L::kStride;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int4 item = a.items[blockIdx.x];
+  const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
+  const int G = SPLIT ? a.group : 1, hy = blockIdx.y, kvh = SPLIT ? hy : hy / a.group;
+  const int rows = lq * G, row0 = SPLIT ? 0 : item.y * kPackTile;
+  const int k0 = item.z, k1 = item.w;
+  const int nt = (max(k1 - k0, 0) + BN - 1) / BN;
+
+  {  // queries
+    const T* p = static_cast<const T*>(a.q.p);
+#pragma unroll 4
+    for (int i = tid; i < kPackTile * L::kChunks; i += 128) {
+      const int r = i / L::kChunks, c = i % L::kChunks, pr = row0 + r;
+      const bool ok = pr < rows && c * L::kPer < a.d;
+      const int tok = SPLIT ? pr / G : pr, head = SPLIT ? hy * G + pr % G : hy;
+      copy16(sq + r * L::kStride + c * 16, ok ? p + (long long)(q0 + tok) * a.q.row + head * a.q.head + c * L::kPer : p, ok);
+    }
+  }
+  auto load = [&](int it) {
+    if (it < nt) {
+      const int buf = it & 1, b = k0 + it * BN;
+      load_rows<T, DP, BN>(sk + buf * BN * L::kStride, a.k, kvh, c0, b, k1, a.d, tid);
+      load_rows<T, DP, BN>(sv + buf * BN * L::kStride, a.v, kvh, c0, b, k1, a.d, tid);
+    }
+    copy_commit();
+  };
+  load(0);
+
+  const int wr = row0 + warp * 16, ra = wr + (lane >> 2), rb = ra + 8;      // this thread's two rows
+  // last key that a row sees
+  const int off = lk - lq, big = 0x7fffffff;
+  const int lim_a = a.causal ? (SPLIT ? ra / G : ra) + off : big, lim_b = a.causal ? (SPLIT ? rb / G : rb) + off : big;
+  const int lim_lo = a.causal ? (SPLIT ? wr / G : wr) + off : big, lim_hi = a.causal ? (SPLIT ? (wr + 15) / G : wr + 15) + off : big;
+  float o[DP / 8][4];
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+  for (int it = 0; it < nt; ++it) {
+    load(it + 1);
+    copy_wait<1>();
+    __syncthreads();
+    const int kb = k0 + it * BN, buf = it & 1;
+    if (wr < rows && kb <= lim_hi) {
+      float p[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) p[n][0] = p[n][1] = p[n][2] = p[n][3] = 0.f;
+      product_nt<T, DP, NT>(p, sq + warp * 16 * L::kStride, sk + buf * BN * L::kStride, lane);
+      if (kb + BN > k1 || kb + BN - 1 > lim_lo) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int j = kb + n * 8 + 2 * (lane & 3) + e;
+            if (j >= k1 || j > lim_a) p[n][e] = -INFINITY;
+            if (j >= k1 || j > lim_b) p[n][2 + e] = -INFINITY;
+          }
+        }
+      }
+      float xa = p[0][0], xb = p[0][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) { xa = fmaxf(xa, fmaxf(p[n][0], p[n][1])); xb = fmaxf(xb, fmaxf(p[n][2], p[n][3])); }
+#pragma unroll
+      for (int x = 1; x < 4; x <<= 1) { xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, x)); xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, x)); }
+      const float na = fmaxf(ma, xa * a.scale_log2), nb = fmaxf(mb, xb * a.scale_log2);
+      const float ua = na == -INFINITY ? 0.f : na, ub = nb == -INFINITY ? 0.f : nb;   // nothing seen yet: every exponential is exp(-inf)
+      const float fa = exp2f(ma - ua), fb = exp2f(mb - ub);
+      ma = na; mb = nb;
+      float ta = 0.f, tb = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        p[n][0] = exp2f(fmaf(p[n][0], a.scale_log2, -ua)); p[n][1] = exp2f(fmaf(p[n][1], a.scale_log2, -ua));
+        p[n][2] = exp2f(fmaf(p[n][2], a.scale_log2, -ub)); p[n][3] = exp2f(fmaf(p[n][3], a.scale_log2, -ub));
+        ta += p[n][0] + p[n][1]; tb += p[n][2] + p[n][3];
+      }
+      la = fmaf(la, fa, ta); lb = fmaf(lb, fb, tb);
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) { o[n][0] *= fa; o[n][1] *= fa; o[n][2] *= fb; o[n][3] *= fb; }
+      product_nn<T, DP, NT>(o, p, sv + buf * BN * L::kStride, lane);
+    }
+    __syncthreads();
+  }
+  copy_wait<0>();
+  if (wr >= rows) return;
+#pragma unroll
+  for (int x = 1; x < 4; x <<= 1) { la += __shfl_xor_sync(0xffffffffu, la, x); lb += __shfl_xor_sync(0xffffffffu, lb, x); }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int pr = half ? rb : ra;
+    if (pr >= rows) continue;
+    const float m = half ? mb : ma, l = half ? lb : la;
+    if (SPLIT && item.y > 1) {
+      const size_t slot = ((size_t)blockIdx.x * a.hk + hy) * a.part_rows + pr;
+      float* dst = a.part_o + slot * DP + 2 * (lane & 3);
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+      if ((lane & 3) == 0) a.part_ml[slot] = make_float2(m, l);
+      continue;
+    }
+    const int tok = SPLIT ? pr / G : pr, head = SPLIT ? hy * G + pr % G : hy;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);               // a row without keys gives zero; NaN stays NaN
+    T* dst = static_cast<T*>(a.out) + ((long long)(q0 + tok) * a.hq + head) * a.d;
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) {
+      const int c = n * 8 + 2 * (lane & 3);
+      if (c < a.d) store2(dst + c, o[n][2 * half] * inv, o[n][2 * half + 1] * inv);
+    }
+    if ((lane & 3) == 0 && a.lse) a.lse[(long long)head * a.nq + q0 + tok] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+  }
+}
+
+// joins the stretches of a structure's keys: a warp per row of the split form
+template <typename T, int DP>
+__global__ void __launch_bounds__(256) combine_kernel(const PackedArgs a) {
+  const int s = blockIdx.x, hy = blockIdx.y, lane = threadIdx.x & 31;
+  const int first = a.split_first[s], n = a.split_first[s + 1] - first;
+  const int q0 = a.start_q[s], rows = (a.start_q[s + 1] - q0) * a.group;
+  if (n <= 1) return;
+  for (int pr = threadIdx.x >> 5; pr < rows; pr += 8) {
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, a.part_ml[((size_t)(first + i) * a.hk + hy) * a.part_rows + pr].x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    const float u = m == -INFINITY ? 0.f : m;
+    float l = 0.f, o[DP / 32];
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c) o[c] = 0.f;
+    for (int i = 0; i < n; ++i) {
+      const size_t slot = ((size_t)(first + i) * a.hk + hy) * a.part_rows + pr;
+      const float2 ml = a.part_ml[slot];
+      const float f = exp2f(ml.x - u);
+      l = fmaf(ml.y, f, l);
+#pragma unroll
+      for (int c = 0; c < DP / 32; ++c) o[c] = fmaf(a.part_o[slot * DP + c * 32 + lane], f, o[c]);
+    }
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const int tok = pr / a.group, head = hy * a.group + pr % a.group;
+    T* dst = static_cast<T*>(a.out) + ((long long)(q0 + tok) * a.hq + head) * a.d;
+#pragma unroll
+    for (int c = 0; c < DP / 32; ++c)
+      if (c * 32 + lane < a.d) dst[c * 32 + lane] = (T)(o[c] * inv);
+    if (lane == 0 && a.lse) a.lse[(long long)head * a.nq + q0 + tok] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+  }
+}
+
+// ---- reverse --------------------------------------------------------------------------------------------------------
+// delta = sum over d of g * o, a thread per 16 bytes, rows of all heads
+template <typename T>
+__global__ void __launch_bounds__(256) delta_kernel(const PackedArgs a, int rows, int width) {
+  constexpr int V = 16 / (int)sizeof(T);
+  const int part = threadIdx.x % width;
+  const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) / width;
+  const long long r = i / a.hq;
+  const int h = (int)(i % a.hq);
+  float sum = 0.f;
+  if (r < rows && part * V < a.d) {
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.g.p) + r * a.g.row + h * a.g.head + part * V);
+    const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o.p) + (r * a.hq + h) * a.d + part * V);
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (sizeof(T) == 2) {
+        const float2 u = Half<T>::unpack(xs[e]), v = Half<T>::unpack(ys[e]);
+        sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
+      } else {
+        sum = fmaf(__uint_as_float(xs[e]), __uint_as_float(ys[e]), sum);
+      }
+    }
+  }
+  for (int x = width >> 1; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+  if (r < rows && part == 0) a.delta[(long long)h * a.nq + r] = sum;
+}
+
+// dq of a tile of 64 queries of one head
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
+  using L = Tile<T, DP>;
+  constexpr int BN = kRevTile, NT = BN / 8;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const uint32_t sq = smem_addr(smem), sg = sq + kPackTile * L::kStride, sk = sg + kPackTile * L::kStride, sv = sk + 2 * BN * L::kStride;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int4 item = a.items[blockIdx.x];
+  const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
+  const int h = blockIdx.y, kvh = h / a.group, row0 = item.y * kPackTile, k0 = item.z, k1 = item.w;
+  const int nt = (max(k1 - k0, 0) + BN - 1) / BN;
+  load_rows<T, DP, kPackTile>(sq, a.q, h, q0, row0, lq, a.d, tid);
+  load_rows<T, DP, kPackTile>(sg, a.g, h, q0, row0, lq, a.d, tid);
+  auto load = [&](int it) {
+    if (it < nt) {
+      const int buf = it & 1, b = k0 + it * BN;
+      load_rows<T, DP, BN>(sk + buf * BN * L::kStride, a.k, kvh, c0, b, k1, a.d, tid);
+      load_rows<T, DP, BN>(sv + buf * BN * L::kStride, a.v, kvh, c0, b, k1, a.d, tid);
+    }
+    copy_commit();
+  };
+  load(0);
+  const int wr = row0 + warp * 16, ra = wr + (lane >> 2), rb = ra + 8, off = lk - lq, big = 0x7fffffff;
+  const int lim_a = a.causal ? ra + off : big, lim_b = a.causal ? rb + off : big, lim_lo = a.causal ? wr + off : big, lim_hi = a.causal ? wr + 15 + off : big;
+  const long long at = (long long)h * a.nq + q0;
+  // rows that are not there: exp(-inf) = 0
+  const float ea = ra < lq ? a.lse[at + ra] * kLog2e : INFINITY, eb = rb < lq ? a.lse[at + rb] * kLog2e : INFINITY;
+  const float da = ra < lq ? a.delta[at + ra] : 0.f, db = rb < lq ? a.delta[at + rb] : 0.f;
+  float dq[DP / 8][4];
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
+  for (int it = 0; it < nt; ++it) {
+    load(it + 1);
+    copy_wait<1>();
+    __syncthreads();
+    const int kb = k0 + it * BN, buf = it & 1;
+    if (wr < lq && kb <= lim_hi) {
+      float p[NT][4], dp[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) { p[n][0] = p[n][1] = p[n][2] = p[n][3] = 0.f; dp[n][0] = dp[n][1] = dp[n][2] = dp[n][3] = 0.f; }
+      product_nt<T, DP, NT>(p, sq + warp * 16 * L::kStride, sk + buf * BN * L::kStride, lane);
+      product_nt<T, DP, NT>(dp, sg + warp * 16 * L::kStride, sv + buf * BN * L::kStride, lane);
+      const bool mask = kb + BN > k1 || kb + BN - 1 > lim_lo;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = kb + n * 8 + 2 * (lane & 3) + e;
+          float x = exp2f(fmaf(p[n][e], a.scale_log2, -ea)) * (dp[n][e] - da);
+          float y = exp2f(fmaf(p[n][2 + e], a.scale_log2, -eb)) * (dp[n][2 + e] - db);
+          if (mask && (j >= k1 || j > lim_a)) x = 0.f;
+          if (mask && (j >= k1 || j > lim_b)) y = 0.f;
+          p[n][e] = x; p[n][2 + e] = y;
+        }
+      }
+      product_nn<T, DP, NT>(dq, p, sk + buf * BN * L::kStride, lane);
+    }
+    __syncthreads();
+  }
+  copy_wait<0>();
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = half ? rb : ra;
+    if (r >= lq) continue;
+    T* dst = static_cast<T*>(a.dq) + ((long long)(q0 + r) * a.hq + h) * a.d;
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) {
+      const int c = n * 8 + 2 * (lane & 3);
+      if (c < a.d) store2(dst + c, dq[n][2 * half] * a.scale, dq[n][2 * half + 1] * a.scale);
+    }
+  }
+}
+
+// dk and dv of a tile of 64 keys of one key head: rows of the products are keys, columns queries
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
+  using L = Tile<T, DP>;
+  constexpr int BN = kRevTile, NT = BN / 8;
+  extern __shared__ __align__(16) unsigned char smem[];
+  const uint32_t sk = smem_addr(smem), sv = sk + kPackTile * L::kStride, sq = sv + kPackTile * L::kStride, sg = sq + 2 * BN * L::kStride;
+  float* se = reinterpret_cast<float*>(smem + (2 * kPackTile + 4 * BN) * L::kStride);   // [2][BN] lse, [2][BN] delta
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int4 item = a.items[blockIdx.x];
+  const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
+  const int kvh = blockIdx.y, row0 = item.y * kPackTile, i0 = item.z, i1 = item.w;
+  const int per = (max(i1 - i0, 0) + BN - 1) / BN, nt = per * a.group;
+  load_rows<T, DP, kPackTile>(sk, a.k, kvh, c0, row0, lk, a.d, tid);
+  load_rows<T, DP, kPackTile>(sv, a.v, kvh, c0, row0, lk, a.d, tid);
+  auto load = [&](int it) {
+    if (it < nt) {
+      const int buf = it & 1, h = kvh * a.group + it / per, b = i0 + (it % per) * BN;
+      load_rows<T, DP, BN>(sq + buf * BN * L::kStride, a.q, h, q0, b, i1, a.d, tid);
+      load_rows<T, DP, BN>(sg + buf * BN * L::kStride, a.g, h, q0, b, i1, a.d, tid);
+      if (tid < BN) {
+        const bool ok = b + tid < i1;
+        const long long at = (long long)h * a.nq + q0 + b + tid;
+        se[buf * BN + tid] = ok ? fmaf(a.lse[at], kLog2e, -prob_shift<T>()) : INFINITY;
+        se[(2 + buf) * BN + tid] = ok ? a.delta[at] * prob_unscale<T>() : 0.f;
+      }
+    }
+    copy_commit();
+  };
+  load(0);
+  const int wr = row0 + warp * 16, ra = wr + (lane >> 2), rb = ra + 8, off = lk - lq, none = -0x7fffffff - 1;
+  // first query that sees a key
+  const int lim_a = a.causal ? ra - off : none, lim_b = a.causal ? rb - off : none, lim_lo = a.causal ? wr - off : none, lim_hi = a.causal ? wr + 15 - off : none;
+  float dk[DP / 8][4], dv[DP / 8][4];
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n) { dk[n][0] = dk[n][1] = dk[n][2] = dk[n][3] = 0.f; dv[n][0] = dv[n][1] = dv[n][2] = dv[n][3] = 0.f; }
+  for (int it = 0; it < nt; ++it) {
+    load(it + 1);
+    copy_wait<1>();
+    __syncthreads();
+    const int ib = i0 + (it % per) * BN, buf = it & 1;
+    if (wr < lk && ib + BN - 1 >= lim_lo) {
+      float p[NT][4], ds[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) { p[n][0] = p[n][1] = p[n][2] = p[n][3] = 0.f; ds[n][0] = ds[n][1] = ds[n][2] = ds[n][3] = 0.f; }
+      product_nt<T, DP, NT>(p, sk + warp * 16 * L::kStride, sq + buf * BN * L::kStride, lane);
+      product_nt<T, DP, NT>(ds, sv + warp * 16 * L::kStride, sg + buf * BN * L::kStride, lane);
+      const bool mask = a.causal && ib < lim_hi;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        const int c = n * 8 + 2 * (lane & 3);
+        const float2 e = *reinterpret_cast<const float2*>(se + buf * BN + c), d = *reinterpret_cast<const float2*>(se + (2 + buf) * BN + c);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int i = ib + c + (x & 1), lim = x < 2 ? lim_a : lim_b;
+          float w = exp2f(fmaf(p[n][x], a.scale_log2, -((x & 1) ? e.y : e.x)));
+          if (mask && i < lim) w = 0.f;
+          ds[n][x] = w == 0.f ? 0.f : w * fmaf(ds[n][x], prob_unscale<T>(), -((x & 1) ? d.y : d.x));
+          p[n][x] = w;
+        }
+      }
+      product_nn<T, DP, NT>(dv, p, sg + buf * BN * L::kStride, lane);
+      product_nn<T, DP, NT>(dk, ds, sq + buf * BN * L::kStride, lane);
+    }
+    __syncthreads();
+  }
+  copy_wait<0>();
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int r = half ? rb : ra;
+    if (r >= lk) continue;
+    const long long at = ((long long)(c0 + r) * a.hk + kvh) * a.d;
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) {
+      const int c = n * 8 + 2 * (lane & 3);
+      if (c < a.d) {
+        store2(static_cast<T*>(a.dk) + at + c, dk[n][2 * half] * a.scale, dk[n][2 * half + 1] * a.scale);
+        store2(static_cast<T*>(a.dv) + at + c, dv[n][2 * half] * prob_unscale<T>(), dv[n][2 * half + 1] * prob_unscale<T>());
+      }
+    }
+  }
+}
+
+template <typename K>
+void launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, const PackedArgs& a) {
+  if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  kernel<<<grid, threads, smem, st>>>(a);
+  count_launch();
+}
+
+#define SO3LR_PACKED_WIDTHS(T, CALL)            \
+  switch (packed_padded(a.d)) {                 \
+    case 32: { CALL(T, 32) } break;             \
+    case 64: { CALL(T, 64) } break;             \
+    case 96: { CALL(T, 96) } break;             \
+    default: { CALL(T, 128) } break;            \
+  }
+
+}  // namespace packed
+
+template <typename T> void packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
+#define CALL(T, DP) packed::launch(packed::forward_kernel<T, DP, false>, dim3(n_items, a.hq), 128, packed::forward_smem<T, DP>(), st, a);
+  SO3LR_PACKED_WIDTHS(T, CALL)
+#undef CALL
+}
+template <typename T> void packed_forward_split(cudaStream_t st, const PackedArgs& a, int n_items, int n_structures, bool combine) {
+#define CALL(T, DP)                                                                                                                 \
+  packed::launch(packed::forward_kernel<T, DP, true>, dim3(n_items, a.hk), 128, packed::forward_smem<T, DP>(), st, a);              \
+  if (combine) packed::launch(packed::combine_kernel<T, DP>, dim3(n_structures, a.hk), 256, 0, st, a);
+  SO3LR_PACKED_WIDTHS(T, CALL)
+#undef CALL
+}
+template <typename T> void packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
+#define CALL(T, DP) packed::launch(packed::dq_kernel<T, DP>, dim3(n_items, a.hq), 128, packed::reverse_smem<T, DP>(), st, a);
+  SO3LR_PACKED_WIDTHS(T, CALL)
+#undef CALL
+}
+template <typename T> void packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
+#define CALL(T, DP) packed::launch(packed::dkv_kernel<T, DP>, dim3(n_items, a.hk), 128, packed::reverse_smem<T, DP>(), st, a);
+  SO3LR_PACKED_WIDTHS(T, CALL)
+#undef CALL
+}
+template <typename T> void packed_delta(cudaStream_t st, const PackedArgs& a, int rows) {
+  int width = 1;
+  while (width * (16 / (int)sizeof(T)) < a.d) width <<= 1;
+  const long long threads = (long long)rows * a.hq * width;
+  if (threads == 0) return;
+  packed::delta_kernel<T><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(a, rows, width);
+  count_launch();
+}
+
+}  // namespace so3lr

@@ -1,0 +1,10 @@
+// The warp-level kernels of packed_mma.cuh for __nv_bfloat16 operands.
+#include "packed_mma.cuh"
+
+namespace so3lr {
+template void packed_forward_mma<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
+template void packed_forward_split<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int, int, bool);
+template void packed_dq_mma<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
+template void packed_dkv_mma<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
+template void packed_delta<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
+}  // namespace so3lr

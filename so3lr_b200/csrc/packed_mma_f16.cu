@@ -1,0 +1,10 @@
+// The warp-level kernels of packed_mma.cuh for __half operands.
+#include "packed_mma.cuh"
+
+namespace so3lr {
+template void packed_forward_mma<__half>(cudaStream_t, const PackedArgs&, int);
+template void packed_forward_split<__half>(cudaStream_t, const PackedArgs&, int, int, bool);
+template void packed_dq_mma<__half>(cudaStream_t, const PackedArgs&, int);
+template void packed_dkv_mma<__half>(cudaStream_t, const PackedArgs&, int);
+template void packed_delta<__half>(cudaStream_t, const PackedArgs&, int);
+}  // namespace so3lr
