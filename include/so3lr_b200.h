@@ -436,6 +436,9 @@ SO3LR_B200_API int so3lr_b200_structure_attention_vjp(const int32_t* image, cons
                                                       const so3lr_b200_attention_shape* shape, const so3lr_b200_rows* q,
                                                       const so3lr_b200_rows* k, const so3lr_b200_rows* v, const void* out, const float* lse,
                                                       const so3lr_b200_rows* g, float* delta, void* d_q, void* d_k, void* d_v);
+/* 1 where a bounded wait of the tensor-core kernels has run out on the current device since the library was loaded (their rows are NaN
+ * then); waits for the device */
+SO3LR_B200_API int so3lr_b200_structure_attention_error(int* out);
 
 /* Host-callable pieces of the device math, exported for the CPU tests (no GPU needed). */
 /* 64-bit total of a device array of per-row pair counts, formed the way the list builder forms it ahead of its 32-bit

@@ -105,6 +105,7 @@ def _load():
         "so3lr_b200_structure_attention_workspace": (i64, [p, p]),
         "so3lr_b200_structure_attention": (i32, [p] * 10 + [i64]),
         "so3lr_b200_structure_attention_vjp": (i32, [p] * 14),
+        "so3lr_b200_structure_attention_error": (i32, [C.POINTER(i32)]),
         "so3lr_b200_host_fail_allocation": (i64, [i64, i32]),
         "so3lr_b200_host_sph_harm": (None, [f32, f32, f32, p]),
         "so3lr_b200_host_sph_harm_vjp": (None, [f32, f32, f32, p, p]),

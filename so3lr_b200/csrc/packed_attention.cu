@@ -14,9 +14,12 @@ namespace so3lr {
 namespace {
 
 // The image of a layout (int32): a header, the offsets of both sides, and tables of work items {structure, tile, first, last}.
+// Tables of query tiles: 64 rows (warp-level kernels), 128 and 256 (tensor cores, reverse and forward); of key tiles: 64 and 128.
 enum Head : int { kMagicAt, kN, kCausal, kRowsQ, kRowsKv, kMaxQ, kStartQ, kStartKv, kItemsQ, kNItemsQ, kItemsKv, kNItemsKv, kItemsSplit, kNItemsSplit,
-                  kSplitFirst, kCombine, kTotal, kHeadInts = 32 };
+                  kSplitFirst, kCombine, kTotal, kItemsQ128, kNItemsQ128, kItemsQ256, kNItemsQ256, kItemsKv128, kNItemsKv128, kMaxKv, kHeadInts = 32 };
 constexpr int kMagic = 0x53334c50;
+constexpr int kTables = 5, kTileRows[kTables] = {kPackTile, kPackTile, 128, 256, 128}, kTableAt[kTables] = {kItemsQ, kItemsKv, kItemsQ128, kItemsQ256, kItemsKv128};
+constexpr bool kOfKeys[kTables] = {false, true, false, false, true};
 
 int64_t align4(int64_t x) { return (x + 3) & ~3LL; }
 
@@ -27,7 +30,7 @@ int split_length(int64_t keys) {
   return (int)std::min<int64_t>(512, std::max<int64_t>(64, (want + 63) / 64 * 64));
 }
 
-struct Counts { int64_t q = 0, kv = 0, split = 0, total = 0; };
+struct Counts { int64_t items[kTables] = {}, split = 0, total = 0; };
 
 bool valid(int n, const int32_t* sq, const int32_t* sk) {
   if (n < 0 || !sq || !sk || sq[0] != 0 || sk[0] != 0) return false;
@@ -40,11 +43,11 @@ Counts count(int n, const int32_t* sq, const int32_t* sk) {
   const int chunk = split_length(sk[n]);
   for (int i = 0; i < n; ++i) {
     const int64_t lq = sq[i + 1] - sq[i], lk = sk[i + 1] - sk[i];
-    c.q += (lq + kPackTile - 1) / kPackTile;
-    c.kv += (lk + kPackTile - 1) / kPackTile;
+    for (int t = 0; t < kTables; ++t) c.items[t] += ((kOfKeys[t] ? lk : lq) + kTileRows[t] - 1) / kTileRows[t];
     if (lq > 0) c.split += std::max<int64_t>(1, (lk + chunk - 1) / chunk);
   }
-  c.total = kHeadInts + 2 * align4(n + 1) + 4 * (c.q + c.kv + c.split) + align4(n + 1);
+  c.total = kHeadInts + 3 * align4(n + 1) + 4 * c.split;
+  for (int t = 0; t < kTables; ++t) c.total += 4 * c.items[t];
   return c;
 }
 
@@ -59,45 +62,47 @@ void put(int32_t* at, std::vector<Item>& items) {
 void build_image(int n, const int32_t* sq, const int32_t* sk, bool causal, int32_t* im) {
   const Counts c = count(n, sq, sk);
   std::fill(im, im + c.total, 0);
-  int max_q = 0;
-  im[kMagicAt] = kMagic; im[kN] = n; im[kCausal] = causal; im[kRowsQ] = sq[n]; im[kRowsKv] = sk[n];
-  im[kStartQ] = kHeadInts; im[kStartKv] = (int32_t)(kHeadInts + align4(n + 1));
-  im[kItemsQ] = (int32_t)(kHeadInts + 2 * align4(n + 1)); im[kNItemsQ] = (int32_t)c.q;
-  im[kItemsKv] = (int32_t)(im[kItemsQ] + 4 * c.q); im[kNItemsKv] = (int32_t)c.kv;
-  im[kItemsSplit] = (int32_t)(im[kItemsKv] + 4 * c.kv); im[kNItemsSplit] = (int32_t)c.split;
-  im[kSplitFirst] = (int32_t)(im[kItemsSplit] + 4 * c.split); im[kTotal] = (int32_t)c.total;
+  im[kMagicAt] = kMagic; im[kN] = n; im[kCausal] = causal; im[kRowsQ] = sq[n]; im[kRowsKv] = sk[n]; im[kTotal] = (int32_t)c.total;
+  int64_t at = kHeadInts;
+  auto place = [&](int field, int64_t ints) { im[field] = (int32_t)at; at += ints; };
+  place(kStartQ, align4(n + 1)); place(kStartKv, align4(n + 1)); place(kSplitFirst, align4(n + 1));
+  for (int t = 0; t < kTables; ++t) { place(kTableAt[t], 4 * c.items[t]); im[kTableAt[t] + 1] = (int32_t)c.items[t]; }
+  place(kItemsSplit, 4 * c.split); im[kNItemsSplit] = (int32_t)c.split;
   std::copy(sq, sq + n + 1, im + im[kStartQ]);
   std::copy(sk, sk + n + 1, im + im[kStartKv]);
-  std::vector<Item> q, kv;
-  q.reserve(c.q); kv.reserve(c.kv);
-  const int chunk = split_length(sk[n]);
-  int32_t* split = im + im[kItemsSplit];
-  int at = 0, combine = 0;
-  for (int s = 0; s < n; ++s) {
-    const int lq = sq[s + 1] - sq[s], lk = sk[s + 1] - sk[s], off = lk - lq;
-    max_q = std::max(max_q, lq);
-    for (int t = 0; (int64_t)t * kPackTile < lq; ++t) {
-      const int64_t end = causal ? std::min<int64_t>(lk, std::max<int64_t>(0, std::min<int64_t>(lq, (t + 1LL) * kPackTile) + off)) : lk;
-      q.push_back({s, t, 0, (int32_t)end});
-    }
-    for (int t = 0; (int64_t)t * kPackTile < lk; ++t) {
-      const int64_t first = causal ? std::min<int64_t>(lq, std::max<int64_t>(0, (int64_t)t * kPackTile - off)) : 0;
-      kv.push_back({s, t, (int32_t)first, lq});
-    }
-    im[im[kSplitFirst] + s] = at;
-    if (lq > 0) {
-      const int pieces = std::max(1, (lk + chunk - 1) / chunk);
-      if (pieces > 1) combine = 1;
-      for (int p = 0; p < pieces; ++p, ++at) {
-        split[4 * at] = s; split[4 * at + 1] = pieces;
-        split[4 * at + 2] = p * chunk; split[4 * at + 3] = (int32_t)std::min<int64_t>(lk, (int64_t)(p + 1) * chunk);
+  std::vector<Item> items;
+  for (int t = 0; t < kTables; ++t) {
+    const int64_t rows = kTileRows[t];
+    items.clear();
+    items.reserve(c.items[t]);
+    for (int s = 0; s < n; ++s) {
+      const int64_t lq = sq[s + 1] - sq[s], lk = sk[s + 1] - sk[s], off = lk - lq;
+      if (!kOfKeys[t]) {      // the keys that a tile's last row sees
+        for (int64_t i = 0; i * rows < lq; ++i)
+          items.push_back({s, (int32_t)i, 0, (int32_t)(causal ? std::min(lk, std::max<int64_t>(0, std::min(lq, (i + 1) * rows) + off)) : lk)});
+      } else {                // the queries from the first one on that sees the tile's first key
+        for (int64_t i = 0; i * rows < lk; ++i)
+          items.push_back({s, (int32_t)i, (int32_t)(causal ? std::min(lq, std::max<int64_t>(0, i * rows - off)) : 0), (int32_t)lq});
       }
     }
+    put(im + im[kTableAt[t]], items);
   }
-  im[im[kSplitFirst] + n] = at;
-  im[kMaxQ] = max_q; im[kCombine] = combine;
-  put(im + im[kItemsQ], q);
-  put(im + im[kItemsKv], kv);
+  const int chunk = split_length(sk[n]);
+  int32_t* split = im + im[kItemsSplit];
+  int k = 0;
+  for (int s = 0; s < n; ++s) {
+    const int lq = sq[s + 1] - sq[s], lk = sk[s + 1] - sk[s];
+    im[kMaxQ] = std::max(im[kMaxQ], lq); im[kMaxKv] = std::max(im[kMaxKv], lk);
+    im[im[kSplitFirst] + s] = k;
+    if (lq == 0) continue;
+    const int pieces = (int)std::max<int64_t>(1, ((int64_t)lk + chunk - 1) / chunk);
+    if (pieces > 1) im[kCombine] = 1;
+    for (int p = 0; p < pieces; ++p, ++k) {
+      split[4 * k] = s; split[4 * k + 1] = pieces;
+      split[4 * k + 2] = (int32_t)((int64_t)p * chunk); split[4 * k + 3] = (int32_t)std::min<int64_t>(lk, (p + 1LL) * chunk);
+    }
+  }
+  im[im[kSplitFirst] + n] = k;
 }
 
 bool rows_ok(const so3lr_b200_rows* r, int type) {
@@ -129,26 +134,50 @@ int64_t part_floats(const int32_t* im, const so3lr_b200_attention_shape* a) {
   return (int64_t)im[kNItemsSplit] * a->heads_kv * im[kMaxQ] * (a->heads_q / a->heads_kv) * packed_padded(a->d);
 }
 
+// Structures of this many rows go to the tensor cores.
+#ifndef SO3LR_PACKED_TC_ROWS
+#define SO3LR_PACKED_TC_ROWS 128
+#endif
+template <typename T> bool on_tensor_cores(const int32_t* im) { return sizeof(T) == 2 && im[kMaxQ] >= SO3LR_PACKED_TC_ROWS && im[kMaxKv] >= SO3LR_PACKED_TC_ROWS; }
+
+const int4* table(const int32_t* im, const int32_t* dev, int field) { return reinterpret_cast<const int4*>(dev + im[field]); }
+
 template <typename T>
 void forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
   if (few_rows(im, a)) {
-    p.items = reinterpret_cast<const int4*>(dev + im[kItemsSplit]);
+    p.items = table(im, dev, kItemsSplit);
     p.part_rows = im[kMaxQ] * p.group;
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + part_floats(im, a));
     packed_forward_split<T>(st, p, im[kNItemsSplit], im[kN], im[kCombine]);
     return;
   }
-  p.items = reinterpret_cast<const int4*>(dev + im[kItemsQ]);
+  if constexpr (sizeof(T) == 2) {
+    if (on_tensor_cores<T>(im)) {
+      p.items = table(im, dev, kItemsQ256);
+      packed_forward_tc<T>(st, p, im[kNItemsQ256]);
+      return;
+    }
+  }
+  p.items = table(im, dev, kItemsQ);
   packed_forward_mma<T>(st, p, im[kNItemsQ]);
 }
 
 template <typename T>
 void reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev) {
   packed_delta<T>(st, p, im[kRowsQ]);
-  p.items = reinterpret_cast<const int4*>(dev + im[kItemsQ]);
+  if constexpr (sizeof(T) == 2) {
+    if (on_tensor_cores<T>(im)) {
+      p.items = table(im, dev, kItemsQ128);
+      packed_dq_tc<T>(st, p, im[kNItemsQ128]);
+      p.items = table(im, dev, kItemsKv128);
+      packed_dkv_tc<T>(st, p, im[kNItemsKv128]);
+      return;
+    }
+  }
+  p.items = table(im, dev, kItemsQ);
   if (im[kNItemsQ]) packed_dq_mma<T>(st, p, im[kNItemsQ]);
-  p.items = reinterpret_cast<const int4*>(dev + im[kItemsKv]);
+  p.items = table(im, dev, kItemsKv);
   if (im[kNItemsKv]) packed_dkv_mma<T>(st, p, im[kNItemsKv]);
 }
 
@@ -223,5 +252,7 @@ int so3lr_b200_structure_attention_vjp(const int32_t* image, const int32_t* imag
   SO3LR_CUDA_CHECK(cudaGetLastError());
   return kOk;
 }
+
+int so3lr_b200_structure_attention_error(int* out) { return out ? packed_error(out) : kInvalidArgument; }
 
 }  // extern "C"

@@ -47,6 +47,12 @@ template <typename T> void packed_dq_mma(cudaStream_t st, const PackedArgs& a, i
 template <typename T> void packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items);
 template <typename T> void packed_delta(cudaStream_t st, const PackedArgs& a, int rows);
 
+// kernels on the tensor cores (16-bit types): tiles of 128 rows, two of them side by side in the forward kernel
+template <typename T> void packed_forward_tc(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> void packed_dq_tc(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> void packed_dkv_tc(cudaStream_t st, const PackedArgs& a, int n_items);
+int packed_error(int* out);
+
 inline int packed_padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
 
 }  // namespace so3lr

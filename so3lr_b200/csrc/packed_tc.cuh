@@ -1,0 +1,196 @@
+// What the tensor-core kernels of attention inside packed structures share: operand tiles, descriptors, barriers, tensor memory.
+//
+// Every operand tile is 128 rows x d values in one image: 16-byte pieces (8 values) of column group c of row r at c * 2048 + r * 16.  That
+// is the core-matrix layout of tcgen05.mma without a swizzle for rows as M or N with d contracted (K-major), and for d as N with the rows
+// contracted (MN-major) as well, so a tile of keys serves q k^T and dS k, a tile of queries k q^T and dS^T q.  Loader warps fill it
+// with 16-byte asynchronous copies, eight rows x four pieces an instruction: 64-byte stretches of global memory, shared memory without
+// bank conflicts, any strides, rows and columns that are not there as zeros.
+#pragma once
+#include "packed_mma.cuh"
+
+namespace so3lr {
+namespace tc {
+
+using packed::copy16;
+using packed::copy_commit;
+using packed::copy_wait;
+using packed::kLn2;
+using packed::kLog2e;
+using packed::smem_addr;
+
+constexpr int kTile = 128;
+constexpr int kComputeWarps = 8, kMmaWarp = 8, kLoadWarps = 3;
+constexpr int kThreads = 384;
+// registers a thread of the compute and of the other warps after the split: 256 x 208 + 128 x 88 = 384 x 168, the launch's total
+constexpr int kComputeRegs = 208, kOtherRegs = 88;
+constexpr long long kWaitNs = 2000000000LL;
+
+__device__ __forceinline__ unsigned long long now_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+__device__ __forceinline__ bool test_bar(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+// Every wait ends: after two seconds, or when another one of this CTA has run out, the kernel carries on to its end, reports through
+// *error, and writes NaN.
+__device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity, volatile int* failed, int* error) {
+  if (test_bar(bar, parity)) return;
+  unsigned long long t0 = 0;
+  for (unsigned it = 1;; ++it) {
+    if (test_bar(bar, parity)) return;
+    if ((it & 63) == 0) {
+      if (*failed) return;
+      const unsigned long long t = now_ns();
+      if (t0 == 0) t0 = t;
+      if (t - t0 > kWaitNs) { *failed = 1; atomicExch(error, 1); return; }
+    }
+  }
+}
+__device__ __forceinline__ void init_bar(uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void more_regs() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void fewer_regs() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t on;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(on));
+  return on;
+}
+__device__ __forceinline__ float pow2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---- matrix instructions ----
+// descriptor of an operand tile: rows as M or N and columns contracted (K-major), or columns as N and rows contracted (MN-major); bytes
+// between core matrices along the contracted index, then along the other one
+__device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn_major) {
+  const uint32_t lbo = mn_major ? 128 : 2048, sbo = mn_major ? 2048 : 128;
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | ((uint64_t)1 << 46);
+}
+constexpr uint32_t kStepK = 4096 >> 4, kStepMn = 256 >> 4;      // 16 contracted entries further, in descriptor units
+template <typename T> __device__ __forceinline__ uint32_t idesc(int n, bool b_mn_major) {
+  const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+}
+// The whole warp runs the issue code, the elected lane (`on`) issues: descriptors stay in uniform registers.
+__device__ __forceinline__ void mma_ss(uint32_t on, uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(on) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc), "r"(on) : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t on, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar), "r"(on) : "memory");
+}
+// D[128 x 128] = A B^T over d columns, both tiles in shared memory
+template <typename T> __device__ __forceinline__ void product_rows(uint32_t on, uint32_t dst, uint32_t a, uint32_t b, int d) {
+  const uint64_t da = desc(a, false), db = desc(b, false);
+  const uint32_t id = idesc<T>(kTile, false);
+#pragma unroll 1
+  for (int k = 0; k < d / 16; ++k) mma_ss(on, dst, da + k * kStepK, db + k * kStepK, id, k > 0);
+}
+// D[128 x d] (+)= A B: A 128 x 128 in tensor memory, 64 packed columns as two halves `gap` columns apart, B a tile with its rows contracted
+template <typename T> __device__ __forceinline__ void product_cols(uint32_t on, uint32_t dst, uint32_t a, int gap, uint32_t b, int d, uint32_t acc) {
+  const uint64_t db = desc(b, true);
+  const uint32_t id = idesc<T>(d, true);
+#pragma unroll 1
+  for (int k = 0; k < 8; ++k) mma_ts(on, dst, a + (k & 3) * 8 + (k >> 2) * gap, db + k * kStepMn, id, acc | (k > 0));
+}
+
+// ---- tensor memory ----
+#define R8(x, o) x[o], x[o + 1], x[o + 2], x[o + 3], x[o + 4], x[o + 5], x[o + 6], x[o + 7]
+#define O8(x, o) "=r"(x[o]), "=r"(x[o + 1]), "=r"(x[o + 2]), "=r"(x[o + 3]), "=r"(x[o + 4]), "=r"(x[o + 5]), "=r"(x[o + 6]), "=r"(x[o + 7])
+#define I8(x, o) "r"(x[o]), "r"(x[o + 1]), "r"(x[o + 2]), "r"(x[o + 3]), "r"(x[o + 4]), "r"(x[o + 5]), "r"(x[o + 6]), "r"(x[o + 7])
+__device__ __forceinline__ void ld32(uint32_t addr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : O8(r, 0), O8(r, 8), O8(r, 16), O8(r, 24) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ld16(uint32_t addr, uint32_t* r) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : O8(r, 0), O8(r, 8) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void st16(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+               ::"r"(addr), I8(r, 0), I8(r, 8) : "memory");
+}
+#undef R8
+#undef O8
+#undef I8
+// waits for the loads of N registers; what reads them stays behind the wait
+template <int N> __device__ __forceinline__ void wait_ld(uint32_t (&r)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// ---- loading ----
+// Groups of copies in order; group j is announced on its barrier when it has landed and is visible to the tensor cores.  At most two
+// stay in flight behind the one just issued; a loader that has to wait for room first announces all it has.
+struct Loader {
+  int lane, warp;            // 0 .. kLoadWarps - 1
+  int issued = 0, told = 0;
+  template <typename T>
+  __device__ __forceinline__ void tile(uint32_t dst, const Rows& src, int head, long long base, int r0, int r1, int d) const {
+    const T* p = static_cast<const T*>(src.p) + head * src.head;
+    const int pieces = d >> 3, groups = (pieces + 3) >> 2;
+    for (int i = warp; i < 16 * groups; i += kLoadWarps) {
+      const int r = (i & 15) * 8 + (lane & 7), c = (i >> 4) * 4 + (lane >> 3);
+      if (c < pieces) {
+        const bool ok = r0 + r < r1;
+        copy16(dst + c * 2048 + r * 16, ok ? p + (base + r0 + r) * src.row + c * 8 : p, ok);
+      }
+    }
+  }
+  // bar(j): barrier of group j
+  template <typename F> __device__ __forceinline__ void tell(int upto, F bar) {
+    if (told >= upto) return;
+    fence_smem();
+    for (; told < upto; ++told) arrive(bar(told));
+  }
+  template <typename F> __device__ __forceinline__ void done(F bar) {
+    copy_commit();
+    ++issued;
+    copy_wait<2>();
+    tell(issued - 2, bar);
+  }
+  template <typename F> __device__ __forceinline__ void flush(F bar) {
+    copy_wait<0>();
+    tell(issued, bar);
+  }
+  template <typename F> __device__ __forceinline__ void room(uint32_t empty, uint32_t parity, volatile int* failed, int* error, F bar) {
+    if (test_bar(empty, parity)) return;
+    flush(bar);
+    wait_bar(empty, parity, failed, error);
+  }
+};
+
+__device__ __forceinline__ uint32_t alloc_tmem(uint32_t* where) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(where)), "r"(512) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  return 0;
+}
+__device__ __forceinline__ void free_tmem(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+}  // namespace tc
+}  // namespace so3lr

@@ -8,7 +8,6 @@ import torch
 from so3lr_b200 import attention as A
 from so3lr_b200._lib import AttentionShape, NormRotateArgs, Rows, lib
 
-TILE = 64
 
 
 def image(lq, lk, causal):
@@ -36,23 +35,25 @@ def test_items_cover_what_is_allowed(lq, lk, causal):
     im = image(lq, lk, causal)
     allowed = [np.arange(b)[None, :] <= np.arange(a)[:, None] + (b - a) if causal else np.ones((a, b), bool) for a, b in zip(lq, lk)]
     # query tiles: once each, and the keys of a tile reach as far as any of its rows sees, no further
-    seen = set()
-    rows = items(im, 8, 9)
-    assert np.all(np.diff(rows[:, 3] - rows[:, 2]) <= 0)          # the longest first
-    for s, t, first, last in rows:
-        assert (s, t) not in seen and first == 0
-        seen.add((s, t))
-        cols = allowed[s][t * TILE:(t + 1) * TILE].any(0)
-        assert last == (cols.nonzero()[0].max() + 1 if cols.any() else 0)
-    assert len(seen) == sum(-(-a // TILE) for a in lq)
+    for at, n, tile in ((8, 9, 64), (17, 18, 128), (19, 20, 256)):
+        seen = set()
+        rows = items(im, at, n)
+        assert np.all(np.diff(rows[:, 3] - rows[:, 2]) <= 0)          # the longest first
+        for s, t, first, last in rows:
+            assert (s, t) not in seen and first == 0
+            seen.add((s, t))
+            cols = allowed[s][t * tile:(t + 1) * tile].any(0)
+            assert last == (cols.nonzero()[0].max() + 1 if cols.any() else 0)
+        assert len(seen) == sum(-(-a // tile) for a in lq)
     # key tiles
-    seen = set()
-    for s, t, first, last in items(im, 10, 11):
-        assert (s, t) not in seen and last == lq[s]
-        seen.add((s, t))
-        r = allowed[s][:, t * TILE:(t + 1) * TILE].any(1)
-        assert first == (r.nonzero()[0].min() if r.any() else lq[s])
-    assert len(seen) == sum(-(-b // TILE) for b in lk)
+    for at, n, tile in ((10, 11, 64), (21, 22, 128)):
+        seen = set()
+        for s, t, first, last in items(im, at, n):
+            assert (s, t) not in seen and last == lq[s]
+            seen.add((s, t))
+            r = allowed[s][:, t * tile:(t + 1) * tile].any(1)
+            assert first == (r.nonzero()[0].min() if r.any() else lq[s])
+        assert len(seen) == sum(-(-b // tile) for b in lk)
     # stretches of the keys: disjoint, in order, all keys, and at least one item per structure with queries
     first_of = im[im[14]:im[14] + len(lq) + 1]
     split = items(im, 12, 13)
@@ -60,7 +61,7 @@ def test_items_cover_what_is_allowed(lq, lk, causal):
         mine = split[first_of[s]:first_of[s + 1]]
         assert len(mine) == 0 if a == 0 else np.all(mine[:, 0] == s) and np.all(mine[:, 1] == len(mine)) and mine[0, 2] == 0 and mine[-1, 3] == b
         assert np.all(mine[1:, 2] == mine[:-1, 3])
-    assert im[13] == first_of[-1] and im[15] == int(len(split) > sum(a > 0 for a in lq)) and im[5] == max(lq)
+    assert im[13] == first_of[-1] and im[15] == int(len(split) > sum(a > 0 for a in lq)) and im[5] == max(lq) and im[23] == max(lk)
 
 
 def test_refused_layouts():
