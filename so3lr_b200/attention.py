@@ -34,12 +34,12 @@ def _p(t):
 
 
 def _head_rows(name, t, dtype, device, d=None):
-    """`t` (rows, heads, d) in a form that the kernels read: as it is where its last axis is contiguous and 16-byte pieces are aligned, else a
-    contiguous copy."""
+    """`t` (rows, heads, d) in a form that the kernels read: as it is where its last axis is contiguous, 16-byte pieces are aligned and no axis
+    is broadcast, else a contiguous copy."""
     if t.ndim != 3 or t.dtype != dtype or t.device != device or (d is not None and t.shape[2] != d):
         raise ValueError(f"{name} must be (rows, heads, {'d' if d is None else d}) {dtype} on {device}, not {tuple(t.shape)} {t.dtype} on {t.device}")
     unit = 16 // t.element_size()
-    if t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % 16:
+    if t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % 16 or 0 in t.stride():
         t = t.contiguous()
         if t.data_ptr() % 16 or t.stride(2) != 1:
             t = t.clone(memory_format=torch.contiguous_format)

@@ -113,14 +113,14 @@ Rows rows_of(const so3lr_b200_rows* r) { return {r->data, r->row_stride, r->head
 
 bool shape_ok(const int32_t* im, const so3lr_b200_attention_shape* a) {
   return im && im[kMagicAt] == kMagic && a && a->type >= 0 && a->type <= 2 && a->heads_q > 0 && a->heads_kv > 0 && a->heads_q % a->heads_kv == 0 &&
-         a->heads_q <= 65535 && a->d >= 16 && a->d <= 128 && a->d % 16 == 0 && a->rows_q >= im[kRowsQ] && a->rows_q < 0x7fffffff && a->rows_kv >= im[kRowsKv] &&
+         a->heads_q <= 65535 && a->d >= 16 && a->d <= 128 && a->d % 16 == 0 && a->rows_q >= im[kRowsQ] && a->rows_q < 0x7fffffff && a->rows_kv >= im[kRowsKv] && a->rows_kv < 0x7fffffff &&
          a->scale > 0.f && std::isfinite(a->scale);
 }
 
 PackedArgs common(const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a) {
   PackedArgs p;
   p.start_q = dev + im[kStartQ]; p.start_kv = dev + im[kStartKv]; p.split_first = dev + im[kSplitFirst];
-  p.nq = (int)a->rows_q; p.hq = a->heads_q; p.hk = a->heads_kv; p.group = a->heads_q / a->heads_kv; p.d = a->d; p.causal = im[kCausal];
+  p.nq = (int)a->rows_q; p.nkv = (int)a->rows_kv; p.hq = a->heads_q; p.hk = a->heads_kv; p.group = a->heads_q / a->heads_kv; p.d = a->d; p.causal = im[kCausal];
   p.scale = a->scale; p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   return p;
 }
@@ -143,42 +143,38 @@ template <typename T> bool on_tensor_cores(const int32_t* im) { return sizeof(T)
 const int4* table(const int32_t* im, const int32_t* dev, int field) { return reinterpret_cast<const int4*>(dev + im[field]); }
 
 template <typename T>
-void forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
+int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
   if (few_rows(im, a)) {
     p.items = table(im, dev, kItemsSplit);
     p.part_rows = im[kMaxQ] * p.group;
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + part_floats(im, a));
     packed_forward_split<T>(st, p, im[kNItemsSplit], im[kN], im[kCombine]);
-    return;
+    return kOk;
   }
   if constexpr (sizeof(T) == 2) {
     if (on_tensor_cores<T>(im)) {
       p.items = table(im, dev, kItemsQ256);
-      packed_forward_tc<T>(st, p, im[kNItemsQ256]);
-      return;
+      return packed_forward_tc<T>(st, p, im[kNItemsQ256]);
     }
   }
   p.items = table(im, dev, kItemsQ);
   packed_forward_mma<T>(st, p, im[kNItemsQ]);
+  return kOk;
 }
 
 template <typename T>
-void reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev) {
+int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev) {
   packed_delta<T>(st, p, im[kRowsQ]);
   if constexpr (sizeof(T) == 2) {
-    if (on_tensor_cores<T>(im)) {
-      p.items = table(im, dev, kItemsQ128);
-      packed_dq_tc<T>(st, p, im[kNItemsQ128]);
-      p.items = table(im, dev, kItemsKv128);
-      packed_dkv_tc<T>(st, p, im[kNItemsKv128]);
-      return;
-    }
+    if (on_tensor_cores<T>(im))
+      return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128]);
   }
   p.items = table(im, dev, kItemsQ);
   if (im[kNItemsQ]) packed_dq_mma<T>(st, p, im[kNItemsQ]);
   p.items = table(im, dev, kItemsKv);
   if (im[kNItemsKv]) packed_dkv_mma<T>(st, p, im[kNItemsKv]);
+  return kOk;
 }
 
 }  // namespace
@@ -224,11 +220,10 @@ int so3lr_b200_structure_attention(const int32_t* image, const int32_t* image_de
   if (image[kRowsKv]) { p.k = rows_of(k); p.v = rows_of(v); } else { p.k = p.v = p.q; }   // never read: no structure has keys
   p.out = out; p.lse = lse;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->type == kBF16) forward<__nv_bfloat16>(st, p, image, image_dev, a, workspace);
-  else if (a->type == kF16) forward<__half>(st, p, image, image_dev, a, workspace);
-  else forward<float>(st, p, image, image_dev, a, workspace);
+  const int rc = a->type == kBF16 ? forward<__nv_bfloat16>(st, p, image, image_dev, a, workspace)
+                 : a->type == kF16 ? forward<__half>(st, p, image, image_dev, a, workspace) : forward<float>(st, p, image, image_dev, a, workspace);
   SO3LR_CUDA_CHECK(cudaGetLastError());
-  return kOk;
+  return rc;
 }
 
 int so3lr_b200_structure_attention_vjp(const int32_t* image, const int32_t* image_dev, void* stream, const so3lr_b200_attention_shape* a,
@@ -246,11 +241,10 @@ int so3lr_b200_structure_attention_vjp(const int32_t* image, const int32_t* imag
   if (!image[kRowsKv]) p.k = p.v = p.q;
   p.o.p = out; p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = d_q; p.dk = d_k; p.dv = d_v;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->type == kBF16) reverse<__nv_bfloat16>(st, p, image, image_dev);
-  else if (a->type == kF16) reverse<__half>(st, p, image, image_dev);
-  else reverse<float>(st, p, image, image_dev);
+  const int rc = a->type == kBF16 ? reverse<__nv_bfloat16>(st, p, image, image_dev)
+                 : a->type == kF16 ? reverse<__half>(st, p, image, image_dev) : reverse<float>(st, p, image, image_dev);
   SO3LR_CUDA_CHECK(cudaGetLastError());
-  return kOk;
+  return rc;
 }
 
 int so3lr_b200_structure_attention_error(int* out) { return out ? packed_error(out) : kInvalidArgument; }

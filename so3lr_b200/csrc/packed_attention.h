@@ -33,7 +33,7 @@ struct PackedArgs {
   float* part_o = nullptr;      // (item, hk, part_rows, DP) of the split form
   float2* part_ml = nullptr;    // (item, hk, part_rows): running maximum (in units of log2) and sum
   int part_rows = 0;            // most rows of a structure: tokens times heads of a group
-  int nq = 0, hq = 0, hk = 0, group = 1, d = 0, causal = 0;
+  int nq = 0, nkv = 0, hq = 0, hk = 0, group = 1, d = 0, causal = 0;
   float scale = 0.f, scale_log2 = 0.f;                // scale * log2(e): the softmax runs on powers of two
   int* err = nullptr;
 };
@@ -48,9 +48,8 @@ template <typename T> void packed_dkv_mma(cudaStream_t st, const PackedArgs& a, 
 template <typename T> void packed_delta(cudaStream_t st, const PackedArgs& a, int rows);
 
 // kernels on the tensor cores (16-bit types): tiles of 128 rows, two of them side by side in the forward kernel
-template <typename T> void packed_forward_tc(cudaStream_t st, const PackedArgs& a, int n_items);
-template <typename T> void packed_dq_tc(cudaStream_t st, const PackedArgs& a, int n_items);
-template <typename T> void packed_dkv_tc(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> int packed_forward_tc(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv);
 int packed_error(int* out);
 
 inline int packed_padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }

@@ -14,27 +14,31 @@ namespace {
 
 using namespace tc;
 
-// barriers and scratch at the end of the dynamic shared memory
+// barriers and scratch behind the tiles
 struct Tail {
-  unsigned long long bars[20];
+  unsigned long long bars[32];
   uint32_t tmem;
   int failed;
 };
+// Tiles that stream through: a ring of four slots (two sub-tiles) or eight, the two kinds of tile in turn; tile j sits in slot j % R.
+__device__ __forceinline__ int ring_slots(int subs) { return subs == 2 ? 4 : 8; }
+// sub-tiles need 1024-byte alignment
+__device__ __forceinline__ unsigned char* aligned_smem(unsigned char* p) { return p + ((1024u - (smem_addr(p) & 1023u)) & 1023u); }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 // 256 queries of one head: two tiles of 128 rows take turns, so that the exponentials of one run beside the products of the other.
 // Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t; P of a tile replaces its logits.
 // The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
 // the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
-enum FwdBar { kQFull, kKFull, kKEmpty = kKFull + 2, kVFull = kKEmpty + 2, kVEmpty = kVFull + 2, kSFull = kVEmpty + 2, kPFull = kSFull + 2,
-              kOFull = kPFull + 2, kFwdBars = kOFull + 2 };
+enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kSFull = kQFull + 2, kPFull = kSFull + 2, kOFull = kPFull + 2, kFix = kOFull + 2, kFwdBars };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int d = a.d, tile_bytes = d * 256;
-  Tail* tail = reinterpret_cast<Tail*>(smem + 6 * tile_bytes);
-  const uint32_t sq = smem_addr(smem), sk = sq + 2 * tile_bytes, sv = sk + 2 * tile_bytes, bar0 = smem_addr(tail->bars);
+__global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
+  extern __shared__ unsigned char raw[];
+  unsigned char* smem = aligned_smem(raw);
+  const int d = a.d, subs = d > 64 ? 2 : 1, tile_bytes = subs * kSub, R = ring_slots(subs);
+  Tail* tail = reinterpret_cast<Tail*>(smem + (2 + R) * tile_bytes);
+  const uint32_t sq = smem_addr(smem), ring = sq + 2 * tile_bytes, bar0 = smem_addr(tail->bars);
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -47,12 +51,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
-    init_bar(bar(kQFull), 32 * kLoadWarps);
-    for (int i = 0; i < 2; ++i) {
-      init_bar(bar(kKFull + i), 32 * kLoadWarps); init_bar(bar(kVFull + i), 32 * kLoadWarps);
-      init_bar(bar(kKEmpty + i), 1); init_bar(bar(kVEmpty + i), 1);
-      init_bar(bar(kSFull + i), 1); init_bar(bar(kPFull + i), kTile); init_bar(bar(kOFull + i), 1);
-    }
+    for (int i = 0; i < kFwdBars; ++i) init_bar(bar(i), i == kPFull || i == kPFull + 1 ? kTile : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
@@ -62,54 +61,51 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
 
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
-    if (warp == kMmaWarp) {
-      if (n > 0) {
-        const uint32_t on = elect_one();
-        wait_bar(bar(kQFull), 0, failed, &g_packed_error);
-        wait_bar(bar(kKFull), 0, failed, &g_packed_error);
-        fence_after();
-        if (n0 > 0) { product_rows<T>(on, tmem, sq, sk, d); commit(on, bar(kSFull)); }
-        if (n1 > 0) { product_rows<T>(on, tmem + kTile, sq + tile_bytes, sk, d); commit(on, bar(kSFull + 1)); }
-        if (n > 2) commit(on, bar(kKEmpty));      // only where a loader waits: nothing is pending when the CTA ends
-        for (int i = 0; i < n; ++i) {
-          const int st = i & 1, nx = (i + 1) & 1;
-          wait_bar(bar(kVFull + st), (i >> 1) & 1, failed, &g_packed_error);
-          if (i + 1 < n) wait_bar(bar(kKFull + nx), ((i + 1) >> 1) & 1, failed, &g_packed_error);
+    if (warp == kMmaWarp && n > 0) {
+      const uint32_t on = elect_one();
+      // keys are tiles 0, 2, .. of the ring, values 1, 3, ..; a slot is given back only where another tile waits for it, so that nothing is
+      // pending when the CTA ends
+      auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
+      auto ready = [&](int j) { wait_bar(bar(kFull + j % R), (j / R) & 1, failed, &g_packed_error); };
+      auto give = [&](int j) { if (j + R < 2 * n) commit(on, bar(kEmpty + j % R)); };
+      ready(0);
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            const int nt = t ? n1 : n0;
-            if (i >= nt) continue;
-            wait_bar(bar(kPFull + t), i & 1, failed, &g_packed_error);
-            fence_after();
-            product_cols<T>(on, tmem + 256 + kTile * t, tmem + kTile * t, 32, sv + st * tile_bytes, d, i > 0);
-            if (i + 1 < nt) {
-              product_rows<T>(on, tmem + kTile * t, sq + t * tile_bytes, sk + nx * tile_bytes, d);
-              commit(on, bar(kSFull + t));
-            } else {
-              commit(on, bar(kOFull + t));
-            }
-          }
-          if (i + 2 < n) commit(on, bar(kVEmpty + st));
-          if (i + 3 < n) commit(on, bar(kKEmpty + nx));
-        }
+      for (int t = 0; t < 2; ++t) {
+        if ((t ? n1 : n0) == 0) continue;
+        wait_bar(bar(kQFull + t), 0, failed, &g_packed_error);
+        fence_after();
+        product_rows<T>(on, tmem + kTile * t, sq + t * tile_bytes, slot(0), d);
+        commit(on, bar(kSFull + t));
       }
-    } else {
-      Loader ld{lane, warp - kMmaWarp - 1};
-      auto which = [&](int j) { return j == 0 ? bar(kQFull) : (j & 1) ? bar(kKFull + (((j - 1) >> 1) & 1)) : bar(kVFull + (((j - 2) >> 1) & 1)); };
-      if (n > 0) {
-        ld.tile<T>(sq, a.q, h, q0, row0, lq, d);
-        ld.tile<T>(sq + tile_bytes, a.q, h, q0, row0 + kTile, lq, d);
-        ld.done(which);
-        for (int i = 0; i < n; ++i) {
-          const int st = i & 1;
-          if (i >= 2) ld.room(bar(kKEmpty + st), ((i >> 1) - 1) & 1, failed, &g_packed_error, which);
-          ld.tile<T>(sk + st * tile_bytes, a.k, kvh, c0, i * kTile, lk, d);
-          ld.done(which);
-          if (i >= 2) ld.room(bar(kVEmpty + st), ((i >> 1) - 1) & 1, failed, &g_packed_error, which);
-          ld.tile<T>(sv + st * tile_bytes, a.v, kvh, c0, i * kTile, lk, d);
-          ld.done(which);
+      give(0);
+      for (int i = 0; i < n; ++i) {
+        ready(2 * i + 1);
+        if (i + 1 < n) ready(2 * i + 2);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          const int nt = t ? n1 : n0;
+          if (i >= nt) continue;
+          wait_bar(bar(kPFull + t), i & 1, failed, &g_packed_error);
+          fence_after();
+          product_cols<T>(on, tmem + 256 + kTile * t, tmem + kTile * t, 32, slot(2 * i + 1), d, i > 0);
+          if (i + 1 < nt) {
+            product_rows<T>(on, tmem + kTile * t, sq + t * tile_bytes, slot(2 * i + 2), d);
+            commit(on, bar(kSFull + t));
+          } else {
+            commit(on, bar(kOFull + t));
+          }
         }
-        ld.flush(which);
+        give(2 * i + 1);
+        if (i + 1 < n) give(2 * i + 2);
+      }
+    } else if (warp == kLoadWarp && n > 0) {
+      Loader ld{lane, subs, bar(kFix)};
+      for (int t = 0; t < 2; ++t)
+        if ((t ? n1 : n0) > 0) ld.tile(sq + t * tile_bytes, &maps.q, q0 + row0 + t * kTile, h, bar(kQFull + t), kTile, false, failed, &g_packed_error);
+      for (int j = 0; j < 2 * n; ++j) {
+        if (j >= R) wait_bar(bar(kEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
+        const int r = (j >> 1) * kTile;
+        ld.tile(ring + (j % R) * tile_bytes, (j & 1) ? &maps.v : &maps.k, c0 + r, kvh, bar(kFull + j % R), lk - r, j & 1, failed, &g_packed_error);
       }
     }
   } else {
@@ -204,15 +200,15 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
 // 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256.  The two groups of four warps
 // have 64 columns each of every row.  The next tile's logits are made as soon as these have been read, so that its exponentials run
 // beside the products dS k and g v^T.
-enum DqBar { kdqQ, kdqKFull, kdqKEmpty = kdqKFull + 2, kdqVFull = kdqKEmpty + 2, kdqVEmpty = kdqVFull + 2, kdqS = kdqVEmpty + 2, kdqSRead, kdqDp, kdqDs,
-             kdqOut, kDqBars };
+enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqS, kdqSRead, kdqDp, kdqDs, kdqOut, kdqFix, kDqBars };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int d = a.d, tile_bytes = d * 256;
-  Tail* tail = reinterpret_cast<Tail*>(smem + 6 * tile_bytes);
-  const uint32_t sq = smem_addr(smem), sg = sq + tile_bytes, sk = sg + tile_bytes, sv = sk + 2 * tile_bytes, bar0 = smem_addr(tail->bars);
+__global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
+  extern __shared__ unsigned char raw[];
+  unsigned char* smem = aligned_smem(raw);
+  const int d = a.d, subs = d > 64 ? 2 : 1, tile_bytes = subs * kSub, R = ring_slots(subs);
+  Tail* tail = reinterpret_cast<Tail*>(smem + (2 + R) * tile_bytes);
+  const uint32_t sq = smem_addr(smem), sg = sq + tile_bytes, ring = sg + tile_bytes, bar0 = smem_addr(tail->bars);
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -222,13 +218,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a) {
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
-    init_bar(bar(kdqQ), 32 * kLoadWarps);
-    for (int i = 0; i < 2; ++i) {
-      init_bar(bar(kdqKFull + i), 32 * kLoadWarps); init_bar(bar(kdqVFull + i), 32 * kLoadWarps);
-      init_bar(bar(kdqKEmpty + i), 1); init_bar(bar(kdqVEmpty + i), 1);
-    }
-    init_bar(bar(kdqS), 1); init_bar(bar(kdqDp), 1); init_bar(bar(kdqOut), 1);
-    init_bar(bar(kdqSRead), 256); init_bar(bar(kdqDs), 256);
+    for (int i = 0; i < kDqBars; ++i) init_bar(bar(i), i == kdqSRead || i == kdqDs ? 256 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
@@ -238,58 +228,52 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a) {
 
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
-    if (warp == kMmaWarp) {
-      if (n > 0) {
-        const uint32_t on = elect_one();
-        wait_bar(bar(kdqQ), 0, failed, &g_packed_error);
-        wait_bar(bar(kdqKFull), 0, failed, &g_packed_error);
-        fence_after();
-        product_rows<T>(on, tmem, sq, sk, d);
-        commit(on, bar(kdqS));
-        wait_bar(bar(kdqVFull), 0, failed, &g_packed_error);
-        fence_after();
-        product_rows<T>(on, tmem + kTile, sg, sv, d);
-        commit(on, bar(kdqDp));
-        if (n > 2) commit(on, bar(kdqVEmpty));
-        for (int i = 0; i < n; ++i) {
-          const int st = i & 1, nx = st ^ 1, ph = ((i + 1) >> 1) & 1;
-          if (i + 1 < n) {
-            wait_bar(bar(kdqKFull + nx), ph, failed, &g_packed_error);
-            wait_bar(bar(kdqSRead), i & 1, failed, &g_packed_error);
-            fence_after();
-            product_rows<T>(on, tmem, sq, sk + nx * tile_bytes, d);
-            commit(on, bar(kdqS));
-          }
-          wait_bar(bar(kdqDs), i & 1, failed, &g_packed_error);
-          fence_after();
-          product_cols<T>(on, tmem + 256, tmem + kTile, 64, sk + st * tile_bytes, d, i > 0);
-          if (i + 2 < n) commit(on, bar(kdqKEmpty + st));
-          if (i + 1 < n) {
-            wait_bar(bar(kdqVFull + nx), ph, failed, &g_packed_error);
-            fence_after();
-            product_rows<T>(on, tmem + kTile, sg, sv + nx * tile_bytes, d);
-            commit(on, bar(kdqDp));
-            if (i + 3 < n) commit(on, bar(kdqVEmpty + nx));
-          }
-        }
-        commit(on, bar(kdqOut));
-      }
-    } else if (n > 0) {
-      Loader ld{lane, warp - kMmaWarp - 1};
-      auto which = [&](int j) { return j == 0 ? bar(kdqQ) : (j & 1) ? bar(kdqKFull + (((j - 1) >> 1) & 1)) : bar(kdqVFull + (((j - 2) >> 1) & 1)); };
-      ld.tile<T>(sq, a.q, h, q0, row0, lq, d);
-      ld.tile<T>(sg, a.g, h, q0, row0, lq, d);
-      ld.done(which);
+    if (warp == kMmaWarp && n > 0) {
+      const uint32_t on = elect_one();
+      auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
+      auto ready = [&](int j) { wait_bar(bar(kdqFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
+      auto give = [&](int j) { if (j + R < 2 * n) commit(on, bar(kdqEmpty + j % R)); };
+      wait_bar(bar(kdqQ), 0, failed, &g_packed_error);
+      ready(0);
+      product_rows<T>(on, tmem, sq, slot(0), d);
+      commit(on, bar(kdqS));
+      ready(1);
+      product_rows<T>(on, tmem + kTile, sg, slot(1), d);
+      commit(on, bar(kdqDp));
+      give(1);
       for (int i = 0; i < n; ++i) {
-        const int st = i & 1;
-        if (i >= 2) ld.room(bar(kdqKEmpty + st), ((i >> 1) - 1) & 1, failed, &g_packed_error, which);
-        ld.tile<T>(sk + st * tile_bytes, a.k, kvh, c0, i * kTile, lk, d);
-        ld.done(which);
-        if (i >= 2) ld.room(bar(kdqVEmpty + st), ((i >> 1) - 1) & 1, failed, &g_packed_error, which);
-        ld.tile<T>(sv + st * tile_bytes, a.v, kvh, c0, i * kTile, lk, d);
-        ld.done(which);
+        if (i + 1 < n) {
+          ready(2 * i + 2);
+          wait_bar(bar(kdqSRead), i & 1, failed, &g_packed_error);
+          fence_after();
+          product_rows<T>(on, tmem, sq, slot(2 * i + 2), d);
+          commit(on, bar(kdqS));
+        }
+        wait_bar(bar(kdqDs), i & 1, failed, &g_packed_error);
+        fence_after();
+        product_cols<T>(on, tmem + 256, tmem + kTile, 64, slot(2 * i), d, i > 0);
+        give(2 * i);
+        if (i + 1 < n) {
+          ready(2 * i + 3);
+          product_rows<T>(on, tmem + kTile, sg, slot(2 * i + 3), d);
+          commit(on, bar(kdqDp));
+          give(2 * i + 3);
+        }
       }
-      ld.flush(which);
+      commit(on, bar(kdqOut));
+    } else if (warp == kLoadWarp && n > 0) {
+      Loader ld{lane, subs, bar(kdqFix)};
+      if (lane == 0) {
+        expect(bar(kdqQ), 2 * tile_bytes);
+        ld.copies(sq, &maps.q, q0 + row0, h, bar(kdqQ));
+        ld.copies(sg, &maps.g, q0 + row0, h, bar(kdqQ));
+      }
+      __syncwarp();
+      for (int j = 0; j < 2 * n; ++j) {
+        if (j >= R) wait_bar(bar(kdqEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
+        const int r = (j >> 1) * kTile;
+        ld.tile(ring + (j % R) * tile_bytes, (j & 1) ? &maps.v : &maps.k, c0 + r, kvh, bar(kdqFull + j % R), lk - r, !(j & 1), failed, &g_packed_error);
+      }
     }
   } else {
     more_regs<kComputeRegs>();
@@ -358,16 +342,17 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a) {
 // 128 keys of one key head: rows of the products are keys, columns the queries of all heads of the group, 128 at a time.  Tensor memory:
 // logits at 0 (P replaces them), dP at 128 (dS replaces it), dv at 256, dk at 384.  The tensor cores work in the order
 // dv(i), logits(i + 1), dk(i), dP(i + 1): each pair runs beside the other half of the elementwise work.
-enum DkvBar { kkvK, kkvQFull, kkvQEmpty = kkvQFull + 2, kkvGFull = kkvQEmpty + 2, kkvGEmpty = kkvGFull + 2, kkvS = kkvGEmpty + 2, kkvP, kkvDp, kkvDs, kkvOut,
-              kDkvBars };
+enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvFix, kkvStat, kkvStatFree = kkvStat + 2,
+              kDkvBars = kkvStatFree + 2 };
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a) {
-  extern __shared__ __align__(128) unsigned char smem[];
-  const int d = a.d, tile_bytes = d * 256;
-  float* stats = reinterpret_cast<float*>(smem + 6 * tile_bytes);      // [2][128] -lse in log2, [2][128] -delta
-  Tail* tail = reinterpret_cast<Tail*>(smem + 6 * tile_bytes + 4 * kTile * 4);
-  const uint32_t sk = smem_addr(smem), sv = sk + tile_bytes, sq = sv + tile_bytes, sg = sq + 2 * tile_bytes, bar0 = smem_addr(tail->bars);
+__global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
+  extern __shared__ unsigned char raw[];
+  unsigned char* smem = aligned_smem(raw);
+  const int d = a.d, subs = d > 64 ? 2 : 1, tile_bytes = subs * kSub, R = ring_slots(subs);
+  float* stats = reinterpret_cast<float*>(smem + (2 + R) * tile_bytes);      // [2][128] -lse in log2, [2][128] -delta
+  Tail* tail = reinterpret_cast<Tail*>(stats + 4 * kTile);
+  const uint32_t sk = smem_addr(smem), sv = sk + tile_bytes, ring = sv + tile_bytes, bar0 = smem_addr(tail->bars);
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -378,13 +363,8 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a) {
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
-    init_bar(bar(kkvK), 32 * kLoadWarps);
-    for (int i = 0; i < 2; ++i) {
-      init_bar(bar(kkvQFull + i), 32 * kLoadWarps); init_bar(bar(kkvGFull + i), 32 * kLoadWarps);
-      init_bar(bar(kkvQEmpty + i), 1); init_bar(bar(kkvGEmpty + i), 1);
-    }
-    init_bar(bar(kkvS), 1); init_bar(bar(kkvDp), 1); init_bar(bar(kkvOut), 1);
-    init_bar(bar(kkvP), 256); init_bar(bar(kkvDs), 256);
+    for (int i = 0; i < kDkvBars; ++i)
+      init_bar(bar(i), i == kkvP || i == kkvDs ? 256 : i == kkvStat || i == kkvStat + 1 ? 64 : i == kkvStatFree || i == kkvStatFree + 1 ? 8 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
@@ -394,67 +374,65 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a) {
 
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
-    if (warp == kMmaWarp) {
-      if (n > 0) {
-        const uint32_t on = elect_one(), dv = tmem + 256, dk = tmem + 256 + kTile;
-        wait_bar(bar(kkvK), 0, failed, &g_packed_error);
-        wait_bar(bar(kkvQFull), 0, failed, &g_packed_error);
-        fence_after();
-        product_rows<T>(on, tmem, sk, sq, d);
-        commit(on, bar(kkvS));
-        wait_bar(bar(kkvGFull), 0, failed, &g_packed_error);
-        fence_after();
-        product_rows<T>(on, tmem + kTile, sv, sg, d);
-        commit(on, bar(kkvDp));
-        for (int i = 0; i < n; ++i) {
-          const int st = i & 1, nx = st ^ 1, ph = ((i + 1) >> 1) & 1;
-          wait_bar(bar(kkvP), i & 1, failed, &g_packed_error);
-          fence_after();
-          product_cols<T>(on, dv, tmem, 64, sg + st * tile_bytes, d, i > 0);
-          if (i + 2 < n) commit(on, bar(kkvGEmpty + st));
-          if (i + 1 < n) {
-            wait_bar(bar(kkvQFull + nx), ph, failed, &g_packed_error);
-            fence_after();
-            product_rows<T>(on, tmem, sk, sq + nx * tile_bytes, d);
-            commit(on, bar(kkvS));
-          }
-          wait_bar(bar(kkvDs), i & 1, failed, &g_packed_error);
-          fence_after();
-          product_cols<T>(on, dk, tmem + kTile, 64, sq + st * tile_bytes, d, i > 0);
-          if (i + 2 < n) commit(on, bar(kkvQEmpty + st));
-          if (i + 1 < n) {
-            wait_bar(bar(kkvGFull + nx), ph, failed, &g_packed_error);
-            fence_after();
-            product_rows<T>(on, tmem + kTile, sv, sg + nx * tile_bytes, d);
-            commit(on, bar(kkvDp));
-          }
-        }
-        commit(on, bar(kkvOut));
-      }
-    } else if (n > 0) {
-      Loader ld{lane, warp - kMmaWarp - 1};
-      auto which = [&](int j) { return j == 0 ? bar(kkvK) : (j & 1) ? bar(kkvQFull + (((j - 1) >> 1) & 1)) : bar(kkvGFull + (((j - 2) >> 1) & 1)); };
-      ld.tile<T>(sk, a.k, kvh, c0, row0, lk, d);
-      ld.tile<T>(sv, a.v, kvh, c0, row0, lk, d);
-      ld.done(which);
+    if (warp == kMmaWarp && n > 0) {
+      const uint32_t on = elect_one(), dv = tmem + 256, dk = tmem + 256 + kTile;
+      auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };      // queries 0, 2, .., cotangents 1, 3, ..
+      auto ready = [&](int j) { wait_bar(bar(kkvFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
+      auto give = [&](int j) { if (j + R < 2 * n) commit(on, bar(kkvEmpty + j % R)); };
+      wait_bar(bar(kkvK), 0, failed, &g_packed_error);
+      ready(0);
+      product_rows<T>(on, tmem, sk, slot(0), d);
+      commit(on, bar(kkvS));
+      ready(1);
+      product_rows<T>(on, tmem + kTile, sv, slot(1), d);
+      commit(on, bar(kkvDp));
       for (int i = 0; i < n; ++i) {
-        const int st = i & 1, h = kvh * a.group + i / per, b = i0 + (i % per) * kTile;
-        // The statistics travel with the queries: their place is free when dk of two tiles ago is done, and the barrier of the queries
-        // makes them visible (plain stores ahead of the arrival).
-        if (i >= 2) ld.room(bar(kkvQEmpty + st), ((i >> 1) - 1) & 1, failed, &g_packed_error, which);
-        ld.tile<T>(sq + st * tile_bytes, a.q, h, q0, b, lq, d);
-        for (int r = ld.warp * 32 + lane; r < kTile; r += 32 * kLoadWarps) {
+        wait_bar(bar(kkvP), i & 1, failed, &g_packed_error);
+        fence_after();
+        product_cols<T>(on, dv, tmem, 64, slot(2 * i + 1), d, i > 0);
+        give(2 * i + 1);
+        if (i + 1 < n) {
+          ready(2 * i + 2);
+          product_rows<T>(on, tmem, sk, slot(2 * i + 2), d);
+          commit(on, bar(kkvS));
+        }
+        wait_bar(bar(kkvDs), i & 1, failed, &g_packed_error);
+        fence_after();
+        product_cols<T>(on, dk, tmem + kTile, 64, slot(2 * i), d, i > 0);
+        give(2 * i);
+        if (i + 1 < n) {
+          ready(2 * i + 3);
+          product_rows<T>(on, tmem + kTile, sv, slot(2 * i + 3), d);
+          commit(on, bar(kkvDp));
+        }
+      }
+      commit(on, bar(kkvOut));
+    } else if (warp == kLoadWarp && n > 0) {
+      Loader ld{lane, subs, bar(kkvFix)};
+      if (lane == 0) {
+        expect(bar(kkvK), 2 * tile_bytes);
+        ld.copies(sk, &maps.k, c0 + row0, kvh, bar(kkvK));
+        ld.copies(sv, &maps.v, c0 + row0, kvh, bar(kkvK));
+      }
+      __syncwarp();
+      for (int j = 0; j < 2 * n; ++j) {
+        if (j >= R) wait_bar(bar(kkvEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
+        const int i = j >> 1, hq = kvh * a.group + i / per, b = i0 + (i % per) * kTile;
+        ld.tile(ring + (j % R) * tile_bytes, (j & 1) ? &maps.g : &maps.q, q0 + b, hq, bar(kkvFull + j % R), lq - b, true, failed, &g_packed_error);
+      }
+    } else if (warp > kLoadWarp) {
+      const int r0 = (warp - kLoadWarp - 1) * 32 + lane;
+      for (int i = 0; i < n; ++i) {
+        const int st = i & 1, hq = kvh * a.group + i / per, b = i0 + (i % per) * kTile;
+        if (i >= 2) wait_bar(bar(kkvStatFree + st), ((i >> 1) - 1) & 1, failed, &g_packed_error);
+        for (int r = r0; r < kTile; r += 64) {
           const bool ok = b + r < lq;
-          const long long at = (long long)h * a.nq + q0 + b + r;
+          const long long at = (long long)hq * a.nq + q0 + b + r;
           stats[st * kTile + r] = ok ? fmaf(-a.lse[at], kLog2e, packed::prob_shift<T>()) : -INFINITY;
           stats[(2 + st) * kTile + r] = ok ? -a.delta[at] * packed::prob_unscale<T>() : 0.f;
         }
-        ld.done(which);
-        if (i >= 2) ld.room(bar(kkvGEmpty + st), ((i >> 1) - 1) & 1, failed, &g_packed_error, which);
-        ld.tile<T>(sg + st * tile_bytes, a.g, h, q0, b, lq, d);
-        ld.done(which);
+        arrive(bar(kkvStat + st));
       }
-      ld.flush(which);
     }
   } else {
     more_regs<kComputeRegs>();
@@ -465,7 +443,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a) {
     for (int i = 0; i < n; ++i) {
       const int st = i & 1, ib = i0 + (i % per) * kTile + col;
       uint32_t x[64], y[64];
-      wait_bar(bar(kkvQFull + st), (i >> 1) & 1, failed, &g_packed_error);      // the statistics
+      wait_bar(bar(kkvStat + st), (i >> 1) & 1, failed, &g_packed_error);
       wait_bar(bar(kkvS), i & 1, failed, &g_packed_error);
       fence_after();
       ld32(lanes + col, x);
@@ -506,6 +484,8 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a) {
         y[2 * c] = packed::Half<T>::pack(s0, s1);
         y[2 * c + 1] = packed::Half<T>::pack(s2, s3);
       }
+      __syncwarp();
+      if (lane == 0) arrive(bar(kkvStatFree + st));
       st16(lanes + kTile + col, y);
       st16(lanes + kTile + col + 16, y + 16);
       wait_st();
@@ -541,30 +521,65 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a) {
   if (warp == kMmaWarp) { fence_after(); free_tmem(tmem); }
 }
 
-static_assert(kFwdBars <= 20 && kDqBars <= 20 && kDkvBars <= 20, "barriers");
-int smem_bytes(int d, bool stats) { return 6 * d * 256 + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail); }
+static_assert(kFwdBars <= 32 && kDqBars <= 32 && kDkvBars <= 32, "barriers");
+int smem_bytes(int d, bool stats) { return 1024 + (d > 64 ? 6 * 2 : 10) * (int)kSub + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail); }
+
+using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                            CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+Encode encoder() {
+  static const Encode fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &found) != cudaSuccess || found != cudaDriverEntryPointSuccess) p = nullptr;
+    return reinterpret_cast<Encode>(p);
+  }();
+  return fn;
+}
+template <typename T> bool map_of(CUtensorMap* m, const Rows& r, long long rows, int heads, int d) {
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)heads};
+  const cuuint64_t strides[2] = {(cuuint64_t)r.row * 2, (cuuint64_t)r.head * 2};
+  const cuuint32_t box[3] = {64, kTile, 1}, ones[3] = {1, 1, 1};
+  return encoder()(m, std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(r.p), dims,
+                   strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+template <typename T> bool maps_of(Maps* m, const PackedArgs& a, bool reverse) {
+  if (!encoder()) return false;
+  return map_of<T>(&m->q, a.q, a.nq, a.hq, a.d) && map_of<T>(&m->k, a.k, a.nkv, a.hk, a.d) && map_of<T>(&m->v, a.v, a.nkv, a.hk, a.d) &&
+         (reverse ? map_of<T>(&m->g, a.g, a.nq, a.hq, a.d) : (m->g = m->q, true));
+}
+template <typename K> int launch(K kernel, dim3 grid, bool stats, cudaStream_t st, const PackedArgs& a, const Maps& m) {
+  const int smem = smem_bytes(a.d, stats);
+  SO3LR_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  kernel<<<grid, kThreads, smem, st>>>(a, m);
+  count_launch();
+  return kOk;
+}
 
 }  // namespace
 
-template <typename T> void packed_forward_tc(cudaStream_t st, const PackedArgs& a, int n_items) {
-  packed::launch(forward_kernel<T>, dim3(n_items, a.hq), kThreads, smem_bytes(a.d, false), st, a);
+template <typename T> int packed_forward_tc(cudaStream_t st, const PackedArgs& a, int n_items) {
+  Maps m;
+  if (!maps_of<T>(&m, a, false)) return kInvalidArgument;
+  return launch(forward_kernel<T>, dim3(n_items, a.hq), false, st, a, m);
 }
-template <typename T> void packed_dq_tc(cudaStream_t st, const PackedArgs& a, int n_items) {
-  packed::launch(dq_kernel<T>, dim3(n_items, a.hq), kThreads, smem_bytes(a.d, false), st, a);
-}
-template <typename T> void packed_dkv_tc(cudaStream_t st, const PackedArgs& a, int n_items) {
-  packed::launch(dkv_kernel<T>, dim3(n_items, a.hk), kThreads, smem_bytes(a.d, true), st, a);
+template <typename T> int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv) {
+  Maps m;
+  if (!maps_of<T>(&m, a, true)) return kInvalidArgument;
+  a.items = items_q;
+  const int rc = launch(dq_kernel<T>, dim3(n_q, a.hq), false, st, a, m);
+  if (rc) return rc;
+  a.items = items_kv;
+  return launch(dkv_kernel<T>, dim3(n_kv, a.hk), true, st, a, m);
 }
 int packed_error(int* out) {
   const cudaError_t e = cudaMemcpyFromSymbol(out, g_packed_error, sizeof(int));
   return e == cudaSuccess ? kOk : kCudaError;
 }
 
-template void packed_forward_tc<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
-template void packed_forward_tc<__half>(cudaStream_t, const PackedArgs&, int);
-template void packed_dq_tc<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
-template void packed_dq_tc<__half>(cudaStream_t, const PackedArgs&, int);
-template void packed_dkv_tc<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
-template void packed_dkv_tc<__half>(cudaStream_t, const PackedArgs&, int);
+template int packed_forward_tc<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
+template int packed_forward_tc<__half>(cudaStream_t, const PackedArgs&, int);
+template int packed_reverse_tc<__nv_bfloat16>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int);
+template int packed_reverse_tc<__half>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int);
 
 }  // namespace so3lr

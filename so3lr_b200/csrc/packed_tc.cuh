@@ -1,25 +1,24 @@
 // What the tensor-core kernels of attention inside packed structures share: operand tiles, descriptors, barriers, tensor memory.
 //
-// Every operand tile is 128 rows x d values in one image: 16-byte pieces (8 values) of column group c of row r at c * 2048 + r * 16.  That
-// is the core-matrix layout of tcgen05.mma without a swizzle for rows as M or N with d contracted (K-major), and for d as N with the rows
-// contracted (MN-major) as well, so a tile of keys serves q k^T and dS k, a tile of queries k q^T and dS^T q.  Loader warps fill it
-// with 16-byte asynchronous copies, eight rows x four pieces an instruction: 64-byte stretches of global memory, shared memory without
-// bank conflicts, any strides, rows and columns that are not there as zeros.
+// An operand tile is 128 rows of 64 values (128 bytes a row, 128-byte swizzle), one or two of them side by side for up to 64 or 128 values
+// a head, brought in by TMA from the strided operand: a map has the dimensions (values, rows, heads), values behind the last one come as
+// zeros.  The same image serves the tensor cores with d contracted (K-major) and with the rows contracted (MN-major), so a tile of keys
+// serves q k^T and dS k, a tile of queries k q^T and dS^T q.  A tile may reach over the end of its structure into the next one's rows: where
+// they would be contracted, the loading warp clears them before it hands the tile over (a zero probability times a neighbour's NaN is NaN).
 #pragma once
+#include <cuda.h>
+
 #include "packed_mma.cuh"
 
 namespace so3lr {
 namespace tc {
 
-using packed::copy16;
-using packed::copy_commit;
-using packed::copy_wait;
 using packed::kLn2;
 using packed::kLog2e;
 using packed::smem_addr;
 
 constexpr int kTile = 128;
-constexpr int kComputeWarps = 8, kMmaWarp = 8, kLoadWarps = 3;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;      // 0 .. 7 compute, 10 and 11 fetch statistics in the kernel of dk and dv
 constexpr int kThreads = 384;
 // registers a thread of the compute and of the other warps after the split: 256 x 208 + 128 x 88 = 384 x 168, the launch's total
 constexpr int kComputeRegs = 208, kOtherRegs = 88;
@@ -72,13 +71,14 @@ __device__ __forceinline__ float pow2(float x) {
 }
 
 // ---- matrix instructions ----
-// descriptor of an operand tile: rows as M or N and columns contracted (K-major), or columns as N and rows contracted (MN-major); bytes
-// between core matrices along the contracted index, then along the other one
+// Descriptor of an operand tile, 128-byte swizzle.  K-major: 16 contracted values are 32 bytes further, 64 are a sub-tile further; groups of
+// eight rows lie 1024 bytes apart.  MN-major: 16 contracted rows are 2048 bytes further, 64 values of N a sub-tile.
+constexpr uint32_t kSub = 128 * 128;       // bytes of a sub-tile
 __device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn_major) {
-  const uint32_t lbo = mn_major ? 128 : 2048, sbo = mn_major ? 2048 : 128;
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(lbo >> 4) << 16) | ((uint64_t)(sbo >> 4) << 32) | ((uint64_t)1 << 46);
+  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(mn_major ? kSub >> 4 : 1) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
-constexpr uint32_t kStepK = 4096 >> 4, kStepMn = 256 >> 4;      // 16 contracted entries further, in descriptor units
+__device__ __forceinline__ uint32_t step_k(int k) { return ((k & 3) * 32 + (k >> 2) * kSub) >> 4; }
+constexpr uint32_t kStepMn = 2048 >> 4;
 template <typename T> __device__ __forceinline__ uint32_t idesc(int n, bool b_mn_major) {
   const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
@@ -104,7 +104,7 @@ template <typename T> __device__ __forceinline__ void product_rows(uint32_t on, 
   const uint64_t da = desc(a, false), db = desc(b, false);
   const uint32_t id = idesc<T>(kTile, false);
 #pragma unroll 1
-  for (int k = 0; k < d / 16; ++k) mma_ss(on, dst, da + k * kStepK, db + k * kStepK, id, k > 0);
+  for (int k = 0; k < d / 16; ++k) mma_ss(on, dst, da + step_k(k), db + step_k(k), id, k > 0);
 }
 // D[128 x d] (+)= A B: A 128 x 128 in tensor memory, 64 packed columns as two halves `gap` columns apart, B a tile with its rows contracted
 template <typename T> __device__ __forceinline__ void product_cols(uint32_t on, uint32_t dst, uint32_t a, int gap, uint32_t b, int d, uint32_t acc) {
@@ -143,50 +143,46 @@ template <int N> __device__ __forceinline__ void wait_ld(uint32_t (&r)[N]) {
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // ---- loading ----
-// Groups of copies in order; group j is announced on its barrier when it has landed and is visible to the tensor cores.  At most two
-// stay in flight behind the one just issued; a loader that has to wait for room first announces all it has.
+struct Maps { CUtensorMap q, k, v, g; };
+__device__ __forceinline__ void tma(uint32_t dst, const CUtensorMap* map, int x, int row, int head, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(map), "r"(x), "r"(row), "r"(head), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// The whole loading warp calls it.  rows: how many of the tile's 128 rows belong to the structure; where `clear`, the others are cleared
+// (through `fix`, a barrier of this warp's own, and its parity).
 struct Loader {
-  int lane, warp;            // 0 .. kLoadWarps - 1
-  int issued = 0, told = 0;
-  template <typename T>
-  __device__ __forceinline__ void tile(uint32_t dst, const Rows& src, int head, long long base, int r0, int r1, int d) const {
-    const T* p = static_cast<const T*>(src.p) + head * src.head;
-    const int pieces = d >> 3, groups = (pieces + 3) >> 2;
-    for (int i = warp; i < 16 * groups; i += kLoadWarps) {
-      const int r = (i & 15) * 8 + (lane & 7), c = (i >> 4) * 4 + (lane >> 3);
-      if (c < pieces) {
-        const bool ok = r0 + r < r1;
-        copy16(dst + c * 2048 + r * 16, ok ? p + (base + r0 + r) * src.row + c * 8 : p, ok);
-      }
+  int lane, subs;
+  uint32_t fix, parity = 0;
+  __device__ __forceinline__ void copies(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t bar) const {
+    for (int x = 0; x < subs; ++x) tma(dst + x * kSub, map, 64 * x, row, head, bar);
+  }
+  __device__ __forceinline__ void tile(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t full, int rows, bool clear, volatile int* failed,
+                                       int* error) {
+    if (!clear || rows >= kTile) {
+      if (lane == 0) { expect(full, subs * kSub); copies(dst, map, row, head, full); }
+      __syncwarp();
+      return;
     }
-  }
-  // bar(j): barrier of group j
-  template <typename F> __device__ __forceinline__ void tell(int upto, F bar) {
-    if (told >= upto) return;
+    if (lane == 0) { expect(fix, subs * kSub); copies(dst, map, row, head, fix); }
+    __syncwarp();
+    wait_bar(fix, parity, failed, error);
+    parity ^= 1;
+    for (int x = 0; x < subs; ++x)
+      for (int b = rows * 128 + lane * 16; b < (int)kSub; b += 512)
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + x * kSub + b), "r"(0) : "memory");
     fence_smem();
-    for (; told < upto; ++told) arrive(bar(told));
-  }
-  template <typename F> __device__ __forceinline__ void done(F bar) {
-    copy_commit();
-    ++issued;
-    copy_wait<2>();
-    tell(issued - 2, bar);
-  }
-  template <typename F> __device__ __forceinline__ void flush(F bar) {
-    copy_wait<0>();
-    tell(issued, bar);
-  }
-  template <typename F> __device__ __forceinline__ void room(uint32_t empty, uint32_t parity, volatile int* failed, int* error, F bar) {
-    if (test_bar(empty, parity)) return;
-    flush(bar);
-    wait_bar(empty, parity, failed, error);
+    __syncwarp();
+    if (lane == 0) arrive(full);
+    __syncwarp();
   }
 };
 
-__device__ __forceinline__ uint32_t alloc_tmem(uint32_t* where) {
+__device__ __forceinline__ void alloc_tmem(uint32_t* where) {
   asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(where)), "r"(512) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  return 0;
 }
 __device__ __forceinline__ void free_tmem(uint32_t tmem) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
