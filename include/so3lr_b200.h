@@ -425,17 +425,20 @@ typedef struct {
   float scale;                     /* of the logits, positive */
 } so3lr_b200_attention_shape;
 
-/* out (rows_q, heads_q, d) contiguous; lse (heads_q, rows_q) float32 or NULL: logarithm of the sum of exponentials (-inf and
- * out = 0 for a row without keys).  Values that are not finite spoil the rows of their own structure only. */
-SO3LR_B200_API int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* shape);
+/* out (rows_q, heads_q, d) contiguous; out_rest the same or NULL: what rounding out to a 16-bit type left, for the transpose; lse (heads_q,
+ * rows_q) float32 or NULL: logarithm to base 2 of the sum of exponentials (-inf and out = 0 for a row without keys).  Values that are not
+ * finite spoil the rows of their own structure only.  `vjp` of the workspace's size: 0 for the forward call, 1 for its transpose. */
+SO3LR_B200_API int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* shape, int vjp);
 SO3LR_B200_API int so3lr_b200_structure_attention(const int32_t* image, const int32_t* image_dev, void* stream,
                                                   const so3lr_b200_attention_shape* shape, const so3lr_b200_rows* q, const so3lr_b200_rows* k,
-                                                  const so3lr_b200_rows* v, void* out, float* lse, void* workspace, int64_t workspace_bytes);
-/* gradients for the cotangent g of out; delta (heads_q, rows_q) float32 is scratch; d_q, d_k, d_v contiguous */
+                                                  const so3lr_b200_rows* v, void* out, void* out_rest, float* lse, void* workspace,
+                                                  int64_t workspace_bytes);
+/* gradients for the cotangent g of out; out_rest may be NULL; delta (heads_q, rows_q) float32 is scratch; d_q, d_k, d_v contiguous */
 SO3LR_B200_API int so3lr_b200_structure_attention_vjp(const int32_t* image, const int32_t* image_dev, void* stream,
                                                       const so3lr_b200_attention_shape* shape, const so3lr_b200_rows* q,
-                                                      const so3lr_b200_rows* k, const so3lr_b200_rows* v, const void* out, const float* lse,
-                                                      const so3lr_b200_rows* g, float* delta, void* d_q, void* d_k, void* d_v);
+                                                      const so3lr_b200_rows* k, const so3lr_b200_rows* v, const void* out, const void* out_rest,
+                                                      const float* lse, const so3lr_b200_rows* g, float* delta, void* d_q, void* d_k, void* d_v,
+                                                      void* workspace, int64_t workspace_bytes);
 /* 1 where a bounded wait of the tensor-core kernels has run out on the current device since the library was loaded (their rows are NaN
  * then); waits for the device */
 SO3LR_B200_API int so3lr_b200_structure_attention_error(int* out);

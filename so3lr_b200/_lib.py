@@ -102,9 +102,9 @@ def _load():
         "so3lr_b200_norm_rotate_vjp": (i32, [p] * 12 + [i64]),
         "so3lr_b200_packing_size": (i64, [i32, p, p]),
         "so3lr_b200_packing_build": (i32, [i32, p, p, i32, p, i64]),
-        "so3lr_b200_structure_attention_workspace": (i64, [p, p]),
-        "so3lr_b200_structure_attention": (i32, [p] * 10 + [i64]),
-        "so3lr_b200_structure_attention_vjp": (i32, [p] * 14),
+        "so3lr_b200_structure_attention_workspace": (i64, [p, p, i32]),
+        "so3lr_b200_structure_attention": (i32, [p] * 11 + [i64]),
+        "so3lr_b200_structure_attention_vjp": (i32, [p] * 16 + [i64]),
         "so3lr_b200_structure_attention_error": (i32, [C.POINTER(i32)]),
         "so3lr_b200_host_fail_allocation": (i64, [i64, i32]),
         "so3lr_b200_host_sph_harm": (None, [f32, f32, f32, p]),

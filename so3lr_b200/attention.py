@@ -112,33 +112,39 @@ class PackedStructures:
 # ------------------------------------------------------------------------------------------------------------
 # attention
 # ------------------------------------------------------------------------------------------------------------
-def _attention_forward(q, k, v, packed, shape, want_lse):
+def _workspace(packed, shape, vjp, device):
+    size = lib.so3lr_b200_structure_attention_workspace(packed._host, C.byref(shape), vjp)
+    return (torch.empty(size, dtype=torch.uint8, device=device), size) if size > 0 else (None, 0)
+
+
+def _attention_forward(q, k, v, packed, shape, train):
+    """(out, what rounding it left or None, lse or None)"""
     with torch.cuda.device(q.device):
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if want_lse else None
+        rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
+        lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if train else None
         if q.shape[0] > packed.rows_q:      # rows behind the last structure belong to none
             out[packed.rows_q:].zero_()
         if packed.rows_q:
-            size = lib.so3lr_b200_structure_attention_workspace(packed._host, C.byref(shape))
-            work = torch.empty(size, dtype=torch.uint8, device=q.device) if size > 0 else None
+            work, size = _workspace(packed, shape, 0, q.device)
             check(lib.so3lr_b200_structure_attention(packed._host, packed._table(q), _stream(q), C.byref(shape), C.byref(_rows(q)),
-                                                     C.byref(_rows(k)), C.byref(_rows(v)), _p(out), _p(lse), _p(work), max(size, 0)),
+                                                     C.byref(_rows(k)), C.byref(_rows(v)), _p(out), _p(rest), _p(lse), _p(work), size),
                   "structure_attention")
-    return out, lse
+    return out, rest, lse
 
 
 class _StructureAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, packed, shape):
-        out, lse = _attention_forward(q, k, v, packed, shape, True)
-        ctx.save_for_backward(q, k, v, out, lse)
+        out, rest, lse = _attention_forward(q, k, v, packed, shape, True)
+        ctx.save_for_backward(q, k, v, out, rest, lse)
         ctx.packed, ctx.shape = packed, shape
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q, k, v, out, lse = ctx.saved_tensors
+        q, k, v, out, rest, lse = ctx.saved_tensors
         packed = ctx.packed
         with torch.cuda.device(q.device):
             g = _head_rows("the cotangent", g, q.dtype, q.device)
@@ -149,9 +155,10 @@ class _StructureAttention(torch.autograd.Function):
                     t[n:].zero_()
             if packed.rows_q or packed.rows_kv:
                 delta = torch.empty_like(lse)
+                work, size = _workspace(packed, ctx.shape, 1, q.device)
                 check(lib.so3lr_b200_structure_attention_vjp(packed._host, packed._table(q), _stream(q), C.byref(ctx.shape), C.byref(_rows(q)),
-                                                             C.byref(_rows(k)), C.byref(_rows(v)), _p(out), _p(lse), C.byref(_rows(g)), _p(delta),
-                                                             _p(dq), _p(dk), _p(dv)), "structure_attention_vjp")
+                                                             C.byref(_rows(k)), C.byref(_rows(v)), _p(out), _p(rest), _p(lse), C.byref(_rows(g)),
+                                                             _p(delta), _p(dq), _p(dk), _p(dv), _p(work), size), "structure_attention_vjp")
         return dq, dk, dv, None, None
 
 

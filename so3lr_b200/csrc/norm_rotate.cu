@@ -8,10 +8,10 @@
 // With gy = g rotated by -theta and xhat = x / sqrt(..):  dw = sum of gy xhat,  dx = (w gy - xhat mean(w gy xhat)) / sqrt(..).
 //
 // Bound by memory: forward reads and writes every value once, the reverse pass reads x and g and writes dx.  A thread owns 16 bytes of both
-// halves of the pairs of one row (8 pairs of a 16-bit type, 4 of float32), so a row of 128 16-bit values takes 8 lanes; it keeps the cosines
-// and sines of its pairs in registers and walks over heads of one token, so that the angles, which are formed and reduced in double (the
-// position of a far token times a frequency near one loses its fraction in float32), cost once per token and not once per head.  With few
-// tokens the heads are spread over more threads instead (`slots`).
+// halves of the pairs of one row (8 pairs of a 16-bit type, 4 of float32), so a row of 128 16-bit values takes 8 lanes, and walks over heads of
+// one token; with few tokens the heads are spread over more threads (`slots`).  The cosines and sines of a CTA's tokens are formed
+// once, spread over its threads, into shared memory: the angle is formed and reduced in double (the position of a far token times a
+// frequency near one loses its fraction in float32), which costs more than all the rest of a row.
 #include "../../include/so3lr_b200.h"
 
 #include "kernels.h"
@@ -97,58 +97,70 @@ __device__ __forceinline__ void cos_sin(double theta, float& c, float& s) {
   if (q >= 2) s = -s;
 }
 
-template <int N>
-__device__ __forceinline__ void angles(const RotateArgs& A, int token, int p0, float* c, float* s) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) { c[i] = 1.f; s[i] = 0.f; }
-  if (!A.axes) return;
-  double th[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) th[i] = 0.0;
-  for (int a = 0; a < A.axes; ++a) {
-    const size_t at = (size_t)token * A.axes + a;
-    const double x = A.pos_f64 ? static_cast<const double*>(A.pos)[at] : (double)static_cast<const float*>(A.pos)[at];
-    const float* f = A.freq + (size_t)a * (A.d / 2) + p0;
-#pragma unroll
-    for (int i = 0; i < N; ++i) th[i] = fma(x, (double)f[i], th[i]);
+// cosines and sines of `tokens` tokens from t0 on, (tokens, d / 2), by the whole CTA
+__device__ __forceinline__ void angle_table(const RotateArgs& A, int t0, int tokens, float* c, float* s) {
+  const int half = A.d / 2;
+  for (int e = threadIdx.x; e < tokens * half; e += kThreads) {
+    const int token = t0 + e / half, p = e % half;
+    float cc = 1.f, ss = 0.f;
+    if (token < A.n && A.axes) {
+      double th = 0.0;
+      for (int a = 0; a < A.axes; ++a) {
+        const size_t at = (size_t)token * A.axes + a;
+        const double x = A.pos_f64 ? static_cast<const double*>(A.pos)[at] : (double)static_cast<const float*>(A.pos)[at];
+        th = fma(x, (double)A.freq[(size_t)a * half + p], th);
+      }
+      cos_sin(th, cc, ss);
+    }
+    c[e] = cc; s[e] = ss;
   }
+}
+// N floats of shared memory
+template <int N>
+__device__ __forceinline__ void take(const float* table, int at, float* out) {
 #pragma unroll
-  for (int i = 0; i < N; ++i) cos_sin(th[i], c[i], s[i]);
+  for (int i = 0; i < N; i += 4) {
+    const float4 v = *reinterpret_cast<const float4*>(table + at + i);
+    out[i] = v.x; out[i + 1] = v.y; out[i + 2] = v.z; out[i + 3] = v.w;
+  }
 }
 
-template <typename T>
-__device__ __forceinline__ float weight(const RotateArgs& A, int side, int i) {
-  return A.w_f32 ? static_cast<const float*>(A.w[side])[i] : (float)static_cast<const T*>(A.w[side])[i];
-}
+// weights of both sides (2, d) into shared memory, in the order of the threads' pieces: those of a piece's a values, then of its b values
 template <typename T, bool NEIGHBORS>
-__device__ __forceinline__ void weights(const RotateArgs& A, int side, int part, float* wa, float* wb) {
+__device__ __forceinline__ void weight_table(const RotateArgs& A, float* w) {
   constexpr int N = Vec<T>::N;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int p = part * N + i;
-    wa[i] = weight<T>(A, side, NEIGHBORS ? 2 * p : p);
-    wb[i] = weight<T>(A, side, NEIGHBORS ? 2 * p + 1 : p + A.d / 2);
+  for (int e = threadIdx.x; e < 2 * A.d; e += kThreads) {
+    const int side = e / A.d, i = e % A.d, part = i / (2 * N), k = i % (2 * N), p = part * N + k % N, second = k / N;
+    const int at = NEIGHBORS ? 2 * p + second : p + second * (A.d / 2);
+    if (A.w[side]) w[e] = A.w_f32 ? static_cast<const float*>(A.w[side])[at] : (float)static_cast<const T*>(A.w[side])[at];
   }
 }
 
 // W lanes per row (the next power of two of the parts), `slots` heads of a token side by side, then tokens
-template <typename T, bool NEIGHBORS, int U>
-__global__ void __launch_bounds__(kThreads) forward_kernel(const RotateArgs A, int W) {
+template <typename T, bool NEIGHBORS, bool NORM, int U>
+__global__ void __launch_bounds__(kThreads, 3) forward_kernel(const RotateArgs A, int W) {
   using P = Piece<T, NEIGHBORS>;
   constexpr int N = Vec<T>::N;
   const int part = threadIdx.x % W, group = threadIdx.x / W, slot = group % A.slots;
-  const int token = blockIdx.x * (kThreads / W / A.slots) + group / A.slots;
+  const int per = kThreads / W / A.slots, token = blockIdx.x * per + group / A.slots;
   const bool on = token < A.n && part * N < A.d / 2;
   const int oa = P::off_a(part, A.d), ob = P::off_b(part, A.d);
+  extern __shared__ __align__(16) float table[];
   float c[N], s[N];
-  if (on) angles<N>(A, token, part * N, c, s);
+  if (NORM) weight_table<T, NEIGHBORS>(A, table + per * A.d);
+  angle_table(A, blockIdx.x * per, per, table, table + per * (A.d / 2));
+  __syncthreads();
+  if (on) {
+    const int at = (group / A.slots) * (A.d / 2) + part * N;
+    take<N>(table, at, c);
+    take<N>(table + per * (A.d / 2), at, s);
+  }
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const Rows x = A.x[side];
     const T* src = static_cast<const T*>(x.p) + (long long)token * x.row;
     T* dst = static_cast<T*>(A.out[side]) + (long long)token * A.heads[side] * A.d;
-    float wa[N], wb[N];
-    if (on && A.norm && A.heads[side]) weights<T, NEIGHBORS>(A, side, part, wa, wb);
+    const float* w = table + per * A.d + side * A.d + part * 2 * N;
     for (int hb = 0; hb < A.heads[side]; hb += U * A.slots) {      // the same trips for all lanes: the sums below are over a warp
       const int h0 = hb + slot;
       uint4 u[U], v[U];
@@ -166,13 +178,16 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const RotateArgs A, i
         const int h = h0 + k * A.slots;
         float a[N], b[N];
         P::split(u[k], v[k], a, b);
-        if (A.norm) {
+        if (NORM) {
           float ss = 0.f;
 #pragma unroll
           for (int i = 0; i < N; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
           for (int o = W >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
           const float r = 1.f / sqrtf(ss / A.d + A.eps);
           if (on) {
+            float wa[N], wb[N];
+            take<N>(w, 0, wa);
+            take<N>(w, N, wb);
 #pragma unroll
             for (int i = 0; i < N; ++i) { a[i] *= r * wa[i]; b[i] *= r * wb[i]; }
           }
@@ -194,10 +209,11 @@ __global__ void __launch_bounds__(kThreads) forward_kernel(const RotateArgs A, i
 }
 
 // CTAs walk over tiles of tokens; the shares of dw of a CTA end in one row of A.part.  The sums have a fixed order.
-template <typename T, bool NEIGHBORS, int U>
-__global__ void __launch_bounds__(kThreads) reverse_kernel(const RotateArgs A, int W) {
+template <typename T, bool NEIGHBORS, bool NORM>
+__global__ void __launch_bounds__(kThreads, 2) reverse_kernel(const RotateArgs A, int W) {
   using P = Piece<T, NEIGHBORS>;
   constexpr int N = Vec<T>::N;
+  extern __shared__ __align__(16) float table[];
   __shared__ float th[kThreads * N];                     // dtheta of every thread
   __shared__ float sw[kThreads / 32][2 * N * 32];        // dw of the warps, one side at a time
   const int part = threadIdx.x % W, group = threadIdx.x / W, slot = group % A.slots, per = kThreads / W / A.slots;
@@ -206,77 +222,77 @@ __global__ void __launch_bounds__(kThreads) reverse_kernel(const RotateArgs A, i
   float dwa[2][N], dwb[2][N];
 #pragma unroll
   for (int i = 0; i < N; ++i) dwa[0][i] = dwa[1][i] = dwb[0][i] = dwb[1][i] = 0.f;
+  if (NORM) weight_table<T, NEIGHBORS>(A, table + per * A.d);
   for (int t0 = blockIdx.x * per; t0 < A.n; t0 += gridDim.x * per) {
     const int token = t0 + group / A.slots;
     const bool on = token < A.n && there;
     float c[N], s[N], dth[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) dth[i] = 0.f;
-    if (on) angles<N>(A, token, part * N, c, s);
+    angle_table(A, t0, per, table, table + per * (A.d / 2));
+    __syncthreads();
+    if (on) {
+      const int at = (group / A.slots) * (A.d / 2) + part * N;
+      take<N>(table, at, c);
+      take<N>(table + per * (A.d / 2), at, s);
+    }
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       const Rows x = A.x[side], g = A.g[side];
       const T* src = static_cast<const T*>(x.p) + (long long)token * x.row;
       const T* gsrc = static_cast<const T*>(g.p) + (long long)token * g.row;
       T* dst = static_cast<T*>(A.dx[side]) + (long long)token * A.heads[side] * A.d;
-      float wa[N], wb[N];
-      if (on && A.norm && A.heads[side]) weights<T, NEIGHBORS>(A, side, part, wa, wb);
-      for (int hb = 0; hb < A.heads[side]; hb += U * A.slots) {      // the same trips for all lanes: the sums below are over a warp
-        const int h0 = hb + slot;
-        uint4 u[U], v[U], gu[U], gv[U];
+      const float* w = table + per * A.d + side * A.d + part * 2 * N;
+      for (int hb = 0; hb < A.heads[side]; hb += A.slots) {      // the same trips for all lanes: the sums below are over a warp
+        const int h = hb + slot;
+        const bool mine = on && h < A.heads[side];
+        uint4 u = make_uint4(0, 0, 0, 0), v = u, gu = u, gv = u;
+        if (mine) {
+          u = __ldg(reinterpret_cast<const uint4*>(src + h * x.head + oa));
+          v = __ldg(reinterpret_cast<const uint4*>(src + h * x.head + ob));
+          gu = __ldg(reinterpret_cast<const uint4*>(gsrc + h * g.head + oa));
+          gv = __ldg(reinterpret_cast<const uint4*>(gsrc + h * g.head + ob));
+        }
+        float a[N], b[N], ga[N], gb[N];
+        P::split(u, v, a, b);
+        P::split(gu, gv, ga, gb);
+        float r = 1.f, dot = 0.f;
+        if (NORM) {
+          float ss = 0.f;
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const int h = h0 + k * A.slots;
-          u[k] = v[k] = gu[k] = gv[k] = make_uint4(0, 0, 0, 0);
-          if (on && h < A.heads[side]) {
-            u[k] = __ldg(reinterpret_cast<const uint4*>(src + h * x.head + oa));
-            v[k] = __ldg(reinterpret_cast<const uint4*>(src + h * x.head + ob));
-            gu[k] = __ldg(reinterpret_cast<const uint4*>(gsrc + h * g.head + oa));
-            gv[k] = __ldg(reinterpret_cast<const uint4*>(gsrc + h * g.head + ob));
+          for (int i = 0; i < N; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+          for (int o = W >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+          r = 1.f / sqrtf(ss / A.d + A.eps);
+        }
+        if (on) {
+          float wa[N], wb[N];
+          if (NORM) { take<N>(w, 0, wa); take<N>(w, N, wb); }
+#pragma unroll
+          for (int i = 0; i < N; ++i) {
+            const float xa = a[i] * r, xb = b[i] * r, ya = NORM ? xa * wa[i] : xa, yb = NORM ? xb * wb[i] : xb;
+            const float o1 = ya * c[i] - yb * s[i], o2 = ya * s[i] + yb * c[i];
+            dth[i] = fmaf(gb[i], o1, fmaf(-ga[i], o2, dth[i]));
+            float va = ga[i] * c[i] + gb[i] * s[i], vb = gb[i] * c[i] - ga[i] * s[i];
+            if (NORM) {
+              dwa[side][i] = fmaf(va, xa, dwa[side][i]); dwb[side][i] = fmaf(vb, xb, dwb[side][i]);
+              va *= wa[i]; vb *= wb[i];
+              dot = fmaf(va, xa, fmaf(vb, xb, dot));
+            }
+            a[i] = xa; b[i] = xb; ga[i] = va; gb[i] = vb;
           }
         }
+        if (NORM) {
+          for (int o = W >> 1; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+          dot /= A.d;
+        }
+        if (mine) {
+          if (NORM) {
 #pragma unroll
-        for (int k = 0; k < U; ++k) {
-          const int h = h0 + k * A.slots;
-          float a[N], b[N], ga[N], gb[N];
-          P::split(u[k], v[k], a, b);
-          P::split(gu[k], gv[k], ga, gb);
-          float r = 1.f, dot = 0.f;
-          if (A.norm) {
-            float ss = 0.f;
-#pragma unroll
-            for (int i = 0; i < N; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-            for (int o = W >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            r = 1.f / sqrtf(ss / A.d + A.eps);
+            for (int i = 0; i < N; ++i) { ga[i] = r * (ga[i] - a[i] * dot); gb[i] = r * (gb[i] - b[i] * dot); }
           }
-          if (on) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) {
-              const float xa = a[i] * r, xb = b[i] * r, ya = A.norm ? xa * wa[i] : xa, yb = A.norm ? xb * wb[i] : xb;
-              const float o1 = ya * c[i] - yb * s[i], o2 = ya * s[i] + yb * c[i];
-              dth[i] = fmaf(gb[i], o1, fmaf(-ga[i], o2, dth[i]));
-              float va = ga[i] * c[i] + gb[i] * s[i], vb = gb[i] * c[i] - ga[i] * s[i];
-              if (A.norm) {
-                dwa[side][i] = fmaf(va, xa, dwa[side][i]); dwb[side][i] = fmaf(vb, xb, dwb[side][i]);
-                va *= wa[i]; vb *= wb[i];
-                dot = fmaf(va, xa, fmaf(vb, xb, dot));
-              }
-              a[i] = xa; b[i] = xb; ga[i] = va; gb[i] = vb;
-            }
-          }
-          if (A.norm) {
-            for (int o = W >> 1; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-            dot /= A.d;
-          }
-          if (on && h < A.heads[side]) {
-            if (A.norm) {
-#pragma unroll
-              for (int i = 0; i < N; ++i) { ga[i] = r * (ga[i] - a[i] * dot); gb[i] = r * (gb[i] - b[i] * dot); }
-            }
-            P::join(ga, gb, gu[k], gv[k]);
-            *reinterpret_cast<uint4*>(dst + (long long)h * A.d + oa) = gu[k];
-            *reinterpret_cast<uint4*>(dst + (long long)h * A.d + ob) = gv[k];
-          }
+          P::join(ga, gb, gu, gv);
+          *reinterpret_cast<uint4*>(dst + (long long)h * A.d + oa) = gu;
+          *reinterpret_cast<uint4*>(dst + (long long)h * A.d + ob) = gv;
         }
       }
     }
@@ -303,31 +319,33 @@ __global__ void __launch_bounds__(kThreads) reverse_kernel(const RotateArgs A, i
           if (A.pos_f64) static_cast<double*>(A.dpos)[at] = sum; else static_cast<float*>(A.dpos)[at] = sum;
         }
       }
+    }
+    __syncthreads();      // the tables are written again
+  }
+  if constexpr (NORM) {
+    if (!A.part) return;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      // lanes with the same part of the row
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        float x = there ? dwa[side][i] : 0.f, y = there ? dwb[side][i] : 0.f;
+        for (int o = W; o < 32; o <<= 1) { x += __shfl_xor_sync(0xffffffffu, x, o); y += __shfl_xor_sync(0xffffffffu, y, o); }
+        const int lane = threadIdx.x & 31;
+        if (lane < W) { sw[threadIdx.x >> 5][(2 * i) * 32 + lane] = x; sw[threadIdx.x >> 5][(2 * i + 1) * 32 + lane] = y; }
+      }
+      __syncthreads();
+      for (int e = threadIdx.x; e < 2 * N * W; e += kThreads) {
+        const int pt = e % W, i = (e / W) >> 1, second = (e / W) & 1, p = pt * N + i;
+        if (p < A.d / 2) {
+          float sum = 0.f;
+          for (int w = 0; w < kThreads / 32; ++w) sum += sw[w][(2 * i + second) * 32 + pt];
+          const int at = NEIGHBORS ? 2 * p + second : p + second * (A.d / 2);
+          A.part[((size_t)blockIdx.x * 2 + side) * A.d + at] = sum;
+        }
+      }
       __syncthreads();
     }
-  }
-  if (!A.part) return;
-#pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    // lanes with the same part of the row
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float x = there ? dwa[side][i] : 0.f, y = there ? dwb[side][i] : 0.f;
-      for (int o = W; o < 32; o <<= 1) { x += __shfl_xor_sync(0xffffffffu, x, o); y += __shfl_xor_sync(0xffffffffu, y, o); }
-      const int lane = threadIdx.x & 31;
-      if (lane < W) { sw[threadIdx.x >> 5][(2 * i) * 32 + lane] = x; sw[threadIdx.x >> 5][(2 * i + 1) * 32 + lane] = y; }
-    }
-    __syncthreads();
-    for (int e = threadIdx.x; e < 2 * N * W; e += kThreads) {
-      const int pt = e % W, i = (e / W) >> 1, second = (e / W) & 1, p = pt * N + i;
-      if (p < A.d / 2) {
-        float sum = 0.f;
-        for (int w = 0; w < kThreads / 32; ++w) sum += sw[w][(2 * i + second) * 32 + pt];
-        const int at = NEIGHBORS ? 2 * p + second : p + second * (A.d / 2);
-        A.part[((size_t)blockIdx.x * 2 + side) * A.d + at] = sum;
-      }
-    }
-    __syncthreads();
   }
 }
 
@@ -361,18 +379,18 @@ void shape(RotateArgs& A, int value_bytes, int& W) {
   while (A.slots < most && (long long)A.n * W * A.slots < 2LL * sm_count() * 2048) A.slots <<= 1;
 }
 
-template <typename T, bool NEIGHBORS>
+template <typename T, bool NEIGHBORS, bool NORM>
 void rotate_launch(cudaStream_t st, RotateArgs A, bool reverse, int grid_max) {
   int W;
   shape(A, sizeof(T), W);
-  const int per = kThreads / W / A.slots, tiles = (A.n + per - 1) / per;
+  const int per = kThreads / W / A.slots, tiles = (A.n + per - 1) / per, smem = (per + 2) * A.d * (int)sizeof(float);
   if (!reverse) {
-    forward_kernel<T, NEIGHBORS, 4><<<tiles, kThreads, 0, st>>>(A, W);
+    forward_kernel<T, NEIGHBORS, NORM, 2><<<tiles, kThreads, smem, st>>>(A, W);
     count_launch();
     return;
   }
   const int grid = tiles < grid_max ? tiles : grid_max;
-  reverse_kernel<T, NEIGHBORS, 2><<<grid, kThreads, 0, st>>>(A, W);
+  reverse_kernel<T, NEIGHBORS, NORM><<<grid, kThreads, smem, st>>>(A, W);
   count_launch();
   if (A.part) {
     weight_kernel<T><<<(2 * A.d + 31) / 32, 256, 0, st>>>(A, grid);
@@ -380,11 +398,18 @@ void rotate_launch(cudaStream_t st, RotateArgs A, bool reverse, int grid_max) {
   }
 }
 
-template <bool NEIGHBORS>
-void rotate_typed(cudaStream_t st, const RotateArgs& A, int type, bool reverse, int grid_max) {
-  if (type == kBF16) rotate_launch<__nv_bfloat16, NEIGHBORS>(st, A, reverse, grid_max);
-  else if (type == kF16) rotate_launch<__half, NEIGHBORS>(st, A, reverse, grid_max);
-  else rotate_launch<float, NEIGHBORS>(st, A, reverse, grid_max);
+template <typename T>
+void rotate_typed(cudaStream_t st, const RotateArgs& A, bool neighbors, bool reverse, int grid_max) {
+  if (neighbors) {
+    if (A.norm) rotate_launch<T, true, true>(st, A, reverse, grid_max); else rotate_launch<T, true, false>(st, A, reverse, grid_max);
+  } else {
+    if (A.norm) rotate_launch<T, false, true>(st, A, reverse, grid_max); else rotate_launch<T, false, false>(st, A, reverse, grid_max);
+  }
+}
+void rotate(cudaStream_t st, const RotateArgs& A, int type, bool neighbors, bool reverse, int grid_max) {
+  if (type == kBF16) rotate_typed<__nv_bfloat16>(st, A, neighbors, reverse, grid_max);
+  else if (type == kF16) rotate_typed<__half>(st, A, neighbors, reverse, grid_max);
+  else rotate_typed<float>(st, A, neighbors, reverse, grid_max);
 }
 
 bool rows_ok(const so3lr_b200_rows* r, int type, int heads) {
@@ -415,8 +440,7 @@ int so3lr_b200_norm_rotate(void* stream, const so3lr_b200_norm_rotate_args* a, c
   A.out[0] = out_q; A.out[1] = out_k; A.w[0] = a->weight_q; A.w[1] = a->weight_k;
   A.pos = a->positions; A.freq = a->frequencies; A.heads[0] = a->heads_q; A.heads[1] = a->heads_k;
   A.n = a->n; A.d = a->d; A.axes = a->axes; A.norm = a->norm; A.w_f32 = a->weights_f32; A.pos_f64 = a->positions_f64; A.eps = a->eps;
-  if (a->neighbors) rotate_typed<true>(static_cast<cudaStream_t>(stream), A, a->type, false, 0);
-  else rotate_typed<false>(static_cast<cudaStream_t>(stream), A, a->type, false, 0);
+  rotate(static_cast<cudaStream_t>(stream), A, a->type, a->neighbors != 0, false, 0);
   SO3LR_CUDA_CHECK(cudaGetLastError());
   return kOk;
 }
@@ -443,8 +467,7 @@ int so3lr_b200_norm_rotate_vjp(void* stream, const so3lr_b200_norm_rotate_args* 
     A.pos = a->positions; A.freq = a->frequencies; A.dpos = d_positions; A.part = want_w ? static_cast<float*>(workspace) : nullptr;
     A.heads[0] = a->heads_q; A.heads[1] = a->heads_k;
     A.n = a->n; A.d = a->d; A.axes = a->axes; A.norm = a->norm; A.w_f32 = a->weights_f32; A.pos_f64 = a->positions_f64; A.eps = a->eps;
-    if (a->neighbors) rotate_typed<true>(st, A, a->type, true, grid_limit());
-    else rotate_typed<false>(st, A, a->type, true, grid_limit());
+    rotate(st, A, a->type, a->neighbors != 0, true, grid_limit());
   } else {
     const size_t wb = (size_t)a->d * (a->weights_f32 || a->type == kF32 ? 4 : 2);
     if (want_w && d_weight_q) SO3LR_CUDA_CHECK(cudaMemsetAsync(d_weight_q, 0, wb, st));

@@ -138,7 +138,12 @@ int64_t part_floats(const int32_t* im, const so3lr_b200_attention_shape* a) {
 #ifndef SO3LR_PACKED_TC_ROWS
 #define SO3LR_PACKED_TC_ROWS 128
 #endif
-template <typename T> bool on_tensor_cores(const int32_t* im) { return sizeof(T) == 2 && im[kMaxQ] >= SO3LR_PACKED_TC_ROWS && im[kMaxKv] >= SO3LR_PACKED_TC_ROWS; }
+bool on_tensor_cores(const int32_t* im, const so3lr_b200_attention_shape* a) {
+  return (a->type != kF32 || a->d <= 64) && im[kMaxQ] >= SO3LR_PACKED_TC_ROWS && im[kMaxKv] >= SO3LR_PACKED_TC_ROWS;
+}
+int64_t split_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool reverse) {
+  return a->type == kF32 && on_tensor_cores(im, a) ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0;
+}
 
 const int4* table(const int32_t* im, const int32_t* dev, int field) { return reinterpret_cast<const int4*>(dev + im[field]); }
 
@@ -152,11 +157,9 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
     packed_forward_split<T>(st, p, im[kNItemsSplit], im[kN], im[kCombine]);
     return kOk;
   }
-  if constexpr (sizeof(T) == 2) {
-    if (on_tensor_cores<T>(im)) {
-      p.items = table(im, dev, kItemsQ256);
-      return packed_forward_tc<T>(st, p, im[kNItemsQ256]);
-    }
+  if (on_tensor_cores(im, a)) {
+    p.items = table(im, dev, kItemsQ256);
+    return packed_forward_tc<T>(st, p, im[kNItemsQ256], workspace);
   }
   p.items = table(im, dev, kItemsQ);
   packed_forward_mma<T>(st, p, im[kNItemsQ]);
@@ -164,12 +167,10 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
 }
 
 template <typename T>
-int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev) {
+int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
   packed_delta<T>(st, p, im[kRowsQ]);
-  if constexpr (sizeof(T) == 2) {
-    if (on_tensor_cores<T>(im))
-      return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128]);
-  }
+  if (on_tensor_cores(im, a))
+    return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128], workspace);
   p.items = table(im, dev, kItemsQ);
   if (im[kNItemsQ]) packed_dq_mma<T>(st, p, im[kNItemsQ]);
   p.items = table(im, dev, kItemsKv);
@@ -201,24 +202,26 @@ int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int
   return kOk;
 }
 
-int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* a) {
+int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* a, int vjp) {
   if (!shape_ok(image, a)) return -1;
-  if (!few_rows(image, a) || !image[kCombine]) return 0;
+  if (vjp) return split_bytes(image, a, true);
+  if (!few_rows(image, a)) return split_bytes(image, a, false);
+  if (!image[kCombine]) return 0;
   return part_floats(image, a) * (int64_t)sizeof(float) + part_floats(image, a) / packed_padded(a->d) * (int64_t)sizeof(float2);
 }
 
 int so3lr_b200_structure_attention(const int32_t* image, const int32_t* image_dev, void* stream, const so3lr_b200_attention_shape* a,
-                                   const so3lr_b200_rows* q, const so3lr_b200_rows* k, const so3lr_b200_rows* v, void* out, float* lse,
-                                   void* workspace, int64_t workspace_bytes) {
+                                   const so3lr_b200_rows* q, const so3lr_b200_rows* k, const so3lr_b200_rows* v, void* out, void* out_rest,
+                                   float* lse, void* workspace, int64_t workspace_bytes) {
   if (!shape_ok(image, a) || !image_dev) return kInvalidArgument;
   if (image[kRowsQ] == 0) return kOk;
   if (!rows_ok(q, a->type) || (image[kRowsKv] && (!rows_ok(k, a->type) || !rows_ok(v, a->type))) || !out) return kInvalidArgument;
-  const int64_t need = so3lr_b200_structure_attention_workspace(image, a);
+  const int64_t need = so3lr_b200_structure_attention_workspace(image, a, 0);
   if (need > 0 && (!workspace || workspace_bytes < need)) return kInvalidArgument;
   PackedArgs p = common(image, image_dev, a);
   p.q = rows_of(q);
   if (image[kRowsKv]) { p.k = rows_of(k); p.v = rows_of(v); } else { p.k = p.v = p.q; }   // never read: no structure has keys
-  p.out = out; p.lse = lse;
+  p.out = out; p.out_rest = a->type == kF32 ? nullptr : out_rest; p.lse = lse;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int rc = a->type == kBF16 ? forward<__nv_bfloat16>(st, p, image, image_dev, a, workspace)
                  : a->type == kF16 ? forward<__half>(st, p, image, image_dev, a, workspace) : forward<float>(st, p, image, image_dev, a, workspace);
@@ -228,21 +231,24 @@ int so3lr_b200_structure_attention(const int32_t* image, const int32_t* image_de
 
 int so3lr_b200_structure_attention_vjp(const int32_t* image, const int32_t* image_dev, void* stream, const so3lr_b200_attention_shape* a,
                                        const so3lr_b200_rows* q, const so3lr_b200_rows* k, const so3lr_b200_rows* v, const void* out,
-                                       const float* lse, const so3lr_b200_rows* g, float* delta, void* d_q, void* d_k, void* d_v) {
+                                       const void* out_rest, const float* lse, const so3lr_b200_rows* g, float* delta, void* d_q, void* d_k,
+                                       void* d_v, void* workspace, int64_t workspace_bytes) {
   if (!shape_ok(image, a) || !image_dev) return kInvalidArgument;
   if (image[kRowsQ] == 0 && image[kRowsKv] == 0) return kOk;
   if ((image[kRowsQ] && (!rows_ok(q, a->type) || !rows_ok(g, a->type) || !out || !lse || !delta || !d_q)) ||
       (image[kRowsKv] && (!rows_ok(k, a->type) || !rows_ok(v, a->type) || !d_k || !d_v)))
     return kInvalidArgument;
+  const int64_t need = so3lr_b200_structure_attention_workspace(image, a, 1);
+  if (need > 0 && (!workspace || workspace_bytes < need)) return kInvalidArgument;
   PackedArgs p = common(image, image_dev, a);
   if (image[kRowsQ]) { p.q = rows_of(q); p.g = rows_of(g); }
   if (image[kRowsKv]) { p.k = rows_of(k); p.v = rows_of(v); }
   if (!image[kRowsQ]) p.q = p.g = p.k;      // never read: one side has no rows
   if (!image[kRowsKv]) p.k = p.v = p.q;
-  p.o.p = out; p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = d_q; p.dk = d_k; p.dv = d_v;
+  p.o.p = out; p.out_rest = const_cast<void*>(a->type == kF32 ? nullptr : out_rest); p.lse = const_cast<float*>(lse); p.delta = delta; p.dq = d_q; p.dk = d_k; p.dv = d_v;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int rc = a->type == kBF16 ? reverse<__nv_bfloat16>(st, p, image, image_dev)
-                 : a->type == kF16 ? reverse<__half>(st, p, image, image_dev) : reverse<float>(st, p, image, image_dev);
+  const int rc = a->type == kBF16 ? reverse<__nv_bfloat16>(st, p, image, image_dev, a, workspace)
+                 : a->type == kF16 ? reverse<__half>(st, p, image, image_dev, a, workspace) : reverse<float>(st, p, image, image_dev, a, workspace);
   SO3LR_CUDA_CHECK(cudaGetLastError());
   return rc;
 }

@@ -23,7 +23,8 @@ struct Rows {
 struct PackedArgs {
   Rows q, k, v, g, o;           // g: cotangent of the output; o: the output (reverse pass)
   void* out = nullptr;          // (nq, hq, d) contiguous
-  float* lse = nullptr;         // (hq, nq) natural logarithm of the sum of exponentials; -inf for a row without keys
+  void* out_rest = nullptr;     // (nq, hq, d) what rounding o to 16 bits left, or null
+  float* lse = nullptr;         // (hq, nq) logarithm to base 2 of the sum of exponentials; -inf for a row without keys
   float* delta = nullptr;       // (hq, nq) sum over d of g * o
   void *dq = nullptr, *dk = nullptr, *dv = nullptr;   // contiguous
   const int *start_q = nullptr, *start_kv = nullptr;
@@ -47,9 +48,14 @@ template <typename T> void packed_dq_mma(cudaStream_t st, const PackedArgs& a, i
 template <typename T> void packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items);
 template <typename T> void packed_delta(cudaStream_t st, const PackedArgs& a, int rows);
 
-// kernels on the tensor cores (16-bit types): tiles of 128 rows, two of them side by side in the forward kernel
-template <typename T> int packed_forward_tc(cudaStream_t st, const PackedArgs& a, int n_items);
-template <typename T> int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv);
+// Kernels on the tensor cores: tiles of 128 rows, two of them side by side in the forward kernel.  float32 (d <= 64) runs on operands that
+// are split into three bfloat16 terms ahead (packed_split_bytes of workspace).
+template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, void* workspace);
+template <typename T> int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, void* workspace);
+inline int packed_split_width(int d) { return d <= 32 ? 32 : 64; }
+inline int64_t packed_split_bytes(int64_t rows_q, int64_t rows_kv, int hq, int hk, int d, bool reverse) {
+  return ((reverse ? 2 : 1) * rows_q * hq + 2 * rows_kv * hk) * 3 * packed_split_width(d) * 2;
+}
 int packed_error(int* out);
 
 inline int packed_padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }

@@ -22,8 +22,6 @@
 namespace so3lr {
 namespace packed {
 
-constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
-
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 // 16 bytes, or zeros where `ok` is false
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool ok) {
@@ -38,12 +36,14 @@ __device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t* r) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 __device__ __forceinline__ void mma_tf32(float* c, const uint32_t* a, const uint32_t* b) {
-  asm volatile("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
+// x = hi + lo, hi rounded to the 11 bits of tf32 in integer arithmetic (the conversion instruction runs at an eighth of its rate); lo is exact,
+// and the matrix instruction reads its upper 11 bits
 __device__ __forceinline__ void tf32_split(float x, uint32_t& hi, uint32_t& lo) {
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(hi) : "f"(x));
-  asm("cvt.rna.tf32.f32 %0, %1;" : "=r"(lo) : "f"(x - __uint_as_float(hi)));
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
+  lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
 template <typename T> struct Half;
@@ -58,7 +58,7 @@ template <> struct Half<__nv_bfloat16> {
   }
   static __device__ __forceinline__ float2 unpack(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u)); }
   static __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
   }
 };
@@ -69,7 +69,7 @@ template <> struct Half<__half> {
   }
   static __device__ __forceinline__ float2 unpack(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
   static __device__ __forceinline__ void mma(float* c, const uint32_t* a, const uint32_t* b) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
   }
 };
@@ -95,28 +95,37 @@ __device__ __forceinline__ void load_rows(uint32_t tile, const Rows& src, int he
 }
 
 // ---- products of a warp's 16 rows -----------------------------------------------------------------------------------
-// acc[16 x 8 NT] += A[16 x DP] B[8 NT x DP]^T, A at `a` (the warp's first row), B at `b`
-template <typename T, int DP, int NT>
-__device__ __forceinline__ void product_nt(float (&acc)[NT][4], uint32_t a, uint32_t b, int lane) {
+// The tensor cores cut what they add to an accumulator to its 24 bits instead of rounding it, which shrinks a long sum by up to 2^-24 a step.
+// With 16-bit operands that does not show; float32 products keep the cross terms apart from the large ones, and start every tile of the
+// walked side in fresh accumulators that are added in ordinary arithmetic: at 5,000 keys 3.5e-5 of the result without, below 1e-6 with it.
+
+// acc[16 x 8 NT] = A[16 x DP] B[8 NT x DP]^T, A at `a` (the warp's first row), B at `b`; columns from `cols` on are not needed
+template <typename T, int DP, int NT, bool PART>
+__device__ __forceinline__ void product_nt_of(float (&acc)[NT][4], uint32_t a, uint32_t b, int lane, int cols) {
   using L = Tile<T, DP>;
+  const uint32_t al = a + (lane & 15) * L::kStride + (lane >> 4) * 16;
+  const uint32_t bl = b + ((lane & 7) + ((lane >> 4) << 3)) * L::kStride + ((lane >> 3) & 1) * 16;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
   if constexpr (sizeof(T) == 2) {
-    const uint32_t al = a + (lane & 15) * L::kStride + (lane >> 4) * 16;
-    const uint32_t bl = b + ((lane & 7) + ((lane >> 4) << 3)) * L::kStride + ((lane >> 3) & 1) * 16;
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) {
       uint32_t fa[4];
       ldsm4(al + ks * 32, fa);
 #pragma unroll
       for (int n = 0; n < NT; n += 2) {
-        uint32_t fb[4];
-        ldsm4(bl + n * 8 * L::kStride + ks * 32, fb);
-        Half<T>::mma(acc[n], fa, fb);
-        Half<T>::mma(acc[n + 1], fa, fb + 2);
+        if (!PART || n * 8 < cols) {
+          uint32_t fb[4];
+          ldsm4(bl + n * 8 * L::kStride + ks * 32, fb);
+          Half<T>::mma(acc[n], fa, fb);
+          Half<T>::mma(acc[n + 1], fa, fb + 2);
+        }
       }
     }
   } else {
-    const uint32_t al = a + (lane & 15) * L::kStride + (lane >> 4) * 16;
-    const uint32_t bl = b + ((lane & 7) + ((lane >> 4) << 3)) * L::kStride + ((lane >> 3) & 1) * 16;
+    float cross[NT][4];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) cross[n][0] = cross[n][1] = cross[n][2] = cross[n][3] = 0.f;
 #pragma unroll 4
     for (int ks = 0; ks < DP / 8; ++ks) {
       uint32_t fa[4], ah[4], alo[4];
@@ -125,61 +134,95 @@ __device__ __forceinline__ void product_nt(float (&acc)[NT][4], uint32_t a, uint
       for (int i = 0; i < 4; ++i) tf32_split(__uint_as_float(fa[i]), ah[i], alo[i]);
 #pragma unroll
       for (int n = 0; n < NT; n += 2) {
-        uint32_t fb[4], bh[4], blo[4];
-        ldsm4(bl + n * 8 * L::kStride + ks * 32, fb);
+        if (!PART || n * 8 < cols) {
+          uint32_t fb[4], bh[4], blo[4];
+          ldsm4(bl + n * 8 * L::kStride + ks * 32, fb);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tf32_split(__uint_as_float(fb[i]), bh[i], blo[i]);
+          for (int i = 0; i < 4; ++i) tf32_split(__uint_as_float(fb[i]), bh[i], blo[i]);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          mma_tf32(acc[n + h], alo, bh + 2 * h);
-          mma_tf32(acc[n + h], ah, blo + 2 * h);
-          mma_tf32(acc[n + h], ah, bh + 2 * h);
+          for (int h = 0; h < 2; ++h) {
+            mma_tf32(acc[n + h], ah, bh + 2 * h);
+            mma_tf32(cross[n + h], alo, bh + 2 * h);
+            mma_tf32(cross[n + h], ah, blo + 2 * h);
+          }
         }
       }
     }
+#pragma unroll
+    for (int n = 0; n < NT; ++n) { acc[n][0] += cross[n][0]; acc[n][1] += cross[n][1]; acc[n][2] += cross[n][2]; acc[n][3] += cross[n][3]; }
   }
 }
 
-// acc[16 x DP] += A[16 x 8 NT] B[8 NT x DP], A the accumulator fragments of an earlier product
-template <typename T, int DP, int NT>
-__device__ __forceinline__ void product_nn(float (&acc)[DP / 8][4], const float (&p)[NT][4], uint32_t b, int lane) {
+// acc[16 x DP] += A[16 x 8 NT] B[8 NT x DP], A the accumulator fragments of an earlier product, zero from column `rows` on
+template <typename T, int DP, int NT, bool PART>
+__device__ __forceinline__ void product_nn_of(float (&acc)[DP / 8][4], const float (&p)[NT][4], uint32_t b, int lane, int rows) {
   using L = Tile<T, DP>;
   if constexpr (sizeof(T) == 2) {
     const uint32_t bl = b + (lane & 15) * L::kStride + (lane >> 4) * 16;
 #pragma unroll
     for (int j = 0; j < NT / 2; ++j) {
-      const uint32_t fa[4] = {Half<T>::pack(p[2 * j][0], p[2 * j][1]), Half<T>::pack(p[2 * j][2], p[2 * j][3]),
-                              Half<T>::pack(p[2 * j + 1][0], p[2 * j + 1][1]), Half<T>::pack(p[2 * j + 1][2], p[2 * j + 1][3])};
+      if (!PART || j * 16 < rows) {
+        const uint32_t fa[4] = {Half<T>::pack(p[2 * j][0], p[2 * j][1]), Half<T>::pack(p[2 * j][2], p[2 * j][3]),
+                                Half<T>::pack(p[2 * j + 1][0], p[2 * j + 1][1]), Half<T>::pack(p[2 * j + 1][2], p[2 * j + 1][3])};
 #pragma unroll
-      for (int n = 0; n < DP / 8; n += 2) {
-        uint32_t fb[4];
-        ldsm4t(bl + j * 16 * L::kStride + n * 16, fb);
-        Half<T>::mma(acc[n], fa, fb);
-        Half<T>::mma(acc[n + 1], fa, fb + 2);
+        for (int n = 0; n < DP / 8; n += 2) {
+          uint32_t fb[4];
+          ldsm4t(bl + j * 16 * L::kStride + n * 16, fb);
+          Half<T>::mma(acc[n], fa, fb);
+          Half<T>::mma(acc[n + 1], fa, fb + 2);
+        }
       }
     }
   } else {
     // the order of the contracted index is free: position t stands for column 2 t, position t + 4 for column 2 t + 1, which is how the
     // accumulator fragment holds them; B follows (rows 2 t and 2 t + 1: banks 8 t + g, all different)
     const uint32_t bl = b + 2 * (lane & 3) * L::kStride + (lane >> 2) * 4;
+    uint32_t ah[NT][4], alo[NT][4];
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      uint32_t ah[4], alo[4];
-      tf32_split(p[j][0], ah[0], alo[0]); tf32_split(p[j][2], ah[1], alo[1]);
-      tf32_split(p[j][1], ah[2], alo[2]); tf32_split(p[j][3], ah[3], alo[3]);
+      tf32_split(p[j][0], ah[j][0], alo[j][0]); tf32_split(p[j][2], ah[j][1], alo[j][1]);
+      tf32_split(p[j][1], ah[j][2], alo[j][2]); tf32_split(p[j][3], ah[j][3], alo[j][3]);
+    }
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        float x, y;
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(bl + j * 8 * L::kStride + n * 32) : "memory");
-        asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(bl + (j * 8 + 1) * L::kStride + n * 32) : "memory");
-        uint32_t bh[2], blo[2];
-        tf32_split(x, bh[0], blo[0]); tf32_split(y, bh[1], blo[1]);
-        mma_tf32(acc[n], alo, bh);
-        mma_tf32(acc[n], ah, blo);
-        mma_tf32(acc[n], ah, bh);
+    for (int n = 0; n < DP / 8; n += 4) {
+      float t[4][4], cross[4][4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) { t[m][0] = t[m][1] = t[m][2] = t[m][3] = 0.f; cross[m][0] = cross[m][1] = cross[m][2] = cross[m][3] = 0.f; }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        if (!PART || j * 8 < rows) {
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            float x, y;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x) : "r"(bl + j * 8 * L::kStride + (n + m) * 32) : "memory");
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(y) : "r"(bl + (j * 8 + 1) * L::kStride + (n + m) * 32) : "memory");
+            uint32_t bh[2], blo[2];
+            tf32_split(x, bh[0], blo[0]); tf32_split(y, bh[1], blo[1]);
+            mma_tf32(t[m], ah[j], bh);
+            mma_tf32(cross[m], alo[j], bh);
+            mma_tf32(cross[m], ah[j], blo);
+          }
+        }
+      }
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        acc[n + m][0] += t[m][0] + cross[m][0]; acc[n + m][1] += t[m][1] + cross[m][1];
+        acc[n + m][2] += t[m][2] + cross[m][2]; acc[n + m][3] += t[m][3] + cross[m][3];
       }
     }
   }
+}
+
+// A tile that is not full leaves out what is empty; the tests between the instructions cost a full one a fifth of its time, so it has none.
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void product_nt(float (&acc)[NT][4], uint32_t a, uint32_t b, int lane, int cols) {
+  if (cols >= 8 * NT) product_nt_of<T, DP, NT, false>(acc, a, b, lane, cols);
+  else product_nt_of<T, DP, NT, true>(acc, a, b, lane, cols);
+}
+template <typename T, int DP, int NT>
+__device__ __forceinline__ void product_nn(float (&acc)[DP / 8][4], const float (&p)[NT][4], uint32_t b, int lane, int rows) {
+  if (rows >= 8 * NT) product_nn_of<T, DP, NT, false>(acc, p, b, lane, rows);
+  else product_nn_of<T, DP, NT, true>(acc, p, b, lane, rows);
 }
 
 // the warp's accumulators (rows g and g + 8 of its 16, columns 8 n + 2 t, + 1) times `f` to a contiguous destination
@@ -187,6 +230,19 @@ template <typename T>
 __device__ __forceinline__ void store2(T* p, float x, float y) {
   if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(p) = Half<T>::pack(x, y);
   else *reinterpret_cast<float2*>(p) = make_float2(x, y);
+}
+
+// x, y rounded, and what the rounding left of 16-bit types (the reverse pass forms g . o with both: with the rounded o alone its error is as
+// large as that of dS itself in short structures)
+template <typename T>
+__device__ __forceinline__ void store_rest(T* p, T* rest, float x, float y) {
+  store2(p, x, y);
+  if constexpr (sizeof(T) == 2) {
+    if (rest) {
+      const float2 r = Half<T>::unpack(Half<T>::pack(x, y));
+      store2(rest, x - r.x, y - r.y);
+    }
+  }
 }
 
 template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 4 && DP > 64 ? 32 : 64; }
@@ -247,9 +303,8 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
     const int kb = k0 + it * BN, buf = it & 1;
     if (wr < rows && kb <= lim_hi) {
       float p[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) p[n][0] = p[n][1] = p[n][2] = p[n][3] = 0.f;
-      product_nt<T, DP, NT>(p, sq + warp * 16 * L::kStride, sk + buf * BN * L::kStride, lane);
+      const int cols = k1 - kb;
+      product_nt<T, DP, NT>(p, sq + warp * 16 * L::kStride, sk + buf * BN * L::kStride, lane, cols);
       if (kb + BN > k1 || kb + BN - 1 > lim_lo) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -280,7 +335,7 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
       la = fmaf(la, fa, ta); lb = fmaf(lb, fb, tb);
 #pragma unroll
       for (int n = 0; n < DP / 8; ++n) { o[n][0] *= fa; o[n][1] *= fa; o[n][2] *= fb; o[n][3] *= fb; }
-      product_nn<T, DP, NT>(o, p, sv + buf * BN * L::kStride, lane);
+      product_nn<T, DP, NT>(o, p, sv + buf * BN * L::kStride, lane, cols);
     }
     __syncthreads();
   }
@@ -303,13 +358,14 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
     }
     const int tok = SPLIT ? pr / G : pr, head = SPLIT ? hy * G + pr % G : hy;
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);               // a row without keys gives zero; NaN stays NaN
-    T* dst = static_cast<T*>(a.out) + ((long long)(q0 + tok) * a.hq + head) * a.d;
+    const long long to = ((long long)(q0 + tok) * a.hq + head) * a.d;
+    T *dst = static_cast<T*>(a.out) + to, *rest = a.out_rest ? static_cast<T*>(a.out_rest) + to : nullptr;
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n) {
       const int c = n * 8 + 2 * (lane & 3);
-      if (c < a.d) store2(dst + c, o[n][2 * half] * inv, o[n][2 * half + 1] * inv);
+      if (c < a.d) store_rest<T>(dst + c, rest ? rest + c : nullptr, o[n][2 * half] * inv, o[n][2 * half + 1] * inv);
     }
-    if ((lane & 3) == 0 && a.lse) a.lse[(long long)head * a.nq + q0 + tok] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+    if ((lane & 3) == 0 && a.lse) a.lse[(long long)head * a.nq + q0 + tok] = l == 0.f ? -INFINITY : m + log2f(l);
   }
 }
 
@@ -339,11 +395,16 @@ __global__ void __launch_bounds__(256) combine_kernel(const PackedArgs a) {
     }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     const int tok = pr / a.group, head = hy * a.group + pr % a.group;
-    T* dst = static_cast<T*>(a.out) + ((long long)(q0 + tok) * a.hq + head) * a.d;
+    const long long to = ((long long)(q0 + tok) * a.hq + head) * a.d;
 #pragma unroll
-    for (int c = 0; c < DP / 32; ++c)
-      if (c * 32 + lane < a.d) dst[c * 32 + lane] = (T)(o[c] * inv);
-    if (lane == 0 && a.lse) a.lse[(long long)head * a.nq + q0 + tok] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+    for (int c = 0; c < DP / 32; ++c) {
+      if (c * 32 + lane >= a.d) continue;
+      const float x = o[c] * inv;
+      const T y = (T)x;
+      static_cast<T*>(a.out)[to + c * 32 + lane] = y;
+      if (sizeof(T) == 2 && a.out_rest) static_cast<T*>(a.out_rest)[to + c * 32 + lane] = (T)(x - (float)y);
+    }
+    if (lane == 0 && a.lse) a.lse[(long long)head * a.nq + q0 + tok] = l == 0.f ? -INFINITY : m + log2f(l);
   }
 }
 
@@ -361,11 +422,16 @@ __global__ void __launch_bounds__(256) delta_kernel(const PackedArgs a, int rows
     const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.g.p) + r * a.g.row + h * a.g.head + part * V);
     const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o.p) + (r * a.hq + h) * a.d + part * V);
     const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    uint32_t zs[4] = {0, 0, 0, 0};
+    if (sizeof(T) == 2 && a.out_rest) {
+      const uint4 z = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.out_rest) + (r * a.hq + h) * a.d + part * V);
+      zs[0] = z.x; zs[1] = z.y; zs[2] = z.z; zs[3] = z.w;
+    }
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if constexpr (sizeof(T) == 2) {
-        const float2 u = Half<T>::unpack(xs[e]), v = Half<T>::unpack(ys[e]);
-        sum = fmaf(u.x, v.x, fmaf(u.y, v.y, sum));
+        const float2 u = Half<T>::unpack(xs[e]), v = Half<T>::unpack(ys[e]), w = Half<T>::unpack(zs[e]);
+        sum = fmaf(u.x, v.x + w.x, fmaf(u.y, v.y + w.y, sum));
       } else {
         sum = fmaf(__uint_as_float(xs[e]), __uint_as_float(ys[e]), sum);
       }
@@ -402,7 +468,7 @@ __global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
   const int lim_a = a.causal ? ra + off : big, lim_b = a.causal ? rb + off : big, lim_lo = a.causal ? wr + off : big, lim_hi = a.causal ? wr + 15 + off : big;
   const long long at = (long long)h * a.nq + q0;
   // rows that are not there: exp(-inf) = 0
-  const float ea = ra < lq ? a.lse[at + ra] * kLog2e : INFINITY, eb = rb < lq ? a.lse[at + rb] * kLog2e : INFINITY;
+  const float ea = ra < lq ? a.lse[at + ra] : INFINITY, eb = rb < lq ? a.lse[at + rb] : INFINITY;
   const float da = ra < lq ? a.delta[at + ra] : 0.f, db = rb < lq ? a.delta[at + rb] : 0.f;
   float dq[DP / 8][4];
 #pragma unroll
@@ -414,10 +480,9 @@ __global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
     const int kb = k0 + it * BN, buf = it & 1;
     if (wr < lq && kb <= lim_hi) {
       float p[NT][4], dp[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) { p[n][0] = p[n][1] = p[n][2] = p[n][3] = 0.f; dp[n][0] = dp[n][1] = dp[n][2] = dp[n][3] = 0.f; }
-      product_nt<T, DP, NT>(p, sq + warp * 16 * L::kStride, sk + buf * BN * L::kStride, lane);
-      product_nt<T, DP, NT>(dp, sg + warp * 16 * L::kStride, sv + buf * BN * L::kStride, lane);
+      const int cols = k1 - kb;
+      product_nt<T, DP, NT>(p, sq + warp * 16 * L::kStride, sk + buf * BN * L::kStride, lane, cols);
+      product_nt<T, DP, NT>(dp, sg + warp * 16 * L::kStride, sv + buf * BN * L::kStride, lane, cols);
       const bool mask = kb + BN > k1 || kb + BN - 1 > lim_lo;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -431,7 +496,7 @@ __global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
           p[n][e] = x; p[n][2 + e] = y;
         }
       }
-      product_nn<T, DP, NT>(dq, p, sk + buf * BN * L::kStride, lane);
+      product_nn<T, DP, NT>(dq, p, sk + buf * BN * L::kStride, lane, cols);
     }
     __syncthreads();
   }
@@ -472,7 +537,7 @@ __global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
       if (tid < BN) {
         const bool ok = b + tid < i1;
         const long long at = (long long)h * a.nq + q0 + b + tid;
-        se[buf * BN + tid] = ok ? fmaf(a.lse[at], kLog2e, -prob_shift<T>()) : INFINITY;
+        se[buf * BN + tid] = ok ? a.lse[at] - prob_shift<T>() : INFINITY;
         se[(2 + buf) * BN + tid] = ok ? a.delta[at] * prob_unscale<T>() : 0.f;
       }
     }
@@ -492,10 +557,9 @@ __global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
     const int ib = i0 + (it % per) * BN, buf = it & 1;
     if (wr < lk && ib + BN - 1 >= lim_lo) {
       float p[NT][4], ds[NT][4];
-#pragma unroll
-      for (int n = 0; n < NT; ++n) { p[n][0] = p[n][1] = p[n][2] = p[n][3] = 0.f; ds[n][0] = ds[n][1] = ds[n][2] = ds[n][3] = 0.f; }
-      product_nt<T, DP, NT>(p, sk + warp * 16 * L::kStride, sq + buf * BN * L::kStride, lane);
-      product_nt<T, DP, NT>(ds, sv + warp * 16 * L::kStride, sg + buf * BN * L::kStride, lane);
+      const int cols = i1 - ib;
+      product_nt<T, DP, NT>(p, sk + warp * 16 * L::kStride, sq + buf * BN * L::kStride, lane, cols);
+      product_nt<T, DP, NT>(ds, sv + warp * 16 * L::kStride, sg + buf * BN * L::kStride, lane, cols);
       const bool mask = a.causal && ib < lim_hi;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -510,8 +574,8 @@ __global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
           p[n][x] = w;
         }
       }
-      product_nn<T, DP, NT>(dv, p, sg + buf * BN * L::kStride, lane);
-      product_nn<T, DP, NT>(dk, ds, sq + buf * BN * L::kStride, lane);
+      product_nn<T, DP, NT>(dv, p, sg + buf * BN * L::kStride, lane, cols);
+      product_nn<T, DP, NT>(dk, ds, sq + buf * BN * L::kStride, lane, cols);
     }
     __syncthreads();
   }

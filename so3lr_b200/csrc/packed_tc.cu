@@ -1,10 +1,14 @@
-// Attention inside the structures of a packed batch on the tensor cores (tcgen05) for 16-bit operands: forward and the two halves of the
-// reverse pass, for structures long enough to fill tiles of 128 rows.  The mathematics is that of packed_mma.cuh.
+// Attention inside the structures of a packed batch on the tensor cores (tcgen05): forward and the two halves of the reverse pass, for
+// structures long enough to fill tiles of 128 rows.  The mathematics is that of packed_mma.cuh.  16-bit operands as they are; float32 with up to 64
+// values a head as three bfloat16 terms each (Geometry), with accumulators over the walked side in registers, because the tensor cores cut
+// what they add to an accumulator (2^-24 of the sum a step).
 //
 // A CTA has the SM to itself: eight warps do the softmax (a thread per row, or per row and half of the columns), one warp issues the
 // matrix instructions, three load tiles.  Accumulators and P / dS live in tensor memory: P and dS go back there packed to 16 bits over
 // the logits they were made from, and are the A operand of the next product, so shared memory carries q, k, v and g only.
 #include "packed_tc.cuh"
+
+#include <algorithm>
 
 namespace so3lr {
 
@@ -20,23 +24,56 @@ struct Tail {
   uint32_t tmem;
   int failed;
 };
-// Tiles that stream through: a ring of four slots (two sub-tiles) or eight, the two kinds of tile in turn; tile j sits in slot j % R.
-__device__ __forceinline__ int ring_slots(int subs) { return subs == 2 ? 4 : 8; }
+template <typename T, int TERMS> struct Operand { using type = T; };
+template <> struct Operand<float, 3> { using type = __nv_bfloat16; };
+// 16 values to a row of the result
+template <typename T> __device__ __forceinline__ void store16(T* p, const float* v) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) u[e] = packed::Half<T>::pack(v[2 * e], v[2 * e + 1]);
+    *reinterpret_cast<uint4*>(p) = make_uint4(u[0], u[1], u[2], u[3]);
+    *reinterpret_cast<uint4*>(p + 8) = make_uint4(u[4], u[5], u[6], u[7]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 16; e += 4) *reinterpret_cast<float4*>(p + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+  }
+}
+// adds W columns of a tile's fresh product to registers; DW = 32: of both halves of D (see product_cols)
+template <int DW, int W> __device__ __forceinline__ void add_cols(uint32_t at, float* o) {
+#pragma unroll
+  for (int c = 0; c < W; c += 16) {
+    uint32_t x[16];
+    ld16(at + c, x);
+    wait_ld(x);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[c + e] += __uint_as_float(x[e]);
+    if (DW == 32) {
+      ld16(at + 32 + c, x);
+      wait_ld(x);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) o[c + e] += __uint_as_float(x[e]);
+    }
+  }
+}
 // sub-tiles need 1024-byte alignment
 __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* p) { return p + ((1024u - (smem_addr(p) & 1023u)) & 1023u); }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 // 256 queries of one head: two tiles of 128 rows take turns, so that the exponentials of one run beside the products of the other.
-// Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t; P of a tile replaces its logits.
+// Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t; P of a tile replaces its logits.  (float32: logits at 256 t, the three
+// terms of P from there on, its output at 256 t + 192.)
 // The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
 // the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
 enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kSFull = kQFull + 2, kPFull = kSFull + 2, kOFull = kPFull + 2, kFix = kOFull + 2, kFwdBars };
 
-template <typename T>
+template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
+  using M = typename Operand<T, TERMS>::type;
+  using G = Geometry<TERMS, DW>;
   extern __shared__ unsigned char raw[];
   unsigned char* smem = aligned_smem(raw);
-  const int d = a.d, subs = d > 64 ? 2 : 1, tile_bytes = subs * kSub, R = ring_slots(subs);
+  const int d = a.d, subs = G::subs(d), tile_bytes = subs * (int)G::kSub, R = G::ring(d);
   Tail* tail = reinterpret_cast<Tail*>(smem + (2 + R) * tile_bytes);
   const uint32_t sq = smem_addr(smem), ring = sq + 2 * tile_bytes, bar0 = smem_addr(tail->bars);
   volatile int* failed = &tail->failed;
@@ -58,6 +95,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
   __syncthreads();
   fence_after();
   const uint32_t tmem = tail->tmem;
+  constexpr uint32_t kStride = TERMS == 1 ? kTile : 256, kOut = TERMS == 1 ? 256 : 192;
 
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
@@ -74,7 +112,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
         if ((t ? n1 : n0) == 0) continue;
         wait_bar(bar(kQFull + t), 0, failed, &g_packed_error);
         fence_after();
-        product_rows<T>(on, tmem + kTile * t, sq + t * tile_bytes, slot(0), d);
+        product_rows<M, TERMS, DW>(on, tmem + kStride * t, sq + t * tile_bytes, slot(0), d);
         commit(on, bar(kSFull + t));
       }
       give(0);
@@ -87,9 +125,10 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
           if (i >= nt) continue;
           wait_bar(bar(kPFull + t), i & 1, failed, &g_packed_error);
           fence_after();
-          product_cols<T>(on, tmem + 256 + kTile * t, tmem + kTile * t, 32, slot(2 * i + 1), d, i > 0);
+          const uint32_t at = tmem + kStride * t;
+          product_cols<M, TERMS, DW>(on, at + kOut, Packed{{at, at + 64, at + 128}, {32, 32, 32}}, slot(2 * i + 1), d, i > 0);
           if (i + 1 < nt) {
-            product_rows<T>(on, tmem + kTile * t, sq + t * tile_bytes, slot(2 * i + 2), d);
+            product_rows<M, TERMS, DW>(on, at, sq + t * tile_bytes, slot(2 * i + 2), d);
             commit(on, bar(kSFull + t));
           } else {
             commit(on, bar(kOFull + t));
@@ -99,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
         if (i + 1 < n) give(2 * i + 2);
       }
     } else if (warp == kLoadWarp && n > 0) {
-      Loader ld{lane, subs, bar(kFix)};
+      Loader<TERMS, DW> ld{lane, subs, bar(kFix)};
       for (int t = 0; t < 2; ++t)
         if ((t ? n1 : n0) > 0) ld.tile(sq + t * tile_bytes, &maps.q, q0 + row0 + t * kTile, h, bar(kQFull + t), kTile, false, failed, &g_packed_error);
       for (int j = 0; j < 2 * n; ++j) {
@@ -112,13 +151,18 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
     more_regs<kComputeRegs>();
     const int t = warp >> 2, w = warp & 3, nt = t ? n1 : n0;
     const int row = row0 + t * kTile + w * 32 + lane, first = row0 + t * kTile + w * 32;
-    const uint32_t ts = tmem + ((uint32_t)(32 * w) << 16) + kTile * t, to = ts + 256;
+    const uint32_t ts = tmem + ((uint32_t)(32 * w) << 16) + kStride * t, to = ts + kOut;
+    constexpr int kOwn = TERMS == 1 ? 1 : DW;
+    float own[kOwn];                         // the output so far (float32)
+#pragma unroll
+    for (int c = 0; c < kOwn; ++c) own[c] = 0.f;
     // last key that this row sees, and that the warp's first row sees
     const int lim = min(a.causal ? row + off : lk - 1, lk - 1), lim_first = min(a.causal ? first + off : lk - 1, lk - 1);
     float m = -INFINITY, l = 0.f;
     for (int i = 0; i < nt; ++i) {
       wait_bar(bar(kSFull + t), i & 1, failed, &g_packed_error);
       fence_after();
+      if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW>(to, own); }
       uint32_t x[kTile];
 #pragma unroll
       for (int c = 0; c < kTile; c += 32) ld32(ts + c, x + c);
@@ -140,7 +184,10 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
         const float f = raise ? pow2(m - mn) : 1.f;
         if (raise) m = mn;
         l *= f;
-        if (i > 0) {
+        if constexpr (TERMS == 3) {
+#pragma unroll
+          for (int c = 0; c < kOwn; ++c) own[c] *= f;
+        } else if (i > 0) {
           for (int c = 0; c < d; c += 16) {
             uint32_t o[16];
             ld16(to + c, o);
@@ -153,16 +200,16 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       }
       const float u = m == -INFINITY ? 0.f : -m;
       float l0 = 0.f, l1 = 0.f;
+      const Packed at{{0, 64, 128}, {}};
 #pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        uint32_t p[16];
+      for (int c = 0; c < kTile; c += 16) {
+        float y[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const float y0 = pow2(fmaf(__uint_as_float(x[c + 2 * e]), a.scale_log2, u)), y1 = pow2(fmaf(__uint_as_float(x[c + 2 * e + 1]), a.scale_log2, u));
-          l0 += y0; l1 += y1;
-          p[e] = packed::Half<T>::pack(y0, y1);
+        for (int e = 0; e < 16; e += 2) {
+          y[e] = pow2(fmaf(__uint_as_float(x[c + e]), a.scale_log2, u)); y[e + 1] = pow2(fmaf(__uint_as_float(x[c + e + 1]), a.scale_log2, u));
+          l0 += y[e]; l1 += y[e + 1];
         }
-        st16(ts + c / 2, p);
+        put16<M, TERMS>(at, ts, c, y);
       }
       l += l0 + l1;
       wait_st();
@@ -173,23 +220,39 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       wait_bar(bar(kOFull + t), 0, failed, &g_packed_error);
       fence_after();
     }
+    if constexpr (TERMS == 3) { if (nt > 0) add_cols<DW, DW>(to, own); }
     const bool there = row < lq, bad = *failed;
     const float inv = bad ? NAN : l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-    T* dst = static_cast<T*>(a.out) + ((long long)(q0 + row) * a.hq + h) * d;
-    for (int c = 0; c < d; c += 16) {
-      uint32_t o[16];
+    const long long at = ((long long)(q0 + row) * a.hq + h) * d;
+    T *dst = static_cast<T*>(a.out) + at, *rest = a.out_rest ? static_cast<T*>(a.out_rest) + at : nullptr;
+    if constexpr (TERMS == 3) {
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[e] = 0;
-      if (nt > 0) { ld16(to + c, o); wait_ld(o); }
-      uint32_t p[8];
+      for (int c = 0; c < kOwn; ++c) own[c] *= inv;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = packed::Half<T>::pack(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
-      if (there) {
-        *reinterpret_cast<uint4*>(dst + c) = make_uint4(p[0], p[1], p[2], p[3]);
-        *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(p[4], p[5], p[6], p[7]);
+      for (int c = 0; c < DW; c += 16) if (there && c < d) store16(dst + c, own + c);
+    } else {
+      for (int c = 0; c < d; c += 16) {
+        uint32_t o[16];
+        float y[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[e] = 0;
+        if (nt > 0) { ld16(to + c, o); wait_ld(o); }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(o[e]) * inv;
+        if (there) {
+          store16(dst + c, y);
+          if (rest) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const float2 r = packed::Half<T>::unpack(packed::Half<T>::pack(y[e], y[e + 1]));
+              y[e] -= r.x; y[e + 1] -= r.y;
+            }
+            store16(rest + c, y);
+          }
+        }
       }
     }
-    if (there && a.lse) a.lse[(long long)h * a.nq + q0 + row] = bad ? NAN : l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+    if (there && a.lse) a.lse[(long long)h * a.nq + q0 + row] = bad ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
     fence_before();
   }
   __syncthreads();
@@ -197,16 +260,18 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
 }
 
 // ---- reverse: dq ----------------------------------------------------------------------------------------------------
-// 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256.  The two groups of four warps
-// have 64 columns each of every row.  The next tile's logits are made as soon as these have been read, so that its exponentials run
+// 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256 (float32: the third term of dS
+// at 256, dq at 320).  The two groups of four warps have 64 columns each of every row.  The next tile's logits are made as soon as these have been read, so that its exponentials run
 // beside the products dS k and g v^T.
 enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqS, kdqSRead, kdqDp, kdqDs, kdqOut, kdqFix, kDqBars };
 
-template <typename T>
+template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
+  using M = typename Operand<T, TERMS>::type;
+  using G = Geometry<TERMS, DW>;
   extern __shared__ unsigned char raw[];
   unsigned char* smem = aligned_smem(raw);
-  const int d = a.d, subs = d > 64 ? 2 : 1, tile_bytes = subs * kSub, R = ring_slots(subs);
+  const int d = a.d, subs = G::subs(d), tile_bytes = subs * (int)G::kSub, R = G::ring(d);
   Tail* tail = reinterpret_cast<Tail*>(smem + (2 + R) * tile_bytes);
   const uint32_t sq = smem_addr(smem), sg = sq + tile_bytes, ring = sg + tile_bytes, bar0 = smem_addr(tail->bars);
   volatile int* failed = &tail->failed;
@@ -225,6 +290,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   __syncthreads();
   fence_after();
   const uint32_t tmem = tail->tmem;
+  constexpr uint32_t kOut = TERMS == 1 ? 256 : 320;
 
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
@@ -235,34 +301,37 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       auto give = [&](int j) { if (j + R < 2 * n) commit(on, bar(kdqEmpty + j % R)); };
       wait_bar(bar(kdqQ), 0, failed, &g_packed_error);
       ready(0);
-      product_rows<T>(on, tmem, sq, slot(0), d);
+      product_rows<M, TERMS, DW>(on, tmem, sq, slot(0), d);
       commit(on, bar(kdqS));
       ready(1);
-      product_rows<T>(on, tmem + kTile, sg, slot(1), d);
+      product_rows<M, TERMS, DW>(on, tmem + kTile, sg, slot(1), d);
       commit(on, bar(kdqDp));
       give(1);
       for (int i = 0; i < n; ++i) {
-        if (i + 1 < n) {
+        auto logits = [&] {
+          if (i + 1 == n) return;
           ready(2 * i + 2);
           wait_bar(bar(kdqSRead), i & 1, failed, &g_packed_error);
           fence_after();
-          product_rows<T>(on, tmem, sq, slot(2 * i + 2), d);
+          product_rows<M, TERMS, DW>(on, tmem, sq, slot(2 * i + 2), d);
           commit(on, bar(kdqS));
-        }
+        };
+        if (!G::kShort) logits();
         wait_bar(bar(kdqDs), i & 1, failed, &g_packed_error);
         fence_after();
-        product_cols<T>(on, tmem + 256, tmem + kTile, 64, slot(2 * i), d, i > 0);
+        product_cols<M, TERMS, DW>(on, tmem + kOut, Packed{{tmem + kTile, tmem + kTile + 32, tmem + 256}, {64, 64, 32}}, slot(2 * i), d, i > 0);
         give(2 * i);
+        if (G::kShort) logits();
         if (i + 1 < n) {
           ready(2 * i + 3);
-          product_rows<T>(on, tmem + kTile, sg, slot(2 * i + 3), d);
+          product_rows<M, TERMS, DW>(on, tmem + kTile, sg, slot(2 * i + 3), d);
           commit(on, bar(kdqDp));
           give(2 * i + 3);
         }
       }
       commit(on, bar(kdqOut));
     } else if (warp == kLoadWarp && n > 0) {
-      Loader ld{lane, subs, bar(kdqFix)};
+      Loader<TERMS, DW> ld{lane, subs, bar(kdqFix)};
       if (lane == 0) {
         expect(bar(kdqQ), 2 * tile_bytes);
         ld.copies(sq, &maps.q, q0 + row0, h, bar(kdqQ));
@@ -282,7 +351,12 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
     const int lim = min(a.causal ? row + off : lk - 1, lk - 1), lim_first = min(a.causal ? first + off : lk - 1, lk - 1);
     const long long at = (long long)h * a.nq + q0 + row;
     const bool there = row < lq;
-    const float e = there ? -a.lse[at] * kLog2e : -INFINITY, delta = there ? a.delta[at] : 0.f;
+    const float e = there ? -a.lse[at] : -INFINITY, delta = there ? a.delta[at] : 0.f;
+    constexpr int kOwn = TERMS == 1 ? 1 : DW / 2;
+    float own[kOwn];                         // dq so far (float32), half of the row
+#pragma unroll
+    for (int c = 0; c < kOwn; ++c) own[c] = 0.f;
+    const Packed to{{kTile + (uint32_t)col, kTile + 32 + (uint32_t)col, 256 + (uint32_t)col / 2}, {}};
     for (int i = 0; i < n; ++i) {
       uint32_t x[64], y[64];
       wait_bar(bar(kdqS), i & 1, failed, &g_packed_error);
@@ -300,6 +374,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       ld32(lanes + kTile + col, y);
       ld32(lanes + kTile + col + 32, y + 32);
       wait_ld(y);
+      if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own); }
 #pragma unroll
       for (int c = 0; c < 64; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * (__uint_as_float(y[c]) - delta));
       if (kb + 63 > lim_first) {
@@ -307,9 +382,12 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
         for (int c = 0; c < 64; ++c) if (kb + c > lim) x[c] = 0;
       }
 #pragma unroll
-      for (int c = 0; c < 32; ++c) y[c] = packed::Half<T>::pack(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1]));
-      st16(lanes + kTile + col, y);
-      st16(lanes + kTile + col + 16, y + 16);
+      for (int c = 0; c < 64; c += 16) {
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(x[c + k]);
+        put16<M, TERMS>(to, lanes, c, v);
+      }
       wait_st();
       fence_before();
       arrive(bar(kdqDs));
@@ -320,16 +398,22 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
     }
     const float f = *failed ? NAN : a.scale;
     T* dst = static_cast<T*>(a.dq) + ((long long)(q0 + row) * a.hq + h) * d;
-    for (int c = 16 * half; c < d; c += 32) {
-      uint32_t o[16], p[8];
+    if constexpr (TERMS == 3) {
+      if (n > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) o[k] = 0;
-      if (n > 0) { ld16(lanes + 256 + c, o); wait_ld(o); }
+      for (int c = 0; c < kOwn; ++c) own[c] *= f;
 #pragma unroll
-      for (int k = 0; k < 8; ++k) p[k] = packed::Half<T>::pack(__uint_as_float(o[2 * k]) * f, __uint_as_float(o[2 * k + 1]) * f);
-      if (there) {
-        *reinterpret_cast<uint4*>(dst + c) = make_uint4(p[0], p[1], p[2], p[3]);
-        *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(p[4], p[5], p[6], p[7]);
+      for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own + c);
+    } else {
+      for (int c = 16 * half; c < d; c += 32) {
+        uint32_t o[16];
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = 0;
+        if (n > 0) { ld16(lanes + kOut + c, o); wait_ld(o); }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(o[k]) * f;
+        if (there) store16(dst + c, v);
       }
     }
     fence_before();
@@ -340,16 +424,19 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
 
 // ---- reverse: dk and dv ---------------------------------------------------------------------------------------------
 // 128 keys of one key head: rows of the products are keys, columns the queries of all heads of the group, 128 at a time.  Tensor memory:
-// logits at 0 (P replaces them), dP at 128 (dS replaces it), dv at 256, dk at 384.  The tensor cores work in the order
+// logits at 0 (P replaces them), dP at 128 (dS replaces it), dv at 256, dk at 384 (float32: the third terms of P and dS at 256 and 320, dv
+// at 384, dk at 448).  The tensor cores work in the order
 // dv(i), logits(i + 1), dk(i), dP(i + 1): each pair runs beside the other half of the elementwise work.
 enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvFix, kkvStat, kkvStatFree = kkvStat + 2,
               kDkvBars = kkvStatFree + 2 };
 
-template <typename T>
+template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
+  using M = typename Operand<T, TERMS>::type;
+  using G = Geometry<TERMS, DW>;
   extern __shared__ unsigned char raw[];
   unsigned char* smem = aligned_smem(raw);
-  const int d = a.d, subs = d > 64 ? 2 : 1, tile_bytes = subs * kSub, R = ring_slots(subs);
+  const int d = a.d, subs = G::subs(d), tile_bytes = subs * (int)G::kSub, R = G::ring(d);
   float* stats = reinterpret_cast<float*>(smem + (2 + R) * tile_bytes);      // [2][128] -lse in log2, [2][128] -delta
   Tail* tail = reinterpret_cast<Tail*>(stats + 4 * kTile);
   const uint32_t sk = smem_addr(smem), sv = sk + tile_bytes, ring = sv + tile_bytes, bar0 = smem_addr(tail->bars);
@@ -371,44 +458,48 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   __syncthreads();
   fence_after();
   const uint32_t tmem = tail->tmem;
+  constexpr uint32_t kDv = TERMS == 1 ? 256 : 384, kDk = TERMS == 1 ? 384 : 448;
 
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
     if (warp == kMmaWarp && n > 0) {
-      const uint32_t on = elect_one(), dv = tmem + 256, dk = tmem + 256 + kTile;
+      const uint32_t on = elect_one();
       auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };      // queries 0, 2, .., cotangents 1, 3, ..
       auto ready = [&](int j) { wait_bar(bar(kkvFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
       auto give = [&](int j) { if (j + R < 2 * n) commit(on, bar(kkvEmpty + j % R)); };
       wait_bar(bar(kkvK), 0, failed, &g_packed_error);
       ready(0);
-      product_rows<T>(on, tmem, sk, slot(0), d);
+      product_rows<M, TERMS, DW>(on, tmem, sk, slot(0), d);
       commit(on, bar(kkvS));
       ready(1);
-      product_rows<T>(on, tmem + kTile, sv, slot(1), d);
+      product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(1), d);
       commit(on, bar(kkvDp));
       for (int i = 0; i < n; ++i) {
         wait_bar(bar(kkvP), i & 1, failed, &g_packed_error);
         fence_after();
-        product_cols<T>(on, dv, tmem, 64, slot(2 * i + 1), d, i > 0);
+        product_cols<M, TERMS, DW>(on, tmem + kDv, Packed{{tmem, tmem + 32, tmem + 256}, {64, 64, 32}}, slot(2 * i + 1), d, i > 0);
         give(2 * i + 1);
-        if (i + 1 < n) {
+        auto logits = [&] {
+          if (i + 1 == n) return;
           ready(2 * i + 2);
-          product_rows<T>(on, tmem, sk, slot(2 * i + 2), d);
+          product_rows<M, TERMS, DW>(on, tmem, sk, slot(2 * i + 2), d);
           commit(on, bar(kkvS));
-        }
+        };
+        if (!G::kShort) logits();
         wait_bar(bar(kkvDs), i & 1, failed, &g_packed_error);
         fence_after();
-        product_cols<T>(on, dk, tmem + kTile, 64, slot(2 * i), d, i > 0);
+        product_cols<M, TERMS, DW>(on, tmem + kDk, Packed{{tmem + kTile, tmem + kTile + 32, tmem + 320}, {64, 64, 32}}, slot(2 * i), d, i > 0);
         give(2 * i);
+        if (G::kShort) logits();
         if (i + 1 < n) {
           ready(2 * i + 3);
-          product_rows<T>(on, tmem + kTile, sv, slot(2 * i + 3), d);
+          product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(2 * i + 3), d);
           commit(on, bar(kkvDp));
         }
       }
       commit(on, bar(kkvOut));
     } else if (warp == kLoadWarp && n > 0) {
-      Loader ld{lane, subs, bar(kkvFix)};
+      Loader<TERMS, DW> ld{lane, subs, bar(kkvFix)};
       if (lane == 0) {
         expect(bar(kkvK), 2 * tile_bytes);
         ld.copies(sk, &maps.k, c0 + row0, kvh, bar(kkvK));
@@ -428,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         for (int r = r0; r < kTile; r += 64) {
           const bool ok = b + r < lq;
           const long long at = (long long)hq * a.nq + q0 + b + r;
-          stats[st * kTile + r] = ok ? fmaf(-a.lse[at], kLog2e, packed::prob_shift<T>()) : -INFINITY;
+          stats[st * kTile + r] = ok ? packed::prob_shift<T>() - a.lse[at] : -INFINITY;
           stats[(2 + st) * kTile + r] = ok ? -a.delta[at] * packed::prob_unscale<T>() : 0.f;
         }
         arrive(bar(kkvStat + st));
@@ -440,6 +531,12 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
     const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16);
     // first query that sees this key, and that sees the warp's last key
     const int lim = a.causal ? row - off : 0, lim_last = a.causal ? last - off : 0;
+    constexpr int kOwn = TERMS == 1 ? 1 : DW / 2;
+    float own[2][kOwn];                      // dv, dk so far (float32), half of the row
+#pragma unroll
+    for (int c = 0; c < kOwn; ++c) own[0][c] = own[1][c] = 0.f;
+    const Packed to_p{{(uint32_t)col, 32 + (uint32_t)col, 256 + (uint32_t)col / 2}, {}},
+        to_s{{kTile + (uint32_t)col, kTile + 32 + (uint32_t)col, 320 + (uint32_t)col / 2}, {}};
     for (int i = 0; i < n; ++i) {
       const int st = i & 1, ib = i0 + (i % per) * kTile + col;
       uint32_t x[64], y[64];
@@ -449,6 +546,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       ld32(lanes + col, x);
       ld32(lanes + col + 32, x + 32);
       wait_ld(x);
+      if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDv + half * (DW / 2), own[0]); }
       const float4* e = reinterpret_cast<const float4*>(stats + st * kTile + col);
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
@@ -463,9 +561,12 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         for (int c = 0; c < 64; ++c) if (ib + c < lim) x[c] = 0;
       }
 #pragma unroll
-      for (int c = 0; c < 32; ++c) y[c] = packed::Half<T>::pack(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1]));
-      st16(lanes + col, y);
-      st16(lanes + col + 16, y + 16);
+      for (int c = 0; c < 64; c += 16) {
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(x[c + k]);
+        put16<M, TERMS>(to_p, lanes, c, v);
+      }
       wait_st();
       fence_before();
       arrive(bar(kkvP));
@@ -474,20 +575,24 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       ld32(lanes + kTile + col, y);
       ld32(lanes + kTile + col + 32, y + 32);
       wait_ld(y);
+      if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDk + half * (DW / 2), own[1]); }
       const float4* dl = reinterpret_cast<const float4*>(stats + (2 + st) * kTile + col);
       constexpr float un = packed::prob_unscale<T>();
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float4 v = dl[c];
-        const float s0 = __uint_as_float(x[4 * c]) * fmaf(__uint_as_float(y[4 * c]), un, v.x), s1 = __uint_as_float(x[4 * c + 1]) * fmaf(__uint_as_float(y[4 * c + 1]), un, v.y);
-        const float s2 = __uint_as_float(x[4 * c + 2]) * fmaf(__uint_as_float(y[4 * c + 2]), un, v.z), s3 = __uint_as_float(x[4 * c + 3]) * fmaf(__uint_as_float(y[4 * c + 3]), un, v.w);
-        y[2 * c] = packed::Half<T>::pack(s0, s1);
-        y[2 * c + 1] = packed::Half<T>::pack(s2, s3);
+      for (int c = 0; c < 64; c += 16) {
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+          const float4 z = dl[(c + k) / 4];
+          v[k] = __uint_as_float(x[c + k]) * fmaf(__uint_as_float(y[c + k]), un, z.x);
+          v[k + 1] = __uint_as_float(x[c + k + 1]) * fmaf(__uint_as_float(y[c + k + 1]), un, z.y);
+          v[k + 2] = __uint_as_float(x[c + k + 2]) * fmaf(__uint_as_float(y[c + k + 2]), un, z.z);
+          v[k + 3] = __uint_as_float(x[c + k + 3]) * fmaf(__uint_as_float(y[c + k + 3]), un, z.w);
+        }
+        put16<M, TERMS>(to_s, lanes, c, v);
       }
       __syncwarp();
       if (lane == 0) arrive(bar(kkvStatFree + st));
-      st16(lanes + kTile + col, y);
-      st16(lanes + kTile + col + 16, y + 16);
       wait_st();
       fence_before();
       arrive(bar(kkvDs));
@@ -501,17 +606,24 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
       const float f = bad ? NAN : which ? a.scale : packed::prob_unscale<T>();
+      const uint32_t from = lanes + (which ? kDk : kDv);
       T* dst = static_cast<T*>(which ? a.dk : a.dv) + at;
-      for (int c = 16 * half; c < d; c += 32) {
-        uint32_t o[16], p[8];
+      if constexpr (TERMS == 3) {
+        if (n > 0) add_cols<DW, DW / 2>(from + half * (DW / 2), own[which]);
 #pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] = 0;
-        if (n > 0) { ld16(lanes + 256 + which * kTile + c, o); wait_ld(o); }
+        for (int c = 0; c < kOwn; ++c) own[which][c] *= f;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) p[k] = packed::Half<T>::pack(__uint_as_float(o[2 * k]) * f, __uint_as_float(o[2 * k + 1]) * f);
-        if (there) {
-          *reinterpret_cast<uint4*>(dst + c) = make_uint4(p[0], p[1], p[2], p[3]);
-          *reinterpret_cast<uint4*>(dst + c + 8) = make_uint4(p[4], p[5], p[6], p[7]);
+        for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own[which] + c);
+      } else {
+        for (int c = 16 * half; c < d; c += 32) {
+          uint32_t o[16];
+          float v[16];
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = 0;
+          if (n > 0) { ld16(from + c, o); wait_ld(o); }
+#pragma unroll
+          for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(o[k]) * f;
+          if (there) store16(dst + c, v);
         }
       }
     }
@@ -522,7 +634,37 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
 }
 
 static_assert(kFwdBars <= 32 && kDqBars <= 32 && kDkvBars <= 32, "barriers");
-int smem_bytes(int d, bool stats) { return 1024 + (d > 64 ? 6 * 2 : 10) * (int)kSub + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail); }
+
+// float32 rows -> three bfloat16 terms, (rows, heads, 3, DW), zeros behind d; a thread per eight values, up to four operands
+struct SplitArgs { Rows src[4]; __nv_bfloat16* dst[4]; int rows[4], heads[4]; };
+template <int DW>
+__global__ void __launch_bounds__(256) split_kernel(const SplitArgs A, int d) {
+  const int o = blockIdx.y;
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x, hr = e / (DW / 8);
+  const int part = (int)(e % (DW / 8)) * 8;
+  if (hr >= (long long)A.rows[o] * A.heads[o]) return;
+  const long long r = hr / A.heads[o];
+  const int h = (int)(hr % A.heads[o]);
+  float v[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] = 0.f;
+  if (part < d) {
+    const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(A.src[o].p) + r * A.src[o].row + h * A.src[o].head + part);
+    const float4 x = p[0], y = p[1];
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+  }
+#pragma unroll
+  for (int term = 0; term < 3; ++term) {
+    uint32_t u[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      u[k] = packed::Half<__nv_bfloat16>::pack(v[2 * k], v[2 * k + 1]);
+      const float2 f = packed::Half<__nv_bfloat16>::unpack(u[k]);
+      v[2 * k] -= f.x; v[2 * k + 1] -= f.y;
+    }
+    *reinterpret_cast<uint4*>(A.dst[o] + (hr * 3 + term) * DW + part) = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
 
 using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                             CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -535,51 +677,85 @@ Encode encoder() {
   }();
   return fn;
 }
-template <typename T> bool map_of(CUtensorMap* m, const Rows& r, long long rows, int heads, int d) {
+// (values, rows, heads) of 16-bit values; boxes of `width` values x 128 rows, a row as long as the swizzle
+bool map_of(CUtensorMap* m, bool bf16, const Rows& r, long long rows, int heads, int d, int width) {
   const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)rows, (cuuint64_t)heads};
   const cuuint64_t strides[2] = {(cuuint64_t)r.row * 2, (cuuint64_t)r.head * 2};
-  const cuuint32_t box[3] = {64, kTile, 1}, ones[3] = {1, 1, 1};
-  return encoder()(m, std::is_same<T, __nv_bfloat16>::value ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(r.p), dims,
-                   strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+  const cuuint32_t box[3] = {(cuuint32_t)width, kTile, 1}, ones[3] = {1, 1, 1};
+  return encoder()(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(r.p), dims, strides, box, ones,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, width == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-template <typename T> bool maps_of(Maps* m, const PackedArgs& a, bool reverse) {
-  if (!encoder()) return false;
-  return map_of<T>(&m->q, a.q, a.nq, a.hq, a.d) && map_of<T>(&m->k, a.k, a.nkv, a.hk, a.d) && map_of<T>(&m->v, a.v, a.nkv, a.hk, a.d) &&
-         (reverse ? map_of<T>(&m->g, a.g, a.nq, a.hq, a.d) : (m->g = m->q, true));
+template <typename T, int TERMS, int DW> int maps_of(Maps* m, cudaStream_t st, const PackedArgs& a, bool reverse, void* workspace) {
+  if (!encoder()) return kCudaError;
+  CUtensorMap* maps[4] = {&m->q, &m->k, &m->v, &m->g};
+  const Rows rows[4] = {a.q, a.k, a.v, a.g};
+  const int n[4] = {a.nq, a.nkv, a.nkv, a.nq}, heads[4] = {a.hq, a.hk, a.hk, a.hq}, operands = reverse ? 4 : 3;
+  if constexpr (TERMS == 1) {
+    for (int i = 0; i < operands; ++i)
+      if (!map_of(maps[i], std::is_same<T, __nv_bfloat16>::value, rows[i], n[i], heads[i], a.d, 64)) return kInvalidArgument;
+  } else {
+    SplitArgs A;
+    __nv_bfloat16* at = static_cast<__nv_bfloat16*>(workspace);
+    long long most = 0;
+    for (int i = 0; i < operands; ++i) {
+      A.src[i] = rows[i]; A.dst[i] = at; A.rows[i] = n[i]; A.heads[i] = heads[i];
+      const long long values = (long long)n[i] * heads[i] * 3 * DW;
+      if (!map_of(maps[i], true, Rows{at, (long long)heads[i] * 3 * DW, DW}, n[i], 3 * heads[i], DW, DW)) return kInvalidArgument;
+      at += values;
+      most = std::max(most, values);
+    }
+    split_kernel<DW><<<dim3((unsigned)((most / 24 + 255) / 256), operands), 256, 0, st>>>(A, a.d);
+    count_launch();
+  }
+  if (!reverse) m->g = m->q;
+  return kOk;
 }
-template <typename K> int launch(K kernel, dim3 grid, bool stats, cudaStream_t st, const PackedArgs& a, const Maps& m) {
-  const int smem = smem_bytes(a.d, stats);
+template <int TERMS, int DW, typename K> int launch(K kernel, dim3 grid, bool stats, cudaStream_t st, const PackedArgs& a, const Maps& m) {
+  using G = Geometry<TERMS, DW>;
+  const int smem = 1024 + (2 + G::ring(a.d)) * G::subs(a.d) * (int)G::kSub + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail);
   SO3LR_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   kernel<<<grid, kThreads, smem, st>>>(a, m);
   count_launch();
   return kOk;
 }
+template <typename T, int TERMS, int DW> int forward_of(cudaStream_t st, const PackedArgs& a, int n_items, void* workspace) {
+  Maps m;
+  const int rc = maps_of<T, TERMS, DW>(&m, st, a, false, workspace);
+  return rc ? rc : launch<TERMS, DW>(forward_kernel<T, TERMS, DW>, dim3(n_items, a.hq), false, st, a, m);
+}
+template <typename T, int TERMS, int DW>
+int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, void* workspace) {
+  Maps m;
+  int rc = maps_of<T, TERMS, DW>(&m, st, a, true, workspace);
+  if (rc) return rc;
+  a.items = items_q;
+  rc = launch<TERMS, DW>(dq_kernel<T, TERMS, DW>, dim3(n_q, a.hq), false, st, a, m);
+  if (rc) return rc;
+  a.items = items_kv;
+  return launch<TERMS, DW>(dkv_kernel<T, TERMS, DW>, dim3(n_kv, a.hk), true, st, a, m);
+}
 
 }  // namespace
 
-template <typename T> int packed_forward_tc(cudaStream_t st, const PackedArgs& a, int n_items) {
-  Maps m;
-  if (!maps_of<T>(&m, a, false)) return kInvalidArgument;
-  return launch(forward_kernel<T>, dim3(n_items, a.hq), false, st, a, m);
+template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, void* workspace) {
+  if constexpr (sizeof(T) == 2) return forward_of<T, 1, 64>(st, a, n_items, workspace);
+  else return a.d <= 32 ? forward_of<T, 3, 32>(st, a, n_items, workspace) : forward_of<T, 3, 64>(st, a, n_items, workspace);
 }
-template <typename T> int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv) {
-  Maps m;
-  if (!maps_of<T>(&m, a, true)) return kInvalidArgument;
-  a.items = items_q;
-  const int rc = launch(dq_kernel<T>, dim3(n_q, a.hq), false, st, a, m);
-  if (rc) return rc;
-  a.items = items_kv;
-  return launch(dkv_kernel<T>, dim3(n_kv, a.hk), true, st, a, m);
+template <typename T> int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, void* workspace) {
+  if constexpr (sizeof(T) == 2) return reverse_of<T, 1, 64>(st, a, items_q, n_q, items_kv, n_kv, workspace);
+  else return a.d <= 32 ? reverse_of<T, 3, 32>(st, a, items_q, n_q, items_kv, n_kv, workspace) : reverse_of<T, 3, 64>(st, a, items_q, n_q, items_kv, n_kv, workspace);
 }
 int packed_error(int* out) {
   const cudaError_t e = cudaMemcpyFromSymbol(out, g_packed_error, sizeof(int));
   return e == cudaSuccess ? kOk : kCudaError;
 }
 
-template int packed_forward_tc<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
-template int packed_forward_tc<__half>(cudaStream_t, const PackedArgs&, int);
-template int packed_reverse_tc<__nv_bfloat16>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int);
-template int packed_reverse_tc<__half>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int);
+template int packed_forward_tc<__nv_bfloat16>(cudaStream_t, PackedArgs, int, void*);
+template int packed_reverse_tc<__nv_bfloat16>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int, void*);
+template int packed_forward_tc<__half>(cudaStream_t, PackedArgs, int, void*);
+template int packed_reverse_tc<__half>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int, void*);
+template int packed_forward_tc<float>(cudaStream_t, PackedArgs, int, void*);
+template int packed_reverse_tc<float>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int, void*);
 
 }  // namespace so3lr

@@ -1,7 +1,6 @@
 // What the tensor-core kernels of attention inside packed structures share: operand tiles, descriptors, barriers, tensor memory.
 //
-// An operand tile is 128 rows of 64 values (128 bytes a row, 128-byte swizzle), one or two of them side by side for up to 64 or 128 values
-// a head, brought in by TMA from the strided operand: a map has the dimensions (values, rows, heads), values behind the last one come as
+// An operand tile is 128 rows of up to 64 values (64 or 128 bytes a row, swizzled), several of them side by side (Geometry), brought in by TMA from the strided operand: a map has the dimensions (values, rows, heads), values behind the last one come as
 // zeros.  The same image serves the tensor cores with d contracted (K-major) and with the rows contracted (MN-major), so a tile of keys
 // serves q k^T and dS k, a tile of queries k q^T and dS^T q.  A tile may reach over the end of its structure into the next one's rows: where
 // they would be contracted, the loading warp clears them before it hands the tile over (a zero probability times a neighbour's NaN is NaN).
@@ -13,8 +12,6 @@
 namespace so3lr {
 namespace tc {
 
-using packed::kLn2;
-using packed::kLog2e;
 using packed::smem_addr;
 
 constexpr int kTile = 128;
@@ -71,14 +68,26 @@ __device__ __forceinline__ float pow2(float x) {
 }
 
 // ---- matrix instructions ----
-// Descriptor of an operand tile, 128-byte swizzle.  K-major: 16 contracted values are 32 bytes further, 64 are a sub-tile further; groups of
-// eight rows lie 1024 bytes apart.  MN-major: 16 contracted rows are 2048 bytes further, 64 values of N a sub-tile.
-constexpr uint32_t kSub = 128 * 128;       // bytes of a sub-tile
-__device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn_major) {
-  return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(mn_major ? kSub >> 4 : 1) << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-__device__ __forceinline__ uint32_t step_k(int k) { return ((k & 3) * 32 + (k >> 2) * kSub) >> 4; }
-constexpr uint32_t kStepMn = 2048 >> 4;
+// Geometry of operand tiles.  TERMS = 1: 16-bit values, sub-tiles of 64 values (128-byte rows and swizzle), one or two.  TERMS = 3: float32
+// values split into three bfloat16 terms, x = t0 + t1 + t2 to 2^-24, a sub-tile per term of DW = 32 or 64 values (64- or 128-byte rows and
+// swizzle).  A product of two such operands takes the six products of terms that are above 2^-24 of it, small ones first.
+template <int TERMS, int DW> struct Geometry {
+  static constexpr int kRow = TERMS == 1 ? 128 : 2 * DW;      // bytes of a row
+  static constexpr uint32_t kSub = kTile * kRow;              // bytes of a sub-tile
+  static __device__ __host__ __forceinline__ int subs(int d) { return TERMS == 1 ? (d > 64 ? 2 : 1) : 3; }
+  // Tiles that stream through: a ring, the two kinds of tile in turn; tile j sits in slot j % R.
+  static __device__ __host__ __forceinline__ int ring(int d) { return TERMS == 1 ? (d > 64 ? 4 : 8) : DW == 32 ? 6 : 2; }
+  // a ring of one tile of each kind: the reverse kernels make the next logits only behind the product that reads the tile in its slot
+  static constexpr bool kShort = TERMS == 3 && DW == 64;
+  // Descriptor.  K-major: 16 contracted values are 32 bytes further, 64 are a sub-tile further; groups of eight rows lie 8 rows apart.
+  // MN-major: 16 contracted rows are 16 rows further, the next values of N a sub-tile.
+  static __device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn_major) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(mn_major ? kSub >> 4 : 1) << 16) | ((uint64_t)(8 * kRow >> 4) << 32) | ((uint64_t)1 << 46) |
+           ((uint64_t)(kRow == 128 ? 2 : 4) << 61);
+  }
+  static __device__ __forceinline__ uint32_t step_k(int k) { return ((k & 3) * 32 + (k >> 2) * kSub) >> 4; }
+  static constexpr uint32_t kStepMn = 16 * kRow >> 4, kStepTerm = kSub >> 4;
+};
 template <typename T> __device__ __forceinline__ uint32_t idesc(int n, bool b_mn_major) {
   const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
@@ -100,18 +109,50 @@ __device__ __forceinline__ void commit(uint32_t on, uint32_t bar) {
       "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}\n" ::"r"(bar), "r"(on) : "memory");
 }
 // D[128 x 128] = A B^T over d columns, both tiles in shared memory
-template <typename T> __device__ __forceinline__ void product_rows(uint32_t on, uint32_t dst, uint32_t a, uint32_t b, int d) {
-  const uint64_t da = desc(a, false), db = desc(b, false);
+template <typename T, int TERMS, int DW> __device__ __forceinline__ void product_rows(uint32_t on, uint32_t dst, uint32_t a, uint32_t b, int d) {
+  using G = Geometry<TERMS, DW>;
+  const uint64_t da = G::desc(a, false), db = G::desc(b, false);
   const uint32_t id = idesc<T>(kTile, false);
+  if constexpr (TERMS == 1) {
 #pragma unroll 1
-  for (int k = 0; k < d / 16; ++k) mma_ss(on, dst, da + step_k(k), db + step_k(k), id, k > 0);
+    for (int k = 0; k < d / 16; ++k) mma_ss(on, dst, da + G::step_k(k), db + G::step_k(k), id, k > 0);
+  } else {
+#pragma unroll 1
+    for (int e = 0; e < 6; ++e) {
+      // (2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)
+      const uint32_t x = e == 0 ? 2 : (e == 2 || e == 3), y = e == 1 ? 2 : (e == 2 || e == 4);
+      const uint64_t ax = da + x * G::kStepTerm, by = db + y * G::kStepTerm;
+      for (int k = 0; k < DW / 16; ++k) mma_ss(on, dst, ax + G::step_k(k), by + G::step_k(k), id, (e | k) > 0);
+    }
+  }
 }
-// D[128 x d] (+)= A B: A 128 x 128 in tensor memory, 64 packed columns as two halves `gap` columns apart, B a tile with its rows contracted
-template <typename T> __device__ __forceinline__ void product_cols(uint32_t on, uint32_t dst, uint32_t a, int gap, uint32_t b, int d, uint32_t acc) {
-  const uint64_t db = desc(b, true);
-  const uint32_t id = idesc<T>(d, true);
+// where a 128 x 128 operand packed to 16 bits sits in tensor memory: 64 columns in two halves `gap` columns apart, for each of its terms
+struct Packed { uint32_t at[3]; int gap[3]; };
+// D[128 x d] (+)= A B: A in tensor memory, B a tile with its rows contracted.  Three terms and DW = 32: two terms of B side by side as N = 64,
+// D = [.. t0 | .. t1 and t2], whose halves are to be added; started afresh every time.
+template <typename T, int TERMS, int DW> __device__ __forceinline__ void product_cols(uint32_t on, uint32_t dst, const Packed& a, uint32_t b, int d, uint32_t acc) {
+  using G = Geometry<TERMS, DW>;
+  const uint64_t db = G::desc(b, true);
+  auto steps = [&](int term, uint64_t bt, uint32_t to, int n, uint32_t add) {
+    const uint32_t id = idesc<T>(n, true);
 #pragma unroll 1
-  for (int k = 0; k < 8; ++k) mma_ts(on, dst, a + (k & 3) * 8 + (k >> 2) * gap, db + k * kStepMn, id, acc | (k > 0));
+    for (int k = 0; k < 8; ++k) mma_ts(on, to, a.at[term] + (k & 3) * 8 + (k >> 2) * a.gap[term], bt + k * G::kStepMn, id, add | (k > 0));
+  };
+  if constexpr (TERMS == 1) {
+    steps(0, db, dst, d, acc);
+  } else if constexpr (DW == 32) {
+    steps(2, db, dst, 32, 0);
+    steps(0, db + 2 * G::kStepTerm, dst + 32, 32, 0);
+    steps(1, db, dst, 64, 1);
+    steps(0, db, dst, 64, 1);
+  } else {
+    steps(2, db, dst, 64, 0);
+    steps(0, db + 2 * G::kStepTerm, dst, 64, 1);
+    steps(1, db + G::kStepTerm, dst, 64, 1);
+    steps(1, db, dst, 64, 1);
+    steps(0, db + G::kStepTerm, dst, 64, 1);
+    steps(0, db, dst, 64, 1);
+  }
 }
 
 // ---- tensor memory ----
@@ -131,6 +172,9 @@ __device__ __forceinline__ void st16(uint32_t addr, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
                ::"r"(addr), I8(r, 0), I8(r, 8) : "memory");
 }
+__device__ __forceinline__ void st8(uint32_t addr, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr), I8(r, 0) : "memory");
+}
 #undef R8
 #undef O8
 #undef I8
@@ -141,6 +185,27 @@ template <int N> __device__ __forceinline__ void wait_ld(uint32_t (&r)[N]) {
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
 __device__ __forceinline__ void wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// sixteen values as eight packed pairs, in one or three terms, to the places of `to` that belong to column `c` (a multiple of 16 of the
+// 64 of a half, or of all 128 where the halves lie together)
+template <typename T, int TERMS> __device__ __forceinline__ void put16(const Packed& to, uint32_t lanes, int c, const float* v) {
+  uint32_t p[8];
+  float r[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) r[i] = v[i];
+#pragma unroll
+  for (int term = 0; term < TERMS; ++term) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      p[i] = packed::Half<T>::pack(r[2 * i], r[2 * i + 1]);
+      if (term + 1 < TERMS) {
+        const float2 u = packed::Half<T>::unpack(p[i]);
+        r[2 * i] -= u.x; r[2 * i + 1] -= u.y;
+      }
+    }
+    st8(lanes + to.at[term] + c / 2, p);
+  }
+}
 
 // ---- loading ----
 struct Maps { CUtensorMap q, k, v, g; };
@@ -153,11 +218,12 @@ __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
 }
 // The whole loading warp calls it.  rows: how many of the tile's 128 rows belong to the structure; where `clear`, the others are cleared
 // (through `fix`, a barrier of this warp's own, and its parity).
-struct Loader {
+template <int TERMS, int DW> struct Loader {
+  static constexpr uint32_t kSub = Geometry<TERMS, DW>::kSub;
   int lane, subs;
   uint32_t fix, parity = 0;
   __device__ __forceinline__ void copies(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t bar) const {
-    for (int x = 0; x < subs; ++x) tma(dst + x * kSub, map, 64 * x, row, head, bar);
+    for (int x = 0; x < subs; ++x) tma(dst + x * kSub, map, TERMS == 1 ? 64 * x : 0, row, TERMS == 1 ? head : 3 * head + x, bar);
   }
   __device__ __forceinline__ void tile(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t full, int rows, bool clear, volatile int* failed,
                                        int* error) {
@@ -171,7 +237,7 @@ struct Loader {
     wait_bar(fix, parity, failed, error);
     parity ^= 1;
     for (int x = 0; x < subs; ++x)
-      for (int b = rows * 128 + lane * 16; b < (int)kSub; b += 512)
+      for (int b = rows * Geometry<TERMS, DW>::kRow + lane * 16; b < (int)kSub; b += 512)
         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + x * kSub + b), "r"(0) : "memory");
     fence_smem();
     __syncwarp();

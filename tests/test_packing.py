@@ -92,8 +92,8 @@ def test_refused_calls_at_the_c_entry():
     def call(shape=None, q=r, image=h, dev=fake, out=fake):
         s = AttentionShape(**{**good, **(shape or {})})
         a = (image, dev, None, C.byref(s), C.byref(q) if q else None, C.byref(r), C.byref(r))
-        return {lib.so3lr_b200_structure_attention(*a, out, None, None, 0),
-                lib.so3lr_b200_structure_attention_vjp(*a, out, fake, C.byref(q) if q else None, fake, out, fake, fake)}
+        return {lib.so3lr_b200_structure_attention(*a, out, None, None, None, 0),
+                lib.so3lr_b200_structure_attention_vjp(*a, out, None, fake, C.byref(q) if q else None, fake, out, fake, fake, None, 0)}
 
     for bad in (dict(type=3), dict(type=-1), dict(heads_q=3), dict(heads_kv=0), dict(heads_q=0), dict(d=24), dict(d=8), dict(d=144), dict(rows_q=4),
                 dict(rows_kv=4), dict(rows_q=2**31), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf"))):
