@@ -23,27 +23,33 @@ from torch.autograd.function import once_differentiable
 from ._lib import AttentionShape, NormRotateArgs, Rows, check, lib
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-
-
-def _stream(t):
-    return C.c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+_UNIT = {torch.float32: 4, torch.bfloat16: 8, torch.float16: 8}      # values of 16 bytes
+_raw_stream = torch._C._cuda_getCurrentRawStream                     # of a device ordinal: torch.cuda.current_stream(..).cuda_stream without its object
 
 
 def _p(t):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return 0 if t is None else t.data_ptr()
+
+
+def _aligned(t, unit):
+    """`t` (rows, heads, d) in a form that the kernels read: as it is where its last axis is contiguous, 16-byte pieces are aligned and no axis
+    is broadcast, else a contiguous copy."""
+    a, b, c = t.stride()
+    if c != 1 or not a or not b or (a | b) % unit or t.data_ptr() % 16:
+        t = t.contiguous()
+        if t.data_ptr() % 16 or 0 in t.stride():
+            t = t.clone(memory_format=torch.contiguous_format)
+    return t
 
 
 def _head_rows(name, t, dtype, device, d=None):
-    """`t` (rows, heads, d) in a form that the kernels read: as it is where its last axis is contiguous, 16-byte pieces are aligned and no axis
-    is broadcast, else a contiguous copy."""
     if t.ndim != 3 or t.dtype != dtype or t.device != device or (d is not None and t.shape[2] != d):
         raise ValueError(f"{name} must be (rows, heads, {'d' if d is None else d}) {dtype} on {device}, not {tuple(t.shape)} {t.dtype} on {t.device}")
-    unit = 16 // t.element_size()
-    if t.stride(2) != 1 or t.stride(0) % unit or t.stride(1) % unit or t.data_ptr() % 16 or 0 in t.stride():
-        t = t.contiguous()
-        if t.data_ptr() % 16 or t.stride(2) != 1:
-            t = t.clone(memory_format=torch.contiguous_format)
-    return t
+
+
+def _cotangent(g, like):
+    """`g` as the kernels read it (autograd hands over what has the output's shape, type and device)."""
+    return _aligned(g, _UNIT[like.dtype])
 
 
 def _rows(t):
@@ -54,6 +60,23 @@ def _first(q):
     if not isinstance(q, torch.Tensor) or q.device.type != "cuda" or q.dtype not in _TYPES or q.ndim != 3:
         got = f"{tuple(q.shape)} {q.dtype} on {q.device}" if isinstance(q, torch.Tensor) else type(q).__name__
         raise ValueError(f"rows must be (n, heads, d) float32, bfloat16 or float16 on a GPU, not {got}")
+
+
+class _On:
+    """Makes a tensor's device the current one where it is not (a context object per call costs more than the launch of a kernel)."""
+    __slots__ = ("index", "back")
+
+    def __init__(self, index):
+        self.index = index
+
+    def __enter__(self):
+        self.back = torch._C._cuda_getDevice()
+        if self.back != self.index:
+            torch._C._cuda_setDevice(self.index)
+
+    def __exit__(self, *_):
+        if self.back != self.index:
+            torch._C._cuda_setDevice(self.back)
 
 
 # ------------------------------------------------------------------------------------------------------------
@@ -88,8 +111,11 @@ class PackedStructures:
             raise RuntimeError("so3lr_b200 needs a CUDA device (sm_100a); there is no CPU path")
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a PackedStructures layout cannot be made while a graph is captured")
-        self._made_on = torch.cuda.current_stream(self.device)
+        self._index = self.device.index
+        self._made_on = _raw_stream(self._index)
         self._dev = torch.from_numpy(self._image).to(self.device)
+        self._dev_ptr = self._dev.data_ptr()
+        self._calls = {}
 
     @staticmethod
     def _starts(name, x):
@@ -101,65 +127,91 @@ class PackedStructures:
             raise ValueError(f"{name} must ascend from 0 and stay below 2**31")
         return np.ascontiguousarray(x, dtype=np.int32)
 
-    def _table(self, t):
-        """The device copy, kept alive for the stream that is about to read it."""
-        s = torch.cuda.current_stream(t.device)
+    def _stream(self):
+        """The current stream, on which the layout's tables stay alive."""
+        s = _raw_stream(self._index)
         if s != self._made_on:
-            self._dev.record_stream(s)
-        return C.c_void_p(self._dev.data_ptr())
+            self._dev.record_stream(torch.cuda.current_stream(self.device))
+        return s
+
+    def _call(self, q, k, scale):
+        """What calls with rows of these shapes have in common: (shape, workspace of the forward call, of its transpose); raises where the
+        shapes do not fit."""
+        key = (q.dtype, q.shape, k.shape, scale)
+        call = self._calls.get(key)
+        if call is None:
+            (n, heads, d), (n_kv, heads_kv, _) = q.shape, k.shape
+            if d % 16 or not 16 <= d <= 128:
+                raise ValueError(f"d must be a multiple of 16 up to 128, not {d}")
+            if not heads or not heads_kv or heads % heads_kv or heads > 65535:
+                raise ValueError(f"{heads} query heads cannot share {heads_kv} key heads")
+            if n < self.rows_q or n_kv < self.rows_kv:
+                raise ValueError(f"the layout has {self.rows_q} and {self.rows_kv} rows, q {n} and k {n_kv}")
+            x = 1.0 / math.sqrt(d) if scale is None else float(scale)
+            if not (x > 0 and math.isfinite(x)):
+                raise ValueError(f"scale must be positive and finite, not {scale}")
+            shape = AttentionShape(_TYPES[q.dtype], heads, heads_kv, d, n, n_kv, x)
+            call = C.byref(shape), *(lib.so3lr_b200_structure_attention_workspace(self._host, C.byref(shape), vjp) for vjp in (0, 1))
+            if len(self._calls) >= 64:
+                self._calls.clear()
+            self._calls[key] = call
+        return call
 
 
 # ------------------------------------------------------------------------------------------------------------
 # attention
 # ------------------------------------------------------------------------------------------------------------
-def _workspace(packed, shape, vjp, device):
-    size = lib.so3lr_b200_structure_attention_workspace(packed._host, C.byref(shape), vjp)
-    return (torch.empty(size, dtype=torch.uint8, device=device), size) if size > 0 else (None, 0)
-
-
-def _attention_forward(q, k, v, packed, shape, train):
+def _attention_forward(q, k, v, packed, call, train):
     """(out, what rounding it left or None, lse or None)"""
-    with torch.cuda.device(q.device):
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        rest = torch.empty_like(out) if train and q.dtype != torch.float32 else None
-        lse = torch.empty(q.shape[1], q.shape[0], dtype=torch.float32, device=q.device) if train else None
+    shape, size, _ = call
+    with _On(packed._index):
+        out = q.new_empty(q.shape)
+        rest = q.new_empty(q.shape) if train and q.dtype != torch.float32 else None
+        lse = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32) if train else None
         if q.shape[0] > packed.rows_q:      # rows behind the last structure belong to none
             out[packed.rows_q:].zero_()
         if packed.rows_q:
-            work, size = _workspace(packed, shape, 0, q.device)
-            check(lib.so3lr_b200_structure_attention(packed._host, packed._table(q), _stream(q), C.byref(shape), C.byref(_rows(q)),
-                                                     C.byref(_rows(k)), C.byref(_rows(v)), _p(out), _p(rest), _p(lse), _p(work), size),
-                  "structure_attention")
+            work = q.new_empty(size, dtype=torch.uint8) if size > 0 else None
+            check(lib.so3lr_b200_structure_attention(packed._host, packed._dev_ptr, packed._stream(), shape, C.byref(_rows(q)), C.byref(_rows(k)),
+                                                     C.byref(_rows(v)), out.data_ptr(), _p(rest), _p(lse), _p(work), size), "structure_attention")
     return out, rest, lse
+
+
+def _attention_backward(ctx, g):
+    q, k, v, out, rest, lse = ctx.saved_tensors
+    packed, (shape, _, size) = ctx.packed, ctx.call
+    with _On(packed._index):
+        g = _cotangent(g, q)
+        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
+        if q.shape[0] > packed.rows_q:
+            dq[packed.rows_q:].zero_()
+        if k.shape[0] > packed.rows_kv:
+            dk[packed.rows_kv:].zero_()
+            dv[packed.rows_kv:].zero_()
+        if packed.rows_q or packed.rows_kv:
+            delta = torch.empty_like(lse)
+            work = q.new_empty(size, dtype=torch.uint8) if size > 0 else None
+            check(lib.so3lr_b200_structure_attention_vjp(packed._host, packed._dev_ptr, packed._stream(), shape, C.byref(_rows(q)), C.byref(_rows(k)),
+                                                         C.byref(_rows(v)), out.data_ptr(), _p(rest), lse.data_ptr(), C.byref(_rows(g)),
+                                                         delta.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _p(work), size),
+                  "structure_attention_vjp")
+    return dq, dk, dv, None, None
+
+
+_attention_backward_once = once_differentiable(_attention_backward)
 
 
 class _StructureAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, packed, shape):
-        out, rest, lse = _attention_forward(q, k, v, packed, shape, True)
+    def forward(ctx, q, k, v, packed, call):
+        out, rest, lse = _attention_forward(q, k, v, packed, call, True)
         ctx.save_for_backward(q, k, v, out, rest, lse)
-        ctx.packed, ctx.shape = packed, shape
+        ctx.packed, ctx.call = packed, call
         return out
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
-        q, k, v, out, rest, lse = ctx.saved_tensors
-        packed = ctx.packed
-        with torch.cuda.device(q.device):
-            g = _head_rows("the cotangent", g, q.dtype, q.device)
-            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
-            for t, n in ((dq, packed.rows_q), (dk, packed.rows_kv), (dv, packed.rows_kv)):
-                if t.shape[0] > n:
-                    t[n:].zero_()
-            if packed.rows_q or packed.rows_kv:
-                delta = torch.empty_like(lse)
-                work, size = _workspace(packed, ctx.shape, 1, q.device)
-                check(lib.so3lr_b200_structure_attention_vjp(packed._host, packed._table(q), _stream(q), C.byref(ctx.shape), C.byref(_rows(q)),
-                                                             C.byref(_rows(k)), C.byref(_rows(v)), _p(out), _p(rest), _p(lse), C.byref(_rows(g)),
-                                                             _p(delta), _p(dq), _p(dk), _p(dv), _p(work), size), "structure_attention_vjp")
-        return dq, dk, dv, None, None
+    def backward(ctx, g):      # differentiable once: the guard against a second time is only needed where a graph is recorded
+        return _attention_backward_once(ctx, g) if torch.is_grad_enabled() else _attention_backward(ctx, g)
 
 
 def structure_attention(q, k, v, packed, scale=None):
@@ -172,47 +224,67 @@ def structure_attention(q, k, v, packed, scale=None):
     _first(q)
     if not isinstance(packed, PackedStructures):
         raise ValueError(f"packed must be a PackedStructures layout, not {type(packed).__name__}")
-    d = q.shape[2]
-    q = _head_rows("q", q, q.dtype, q.device)
-    k, v = (_head_rows(name, t, q.dtype, q.device, d) for name, t in (("k", k), ("v", v)))
-    if packed.device != q.device:
-        raise ValueError(f"the layout is on {packed.device}, the rows on {q.device}")
+    dtype, device = q.dtype, q.device
+    if packed.device != device:
+        raise ValueError(f"the layout is on {packed.device}, the rows on {device}")
+    _head_rows("k", k, dtype, device, q.shape[2])
+    _head_rows("v", v, dtype, device)
     if k.shape != v.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
-    if d % 16 or not 16 <= d <= 128:
-        raise ValueError(f"d must be a multiple of 16 up to 128, not {d}")
-    if not q.shape[1] or not k.shape[1] or q.shape[1] % k.shape[1] or q.shape[1] > 65535:
-        raise ValueError(f"{q.shape[1]} query heads cannot share {k.shape[1]} key heads")
-    if q.shape[0] < packed.rows_q or k.shape[0] < packed.rows_kv:
-        raise ValueError(f"the layout has {packed.rows_q} and {packed.rows_kv} rows, q {q.shape[0]} and k {k.shape[0]}")
-    scale = 1.0 / math.sqrt(d) if scale is None else float(scale)
-    if not (scale > 0 and math.isfinite(scale)):
-        raise ValueError(f"scale must be positive and finite, not {scale}")
-    shape = AttentionShape(_TYPES[q.dtype], q.shape[1], k.shape[1], d, q.shape[0], k.shape[0], scale)
+    call = packed._call(q, k, scale)
+    unit = _UNIT[dtype]
+    q, k, v = _aligned(q, unit), _aligned(k, unit), _aligned(v, unit)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return _StructureAttention.apply(q, k, v, packed, shape)
-    return _attention_forward(q, k, v, packed, shape, False)[0]
+        return _StructureAttention.apply(q, k, v, packed, call)
+    return _attention_forward(q, k, v, packed, call, False)[0]
 
 
 # ------------------------------------------------------------------------------------------------------------
 # norm and rotation
 # ------------------------------------------------------------------------------------------------------------
 def _rotate_args(q, k, positions, frequencies, wq, wk, eps, neighbors):
+    n, heads, d = q.shape
     w = wq if wq is not None else wk
-    return NormRotateArgs(q.shape[0], q.shape[2], q.shape[1], 0 if k is None else k.shape[1], _TYPES[q.dtype],
-                          0 if positions is None else positions.shape[1], int(neighbors), int(w is not None),
-                          int(w is not None and w.dtype == torch.float32), int(positions is not None and positions.dtype == torch.float64), eps,
+    return NormRotateArgs(n, d, heads, 0 if k is None else k.shape[1], _TYPES[q.dtype], 0 if positions is None else positions.shape[1], neighbors,
+                          w is not None, w is not None and w.dtype == torch.float32, positions is not None and positions.dtype == torch.float64, eps,
                           _p(positions), _p(frequencies), _p(wq), _p(wk))
 
 
 def _norm_rotate_forward(q, k, positions, frequencies, wq, wk, eps, neighbors):
-    with torch.cuda.device(q.device):
-        oq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        ok = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
+    index = q.device.index
+    with _On(index):
+        oq = q.new_empty(q.shape)
+        ok = None if k is None else k.new_empty(k.shape)
         a = _rotate_args(q, k, positions, frequencies, wq, wk, eps, neighbors)
-        check(lib.so3lr_b200_norm_rotate(_stream(q), C.byref(a), C.byref(_rows(q)), None if k is None else C.byref(_rows(k)), _p(oq), _p(ok)),
-              "norm_rotate")
+        check(lib.so3lr_b200_norm_rotate(_raw_stream(index), C.byref(a), C.byref(_rows(q)), None if k is None else C.byref(_rows(k)), oq.data_ptr(),
+                                         _p(ok)), "norm_rotate")
     return oq, ok
+
+
+def _norm_rotate_backward(ctx, gq, gk):
+    q, k, positions, frequencies, wq, wk = ctx.saved_tensors
+    if gq is None and gk is None:
+        return (None,) * 8
+    index, need = q.device.index, ctx.needs_input_grad
+    with _On(index):
+        gq = _cotangent(torch.zeros_like(q) if gq is None else gq, q)
+        dq, dk, gk_rows = q.new_empty(q.shape), None, None
+        if k is not None:
+            gk = _cotangent(torch.zeros_like(k) if gk is None else gk, k)
+            dk, gk_rows = k.new_empty(k.shape), C.byref(_rows(gk))
+        dpos = torch.empty_like(positions) if positions is not None and need[2] else None
+        dwq = torch.empty_like(wq) if wq is not None and need[4] else None
+        dwk = torch.empty_like(wk) if wk is not None and need[5] else None
+        size = lib.so3lr_b200_norm_rotate_workspace(q.shape[2]) if dwq is not None or dwk is not None else 0
+        work = q.new_empty(size, dtype=torch.uint8) if size else None
+        a = _rotate_args(q, k, positions, frequencies, wq, wk, *ctx.rest)
+        check(lib.so3lr_b200_norm_rotate_vjp(_raw_stream(index), C.byref(a), C.byref(_rows(q)), None if k is None else C.byref(_rows(k)),
+                                             C.byref(_rows(gq)), gk_rows, dq.data_ptr(), _p(dk), _p(dpos), _p(dwq), _p(dwk), _p(work), size),
+              "norm_rotate_vjp")
+    return dq, dk, dpos, None, dwq, dwk, None, None
+
+
+_norm_rotate_backward_once = once_differentiable(_norm_rotate_backward)
 
 
 class _NormRotate(torch.autograd.Function):
@@ -224,27 +296,8 @@ class _NormRotate(torch.autograd.Function):
         return _norm_rotate_forward(q, k, positions, frequencies, wq, wk, eps, neighbors)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gq, gk):
-        q, k, positions, frequencies, wq, wk = ctx.saved_tensors
-        if gq is None and gk is None:
-            return (None,) * 8
-        with torch.cuda.device(q.device):
-            gq = torch.zeros_like(q) if gq is None else gq
-            gq = _head_rows("the cotangent", gq, q.dtype, q.device)
-            if k is not None:
-                gk = _head_rows("the cotangent", torch.zeros_like(k) if gk is None else gk, q.dtype, q.device)
-            dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            dk = None if k is None else torch.empty(k.shape, dtype=q.dtype, device=q.device)
-            dpos = torch.empty_like(positions) if positions is not None and ctx.needs_input_grad[2] else None
-            dwq, dwk = (torch.empty_like(w) if w is not None and n else None for w, n in ((wq, ctx.needs_input_grad[4]), (wk, ctx.needs_input_grad[5])))
-            size = lib.so3lr_b200_norm_rotate_workspace(q.shape[2]) if dwq is not None or dwk is not None else 0
-            work = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-            a = _rotate_args(q, k, positions, frequencies, wq, wk, *ctx.rest)
-            check(lib.so3lr_b200_norm_rotate_vjp(_stream(q), C.byref(a), C.byref(_rows(q)), None if k is None else C.byref(_rows(k)),
-                                                 C.byref(_rows(gq)), None if k is None else C.byref(_rows(gk)), _p(dq), _p(dk), _p(dpos), _p(dwq),
-                                                 _p(dwk), _p(work), size), "norm_rotate_vjp")
-        return dq, dk, dpos, None, dwq, dwk, None, None
+        return _norm_rotate_backward_once(ctx, gq, gk) if torch.is_grad_enabled() else _norm_rotate_backward(ctx, gq, gk)
 
 
 def norm_rotate(q, k=None, positions=None, frequencies=None, *, q_weight=None, k_weight=None, eps=1e-6, pairing="halves"):
@@ -257,12 +310,12 @@ def norm_rotate(q, k=None, positions=None, frequencies=None, *, q_weight=None, k
     k (n, heads_k, d), or None, float32, bfloat16 or float16 on one GPU, d a multiple of 16 up to 256, any strides.  Gradients: q, k, positions and the
     weights (frequencies are constants).  Returns new (q, k), contiguous."""
     _first(q)
-    d = q.shape[2]
-    q = _head_rows("q", q, q.dtype, q.device)
+    n, _, d = q.shape
+    dtype, device = q.dtype, q.device
     if k is not None:
-        k = _head_rows("k", k, q.dtype, q.device, d)
-        if k.shape[0] != q.shape[0]:
-            raise ValueError(f"q has {q.shape[0]} rows, k {k.shape[0]}")
+        _head_rows("k", k, dtype, device, d)
+        if k.shape[0] != n:
+            raise ValueError(f"q has {n} rows, k {k.shape[0]}")
     if d % 16 or not 16 <= d <= 256:
         raise ValueError(f"d must be a multiple of 16 up to 256, not {d}")
     if pairing not in ("halves", "neighbors"):
@@ -275,24 +328,28 @@ def norm_rotate(q, k=None, positions=None, frequencies=None, *, q_weight=None, k
     if norm and (q_weight is None or (k_weight is None) != (k is None)):
         raise ValueError("weights come for both sides or for neither")
     if positions is not None:
-        if positions.ndim != 2 or positions.shape[0] != q.shape[0] or not 1 <= positions.shape[1] <= 16 or positions.device != q.device or \
+        if positions.ndim != 2 or positions.shape[0] != n or not 1 <= positions.shape[1] <= 16 or positions.device != device or \
                 positions.dtype not in (torch.float32, torch.float64):
-            raise ValueError(f"positions must be ({q.shape[0]}, axes) float32 or float64 on {q.device}, not {tuple(positions.shape)} {positions.dtype} "
+            raise ValueError(f"positions must be ({n}, axes) float32 or float64 on {device}, not {tuple(positions.shape)} {positions.dtype} "
                              f"on {positions.device}")
-        if tuple(frequencies.shape) != (positions.shape[1], d // 2) or frequencies.dtype != torch.float32 or frequencies.device != q.device:
-            raise ValueError(f"frequencies must be ({positions.shape[1]}, {d // 2}) float32 on {q.device}, not {tuple(frequencies.shape)} "
+        if frequencies.shape != (positions.shape[1], d // 2) or frequencies.dtype != torch.float32 or frequencies.device != device:
+            raise ValueError(f"frequencies must be ({positions.shape[1]}, {d // 2}) float32 on {device}, not {tuple(frequencies.shape)} "
                              f"{frequencies.dtype} on {frequencies.device}")
         if frequencies.requires_grad and torch.is_grad_enabled():
             raise ValueError("frequencies are constants: no gradient is formed for them")
         positions, frequencies = positions.contiguous(), frequencies.contiguous()
-    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (tuple(w.shape) != (d,) or w.device != q.device or w.dtype not in (torch.float32, q.dtype) or w.dtype != q_weight.dtype):
-            raise ValueError(f"{name} must be ({d},) float32 or {q.dtype} on {q.device}, both sides alike, not {tuple(w.shape)} {w.dtype} on {w.device}")
-    q_weight, k_weight = (None if w is None else w.contiguous() for w in (q_weight, k_weight))
+    if norm:
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None and (w.shape != (d,) or w.device != device or w.dtype not in (torch.float32, dtype) or w.dtype != q_weight.dtype):
+                raise ValueError(f"{name} must be ({d},) float32 or {dtype} on {device}, both sides alike, not {tuple(w.shape)} {w.dtype} on {w.device}")
+        q_weight, k_weight = q_weight.contiguous(), None if k_weight is None else k_weight.contiguous()
     eps = float(eps)
-    if not (eps >= 0 and math.isfinite(eps)):
+    if not 0 <= eps < math.inf:
         raise ValueError(f"eps must not be negative, not {eps}")
+    unit = _UNIT[dtype]
+    q, k = _aligned(q, unit), None if k is None else _aligned(k, unit)
     args = (q, k, positions, frequencies, q_weight, k_weight, eps, pairing == "neighbors")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:6]):
+    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad) or (positions is not None and positions.requires_grad) or
+                                    (norm and (q_weight.requires_grad or (k_weight is not None and k_weight.requires_grad)))):
         return _NormRotate.apply(*args)
     return _norm_rotate_forward(*args)

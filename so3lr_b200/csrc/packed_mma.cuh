@@ -15,6 +15,7 @@
 // input).  float32 runs as three products of operands split into two tf32 numbers each (hi hi + hi lo + lo hi): 2^-21 of the
 // product, where a single tf32 product has 2^-11.
 #pragma once
+#include <atomic>
 #include <type_traits>
 
 #include "packed_attention.h"
@@ -596,9 +597,18 @@ __global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
   }
 }
 
-template <typename K>
-void launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, const PackedArgs& a) {
-  if (smem > 48 * 1024) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+// The attribute holds per device for good: set once (a repeated call costs a microsecond).  A lost race sets it twice.
+template <auto kernel>
+void allow_smem(int smem) {
+  static std::atomic<int> most[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev >= 64 || most[dev].load(std::memory_order_acquire) < smem) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess && dev < 64) most[dev].store(smem, std::memory_order_release);
+  }
+}
+template <auto kernel>
+void launch(dim3 grid, int threads, int smem, cudaStream_t st, const PackedArgs& a) {
+  if (smem > 48 * 1024) allow_smem<kernel>(smem);
   kernel<<<grid, threads, smem, st>>>(a);
   count_launch();
 }
@@ -614,24 +624,24 @@ void launch(K kernel, dim3 grid, int threads, int smem, cudaStream_t st, const P
 }  // namespace packed
 
 template <typename T> void packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) packed::launch(packed::forward_kernel<T, DP, false>, dim3(n_items, a.hq), 128, packed::forward_smem<T, DP>(), st, a);
+#define CALL(T, DP) packed::launch<packed::forward_kernel<T, DP, false>>(dim3(n_items, a.hq), 128, packed::forward_smem<T, DP>(), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
 template <typename T> void packed_forward_split(cudaStream_t st, const PackedArgs& a, int n_items, int n_structures, bool combine) {
 #define CALL(T, DP)                                                                                                                 \
-  packed::launch(packed::forward_kernel<T, DP, true>, dim3(n_items, a.hk), 128, packed::forward_smem<T, DP>(), st, a);              \
-  if (combine) packed::launch(packed::combine_kernel<T, DP>, dim3(n_structures, a.hk), 256, 0, st, a);
+  packed::launch<packed::forward_kernel<T, DP, true>>(dim3(n_items, a.hk), 128, packed::forward_smem<T, DP>(), st, a);              \
+  if (combine) packed::launch<packed::combine_kernel<T, DP>>(dim3(n_structures, a.hk), 256, 0, st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
 template <typename T> void packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) packed::launch(packed::dq_kernel<T, DP>, dim3(n_items, a.hq), 128, packed::reverse_smem<T, DP>(), st, a);
+#define CALL(T, DP) packed::launch<packed::dq_kernel<T, DP>>(dim3(n_items, a.hq), 128, packed::reverse_smem<T, DP>(), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
 template <typename T> void packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) packed::launch(packed::dkv_kernel<T, DP>, dim3(n_items, a.hk), 128, packed::reverse_smem<T, DP>(), st, a);
+#define CALL(T, DP) packed::launch<packed::dkv_kernel<T, DP>>(dim3(n_items, a.hk), 128, packed::reverse_smem<T, DP>(), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }

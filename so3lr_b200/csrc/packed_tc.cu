@@ -711,10 +711,10 @@ template <typename T, int TERMS, int DW> int maps_of(Maps* m, cudaStream_t st, c
   if (!reverse) m->g = m->q;
   return kOk;
 }
-template <int TERMS, int DW, typename K> int launch(K kernel, dim3 grid, bool stats, cudaStream_t st, const PackedArgs& a, const Maps& m) {
+template <int TERMS, int DW, auto kernel> int launch(dim3 grid, bool stats, cudaStream_t st, const PackedArgs& a, const Maps& m) {
   using G = Geometry<TERMS, DW>;
   const int smem = 1024 + (2 + G::ring(a.d)) * G::subs(a.d) * (int)G::kSub + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail);
-  SO3LR_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  packed::allow_smem<kernel>(smem);
   kernel<<<grid, kThreads, smem, st>>>(a, m);
   count_launch();
   return kOk;
@@ -722,7 +722,7 @@ template <int TERMS, int DW, typename K> int launch(K kernel, dim3 grid, bool st
 template <typename T, int TERMS, int DW> int forward_of(cudaStream_t st, const PackedArgs& a, int n_items, void* workspace) {
   Maps m;
   const int rc = maps_of<T, TERMS, DW>(&m, st, a, false, workspace);
-  return rc ? rc : launch<TERMS, DW>(forward_kernel<T, TERMS, DW>, dim3(n_items, a.hq), false, st, a, m);
+  return rc ? rc : launch<TERMS, DW, forward_kernel<T, TERMS, DW>>(dim3(n_items, a.hq), false, st, a, m);
 }
 template <typename T, int TERMS, int DW>
 int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, void* workspace) {
@@ -730,10 +730,10 @@ int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, cons
   int rc = maps_of<T, TERMS, DW>(&m, st, a, true, workspace);
   if (rc) return rc;
   a.items = items_q;
-  rc = launch<TERMS, DW>(dq_kernel<T, TERMS, DW>, dim3(n_q, a.hq), false, st, a, m);
+  rc = launch<TERMS, DW, dq_kernel<T, TERMS, DW>>(dim3(n_q, a.hq), false, st, a, m);
   if (rc) return rc;
   a.items = items_kv;
-  return launch<TERMS, DW>(dkv_kernel<T, TERMS, DW>, dim3(n_kv, a.hk), true, st, a, m);
+  return launch<TERMS, DW, dkv_kernel<T, TERMS, DW>>(dim3(n_kv, a.hk), true, st, a, m);
 }
 
 }  // namespace
