@@ -79,9 +79,9 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x];
+  const int4 item = a.items[blockIdx.x / a.hq];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = blockIdx.y, kvh = h / a.group, row0 = item.y * 2 * kTile, off = lk - lq;
+  const int h = blockIdx.x % a.hq, kvh = h / a.group, row0 = item.y * 2 * kTile, off = lk - lq;
   // keys that a tile meets: [0, end[t]), and tiles of keys
   const int end1 = item.w, end0 = a.causal ? min(end1, max(0, min(lq, row0 + kTile) + off)) : end1;
   const int n0 = (end0 + kTile - 1) / kTile, n1 = row0 + kTile < lq ? (end1 + kTile - 1) / kTile : 0, n = max(n0, n1);
@@ -277,9 +277,9 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x];
+  const int4 item = a.items[blockIdx.x / a.hq];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = blockIdx.y, kvh = h / a.group, row0 = item.y * kTile, off = lk - lq, n = (item.w + kTile - 1) / kTile;
+  const int h = blockIdx.x % a.hq, kvh = h / a.group, row0 = item.y * kTile, off = lk - lq, n = (item.w + kTile - 1) / kTile;
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
@@ -443,9 +443,9 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x];
+  const int4 item = a.items[blockIdx.x / a.hk];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int kvh = blockIdx.y, row0 = item.y * kTile, off = lk - lq, i0 = item.z;
+  const int kvh = blockIdx.x % a.hk, row0 = item.y * kTile, off = lk - lq, i0 = item.z;
   const int per = (max(lq - i0, 0) + kTile - 1) / kTile, n = per * a.group;
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
@@ -711,18 +711,19 @@ template <typename T, int TERMS, int DW> int maps_of(Maps* m, cudaStream_t st, c
   if (!reverse) m->g = m->q;
   return kOk;
 }
-template <int TERMS, int DW, auto kernel> int launch(dim3 grid, bool stats, cudaStream_t st, const PackedArgs& a, const Maps& m) {
+template <int TERMS, int DW, auto kernel> int launch(int64_t grid, bool stats, cudaStream_t st, const PackedArgs& a, const Maps& m) {
   using G = Geometry<TERMS, DW>;
   const int smem = 1024 + (2 + G::ring(a.d)) * G::subs(a.d) * (int)G::kSub + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail);
   packed::allow_smem<kernel>(smem);
-  kernel<<<grid, kThreads, smem, st>>>(a, m);
+  if (grid > 0x7fffffff) return kTooLarge;
+  kernel<<<(unsigned)grid, kThreads, smem, st>>>(a, m);
   count_launch();
   return kOk;
 }
 template <typename T, int TERMS, int DW> int forward_of(cudaStream_t st, const PackedArgs& a, int n_items, void* workspace) {
   Maps m;
   const int rc = maps_of<T, TERMS, DW>(&m, st, a, false, workspace);
-  return rc ? rc : launch<TERMS, DW, forward_kernel<T, TERMS, DW>>(dim3(n_items, a.hq), false, st, a, m);
+  return rc ? rc : launch<TERMS, DW, forward_kernel<T, TERMS, DW>>((int64_t)n_items * a.hq, false, st, a, m);
 }
 template <typename T, int TERMS, int DW>
 int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, void* workspace) {
@@ -730,10 +731,10 @@ int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, cons
   int rc = maps_of<T, TERMS, DW>(&m, st, a, true, workspace);
   if (rc) return rc;
   a.items = items_q;
-  rc = launch<TERMS, DW, dq_kernel<T, TERMS, DW>>(dim3(n_q, a.hq), false, st, a, m);
+  rc = launch<TERMS, DW, dq_kernel<T, TERMS, DW>>((int64_t)n_q * a.hq, false, st, a, m);
   if (rc) return rc;
   a.items = items_kv;
-  return launch<TERMS, DW, dkv_kernel<T, TERMS, DW>>(dim3(n_kv, a.hk), true, st, a, m);
+  return launch<TERMS, DW, dkv_kernel<T, TERMS, DW>>((int64_t)n_kv * a.hk, true, st, a, m);
 }
 
 }  // namespace

@@ -79,29 +79,31 @@ template <int TERMS, int DW> struct Geometry {
   static __device__ __host__ __forceinline__ int ring(int d) { return TERMS == 1 ? (d > 64 ? 4 : 8) : DW == 32 ? 6 : 2; }
   // a ring of one tile of each kind: the reverse kernels make the next logits only behind the product that reads the tile in its slot
   static constexpr bool kShort = TERMS == 3 && DW == 64;
-  // Descriptor.  K-major: 16 contracted values are 32 bytes further, 64 are a sub-tile further; groups of eight rows lie 8 rows apart.
-  // MN-major: 16 contracted rows are 16 rows further, the next values of N a sub-tile.
-  static __device__ __forceinline__ uint64_t desc(uint32_t addr, bool mn_major) {
-    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(mn_major ? kSub >> 4 : 1) << 16) | ((uint64_t)(8 * kRow >> 4) << 32) | ((uint64_t)1 << 46) |
-           ((uint64_t)(kRow == 128 ? 2 : 4) << 61);
-  }
-  static __device__ __forceinline__ uint32_t step_k(int k) { return ((k & 3) * 32 + (k >> 2) * kSub) >> 4; }
+  // Descriptor: its low word holds the address, so that steps are additions to it; the high word is a constant.  K-major: 16 contracted values
+  // are 32 bytes further, 64 are a sub-tile further; groups of eight rows lie 8 rows apart.  MN-major: 16 contracted rows are 16 rows
+  // further, the next values of N a sub-tile.
+  static constexpr uint32_t kHigh = (8 * kRow >> 4) | (1u << 14) | ((kRow == 128 ? 2u : 4u) << 29);
+  static __device__ __forceinline__ uint32_t low(uint32_t addr, bool mn_major) { return ((addr >> 4) & 0x3FFF) | ((mn_major ? kSub >> 4 : 1) << 16); }
+  static constexpr uint32_t step_k(int k) { return ((k & 3) * 32 + (k >> 2) * kSub) >> 4; }
   static constexpr uint32_t kStepMn = 16 * kRow >> 4, kStepTerm = kSub >> 4;
 };
 template <typename T> __device__ __forceinline__ uint32_t idesc(int n, bool b_mn_major) {
   const uint32_t type = std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return (1u << 4) | (type << 7) | (type << 10) | ((uint32_t)b_mn_major << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
 }
-// The whole warp runs the issue code, the elected lane (`on`) issues: descriptors stay in uniform registers.
-__device__ __forceinline__ void mma_ss(uint32_t on, uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+// The whole warp runs the issue code, the elected lane (`on`) issues: descriptors stay in uniform registers.  All loops around these are
+// unrolled: with addresses formed between two instructions a thread got one out every 120 to 170 cycles, twice what it takes to run.
+template <uint32_t HIGH> __device__ __forceinline__ void mma_ss(uint32_t on, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(id), "r"(acc), "r"(on) : "memory");
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 x, {%1, %6};\n\tmov.b64 y, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}\n" ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(acc), "r"(on), "n"(HIGH) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d, uint32_t a, uint64_t b, uint32_t id, uint32_t acc) {
+template <uint32_t HIGH> __device__ __forceinline__ void mma_ts(uint32_t on, uint32_t d, uint32_t a, uint32_t b, uint32_t id, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}\n" ::"r"(d), "r"(a), "l"(b), "r"(id), "r"(acc), "r"(on) : "memory");
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "mov.b64 y, {%2, %6};\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}\n" ::"r"(d), "r"(a), "r"(b), "r"(id), "r"(acc), "r"(on), "n"(HIGH) : "memory");
 }
 __device__ __forceinline__ void commit(uint32_t on, uint32_t bar) {
   asm volatile(
@@ -111,18 +113,19 @@ __device__ __forceinline__ void commit(uint32_t on, uint32_t bar) {
 // D[128 x 128] = A B^T over d columns, both tiles in shared memory
 template <typename T, int TERMS, int DW> __device__ __forceinline__ void product_rows(uint32_t on, uint32_t dst, uint32_t a, uint32_t b, int d) {
   using G = Geometry<TERMS, DW>;
-  const uint64_t da = G::desc(a, false), db = G::desc(b, false);
-  const uint32_t id = idesc<T>(kTile, false);
+  const uint32_t la = G::low(a, false), lb = G::low(b, false), id = idesc<T>(kTile, false);
   if constexpr (TERMS == 1) {
-#pragma unroll 1
-    for (int k = 0; k < d / 16; ++k) mma_ss(on, dst, da + G::step_k(k), db + G::step_k(k), id, k > 0);
+    const int steps = d / 16;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < steps) mma_ss<G::kHigh>(on, dst, la + G::step_k(k), lb + G::step_k(k), id, k > 0);
   } else {
-#pragma unroll 1
+#pragma unroll
     for (int e = 0; e < 6; ++e) {
       // (2, 0), (0, 2), (1, 1), (1, 0), (0, 1), (0, 0)
       const uint32_t x = e == 0 ? 2 : (e == 2 || e == 3), y = e == 1 ? 2 : (e == 2 || e == 4);
-      const uint64_t ax = da + x * G::kStepTerm, by = db + y * G::kStepTerm;
-      for (int k = 0; k < DW / 16; ++k) mma_ss(on, dst, ax + G::step_k(k), by + G::step_k(k), id, (e | k) > 0);
+#pragma unroll
+      for (int k = 0; k < DW / 16; ++k) mma_ss<G::kHigh>(on, dst, la + x * G::kStepTerm + G::step_k(k), lb + y * G::kStepTerm + G::step_k(k), id, (e | k) > 0);
     }
   }
 }
@@ -130,28 +133,28 @@ template <typename T, int TERMS, int DW> __device__ __forceinline__ void product
 struct Packed { uint32_t at[3]; int gap[3]; };
 // D[128 x d] (+)= A B: A in tensor memory, B a tile with its rows contracted.  Three terms and DW = 32: two terms of B side by side as N = 64,
 // D = [.. t0 | .. t1 and t2], whose halves are to be added; started afresh every time.
-template <typename T, int TERMS, int DW> __device__ __forceinline__ void product_cols(uint32_t on, uint32_t dst, const Packed& a, uint32_t b, int d, uint32_t acc) {
+template <typename T, int TERMS, int DW> __device__ __forceinline__ void product_cols(uint32_t on, uint32_t dst, const Packed a, uint32_t b, int d, uint32_t acc) {
   using G = Geometry<TERMS, DW>;
-  const uint64_t db = G::desc(b, true);
-  auto steps = [&](int term, uint64_t bt, uint32_t to, int n, uint32_t add) {
+  const uint32_t lb = G::low(b, true);
+  auto steps = [&](int term, uint32_t bt, uint32_t to, int n, uint32_t add) {
     const uint32_t id = idesc<T>(n, true);
-#pragma unroll 1
-    for (int k = 0; k < 8; ++k) mma_ts(on, to, a.at[term] + (k & 3) * 8 + (k >> 2) * a.gap[term], bt + k * G::kStepMn, id, add | (k > 0));
+#pragma unroll
+    for (int k = 0; k < 8; ++k) mma_ts<G::kHigh>(on, to, a.at[term] + (k & 3) * 8 + (k >> 2) * a.gap[term], bt + k * G::kStepMn, id, add | (k > 0));
   };
   if constexpr (TERMS == 1) {
-    steps(0, db, dst, d, acc);
+    steps(0, lb, dst, d, acc);
   } else if constexpr (DW == 32) {
-    steps(2, db, dst, 32, 0);
-    steps(0, db + 2 * G::kStepTerm, dst + 32, 32, 0);
-    steps(1, db, dst, 64, 1);
-    steps(0, db, dst, 64, 1);
+    steps(2, lb, dst, 32, 0);
+    steps(0, lb + 2 * G::kStepTerm, dst + 32, 32, 0);
+    steps(1, lb, dst, 64, 1);
+    steps(0, lb, dst, 64, 1);
   } else {
-    steps(2, db, dst, 64, 0);
-    steps(0, db + 2 * G::kStepTerm, dst, 64, 1);
-    steps(1, db + G::kStepTerm, dst, 64, 1);
-    steps(1, db, dst, 64, 1);
-    steps(0, db + G::kStepTerm, dst, 64, 1);
-    steps(0, db, dst, 64, 1);
+    steps(2, lb, dst, 64, 0);
+    steps(0, lb + 2 * G::kStepTerm, dst, 64, 1);
+    steps(1, lb + G::kStepTerm, dst, 64, 1);
+    steps(1, lb, dst, 64, 1);
+    steps(0, lb + G::kStepTerm, dst, 64, 1);
+    steps(0, lb, dst, 64, 1);
   }
 }
 
