@@ -65,7 +65,7 @@ __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* p) { retur
 // terms of P from there on, its output at 256 t + 192.)
 // The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
 // the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
-enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kSFull = kQFull + 2, kPFull = kSFull + 2, kOFull = kPFull + 2, kFix = kOFull + 2, kFwdBars };
+enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kSFull = kQFull + 2, kPFull = kSFull + 2 /* tile + 2 half */, kOFull = kPFull + 4, kFix = kOFull + 2, kFwdBars };
 
 template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
-    for (int i = 0; i < kFwdBars; ++i) init_bar(bar(i), i == kPFull || i == kPFull + 1 ? kTile : 1);
+    for (int i = 0; i < kFwdBars; ++i) init_bar(bar(i), i >= kPFull && i < kPFull + 4 ? kTile : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
@@ -126,7 +126,15 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
           wait_bar(bar(kPFull + t), i & 1, failed, &g_packed_error);
           fence_after();
           const uint32_t at = tmem + kStride * t;
-          product_cols<M, TERMS, DW>(on, at + kOut, Packed{{at, at + 64, at + 128}, {32, 32, 32}}, slot(2 * i + 1), d, i > 0);
+          const Packed p{{at, at + 64, at + 128}, {32, 32, 32}};
+          if constexpr (TERMS == 1) {      // the first half of the keys while the exponentials of the second are formed
+            product_cols<M, TERMS, DW, 0, 4>(on, at + kOut, p, slot(2 * i + 1), d, i > 0);
+            wait_bar(bar(kPFull + 2 + t), i & 1, failed, &g_packed_error);
+            fence_after();
+            product_cols<M, TERMS, DW, 4, 8>(on, at + kOut, p, slot(2 * i + 1), d, 1);
+          } else {
+            product_cols<M, TERMS, DW>(on, at + kOut, p, slot(2 * i + 1), d, 0);
+          }
           if (i + 1 < nt) {
             product_rows<M, TERMS, DW>(on, at, sq + t * tile_bytes, slot(2 * i + 2), d);
             commit(on, bar(kSFull + t));
@@ -168,17 +176,18 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       for (int c = 0; c < kTile; c += 32) ld32(ts + c, x + c);
       wait_ld(x);
       const int kb = i * kTile;
-      if (kb + kTile - 1 > lim_first) {
+      const bool masked = kb + kTile - 1 > lim_first;
+      if (masked) {
 #pragma unroll
         for (int c = 0; c < kTile; ++c) if (kb + c > lim) x[c] = 0xff800000u;
       }
-      float m0 = -INFINITY, m1 = -INFINITY, m2 = -INFINITY, m3 = -INFINITY;
+      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < kTile; c += 4) {
-        m0 = fmaxf(m0, __uint_as_float(x[c])); m1 = fmaxf(m1, __uint_as_float(x[c + 1]));
-        m2 = fmaxf(m2, __uint_as_float(x[c + 2])); m3 = fmaxf(m3, __uint_as_float(x[c + 3]));
+      for (int c = 0; c < kTile; c += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
       }
-      const float mn = fmaxf(m, fmaxf(fmaxf(m0, m1), fmaxf(m2, m3)) * a.scale_log2);
+      const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2);
       const bool raise = mn > m + 8.f;      // true where there was none yet
       if (__any_sync(0xffffffffu, raise)) {
         const float f = raise ? pow2(m - mn) : 1.f;
@@ -199,22 +208,32 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
         }
       }
       const float u = m == -INFINITY ? 0.f : -m;
-      float l0 = 0.f, l1 = 0.f;
+      float2 sums[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sums[e] = make_float2(0.f, 0.f);
       const Packed at{{0, 64, 128}, {}};
+      const float2 scale = make_float2(a.scale_log2, a.scale_log2), ref = make_float2(u, u);
 #pragma unroll
-      for (int c = 0; c < kTile; c += 16) {
-        float y[16];
+      for (int c = 0; c < kTile; c += 32) {
+        float y[32];
+        // a masked logit has to give zero, which the polynomial does not
+        if (TERMS == 1 && !masked) { pow2_16<true>(x + c, scale, ref, y); pow2_16<true>(x + c + 16, scale, ref, y + 16); }
+        else { pow2_16<false>(x + c, scale, ref, y); pow2_16<false>(x + c + 16, scale, ref, y + 16); }
 #pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-          y[e] = pow2(fmaf(__uint_as_float(x[c + e]), a.scale_log2, u)); y[e + 1] = pow2(fmaf(__uint_as_float(x[c + e + 1]), a.scale_log2, u));
-          l0 += y[e]; l1 += y[e + 1];
-        }
+        for (int e = 0; e < 32; e += 2) sums[(e >> 1) & 3] = __fadd2_rn(sums[(e >> 1) & 3], make_float2(y[e], y[e + 1]));
         put16<M, TERMS>(at, ts, c, y);
+        put16<M, TERMS>(at, ts, c + 16, y + 16);
+        if (TERMS == 1 && c == kTile / 2 - 32) {
+          wait_st();
+          fence_before();
+          arrive(bar(kPFull + t));
+        }
       }
-      l += l0 + l1;
+      const float2 sum = __fadd2_rn(__fadd2_rn(sums[0], sums[1]), __fadd2_rn(sums[2], sums[3]));
+      l += sum.x + sum.y;
       wait_st();
       fence_before();
-      arrive(bar(kPFull + t));
+      arrive(bar(kPFull + t + (TERMS == 1 ? 2 : 0)));
     }
     if (nt > 0) {
       wait_bar(bar(kOFull + t), 0, failed, &g_packed_error);
@@ -357,6 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
 #pragma unroll
     for (int c = 0; c < kOwn; ++c) own[c] = 0.f;
     const Packed to{{kTile + (uint32_t)col, kTile + 32 + (uint32_t)col, 256 + (uint32_t)col / 2}, {}};
+    const float2 scale = make_float2(a.scale_log2, a.scale_log2), ref = make_float2(e, e);
     for (int i = 0; i < n; ++i) {
       uint32_t x[64], y[64];
       wait_bar(bar(kdqS), i & 1, failed, &g_packed_error);
@@ -367,7 +387,12 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       fence_before();
       arrive(bar(kdqSRead));
 #pragma unroll
-      for (int c = 0; c < 64; ++c) x[c] = __float_as_uint(pow2(fmaf(__uint_as_float(x[c]), a.scale_log2, e)));
+      for (int c = 0; c < 64; c += 16) {
+        float v[16];
+        pow2_16<TERMS == 1>(x + c, scale, ref, v);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[c + k] = __float_as_uint(v[k]);
+      }
       const int kb = i * kTile + col;
       wait_bar(bar(kdqDp), i & 1, failed, &g_packed_error);
       fence_after();
@@ -535,6 +560,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
     float own[2][kOwn];                      // dv, dk so far (float32), half of the row
 #pragma unroll
     for (int c = 0; c < kOwn; ++c) own[0][c] = own[1][c] = 0.f;
+    const float2 scale = make_float2(a.scale_log2, a.scale_log2);
     const Packed to_p{{(uint32_t)col, 32 + (uint32_t)col, 256 + (uint32_t)col / 2}, {}},
         to_s{{kTile + (uint32_t)col, kTile + 32 + (uint32_t)col, 320 + (uint32_t)col / 2}, {}};
     for (int i = 0; i < n; ++i) {
@@ -551,10 +577,11 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
 #pragma unroll
       for (int c = 0; c < 16; ++c) {
         const float4 v = e[c];
-        x[4 * c] = __float_as_uint(pow2(fmaf(__uint_as_float(x[4 * c]), a.scale_log2, v.x)));
-        x[4 * c + 1] = __float_as_uint(pow2(fmaf(__uint_as_float(x[4 * c + 1]), a.scale_log2, v.y)));
-        x[4 * c + 2] = __float_as_uint(pow2(fmaf(__uint_as_float(x[4 * c + 2]), a.scale_log2, v.z)));
-        x[4 * c + 3] = __float_as_uint(pow2(fmaf(__uint_as_float(x[4 * c + 3]), a.scale_log2, v.w)));
+        const float2 z0 = __ffma2_rn(make_float2(__uint_as_float(x[4 * c]), __uint_as_float(x[4 * c + 1])), scale, make_float2(v.x, v.y));
+        const float2 z1 = __ffma2_rn(make_float2(__uint_as_float(x[4 * c + 2]), __uint_as_float(x[4 * c + 3])), scale, make_float2(v.z, v.w));
+        const float2 r1 = TERMS == 1 && (c & 1) ? pow2_poly(z1) : make_float2(pow2(z1.x), pow2(z1.y));
+        x[4 * c] = __float_as_uint(pow2(z0.x)); x[4 * c + 1] = __float_as_uint(pow2(z0.y));
+        x[4 * c + 2] = __float_as_uint(r1.x); x[4 * c + 3] = __float_as_uint(r1.y);
       }
       if (a.causal && ib < lim_last) {
 #pragma unroll
@@ -688,6 +715,11 @@ bool map_of(CUtensorMap* m, bool bf16, const Rows& r, long long rows, int heads,
 }
 template <typename T, int TERMS, int DW> int maps_of(Maps* m, cudaStream_t st, const PackedArgs& a, bool reverse, void* workspace) {
   if (!encoder()) return kCudaError;
+  // Encoding a map goes to the driver, which wants the device's context current on this thread; the runtime makes it so at a thread's first
+  // call that needs it, and autograd's threads may come here first.
+  int device = 0;
+  SO3LR_CUDA_CHECK(cudaGetDevice(&device));
+  SO3LR_CUDA_CHECK(cudaSetDevice(device));
   CUtensorMap* maps[4] = {&m->q, &m->k, &m->v, &m->g};
   const Rows rows[4] = {a.q, a.k, a.v, a.g};
   const int n[4] = {a.nq, a.nkv, a.nkv, a.nq}, heads[4] = {a.hq, a.hk, a.hk, a.hq}, operands = reverse ? 4 : 3;

@@ -67,6 +67,35 @@ __device__ __forceinline__ float pow2(float x) {
   return y;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// 2^x of a pair without the special function unit, which gives 16 results a cycle and is as busy as the tensor cores: x = n + f with n the
+// nearest integer (found by adding 1.5 2^23), 2^f by the polynomial of degree 4 with the least relative error on [-1/2, 1/2] (2.6e-6, a
+// hundredth of a 16-bit rounding; fitted by reweighted least squares), n added to its exponent.  Not below 2^-126.
+__device__ __forceinline__ float2 pow2_poly(float2 x) {
+  const float2 magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);
+  x.x = fmaxf(x.x, -126.f); x.y = fmaxf(x.y, -126.f);
+  const float2 t = __fadd2_rn(x, magic), n = __fadd2_rn(t, minus), f = __fadd2_rn(x, make_float2(-n.x, -n.y));
+  float2 p = make_float2(0.009570102207362652f, 0.009570102207362652f);
+  p = __ffma2_rn(p, f, make_float2(0.05591786280274391f, 0.05591786280274391f));
+  p = __ffma2_rn(p, f, make_float2(0.240247443318367f, 0.240247443318367f));
+  p = __ffma2_rn(p, f, make_float2(0.6931217908859253f, 0.6931217908859253f));
+  p = __ffma2_rn(p, f, make_float2(0.9999992847442627f, 0.9999992847442627f));
+  return make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + __float_as_uint(p.x)), __uint_as_float((__float_as_uint(t.y) << 23) + __float_as_uint(p.y)));
+}
+// 2^(a x + b) of sixteen values; POLY: a quarter of them by the polynomial
+template <bool POLY> __device__ __forceinline__ void pow2_16(const uint32_t* x, float2 a, float2 b, float* y) {
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) {
+    const float2 z = __ffma2_rn(make_float2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), a, b);
+    const float2 r = POLY && (e & 7) == 6 ? pow2_poly(z) : make_float2(pow2(z.x), pow2(z.y));
+    y[e] = r.x; y[e + 1] = r.y;
+  }
+}
+
 // ---- matrix instructions ----
 // Geometry of operand tiles.  TERMS = 1: 16-bit values, sub-tiles of 64 values (128-byte rows and swizzle), one or two.  TERMS = 3: float32
 // values split into three bfloat16 terms, x = t0 + t1 + t2 to 2^-24, a sub-tile per term of DW = 32 or 64 values (64- or 128-byte rows and
@@ -133,13 +162,16 @@ template <typename T, int TERMS, int DW> __device__ __forceinline__ void product
 struct Packed { uint32_t at[3]; int gap[3]; };
 // D[128 x d] (+)= A B: A in tensor memory, B a tile with its rows contracted.  Three terms and DW = 32: two terms of B side by side as N = 64,
 // D = [.. t0 | .. t1 and t2], whose halves are to be added; started afresh every time.
-template <typename T, int TERMS, int DW> __device__ __forceinline__ void product_cols(uint32_t on, uint32_t dst, const Packed a, uint32_t b, int d, uint32_t acc) {
+// FIRST, LAST: 16ths of the contracted index, [0, 8) for all.
+template <typename T, int TERMS, int DW, int FIRST = 0, int LAST = 8>
+__device__ __forceinline__ void product_cols(uint32_t on, uint32_t dst, const Packed a, uint32_t b, int d, uint32_t acc) {
   using G = Geometry<TERMS, DW>;
+  static_assert(TERMS == 1 || LAST - FIRST == 8, "three terms take the whole index at once");
   const uint32_t lb = G::low(b, true);
   auto steps = [&](int term, uint32_t bt, uint32_t to, int n, uint32_t add) {
     const uint32_t id = idesc<T>(n, true);
 #pragma unroll
-    for (int k = 0; k < 8; ++k) mma_ts<G::kHigh>(on, to, a.at[term] + (k & 3) * 8 + (k >> 2) * a.gap[term], bt + k * G::kStepMn, id, add | (k > 0));
+    for (int k = FIRST; k < LAST; ++k) mma_ts<G::kHigh>(on, to, a.at[term] + (k & 3) * 8 + (k >> 2) * a.gap[term], bt + k * G::kStepMn, id, add | (k > 0));
   };
   if constexpr (TERMS == 1) {
     steps(0, lb, dst, d, acc);
