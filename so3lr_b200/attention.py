@@ -24,6 +24,7 @@ from ._lib import AttentionShape, NormRotateArgs, Rows, check, lib
 
 _TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _UNIT = {torch.float32: 4, torch.bfloat16: 8, torch.float16: 8}      # values of 16 bytes
+_CONTIGUOUS = torch.contiguous_format
 _raw_stream = torch._C._cuda_getCurrentRawStream                     # of a device ordinal: torch.cuda.current_stream(..).cuda_stream without its object
 
 
@@ -165,8 +166,8 @@ def _attention_forward(q, k, v, packed, call, train):
     """(out, what rounding it left or None, lse or None)"""
     shape, size, _ = call
     with _On(packed._index):
-        out = q.new_empty(q.shape)
-        rest = q.new_empty(q.shape) if train and q.dtype != torch.float32 else None
+        out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+        rest = torch.empty_like(q, memory_format=_CONTIGUOUS) if train and q.dtype != torch.float32 else None
         lse = q.new_empty((q.shape[1], q.shape[0]), dtype=torch.float32) if train else None
         if q.shape[0] > packed.rows_q:      # rows behind the last structure belong to none
             out[packed.rows_q:].zero_()
@@ -182,7 +183,7 @@ def _attention_backward(ctx, g):
     packed, (shape, _, size) = ctx.packed, ctx.call
     with _On(packed._index):
         g = _cotangent(g, q)
-        dq, dk, dv = q.new_empty(q.shape), k.new_empty(k.shape), k.new_empty(k.shape)
+        dq, dk, dv = torch.empty_like(q, memory_format=_CONTIGUOUS), torch.empty_like(k, memory_format=_CONTIGUOUS), torch.empty_like(k, memory_format=_CONTIGUOUS)
         if q.shape[0] > packed.rows_q:
             dq[packed.rows_q:].zero_()
         if k.shape[0] > packed.rows_kv:
@@ -253,8 +254,8 @@ def _rotate_args(q, k, positions, frequencies, wq, wk, eps, neighbors):
 def _norm_rotate_forward(q, k, positions, frequencies, wq, wk, eps, neighbors):
     index = q.device.index
     with _On(index):
-        oq = q.new_empty(q.shape)
-        ok = None if k is None else k.new_empty(k.shape)
+        oq = torch.empty_like(q, memory_format=_CONTIGUOUS)
+        ok = None if k is None else torch.empty_like(k, memory_format=_CONTIGUOUS)
         a = _rotate_args(q, k, positions, frequencies, wq, wk, eps, neighbors)
         check(lib.so3lr_b200_norm_rotate(_raw_stream(index), C.byref(a), C.byref(_rows(q)), None if k is None else C.byref(_rows(k)), oq.data_ptr(),
                                          _p(ok)), "norm_rotate")
@@ -268,10 +269,10 @@ def _norm_rotate_backward(ctx, gq, gk):
     index, need = q.device.index, ctx.needs_input_grad
     with _On(index):
         gq = _cotangent(torch.zeros_like(q) if gq is None else gq, q)
-        dq, dk, gk_rows = q.new_empty(q.shape), None, None
+        dq, dk, gk_rows = torch.empty_like(q, memory_format=_CONTIGUOUS), None, None
         if k is not None:
             gk = _cotangent(torch.zeros_like(k) if gk is None else gk, k)
-            dk, gk_rows = k.new_empty(k.shape), C.byref(_rows(gk))
+            dk, gk_rows = torch.empty_like(k, memory_format=_CONTIGUOUS), C.byref(_rows(gk))
         dpos = torch.empty_like(positions) if positions is not None and need[2] else None
         dwq = torch.empty_like(wq) if wq is not None and need[4] else None
         dwk = torch.empty_like(wk) if wk is not None and need[5] else None

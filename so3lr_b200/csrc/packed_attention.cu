@@ -154,28 +154,26 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
     p.part_rows = im[kMaxQ] * p.group;
     p.part_o = static_cast<float*>(workspace);
     p.part_ml = reinterpret_cast<float2*>(p.part_o + part_floats(im, a));
-    packed_forward_split<T>(st, p, im[kNItemsSplit], im[kN], im[kCombine]);
-    return kOk;
+    return packed_forward_split<T>(st, p, im[kNItemsSplit], im[kN], im[kCombine]);
   }
   if (on_tensor_cores(im, a)) {
     p.items = table(im, dev, kItemsQ256);
     return packed_forward_tc<T>(st, p, im[kNItemsQ256], workspace);
   }
   p.items = table(im, dev, kItemsQ);
-  packed_forward_mma<T>(st, p, im[kNItemsQ]);
-  return kOk;
+  return packed_forward_mma<T>(st, p, im[kNItemsQ]);
 }
 
 template <typename T>
 int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
-  packed_delta<T>(st, p, im[kRowsQ]);
+  int rc = packed_delta<T>(st, p, im[kRowsQ]);
+  if (rc) return rc;
   if (on_tensor_cores(im, a))
     return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128], workspace);
   p.items = table(im, dev, kItemsQ);
-  if (im[kNItemsQ]) packed_dq_mma<T>(st, p, im[kNItemsQ]);
+  if (im[kNItemsQ]) rc = packed_dq_mma<T>(st, p, im[kNItemsQ]);
   p.items = table(im, dev, kItemsKv);
-  if (im[kNItemsKv]) packed_dkv_mma<T>(st, p, im[kNItemsKv]);
-  return kOk;
+  return rc || !im[kNItemsKv] ? rc : packed_dkv_mma<T>(st, p, im[kNItemsKv]);
 }
 
 }  // namespace

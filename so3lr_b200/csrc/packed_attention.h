@@ -42,11 +42,11 @@ struct PackedArgs {
 constexpr int kPackTile = 64;   // rows of a tile of the mma kernels
 
 // kernels on the warp-level matrix instructions, one translation unit per type
-template <typename T> void packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items);
-template <typename T> void packed_forward_split(cudaStream_t st, const PackedArgs& a, int n_items, int n_structures, bool combine);
-template <typename T> void packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items);
-template <typename T> void packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items);
-template <typename T> void packed_delta(cudaStream_t st, const PackedArgs& a, int rows);
+template <typename T> int packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> int packed_forward_split(cudaStream_t st, const PackedArgs& a, int n_items, int n_structures, bool combine);
+template <typename T> int packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> int packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items);
+template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, int rows);
 
 // Kernels on the tensor cores: tiles of 128 rows, two of them side by side in the forward kernel.  float32 (d <= 64) runs on operands that
 // are split into three bfloat16 terms ahead (packed_split_bytes of workspace).

@@ -261,9 +261,10 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const uint32_t sq = smem_addr(smem), sk = sq + kPackTile * L::kStride, sv = sk + 2 * BN * L::kStride;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x];
+  const int heads = SPLIT ? a.hk : a.hq, unit = blockIdx.x / heads;
+  const int4 item = a.items[unit];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int G = SPLIT ? a.group : 1, hy = blockIdx.y, kvh = SPLIT ? hy : hy / a.group;
+  const int G = SPLIT ? a.group : 1, hy = blockIdx.x % heads, kvh = SPLIT ? hy : hy / a.group;
   const int rows = lq * G, row0 = SPLIT ? 0 : item.y * kPackTile;
   const int k0 = item.z, k1 = item.w;
   const int nt = (max(k1 - k0, 0) + BN - 1) / BN;
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
     if (pr >= rows) continue;
     const float m = half ? mb : ma, l = half ? lb : la;
     if (SPLIT && item.y > 1) {
-      const size_t slot = ((size_t)blockIdx.x * a.hk + hy) * a.part_rows + pr;
+      const size_t slot = ((size_t)unit * a.hk + hy) * a.part_rows + pr;
       float* dst = a.part_o + slot * DP + 2 * (lane & 3);
 #pragma unroll
       for (int n = 0; n < DP / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
@@ -370,10 +371,149 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
   }
 }
 
+// The split form for up to 16 rows (a new token of a few heads): bound by the keys and values that go by, so every warp streams its own 16 of
+// 64 keys through buffers of its own, without a barrier of the CTA, and the four partial results meet at the end.
+constexpr int kNarrowRows = 16;
+template <typename T, int DP> constexpr int narrow_stages() { return sizeof(T) == 4 && DP > 64 ? 2 : 3; }
+template <typename T, int DP> constexpr int narrow_smem() { return (kNarrowRows + 4 * narrow_stages<T, DP>() * 32) * Tile<T, DP>::kStride; }
+template <typename T, int DP>
+__global__ void __launch_bounds__(128) narrow_kernel(const PackedArgs a) {
+  using L = Tile<T, DP>;
+  constexpr int ST = narrow_stages<T, DP>();
+  extern __shared__ __align__(16) unsigned char smem[];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const uint32_t sq = smem_addr(smem), sk = sq + (kNarrowRows + warp * ST * 32) * L::kStride;      // stages of 16 keys, then 16 values
+  const int4 item = a.items[blockIdx.x / a.hk];
+  const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
+  const int G = a.group, hy = blockIdx.x % a.hk, rows = lq * G, k0 = item.z + warp * 16, k1 = item.w;
+  const int nt = k1 > k0 ? (k1 - k0 + 63) / 64 : 0;
+  const T *kp = static_cast<const T*>(a.k.p) + hy * a.k.head, *vp = static_cast<const T*>(a.v.p) + hy * a.v.head;
+  auto load = [&](int it) {
+    if (it < nt) {
+      const uint32_t at = sk + (it % ST) * 32 * L::kStride;
+      const int b = k0 + it * 64;
+#pragma unroll
+      for (int i = lane; i < 16 * L::kChunks; i += 32) {
+        const int r = i / L::kChunks, c = i % L::kChunks;
+        const bool ok = b + r < k1 && c * L::kPer < a.d;
+        copy16(at + r * L::kStride + c * 16, ok ? kp + (long long)(c0 + b + r) * a.k.row + c * L::kPer : kp, ok);
+        copy16(at + (16 + r) * L::kStride + c * 16, ok ? vp + (long long)(c0 + b + r) * a.v.row + c * L::kPer : vp, ok);
+      }
+    }
+    copy_commit();
+  };
+#pragma unroll
+  for (int it = 0; it < ST - 1; ++it) load(it);
+  {  // queries, with the first group of every warp's copies waited for below
+    const T* p = static_cast<const T*>(a.q.p);
+    for (int i = tid; i < kNarrowRows * L::kChunks; i += 128) {
+      const int r = i / L::kChunks, c = i % L::kChunks;
+      const bool ok = r < rows && c * L::kPer < a.d;
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (ok) v = *reinterpret_cast<const uint4*>(p + (long long)(q0 + r / G) * a.q.row + (hy * G + r % G) * a.q.head + c * L::kPer);
+      *reinterpret_cast<uint4*>(smem + r * L::kStride + c * 16) = v;
+    }
+  }
+  __syncthreads();
+  const int ra = lane >> 2, rb = ra + 8, off = lk - lq, big = 0x7fffffff;
+  const int lim_a = a.causal ? ra / G + off : big, lim_b = a.causal ? rb / G + off : big, lim_lo = a.causal ? off : big;
+  float o[DP / 8][4];
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+  for (int it = 0; it < nt; ++it) {
+    load(it + ST - 1);
+    copy_wait<ST - 1>();
+    __syncwarp();
+    const int kb = k0 + it * 64;
+    const uint32_t at = sk + (it % ST) * 32 * L::kStride;
+    float p[2][4];
+    product_nt<T, DP, 2>(p, sq, at, lane, 16);
+    if (kb + 16 > k1 || kb + 15 > lim_lo) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = kb + n * 8 + 2 * (lane & 3) + e;
+          if (j >= k1 || j > lim_a) p[n][e] = -INFINITY;
+          if (j >= k1 || j > lim_b) p[n][2 + e] = -INFINITY;
+        }
+      }
+    }
+    float xa = fmaxf(fmaxf(p[0][0], p[0][1]), fmaxf(p[1][0], p[1][1])), xb = fmaxf(fmaxf(p[0][2], p[0][3]), fmaxf(p[1][2], p[1][3]));
+#pragma unroll
+    for (int x = 1; x < 4; x <<= 1) { xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, x)); xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, x)); }
+    const float na = fmaxf(ma, xa * a.scale_log2), nb = fmaxf(mb, xb * a.scale_log2);
+    const float ua = na == -INFINITY ? 0.f : na, ub = nb == -INFINITY ? 0.f : nb;
+    const float fa = exp2f(ma - ua), fb = exp2f(mb - ub);
+    ma = na; mb = nb;
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+      p[n][0] = exp2f(fmaf(p[n][0], a.scale_log2, -ua)); p[n][1] = exp2f(fmaf(p[n][1], a.scale_log2, -ua));
+      p[n][2] = exp2f(fmaf(p[n][2], a.scale_log2, -ub)); p[n][3] = exp2f(fmaf(p[n][3], a.scale_log2, -ub));
+    }
+    la = fmaf(la, fa, p[0][0] + p[0][1] + p[1][0] + p[1][1]);
+    lb = fmaf(lb, fb, p[0][2] + p[0][3] + p[1][2] + p[1][3]);
+    if (__any_sync(0xffffffffu, fa != 1.f || fb != 1.f)) {
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) { o[n][0] *= fa; o[n][1] *= fa; o[n][2] *= fb; o[n][3] *= fb; }
+    }
+    product_nn<T, DP, 2>(o, p, at + 16 * L::kStride, lane, 16);
+    __syncwarp();
+  }
+  copy_wait<0>();
+#pragma unroll
+  for (int x = 1; x < 4; x <<= 1) { la += __shfl_xor_sync(0xffffffffu, la, x); lb += __shfl_xor_sync(0xffffffffu, lb, x); }
+  // the four warps' shares: (m, l) and o of every row in shared memory, over the buffers
+  __syncthreads();
+  float* so = reinterpret_cast<float*>(smem);                       // [4][16][DP + 2]
+  constexpr int W = DP + 2;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    float* dst = so + (warp * kNarrowRows + (half ? rb : ra)) * W;
+#pragma unroll
+    for (int n = 0; n < DP / 8; ++n) *reinterpret_cast<float2*>(dst + n * 8 + 2 * (lane & 3)) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+    if ((lane & 3) == 0) *reinterpret_cast<float2*>(dst + DP) = make_float2(half ? mb : ma, half ? lb : la);
+  }
+  __syncthreads();
+  for (int r = warp; r < rows; r += 4) {
+    float m = -INFINITY, l = 0.f, f[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) m = fmaxf(m, so[(w * kNarrowRows + r) * W + DP]);
+    const float u = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      f[w] = exp2f(so[(w * kNarrowRows + r) * W + DP] - u);
+      l = fmaf(so[(w * kNarrowRows + r) * W + DP + 1], f[w], l);
+    }
+    const size_t slot = ((size_t)(blockIdx.x / a.hk) * a.hk + hy) * a.part_rows + r;
+    const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+    const long long to = ((long long)(q0 + r / G) * a.hq + hy * G + r % G) * a.d;
+#pragma unroll
+    for (int c = lane; c < DP; c += 32) {
+      float x = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) x = fmaf(so[(w * kNarrowRows + r) * W + c], f[w], x);
+      if (item.y > 1) {
+        a.part_o[slot * DP + c] = x;
+      } else if (c < a.d) {
+        x *= inv;
+        const T y = (T)x;
+        static_cast<T*>(a.out)[to + c] = y;
+        if (sizeof(T) == 2 && a.out_rest) static_cast<T*>(a.out_rest)[to + c] = (T)(x - (float)y);
+      }
+    }
+    if (lane == 0) {
+      if (item.y > 1) a.part_ml[slot] = make_float2(m, l);
+      else if (a.lse) a.lse[(long long)(hy * G + r % G) * a.nq + q0 + r / G] = l == 0.f ? -INFINITY : m + log2f(l);
+    }
+  }
+}
+
 // joins the stretches of a structure's keys: a warp per row of the split form
 template <typename T, int DP>
 __global__ void __launch_bounds__(256) combine_kernel(const PackedArgs a) {
-  const int s = blockIdx.x, hy = blockIdx.y, lane = threadIdx.x & 31;
+  const int s = blockIdx.x / a.hk, hy = blockIdx.x % a.hk, lane = threadIdx.x & 31;
   const int first = a.split_first[s], n = a.split_first[s + 1] - first;
   const int q0 = a.start_q[s], rows = (a.start_q[s + 1] - q0) * a.group;
   if (n <= 1) return;
@@ -450,9 +590,9 @@ __global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const uint32_t sq = smem_addr(smem), sg = sq + kPackTile * L::kStride, sk = sg + kPackTile * L::kStride, sv = sk + 2 * BN * L::kStride;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x];
+  const int4 item = a.items[blockIdx.x / a.hq];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = blockIdx.y, kvh = h / a.group, row0 = item.y * kPackTile, k0 = item.z, k1 = item.w;
+  const int h = blockIdx.x % a.hq, kvh = h / a.group, row0 = item.y * kPackTile, k0 = item.z, k1 = item.w;
   const int nt = (max(k1 - k0, 0) + BN - 1) / BN;
   load_rows<T, DP, kPackTile>(sq, a.q, h, q0, row0, lq, a.d, tid);
   load_rows<T, DP, kPackTile>(sg, a.g, h, q0, row0, lq, a.d, tid);
@@ -524,9 +664,9 @@ __global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
   const uint32_t sk = smem_addr(smem), sv = sk + kPackTile * L::kStride, sq = sv + kPackTile * L::kStride, sg = sq + 2 * BN * L::kStride;
   float* se = reinterpret_cast<float*>(smem + (2 * kPackTile + 4 * BN) * L::kStride);   // [2][BN] lse, [2][BN] delta
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x];
+  const int4 item = a.items[blockIdx.x / a.hk];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int kvh = blockIdx.y, row0 = item.y * kPackTile, i0 = item.z, i1 = item.w;
+  const int kvh = blockIdx.x % a.hk, row0 = item.y * kPackTile, i0 = item.z, i1 = item.w;
   const int per = (max(i1 - i0, 0) + BN - 1) / BN, nt = per * a.group;
   load_rows<T, DP, kPackTile>(sk, a.k, kvh, c0, row0, lk, a.d, tid);
   load_rows<T, DP, kPackTile>(sv, a.v, kvh, c0, row0, lk, a.d, tid);
@@ -607,51 +747,57 @@ void allow_smem(int smem) {
   }
 }
 template <auto kernel>
-void launch(dim3 grid, int threads, int smem, cudaStream_t st, const PackedArgs& a) {
+int launch(int64_t grid, int threads, int smem, cudaStream_t st, const PackedArgs& a) {
+  if (grid > 0x7fffffff) return kTooLarge;
   if (smem > 48 * 1024) allow_smem<kernel>(smem);
-  kernel<<<grid, threads, smem, st>>>(a);
+  kernel<<<(unsigned)grid, threads, smem, st>>>(a);
   count_launch();
+  return kOk;
 }
 
 #define SO3LR_PACKED_WIDTHS(T, CALL)            \
   switch (packed_padded(a.d)) {                 \
-    case 32: { CALL(T, 32) } break;             \
-    case 64: { CALL(T, 64) } break;             \
-    case 96: { CALL(T, 96) } break;             \
-    default: { CALL(T, 128) } break;            \
+    case 32: { CALL(T, 32) }                    \
+    case 64: { CALL(T, 64) }                    \
+    case 96: { CALL(T, 96) }                    \
+    default: { CALL(T, 128) }                   \
   }
 
 }  // namespace packed
 
-template <typename T> void packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) packed::launch<packed::forward_kernel<T, DP, false>>(dim3(n_items, a.hq), 128, packed::forward_smem<T, DP>(), st, a);
+template <typename T> int packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
+#define CALL(T, DP) return packed::launch<packed::forward_kernel<T, DP, false>>((int64_t)n_items * a.hq, 128, packed::forward_smem<T, DP>(), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
-template <typename T> void packed_forward_split(cudaStream_t st, const PackedArgs& a, int n_items, int n_structures, bool combine) {
-#define CALL(T, DP)                                                                                                                 \
-  packed::launch<packed::forward_kernel<T, DP, true>>(dim3(n_items, a.hk), 128, packed::forward_smem<T, DP>(), st, a);              \
-  if (combine) packed::launch<packed::combine_kernel<T, DP>>(dim3(n_structures, a.hk), 256, 0, st, a);
+template <typename T> int packed_forward_split(cudaStream_t st, const PackedArgs& a, int n_items, int n_structures, bool combine) {
+#define CALL(T, DP)                                                                                                                           \
+  const int rc = a.part_rows <= packed::kNarrowRows                                                                                           \
+                     ? packed::launch<packed::narrow_kernel<T, DP>>((int64_t)n_items * a.hk, 128, packed::narrow_smem<T, DP>(), st, a)        \
+                     : packed::launch<packed::forward_kernel<T, DP, true>>((int64_t)n_items * a.hk, 128, packed::forward_smem<T, DP>(), st, a); \
+  return rc || !combine ? rc : packed::launch<packed::combine_kernel<T, DP>>((int64_t)n_structures * a.hk, 256, 0, st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
-template <typename T> void packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) packed::launch<packed::dq_kernel<T, DP>>(dim3(n_items, a.hq), 128, packed::reverse_smem<T, DP>(), st, a);
+template <typename T> int packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
+#define CALL(T, DP) return packed::launch<packed::dq_kernel<T, DP>>((int64_t)n_items * a.hq, 128, packed::reverse_smem<T, DP>(), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
-template <typename T> void packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) packed::launch<packed::dkv_kernel<T, DP>>(dim3(n_items, a.hk), 128, packed::reverse_smem<T, DP>(), st, a);
+template <typename T> int packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
+#define CALL(T, DP) return packed::launch<packed::dkv_kernel<T, DP>>((int64_t)n_items * a.hk, 128, packed::reverse_smem<T, DP>(), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
-template <typename T> void packed_delta(cudaStream_t st, const PackedArgs& a, int rows) {
+template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, int rows) {
   int width = 1;
   while (width * (16 / (int)sizeof(T)) < a.d) width <<= 1;
-  const long long threads = (long long)rows * a.hq * width;
-  if (threads == 0) return;
-  packed::delta_kernel<T><<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(a, rows, width);
+  const int64_t ctas = ((int64_t)rows * a.hq * width + 255) / 256;
+  if (ctas > 0x7fffffff) return kTooLarge;
+  if (ctas == 0) return kOk;
+  packed::delta_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, rows, width);
   count_launch();
+  return kOk;
 }
 
 }  // namespace so3lr

@@ -2,9 +2,9 @@
 #include "packed_mma.cuh"
 
 namespace so3lr {
-template void packed_forward_mma<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
-template void packed_forward_split<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int, int, bool);
-template void packed_dq_mma<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
-template void packed_dkv_mma<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
-template void packed_delta<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
+template int packed_forward_mma<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
+template int packed_forward_split<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int, int, bool);
+template int packed_dq_mma<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
+template int packed_dkv_mma<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
+template int packed_delta<__nv_bfloat16>(cudaStream_t, const PackedArgs&, int);
 }  // namespace so3lr
