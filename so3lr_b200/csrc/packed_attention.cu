@@ -16,7 +16,8 @@ namespace {
 // The image of a layout (int32): a header, the offsets of both sides, and tables of work items {structure, tile, first, last}.
 // Tables of query tiles: 64 rows (warp-level kernels), 128 and 256 (tensor cores, reverse and forward); of key tiles: 64 and 128.
 enum Head : int { kMagicAt, kN, kCausal, kRowsQ, kRowsKv, kMaxQ, kStartQ, kStartKv, kItemsQ, kNItemsQ, kItemsKv, kNItemsKv, kItemsSplit, kNItemsSplit,
-                  kSplitFirst, kCombine, kTotal, kItemsQ128, kNItemsQ128, kItemsQ256, kNItemsQ256, kItemsKv128, kNItemsKv128, kMaxKv, kHeadInts = 32 };
+                  kSplitFirst, kCombine, kTotal, kItemsQ128, kNItemsQ128, kItemsQ256, kNItemsQ256, kItemsKv128, kNItemsKv128, kMaxKv,
+                  kWalkQ128, kWalkQ256, kWalkKv128 /* tiles of 128 that the items of a table walk over in all */, kHeadInts = 32 };
 constexpr int kMagic = 0x53334c50;
 constexpr int kTables = 5, kTileRows[kTables] = {kPackTile, kPackTile, 128, 256, 128}, kTableAt[kTables] = {kItemsQ, kItemsKv, kItemsQ128, kItemsQ256, kItemsKv128};
 constexpr bool kOfKeys[kTables] = {false, true, false, false, true};
@@ -86,6 +87,11 @@ void build_image(int n, const int32_t* sq, const int32_t* sk, bool causal, int32
       }
     }
     put(im + im[kTableAt[t]], items);
+    if (t >= 2) {
+      int64_t walk = 0;
+      for (const Item& i : items) walk += (i.last - i.first + 127) / 128;
+      im[kWalkQ128 + t - 2] = (int32_t)std::min<int64_t>(walk, 0x7fffffff);
+    }
   }
   const int chunk = split_length(sk[n]);
   int32_t* split = im + im[kItemsSplit];
@@ -120,6 +126,7 @@ bool shape_ok(const int32_t* im, const so3lr_b200_attention_shape* a) {
 PackedArgs common(const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a) {
   PackedArgs p;
   p.start_q = dev + im[kStartQ]; p.start_kv = dev + im[kStartKv]; p.split_first = dev + im[kSplitFirst];
+  p.rows = im[kRowsQ]; p.rows_kv = im[kRowsKv];
   p.nq = (int)a->rows_q; p.nkv = (int)a->rows_kv; p.hq = a->heads_q; p.hk = a->heads_kv; p.group = a->heads_q / a->heads_kv; p.d = a->d; p.causal = im[kCausal];
   p.scale = a->scale; p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   return p;
@@ -141,8 +148,34 @@ int64_t part_floats(const int32_t* im, const so3lr_b200_attention_shape* a) {
 bool on_tensor_cores(const int32_t* im, const so3lr_b200_attention_shape* a) {
   return (a->type != kF32 || a->d <= 64) && im[kMaxQ] >= SO3LR_PACKED_TC_ROWS && im[kMaxKv] >= SO3LR_PACKED_TC_ROWS;
 }
-int64_t split_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool reverse) {
-  return a->type == kF32 && on_tensor_cores(im, a) ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0;
+// Into how many pieces the walks of a kernel's items are cut.  With few CTAs for the chip the last round of them leaves most SMs idle (160
+// equal ones on 148: half of the time), so the time is that of the work on all SMs, plus half of a CTA that ends last, plus what a CTA costs
+// besides its tiles (a start and an end: two tiles' time) and a round of the join.
+int pieces_of(int64_t items, int heads, int64_t walk, int longest) {
+  if (items == 0 || walk == 0) return 1;
+  const double sms = sm_count(), ctas = (double)items * heads, tiles = (double)walk * heads;
+  double best = 0;
+  int at = 1;
+  for (int p = 1; p <= 16 && (p == 1 || longest >= 3 * p); ++p) {
+    const double one = (double)longest / p + 2, rounds = std::max(1.0, ctas * p / sms);
+    const double even = (tiles + 2 * ctas * p) / sms, quantised = std::ceil(ctas * p / sms) * (tiles / (ctas * p) + 2);
+    const double cost = std::max(even + 0.5 * one / rounds, std::min(quantised, even + one)) + (p > 1 ? 1.5 + 0.1 * p : 0);
+    if (p == 1 || cost < 0.95 * best) { best = cost; at = p; }
+  }
+  return at;
+}
+PackedPieces pieces(const int32_t* im, const so3lr_b200_attention_shape* a) {
+  PackedPieces p;
+  const int long_q = (im[kMaxQ] + 127) / 128, long_kv = (im[kMaxKv] + 127) / 128, group = a->heads_q / a->heads_kv;
+  p.forward = pieces_of(im[kNItemsQ256], a->heads_q, im[kWalkQ256], long_kv);
+  p.dq = pieces_of(im[kNItemsQ128], a->heads_q, im[kWalkQ128], long_kv);
+  p.dkv = pieces_of(im[kNItemsKv128], a->heads_kv, (int64_t)im[kWalkKv128] * group, long_q * group);
+  return p;
+}
+int64_t tc_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool reverse) {
+  if (!on_tensor_cores(im, a)) return 0;
+  return (a->type == kF32 ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0) +
+         packed_share_bytes(pieces(im, a), a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse);
 }
 
 const int4* table(const int32_t* im, const int32_t* dev, int field) { return reinterpret_cast<const int4*>(dev + im[field]); }
@@ -158,7 +191,7 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
   }
   if (on_tensor_cores(im, a)) {
     p.items = table(im, dev, kItemsQ256);
-    return packed_forward_tc<T>(st, p, im[kNItemsQ256], workspace);
+    return packed_forward_tc<T>(st, p, im[kNItemsQ256], pieces(im, a), workspace);
   }
   p.items = table(im, dev, kItemsQ);
   return packed_forward_mma<T>(st, p, im[kNItemsQ]);
@@ -169,7 +202,7 @@ int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
   int rc = packed_delta<T>(st, p, im[kRowsQ]);
   if (rc) return rc;
   if (on_tensor_cores(im, a))
-    return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128], workspace);
+    return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128], pieces(im, a), workspace);
   p.items = table(im, dev, kItemsQ);
   if (im[kNItemsQ]) rc = packed_dq_mma<T>(st, p, im[kNItemsQ]);
   p.items = table(im, dev, kItemsKv);
@@ -202,8 +235,8 @@ int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int
 
 int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* a, int vjp) {
   if (!shape_ok(image, a)) return -1;
-  if (vjp) return split_bytes(image, a, true);
-  if (!few_rows(image, a)) return split_bytes(image, a, false);
+  if (vjp) return tc_bytes(image, a, true);
+  if (!few_rows(image, a)) return tc_bytes(image, a, false);
   if (!image[kCombine]) return 0;
   return part_floats(image, a) * (int64_t)sizeof(float) + part_floats(image, a) / packed_padded(a->d) * (int64_t)sizeof(float2);
 }

@@ -34,6 +34,9 @@ struct PackedArgs {
   float* part_o = nullptr;      // (item, hk, part_rows, DP) of the split form
   float2* part_ml = nullptr;    // (item, hk, part_rows): running maximum (in units of log2) and sum
   int part_rows = 0;            // most rows of a structure: tokens times heads of a group
+  int pieces = 1;               // tensor-core kernels: pieces that an item's walk is cut into; each leaves its share in part_o / part_ml or
+  float* share[3] = {};         // (reverse) in share: (pieces, heads, rows, d) of dq, dk, dv
+  int rows = 0, rows_kv = 0;    // of the layout
   int nq = 0, nkv = 0, hq = 0, hk = 0, group = 1, d = 0, causal = 0;
   float scale = 0.f, scale_log2 = 0.f;                // scale * log2(e): the softmax runs on powers of two
   int* err = nullptr;
@@ -50,13 +53,21 @@ template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, int
 
 // Kernels on the tensor cores: tiles of 128 rows, two of them side by side in the forward kernel.  float32 (d <= 64) runs on operands that
 // are split into three bfloat16 terms ahead (packed_split_bytes of workspace).
-template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, void* workspace);
-template <typename T> int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, void* workspace);
+struct PackedPieces { int forward = 1, dq = 1, dkv = 1; };
+template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace);
+template <typename T>
+int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, const PackedPieces& pieces, void* workspace);
 inline int packed_split_width(int d) { return d <= 32 ? 32 : 64; }
 inline int64_t packed_split_bytes(int64_t rows_q, int64_t rows_kv, int hq, int hk, int d, bool reverse) {
   return ((reverse ? 2 : 1) * rows_q * hq + 2 * rows_kv * hk) * 3 * packed_split_width(d) * 2;
 }
 int packed_error(int* out);
+
+// shares of the pieces, behind the split operands
+inline int64_t packed_share_bytes(const PackedPieces& p, int64_t rows_q, int64_t rows_kv, int hq, int hk, int d, bool reverse) {
+  if (!reverse) return p.forward > 1 ? p.forward * rows_q * hq * (d + 2) * 4 : 0;
+  return (p.dq > 1 ? p.dq * rows_q * hq * d * 4 : 0) + (p.dkv > 1 ? 2 * p.dkv * rows_kv * hk * d * 4 : 0);
+}
 
 inline int packed_padded(int d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
 

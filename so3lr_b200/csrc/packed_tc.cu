@@ -79,12 +79,15 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x / a.hq];
+  const int unit = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
+  const int4 item = a.items[unit / a.hq];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = blockIdx.x % a.hq, kvh = h / a.group, row0 = item.y * 2 * kTile, off = lk - lq;
+  const int h = unit % a.hq, kvh = h / a.group, row0 = item.y * 2 * kTile, off = lk - lq;
   // keys that a tile meets: [0, end[t]), and tiles of keys
   const int end1 = item.w, end0 = a.causal ? min(end1, max(0, min(lq, row0 + kTile) + off)) : end1;
-  const int n0 = (end0 + kTile - 1) / kTile, n1 = row0 + kTile < lq ? (end1 + kTile - 1) / kTile : 0, n = max(n0, n1);
+  const int all0 = (end0 + kTile - 1) / kTile, all1 = row0 + kTile < lq ? (end1 + kTile - 1) / kTile : 0, per = (max(all0, all1) + a.pieces - 1) / a.pieces;
+  // this piece's: tiles from k0 / 128 on
+  const int k0 = piece * per * kTile, n0 = min(per, max(0, all0 - piece * per)), n1 = min(per, max(0, all1 - piece * per)), n = max(n0, n1);
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
@@ -151,7 +154,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
         if ((t ? n1 : n0) > 0) ld.tile(sq + t * tile_bytes, &maps.q, q0 + row0 + t * kTile, h, bar(kQFull + t), kTile, false, failed, &g_packed_error);
       for (int j = 0; j < 2 * n; ++j) {
         if (j >= R) wait_bar(bar(kEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
-        const int r = (j >> 1) * kTile;
+        const int r = k0 + (j >> 1) * kTile;
         ld.tile(ring + (j % R) * tile_bytes, (j & 1) ? &maps.v : &maps.k, c0 + r, kvh, bar(kFull + j % R), lk - r, j & 1, failed, &g_packed_error);
       }
     }
@@ -175,7 +178,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
 #pragma unroll
       for (int c = 0; c < kTile; c += 32) ld32(ts + c, x + c);
       wait_ld(x);
-      const int kb = i * kTile;
+      const int kb = k0 + i * kTile;
       const bool masked = kb + kTile - 1 > lim_first;
       if (masked) {
 #pragma unroll
@@ -241,6 +244,27 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
     }
     if constexpr (TERMS == 3) { if (nt > 0) add_cols<DW, DW>(to, own); }
     const bool there = row < lq, bad = *failed;
+    if (a.pieces > 1) {      // the share: o as it is, with its maximum and sum
+      const long long slot = ((long long)piece * a.hq + h) * a.nq + q0 + row;
+      if (there) a.part_ml[slot] = make_float2(m, bad ? NAN : l);
+      float* dst = a.part_o + slot * d;
+      if (nt > 0) {
+        if constexpr (TERMS == 3) {
+#pragma unroll
+          for (int c = 0; c < DW; c += 16) if (there && c < d) store16(dst + c, own + c);
+        } else {
+          for (int c = 0; c < d; c += 16) {
+            uint32_t o[16];
+            float y[16];
+            ld16(to + c, o);
+            wait_ld(o);
+#pragma unroll
+            for (int k = 0; k < 16; ++k) y[k] = __uint_as_float(o[k]);
+            if (there) store16(dst + c, y);
+          }
+        }
+      }
+    } else {
     const float inv = bad ? NAN : l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
     const long long at = ((long long)(q0 + row) * a.hq + h) * d;
     T *dst = static_cast<T*>(a.out) + at, *rest = a.out_rest ? static_cast<T*>(a.out_rest) + at : nullptr;
@@ -272,6 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       }
     }
     if (there && a.lse) a.lse[(long long)h * a.nq + q0 + row] = bad ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
+    }
     fence_before();
   }
   __syncthreads();
@@ -296,9 +321,11 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x / a.hq];
+  const int unit = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
+  const int4 item = a.items[unit / a.hq];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = blockIdx.x % a.hq, kvh = h / a.group, row0 = item.y * kTile, off = lk - lq, n = (item.w + kTile - 1) / kTile;
+  const int h = unit % a.hq, kvh = h / a.group, row0 = item.y * kTile, off = lk - lq;
+  const int all = (item.w + kTile - 1) / kTile, per = (all + a.pieces - 1) / a.pieces, k0 = piece * per * kTile, n = min(per, max(0, all - piece * per));
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
@@ -359,7 +386,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       __syncwarp();
       for (int j = 0; j < 2 * n; ++j) {
         if (j >= R) wait_bar(bar(kdqEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
-        const int r = (j >> 1) * kTile;
+        const int r = k0 + (j >> 1) * kTile;
         ld.tile(ring + (j % R) * tile_bytes, (j & 1) ? &maps.v : &maps.k, c0 + r, kvh, bar(kdqFull + j % R), lk - r, !(j & 1), failed, &g_packed_error);
       }
     }
@@ -393,7 +420,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
 #pragma unroll
         for (int k = 0; k < 16; ++k) x[c + k] = __float_as_uint(v[k]);
       }
-      const int kb = i * kTile + col;
+      const int kb = k0 + i * kTile + col;
       wait_bar(bar(kdqDp), i & 1, failed, &g_packed_error);
       fence_after();
       ld32(lanes + kTile + col, y);
@@ -422,25 +449,29 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       fence_after();
     }
     const float f = *failed ? NAN : a.scale;
-    T* dst = static_cast<T*>(a.dq) + ((long long)(q0 + row) * a.hq + h) * d;
-    if constexpr (TERMS == 3) {
-      if (n > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own);
+    const long long at_row = ((long long)(q0 + row) * a.hq + h) * d;
+    auto put = [&](auto* dst) {
+      if constexpr (TERMS == 3) {
+        if (n > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own);
 #pragma unroll
-      for (int c = 0; c < kOwn; ++c) own[c] *= f;
+        for (int c = 0; c < kOwn; ++c) own[c] *= f;
 #pragma unroll
-      for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own + c);
-    } else {
-      for (int c = 16 * half; c < d; c += 32) {
-        uint32_t o[16];
-        float v[16];
+        for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own + c);
+      } else {
+        for (int c = 16 * half; c < d; c += 32) {
+          uint32_t o[16];
+          float v[16];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] = 0;
-        if (n > 0) { ld16(lanes + kOut + c, o); wait_ld(o); }
+          for (int k = 0; k < 16; ++k) o[k] = 0;
+          if (n > 0) { ld16(lanes + kOut + c, o); wait_ld(o); }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(o[k]) * f;
-        if (there) store16(dst + c, v);
+          for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(o[k]) * f;
+          if (there) store16(dst + c, v);
+        }
       }
-    }
+    };
+    if (a.pieces > 1) put(a.share[0] + (long long)piece * a.nq * a.hq * d + at_row);
+    else put(static_cast<T*>(a.dq) + at_row);
     fence_before();
   }
   __syncthreads();
@@ -468,10 +499,13 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x / a.hk];
+  const int unit = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
+  const int4 item = a.items[unit / a.hk];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int kvh = blockIdx.x % a.hk, row0 = item.y * kTile, off = lk - lq, i0 = item.z;
-  const int per = (max(lq - i0, 0) + kTile - 1) / kTile, n = per * a.group;
+  const int kvh = unit % a.hk, row0 = item.y * kTile, off = lk - lq, i0 = item.z;
+  // tiles of queries of a head, of all heads of the group, and of this piece: from j0 on
+  const int per = (max(lq - i0, 0) + kTile - 1) / kTile, all = per * a.group, share = (all + a.pieces - 1) / a.pieces, j0 = piece * share;
+  const int n = min(share, max(0, all - j0));
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
@@ -533,13 +567,13 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       __syncwarp();
       for (int j = 0; j < 2 * n; ++j) {
         if (j >= R) wait_bar(bar(kkvEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
-        const int i = j >> 1, hq = kvh * a.group + i / per, b = i0 + (i % per) * kTile;
+        const int i = j0 + (j >> 1), hq = kvh * a.group + i / per, b = i0 + (i % per) * kTile;
         ld.tile(ring + (j % R) * tile_bytes, (j & 1) ? &maps.g : &maps.q, q0 + b, hq, bar(kkvFull + j % R), lq - b, true, failed, &g_packed_error);
       }
     } else if (warp > kLoadWarp) {
       const int r0 = (warp - kLoadWarp - 1) * 32 + lane;
       for (int i = 0; i < n; ++i) {
-        const int st = i & 1, hq = kvh * a.group + i / per, b = i0 + (i % per) * kTile;
+        const int st = i & 1, hq = kvh * a.group + (j0 + i) / per, b = i0 + ((j0 + i) % per) * kTile;
         if (i >= 2) wait_bar(bar(kkvStatFree + st), ((i >> 1) - 1) & 1, failed, &g_packed_error);
         for (int r = r0; r < kTile; r += 64) {
           const bool ok = b + r < lq;
@@ -564,7 +598,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
     const Packed to_p{{(uint32_t)col, 32 + (uint32_t)col, 256 + (uint32_t)col / 2}, {}},
         to_s{{kTile + (uint32_t)col, kTile + 32 + (uint32_t)col, 320 + (uint32_t)col / 2}, {}};
     for (int i = 0; i < n; ++i) {
-      const int st = i & 1, ib = i0 + (i % per) * kTile + col;
+      const int st = i & 1, ib = i0 + ((j0 + i) % per) * kTile + col;
       uint32_t x[64], y[64];
       wait_bar(bar(kkvStat + st), (i >> 1) & 1, failed, &g_packed_error);
       wait_bar(bar(kkvS), i & 1, failed, &g_packed_error);
@@ -634,25 +668,28 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
     for (int which = 0; which < 2; ++which) {
       const float f = bad ? NAN : which ? a.scale : packed::prob_unscale<T>();
       const uint32_t from = lanes + (which ? kDk : kDv);
-      T* dst = static_cast<T*>(which ? a.dk : a.dv) + at;
-      if constexpr (TERMS == 3) {
-        if (n > 0) add_cols<DW, DW / 2>(from + half * (DW / 2), own[which]);
+      auto put = [&](auto* dst) {
+        if constexpr (TERMS == 3) {
+          if (n > 0) add_cols<DW, DW / 2>(from + half * (DW / 2), own[which]);
 #pragma unroll
-        for (int c = 0; c < kOwn; ++c) own[which][c] *= f;
+          for (int c = 0; c < kOwn; ++c) own[which][c] *= f;
 #pragma unroll
-        for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own[which] + c);
-      } else {
-        for (int c = 16 * half; c < d; c += 32) {
-          uint32_t o[16];
-          float v[16];
+          for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own[which] + c);
+        } else {
+          for (int c = 16 * half; c < d; c += 32) {
+            uint32_t o[16];
+            float v[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = 0;
-          if (n > 0) { ld16(from + c, o); wait_ld(o); }
+            for (int k = 0; k < 16; ++k) o[k] = 0;
+            if (n > 0) { ld16(from + c, o); wait_ld(o); }
 #pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(o[k]) * f;
-          if (there) store16(dst + c, v);
+            for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(o[k]) * f;
+            if (there) store16(dst + c, v);
+          }
         }
-      }
+      };
+      if (a.pieces > 1) put(a.share[which ? 1 : 2] + (long long)piece * a.nkv * a.hk * d + at);
+      else put(static_cast<T*>(which ? a.dk : a.dv) + at);
     }
     fence_before();
   }
@@ -661,6 +698,56 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
 }
 
 static_assert(kFwdBars <= 32 && kDqBars <= 32 && kDkvBars <= 32, "barriers");
+
+// joins the pieces of the forward kernel: a thread per eight values of a row
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const PackedArgs a, int rows) {
+  const int parts = a.d / 8;
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x, hr = e / parts;
+  const int c = (int)(e % parts) * 8;
+  if (hr >= (long long)rows * a.hq) return;
+  const long long r = hr / a.hq;
+  const int h = (int)(hr % a.hq);
+  float m = -INFINITY, l = 0.f, o[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) o[k] = 0.f;
+  for (int p = 0; p < a.pieces; ++p) m = fmaxf(m, a.part_ml[((long long)p * a.hq + h) * a.nq + r].x);
+  const float u = m == -INFINITY ? 0.f : m;
+  for (int p = 0; p < a.pieces; ++p) {
+    const long long slot = ((long long)p * a.hq + h) * a.nq + r;
+    const float2 ml = a.part_ml[slot];
+    if (ml.y == 0.f) continue;      // no key of the piece was seen: its share was not written where it has no tile
+    const float f = exp2f(ml.x - u);
+    l = fmaf(ml.y, f, l);
+    const float4 x = *reinterpret_cast<const float4*>(a.part_o + slot * a.d + c), y = *reinterpret_cast<const float4*>(a.part_o + slot * a.d + c + 4);
+    o[0] = fmaf(x.x, f, o[0]); o[1] = fmaf(x.y, f, o[1]); o[2] = fmaf(x.z, f, o[2]); o[3] = fmaf(x.w, f, o[3]);
+    o[4] = fmaf(y.x, f, o[4]); o[5] = fmaf(y.y, f, o[5]); o[6] = fmaf(y.z, f, o[6]); o[7] = fmaf(y.w, f, o[7]);
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const long long at = hr * a.d + c;
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) packed::store_rest<T>(static_cast<T*>(a.out) + at + k, a.out_rest ? static_cast<T*>(a.out_rest) + at + k : nullptr, o[k] * inv, o[k + 1] * inv);
+  if (c == 0 && a.lse) a.lse[(long long)h * a.nq + r] = l == 0.f ? -INFINITY : m + log2f(l);
+}
+// sums the pieces' shares of dq, dk, dv (blockIdx.y), a thread per eight values
+template <typename T>
+__global__ void __launch_bounds__(256) sum_kernel(const PackedArgs a, int first, int pieces_q, int pieces_kv, long long values_q, long long values_kv,
+                                                  long long stride_q, long long stride_kv) {
+  const int which = first + blockIdx.y, pieces = which ? pieces_kv : pieces_q;
+  const long long e = ((long long)blockIdx.x * 256 + threadIdx.x) * 8, values = which ? values_kv : values_q, stride = which ? stride_kv : stride_q;
+  if (e >= values) return;
+  const float* src = a.share[which] + e;
+  float o[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) o[k] = 0.f;
+  for (int p = 0; p < pieces; ++p) {
+    const float4 x = *reinterpret_cast<const float4*>(src + p * stride), y = *reinterpret_cast<const float4*>(src + p * stride + 4);
+    o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w; o[4] += y.x; o[5] += y.y; o[6] += y.z; o[7] += y.w;
+  }
+  T* dst = static_cast<T*>(which == 0 ? a.dq : which == 1 ? a.dk : a.dv) + e;
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) packed::store2(dst + k, o[k], o[k + 1]);
+}
 
 // float32 rows -> three bfloat16 terms, (rows, heads, 3, DW), zeros behind d; a thread per eight values, up to four operands
 struct SplitArgs { Rows src[4]; __nv_bfloat16* dst[4]; int rows[4], heads[4]; };
@@ -752,43 +839,71 @@ template <int TERMS, int DW, auto kernel> int launch(int64_t grid, bool stats, c
   count_launch();
   return kOk;
 }
-template <typename T, int TERMS, int DW> int forward_of(cudaStream_t st, const PackedArgs& a, int n_items, void* workspace) {
+template <typename T, int TERMS, int DW> int forward_of(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace) {
   Maps m;
-  const int rc = maps_of<T, TERMS, DW>(&m, st, a, false, workspace);
-  return rc ? rc : launch<TERMS, DW, forward_kernel<T, TERMS, DW>>((int64_t)n_items * a.hq, false, st, a, m);
+  int rc = maps_of<T, TERMS, DW>(&m, st, a, false, workspace);
+  if (rc) return rc;
+  a.pieces = pieces.forward;
+  if (a.pieces > 1) {
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (TERMS == 3 ? packed_split_bytes(a.nq, a.nkv, a.hq, a.hk, a.d, false) : 0));
+    a.part_ml = reinterpret_cast<float2*>(a.part_o + (long long)a.pieces * a.nq * a.hq * a.d);
+  }
+  rc = launch<TERMS, DW, forward_kernel<T, TERMS, DW>>((int64_t)n_items * a.hq * a.pieces, false, st, a, m);
+  if (rc || a.pieces == 1) return rc;
+  const int64_t ctas = ((int64_t)a.rows * a.hq * (a.d / 8) + 255) / 256;
+  if (ctas > 0x7fffffff) return kTooLarge;
+  join_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, a.rows);
+  count_launch();
+  return kOk;
 }
 template <typename T, int TERMS, int DW>
-int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, void* workspace) {
+int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, const PackedPieces& pieces, void* workspace) {
   Maps m;
   int rc = maps_of<T, TERMS, DW>(&m, st, a, true, workspace);
   if (rc) return rc;
+  const long long stride_q = (long long)a.nq * a.hq * a.d, stride_kv = (long long)a.nkv * a.hk * a.d;
+  float* share = reinterpret_cast<float*>(static_cast<char*>(workspace) + (TERMS == 3 ? packed_split_bytes(a.nq, a.nkv, a.hq, a.hk, a.d, true) : 0));
+  if (pieces.dq > 1) { a.share[0] = share; share += pieces.dq * stride_q; }
+  if (pieces.dkv > 1) { a.share[1] = share; a.share[2] = share + pieces.dkv * stride_kv; }
   a.items = items_q;
-  rc = launch<TERMS, DW, dq_kernel<T, TERMS, DW>>((int64_t)n_q * a.hq, false, st, a, m);
+  a.pieces = pieces.dq;
+  rc = launch<TERMS, DW, dq_kernel<T, TERMS, DW>>((int64_t)n_q * a.hq * a.pieces, false, st, a, m);
   if (rc) return rc;
   a.items = items_kv;
-  return launch<TERMS, DW, dkv_kernel<T, TERMS, DW>>((int64_t)n_kv * a.hk, true, st, a, m);
+  a.pieces = pieces.dkv;
+  rc = launch<TERMS, DW, dkv_kernel<T, TERMS, DW>>((int64_t)n_kv * a.hk * a.pieces, true, st, a, m);
+  if (rc || (pieces.dq == 1 && pieces.dkv == 1)) return rc;
+  const long long values_q = (long long)a.rows * a.hq * a.d, values_kv = (long long)a.rows_kv * a.hk * a.d;
+  const int first = pieces.dq > 1 ? 0 : 1, many = (pieces.dkv > 1 ? 3 : 1) - first;
+  const int64_t ctas = (std::max(pieces.dq > 1 ? values_q : 0, pieces.dkv > 1 ? values_kv : 0) / 8 + 255) / 256;
+  if (ctas > 0x7fffffff) return kTooLarge;
+  sum_kernel<T><<<dim3((unsigned)ctas, many), 256, 0, st>>>(a, first, pieces.dq, pieces.dkv, values_q, values_kv, stride_q, stride_kv);
+  count_launch();
+  return kOk;
 }
 
 }  // namespace
 
-template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, void* workspace) {
-  if constexpr (sizeof(T) == 2) return forward_of<T, 1, 64>(st, a, n_items, workspace);
-  else return a.d <= 32 ? forward_of<T, 3, 32>(st, a, n_items, workspace) : forward_of<T, 3, 64>(st, a, n_items, workspace);
+template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace) {
+  if constexpr (sizeof(T) == 2) return forward_of<T, 1, 64>(st, a, n_items, pieces, workspace);
+  else return a.d <= 32 ? forward_of<T, 3, 32>(st, a, n_items, pieces, workspace) : forward_of<T, 3, 64>(st, a, n_items, pieces, workspace);
 }
-template <typename T> int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, void* workspace) {
-  if constexpr (sizeof(T) == 2) return reverse_of<T, 1, 64>(st, a, items_q, n_q, items_kv, n_kv, workspace);
-  else return a.d <= 32 ? reverse_of<T, 3, 32>(st, a, items_q, n_q, items_kv, n_kv, workspace) : reverse_of<T, 3, 64>(st, a, items_q, n_q, items_kv, n_kv, workspace);
+template <typename T>
+int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, const PackedPieces& pieces, void* workspace) {
+  if constexpr (sizeof(T) == 2) return reverse_of<T, 1, 64>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace);
+  else return a.d <= 32 ? reverse_of<T, 3, 32>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace)
+                        : reverse_of<T, 3, 64>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace);
 }
 int packed_error(int* out) {
   const cudaError_t e = cudaMemcpyFromSymbol(out, g_packed_error, sizeof(int));
   return e == cudaSuccess ? kOk : kCudaError;
 }
 
-template int packed_forward_tc<__nv_bfloat16>(cudaStream_t, PackedArgs, int, void*);
-template int packed_reverse_tc<__nv_bfloat16>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int, void*);
-template int packed_forward_tc<__half>(cudaStream_t, PackedArgs, int, void*);
-template int packed_reverse_tc<__half>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int, void*);
-template int packed_forward_tc<float>(cudaStream_t, PackedArgs, int, void*);
-template int packed_reverse_tc<float>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int, void*);
+template int packed_forward_tc<__nv_bfloat16>(cudaStream_t, PackedArgs, int, const PackedPieces&, void*);
+template int packed_reverse_tc<__nv_bfloat16>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int, const PackedPieces&, void*);
+template int packed_forward_tc<__half>(cudaStream_t, PackedArgs, int, const PackedPieces&, void*);
+template int packed_reverse_tc<__half>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int, const PackedPieces&, void*);
+template int packed_forward_tc<float>(cudaStream_t, PackedArgs, int, const PackedPieces&, void*);
+template int packed_reverse_tc<float>(cudaStream_t, PackedArgs, const int4*, int, const int4*, int, const PackedPieces&, void*);
 
 }  // namespace so3lr
