@@ -150,8 +150,8 @@ bool on_tensor_cores(const int32_t* im, const so3lr_b200_attention_shape* a) {
 }
 // Into how many pieces the walks of a kernel's items are cut.  With few CTAs for the chip the last round of them leaves most SMs idle (160
 // equal ones on 148: half of the time), so the time is that of the work on all SMs, plus half of a CTA that ends last, plus what a CTA costs
-// besides its tiles (a start and an end: two tiles' time) and a round of the join.
-int pieces_of(int64_t items, int heads, int64_t walk, int longest) {
+// besides its tiles (a start and an end: two tiles' time, `tile` us each), plus the shares' way through memory and the launch that joins them.
+int pieces_of(int64_t items, int heads, int64_t walk, int longest, double tile, double share_bytes) {
   if (items == 0 || walk == 0) return 1;
   const double sms = sm_count(), ctas = (double)items * heads, tiles = (double)walk * heads;
   double best = 0;
@@ -159,7 +159,7 @@ int pieces_of(int64_t items, int heads, int64_t walk, int longest) {
   for (int p = 1; p <= 16 && (p == 1 || longest >= 3 * p); ++p) {
     const double one = (double)longest / p + 2, rounds = std::max(1.0, ctas * p / sms);
     const double even = (tiles + 2 * ctas * p) / sms, quantised = std::ceil(ctas * p / sms) * (tiles / (ctas * p) + 2);
-    const double cost = std::max(even + 0.5 * one / rounds, std::min(quantised, even + one)) + (p > 1 ? 1.5 + 0.1 * p : 0);
+    const double cost = tile * std::max(even + 0.5 * one / rounds, std::min(quantised, even + one)) + (p > 1 ? 3 + p * share_bytes * 2 / 4e6 : 0);
     if (p == 1 || cost < 0.95 * best) { best = cost; at = p; }
   }
   return at;
@@ -167,9 +167,13 @@ int pieces_of(int64_t items, int heads, int64_t walk, int longest) {
 PackedPieces pieces(const int32_t* im, const so3lr_b200_attention_shape* a) {
   PackedPieces p;
   const int long_q = (im[kMaxQ] + 127) / 128, long_kv = (im[kMaxKv] + 127) / 128, group = a->heads_q / a->heads_kv;
-  p.forward = pieces_of(im[kNItemsQ256], a->heads_q, im[kWalkQ256], long_kv);
-  p.dq = pieces_of(im[kNItemsQ128], a->heads_q, im[kWalkQ128], long_kv);
-  p.dkv = pieces_of(im[kNItemsKv128], a->heads_kv, (int64_t)im[kWalkKv128] * group, long_q * group);
+  // a tile's time as measured: 256 x 128 forward, 128 x 128 reverse
+  const bool f32 = a->type == kF32, wide = a->d > 64;
+  const double fwd = f32 ? 3.0 : wide ? 2.1 : 1.4, dq = f32 ? 2.0 : wide ? 1.4 : 1.0, dkv = f32 ? 3.0 : wide ? 1.6 : 1.2;
+  const double bytes_q = 4.0 * im[kRowsQ] * a->heads_q * a->d, bytes_kv = 4.0 * im[kRowsKv] * a->heads_kv * a->d;
+  p.forward = pieces_of(im[kNItemsQ256], a->heads_q, im[kWalkQ256], long_kv, fwd, bytes_q);
+  p.dq = pieces_of(im[kNItemsQ128], a->heads_q, im[kWalkQ128], long_kv, dq, bytes_q);
+  p.dkv = pieces_of(im[kNItemsKv128], a->heads_kv, (int64_t)im[kWalkKv128] * group, long_q * group, dkv, 2 * bytes_kv);
   return p;
 }
 int64_t tc_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool reverse) {

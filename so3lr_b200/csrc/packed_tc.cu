@@ -61,11 +61,12 @@ __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* p) { retur
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 // 256 queries of one head: two tiles of 128 rows take turns, so that the exponentials of one run beside the products of the other.
-// Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t; P of a tile replaces its logits.  (float32: logits at 256 t, the three
-// terms of P from there on, its output at 256 t + 192.)
+// Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t; P of a tile replaces its logits.  (Up to 64 values a head: output at
+// 256 + 64 t, P at 384 + 64 t.  float32: logits at 256 t, the three terms of P from there on, its output at 256 t + 192.)
 // The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
 // the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
-enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kSFull = kQFull + 2, kPFull = kSFull + 2 /* tile + 2 half */, kOFull = kPFull + 4, kFix = kOFull + 2, kFwdBars };
+enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kSFull = kQFull + 2, kPFull = kSFull + 2 /* tile + 2 half */, kOFull = kPFull + 4, kFix = kOFull + 2,
+              kSRead, kFwdBars = kSRead + 2 };
 
 template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
@@ -73,7 +74,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
   using G = Geometry<TERMS, DW>;
   extern __shared__ unsigned char raw[];
   unsigned char* smem = aligned_smem(raw);
-  const int d = a.d, subs = G::subs(d), tile_bytes = subs * (int)G::kSub, R = G::ring(d);
+  const int d = a.d;
+  constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = G::kRing;
   Tail* tail = reinterpret_cast<Tail*>(smem + (2 + R) * tile_bytes);
   const uint32_t sq = smem_addr(smem), ring = sq + 2 * tile_bytes, bar0 = smem_addr(tail->bars);
   volatile int* failed = &tail->failed;
@@ -91,14 +93,16 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
-    for (int i = 0; i < kFwdBars; ++i) init_bar(bar(i), i >= kPFull && i < kPFull + 4 ? kTile : 1);
+    for (int i = 0; i < kFwdBars; ++i) init_bar(bar(i), (i >= kPFull && i < kPFull + 4) || i >= kSRead ? kTile : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = tail->tmem;
-  constexpr uint32_t kStride = TERMS == 1 ? kTile : 256, kOut = TERMS == 1 ? 256 : 192;
+  // columns from one tile's logits to the other's, output of a tile, columns from one output to the other, P
+  constexpr uint32_t kStride = TERMS == 1 ? kTile : 256, kOut = TERMS == 1 ? 256 : 192, kOutStride = TERMS == 1 ? DW : 256;
+  auto p_at = [](int t) { return G::kEarly ? 384u + 64 * t : kStride * t; };
 
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
@@ -120,36 +124,47 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       }
       give(0);
       for (int i = 0; i < n; ++i) {
-        ready(2 * i + 1);
+        auto logits = [&](int t) {
+          if (i + 1 >= (t ? n1 : n0)) return;
+          product_rows<M, TERMS, DW>(on, tmem + kStride * t, sq + t * tile_bytes, slot(2 * i + 2), d);
+          commit(on, bar(kSFull + t));
+        };
         if (i + 1 < n) ready(2 * i + 2);
+        if (G::kEarly) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (i + 1 >= (t ? n1 : n0)) continue;
+            wait_bar(bar(kSRead + t), i & 1, failed, &g_packed_error);
+            fence_after();
+            logits(t);
+          }
+          if (i + 1 < n) give(2 * i + 2);
+        }
+        ready(2 * i + 1);
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int nt = t ? n1 : n0;
           if (i >= nt) continue;
           wait_bar(bar(kPFull + t), i & 1, failed, &g_packed_error);
           fence_after();
-          const uint32_t at = tmem + kStride * t;
+          const uint32_t at = tmem + p_at(t), out = tmem + kOut + kOutStride * t;
           const Packed p{{at, at + 64, at + 128}, {32, 32, 32}};
           if constexpr (TERMS == 1) {      // the first half of the keys while the exponentials of the second are formed
-            product_cols<M, TERMS, DW, 0, 4>(on, at + kOut, p, slot(2 * i + 1), d, i > 0);
+            product_cols<M, TERMS, DW, 0, 4>(on, out, p, slot(2 * i + 1), d, i > 0);
             wait_bar(bar(kPFull + 2 + t), i & 1, failed, &g_packed_error);
             fence_after();
-            product_cols<M, TERMS, DW, 4, 8>(on, at + kOut, p, slot(2 * i + 1), d, 1);
+            product_cols<M, TERMS, DW, 4, 8>(on, out, p, slot(2 * i + 1), d, 1);
           } else {
-            product_cols<M, TERMS, DW>(on, at + kOut, p, slot(2 * i + 1), d, 0);
+            product_cols<M, TERMS, DW>(on, out, p, slot(2 * i + 1), d, 0);
           }
-          if (i + 1 < nt) {
-            product_rows<M, TERMS, DW>(on, at, sq + t * tile_bytes, slot(2 * i + 2), d);
-            commit(on, bar(kSFull + t));
-          } else {
-            commit(on, bar(kOFull + t));
-          }
+          if (!G::kEarly) logits(t);
+          if (G::kEarly || i + 1 == nt) commit(on, bar(kOFull + t));
         }
         give(2 * i + 1);
-        if (i + 1 < n) give(2 * i + 2);
+        if (!G::kEarly && i + 1 < n) give(2 * i + 2);
       }
     } else if (warp == kLoadWarp && n > 0) {
-      Loader<TERMS, DW> ld{lane, subs, bar(kFix)};
+      Loader<TERMS, DW> ld{lane, bar(kFix)};
       for (int t = 0; t < 2; ++t)
         if ((t ? n1 : n0) > 0) ld.tile(sq + t * tile_bytes, &maps.q, q0 + row0 + t * kTile, h, bar(kQFull + t), kTile, false, failed, &g_packed_error);
       for (int j = 0; j < 2 * n; ++j) {
@@ -162,7 +177,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
     more_regs<kComputeRegs>();
     const int t = warp >> 2, w = warp & 3, nt = t ? n1 : n0;
     const int row = row0 + t * kTile + w * 32 + lane, first = row0 + t * kTile + w * 32;
-    const uint32_t ts = tmem + ((uint32_t)(32 * w) << 16) + kStride * t, to = ts + kOut;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16), ts = lanes + kStride * t, to = lanes + kOut + kOutStride * t;
     constexpr int kOwn = TERMS == 1 ? 1 : DW;
     float own[kOwn];                         // the output so far (float32)
 #pragma unroll
@@ -178,6 +193,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
 #pragma unroll
       for (int c = 0; c < kTile; c += 32) ld32(ts + c, x + c);
       wait_ld(x);
+      if (G::kEarly) { fence_before(); arrive(bar(kSRead + t)); }
       const int kb = k0 + i * kTile;
       const bool masked = kb + kTile - 1 > lim_first;
       if (masked) {
@@ -192,6 +208,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       }
       const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2);
       const bool raise = mn > m + 8.f;      // true where there was none yet
+      if (G::kEarly && i > 0) { wait_bar(bar(kOFull + t), (i - 1) & 1, failed, &g_packed_error); fence_after(); }      // the output and P are free
       if (__any_sync(0xffffffffu, raise)) {
         const float f = raise ? pow2(m - mn) : 1.f;
         if (raise) m = mn;
@@ -214,7 +231,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       float2 sums[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) sums[e] = make_float2(0.f, 0.f);
-      const Packed at{{0, 64, 128}, {}};
+      const Packed at{{p_at(t), p_at(t) + 64, p_at(t) + 128}, {}};
       const float2 scale = make_float2(a.scale_log2, a.scale_log2), ref = make_float2(u, u);
 #pragma unroll
       for (int c = 0; c < kTile; c += 32) {
@@ -224,8 +241,8 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
         else { pow2_16<false>(x + c, scale, ref, y); pow2_16<false>(x + c + 16, scale, ref, y + 16); }
 #pragma unroll
         for (int e = 0; e < 32; e += 2) sums[(e >> 1) & 3] = __fadd2_rn(sums[(e >> 1) & 3], make_float2(y[e], y[e + 1]));
-        put16<M, TERMS>(at, ts, c, y);
-        put16<M, TERMS>(at, ts, c + 16, y + 16);
+        put16<M, TERMS>(at, lanes, c, y);
+        put16<M, TERMS>(at, lanes, c + 16, y + 16);
         if (TERMS == 1 && c == kTile / 2 - 32) {
           wait_st();
           fence_before();
@@ -239,7 +256,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       arrive(bar(kPFull + t + (TERMS == 1 ? 2 : 0)));
     }
     if (nt > 0) {
-      wait_bar(bar(kOFull + t), 0, failed, &g_packed_error);
+      wait_bar(bar(kOFull + t), G::kEarly ? (nt - 1) & 1 : 0, failed, &g_packed_error);
       fence_after();
     }
     if constexpr (TERMS == 3) { if (nt > 0) add_cols<DW, DW>(to, own); }
@@ -305,9 +322,9 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
 
 // ---- reverse: dq ----------------------------------------------------------------------------------------------------
 // 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256 (float32: the third term of dS
-// at 256, dq at 320).  The two groups of four warps have 64 columns each of every row.  The next tile's logits are made as soon as these have been read, so that its exponentials run
+// at 256, dq at 320; where there is room dS at 256 and dq behind it).  The two groups of four warps have 64 columns each of every row.  The next tile's logits are made as soon as these have been read, so that its exponentials run
 // beside the products dS k and g v^T.
-enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqS, kdqSRead, kdqDp, kdqDs, kdqOut, kdqFix, kDqBars };
+enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqS, kdqSRead, kdqDp, kdqDpRead, kdqDs, kdqDsDone, kdqOut, kdqFix, kDqBars };
 
 template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
@@ -315,7 +332,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   using G = Geometry<TERMS, DW>;
   extern __shared__ unsigned char raw[];
   unsigned char* smem = aligned_smem(raw);
-  const int d = a.d, subs = G::subs(d), tile_bytes = subs * (int)G::kSub, R = G::ring(d);
+  const int d = a.d;
+  constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = G::kRing;
   Tail* tail = reinterpret_cast<Tail*>(smem + (2 + R) * tile_bytes);
   const uint32_t sq = smem_addr(smem), sg = sq + tile_bytes, ring = sg + tile_bytes, bar0 = smem_addr(tail->bars);
   volatile int* failed = &tail->failed;
@@ -329,14 +347,15 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
-    for (int i = 0; i < kDqBars; ++i) init_bar(bar(i), i == kdqSRead || i == kdqDs ? 256 : 1);
+    for (int i = 0; i < kDqBars; ++i) init_bar(bar(i), i == kdqSRead || i == kdqDpRead || i == kdqDs ? 256 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = tail->tmem;
-  constexpr uint32_t kOut = TERMS == 1 ? 256 : 320;
+  constexpr bool E = G::kEarlyDq;
+  constexpr uint32_t kDs = E ? 256 : kTile, kOut = E ? (TERMS == 1 ? 320 : 448) : (TERMS == 1 ? 256 : 320);
 
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
@@ -354,30 +373,38 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       commit(on, bar(kdqDp));
       give(1);
       for (int i = 0; i < n; ++i) {
+        const bool more = i + 1 < n;
         auto logits = [&] {
-          if (i + 1 == n) return;
+          if (!more) return;
           ready(2 * i + 2);
           wait_bar(bar(kdqSRead), i & 1, failed, &g_packed_error);
           fence_after();
           product_rows<M, TERMS, DW>(on, tmem, sq, slot(2 * i + 2), d);
           commit(on, bar(kdqS));
         };
-        if (!G::kShort) logits();
-        wait_bar(bar(kdqDs), i & 1, failed, &g_packed_error);
-        fence_after();
-        product_cols<M, TERMS, DW>(on, tmem + kOut, Packed{{tmem + kTile, tmem + kTile + 32, tmem + 256}, {64, 64, 32}}, slot(2 * i), d, i > 0);
-        give(2 * i);
-        if (G::kShort) logits();
-        if (i + 1 < n) {
+        auto dp = [&] {
+          if (!more) return;
           ready(2 * i + 3);
+          if (E) { wait_bar(bar(kdqDpRead), i & 1, failed, &g_packed_error); fence_after(); }
           product_rows<M, TERMS, DW>(on, tmem + kTile, sg, slot(2 * i + 3), d);
           commit(on, bar(kdqDp));
           give(2 * i + 3);
-        }
+        };
+        if (!G::kShort) logits();
+        if (E) dp();
+        wait_bar(bar(kdqDs), i & 1, failed, &g_packed_error);
+        fence_after();
+        const uint32_t at = tmem + kDs;
+        product_cols<M, TERMS, DW>(on, tmem + kOut, E ? Packed{{at, at + 64, at + 128}, {32, 32, 32}} : Packed{{at, at + 32, tmem + 256}, {64, 64, 32}},
+                                   slot(2 * i), d, i > 0);
+        if (E) commit(on, bar(kdqDsDone));
+        give(2 * i);
+        if (G::kShort) logits();
+        if (!E) dp();
       }
       commit(on, bar(kdqOut));
     } else if (warp == kLoadWarp && n > 0) {
-      Loader<TERMS, DW> ld{lane, subs, bar(kdqFix)};
+      Loader<TERMS, DW> ld{lane, bar(kdqFix)};
       if (lane == 0) {
         expect(bar(kdqQ), 2 * tile_bytes);
         ld.copies(sq, &maps.q, q0 + row0, h, bar(kdqQ));
@@ -402,7 +429,8 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
     float own[kOwn];                         // dq so far (float32), half of the row
 #pragma unroll
     for (int c = 0; c < kOwn; ++c) own[c] = 0.f;
-    const Packed to{{kTile + (uint32_t)col, kTile + 32 + (uint32_t)col, 256 + (uint32_t)col / 2}, {}};
+    const uint32_t c2 = col / 2;
+    const Packed to = E ? Packed{{kDs + c2, kDs + 64 + c2, kDs + 128 + c2}, {}} : Packed{{kDs + (uint32_t)col, kDs + 32 + (uint32_t)col, 256 + c2}, {}};
     const float2 scale = make_float2(a.scale_log2, a.scale_log2), ref = make_float2(e, e);
     for (int i = 0; i < n; ++i) {
       uint32_t x[64], y[64];
@@ -426,6 +454,11 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       ld32(lanes + kTile + col, y);
       ld32(lanes + kTile + col + 32, y + 32);
       wait_ld(y);
+      if (E) {
+        fence_before();
+        arrive(bar(kdqDpRead));
+        if (i > 0) { wait_bar(bar(kdqDsDone), (i - 1) & 1, failed, &g_packed_error); fence_after(); }
+      }
       if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own); }
 #pragma unroll
       for (int c = 0; c < 64; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * (__uint_as_float(y[c]) - delta));
@@ -481,10 +514,10 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
 // ---- reverse: dk and dv ---------------------------------------------------------------------------------------------
 // 128 keys of one key head: rows of the products are keys, columns the queries of all heads of the group, 128 at a time.  Tensor memory:
 // logits at 0 (P replaces them), dP at 128 (dS replaces it), dv at 256, dk at 384 (float32: the third terms of P and dS at 256 and 320, dv
-// at 384, dk at 448).  The tensor cores work in the order
+// at 384, dk at 448; up to 64 values a head in 16 bits: P at 256, dS at 320, dv at 384, dk at 448).  The tensor cores work in the order
 // dv(i), logits(i + 1), dk(i), dP(i + 1): each pair runs beside the other half of the elementwise work.
 enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvFix, kkvStat, kkvStatFree = kkvStat + 2,
-              kDkvBars = kkvStatFree + 2 };
+              kkvSRead = kkvStatFree + 2, kkvDpRead, kkvPDone, kkvDsDone, kDkvBars };
 
 template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
@@ -492,7 +525,8 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   using G = Geometry<TERMS, DW>;
   extern __shared__ unsigned char raw[];
   unsigned char* smem = aligned_smem(raw);
-  const int d = a.d, subs = G::subs(d), tile_bytes = subs * (int)G::kSub, R = G::ring(d);
+  const int d = a.d;
+  constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = G::kRing;
   float* stats = reinterpret_cast<float*>(smem + (2 + R) * tile_bytes);      // [2][128] -lse in log2, [2][128] -delta
   Tail* tail = reinterpret_cast<Tail*>(stats + 4 * kTile);
   const uint32_t sk = smem_addr(smem), sv = sk + tile_bytes, ring = sv + tile_bytes, bar0 = smem_addr(tail->bars);
@@ -510,14 +544,15 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   if (tid == 0) {
     tail->failed = 0;
     for (int i = 0; i < kDkvBars; ++i)
-      init_bar(bar(i), i == kkvP || i == kkvDs ? 256 : i == kkvStat || i == kkvStat + 1 ? 64 : i == kkvStatFree || i == kkvStatFree + 1 ? 8 : 1);
+      init_bar(bar(i), i == kkvP || i == kkvDs || i == kkvSRead || i == kkvDpRead ? 256 : i == kkvStat || i == kkvStat + 1 ? 64 : i == kkvStatFree || i == kkvStatFree + 1 ? 8 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = tail->tmem;
-  constexpr uint32_t kDv = TERMS == 1 ? 256 : 384, kDk = TERMS == 1 ? 384 : 448;
+  constexpr bool E = G::kEarly;
+  constexpr uint32_t kP = E ? 256 : 0, kDs = E ? 320 : kTile, kDv = E || TERMS == 3 ? 384 : 256, kDk = E || TERMS == 3 ? 448 : 384;
 
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
@@ -534,31 +569,41 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(1), d);
       commit(on, bar(kkvDp));
       for (int i = 0; i < n; ++i) {
-        wait_bar(bar(kkvP), i & 1, failed, &g_packed_error);
-        fence_after();
-        product_cols<M, TERMS, DW>(on, tmem + kDv, Packed{{tmem, tmem + 32, tmem + 256}, {64, 64, 32}}, slot(2 * i + 1), d, i > 0);
-        give(2 * i + 1);
+        const bool more = i + 1 < n;
         auto logits = [&] {
-          if (i + 1 == n) return;
+          if (!more) return;
           ready(2 * i + 2);
+          if (E) { wait_bar(bar(kkvSRead), i & 1, failed, &g_packed_error); fence_after(); }
           product_rows<M, TERMS, DW>(on, tmem, sk, slot(2 * i + 2), d);
           commit(on, bar(kkvS));
         };
-        if (!G::kShort) logits();
-        wait_bar(bar(kkvDs), i & 1, failed, &g_packed_error);
-        fence_after();
-        product_cols<M, TERMS, DW>(on, tmem + kDk, Packed{{tmem + kTile, tmem + kTile + 32, tmem + 320}, {64, 64, 32}}, slot(2 * i), d, i > 0);
-        give(2 * i);
-        if (G::kShort) logits();
-        if (i + 1 < n) {
+        auto dp = [&] {
+          if (!more) return;
           ready(2 * i + 3);
+          if (E) { wait_bar(bar(kkvDpRead), i & 1, failed, &g_packed_error); fence_after(); }
           product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(2 * i + 3), d);
           commit(on, bar(kkvDp));
-        }
+        };
+        auto packed_at = [&](uint32_t at, uint32_t third) { return E ? Packed{{at}, {32}} : Packed{{at, at + 32, third}, {64, 64, 32}}; };
+        if (E) logits();
+        wait_bar(bar(kkvP), i & 1, failed, &g_packed_error);
+        fence_after();
+        product_cols<M, TERMS, DW>(on, tmem + kDv, packed_at(tmem + kP, tmem + 256), slot(2 * i + 1), d, i > 0);
+        if (E) commit(on, bar(kkvPDone));
+        give(2 * i + 1);
+        if (!E && !G::kShort) logits();
+        if (E) dp();
+        wait_bar(bar(kkvDs), i & 1, failed, &g_packed_error);
+        fence_after();
+        product_cols<M, TERMS, DW>(on, tmem + kDk, packed_at(tmem + kDs, tmem + 320), slot(2 * i), d, i > 0);
+        if (E) commit(on, bar(kkvDsDone));
+        give(2 * i);
+        if (G::kShort) logits();
+        if (!E) dp();
       }
       commit(on, bar(kkvOut));
     } else if (warp == kLoadWarp && n > 0) {
-      Loader<TERMS, DW> ld{lane, subs, bar(kkvFix)};
+      Loader<TERMS, DW> ld{lane, bar(kkvFix)};
       if (lane == 0) {
         expect(bar(kkvK), 2 * tile_bytes);
         ld.copies(sk, &maps.k, c0 + row0, kvh, bar(kkvK));
@@ -595,8 +640,9 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
 #pragma unroll
     for (int c = 0; c < kOwn; ++c) own[0][c] = own[1][c] = 0.f;
     const float2 scale = make_float2(a.scale_log2, a.scale_log2);
-    const Packed to_p{{(uint32_t)col, 32 + (uint32_t)col, 256 + (uint32_t)col / 2}, {}},
-        to_s{{kTile + (uint32_t)col, kTile + 32 + (uint32_t)col, 320 + (uint32_t)col / 2}, {}};
+    const uint32_t c2 = col / 2;
+    const Packed to_p = E ? Packed{{kP + c2}, {}} : Packed{{kP + (uint32_t)col, kP + 32 + (uint32_t)col, 256 + c2}, {}};
+    const Packed to_s = E ? Packed{{kDs + c2}, {}} : Packed{{kDs + (uint32_t)col, kDs + 32 + (uint32_t)col, 320 + c2}, {}};
     for (int i = 0; i < n; ++i) {
       const int st = i & 1, ib = i0 + ((j0 + i) % per) * kTile + col;
       uint32_t x[64], y[64];
@@ -606,6 +652,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       ld32(lanes + col, x);
       ld32(lanes + col + 32, x + 32);
       wait_ld(x);
+      if (E) { fence_before(); arrive(bar(kkvSRead)); }
       if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDv + half * (DW / 2), own[0]); }
       const float4* e = reinterpret_cast<const float4*>(stats + st * kTile + col);
 #pragma unroll
@@ -617,6 +664,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         x[4 * c] = __float_as_uint(pow2(z0.x)); x[4 * c + 1] = __float_as_uint(pow2(z0.y));
         x[4 * c + 2] = __float_as_uint(r1.x); x[4 * c + 3] = __float_as_uint(r1.y);
       }
+      if (E && i > 0) { wait_bar(bar(kkvPDone), (i - 1) & 1, failed, &g_packed_error); fence_after(); }
       if (a.causal && ib < lim_last) {
 #pragma unroll
         for (int c = 0; c < 64; ++c) if (ib + c < lim) x[c] = 0;
@@ -636,6 +684,11 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       ld32(lanes + kTile + col, y);
       ld32(lanes + kTile + col + 32, y + 32);
       wait_ld(y);
+      if (E) {
+        fence_before();
+        arrive(bar(kkvDpRead));
+        if (i > 0) { wait_bar(bar(kkvDsDone), (i - 1) & 1, failed, &g_packed_error); fence_after(); }
+      }
       if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDk + half * (DW / 2), own[1]); }
       const float4* dl = reinterpret_cast<const float4*>(stats + (2 + st) * kTile + col);
       constexpr float un = packed::prob_unscale<T>();
@@ -832,7 +885,7 @@ template <typename T, int TERMS, int DW> int maps_of(Maps* m, cudaStream_t st, c
 }
 template <int TERMS, int DW, auto kernel> int launch(int64_t grid, bool stats, cudaStream_t st, const PackedArgs& a, const Maps& m) {
   using G = Geometry<TERMS, DW>;
-  const int smem = 1024 + (2 + G::ring(a.d)) * G::subs(a.d) * (int)G::kSub + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail);
+  const int smem = 1024 + (2 + G::kRing) * G::kSubs * (int)G::kSub + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail);
   packed::allow_smem<kernel>(smem);
   if (grid > 0x7fffffff) return kTooLarge;
   kernel<<<(unsigned)grid, kThreads, smem, st>>>(a, m);
@@ -885,12 +938,13 @@ int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, cons
 }  // namespace
 
 template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace) {
-  if constexpr (sizeof(T) == 2) return forward_of<T, 1, 64>(st, a, n_items, pieces, workspace);
+  if constexpr (sizeof(T) == 2) return a.d <= 64 ? forward_of<T, 1, 64>(st, a, n_items, pieces, workspace) : forward_of<T, 1, 128>(st, a, n_items, pieces, workspace);
   else return a.d <= 32 ? forward_of<T, 3, 32>(st, a, n_items, pieces, workspace) : forward_of<T, 3, 64>(st, a, n_items, pieces, workspace);
 }
 template <typename T>
 int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, const PackedPieces& pieces, void* workspace) {
-  if constexpr (sizeof(T) == 2) return reverse_of<T, 1, 64>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace);
+  if constexpr (sizeof(T) == 2) return a.d <= 64 ? reverse_of<T, 1, 64>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace)
+                                                 : reverse_of<T, 1, 128>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace);
   else return a.d <= 32 ? reverse_of<T, 3, 32>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace)
                         : reverse_of<T, 3, 64>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace);
 }

@@ -97,17 +97,20 @@ template <bool POLY> __device__ __forceinline__ void pow2_16(const uint32_t* x, 
 }
 
 // ---- matrix instructions ----
-// Geometry of operand tiles.  TERMS = 1: 16-bit values, sub-tiles of 64 values (128-byte rows and swizzle), one or two.  TERMS = 3: float32
+// Geometry of operand tiles.  TERMS = 1: 16-bit values, sub-tiles of 64 values (128-byte rows and swizzle), one for DW = 64, two for 128.  TERMS = 3: float32
 // values split into three bfloat16 terms, x = t0 + t1 + t2 to 2^-24, a sub-tile per term of DW = 32 or 64 values (64- or 128-byte rows and
 // swizzle).  A product of two such operands takes the six products of terms that are above 2^-24 of it, small ones first.
 template <int TERMS, int DW> struct Geometry {
   static constexpr int kRow = TERMS == 1 ? 128 : 2 * DW;      // bytes of a row
   static constexpr uint32_t kSub = kTile * kRow;              // bytes of a sub-tile
-  static __device__ __host__ __forceinline__ int subs(int d) { return TERMS == 1 ? (d > 64 ? 2 : 1) : 3; }
+  static constexpr int kSubs = TERMS == 1 ? DW / 64 : 3;
   // Tiles that stream through: a ring, the two kinds of tile in turn; tile j sits in slot j % R.
-  static __device__ __host__ __forceinline__ int ring(int d) { return TERMS == 1 ? (d > 64 ? 4 : 8) : DW == 32 ? 6 : 2; }
+  static constexpr int kRing = TERMS == 1 ? (DW == 128 ? 4 : 8) : DW == 32 ? 6 : 2;
   // a ring of one tile of each kind: the reverse kernels make the next logits only behind the product that reads the tile in its slot
   static constexpr bool kShort = TERMS == 3 && DW == 64;
+  // Where tensor memory has room for P and dS beside the logits and dP they are made from, the next tile's logits are made as soon as these
+  // have been read, and not behind the product that reads P: a product's way through barriers and back is longer than itself.
+  static constexpr bool kEarly = TERMS == 1 && DW == 64, kEarlyDq = kEarly || (TERMS == 3 && DW == 32);
   // Descriptor: its low word holds the address, so that steps are additions to it; the high word is a constant.  K-major: 16 contracted values
   // are 32 bytes further, 64 are a sub-tile further; groups of eight rows lie 8 rows apart.  MN-major: 16 contracted rows are 16 rows
   // further, the next values of N a sub-tile.
@@ -146,7 +149,7 @@ template <typename T, int TERMS, int DW> __device__ __forceinline__ void product
   if constexpr (TERMS == 1) {
     const int steps = d / 16;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < DW / 16; ++k)
       if (k < steps) mma_ss<G::kHigh>(on, dst, la + G::step_k(k), lb + G::step_k(k), id, k > 0);
   } else {
 #pragma unroll
@@ -255,7 +258,8 @@ __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
 // (through `fix`, a barrier of this warp's own, and its parity).
 template <int TERMS, int DW> struct Loader {
   static constexpr uint32_t kSub = Geometry<TERMS, DW>::kSub;
-  int lane, subs;
+  static constexpr int subs = Geometry<TERMS, DW>::kSubs;
+  int lane;
   uint32_t fix, parity = 0;
   __device__ __forceinline__ void copies(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t bar) const {
     for (int x = 0; x < subs; ++x) tma(dst + x * kSub, map, TERMS == 1 ? 64 * x : 0, row, TERMS == 1 ? head : 3 * head + x, bar);
