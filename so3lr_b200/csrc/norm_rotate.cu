@@ -136,16 +136,38 @@ __device__ __forceinline__ void weight_table(const RotateArgs& A, float* w) {
   }
 }
 
-// W lanes per row (the next power of two of the parts), `slots` heads of a token side by side, then tokens
+// Heads of queries and keys as one range [0, heads of both): side, row piece and weights of head h
+template <typename T> struct Head {
+  int side, h;
+  bool there;
+  __device__ __forceinline__ Head(const RotateArgs& A, int i) : side(i >= A.heads[0]), h(i - (i >= A.heads[0] ? A.heads[0] : 0)), there(i < A.heads[0] + A.heads[1]) {}
+};
+
+// W lanes per row (the next power of two of the parts), `slots` heads of a token side by side, then tokens.  The next heads' rows are
+// asked for before the present ones are worked on, the first ones before the angles are formed.
 template <typename T, bool NEIGHBORS, bool NORM, int U>
-__global__ void __launch_bounds__(kThreads, 3) forward_kernel(const RotateArgs A, int W) {
+__global__ void __launch_bounds__(kThreads, 4) forward_kernel(const RotateArgs A, int W) {
   using P = Piece<T, NEIGHBORS>;
   constexpr int N = Vec<T>::N;
   const int part = threadIdx.x % W, group = threadIdx.x / W, slot = group % A.slots;
-  const int per = kThreads / W / A.slots, token = blockIdx.x * per + group / A.slots;
+  const int per = kThreads / W / A.slots, token = blockIdx.x * per + group / A.slots, heads = A.heads[0] + A.heads[1];
   const bool on = token < A.n && part * N < A.d / 2;
   const int oa = P::off_a(part, A.d), ob = P::off_b(part, A.d);
   extern __shared__ __align__(16) float table[];
+  uint4 u[U], v[U];
+  auto load = [&](int hb) {
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const Head<T> h(A, hb + slot + k * A.slots);
+      u[k] = v[k] = make_uint4(0, 0, 0, 0);
+      if (on && h.there) {
+        const T* src = static_cast<const T*>(A.x[h.side].p) + (long long)token * A.x[h.side].row + h.h * A.x[h.side].head;
+        u[k] = __ldcs(reinterpret_cast<const uint4*>(src + oa));
+        v[k] = __ldcs(reinterpret_cast<const uint4*>(src + ob));
+      }
+    }
+  };
+  load(0);
   float c[N], s[N];
   if (NORM) weight_table<T, NEIGHBORS>(A, table + per * A.d);
   angle_table(A, blockIdx.x * per, per, table, table + per * (A.d / 2));
@@ -155,54 +177,41 @@ __global__ void __launch_bounds__(kThreads, 3) forward_kernel(const RotateArgs A
     take<N>(table, at, c);
     take<N>(table + per * (A.d / 2), at, s);
   }
+  for (int hb = 0; hb < heads; hb += U * A.slots) {      // the same trips for all lanes: the sums below are over a warp
+    float a[U][N], b[U][N];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    const Rows x = A.x[side];
-    const T* src = static_cast<const T*>(x.p) + (long long)token * x.row;
-    T* dst = static_cast<T*>(A.out[side]) + (long long)token * A.heads[side] * A.d;
-    const float* w = table + per * A.d + side * A.d + part * 2 * N;
-    for (int hb = 0; hb < A.heads[side]; hb += U * A.slots) {      // the same trips for all lanes: the sums below are over a warp
-      const int h0 = hb + slot;
-      uint4 u[U], v[U];
+    for (int k = 0; k < U; ++k) P::split(u[k], v[k], a[k], b[k]);
+    if (hb + U * A.slots < heads) load(hb + U * A.slots);
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int h = h0 + k * A.slots;
-        u[k] = v[k] = make_uint4(0, 0, 0, 0);
-        if (on && h < A.heads[side]) {
-          u[k] = __ldg(reinterpret_cast<const uint4*>(src + h * x.head + oa));
-          v[k] = __ldg(reinterpret_cast<const uint4*>(src + h * x.head + ob));
+    for (int k = 0; k < U; ++k) {
+      const Head<T> h(A, hb + slot + k * A.slots);
+      if (NORM) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) ss = fmaf(a[k][i], a[k][i], fmaf(b[k][i], b[k][i], ss));
+        for (int o = W >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = 1.f / sqrtf(ss / A.d + A.eps);
+        if (on) {
+          const float* w = table + per * A.d + h.side * A.d + part * 2 * N;
+          float wa[N], wb[N];
+          take<N>(w, 0, wa);
+          take<N>(w, N, wb);
+#pragma unroll
+          for (int i = 0; i < N; ++i) { a[k][i] *= r * wa[i]; b[k][i] *= r * wb[i]; }
         }
       }
+      if (on && h.there) {
+        T* dst = static_cast<T*>(A.out[h.side]) + ((long long)token * A.heads[h.side] + h.h) * A.d;
 #pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int h = h0 + k * A.slots;
-        float a[N], b[N];
-        P::split(u[k], v[k], a, b);
-        if (NORM) {
-          float ss = 0.f;
-#pragma unroll
-          for (int i = 0; i < N; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-          for (int o = W >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          const float r = 1.f / sqrtf(ss / A.d + A.eps);
-          if (on) {
-            float wa[N], wb[N];
-            take<N>(w, 0, wa);
-            take<N>(w, N, wb);
-#pragma unroll
-            for (int i = 0; i < N; ++i) { a[i] *= r * wa[i]; b[i] *= r * wb[i]; }
-          }
+        for (int i = 0; i < N; ++i) {
+          const float t = a[k][i] * c[i] - b[k][i] * s[i];
+          b[k][i] = a[k][i] * s[i] + b[k][i] * c[i];
+          a[k][i] = t;
         }
-        if (on && h < A.heads[side]) {
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float t = a[i] * c[i] - b[i] * s[i];
-            b[i] = a[i] * s[i] + b[i] * c[i];
-            a[i] = t;
-          }
-          P::join(a, b, u[k], v[k]);
-          *reinterpret_cast<uint4*>(dst + (long long)h * A.d + oa) = u[k];
-          *reinterpret_cast<uint4*>(dst + (long long)h * A.d + ob) = v[k];
-        }
+        uint4 x, y;
+        P::join(a[k], b[k], x, y);
+        *reinterpret_cast<uint4*>(dst + oa) = x;
+        *reinterpret_cast<uint4*>(dst + ob) = y;
       }
     }
   }
@@ -210,22 +219,36 @@ __global__ void __launch_bounds__(kThreads, 3) forward_kernel(const RotateArgs A
 
 // CTAs walk over tiles of tokens; the shares of dw of a CTA end in one row of A.part.  The sums have a fixed order.
 template <typename T, bool NEIGHBORS, bool NORM>
-__global__ void __launch_bounds__(kThreads, 2) reverse_kernel(const RotateArgs A, int W) {
+__global__ void __launch_bounds__(kThreads, 3) reverse_kernel(const RotateArgs A, int W) {
   using P = Piece<T, NEIGHBORS>;
   constexpr int N = Vec<T>::N;
   extern __shared__ __align__(16) float table[];
   __shared__ float th[kThreads * N];                     // dtheta of every thread
   __shared__ float sw[kThreads / 32][2 * N * 32];        // dw of the warps, one side at a time
-  const int part = threadIdx.x % W, group = threadIdx.x / W, slot = group % A.slots, per = kThreads / W / A.slots;
+  const int part = threadIdx.x % W, group = threadIdx.x / W, slot = group % A.slots, per = kThreads / W / A.slots, heads = A.heads[0] + A.heads[1];
   const bool there = part * N < A.d / 2;
   const int oa = P::off_a(part, A.d), ob = P::off_b(part, A.d);
   float dwa[2][N], dwb[2][N];
 #pragma unroll
   for (int i = 0; i < N; ++i) dwa[0][i] = dwa[1][i] = dwb[0][i] = dwb[1][i] = 0.f;
   if (NORM) weight_table<T, NEIGHBORS>(A, table + per * A.d);
+  uint4 u, v, gu, gv;
+  auto load = [&](int token, int hb) {
+    const Head<T> h(A, hb + slot);
+    u = v = gu = gv = make_uint4(0, 0, 0, 0);
+    if (token < A.n && there && h.there) {
+      const T* src = static_cast<const T*>(A.x[h.side].p) + (long long)token * A.x[h.side].row + h.h * A.x[h.side].head;
+      const T* gsrc = static_cast<const T*>(A.g[h.side].p) + (long long)token * A.g[h.side].row + h.h * A.g[h.side].head;
+      u = __ldcs(reinterpret_cast<const uint4*>(src + oa));
+      v = __ldcs(reinterpret_cast<const uint4*>(src + ob));
+      gu = __ldcs(reinterpret_cast<const uint4*>(gsrc + oa));
+      gv = __ldcs(reinterpret_cast<const uint4*>(gsrc + ob));
+    }
+  };
   for (int t0 = blockIdx.x * per; t0 < A.n; t0 += gridDim.x * per) {
     const int token = t0 + group / A.slots;
     const bool on = token < A.n && there;
+    load(token, 0);
     float c[N], s[N], dth[N];
 #pragma unroll
     for (int i = 0; i < N; ++i) dth[i] = 0.f;
@@ -236,64 +259,56 @@ __global__ void __launch_bounds__(kThreads, 2) reverse_kernel(const RotateArgs A
       take<N>(table, at, c);
       take<N>(table + per * (A.d / 2), at, s);
     }
+    for (int hb = 0; hb < heads; hb += A.slots) {      // the same trips for all lanes: the sums below are over a warp
+      const Head<T> h(A, hb + slot);
+      float a[N], b[N], ga[N], gb[N];
+      P::split(u, v, a, b);
+      P::split(gu, gv, ga, gb);
+      if (hb + A.slots < heads) load(token, hb + A.slots);
+      float r = 1.f, dot = 0.f;
+      if (NORM) {
+        float ss = 0.f;
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const Rows x = A.x[side], g = A.g[side];
-      const T* src = static_cast<const T*>(x.p) + (long long)token * x.row;
-      const T* gsrc = static_cast<const T*>(g.p) + (long long)token * g.row;
-      T* dst = static_cast<T*>(A.dx[side]) + (long long)token * A.heads[side] * A.d;
-      const float* w = table + per * A.d + side * A.d + part * 2 * N;
-      for (int hb = 0; hb < A.heads[side]; hb += A.slots) {      // the same trips for all lanes: the sums below are over a warp
-        const int h = hb + slot;
-        const bool mine = on && h < A.heads[side];
-        uint4 u = make_uint4(0, 0, 0, 0), v = u, gu = u, gv = u;
-        if (mine) {
-          u = __ldg(reinterpret_cast<const uint4*>(src + h * x.head + oa));
-          v = __ldg(reinterpret_cast<const uint4*>(src + h * x.head + ob));
-          gu = __ldg(reinterpret_cast<const uint4*>(gsrc + h * g.head + oa));
-          gv = __ldg(reinterpret_cast<const uint4*>(gsrc + h * g.head + ob));
-        }
-        float a[N], b[N], ga[N], gb[N];
-        P::split(u, v, a, b);
-        P::split(gu, gv, ga, gb);
-        float r = 1.f, dot = 0.f;
+        for (int i = 0; i < N; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+        for (int o = W >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        r = 1.f / sqrtf(ss / A.d + A.eps);
+      }
+      if (on) {
+        float wa[N], wb[N];
         if (NORM) {
-          float ss = 0.f;
+          const float* w = table + per * A.d + h.side * A.d + part * 2 * N;
+          take<N>(w, 0, wa);
+          take<N>(w, N, wb);
+        }
 #pragma unroll
-          for (int i = 0; i < N; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-          for (int o = W >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-          r = 1.f / sqrtf(ss / A.d + A.eps);
-        }
-        if (on) {
-          float wa[N], wb[N];
-          if (NORM) { take<N>(w, 0, wa); take<N>(w, N, wb); }
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const float xa = a[i] * r, xb = b[i] * r, ya = NORM ? xa * wa[i] : xa, yb = NORM ? xb * wb[i] : xb;
-            const float o1 = ya * c[i] - yb * s[i], o2 = ya * s[i] + yb * c[i];
-            dth[i] = fmaf(gb[i], o1, fmaf(-ga[i], o2, dth[i]));
-            float va = ga[i] * c[i] + gb[i] * s[i], vb = gb[i] * c[i] - ga[i] * s[i];
-            if (NORM) {
-              dwa[side][i] = fmaf(va, xa, dwa[side][i]); dwb[side][i] = fmaf(vb, xb, dwb[side][i]);
-              va *= wa[i]; vb *= wb[i];
-              dot = fmaf(va, xa, fmaf(vb, xb, dot));
-            }
-            a[i] = xa; b[i] = xb; ga[i] = va; gb[i] = vb;
-          }
-        }
-        if (NORM) {
-          for (int o = W >> 1; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
-          dot /= A.d;
-        }
-        if (mine) {
+        for (int i = 0; i < N; ++i) {
+          const float xa = a[i] * r, xb = b[i] * r, ya = NORM ? xa * wa[i] : xa, yb = NORM ? xb * wb[i] : xb;
+          const float o1 = ya * c[i] - yb * s[i], o2 = ya * s[i] + yb * c[i];
+          dth[i] = fmaf(gb[i], o1, fmaf(-ga[i], o2, dth[i]));
+          float va = ga[i] * c[i] + gb[i] * s[i], vb = gb[i] * c[i] - ga[i] * s[i];
           if (NORM) {
-#pragma unroll
-            for (int i = 0; i < N; ++i) { ga[i] = r * (ga[i] - a[i] * dot); gb[i] = r * (gb[i] - b[i] * dot); }
+            const float pa = va * xa, pb = vb * xb;
+            if (h.side) { dwa[1][i] += pa; dwb[1][i] += pb; } else { dwa[0][i] += pa; dwb[0][i] += pb; }
+            va *= wa[i]; vb *= wb[i];
+            dot = fmaf(va, xa, fmaf(vb, xb, dot));
           }
-          P::join(ga, gb, gu, gv);
-          *reinterpret_cast<uint4*>(dst + (long long)h * A.d + oa) = gu;
-          *reinterpret_cast<uint4*>(dst + (long long)h * A.d + ob) = gv;
+          a[i] = xa; b[i] = xb; ga[i] = va; gb[i] = vb;
         }
+      }
+      if (NORM) {
+        for (int o = W >> 1; o; o >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, o);
+        dot /= A.d;
+      }
+      if (on && h.there) {
+        T* dst = static_cast<T*>(A.dx[h.side]) + ((long long)token * A.heads[h.side] + h.h) * A.d;
+        if (NORM) {
+#pragma unroll
+          for (int i = 0; i < N; ++i) { ga[i] = r * (ga[i] - a[i] * dot); gb[i] = r * (gb[i] - b[i] * dot); }
+        }
+        uint4 x, y;
+        P::join(ga, gb, x, y);
+        *reinterpret_cast<uint4*>(dst + oa) = x;
+        *reinterpret_cast<uint4*>(dst + ob) = y;
       }
     }
     if (A.dpos) {
@@ -370,22 +385,26 @@ __global__ void __launch_bounds__(256) weight_kernel(const RotateArgs A, int row
 }
 
 int next_pow2(int x) { int p = 1; while (p < x) p <<= 1; return p; }
-// lanes per row, and heads of a token that run side by side: as few as keep the chip's threads busy twice over
-void shape(RotateArgs& A, int value_bytes, int& W) {
+// Lanes per row, and heads of a token that run side by side: as few as give every SM `busy` threads.  A thread with several heads asks for
+// the next one's rows while it works on the present one, and the angles of a token are formed once for all of them; more threads hide more.
+// 32,771 rows of 40 heads x 128 forward, busy 1,024 / 2,048 / 4,096: 155 / 147 / 139 us (4.8 TB/s; a copy of the bytes takes 103); 16,411
+// rows of 32 heads x 64 reverse, 512 / 1,024 / 2,048: 56 / 47 / 53 us; 12,803 rows of 8 heads x 32 float32 reverse: 16 / 19 / 28.
+void shape(RotateArgs& A, int value_bytes, bool reverse, int& W) {
   W = next_pow2(A.d / 2 / (16 / value_bytes));
-  const int heads = A.heads[0] > A.heads[1] ? A.heads[0] : A.heads[1];
+  const int heads = A.heads[0] + A.heads[1];
   const int most = next_pow2(heads < 1 ? 1 : heads) < kThreads / W ? next_pow2(heads < 1 ? 1 : heads) : kThreads / W;
+  const long long busy = reverse ? 1024 : 4096;
   A.slots = 1;
-  while (A.slots < most && (long long)A.n * W * A.slots < 2LL * sm_count() * 2048) A.slots <<= 1;
+  while (A.slots < most && (long long)A.n * W * A.slots < busy * sm_count()) A.slots <<= 1;
 }
 
 template <typename T, bool NEIGHBORS, bool NORM>
 void rotate_launch(cudaStream_t st, RotateArgs A, bool reverse, int grid_max) {
   int W;
-  shape(A, sizeof(T), W);
+  shape(A, sizeof(T), reverse, W);
   const int per = kThreads / W / A.slots, tiles = (A.n + per - 1) / per, smem = (per + 2) * A.d * (int)sizeof(float);
   if (!reverse) {
-    forward_kernel<T, NEIGHBORS, NORM, 2><<<tiles, kThreads, smem, st>>>(A, W);
+    forward_kernel<T, NEIGHBORS, NORM, 1><<<tiles, kThreads, smem, st>>>(A, W);
     count_launch();
     return;
   }
@@ -418,7 +437,7 @@ bool rows_ok(const so3lr_b200_rows* r, int type, int heads) {
   return r && r->data && reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->row_stride % unit == 0 && r->head_stride % unit == 0;
 }
 Rows rows_of(const so3lr_b200_rows* r) { return r ? Rows{r->data, r->row_stride, r->head_stride} : Rows{}; }
-int grid_limit() { return 4 * sm_count(); }
+int grid_limit() { return 3 * sm_count(); }      // CTAs of the reverse kernel that are resident at a time
 
 }  // namespace
 }  // namespace so3lr

@@ -127,6 +127,7 @@ PackedArgs common(const int32_t* im, const int32_t* dev, const so3lr_b200_attent
   PackedArgs p;
   p.start_q = dev + im[kStartQ]; p.start_kv = dev + im[kStartKv]; p.split_first = dev + im[kSplitFirst];
   p.rows = im[kRowsQ]; p.rows_kv = im[kRowsKv];
+  p.stages = im[kMaxKv] <= (a->type == kF32 && a->d > 64 ? 32 : 64) ? 1 : 2;
   p.nq = (int)a->rows_q; p.nkv = (int)a->rows_kv; p.hq = a->heads_q; p.hk = a->heads_kv; p.group = a->heads_q / a->heads_kv; p.d = a->d; p.causal = im[kCausal];
   p.scale = a->scale; p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   return p;
@@ -141,12 +142,19 @@ int64_t part_floats(const int32_t* im, const so3lr_b200_attention_shape* a) {
   return (int64_t)im[kNItemsSplit] * a->heads_kv * im[kMaxQ] * (a->heads_q / a->heads_kv) * packed_padded(a->d);
 }
 
-// Structures of this many rows go to the tensor cores.
-#ifndef SO3LR_PACKED_TC_ROWS
-#define SO3LR_PACKED_TC_ROWS 128
-#endif
+// Batches whose longest structure has this many rows on both sides go to the tensor-core kernels, whose CTAs take 6 us to start and end and
+// whose tiles hold 128 rows.  Forward and backward together in us, tensor cores / warp-level, about 8,200 rows in structures between half
+// and all of the longest, which has L rows:
+//   16-bit, 4 heads x 32:   L = 512  69 / 65,    1,024  81 / 116     float32, 4 x 32:  L = 192  93 / 92,   256 101 / 117
+//   16-bit, 8 x 64:         L = 192 107 / 94,      256 102 / 107     float32, 8 x 64:  L = 96 263 / 245,   128 230 / 255
+//   16-bit, 8 x 128:        L = 96  150 / 155,     128 128 / 161     (float32 above 64 values has warp-level kernels only)
+int tensor_core_rows(int type, int d) {
+  if (type == kF32) return d <= 32 ? 200 : d <= 64 ? 128 : 0x7fffffff;
+  return d <= 32 ? 600 : d <= 64 ? 256 : 100;
+}
 bool on_tensor_cores(const int32_t* im, const so3lr_b200_attention_shape* a) {
-  return (a->type != kF32 || a->d <= 64) && im[kMaxQ] >= SO3LR_PACKED_TC_ROWS && im[kMaxKv] >= SO3LR_PACKED_TC_ROWS;
+  const int rows = tensor_core_rows(a->type, a->d);
+  return im[kMaxQ] >= rows && im[kMaxKv] >= rows;
 }
 // Into how many pieces the walks of a kernel's items are cut.  With few CTAs for the chip the last round of them leaves most SMs idle (160
 // equal ones on 148: half of the time), so the time is that of the work on all SMs, plus half of a CTA that ends last, plus what a CTA costs

@@ -37,6 +37,7 @@ struct PackedArgs {
   int pieces = 1;               // tensor-core kernels: pieces that an item's walk is cut into; each leaves its share in part_o / part_ml or
   float* share[3] = {};         // (reverse) in share: (pieces, heads, rows, d) of dq, dk, dv
   int rows = 0, rows_kv = 0;    // of the layout
+  int stages = 2;               // buffers for the keys in the warp-level forward kernel: one where they all fit into it
   int nq = 0, nkv = 0, hq = 0, hk = 0, group = 1, d = 0, causal = 0;
   float scale = 0.f, scale_log2 = 0.f;                // scale * log2(e): the softmax runs on powers of two
   int* err = nullptr;

@@ -247,7 +247,7 @@ __device__ __forceinline__ void store_rest(T* p, T* rest, float x, float y) {
 }
 
 template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 4 && DP > 64 ? 32 : 64; }
-template <typename T, int DP> constexpr int forward_smem() { return (kPackTile + 4 * key_tile<T, DP>()) * Tile<T, DP>::kStride; }
+template <typename T, int DP> int forward_smem(int stages) { return (kPackTile + 2 * stages * key_tile<T, DP>()) * Tile<T, DP>::kStride; }
 constexpr int kRevTile = 32;   // rows of the walked side in the reverse kernels: two accumulators of 16 x DP are held at the same time
 template <typename T, int DP> constexpr int reverse_smem() { return (2 * kPackTile + 4 * kRevTile) * Tile<T, DP>::kStride + 4 * kRevTile * 4; }
 
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
   using L = Tile<T, DP>;
   constexpr int BN = key_tile<T, DP>(), NT = BN / 8;
   extern __shared__ __align__(16) unsigned char smem[];
-  const uint32_t sq = smem_addr(smem), sk = sq + kPackTile * L::kStride, sv = sk + 2 * BN * L::kStride;
+  const uint32_t sq = smem_addr(smem), sk = sq + kPackTile * L::kStride;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int heads = SPLIT ? a.hk : a.hq, unit = blockIdx.x / heads;
   const int4 item = a.items[unit];
@@ -267,7 +267,8 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
   const int G = SPLIT ? a.group : 1, hy = blockIdx.x % heads, kvh = SPLIT ? hy : hy / a.group;
   const int rows = lq * G, row0 = SPLIT ? 0 : item.y * kPackTile;
   const int k0 = item.z, k1 = item.w;
-  const int nt = (max(k1 - k0, 0) + BN - 1) / BN;
+  const int nt = (max(k1 - k0, 0) + BN - 1) / BN, stages = a.stages;
+  const uint32_t sv = sk + stages * BN * L::kStride;
 
   {  // queries
     const T* p = static_cast<const T*>(a.q.p);
@@ -281,7 +282,7 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
   }
   auto load = [&](int it) {
     if (it < nt) {
-      const int buf = it & 1, b = k0 + it * BN;
+      const int buf = it & (stages - 1), b = k0 + it * BN;
       load_rows<T, DP, BN>(sk + buf * BN * L::kStride, a.k, kvh, c0, b, k1, a.d, tid);
       load_rows<T, DP, BN>(sv + buf * BN * L::kStride, a.v, kvh, c0, b, k1, a.d, tid);
     }
@@ -299,10 +300,9 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
   for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
   for (int it = 0; it < nt; ++it) {
-    load(it + 1);
-    copy_wait<1>();
+    if (stages == 2) { load(it + 1); copy_wait<1>(); } else { if (it > 0) load(it); copy_wait<0>(); }
     __syncthreads();
-    const int kb = k0 + it * BN, buf = it & 1;
+    const int kb = k0 + it * BN, buf = it & (stages - 1);
     if (wr < rows && kb <= lim_hi) {
       float p[NT][4];
       const int cols = k1 - kb;
@@ -766,7 +766,7 @@ int launch(int64_t grid, int threads, int smem, cudaStream_t st, const PackedArg
 }  // namespace packed
 
 template <typename T> int packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) return packed::launch<packed::forward_kernel<T, DP, false>>((int64_t)n_items * a.hq, 128, packed::forward_smem<T, DP>(), st, a);
+#define CALL(T, DP) return packed::launch<packed::forward_kernel<T, DP, false>>((int64_t)n_items * a.hq, 128, packed::forward_smem<T, DP>(a.stages), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
@@ -774,7 +774,7 @@ template <typename T> int packed_forward_split(cudaStream_t st, const PackedArgs
 #define CALL(T, DP)                                                                                                                           \
   const int rc = a.part_rows <= packed::kNarrowRows                                                                                           \
                      ? packed::launch<packed::narrow_kernel<T, DP>>((int64_t)n_items * a.hk, 128, packed::narrow_smem<T, DP>(), st, a)        \
-                     : packed::launch<packed::forward_kernel<T, DP, true>>((int64_t)n_items * a.hk, 128, packed::forward_smem<T, DP>(), st, a); \
+                     : packed::launch<packed::forward_kernel<T, DP, true>>((int64_t)n_items * a.hk, 128, packed::forward_smem<T, DP>(a.stages), st, a); \
   return rc || !combine ? rc : packed::launch<packed::combine_kernel<T, DP>>((int64_t)n_structures * a.hk, 256, 0, st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL

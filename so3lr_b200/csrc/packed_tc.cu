@@ -660,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         const float4 v = e[c];
         const float2 z0 = __ffma2_rn(make_float2(__uint_as_float(x[4 * c]), __uint_as_float(x[4 * c + 1])), scale, make_float2(v.x, v.y));
         const float2 z1 = __ffma2_rn(make_float2(__uint_as_float(x[4 * c + 2]), __uint_as_float(x[4 * c + 3])), scale, make_float2(v.z, v.w));
-        const float2 r1 = TERMS == 1 && (c & 1) ? pow2_poly(z1) : make_float2(pow2(z1.x), pow2(z1.y));
+        const float2 r1 = TERMS == 1 ? pow2_poly(z1) : make_float2(pow2(z1.x), pow2(z1.y));
         x[4 * c] = __float_as_uint(pow2(z0.x)); x[4 * c + 1] = __float_as_uint(pow2(z0.y));
         x[4 * c + 2] = __float_as_uint(r1.x); x[4 * c + 3] = __float_as_uint(r1.y);
       }
