@@ -113,6 +113,11 @@ SO3LR_B200_API int so3lr_b200_system_graph_replays(so3lr_b200_system* sys, int64
 SO3LR_B200_API int so3lr_b200_system_aux(so3lr_b200_system* sys, const float** zbl_dev, const float** coulomb_dev,
                           const float** dispersion_dev);
 
+/* Per-atom features of the network's last layer (n_atoms x 128 float32, caller's atom order) at the latest evaluation, copied to
+ * out_dev on `stream`.  INVALID_ARGUMENT before the first evaluation and for decomposed contexts.  The reference keeps them inside its
+ * network; here they are what a readout trained on top of it reads. */
+SO3LR_B200_API int so3lr_b200_system_features(so3lr_b200_system* sys, void* stream, float* out_dev);
+
 /* Counters: number of list rebuilds, short-range edges and long-range pairs of the latest build of each list (an export builds the
  * asked list only), kernels launched so far. */
 SO3LR_B200_API int so3lr_b200_system_stats(so3lr_b200_system* sys, int64_t* n_rebuilds, int64_t* n_edges, int64_t* n_pairs,

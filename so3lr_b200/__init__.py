@@ -13,3 +13,4 @@ from .api import make_potential_fn as So3lrPotential  # noqa: F401
 from .api import make_so3lr as So3lr  # noqa: F401
 from .api import neighbor_list  # noqa: F401
 from .attention import PackedStructures, norm_rotate, structure_attention  # noqa: F401
+from .readout import StructureReadout  # noqa: F401

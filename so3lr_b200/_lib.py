@@ -97,6 +97,7 @@ def _load():
         "so3lr_b200_system_profile_read": (i32, [p, i32, p, p, p]),
         "so3lr_b200_neighbor_list_noalloc": (i32, [p, i32, p, p, f32, i32, p, i64, p, p]),
         "so3lr_b200_list_row_total": (i32, [p, p, i32, C.POINTER(i64)]),
+        "so3lr_b200_system_features": (i32, [p, p, p]),
         "so3lr_b200_norm_rotate": (i32, [p, p, p, p, p, p]),
         "so3lr_b200_norm_rotate_workspace": (i64, [i32]),
         "so3lr_b200_norm_rotate_vjp": (i32, [p] * 12 + [i64]),

@@ -524,9 +524,11 @@ def to_jax_md(potential, displacement_or_metric, box_size, species=None, dr_thre
 # ------------------------------------------------------------------------------------------------------------
 # batched calculator
 # ------------------------------------------------------------------------------------------------------------
-def make_so3lr(lr_cutoff=12.0, dispersion_energy_cutoff_lr_damping=2.0, calculate_forces=True, workdir=None, device=None):
+def make_so3lr(lr_cutoff=12.0, dispersion_energy_cutoff_lr_damping=2.0, calculate_forces=True, workdir=None, device=None, readout=None):
     """so3lr/base_calculator.py:8-124.  Returns so3lr_fn(inputs) -> outputs with keys energy (n_graph,),
-    forces (n_node,3), dipole_vec (n_graph,3), hirshfeld_ratios (n_node,), partial_charges (n_node,).
+    forces (n_node,3), dipole_vec (n_graph,3), hirshfeld_ratios (n_node,), partial_charges (n_node,).  With a `readout`
+    (so3lr_b200.StructureReadout, or anything called like it) also features (n_node,128), the network's last layer, and
+    readout (n_graph, ..) = readout(features, positions, graph_start), zero for masked graphs; gradients reach the readout's parameters.
     `inputs` carries the same keys the reference passes to model.apply (positions, atomic_numbers, idx_i, idx_j,
     idx_i_lr, idx_j_lr, cell, total_charge, num_unpaired_electrons, batch_segments, node_mask, graph_mask);
     long-range lists hold both directions ('sparse', :31)."""
@@ -596,6 +598,10 @@ def make_so3lr(lr_cutoff=12.0, dispersion_energy_cutoff_lr_damping=2.0, calculat
             # dE/dd is zero for entries with an end outside the structure (padding): only real pairs contribute
             F = _displacements_vjp(n, torch.float32, dev, [(ii, jj, out["g_edges"]), (il, jl, out["g_edges_lr"])], sign=-1.0)
             res["forces"] = F
+        if readout is not None:
+            res["features"] = s.features() * node_mask[:, None]
+            y = readout(res["features"], R, graph_start)
+            res["readout"] = y * gm_t.to(y.dtype).view(-1, *[1] * (y.ndim - 1))
         return res
 
     return so3lr_fn

@@ -150,6 +150,13 @@ __global__ void gather_int_kernel(int n, const int* __restrict__ perm, const int
   int k = blockIdx.x * blockDim.x + threadIdx.x;
   if (k < n) dst[k] = src[perm[k]];
 }
+// rows of kF floats in slot order -> atom order (perm null: as they are), 16 bytes a thread
+__global__ void __launch_bounds__(256) feature_rows_kernel(long long n4, const int* __restrict__ perm, const float4* __restrict__ x, float4* __restrict__ out) {
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= n4) return;
+  const long long k = e / (kF / 4);
+  out[(perm ? (long long)perm[k] : k) * (kF / 4) + e % (kF / 4)] = x[e];
+}
 struct UnsortArgs {
   const float* src[7];
   float* dst[7];
@@ -356,6 +363,7 @@ struct so3lr_b200_system {
     bool broken = false;        // a capture failed: the context stays on plain launches
   } step_graph;
   bool have_lists = false;
+  int features_order = 0;      // rows of x[kNumLayers]: 0 none yet, 1 in the caller's order, 2 in that of d_perm
   // graph-level row pointers
   int *d_rowptr_g = nullptr, *d_rowptr_lr_g = nullptr;
   // activations
@@ -671,6 +679,7 @@ int evaluate_graph(so3lr_b200_system* S, cudaStream_t st, const int* row_ptr, co
     S->prof.end(st);
   }
   S->prof.begin(kPHeads, st);
+  S->features_order = 1;
   heads_fwd_dispatch(st, M, n, S->d_Z, S->x[kNumLayers], S->ze, S->zq, S->zh, S->e_nn, S->q_raw, S->hv, S->d_flag + 1);
   S->prof.end(st);
   launch_charge_conserve(st, S->n_graphs, S->d_graph_start, S->q_raw, S->d_total_charge, S->hv, S->q, S->h, S->n, S->red_scratch);
@@ -829,6 +838,7 @@ int fused_forward(so3lr_b200_system* S, cudaStream_t st, const float* R, const S
     S->prof.end(st);
   }
   S->prof.begin(kPHeads, st);
+  S->features_order = S->sorted ? 2 : 1;
   heads_fwd_dispatch(st, M, c.n0, S->d_Z, S->x[kNumLayers], S->ze, S->zq, S->zh, S->e_nn, S->q_raw, S->hv, S->d_flag + 1);
   S->prof.end(st);
   SO3LR_CUDA_CHECK(cudaGetLastError());
@@ -1358,6 +1368,7 @@ SO3LR_B200_API int so3lr_b200_system_compute(so3lr_b200_system* S, void* stream,
                         S->n_rebuilds == rebuilds_before && st != nullptr && st != cudaStreamLegacy && st != cudaStreamPerThread;
   if (graph_ok && G.exec && G.R == R && G.F == Fout && G.stamp == S->n_rebuilds && G.virial == S->want_virial) {
     SO3LR_CUDA_CHECK(cudaGraphLaunch(G.exec, st));
+    S->features_order = S->sorted ? 2 : 1;
     S->n_launches += G.launches;
     ++G.replays;
     if (S->want_virial) S->virial_fresh = true;
@@ -1398,6 +1409,7 @@ SO3LR_B200_API int so3lr_b200_system_compute(so3lr_b200_system* S, void* stream,
         } else {
           G.R = R; G.F = Fout; G.stamp = S->n_rebuilds; G.virial = S->want_virial; G.launches = S->n_launches - l0;
           SO3LR_CUDA_CHECK(cudaGraphLaunch(G.exec, st));
+          S->features_order = S->sorted ? 2 : 1;
         }
       }
     }
@@ -1452,6 +1464,19 @@ SO3LR_B200_API int so3lr_b200_system_aux(so3lr_b200_system* S, const float** zbl
   if (zbl) *zbl = S->o_zbl ? S->o_zbl : S->e_zbl;
   if (coul) *coul = S->o_coul ? S->o_coul : S->e_coul;
   if (disp) *disp = S->o_disp ? S->o_disp : S->e_disp;
+  return kOk;
+}
+
+SO3LR_B200_API int so3lr_b200_system_features(so3lr_b200_system* S, void* stream, float* out) {
+  if (!S || !out || reinterpret_cast<uintptr_t>(out) % 16 || !S->features_order || S->shells[3]) return kInvalidArgument;
+  SO3LR_CUDA_CHECK(cudaSetDevice(S->model->device));
+  tl_launch_counter = &S->n_launches;
+  const long long n4 = (long long)S->n * (kF / 4);
+  feature_rows_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, (cudaStream_t)stream>>>(n4, S->features_order == 2 ? S->d_perm : nullptr,
+                                                                                      reinterpret_cast<const float4*>(S->x[kNumLayers]),
+                                                                                      reinterpret_cast<float4*>(out));
+  count_launch();
+  SO3LR_CUDA_CHECK(cudaGetLastError());
   return kOk;
 }
 

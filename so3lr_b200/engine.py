@@ -154,6 +154,14 @@ class System:
             out[name] = _from_ptr(p.value, self.n, self.device).clone()
         return out
 
+    def features(self, stream=None):
+        """(n, 128) float32 features of the network's last layer, one row per atom, at the latest evaluation (a copy)."""
+        s = stream if stream is not None else torch.cuda.current_stream(self.device)
+        with torch.cuda.stream(s):
+            out = torch.empty(self.n, 128, device=self.device)
+        check(lib.so3lr_b200_system_features(self._h, C.c_void_p(s.cuda_stream), _ptr(out)), "system_features")
+        return out
+
     def kspace_vectors(self):
         """Number of k vectors the reciprocal sum runs over (both members of every pair (k, -k) counted; mesh points of the
         mesh variant) or None."""
