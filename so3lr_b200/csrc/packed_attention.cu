@@ -17,7 +17,7 @@ namespace {
 // Tables of query tiles: 64 rows (warp-level kernels), 128 and 256 (tensor cores, reverse and forward); of key tiles: 64 and 128.
 enum Head : int { kMagicAt, kN, kCausal, kRowsQ, kRowsKv, kMaxQ, kStartQ, kStartKv, kItemsQ, kNItemsQ, kItemsKv, kNItemsKv, kItemsSplit, kNItemsSplit,
                   kSplitFirst, kCombine, kTotal, kItemsQ128, kNItemsQ128, kItemsQ256, kNItemsQ256, kItemsKv128, kNItemsKv128, kMaxKv,
-                  kWalkQ128, kWalkQ256, kWalkKv128 /* tiles of 128 that the items of a table walk over in all */, kHeadInts = 32 };
+                  kWalkQ, kWalkKv /* tiles of 64 that the items of a table walk over in all */, kWalkQ128, kWalkQ256, kWalkKv128 /* tiles of 128 that the items of a table walk over in all */, kHeadInts = 32 };
 constexpr int kMagic = 0x53334c50;
 constexpr int kTables = 5, kTileRows[kTables] = {kPackTile, kPackTile, 128, 256, 128}, kTableAt[kTables] = {kItemsQ, kItemsKv, kItemsQ128, kItemsQ256, kItemsKv128};
 constexpr bool kOfKeys[kTables] = {false, true, false, false, true};
@@ -87,11 +87,9 @@ void build_image(int n, const int32_t* sq, const int32_t* sk, bool causal, int32
       }
     }
     put(im + im[kTableAt[t]], items);
-    if (t >= 2) {
-      int64_t walk = 0;
-      for (const Item& i : items) walk += (i.last - i.first + 127) / 128;
-      im[kWalkQ128 + t - 2] = (int32_t)std::min<int64_t>(walk, 0x7fffffff);
-    }
+    int64_t walk = 0;
+    for (const Item& i : items) walk += t < 2 ? (i.last - i.first + 63) / 64 : (i.last - i.first + 127) / 128;
+    im[kWalkQ + t] = (int32_t)std::min<int64_t>(walk, 0x7fffffff);
   }
   const int chunk = split_length(sk[n]);
   int32_t* split = im + im[kItemsSplit];
@@ -126,18 +124,13 @@ bool shape_ok(const int32_t* im, const so3lr_b200_attention_shape* a) {
 PackedArgs common(const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a) {
   PackedArgs p;
   p.start_q = dev + im[kStartQ]; p.start_kv = dev + im[kStartKv]; p.split_first = dev + im[kSplitFirst];
-  p.rows = im[kRowsQ]; p.rows_kv = im[kRowsKv];
+  p.rows = im[kRowsQ]; p.rows_kv = im[kRowsKv]; p.longest_kv = im[kMaxKv];
   p.stages = im[kMaxKv] <= (a->type == kF32 && a->d > 64 ? 32 : 64) ? 1 : 2;
   p.nq = (int)a->rows_q; p.nkv = (int)a->rows_kv; p.hq = a->heads_q; p.hk = a->heads_kv; p.group = a->heads_q / a->heads_kv; p.d = a->d; p.causal = im[kCausal];
   p.scale = a->scale; p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   return p;
 }
 
-// Few queries: the heads of a group share one tile of rows with their token, and the keys are cut into stretches.  The keys are then
-// read once per group and not once per head.
-bool few_rows(const int32_t* im, const so3lr_b200_attention_shape* a) {
-  return (int64_t)im[kMaxQ] * (a->heads_q / a->heads_kv) <= kPackTile;
-}
 int64_t part_floats(const int32_t* im, const so3lr_b200_attention_shape* a) {
   return (int64_t)im[kNItemsSplit] * a->heads_kv * im[kMaxQ] * (a->heads_q / a->heads_kv) * packed_padded(a->d);
 }
@@ -156,12 +149,17 @@ bool on_tensor_cores(const int32_t* im, const so3lr_b200_attention_shape* a) {
   const int rows = tensor_core_rows(a->type, a->d);
   return im[kMaxQ] >= rows && im[kMaxKv] >= rows;
 }
+// Few queries: the heads of a group share one tile of rows with their token, and the keys are cut into stretches.  The keys are then
+// read once per group and not once per head.
+bool few_rows(const int32_t* im, const so3lr_b200_attention_shape* a) {
+  return (int64_t)im[kMaxQ] * (a->heads_q / a->heads_kv) <= kPackTile;
+}
 // Into how many pieces the walks of a kernel's items are cut.  With few CTAs for the chip the last round of them leaves most SMs idle (160
 // equal ones on 148: half of the time), so the time is that of the work on all SMs, plus half of a CTA that ends last, plus what a CTA costs
 // besides its tiles (a start and an end: two tiles' time, `tile` us each), plus the shares' way through memory and the launch that joins them.
-int pieces_of(int64_t items, int heads, int64_t walk, int longest, double tile, double share_bytes) {
+int pieces_of(int64_t items, int heads, int64_t walk, int longest, double tile, double share_bytes, int per_sm = 1) {
   if (items == 0 || walk == 0) return 1;
-  const double sms = sm_count(), ctas = (double)items * heads, tiles = (double)walk * heads;
+  const double sms = (double)sm_count() * per_sm, ctas = (double)items * heads, tiles = (double)walk * heads;
   double best = 0;
   int at = 1;
   for (int p = 1; p <= 16 && (p == 1 || longest >= 3 * p); ++p) {
@@ -174,19 +172,28 @@ int pieces_of(int64_t items, int heads, int64_t walk, int longest, double tile, 
 }
 PackedPieces pieces(const int32_t* im, const so3lr_b200_attention_shape* a) {
   PackedPieces p;
+  if (!on_tensor_cores(im, a)) {      // 64 x 64 tiles of the warp-level kernels, two CTAs on an SM
+    const int long_q = (im[kMaxQ] + 63) / 64, long_kv = (im[kMaxKv] + 63) / 64, group = a->heads_q / a->heads_kv;
+    const double bytes_q = 4.0 * im[kRowsQ] * a->heads_q * a->d, bytes_kv = 4.0 * im[kRowsKv] * a->heads_kv * a->d;
+    const double tile = (a->type == kF32 ? 3.0 : 1.5) * (a->d <= 32 ? 0.4 : a->d <= 64 ? 0.7 : 1.3);
+    if (!few_rows(im, a)) p.forward = pieces_of(im[kNItemsQ], a->heads_q, im[kWalkQ], long_kv, tile, bytes_q, 2);
+    p.dq = pieces_of(im[kNItemsQ], a->heads_q, im[kWalkQ], long_kv, 1.5 * tile, bytes_q, 2);
+    p.dkv = pieces_of(im[kNItemsKv], a->heads_kv, (int64_t)im[kWalkKv] * group, long_q * group, 2 * tile, 2 * bytes_kv, 2);
+    return p;
+  }
   const int long_q = (im[kMaxQ] + 127) / 128, long_kv = (im[kMaxKv] + 127) / 128, group = a->heads_q / a->heads_kv;
   // a tile's time as measured: 256 x 128 forward, 128 x 128 reverse
   const bool f32 = a->type == kF32, wide = a->d > 64;
   const double fwd = f32 ? 3.0 : wide ? 2.1 : 1.4, dq = f32 ? 2.0 : wide ? 1.4 : 1.0, dkv = f32 ? 3.0 : wide ? 1.6 : 1.2;
   const double bytes_q = 4.0 * im[kRowsQ] * a->heads_q * a->d, bytes_kv = 4.0 * im[kRowsKv] * a->heads_kv * a->d;
-  p.forward = pieces_of(im[kNItemsQ256], a->heads_q, im[kWalkQ256], long_kv, fwd, bytes_q);
+  if (packed_one_tile(f32, a->d, im[kMaxKv])) p.forward = pieces_of(im[kNItemsQ128], a->heads_q, im[kWalkQ128], long_kv, fwd, bytes_q, 2);
+  else p.forward = pieces_of(im[kNItemsQ256], a->heads_q, im[kWalkQ256], long_kv, fwd, bytes_q);
   p.dq = pieces_of(im[kNItemsQ128], a->heads_q, im[kWalkQ128], long_kv, dq, bytes_q);
   p.dkv = pieces_of(im[kNItemsKv128], a->heads_kv, (int64_t)im[kWalkKv128] * group, long_q * group, dkv, 2 * bytes_kv);
   return p;
 }
-int64_t tc_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool reverse) {
-  if (!on_tensor_cores(im, a)) return 0;
-  return (a->type == kF32 ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0) +
+int64_t whole_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool reverse) {
+  return (a->type == kF32 && on_tensor_cores(im, a) ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0) +
          packed_share_bytes(pieces(im, a), a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse);
 }
 
@@ -202,11 +209,16 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
     return packed_forward_split<T>(st, p, im[kNItemsSplit], im[kN], im[kCombine]);
   }
   if (on_tensor_cores(im, a)) {
-    p.items = table(im, dev, kItemsQ256);
-    return packed_forward_tc<T>(st, p, im[kNItemsQ256], pieces(im, a), workspace);
+    const bool one = packed_one_tile(a->type == kF32, a->d, im[kMaxKv]);
+    p.items = table(im, dev, one ? kItemsQ128 : kItemsQ256);
+    return packed_forward_tc<T>(st, p, im[one ? kNItemsQ128 : kNItemsQ256], pieces(im, a), workspace);
   }
   p.items = table(im, dev, kItemsQ);
-  return packed_forward_mma<T>(st, p, im[kNItemsQ]);
+  p.pieces = pieces(im, a).forward;
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)p.pieces * p.nq * p.hq * p.d);
+  const int rc = packed_forward_mma<T>(st, p, im[kNItemsQ]);
+  return rc || p.pieces == 1 ? rc : packed_join<T>(st, p);
 }
 
 template <typename T>
@@ -215,10 +227,19 @@ int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
   if (rc) return rc;
   if (on_tensor_cores(im, a))
     return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128], pieces(im, a), workspace);
+  const PackedPieces n = pieces(im, a);
+  const int64_t stride_q = (int64_t)p.nq * p.hq * p.d, stride_kv = (int64_t)p.nkv * p.hk * p.d;
+  float* share = static_cast<float*>(workspace);
+  if (n.dq > 1) { p.share[0] = share; share += n.dq * stride_q; }
+  if (n.dkv > 1) { p.share[1] = share; p.share[2] = share + n.dkv * stride_kv; }
   p.items = table(im, dev, kItemsQ);
+  p.pieces = n.dq;
   if (im[kNItemsQ]) rc = packed_dq_mma<T>(st, p, im[kNItemsQ]);
+  if (rc) return rc;
   p.items = table(im, dev, kItemsKv);
-  return rc || !im[kNItemsKv] ? rc : packed_dkv_mma<T>(st, p, im[kNItemsKv]);
+  p.pieces = n.dkv;
+  if (im[kNItemsKv]) rc = packed_dkv_mma<T>(st, p, im[kNItemsKv]);
+  return rc || (n.dq == 1 && n.dkv == 1) ? rc : packed_sum<T>(st, p, n.dq, n.dkv);
 }
 
 }  // namespace
@@ -247,8 +268,8 @@ int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int
 
 int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* a, int vjp) {
   if (!shape_ok(image, a)) return -1;
-  if (vjp) return tc_bytes(image, a, true);
-  if (!few_rows(image, a)) return tc_bytes(image, a, false);
+  if (vjp) return whole_bytes(image, a, true);
+  if (!few_rows(image, a)) return whole_bytes(image, a, false);
   if (!image[kCombine]) return 0;
   return part_floats(image, a) * (int64_t)sizeof(float) + part_floats(image, a) / packed_padded(a->d) * (int64_t)sizeof(float2);
 }

@@ -37,6 +37,7 @@ struct PackedArgs {
   int pieces = 1;               // tensor-core kernels: pieces that an item's walk is cut into; each leaves its share in part_o / part_ml or
   float* share[3] = {};         // (reverse) in share: (pieces, heads, rows, d) of dq, dk, dv
   int rows = 0, rows_kv = 0;    // of the layout
+  int longest_kv = 0;           // keys of its longest structure
   int stages = 2;               // buffers for the keys in the warp-level forward kernel: one where they all fit into it
   int nq = 0, nkv = 0, hq = 0, hk = 0, group = 1, d = 0, causal = 0;
   float scale = 0.f, scale_log2 = 0.f;                // scale * log2(e): the softmax runs on powers of two
@@ -51,9 +52,17 @@ template <typename T> int packed_forward_split(cudaStream_t st, const PackedArgs
 template <typename T> int packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items);
 template <typename T> int packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items);
 template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, int rows);
+// joins of the pieces' shares (a.pieces of the forward kernel; of dq, of dk and dv)
+template <typename T> int packed_join(cudaStream_t st, const PackedArgs& a);
+template <typename T> int packed_sum(cudaStream_t st, const PackedArgs& a, int pieces_q, int pieces_kv);
 
 // Kernels on the tensor cores: tiles of 128 rows, two of them side by side in the forward kernel.  float32 (d <= 64) runs on operands that
 // are split into three bfloat16 terms ahead (packed_split_bytes of workspace).
+// Whether the forward kernel's CTAs have one tile of 128 rows and half of an SM, or two and all of it.  About 8,200 rows in structures of up to L, one
+// tile / two, us: 8 heads x 128, L = 128 22 / 32, 512 38 / 38, 1,024 46 / 53, but 16,001 rows to 8,192 697 / 666 (keys and values come in
+// twice as often, through half the buffers); 8 x 64 512 29 / 34, 1,024 36 / 47, 9 heads of 8,192 rows 231 / 234; float32 4 x 32, 256
+// 27 / 29, 1,024 41 / 47, 5,000 rows 105 / 100.
+inline bool packed_one_tile(bool f32, int d, int longest_kv) { return f32 ? d <= 32 && longest_kv < 2048 : d <= 64 || longest_kv < 2048; }
 struct PackedPieces { int forward = 1, dq = 1, dkv = 1; };
 template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace);
 template <typename T>

@@ -261,12 +261,13 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const uint32_t sq = smem_addr(smem), sk = sq + kPackTile * L::kStride;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int heads = SPLIT ? a.hk : a.hq, unit = blockIdx.x / heads;
+  const int heads = SPLIT ? a.hk : a.hq, piece = SPLIT ? 0 : blockIdx.x % a.pieces, index = SPLIT ? blockIdx.x : blockIdx.x / a.pieces, unit = index / heads;
   const int4 item = a.items[unit];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int G = SPLIT ? a.group : 1, hy = blockIdx.x % heads, kvh = SPLIT ? hy : hy / a.group;
+  const int G = SPLIT ? a.group : 1, hy = index % heads, kvh = SPLIT ? hy : hy / a.group;
   const int rows = lq * G, row0 = SPLIT ? 0 : item.y * kPackTile;
-  const int k0 = item.z, k1 = item.w;
+  const int share = SPLIT ? 0 : ((item.w + BN - 1) / BN + a.pieces - 1) / a.pieces * BN;      // keys of a piece
+  const int k0 = SPLIT ? item.z : min(item.w, piece * share), k1 = SPLIT ? item.w : min(item.w, k0 + share);
   const int nt = (max(k1 - k0, 0) + BN - 1) / BN, stages = a.stages;
   const uint32_t sv = sk + stages * BN * L::kStride;
 
@@ -359,6 +360,16 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
       continue;
     }
     const int tok = SPLIT ? pr / G : pr, head = SPLIT ? hy * G + pr % G : hy;
+    if (!SPLIT && a.pieces > 1) {
+      const long long slot = ((long long)piece * a.hq + head) * a.nq + q0 + tok;
+#pragma unroll
+      for (int n = 0; n < DP / 8; ++n) {
+        const int c = n * 8 + 2 * (lane & 3);
+        if (c < a.d) *reinterpret_cast<float2*>(a.part_o + slot * a.d + c) = make_float2(o[n][2 * half], o[n][2 * half + 1]);
+      }
+      if ((lane & 3) == 0) a.part_ml[slot] = make_float2(m, l);
+      continue;
+    }
     const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);               // a row without keys gives zero; NaN stays NaN
     const long long to = ((long long)(q0 + tok) * a.hq + head) * a.d;
     T *dst = static_cast<T*>(a.out) + to, *rest = a.out_rest ? static_cast<T*>(a.out_rest) + to : nullptr;
@@ -549,6 +560,57 @@ __global__ void __launch_bounds__(256) combine_kernel(const PackedArgs a) {
   }
 }
 
+// ---- pieces ----
+// joins the pieces of the forward kernel: a thread per eight values of a row
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const PackedArgs a, int rows) {
+  const int parts = a.d / 8;
+  const long long e = (long long)blockIdx.x * 256 + threadIdx.x, hr = e / parts;
+  const int c = (int)(e % parts) * 8;
+  if (hr >= (long long)rows * a.hq) return;
+  const long long r = hr / a.hq;
+  const int h = (int)(hr % a.hq);
+  float m = -INFINITY, l = 0.f, o[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) o[k] = 0.f;
+  for (int p = 0; p < a.pieces; ++p) m = fmaxf(m, a.part_ml[((long long)p * a.hq + h) * a.nq + r].x);
+  const float u = m == -INFINITY ? 0.f : m;
+  for (int p = 0; p < a.pieces; ++p) {
+    const long long slot = ((long long)p * a.hq + h) * a.nq + r;
+    const float2 ml = a.part_ml[slot];
+    if (ml.y == 0.f) continue;      // no key of the piece was seen: its share was not written where it has no tile
+    const float f = exp2f(ml.x - u);
+    l = fmaf(ml.y, f, l);
+    const float4 x = *reinterpret_cast<const float4*>(a.part_o + slot * a.d + c), y = *reinterpret_cast<const float4*>(a.part_o + slot * a.d + c + 4);
+    o[0] = fmaf(x.x, f, o[0]); o[1] = fmaf(x.y, f, o[1]); o[2] = fmaf(x.z, f, o[2]); o[3] = fmaf(x.w, f, o[3]);
+    o[4] = fmaf(y.x, f, o[4]); o[5] = fmaf(y.y, f, o[5]); o[6] = fmaf(y.z, f, o[6]); o[7] = fmaf(y.w, f, o[7]);
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  const long long at = hr * a.d + c;
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) store_rest<T>(static_cast<T*>(a.out) + at + k, a.out_rest ? static_cast<T*>(a.out_rest) + at + k : nullptr, o[k] * inv, o[k + 1] * inv);
+  if (c == 0 && a.lse) a.lse[(long long)h * a.nq + r] = l == 0.f ? -INFINITY : m + log2f(l);
+}
+// sums the pieces' shares of dq, dk, dv (blockIdx.y), a thread per eight values
+template <typename T>
+__global__ void __launch_bounds__(256) sum_kernel(const PackedArgs a, int first, int pieces_q, int pieces_kv, long long values_q, long long values_kv,
+                                                  long long stride_q, long long stride_kv) {
+  const int which = first + blockIdx.y, pieces = which ? pieces_kv : pieces_q;
+  const long long e = ((long long)blockIdx.x * 256 + threadIdx.x) * 8, values = which ? values_kv : values_q, stride = which ? stride_kv : stride_q;
+  if (e >= values) return;
+  const float* src = a.share[which] + e;
+  float o[8];
+#pragma unroll
+  for (int k = 0; k < 8; ++k) o[k] = 0.f;
+  for (int p = 0; p < pieces; ++p) {
+    const float4 x = *reinterpret_cast<const float4*>(src + p * stride), y = *reinterpret_cast<const float4*>(src + p * stride + 4);
+    o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w; o[4] += y.x; o[5] += y.y; o[6] += y.z; o[7] += y.w;
+  }
+  T* dst = static_cast<T*>(which == 0 ? a.dq : which == 1 ? a.dk : a.dv) + e;
+#pragma unroll
+  for (int k = 0; k < 8; k += 2) store2(dst + k, o[k], o[k + 1]);
+}
+
 // ---- reverse --------------------------------------------------------------------------------------------------------
 // delta = sum over d of g * o, a thread per 16 bytes, rows of all heads
 template <typename T>
@@ -590,9 +652,11 @@ __global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
   extern __shared__ __align__(16) unsigned char smem[];
   const uint32_t sq = smem_addr(smem), sg = sq + kPackTile * L::kStride, sk = sg + kPackTile * L::kStride, sv = sk + 2 * BN * L::kStride;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x / a.hq];
+  const int piece = blockIdx.x % a.pieces, index = blockIdx.x / a.pieces;
+  const int4 item = a.items[index / a.hq];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = blockIdx.x % a.hq, kvh = h / a.group, row0 = item.y * kPackTile, k0 = item.z, k1 = item.w;
+  const int h = index % a.hq, kvh = h / a.group, row0 = item.y * kPackTile;
+  const int share = ((item.w + BN - 1) / BN + a.pieces - 1) / a.pieces * BN, k0 = min(item.w, piece * share), k1 = min(item.w, k0 + share);
   const int nt = (max(k1 - k0, 0) + BN - 1) / BN;
   load_rows<T, DP, kPackTile>(sq, a.q, h, q0, row0, lq, a.d, tid);
   load_rows<T, DP, kPackTile>(sg, a.g, h, q0, row0, lq, a.d, tid);
@@ -607,10 +671,10 @@ __global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
   load(0);
   const int wr = row0 + warp * 16, ra = wr + (lane >> 2), rb = ra + 8, off = lk - lq, big = 0x7fffffff;
   const int lim_a = a.causal ? ra + off : big, lim_b = a.causal ? rb + off : big, lim_lo = a.causal ? wr + off : big, lim_hi = a.causal ? wr + 15 + off : big;
-  const long long at = (long long)h * a.nq + q0;
+  const long long at_row = (long long)h * a.nq + q0;
   // rows that are not there: exp(-inf) = 0
-  const float ea = ra < lq ? a.lse[at + ra] : INFINITY, eb = rb < lq ? a.lse[at + rb] : INFINITY;
-  const float da = ra < lq ? a.delta[at + ra] : 0.f, db = rb < lq ? a.delta[at + rb] : 0.f;
+  const float ea = ra < lq ? a.lse[at_row + ra] : INFINITY, eb = rb < lq ? a.lse[at_row + rb] : INFINITY;
+  const float da = ra < lq ? a.delta[at_row + ra] : 0.f, db = rb < lq ? a.delta[at_row + rb] : 0.f;
   float dq[DP / 8][4];
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
@@ -646,11 +710,14 @@ __global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
   for (int half = 0; half < 2; ++half) {
     const int r = half ? rb : ra;
     if (r >= lq) continue;
-    T* dst = static_cast<T*>(a.dq) + ((long long)(q0 + r) * a.hq + h) * a.d;
+    const long long at = ((long long)(q0 + r) * a.hq + h) * a.d;
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n) {
       const int c = n * 8 + 2 * (lane & 3);
-      if (c < a.d) store2(dst + c, dq[n][2 * half] * a.scale, dq[n][2 * half + 1] * a.scale);
+      if (c >= a.d) continue;
+      const float x = dq[n][2 * half] * a.scale, y = dq[n][2 * half + 1] * a.scale;
+      if (a.pieces > 1) store2(a.share[0] + (long long)piece * a.nq * a.hq * a.d + at + c, x, y);
+      else store2(static_cast<T*>(a.dq) + at + c, x, y);
     }
   }
 }
@@ -664,15 +731,17 @@ __global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
   const uint32_t sk = smem_addr(smem), sv = sk + kPackTile * L::kStride, sq = sv + kPackTile * L::kStride, sg = sq + 2 * BN * L::kStride;
   float* se = reinterpret_cast<float*>(smem + (2 * kPackTile + 4 * BN) * L::kStride);   // [2][BN] lse, [2][BN] delta
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int4 item = a.items[blockIdx.x / a.hk];
+  const int piece = blockIdx.x % a.pieces, index = blockIdx.x / a.pieces;
+  const int4 item = a.items[index / a.hk];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int kvh = blockIdx.x % a.hk, row0 = item.y * kPackTile, i0 = item.z, i1 = item.w;
-  const int per = (max(i1 - i0, 0) + BN - 1) / BN, nt = per * a.group;
+  const int kvh = index % a.hk, row0 = item.y * kPackTile, i0 = item.z, i1 = item.w;
+  const int per = (max(i1 - i0, 0) + BN - 1) / BN, all = per * a.group, share = (all + a.pieces - 1) / a.pieces, j0 = min(all, piece * share);
+  const int nt = min(share, all - j0);      // from tile j0 on
   load_rows<T, DP, kPackTile>(sk, a.k, kvh, c0, row0, lk, a.d, tid);
   load_rows<T, DP, kPackTile>(sv, a.v, kvh, c0, row0, lk, a.d, tid);
   auto load = [&](int it) {
     if (it < nt) {
-      const int buf = it & 1, h = kvh * a.group + it / per, b = i0 + (it % per) * BN;
+      const int buf = it & 1, h = kvh * a.group + (j0 + it) / per, b = i0 + ((j0 + it) % per) * BN;
       load_rows<T, DP, BN>(sq + buf * BN * L::kStride, a.q, h, q0, b, i1, a.d, tid);
       load_rows<T, DP, BN>(sg + buf * BN * L::kStride, a.g, h, q0, b, i1, a.d, tid);
       if (tid < BN) {
@@ -695,7 +764,7 @@ __global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
     load(it + 1);
     copy_wait<1>();
     __syncthreads();
-    const int ib = i0 + (it % per) * BN, buf = it & 1;
+    const int ib = i0 + ((j0 + it) % per) * BN, buf = it & 1;
     if (wr < lk && ib + BN - 1 >= lim_lo) {
       float p[NT][4], ds[NT][4];
       const int cols = i1 - ib;
@@ -729,9 +798,16 @@ __global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n) {
       const int c = n * 8 + 2 * (lane & 3);
-      if (c < a.d) {
-        store2(static_cast<T*>(a.dk) + at + c, dk[n][2 * half] * a.scale, dk[n][2 * half + 1] * a.scale);
-        store2(static_cast<T*>(a.dv) + at + c, dv[n][2 * half] * prob_unscale<T>(), dv[n][2 * half + 1] * prob_unscale<T>());
+      if (c >= a.d) continue;
+      const float k0 = dk[n][2 * half] * a.scale, k1 = dk[n][2 * half + 1] * a.scale;
+      const float v0 = dv[n][2 * half] * prob_unscale<T>(), v1 = dv[n][2 * half + 1] * prob_unscale<T>();
+      if (a.pieces > 1) {
+        const long long to = (long long)piece * a.nkv * a.hk * a.d + at + c;
+        store2(a.share[1] + to, k0, k1);
+        store2(a.share[2] + to, v0, v1);
+      } else {
+        store2(static_cast<T*>(a.dk) + at + c, k0, k1);
+        store2(static_cast<T*>(a.dv) + at + c, v0, v1);
       }
     }
   }
@@ -766,7 +842,7 @@ int launch(int64_t grid, int threads, int smem, cudaStream_t st, const PackedArg
 }  // namespace packed
 
 template <typename T> int packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) return packed::launch<packed::forward_kernel<T, DP, false>>((int64_t)n_items * a.hq, 128, packed::forward_smem<T, DP>(a.stages), st, a);
+#define CALL(T, DP) return packed::launch<packed::forward_kernel<T, DP, false>>((int64_t)n_items * a.hq * a.pieces, 128, packed::forward_smem<T, DP>(a.stages), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
@@ -780,14 +856,32 @@ template <typename T> int packed_forward_split(cudaStream_t st, const PackedArgs
 #undef CALL
 }
 template <typename T> int packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) return packed::launch<packed::dq_kernel<T, DP>>((int64_t)n_items * a.hq, 128, packed::reverse_smem<T, DP>(), st, a);
+#define CALL(T, DP) return packed::launch<packed::dq_kernel<T, DP>>((int64_t)n_items * a.hq * a.pieces, 128, packed::reverse_smem<T, DP>(), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
 template <typename T> int packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) return packed::launch<packed::dkv_kernel<T, DP>>((int64_t)n_items * a.hk, 128, packed::reverse_smem<T, DP>(), st, a);
+#define CALL(T, DP) return packed::launch<packed::dkv_kernel<T, DP>>((int64_t)n_items * a.hk * a.pieces, 128, packed::reverse_smem<T, DP>(), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
+}
+template <typename T> int packed_join(cudaStream_t st, const PackedArgs& a) {
+  const int64_t ctas = ((int64_t)a.rows * a.hq * (a.d / 8) + 255) / 256;
+  if (ctas > 0x7fffffff) return kTooLarge;
+  packed::join_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, a.rows);
+  count_launch();
+  return kOk;
+}
+template <typename T> int packed_sum(cudaStream_t st, const PackedArgs& a, int pieces_q, int pieces_kv) {
+  const long long values_q = (long long)a.rows * a.hq * a.d, values_kv = (long long)a.rows_kv * a.hk * a.d;
+  const int first = pieces_q > 1 ? 0 : 1, many = (pieces_kv > 1 ? 3 : 1) - first;
+  const long long most = pieces_q > 1 && (pieces_kv == 1 || values_q > values_kv) ? values_q : values_kv;
+  const int64_t ctas = (most / 8 + 255) / 256;
+  if (ctas > 0x7fffffff) return kTooLarge;
+  packed::sum_kernel<T><<<dim3((unsigned)ctas, many), 256, 0, st>>>(a, first, pieces_q, pieces_kv, values_q, values_kv, (long long)a.nq * a.hq * a.d,
+                                                                    (long long)a.nkv * a.hk * a.d);
+  count_launch();
+  return kOk;
 }
 template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, int rows) {
   int width = 1;

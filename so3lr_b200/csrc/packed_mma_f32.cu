@@ -7,4 +7,6 @@ template int packed_forward_split<float>(cudaStream_t, const PackedArgs&, int, i
 template int packed_dq_mma<float>(cudaStream_t, const PackedArgs&, int);
 template int packed_dkv_mma<float>(cudaStream_t, const PackedArgs&, int);
 template int packed_delta<float>(cudaStream_t, const PackedArgs&, int);
+template int packed_join<float>(cudaStream_t, const PackedArgs&);
+template int packed_sum<float>(cudaStream_t, const PackedArgs&, int, int);
 }  // namespace so3lr

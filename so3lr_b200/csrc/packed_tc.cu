@@ -62,35 +62,46 @@ __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* p) { retur
 // ---- forward --------------------------------------------------------------------------------------------------------
 // 256 queries of one head: two tiles of 128 rows take turns, so that the exponentials of one run beside the products of the other.
 // Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t; P of a tile replaces its logits.  (Up to 64 values a head: output at
-// 256 + 64 t, P at 384 + 64 t.  float32: logits at 256 t, the three terms of P from there on, its output at 256 t + 192.)
+// 256 + 64 t, P at 384 + 64 t; one tile: logits at 0, output at 128, P at 192.  float32: logits at 256 t, the three terms of P from there on, its output at 256 t + 192.)
 // The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
 // the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
 enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kSFull = kQFull + 2, kPFull = kSFull + 2 /* tile + 2 half */, kOFull = kPFull + 4, kFix = kOFull + 2,
               kSRead, kFwdBars = kSRead + 2 };
 
-template <typename T, int TERMS, int DW>
-__global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
+// TILES = 1: a CTA has one tile and half of an SM, which two of them share: one's start and end pass beside the other's work.
+template <int TERMS, int DW, int TILES> struct Forward {
+  static constexpr int kMma = 4 * TILES, kLoad = kMma + 1, kThreads = 128 * TILES + 128;
+  // registers: 256 x 208 + 128 x 88 = 384 x 168; 128 x 200 + 128 x 56 = 256 x 128
+  static constexpr int kRegs = TILES == 2 ? 208 : 200, kOtherRegs = TILES == 2 ? 88 : 56;
+  static constexpr int kRing = TILES == 2 ? Geometry<TERMS, DW>::kRing : TERMS == 3 ? 3 : DW == 128 ? 2 : 4;
+  static constexpr int kSmem = 1024 + (TILES + kRing) * Geometry<TERMS, DW>::kSubs * (int)Geometry<TERMS, DW>::kSub + (int)sizeof(Tail);
+  static_assert(TILES == 2 || kSmem <= 232448 / 2, "two CTAs on an SM");
+};
+template <typename T, int TERMS, int DW, int TILES>
+__global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 2 ? 1 : 2) forward_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
   using M = typename Operand<T, TERMS>::type;
   using G = Geometry<TERMS, DW>;
+  using F = Forward<TERMS, DW, TILES>;
+  constexpr int kMmaWarp = F::kMma, kLoadWarp = F::kLoad;
   extern __shared__ unsigned char raw[];
   unsigned char* smem = aligned_smem(raw);
   const int d = a.d;
-  constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = G::kRing;
-  Tail* tail = reinterpret_cast<Tail*>(smem + (2 + R) * tile_bytes);
-  const uint32_t sq = smem_addr(smem), ring = sq + 2 * tile_bytes, bar0 = smem_addr(tail->bars);
+  constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = F::kRing;
+  Tail* tail = reinterpret_cast<Tail*>(smem + (TILES + R) * tile_bytes);
+  const uint32_t sq = smem_addr(smem), ring = sq + TILES * tile_bytes, bar0 = smem_addr(tail->bars);
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int unit = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
   const int4 item = a.items[unit / a.hq];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = unit % a.hq, kvh = h / a.group, row0 = item.y * 2 * kTile, off = lk - lq;
+  const int h = unit % a.hq, kvh = h / a.group, row0 = item.y * TILES * kTile, off = lk - lq;
   // keys that a tile meets: [0, end[t]), and tiles of keys
-  const int end1 = item.w, end0 = a.causal ? min(end1, max(0, min(lq, row0 + kTile) + off)) : end1;
-  const int all0 = (end0 + kTile - 1) / kTile, all1 = row0 + kTile < lq ? (end1 + kTile - 1) / kTile : 0, per = (max(all0, all1) + a.pieces - 1) / a.pieces;
+  const int end1 = item.w, end0 = TILES == 2 && a.causal ? min(end1, max(0, min(lq, row0 + kTile) + off)) : end1;
+  const int all0 = (end0 + kTile - 1) / kTile, all1 = TILES == 2 && row0 + kTile < lq ? (end1 + kTile - 1) / kTile : 0, per = (max(all0, all1) + a.pieces - 1) / a.pieces;
   // this piece's: tiles from k0 / 128 on
   const int k0 = piece * per * kTile, n0 = min(per, max(0, all0 - piece * per)), n1 = min(per, max(0, all1 - piece * per)), n = max(n0, n1);
-  if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
+  if (warp == kMmaWarp) alloc_tmem(&tail->tmem, 256 * TILES);
   if (tid == 0) {
     tail->failed = 0;
     for (int i = 0; i < kFwdBars; ++i) init_bar(bar(i), (i >= kPFull && i < kPFull + 4) || i >= kSRead ? kTile : 1);
@@ -101,11 +112,11 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
   fence_after();
   const uint32_t tmem = tail->tmem;
   // columns from one tile's logits to the other's, output of a tile, columns from one output to the other, P
-  constexpr uint32_t kStride = TERMS == 1 ? kTile : 256, kOut = TERMS == 1 ? 256 : 192, kOutStride = TERMS == 1 ? DW : 256;
-  auto p_at = [](int t) { return G::kEarly ? 384u + 64 * t : kStride * t; };
+  constexpr uint32_t kStride = TERMS == 1 ? kTile : 256, kOut = TERMS == 1 ? kTile * TILES : 192, kOutStride = TERMS == 1 ? DW : 256;
+  auto p_at = [](int t) { return G::kEarly ? kOut + 64 * TILES + 64 * t : kStride * t; };
 
   if (warp >= kMmaWarp) {
-    fewer_regs<kOtherRegs>();
+    fewer_regs<F::kOtherRegs>();
     if (warp == kMmaWarp && n > 0) {
       const uint32_t on = elect_one();
       // keys are tiles 0, 2, .. of the ring, values 1, 3, ..; a slot is given back only where another tile waits for it, so that nothing is
@@ -115,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       auto give = [&](int j) { if (j + R < 2 * n) commit(on, bar(kEmpty + j % R)); };
       ready(0);
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < TILES; ++t) {
         if ((t ? n1 : n0) == 0) continue;
         wait_bar(bar(kQFull + t), 0, failed, &g_packed_error);
         fence_after();
@@ -132,7 +143,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
         if (i + 1 < n) ready(2 * i + 2);
         if (G::kEarly) {
 #pragma unroll
-          for (int t = 0; t < 2; ++t) {
+          for (int t = 0; t < TILES; ++t) {
             if (i + 1 >= (t ? n1 : n0)) continue;
             wait_bar(bar(kSRead + t), i & 1, failed, &g_packed_error);
             fence_after();
@@ -142,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
         }
         ready(2 * i + 1);
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < TILES; ++t) {
           const int nt = t ? n1 : n0;
           if (i >= nt) continue;
           wait_bar(bar(kPFull + t), i & 1, failed, &g_packed_error);
@@ -165,7 +176,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       }
     } else if (warp == kLoadWarp && n > 0) {
       Loader<TERMS, DW> ld{lane, bar(kFix)};
-      for (int t = 0; t < 2; ++t)
+      for (int t = 0; t < TILES; ++t)
         if ((t ? n1 : n0) > 0) ld.tile(sq + t * tile_bytes, &maps.q, q0 + row0 + t * kTile, h, bar(kQFull + t), kTile, false, failed, &g_packed_error);
       for (int j = 0; j < 2 * n; ++j) {
         if (j >= R) wait_bar(bar(kEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
@@ -174,7 +185,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
       }
     }
   } else {
-    more_regs<kComputeRegs>();
+    more_regs<F::kRegs>();
     const int t = warp >> 2, w = warp & 3, nt = t ? n1 : n0;
     const int row = row0 + t * kTile + w * 32 + lane, first = row0 + t * kTile + w * 32;
     const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16), ts = lanes + kStride * t, to = lanes + kOut + kOutStride * t;
@@ -317,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1) forward_kernel(const PackedArgs a
     fence_before();
   }
   __syncthreads();
-  if (warp == kMmaWarp) { fence_after(); free_tmem(tmem); }
+  if (warp == kMmaWarp) { fence_after(); free_tmem(tmem, 256 * TILES); }
 }
 
 // ---- reverse: dq ----------------------------------------------------------------------------------------------------
@@ -752,56 +763,6 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
 
 static_assert(kFwdBars <= 32 && kDqBars <= 32 && kDkvBars <= 32, "barriers");
 
-// joins the pieces of the forward kernel: a thread per eight values of a row
-template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const PackedArgs a, int rows) {
-  const int parts = a.d / 8;
-  const long long e = (long long)blockIdx.x * 256 + threadIdx.x, hr = e / parts;
-  const int c = (int)(e % parts) * 8;
-  if (hr >= (long long)rows * a.hq) return;
-  const long long r = hr / a.hq;
-  const int h = (int)(hr % a.hq);
-  float m = -INFINITY, l = 0.f, o[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) o[k] = 0.f;
-  for (int p = 0; p < a.pieces; ++p) m = fmaxf(m, a.part_ml[((long long)p * a.hq + h) * a.nq + r].x);
-  const float u = m == -INFINITY ? 0.f : m;
-  for (int p = 0; p < a.pieces; ++p) {
-    const long long slot = ((long long)p * a.hq + h) * a.nq + r;
-    const float2 ml = a.part_ml[slot];
-    if (ml.y == 0.f) continue;      // no key of the piece was seen: its share was not written where it has no tile
-    const float f = exp2f(ml.x - u);
-    l = fmaf(ml.y, f, l);
-    const float4 x = *reinterpret_cast<const float4*>(a.part_o + slot * a.d + c), y = *reinterpret_cast<const float4*>(a.part_o + slot * a.d + c + 4);
-    o[0] = fmaf(x.x, f, o[0]); o[1] = fmaf(x.y, f, o[1]); o[2] = fmaf(x.z, f, o[2]); o[3] = fmaf(x.w, f, o[3]);
-    o[4] = fmaf(y.x, f, o[4]); o[5] = fmaf(y.y, f, o[5]); o[6] = fmaf(y.z, f, o[6]); o[7] = fmaf(y.w, f, o[7]);
-  }
-  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  const long long at = hr * a.d + c;
-#pragma unroll
-  for (int k = 0; k < 8; k += 2) packed::store_rest<T>(static_cast<T*>(a.out) + at + k, a.out_rest ? static_cast<T*>(a.out_rest) + at + k : nullptr, o[k] * inv, o[k + 1] * inv);
-  if (c == 0 && a.lse) a.lse[(long long)h * a.nq + r] = l == 0.f ? -INFINITY : m + log2f(l);
-}
-// sums the pieces' shares of dq, dk, dv (blockIdx.y), a thread per eight values
-template <typename T>
-__global__ void __launch_bounds__(256) sum_kernel(const PackedArgs a, int first, int pieces_q, int pieces_kv, long long values_q, long long values_kv,
-                                                  long long stride_q, long long stride_kv) {
-  const int which = first + blockIdx.y, pieces = which ? pieces_kv : pieces_q;
-  const long long e = ((long long)blockIdx.x * 256 + threadIdx.x) * 8, values = which ? values_kv : values_q, stride = which ? stride_kv : stride_q;
-  if (e >= values) return;
-  const float* src = a.share[which] + e;
-  float o[8];
-#pragma unroll
-  for (int k = 0; k < 8; ++k) o[k] = 0.f;
-  for (int p = 0; p < pieces; ++p) {
-    const float4 x = *reinterpret_cast<const float4*>(src + p * stride), y = *reinterpret_cast<const float4*>(src + p * stride + 4);
-    o[0] += x.x; o[1] += x.y; o[2] += x.z; o[3] += x.w; o[4] += y.x; o[5] += y.y; o[6] += y.z; o[7] += y.w;
-  }
-  T* dst = static_cast<T*>(which == 0 ? a.dq : which == 1 ? a.dk : a.dv) + e;
-#pragma unroll
-  for (int k = 0; k < 8; k += 2) packed::store2(dst + k, o[k], o[k + 1]);
-}
-
 // float32 rows -> three bfloat16 terms, (rows, heads, 3, DW), zeros behind d; a thread per eight values, up to four operands
 struct SplitArgs { Rows src[4]; __nv_bfloat16* dst[4]; int rows[4], heads[4]; };
 template <int DW>
@@ -883,16 +844,18 @@ template <typename T, int TERMS, int DW> int maps_of(Maps* m, cudaStream_t st, c
   if (!reverse) m->g = m->q;
   return kOk;
 }
-template <int TERMS, int DW, auto kernel> int launch(int64_t grid, bool stats, cudaStream_t st, const PackedArgs& a, const Maps& m) {
+template <int TERMS, int DW> constexpr int reverse_smem(bool stats) {
   using G = Geometry<TERMS, DW>;
-  const int smem = 1024 + (2 + G::kRing) * G::kSubs * (int)G::kSub + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail);
+  return 1024 + (2 + G::kRing) * G::kSubs * (int)G::kSub + (stats ? 4 * kTile * 4 : 0) + (int)sizeof(Tail);
+}
+template <auto kernel> int launch(int64_t grid, int threads, int smem, cudaStream_t st, const PackedArgs& a, const Maps& m) {
   packed::allow_smem<kernel>(smem);
   if (grid > 0x7fffffff) return kTooLarge;
-  kernel<<<(unsigned)grid, kThreads, smem, st>>>(a, m);
+  kernel<<<(unsigned)grid, threads, smem, st>>>(a, m);
   count_launch();
   return kOk;
 }
-template <typename T, int TERMS, int DW> int forward_of(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace) {
+template <typename T, int TERMS, int DW, int TILES> int forward_of(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace) {
   Maps m;
   int rc = maps_of<T, TERMS, DW>(&m, st, a, false, workspace);
   if (rc) return rc;
@@ -901,13 +864,10 @@ template <typename T, int TERMS, int DW> int forward_of(cudaStream_t st, PackedA
     a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + (TERMS == 3 ? packed_split_bytes(a.nq, a.nkv, a.hq, a.hk, a.d, false) : 0));
     a.part_ml = reinterpret_cast<float2*>(a.part_o + (long long)a.pieces * a.nq * a.hq * a.d);
   }
-  rc = launch<TERMS, DW, forward_kernel<T, TERMS, DW>>((int64_t)n_items * a.hq * a.pieces, false, st, a, m);
+  using F = Forward<TERMS, DW, TILES>;
+  rc = launch<forward_kernel<T, TERMS, DW, TILES>>((int64_t)n_items * a.hq * a.pieces, F::kThreads, F::kSmem, st, a, m);
   if (rc || a.pieces == 1) return rc;
-  const int64_t ctas = ((int64_t)a.rows * a.hq * (a.d / 8) + 255) / 256;
-  if (ctas > 0x7fffffff) return kTooLarge;
-  join_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, a.rows);
-  count_launch();
-  return kOk;
+  return packed_join<T>(st, a);
 }
 template <typename T, int TERMS, int DW>
 int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, const PackedPieces& pieces, void* workspace) {
@@ -920,26 +880,26 @@ int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, cons
   if (pieces.dkv > 1) { a.share[1] = share; a.share[2] = share + pieces.dkv * stride_kv; }
   a.items = items_q;
   a.pieces = pieces.dq;
-  rc = launch<TERMS, DW, dq_kernel<T, TERMS, DW>>((int64_t)n_q * a.hq * a.pieces, false, st, a, m);
+  rc = launch<dq_kernel<T, TERMS, DW>>((int64_t)n_q * a.hq * a.pieces, kThreads, reverse_smem<TERMS, DW>(false), st, a, m);
   if (rc) return rc;
   a.items = items_kv;
   a.pieces = pieces.dkv;
-  rc = launch<TERMS, DW, dkv_kernel<T, TERMS, DW>>((int64_t)n_kv * a.hk * a.pieces, true, st, a, m);
+  rc = launch<dkv_kernel<T, TERMS, DW>>((int64_t)n_kv * a.hk * a.pieces, kThreads, reverse_smem<TERMS, DW>(true), st, a, m);
   if (rc || (pieces.dq == 1 && pieces.dkv == 1)) return rc;
-  const long long values_q = (long long)a.rows * a.hq * a.d, values_kv = (long long)a.rows_kv * a.hk * a.d;
-  const int first = pieces.dq > 1 ? 0 : 1, many = (pieces.dkv > 1 ? 3 : 1) - first;
-  const int64_t ctas = (std::max(pieces.dq > 1 ? values_q : 0, pieces.dkv > 1 ? values_kv : 0) / 8 + 255) / 256;
-  if (ctas > 0x7fffffff) return kTooLarge;
-  sum_kernel<T><<<dim3((unsigned)ctas, many), 256, 0, st>>>(a, first, pieces.dq, pieces.dkv, values_q, values_kv, stride_q, stride_kv);
-  count_launch();
-  return kOk;
+  return packed_sum<T>(st, a, pieces.dq, pieces.dkv);
 }
 
 }  // namespace
 
 template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace) {
-  if constexpr (sizeof(T) == 2) return a.d <= 64 ? forward_of<T, 1, 64>(st, a, n_items, pieces, workspace) : forward_of<T, 1, 128>(st, a, n_items, pieces, workspace);
-  else return a.d <= 32 ? forward_of<T, 3, 32>(st, a, n_items, pieces, workspace) : forward_of<T, 3, 64>(st, a, n_items, pieces, workspace);
+  const bool one = packed_one_tile(sizeof(T) == 4, a.d, a.longest_kv);
+  if constexpr (sizeof(T) == 2) {
+    if (a.d > 64) return one ? forward_of<T, 1, 128, 1>(st, a, n_items, pieces, workspace) : forward_of<T, 1, 128, 2>(st, a, n_items, pieces, workspace);
+    return one ? forward_of<T, 1, 64, 1>(st, a, n_items, pieces, workspace) : forward_of<T, 1, 64, 2>(st, a, n_items, pieces, workspace);
+  } else {
+    if (a.d > 32) return forward_of<T, 3, 64, 2>(st, a, n_items, pieces, workspace);
+    return one ? forward_of<T, 3, 32, 1>(st, a, n_items, pieces, workspace) : forward_of<T, 3, 32, 2>(st, a, n_items, pieces, workspace);
+  }
 }
 template <typename T>
 int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, const int4* items_kv, int n_kv, const PackedPieces& pieces, void* workspace) {

@@ -286,12 +286,12 @@ template <int TERMS, int DW> struct Loader {
   }
 };
 
-__device__ __forceinline__ void alloc_tmem(uint32_t* where) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(where)), "r"(512) : "memory");
+__device__ __forceinline__ void alloc_tmem(uint32_t* where, int columns = 512) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(where)), "r"(columns) : "memory");
   asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
 }
-__device__ __forceinline__ void free_tmem(uint32_t tmem) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+__device__ __forceinline__ void free_tmem(uint32_t tmem, int columns = 512) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
 }  // namespace tc
