@@ -14,13 +14,17 @@ namespace so3lr {
 namespace {
 
 // The image of a layout (int32): a header, the offsets of both sides, and tables of work items {structure, tile, first, last}.
-// Tables of query tiles: 64 rows (warp-level kernels), 128 and 256 (tensor cores, reverse and forward); of key tiles: 64 and 128.
+// Tables of query tiles: 64 rows (warp-level kernels), 128 and 256 (tensor cores, reverse and forward); of key tiles: 64 and 128; of both
+// with 16 rows where no structure has more than kShortRows.
 enum Head : int { kMagicAt, kN, kCausal, kRowsQ, kRowsKv, kMaxQ, kStartQ, kStartKv, kItemsQ, kNItemsQ, kItemsKv, kNItemsKv, kItemsSplit, kNItemsSplit,
                   kSplitFirst, kCombine, kTotal, kItemsQ128, kNItemsQ128, kItemsQ256, kNItemsQ256, kItemsKv128, kNItemsKv128, kMaxKv,
-                  kWalkQ, kWalkKv /* tiles of 64 that the items of a table walk over in all */, kWalkQ128, kWalkQ256, kWalkKv128 /* tiles of 128 that the items of a table walk over in all */, kHeadInts = 32 };
+                  kWalkQ, kWalkKv /* tiles of 64 that the items of a table walk over in all */, kWalkQ128, kWalkQ256, kWalkKv128 /* tiles of 128 that the items of a table walk over in all */,
+                  kItemsQ16, kNItemsQ16, kItemsKv16, kNItemsKv16, kHeadInts = 48 };
 constexpr int kMagic = 0x53334c50;
-constexpr int kTables = 5, kTileRows[kTables] = {kPackTile, kPackTile, 128, 256, 128}, kTableAt[kTables] = {kItemsQ, kItemsKv, kItemsQ128, kItemsQ256, kItemsKv128};
-constexpr bool kOfKeys[kTables] = {false, true, false, false, true};
+constexpr int kTables = 7, kTileRows[kTables] = {kPackTile, kPackTile, 128, 256, 128, 16, 16};
+constexpr int kTableAt[kTables] = {kItemsQ, kItemsKv, kItemsQ128, kItemsQ256, kItemsKv128, kItemsQ16, kItemsKv16};
+constexpr bool kOfKeys[kTables] = {false, true, false, false, true, false, true};
+constexpr int kShortRows = 48;
 
 int64_t align4(int64_t x) { return (x + 3) & ~3LL; }
 
@@ -39,6 +43,11 @@ bool valid(int n, const int32_t* sq, const int32_t* sk) {
   return true;
 }
 
+bool all_short(int n, const int32_t* sq, const int32_t* sk) {
+  for (int i = 0; i < n; ++i) if (sq[i + 1] - sq[i] > kShortRows || sk[i + 1] - sk[i] > kShortRows) return false;
+  return true;
+}
+
 Counts count(int n, const int32_t* sq, const int32_t* sk) {
   Counts c;
   const int chunk = split_length(sk[n]);
@@ -47,6 +56,7 @@ Counts count(int n, const int32_t* sq, const int32_t* sk) {
     for (int t = 0; t < kTables; ++t) c.items[t] += ((kOfKeys[t] ? lk : lq) + kTileRows[t] - 1) / kTileRows[t];
     if (lq > 0) c.split += std::max<int64_t>(1, (lk + chunk - 1) / chunk);
   }
+  if (!all_short(n, sq, sk)) c.items[5] = c.items[6] = 0;
   c.total = kHeadInts + 3 * align4(n + 1) + 4 * c.split;
   for (int t = 0; t < kTables; ++t) c.total += 4 * c.items[t];
   return c;
@@ -74,6 +84,7 @@ void build_image(int n, const int32_t* sq, const int32_t* sk, bool causal, int32
   std::vector<Item> items;
   for (int t = 0; t < kTables; ++t) {
     const int64_t rows = kTileRows[t];
+    if (c.items[t] == 0) continue;
     items.clear();
     items.reserve(c.items[t]);
     for (int s = 0; s < n; ++s) {
@@ -89,7 +100,7 @@ void build_image(int n, const int32_t* sq, const int32_t* sk, bool causal, int32
     put(im + im[kTableAt[t]], items);
     int64_t walk = 0;
     for (const Item& i : items) walk += t < 2 ? (i.last - i.first + 63) / 64 : (i.last - i.first + 127) / 128;
-    im[kWalkQ + t] = (int32_t)std::min<int64_t>(walk, 0x7fffffff);
+    if (t < 5) im[kWalkQ + t] = (int32_t)std::min<int64_t>(walk, 0x7fffffff);
   }
   const int chunk = split_length(sk[n]);
   int32_t* split = im + im[kItemsSplit];
@@ -121,11 +132,18 @@ bool shape_ok(const int32_t* im, const so3lr_b200_attention_shape* a) {
          a->scale > 0.f && std::isfinite(a->scale);
 }
 
+// Batches of structures this short take warp-level CTAs of one warp and 16 rows.  Forward and backward, 16 rows / 64 rows, us: 512 structures of 10
+// to 40, float32 4 heads x 32, 74 / 86; 160 of 28 to 56, bfloat16 8 x 32 41 / 39; 300 of 10 to 32, bfloat16 8 x 64, 48 / 74, 160 of 28 to
+// 56 67 / 58; 600 of up to 17, bfloat16 32 x 96, 290 / 591; 316 of 17 to 32, float32 2 x 128, 144 / 132.
+int short_rows(int d) { return d <= 32 ? kShortRows : d <= 64 ? 40 : 24; }
+
 PackedArgs common(const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a) {
   PackedArgs p;
   p.start_q = dev + im[kStartQ]; p.start_kv = dev + im[kStartKv]; p.split_first = dev + im[kSplitFirst];
   p.rows = im[kRowsQ]; p.rows_kv = im[kRowsKv]; p.longest_kv = im[kMaxKv];
-  p.stages = im[kMaxKv] <= (a->type == kF32 && a->d > 64 ? 32 : 64) ? 1 : 2;
+  if (std::max(im[kMaxQ], im[kMaxKv]) <= short_rows(a->d)) p.tile_rows = 16;
+  p.stages = im[kMaxKv] <= (p.tile_rows == 16 || (a->type == kF32 && a->d > 64) ? 32 : 64) ? 1 : 2;
+  p.rev_stages = im[kMaxKv] <= 32 && (int64_t)im[kMaxQ] * p.group <= 32 ? 1 : 2;
   p.nq = (int)a->rows_q; p.nkv = (int)a->rows_kv; p.hq = a->heads_q; p.hk = a->heads_kv; p.group = a->heads_q / a->heads_kv; p.d = a->d; p.causal = im[kCausal];
   p.scale = a->scale; p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   return p;
@@ -201,7 +219,7 @@ const int4* table(const int32_t* im, const int32_t* dev, int field) { return rei
 
 template <typename T>
 int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
-  if (few_rows(im, a)) {
+  if (few_rows(im, a) && (p.tile_rows != 16 || im[kMaxQ] * p.group <= 16)) {
     p.items = table(im, dev, kItemsSplit);
     p.part_rows = im[kMaxQ] * p.group;
     p.part_o = static_cast<float*>(workspace);
@@ -213,11 +231,12 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
     p.items = table(im, dev, one ? kItemsQ128 : kItemsQ256);
     return packed_forward_tc<T>(st, p, im[one ? kNItemsQ128 : kNItemsQ256], pieces(im, a), workspace);
   }
-  p.items = table(im, dev, kItemsQ);
+  const bool small = p.tile_rows == 16;
+  p.items = table(im, dev, small ? kItemsQ16 : kItemsQ);
   p.pieces = pieces(im, a).forward;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)p.pieces * p.nq * p.hq * p.d);
-  const int rc = packed_forward_mma<T>(st, p, im[kNItemsQ]);
+  const int rc = packed_forward_mma<T>(st, p, im[small ? kNItemsQ16 : kNItemsQ]);
   return rc || p.pieces == 1 ? rc : packed_join<T>(st, p);
 }
 
@@ -232,13 +251,14 @@ int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
   float* share = static_cast<float*>(workspace);
   if (n.dq > 1) { p.share[0] = share; share += n.dq * stride_q; }
   if (n.dkv > 1) { p.share[1] = share; p.share[2] = share + n.dkv * stride_kv; }
-  p.items = table(im, dev, kItemsQ);
+  const bool small = p.tile_rows == 16;
+  p.items = table(im, dev, small ? kItemsQ16 : kItemsQ);
   p.pieces = n.dq;
-  if (im[kNItemsQ]) rc = packed_dq_mma<T>(st, p, im[kNItemsQ]);
+  if (im[kNItemsQ]) rc = packed_dq_mma<T>(st, p, im[small ? kNItemsQ16 : kNItemsQ]);
   if (rc) return rc;
-  p.items = table(im, dev, kItemsKv);
+  p.items = table(im, dev, small ? kItemsKv16 : kItemsKv);
   p.pieces = n.dkv;
-  if (im[kNItemsKv]) rc = packed_dkv_mma<T>(st, p, im[kNItemsKv]);
+  if (im[kNItemsKv]) rc = packed_dkv_mma<T>(st, p, im[small ? kNItemsKv16 : kNItemsKv]);
   return rc || (n.dq == 1 && n.dkv == 1) ? rc : packed_sum<T>(st, p, n.dq, n.dkv);
 }
 

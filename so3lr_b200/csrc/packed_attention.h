@@ -38,7 +38,8 @@ struct PackedArgs {
   float* share[3] = {};         // (reverse) in share: (pieces, heads, rows, d) of dq, dk, dv
   int rows = 0, rows_kv = 0;    // of the layout
   int longest_kv = 0;           // keys of its longest structure
-  int stages = 2;               // buffers for the keys in the warp-level forward kernel: one where they all fit into it
+  int stages = 2, rev_stages = 2;         // buffers for the walked side in the warp-level kernels: one where all of it fits into it
+  int tile_rows = 64;           // rows of a CTA there: 64 or 16
   int nq = 0, nkv = 0, hq = 0, hk = 0, group = 1, d = 0, causal = 0;
   float scale = 0.f, scale_log2 = 0.f;                // scale * log2(e): the softmax runs on powers of two
   int* err = nullptr;

@@ -9,7 +9,8 @@
 // Two kernels form the exponentials twice, but every sum has one owner: no atomics, results do not change from run to run, and the
 // gradients of shared keys need no second pass.
 //
-// A CTA has four warps with 16 rows each; the tile of the other side is double-buffered by 16-byte asynchronous copies that fill rows and
+// A CTA has four warps with 16 rows each, or one where all structures are short (a CTA per 16 rows and head: no warp is without rows, and many
+// CTAs hide each other's start); the tile of the other side is double-buffered by 16-byte asynchronous copies that fill rows and
 // columns that are not there with zeros.  The accumulator fragment of one product is the A fragment of the next, so P and dS never leave
 // the registers (and are rounded to the inputs' type on the way into the second product: their error then is that of one rounding of an
 // input).  float32 runs as three products of operands split into two tf32 numbers each (hi hi + hi lo + lo hi): 2^-21 of the
@@ -83,12 +84,12 @@ template <typename T, int DP> struct Tile {
 };
 
 // rows [r0, r0 + N) of one head into a tile; row r is there where r < r1
-template <typename T, int DP, int N>
+template <typename T, int DP, int N, int THREADS>
 __device__ __forceinline__ void load_rows(uint32_t tile, const Rows& src, int head, long long base, int r0, int r1, int d, int tid) {
   using L = Tile<T, DP>;
   const T* p = static_cast<const T*>(src.p) + head * src.head;
 #pragma unroll
-  for (int i = tid; i < N * L::kChunks; i += 128) {
+  for (int i = tid; i < N * L::kChunks; i += THREADS) {
     const int r = i / L::kChunks, c = i % L::kChunks;
     const bool ok = r0 + r < r1 && c * L::kPer < d;
     copy16(tile + r * L::kStride + c * 16, ok ? p + (base + r0 + r) * src.row + c * L::kPer : p, ok);
@@ -246,26 +247,26 @@ __device__ __forceinline__ void store_rest(T* p, T* rest, float x, float y) {
   }
 }
 
-template <typename T, int DP> constexpr int key_tile() { return sizeof(T) == 4 && DP > 64 ? 32 : 64; }
-template <typename T, int DP> int forward_smem(int stages) { return (kPackTile + 2 * stages * key_tile<T, DP>()) * Tile<T, DP>::kStride; }
+template <typename T, int DP, int NW> constexpr int key_tile() { return NW == 1 || (sizeof(T) == 4 && DP > 64) ? 32 : 64; }
+template <typename T, int DP, int NW> int forward_smem(int stages) { return (16 * NW + 2 * stages * key_tile<T, DP, NW>()) * Tile<T, DP>::kStride; }
 constexpr int kRevTile = 32;   // rows of the walked side in the reverse kernels: two accumulators of 16 x DP are held at the same time
-template <typename T, int DP> constexpr int reverse_smem() { return (2 * kPackTile + 4 * kRevTile) * Tile<T, DP>::kStride + 4 * kRevTile * 4; }
+template <typename T, int DP, int NW> int reverse_smem(int stages) { return (32 * NW + 2 * stages * kRevTile) * Tile<T, DP>::kStride + 4 * kRevTile * 4; }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 // SPLIT: rows are (token, head of the group) of ONE key head, a structure has at most 64 of them, and the item is a stretch of the keys;
 // what it finds is joined by combine_kernel, or written where the structure has one stretch only.
-template <typename T, int DP, bool SPLIT>
-__global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
+template <typename T, int DP, bool SPLIT, int NW>
+__global__ void __launch_bounds__(32 * NW) forward_kernel(const PackedArgs a) {
   using L = Tile<T, DP>;
-  constexpr int BN = key_tile<T, DP>(), NT = BN / 8;
+  constexpr int BN = key_tile<T, DP, NW>(), NT = BN / 8, kRows = 16 * NW, kThreads = 32 * NW;
   extern __shared__ __align__(16) unsigned char smem[];
-  const uint32_t sq = smem_addr(smem), sk = sq + kPackTile * L::kStride;
+  const uint32_t sq = smem_addr(smem), sk = sq + kRows * L::kStride;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int heads = SPLIT ? a.hk : a.hq, piece = SPLIT ? 0 : blockIdx.x % a.pieces, index = SPLIT ? blockIdx.x : blockIdx.x / a.pieces, unit = index / heads;
   const int4 item = a.items[unit];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
   const int G = SPLIT ? a.group : 1, hy = index % heads, kvh = SPLIT ? hy : hy / a.group;
-  const int rows = lq * G, row0 = SPLIT ? 0 : item.y * kPackTile;
+  const int rows = lq * G, row0 = SPLIT ? 0 : item.y * kRows;
   const int share = SPLIT ? 0 : ((item.w + BN - 1) / BN + a.pieces - 1) / a.pieces * BN;      // keys of a piece
   const int k0 = SPLIT ? item.z : min(item.w, piece * share), k1 = SPLIT ? item.w : min(item.w, k0 + share);
   const int nt = (max(k1 - k0, 0) + BN - 1) / BN, stages = a.stages;
@@ -274,7 +275,7 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
   {  // queries
     const T* p = static_cast<const T*>(a.q.p);
 #pragma unroll 4
-    for (int i = tid; i < kPackTile * L::kChunks; i += 128) {
+    for (int i = tid; i < kRows * L::kChunks; i += kThreads) {
       const int r = i / L::kChunks, c = i % L::kChunks, pr = row0 + r;
       const bool ok = pr < rows && c * L::kPer < a.d;
       const int tok = SPLIT ? pr / G : pr, head = SPLIT ? hy * G + pr % G : hy;
@@ -284,8 +285,8 @@ __global__ void __launch_bounds__(128) forward_kernel(const PackedArgs a) {
   auto load = [&](int it) {
     if (it < nt) {
       const int buf = it & (stages - 1), b = k0 + it * BN;
-      load_rows<T, DP, BN>(sk + buf * BN * L::kStride, a.k, kvh, c0, b, k1, a.d, tid);
-      load_rows<T, DP, BN>(sv + buf * BN * L::kStride, a.v, kvh, c0, b, k1, a.d, tid);
+      load_rows<T, DP, BN, kThreads>(sk + buf * BN * L::kStride, a.k, kvh, c0, b, k1, a.d, tid);
+      load_rows<T, DP, BN, kThreads>(sv + buf * BN * L::kStride, a.v, kvh, c0, b, k1, a.d, tid);
     }
     copy_commit();
   };
@@ -644,27 +645,27 @@ __global__ void __launch_bounds__(256) delta_kernel(const PackedArgs a, int rows
   if (r < rows && part == 0) a.delta[(long long)h * a.nq + r] = sum;
 }
 
-// dq of a tile of 64 queries of one head
-template <typename T, int DP>
-__global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
+// dq of a tile of 16 NW queries of one head
+template <typename T, int DP, int NW>
+__global__ void __launch_bounds__(32 * NW) dq_kernel(const PackedArgs a) {
   using L = Tile<T, DP>;
-  constexpr int BN = kRevTile, NT = BN / 8;
+  constexpr int BN = kRevTile, NT = BN / 8, kRows = 16 * NW, kThreads = 32 * NW;
   extern __shared__ __align__(16) unsigned char smem[];
-  const uint32_t sq = smem_addr(smem), sg = sq + kPackTile * L::kStride, sk = sg + kPackTile * L::kStride, sv = sk + 2 * BN * L::kStride;
+  const uint32_t sq = smem_addr(smem), sg = sq + kRows * L::kStride, sk = sg + kRows * L::kStride, sv = sk + a.rev_stages * BN * L::kStride;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int piece = blockIdx.x % a.pieces, index = blockIdx.x / a.pieces;
   const int4 item = a.items[index / a.hq];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = index % a.hq, kvh = h / a.group, row0 = item.y * kPackTile;
+  const int h = index % a.hq, kvh = h / a.group, row0 = item.y * kRows;
   const int share = ((item.w + BN - 1) / BN + a.pieces - 1) / a.pieces * BN, k0 = min(item.w, piece * share), k1 = min(item.w, k0 + share);
   const int nt = (max(k1 - k0, 0) + BN - 1) / BN;
-  load_rows<T, DP, kPackTile>(sq, a.q, h, q0, row0, lq, a.d, tid);
-  load_rows<T, DP, kPackTile>(sg, a.g, h, q0, row0, lq, a.d, tid);
+  load_rows<T, DP, kRows, kThreads>(sq, a.q, h, q0, row0, lq, a.d, tid);
+  load_rows<T, DP, kRows, kThreads>(sg, a.g, h, q0, row0, lq, a.d, tid);
   auto load = [&](int it) {
     if (it < nt) {
-      const int buf = it & 1, b = k0 + it * BN;
-      load_rows<T, DP, BN>(sk + buf * BN * L::kStride, a.k, kvh, c0, b, k1, a.d, tid);
-      load_rows<T, DP, BN>(sv + buf * BN * L::kStride, a.v, kvh, c0, b, k1, a.d, tid);
+      const int buf = it & (a.rev_stages - 1), b = k0 + it * BN;
+      load_rows<T, DP, BN, kThreads>(sk + buf * BN * L::kStride, a.k, kvh, c0, b, k1, a.d, tid);
+      load_rows<T, DP, BN, kThreads>(sv + buf * BN * L::kStride, a.v, kvh, c0, b, k1, a.d, tid);
     }
     copy_commit();
   };
@@ -679,10 +680,9 @@ __global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
   for (int it = 0; it < nt; ++it) {
-    load(it + 1);
-    copy_wait<1>();
+    if (a.rev_stages == 2) { load(it + 1); copy_wait<1>(); } else { if (it > 0) load(it); copy_wait<0>(); }
     __syncthreads();
-    const int kb = k0 + it * BN, buf = it & 1;
+    const int kb = k0 + it * BN, buf = it & (a.rev_stages - 1);
     if (wr < lq && kb <= lim_hi) {
       float p[NT][4], dp[NT][4];
       const int cols = k1 - kb;
@@ -722,28 +722,28 @@ __global__ void __launch_bounds__(128) dq_kernel(const PackedArgs a) {
   }
 }
 
-// dk and dv of a tile of 64 keys of one key head: rows of the products are keys, columns queries
-template <typename T, int DP>
-__global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
+// dk and dv of a tile of 16 NW keys of one key head: rows of the products are keys, columns queries
+template <typename T, int DP, int NW>
+__global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
   using L = Tile<T, DP>;
-  constexpr int BN = kRevTile, NT = BN / 8;
+  constexpr int BN = kRevTile, NT = BN / 8, kRows = 16 * NW, kThreads = 32 * NW;
   extern __shared__ __align__(16) unsigned char smem[];
-  const uint32_t sk = smem_addr(smem), sv = sk + kPackTile * L::kStride, sq = sv + kPackTile * L::kStride, sg = sq + 2 * BN * L::kStride;
-  float* se = reinterpret_cast<float*>(smem + (2 * kPackTile + 4 * BN) * L::kStride);   // [2][BN] lse, [2][BN] delta
+  const uint32_t sk = smem_addr(smem), sv = sk + kRows * L::kStride, sq = sv + kRows * L::kStride, sg = sq + a.rev_stages * BN * L::kStride;
+  float* se = reinterpret_cast<float*>(smem + (2 * kRows + 2 * a.rev_stages * BN) * L::kStride);   // [2][BN] lse, [2][BN] delta
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int piece = blockIdx.x % a.pieces, index = blockIdx.x / a.pieces;
   const int4 item = a.items[index / a.hk];
   const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int kvh = index % a.hk, row0 = item.y * kPackTile, i0 = item.z, i1 = item.w;
+  const int kvh = index % a.hk, row0 = item.y * kRows, i0 = item.z, i1 = item.w;
   const int per = (max(i1 - i0, 0) + BN - 1) / BN, all = per * a.group, share = (all + a.pieces - 1) / a.pieces, j0 = min(all, piece * share);
   const int nt = min(share, all - j0);      // from tile j0 on
-  load_rows<T, DP, kPackTile>(sk, a.k, kvh, c0, row0, lk, a.d, tid);
-  load_rows<T, DP, kPackTile>(sv, a.v, kvh, c0, row0, lk, a.d, tid);
+  load_rows<T, DP, kRows, kThreads>(sk, a.k, kvh, c0, row0, lk, a.d, tid);
+  load_rows<T, DP, kRows, kThreads>(sv, a.v, kvh, c0, row0, lk, a.d, tid);
   auto load = [&](int it) {
     if (it < nt) {
-      const int buf = it & 1, h = kvh * a.group + (j0 + it) / per, b = i0 + ((j0 + it) % per) * BN;
-      load_rows<T, DP, BN>(sq + buf * BN * L::kStride, a.q, h, q0, b, i1, a.d, tid);
-      load_rows<T, DP, BN>(sg + buf * BN * L::kStride, a.g, h, q0, b, i1, a.d, tid);
+      const int buf = it & (a.rev_stages - 1), h = kvh * a.group + (j0 + it) / per, b = i0 + ((j0 + it) % per) * BN;
+      load_rows<T, DP, BN, kThreads>(sq + buf * BN * L::kStride, a.q, h, q0, b, i1, a.d, tid);
+      load_rows<T, DP, BN, kThreads>(sg + buf * BN * L::kStride, a.g, h, q0, b, i1, a.d, tid);
       if (tid < BN) {
         const bool ok = b + tid < i1;
         const long long at = (long long)h * a.nq + q0 + b + tid;
@@ -761,10 +761,9 @@ __global__ void __launch_bounds__(128) dkv_kernel(const PackedArgs a) {
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) { dk[n][0] = dk[n][1] = dk[n][2] = dk[n][3] = 0.f; dv[n][0] = dv[n][1] = dv[n][2] = dv[n][3] = 0.f; }
   for (int it = 0; it < nt; ++it) {
-    load(it + 1);
-    copy_wait<1>();
+    if (a.rev_stages == 2) { load(it + 1); copy_wait<1>(); } else { if (it > 0) load(it); copy_wait<0>(); }
     __syncthreads();
-    const int ib = i0 + ((j0 + it) % per) * BN, buf = it & 1;
+    const int ib = i0 + ((j0 + it) % per) * BN, buf = it & (a.rev_stages - 1);
     if (wr < lk && ib + BN - 1 >= lim_lo) {
       float p[NT][4], ds[NT][4];
       const int cols = i1 - ib;
@@ -842,26 +841,36 @@ int launch(int64_t grid, int threads, int smem, cudaStream_t st, const PackedArg
 }  // namespace packed
 
 template <typename T> int packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) return packed::launch<packed::forward_kernel<T, DP, false>>((int64_t)n_items * a.hq * a.pieces, 128, packed::forward_smem<T, DP>(a.stages), st, a);
+  const int64_t grid = (int64_t)n_items * a.hq * a.pieces;
+#define CALL(T, DP)                                                                                                                             \
+  return a.tile_rows == 16 ? packed::launch<packed::forward_kernel<T, DP, false, 1>>(grid, 32, packed::forward_smem<T, DP, 1>(a.stages), st, a) \
+                           : packed::launch<packed::forward_kernel<T, DP, false, 4>>(grid, 128, packed::forward_smem<T, DP, 4>(a.stages), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
 template <typename T> int packed_forward_split(cudaStream_t st, const PackedArgs& a, int n_items, int n_structures, bool combine) {
-#define CALL(T, DP)                                                                                                                           \
-  const int rc = a.part_rows <= packed::kNarrowRows                                                                                           \
-                     ? packed::launch<packed::narrow_kernel<T, DP>>((int64_t)n_items * a.hk, 128, packed::narrow_smem<T, DP>(), st, a)        \
-                     : packed::launch<packed::forward_kernel<T, DP, true>>((int64_t)n_items * a.hk, 128, packed::forward_smem<T, DP>(a.stages), st, a); \
+  const int64_t grid = (int64_t)n_items * a.hk;
+#define CALL(T, DP)                                                                                                                             \
+  const int rc = a.part_rows <= packed::kNarrowRows                                                                                             \
+                     ? packed::launch<packed::narrow_kernel<T, DP>>(grid, 128, packed::narrow_smem<T, DP>(), st, a)                             \
+                     : packed::launch<packed::forward_kernel<T, DP, true, 4>>(grid, 128, packed::forward_smem<T, DP, 4>(a.stages), st, a);      \
   return rc || !combine ? rc : packed::launch<packed::combine_kernel<T, DP>>((int64_t)n_structures * a.hk, 256, 0, st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
 template <typename T> int packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) return packed::launch<packed::dq_kernel<T, DP>>((int64_t)n_items * a.hq * a.pieces, 128, packed::reverse_smem<T, DP>(), st, a);
+  const int64_t grid = (int64_t)n_items * a.hq * a.pieces;
+#define CALL(T, DP)                                                                                                                        \
+  return a.tile_rows == 16 ? packed::launch<packed::dq_kernel<T, DP, 1>>(grid, 32, packed::reverse_smem<T, DP, 1>(a.rev_stages), st, a)    \
+                           : packed::launch<packed::dq_kernel<T, DP, 4>>(grid, 128, packed::reverse_smem<T, DP, 4>(a.rev_stages), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }
 template <typename T> int packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items) {
-#define CALL(T, DP) return packed::launch<packed::dkv_kernel<T, DP>>((int64_t)n_items * a.hk * a.pieces, 128, packed::reverse_smem<T, DP>(), st, a);
+  const int64_t grid = (int64_t)n_items * a.hk * a.pieces;
+#define CALL(T, DP)                                                                                                                        \
+  return a.tile_rows == 16 ? packed::launch<packed::dkv_kernel<T, DP, 1>>(grid, 32, packed::reverse_smem<T, DP, 1>(a.rev_stages), st, a)   \
+                           : packed::launch<packed::dkv_kernel<T, DP, 4>>(grid, 128, packed::reverse_smem<T, DP, 4>(a.rev_stages), st, a);
   SO3LR_PACKED_WIDTHS(T, CALL)
 #undef CALL
 }

@@ -97,6 +97,7 @@ CASES = [
     (ODD + [650], None, 2, 2, 32, False), (ODD + [650], None, 4, 2, 64, True), ([601, 7, 0, 640], None, 2, 1, 16, True),
     (ODD + [301], None, 3, 1, 112, False), ([650, 40, 1], [5, 700, 130], 2, 1, 48, True), ([1300], None, 2, 2, 64, False),
     ([20, 31, 5, 1, 0, 16], None, 2, 2, 64, False), ([33, 40, 10], None, 4, 2, 32, True), ([9, 2, 16], None, 2, 1, 128, True),
+    ([17, 24, 1, 0, 16], None, 4, 2, 96, False), ([48, 31, 16, 2], None, 2, 2, 16, True), ([3, 30, 8], [40, 2, 0], 8, 2, 64, False),
     ([300, 1, 77], None, 4, 4, 80, True), ([257], None, 2, 1, 16, True), ([511, 513], None, 1, 1, 128, False), ([1000], None, 2, 2, 48, True),
     # more keys than queries, fewer (rows that see nothing), none at all
     ([5, 70, 100, 3, 0, 90], [64, 200, 40, 0, 10, 1], 4, 2, 64, True), ([5, 70, 100, 3, 0, 90], [64, 200, 40, 0, 10, 1], 4, 2, 64, False),

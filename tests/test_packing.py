@@ -26,7 +26,7 @@ def items(im, at, n):
 
 
 LAYOUTS = [([0], [0]), ([1], [1]), ([64], [64]), ([65, 0, 63], [65, 0, 63]), ([3, 70, 129], [200, 0, 65]), ([1] * 5, [17, 0, 513, 1024, 4000]),
-           ([130, 5], [3, 1])]
+           ([130, 5], [3, 1]), ([32, 0, 17, 5], [16, 3, 32, 1])]
 
 
 @pytest.mark.parametrize("causal", [False, True])
@@ -35,7 +35,8 @@ def test_items_cover_what_is_allowed(lq, lk, causal):
     im = image(lq, lk, causal)
     allowed = [np.arange(b)[None, :] <= np.arange(a)[:, None] + (b - a) if causal else np.ones((a, b), bool) for a, b in zip(lq, lk)]
     # query tiles: once each, and the keys of a tile reach as far as any of its rows sees, no further
-    for at, n, tile in ((8, 9, 64), (17, 18, 128), (19, 20, 256)):
+    short = max(lq + lk) <= 48          # tables of 16 rows only where all structures are short
+    for at, n, tile in ((8, 9, 64), (17, 18, 128), (19, 20, 256)) + (((29, 30, 16),) if short else ()):
         seen = set()
         rows = items(im, at, n)
         assert np.all(np.diff(rows[:, 3] - rows[:, 2]) <= 0)          # the longest first
@@ -46,7 +47,8 @@ def test_items_cover_what_is_allowed(lq, lk, causal):
             assert last == (cols.nonzero()[0].max() + 1 if cols.any() else 0)
         assert len(seen) == sum(-(-a // tile) for a in lq)
     # key tiles
-    for at, n, tile in ((10, 11, 64), (21, 22, 128)):
+    assert short or im[30] == im[32] == 0
+    for at, n, tile in ((10, 11, 64), (21, 22, 128)) + (((31, 32, 16),) if short else ()):
         seen = set()
         for s, t, first, last in items(im, at, n):
             assert (s, t) not in seen and last == lq[s]
