@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kThreads, 3) reverse_kernel(const RotateArgs A
         for (int o = W >> 1; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
         r = 1.f / sqrtf(ss / A.d + A.eps);
       }
-      if (on) {
+      if (on && h.there) {      // a head that is not there has neither weights nor, with eps = 0, a finite norm
         float wa[N], wb[N];
         if (NORM) {
           const float* w = table + per * A.d + h.side * A.d + part * 2 * N;
@@ -448,7 +448,7 @@ extern "C" {
 
 int so3lr_b200_norm_rotate(void* stream, const so3lr_b200_norm_rotate_args* a, const so3lr_b200_rows* q, const so3lr_b200_rows* k,
                            void* out_q, void* out_k) {
-  if (!a || a->n < 0 || a->type < 0 || a->type > 2 || a->d < 16 || a->d > 256 || a->d % 16 || a->heads_q < 0 || a->heads_k < 0 || a->axes < 0 ||
+  if (!a || a->n < 0 || a->n > 0x7ff00000 || a->type < 0 || a->type > 2 || a->d < 16 || a->d > 256 || a->d % 16 || a->heads_q < 0 || a->heads_k < 0 || a->axes < 0 ||
       a->axes > 16 || (a->axes && a->n && (!a->positions || !a->frequencies)))
     return kInvalidArgument;
   if (a->n == 0 || a->heads_q + a->heads_k == 0) return kOk;
@@ -469,7 +469,7 @@ int64_t so3lr_b200_norm_rotate_workspace(int d) { return (int64_t)grid_limit() *
 int so3lr_b200_norm_rotate_vjp(void* stream, const so3lr_b200_norm_rotate_args* a, const so3lr_b200_rows* q, const so3lr_b200_rows* k,
                                const so3lr_b200_rows* g_q, const so3lr_b200_rows* g_k, void* d_q, void* d_k, void* d_positions,
                                void* d_weight_q, void* d_weight_k, void* workspace, int64_t workspace_bytes) {
-  if (!a || a->n < 0 || a->type < 0 || a->type > 2 || a->d < 16 || a->d > 256 || a->d % 16 || a->heads_q < 0 || a->heads_k < 0 || a->axes < 0 ||
+  if (!a || a->n < 0 || a->n > 0x7ff00000 || a->type < 0 || a->type > 2 || a->d < 16 || a->d > 256 || a->d % 16 || a->heads_q < 0 || a->heads_k < 0 || a->axes < 0 ||
       a->axes > 16 || (a->axes && a->n && (!a->positions || !a->frequencies)) || (d_positions && !a->axes))
     return kInvalidArgument;
   const bool want_w = a->norm && (d_weight_q || d_weight_k);
