@@ -72,12 +72,19 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
+// NaN where one of them is
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
 // 2^x of a pair without the special function unit, which gives 16 results a cycle and is as busy as the tensor cores: x = n + f with n the
 // nearest integer (found by adding 1.5 2^23), 2^f by the polynomial of degree 4 with the least relative error on [-1/2, 1/2] (2.6e-6, a
-// hundredth of a 16-bit rounding; fitted by reweighted least squares), n added to its exponent.  Not below 2^-126.
+// hundredth of a 16-bit rounding; fitted by reweighted least squares), n added to its exponent.  Not below 2^-126.  A NaN, which an infinite logit
+// becomes too, gives 2^128 (1 - 2^-24), infinite in 16 bits.
 __device__ __forceinline__ float2 pow2_poly(float2 x) {
   const float2 magic = make_float2(12582912.f, 12582912.f), minus = make_float2(-12582912.f, -12582912.f);
-  x.x = fmaxf(x.x, -126.f); x.y = fmaxf(x.y, -126.f);
+  x.x = max_nan(x.x, -126.f); x.y = max_nan(x.y, -126.f);
   const float2 t = __fadd2_rn(x, magic), n = __fadd2_rn(t, minus), f = __fadd2_rn(x, make_float2(-n.x, -n.y));
   float2 p = make_float2(0.009570102207362652f, 0.009570102207362652f);
   p = __ffma2_rn(p, f, make_float2(0.05591786280274391f, 0.05591786280274391f));
