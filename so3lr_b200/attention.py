@@ -38,7 +38,8 @@ def _aligned(t, unit):
     a, b, c = t.stride()
     if c != 1 or not a or not b or (a | b) % unit or t.data_ptr() % 16:
         t = t.contiguous()
-        if t.data_ptr() % 16 or 0 in t.stride():
+        a, b, _ = t.stride()
+        if not a or not b or (a | b) % unit or t.data_ptr() % 16:      # as it was: the stride of an axis of one is free
             t = t.clone(memory_format=torch.contiguous_format)
     return t
 
@@ -88,7 +89,7 @@ class PackedStructures:
     of rows; `graph_start_kv` the same for the keys where they are other rows than the queries (one query per structure, new frames
     of trajectories).  causal: query i of lq sees key j of lk where j <= i + lk - lq, so the last query sees all keys.  Structures
     may be empty on either side; a query that sees no key gives zero.  Make it outside of a graph capture: it copies its tables to the device
-    and waits for that."""
+    and waits for that.  A captured graph reads these tables: the layout has to live as long as the graph is replayed."""
 
     def __init__(self, graph_start, graph_start_kv=None, causal=False, device=0):
         q = self._starts("graph_start", graph_start)
@@ -138,6 +139,7 @@ class PackedStructures:
     def _call(self, q, k, scale):
         """What calls with rows of these shapes have in common: (shape, workspace of the forward call, of its transpose); raises where the
         shapes do not fit."""
+        scale = None if scale is None else float(scale)
         key = (q.dtype, q.shape, k.shape, scale)
         call = self._calls.get(key)
         if call is None:
@@ -148,7 +150,9 @@ class PackedStructures:
                 raise ValueError(f"{heads} query heads cannot share {heads_kv} key heads")
             if n < self.rows_q or n_kv < self.rows_kv:
                 raise ValueError(f"the layout has {self.rows_q} and {self.rows_kv} rows, q {n} and k {n_kv}")
-            x = 1.0 / math.sqrt(d) if scale is None else float(scale)
+            if max(n, n_kv) >= 2**31 - 1:
+                raise ValueError(f"q has {n} and k {n_kv} rows; at most 2**31 - 2 are supported")
+            x = 1.0 / math.sqrt(d) if scale is None else scale
             if not (x > 0 and math.isfinite(x)):
                 raise ValueError(f"scale must be positive and finite, not {scale}")
             shape = AttentionShape(_TYPES[q.dtype], heads, heads_kv, d, n, n_kv, x)
@@ -319,6 +323,8 @@ def norm_rotate(q, k=None, positions=None, frequencies=None, *, q_weight=None, k
             raise ValueError(f"q has {n} rows, k {k.shape[0]}")
     if d % 16 or not 16 <= d <= 256:
         raise ValueError(f"d must be a multiple of 16 up to 256, not {d}")
+    if n > 2**31 - 2**20:
+        raise ValueError(f"q has {n} rows; at most 2**31 - 2**20 are supported")
     if pairing not in ("halves", "neighbors"):
         raise ValueError(f"pairing must be 'halves' or 'neighbors', not {pairing!r}")
     if (positions is None) != (frequencies is None):

@@ -5,7 +5,7 @@
 
 #include <algorithm>
 #include <cmath>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "kernels.h"
@@ -143,7 +143,7 @@ PackedArgs common(const int32_t* im, const int32_t* dev, const so3lr_b200_attent
   p.rows = im[kRowsQ]; p.rows_kv = im[kRowsKv]; p.longest_kv = im[kMaxKv];
   if (std::max(im[kMaxQ], im[kMaxKv]) <= short_rows(a->d)) p.tile_rows = 16;
   p.stages = im[kMaxKv] <= (p.tile_rows == 16 || (a->type == kF32 && a->d > 64) ? 32 : 64) ? 1 : 2;
-  p.rev_stages = im[kMaxKv] <= 32 && (int64_t)im[kMaxQ] * p.group <= 32 ? 1 : 2;
+  p.rev_stages = im[kMaxKv] <= 32 && im[kMaxQ] <= 32 && a->heads_q == a->heads_kv ? 1 : 2;
   p.nq = (int)a->rows_q; p.nkv = (int)a->rows_kv; p.hq = a->heads_q; p.hk = a->heads_kv; p.group = a->heads_q / a->heads_kv; p.d = a->d; p.causal = im[kCausal];
   p.scale = a->scale; p.scale_log2 = (float)((double)a->scale * 1.4426950408889634);
   return p;
@@ -280,7 +280,7 @@ int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int
   if (need < 0 || !image || capacity < need) return kInvalidArgument;
   try {
     build_image(n_structures, start_q, start_kv, causal != 0, image);
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {
     return kTooLarge;
   }
   return kOk;

@@ -42,7 +42,6 @@ struct PackedArgs {
   int tile_rows = 64;           // rows of a CTA there: 64 or 16
   int nq = 0, nkv = 0, hq = 0, hk = 0, group = 1, d = 0, causal = 0;
   float scale = 0.f, scale_log2 = 0.f;                // scale * log2(e): the softmax runs on powers of two
-  int* err = nullptr;
 };
 
 constexpr int kPackTile = 64;   // rows of a tile of the mma kernels

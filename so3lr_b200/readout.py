@@ -49,15 +49,20 @@ class StructureReadout(torch.nn.Module):
         f = torch.zeros(3, d // 2, dtype=torch.float64)
         f[p % 3, p] = 2 * math.pi / (wavelengths[0] * (wavelengths[1] / wavelengths[0]) ** k)
         self.register_buffer("frequencies", f.float().to(dev))
-        self._layouts = {}
+        self._layouts, self._captured = {}, {}
+
+    def __getstate__(self):      # layouts hold device tables: a copy makes its own
+        return self.__dict__ | {"_layouts": {}, "_captured": {}}
 
     def _layout(self, graph_start):
-        gs = np.ascontiguousarray(graph_start, dtype=np.int64)
-        key = gs.tobytes()
-        pair = self._layouts.pop(key, None)
+        gs, dev = PackedStructures._starts("graph_start", graph_start), self.qkv.device
+        key = gs.tobytes(), dev
+        pair = self._captured.get(key) or self._layouts.pop(key, None)
         if pair is None:
-            dev = self.qkv.device
             pair = PackedStructures(gs, device=dev), PackedStructures(np.arange(len(gs)), gs, device=dev)
+        if torch.cuda.is_current_stream_capturing():
+            self._captured[key] = pair              # a graph reads its tables from now on: kept for good
+            return pair
         self._layouts[key] = pair                   # most recently used last
         while len(self._layouts) > self.MAX_CACHED_LAYOUTS:
             self._layouts.pop(next(iter(self._layouts)))

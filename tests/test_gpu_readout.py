@@ -142,3 +142,31 @@ def test_batched_calculator_with_a_readout(pad):
     # trained on the frozen features: every parameter gets a gradient, and a step along it changes the result
     (out["readout"] ** 2).sum().backward()
     assert all(p.grad is not None and torch.isfinite(p.grad).all() and (p.grad != 0).any() for p in r.parameters())
+
+
+def test_copies_and_captured_readouts():
+    import copy
+
+    from so3lr_b200 import StructureReadout
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    r = StructureReadout(n_out=2, seed=1)
+    with torch.no_grad():
+        r.last.normal_(generator=gen)
+    x, pos, gs = torch.randn(50, 128, generator=gen, device="cuda"), torch.rand(50, 3, generator=gen, device="cuda") * 9, np.array([0, 30, 50])
+    with torch.no_grad():
+        want = r(x, pos, gs)
+        assert torch.equal(copy.deepcopy(r)(x, pos, gs), want)      # its layouts stay with the original
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(stream):
+            r(x, pos, gs)
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            got = r(x, pos, gs)
+        for i in range(1, r.MAX_CACHED_LAYOUTS + 4):                # the graph's layout is not among those that make room
+            r(x, pos, np.array([0, i, 50]))
+        assert any(k[0] == np.asarray(gs, np.int32).tobytes() for k in r._captured)
+        got.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)

@@ -416,3 +416,72 @@ def test_norm_rotate_refusals():
                      ((q[..., :24], k[..., :24], pos, f[:, :12]), {}), ((q, k, pos[:, :0], f[:0]), {})):
         with pytest.raises(ValueError):
             norm_rotate(*args, **kw)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lk,d", [(300, 32), (300, 64), (300, 128), (40, 64), (1000, 128)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_one_value_that_is_not_finite_shows(lk, d, dtype, value):
+    # one key of the first structure: every one of its rows attends to it, wherever it stands in its tile; the second structure is spared
+    q, k, v, _ = inputs([lk, 280], [lk, 280], 1, 1, d, TYPES[dtype], seed=2)
+    q[:, :, 0] = 1.0
+    packed = PackedStructures(starts([lk, 280]))
+    clean = structure_attention(q, k, v, packed)
+    for j in list(range(8)) + [lk - 1, lk - 2, lk - 3, lk - 4]:
+        bad = k.clone()
+        bad[j, 0, 0] = value
+        out = structure_attention(q, bad, v, packed)
+        assert not torch.isfinite(out[:lk]).any(), j
+        assert torch.equal(out[lk:], clean[lk:])
+
+
+def test_rows_with_free_strides_and_scales_that_change():
+    # one row, one head: the strides of these axes mean nothing, whatever they are
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    q = torch.randn(40, generator=gen, device="cuda").as_strided((1, 2, 16), (33, 16, 1))
+    k = torch.randn(40, 20, generator=gen, device="cuda")[:, None, :16].as_strided((40, 1, 16), (20, 3, 1))
+    packed = PackedStructures([0, 1], [0, 40])
+    assert q.stride(0) % 4 and k.stride(1) % 4
+    want = torch.softmax(0.25 * torch.einsum("qhd,kd->hqk", q.double(), k[:, 0].double()), -1)
+    want = torch.einsum("hqk,kd->qhd", want, k[:, 0].double())
+    got = structure_attention(q, k, k, packed)
+    # 16 terms a logit of size 4 and 40 a value: below 100 roundings of 2^-24
+    assert (got.double() - want).abs().max() <= 100 * 2.0 ** -24 * k.abs().max()
+    turned = norm_rotate(q, None, torch.ones(1, 1, device="cuda"), torch.zeros(1, 8, device="cuda"))[0]
+    assert torch.equal(turned, q)
+    scale = torch.tensor(0.5)
+    first = structure_attention(q, k, k, packed, scale=scale)
+    scale.fill_(2.0)
+    assert torch.equal(structure_attention(q, k, k, packed, scale=scale), structure_attention(q, k, k, packed, scale=2.0))
+    assert not torch.equal(structure_attention(q, k, k, packed, scale=scale), first)
+
+
+@pytest.mark.parametrize("heads", [1, 3, 5])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_norm_rotate_without_eps_and_keys(heads, dtype):
+    # counts of heads that are no power of two leave lanes without a head
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    x = torch.randn(9, heads, 32, generator=gen, device="cuda").to(TYPES[dtype])
+    pos, f, w = torch.rand(9, 3, generator=gen, device="cuda"), torch.rand(3, 16, generator=gen, device="cuda"), torch.rand(32, generator=gen, device="cuda") + 0.5
+    leaves = [t.clone().requires_grad_() for t in (x, pos, w)]
+    g = torch.randn(9, heads, 32, generator=gen, device="cuda").to(TYPES[dtype])
+    out = norm_rotate(leaves[0], None, leaves[1], f, q_weight=leaves[2], eps=0.0)[0]
+    got = torch.autograd.grad(out, leaves, g)
+    ref = [t.detach().double().requires_grad_() for t in leaves]
+    y = rotate_reference(ref[0], ref[2], ref[1] @ f.double(), "halves", eps=0.0)
+    want = torch.autograd.grad(y, ref, g.double())
+    for name, a, b in zip(("x", "positions", "weight"), got, want):
+        # sums of up to 9 heads rows of a hundred float32 operations, and a rounding of 16-bit results
+        step = 2.0 ** -8 if a.dtype == torch.bfloat16 else 2.0 ** -15
+        assert (a.double() - b).abs().max() <= step * b.abs().max(), name
+
+
+def test_more_rows_than_an_index_holds_are_refused():
+    many = torch.zeros(1, 1, 16, dtype=torch.bfloat16, device="cuda").expand(2 ** 31, 1, 16)
+    one = torch.zeros(1, 1, 16, dtype=torch.bfloat16, device="cuda")
+    packed = PackedStructures([0, 1])
+    for q, k in ((many, one), (one, many)):
+        with pytest.raises(ValueError, match="rows"):
+            structure_attention(q, k, k, packed)
+    with pytest.raises(ValueError, match="rows"):
+        norm_rotate(many, None, torch.zeros(1, 1, device="cuda").expand(2 ** 31, 1), torch.zeros(1, 8, device="cuda"))
