@@ -85,13 +85,19 @@ template <typename T, bool NEIGHBORS> struct Piece {
   }
 };
 
-// cos and sin of theta: reduced to [-pi/4, pi/4] in double, so that one rounding to float32 costs 2^-25 of an angle below one
+// cos and sin of theta: reduced to x in [-pi/4, pi/4] in double, so that one rounding to float32 costs 2^-25 of an angle below one, then
+// x + x^3 P(x^2) and 1 - x^2/2 + x^4 Q(x^2) with P and Q of degree 2 fitted for the least largest error there (1.8e-9 and 1e-10; least
+// squares reweighted by the error).  The library's pair carries its reduction of large arguments along (32,771 rows of 40 heads x
+// 128: 139 us with it, 131 without).  Beyond 2^53 nothing is left of an angle: where the reduction fails there, the row stays unturned.
 __device__ __forceinline__ void cos_sin(double theta, float& c, float& s) {
   const double n = rint(theta * 0.6366197723675814);
   const double r = fma(-n, 6.123233995736766e-17, fma(-n, 1.5707963267948966, theta));
   const int q = (int)((long long)n & 3);
-  float sr, cr;
-  sincosf((float)r, &sr, &cr);
+  float x = (float)r;
+  if (fabsf(x) > 1.f) x *= 0.f;      // infinite ones become NaN
+  const float z = x * x;
+  const float sr = fmaf(x * z, fmaf(z, fmaf(z, -1.9495567539706826e-4f, 8.331977762281895e-3f), -0.16666650772094727f), x);
+  const float cr = fmaf(z * z, fmaf(z, fmaf(z, 2.4438379114144482e-5f, -1.3887366512790322e-3f), 4.166664555668831e-2f), fmaf(z, -0.5f, 1.f));
   c = (q & 1) ? sr : cr; s = (q & 1) ? cr : sr;
   if (q == 1 || q == 2) c = -c;
   if (q >= 2) s = -s;
@@ -387,8 +393,9 @@ __global__ void __launch_bounds__(256) weight_kernel(const RotateArgs A, int row
 int next_pow2(int x) { int p = 1; while (p < x) p <<= 1; return p; }
 // Lanes per row, and heads of a token that run side by side: as few as give every SM `busy` threads.  A thread with several heads asks for
 // the next one's rows while it works on the present one, and the angles of a token are formed once for all of them; more threads hide more.
-// 32,771 rows of 40 heads x 128 forward, busy 1,024 / 2,048 / 4,096: 155 / 147 / 139 us (4.8 TB/s; a copy of the bytes takes 103); 16,411
-// rows of 32 heads x 64 reverse, 512 / 1,024 / 2,048: 56 / 47 / 53 us; 12,803 rows of 8 heads x 32 float32 reverse: 16 / 19 / 28.
+// 32,771 rows of 40 heads x 128 forward, busy 2,048 / 4,096 / 8,192: 140 / 131 / 140 us (5.1 TB/s; a copy of the bytes takes 103; with more than
+// four CTAs on an SM the registers spill: 198); 16,411 rows of 32 heads x 64 reverse, 512 / 1,024 / 2,048: 56 / 47 / 53 us; 12,803 rows
+// of 8 heads x 32 float32 reverse: 16 / 19 / 28.
 void shape(RotateArgs& A, int value_bytes, bool reverse, int& W) {
   W = next_pow2(A.d / 2 / (16 / value_bytes));
   const int heads = A.heads[0] + A.heads[1];

@@ -18,7 +18,8 @@ namespace {
 // with 16 rows where no structure has more than kShortRows.
 enum Head : int { kMagicAt, kN, kCausal, kRowsQ, kRowsKv, kMaxQ, kStartQ, kStartKv, kItemsQ, kNItemsQ, kItemsKv, kNItemsKv, kItemsSplit, kNItemsSplit,
                   kSplitFirst, kCombine, kTotal, kItemsQ128, kNItemsQ128, kItemsQ256, kNItemsQ256, kItemsKv128, kNItemsKv128, kMaxKv,
-                  kWalkQ, kWalkKv /* tiles of 64 that the items of a table walk over in all */, kWalkQ128, kWalkQ256, kWalkKv128 /* tiles of 128 that the items of a table walk over in all */,
+                  // tiles of 64 and of 128 that the items of a table walk over in all
+                  kWalkQ, kWalkKv, kWalkQ128, kWalkQ256, kWalkKv128,
                   kItemsQ16, kNItemsQ16, kItemsKv16, kNItemsKv16, kHeadInts = 48 };
 constexpr int kMagic = 0x53334c50;
 constexpr int kTables = 7, kTileRows[kTables] = {kPackTile, kPackTile, 128, 256, 128, 16, 16};

@@ -28,14 +28,14 @@ struct PackedArgs {
   float* delta = nullptr;       // (hq, nq) sum over d of g * o
   void *dq = nullptr, *dk = nullptr, *dv = nullptr;   // contiguous
   const int *start_q = nullptr, *start_kv = nullptr;
-  // one work item per CTA and head: {structure, tile, first, last}; [first, last) are the rows of the other side that the tile meets
+  // one work item per CTA, head and piece: {structure, tile, first, last}; [first, last) are the rows of the other side that the tile meets
   const int4* items = nullptr;
   const int* split_first = nullptr;                   // items of structure s: [split_first[s], split_first[s + 1])
   float* part_o = nullptr;      // (item, hk, part_rows, DP) of the split form
   float2* part_ml = nullptr;    // (item, hk, part_rows): running maximum (in units of log2) and sum
   int part_rows = 0;            // most rows of a structure: tokens times heads of a group
-  int pieces = 1;               // tensor-core kernels: pieces that an item's walk is cut into; each leaves its share in part_o / part_ml or
-  float* share[3] = {};         // (reverse) in share: (pieces, heads, rows, d) of dq, dk, dv
+  int pieces = 1;               // into which an item's walk is cut; each leaves its share in part_o (pieces, hq, nq, d) and part_ml, or
+  float* share[3] = {};         // (reverse) in share: (pieces, rows, heads, d) of dq, dk, dv
   int rows = 0, rows_kv = 0;    // of the layout
   int longest_kv = 0;           // keys of its longest structure
   int stages = 2, rev_stages = 2;         // buffers for the walked side in the warp-level kernels: one where all of it fits into it

@@ -1,7 +1,7 @@
 // What the tensor-core kernels of attention inside packed structures share: operand tiles, descriptors, barriers, tensor memory.
 //
-// An operand tile is 128 rows of up to 64 values (64 or 128 bytes a row, swizzled), several of them side by side (Geometry), brought in by TMA from the strided operand: a map has the dimensions (values, rows, heads), values behind the last one come as
-// zeros.  The same image serves the tensor cores with d contracted (K-major) and with the rows contracted (MN-major), so a tile of keys
+// An operand tile is 128 rows of up to 64 values (64 or 128 bytes a row, swizzled), several of them side by side (Geometry), brought in by TMA
+// from the strided operand: a map has the dimensions (values, rows, heads), values behind the last one come as zeros.  The same image serves the tensor cores with d contracted (K-major) and with the rows contracted (MN-major), so a tile of keys
 // serves q k^T and dS k, a tile of queries k q^T and dS^T q.  A tile may reach over the end of its structure into the next one's rows: where
 // they would be contracted, the loading warp clears them before it hands the tile over (a zero probability times a neighbour's NaN is NaN).
 #pragma once
