@@ -215,6 +215,7 @@ int64_t whole_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool
   return (a->type == kF32 && on_tensor_cores(im, a) ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0) +
          packed_share_bytes(pieces(im, a), a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse);
 }
+constexpr int64_t kQueueBytes = 16;      // behind these: PackedArgs::queue
 
 const int4* table(const int32_t* im, const int32_t* dev, int field) { return reinterpret_cast<const int4*>(dev + im[field]); }
 
@@ -243,6 +244,7 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
 
 template <typename T>
 int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
+  if (on_tensor_cores(im, a)) p.queue = reinterpret_cast<int*>(static_cast<char*>(workspace) + whole_bytes(im, a, true));
   int rc = packed_delta<T>(st, p, im[kRowsQ]);
   if (rc) return rc;
   if (on_tensor_cores(im, a))
@@ -289,7 +291,7 @@ int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int
 
 int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* a, int vjp) {
   if (!shape_ok(image, a)) return -1;
-  if (vjp) return whole_bytes(image, a, true);
+  if (vjp) return whole_bytes(image, a, true) + (on_tensor_cores(image, a) ? kQueueBytes : 0);
   if (!few_rows(image, a)) return whole_bytes(image, a, false);
   if (!image[kCombine]) return 0;
   return part_floats(image, a) * (int64_t)sizeof(float) + part_floats(image, a) / packed_padded(a->d) * (int64_t)sizeof(float2);

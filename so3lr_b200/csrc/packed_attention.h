@@ -36,6 +36,8 @@ struct PackedArgs {
   int part_rows = 0;            // most rows of a structure: tokens times heads of a group
   int pieces = 1;               // into which an item's walk is cut; each leaves its share in part_o (pieces, hq, nq, d) and part_ml, or
   float* share[3] = {};         // (reverse) in share: (pieces, rows, heads, d) of dq, dk, dv
+  int jobs = 0;                 // of the tensor-core reverse kernels: items times heads times pieces
+  int* queue = nullptr;         // jobs of dq and of dk and dv that were handed out besides each CTA's first
   int rows = 0, rows_kv = 0;    // of the layout
   int longest_kv = 0;           // keys of its longest structure
   int stages = 2, rev_stages = 2;         // buffers for the walked side in the warp-level kernels: one where all of it fits into it

@@ -613,10 +613,11 @@ __global__ void __launch_bounds__(256) sum_kernel(const PackedArgs a, int first,
 }
 
 // ---- reverse --------------------------------------------------------------------------------------------------------
-// delta = sum over d of g * o, a thread per 16 bytes, rows of all heads
+// delta = sum over d of g * o, a thread per 16 bytes, rows of all heads; empties the queues of the kernels behind it
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(const PackedArgs a, int rows, int width) {
   constexpr int V = 16 / (int)sizeof(T);
+  if (a.queue && blockIdx.x == 0 && threadIdx.x < 2) a.queue[threadIdx.x] = 0;
   const int part = threadIdx.x % width;
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) / width;
   const long long r = i / a.hq;

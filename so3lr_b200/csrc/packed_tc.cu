@@ -26,10 +26,13 @@ namespace {
 using namespace tc;
 
 // barriers and scratch behind the tiles
+constexpr int kBars = 40;
 struct Tail {
-  unsigned long long bars[32];
+  unsigned long long bars[kBars];
   uint32_t tmem;
   int failed;
+  int jobs[2];       // reverse kernels: indices of the jobs at hand, -1 behind the last one
+  int tiles[2];      // and tiles of those that have any, 0 behind the last one
 };
 template <typename T, int TERMS> struct Operand { using type = T; };
 template <> struct Operand<float, 3> { using type = __nv_bfloat16; };
@@ -338,11 +341,45 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
   if (warp == kMmaWarp) { fence_after(); free_tmem(tmem, 256 * TILES); }
 }
 
-// ---- reverse: dq ----------------------------------------------------------------------------------------------------
-// 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256 (float32: the third term of dS
-// at 256, dq at 320; where there is room dS at 256 and dq behind it).  The two groups of four warps have 64 columns each of every row.  The next tile's logits are made as soon as these have been read, so that its exponentials run
-// beside the products dS k and g v^T.
-enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqS, kdqSRead, kdqDp, kdqDpRead, kdqDs, kdqDsDone, kdqOut, kdqFix, kDqBars };
+// ---- reverse --------------------------------------------------------------------------------------------------------
+// A CTA stays on its SM and works through jobs (an item's piece of one head), so that a job's first tiles come in and its first products run
+// while the last results of the one before leave: with a CTA per job 6 of the 11 us of a job of 500 rows went by in its start and end (24 structures of
+// 150 to 900 rows, 16 heads x 64: dq @DQ0 -> @DQ1 us, dk and dv @KV0 -> @KV1).  The loading warp takes jobs from a queue, the
+// longest first (equal shares instead: SMs differ in their pace, @EQ), and passes them on through shared memory.
+__device__ __forceinline__ void publish_job(Tail* tail, int m, int index, int jobs, uint32_t full, uint32_t free, int lane, volatile int* failed) {
+  if (m >= 2) wait_bar(free + 8 * (m & 1), ((m >> 1) - 1) & 1, failed, &g_packed_error);
+  if (lane == 0) { tail->jobs[m & 1] = index < jobs ? index : -1; arrive(full + 8 * (m & 1)); }
+  __syncwarp();
+}
+// index of a warp's m-th job
+__device__ __forceinline__ int take_job(const Tail* tail, int m, uint32_t full, uint32_t free, int lane, volatile int* failed) {
+  wait_bar(full + 8 * (m & 1), (m >> 1) & 1, failed, &g_packed_error);
+  const int index = __shfl_sync(0xffffffffu, *failed ? -1 : *const_cast<const volatile int*>(tail->jobs + (m & 1)), 0);
+  if (lane == 0) arrive(free + 8 * (m & 1));
+  return index;
+}
+
+// dq: 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256 (float32: the third term of dS
+// at 256, dq at 320; where there is room dS at 256 and dq behind it).  The two groups of four warps have 64 columns each of every row.  The
+// next tile's logits are made as soon as these have been read, so that its exponentials run beside the products dS k and g v^T.
+enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqQFree, kdqS, kdqSRead, kdqDp, kdqDpRead, kdqDs, kdqDsDone, kdqOut, kdqOutRead, kdqFix, kdqJob,
+             kdqJobFree = kdqJob + 2, kDqBars = kdqJobFree + 2 };
+struct DqJob {
+  bool on;
+  int q0, lq, c0, lk, h, row0, off, k0, n, piece;      // n tiles of keys from key k0 on
+  __device__ __forceinline__ DqJob(const PackedArgs& a, int index) {
+    on = index >= 0;
+    n = 0;
+    if (!on) return;
+    const int unit = index / a.pieces;
+    piece = index % a.pieces; h = unit % a.hq;
+    const int4 item = __ldg(a.items + unit / a.hq);
+    q0 = __ldg(a.start_q + item.x); lq = __ldg(a.start_q + item.x + 1) - q0; c0 = __ldg(a.start_kv + item.x); lk = __ldg(a.start_kv + item.x + 1) - c0;
+    row0 = item.y * kTile; off = lk - lq;
+    const int all = (item.w + kTile - 1) / kTile, share = all / a.pieces, more = all % a.pieces;
+    k0 = (piece * share + min(piece, more)) * kTile; n = share + (piece < more);
+  }
+};
 
 template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
@@ -357,15 +394,10 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int unit = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
-  const int4 item = a.items[unit / a.hq];
-  const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = unit % a.hq, kvh = h / a.group, row0 = item.y * kTile, off = lk - lq;
-  const int all = (item.w + kTile - 1) / kTile, per = (all + a.pieces - 1) / a.pieces, k0 = piece * per * kTile, n = min(per, max(0, all - piece * per));
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
-    for (int i = 0; i < kDqBars; ++i) init_bar(bar(i), i == kdqSRead || i == kdqDpRead || i == kdqDs ? 256 : 1);
+    for (int i = 0; i < kDqBars; ++i) init_bar(bar(i), i == kdqSRead || i == kdqDpRead || i == kdqDs || i == kdqOutRead ? 256 : i >= kdqJobFree ? 8 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
@@ -375,167 +407,225 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   constexpr bool E = G::kEarlyDq;
   constexpr uint32_t kDs = E ? 256 : kTile, kOut = E ? (TERMS == 1 ? 320 : 448) : (TERMS == 1 ? 256 : 320);
 
+  // Tiles are counted over all jobs (keys are tiles 0, 2, .. of the ring, values 1, 3, ..), and so are jobs that have any: barriers turn with these.
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
-    if (warp == kMmaWarp && n > 0) {
+    if (warp == kMmaWarp) {
       const uint32_t on = elect_one();
       auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
       auto ready = [&](int j) { wait_bar(bar(kdqFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
-      auto give = [&](int j) { if (j + R < 2 * n) commit(on, bar(kdqEmpty + j % R)); };
-      wait_bar(bar(kdqQ), 0, failed, &g_packed_error);
-      ready(0);
-      product_rows<M, TERMS, DW>(on, tmem, sq, slot(0), d);
-      commit(on, bar(kdqS));
-      ready(1);
-      product_rows<M, TERMS, DW>(on, tmem + kTile, sg, slot(1), d);
-      commit(on, bar(kdqDp));
-      give(1);
-      for (int i = 0; i < n; ++i) {
-        const bool more = i + 1 < n;
-        auto logits = [&] {
-          if (!more) return;
-          ready(2 * i + 2);
-          wait_bar(bar(kdqSRead), i & 1, failed, &g_packed_error);
-          fence_after();
-          product_rows<M, TERMS, DW>(on, tmem, sq, slot(2 * i + 2), d);
-          commit(on, bar(kdqS));
-        };
-        auto dp = [&] {
-          if (!more) return;
-          ready(2 * i + 3);
-          if (E) { wait_bar(bar(kdqDpRead), i & 1, failed, &g_packed_error); fence_after(); }
-          product_rows<M, TERMS, DW>(on, tmem + kTile, sg, slot(2 * i + 3), d);
-          commit(on, bar(kdqDp));
-          give(2 * i + 3);
-        };
+      auto give = [&](int j) { commit(on, bar(kdqEmpty + j % R)); };
+      // Logits and dP run a tile ahead: tile g + 1 of all, the il-th of `ahead` of job jl.  The loop is as short as it can be (the loading warp says
+      // how many tiles a job has, every product stands in one place, so the walk starts a step early), and addresses come from g, which is
+      // the same in all lanes as the compiler sees it: what this warp does between two instructions keeps the tensor cores waiting.
+      int g = -1, il = 0, jl = 0, ahead = 0;
+      bool done = false, first = false, last = false, first_next = false, last_next = false;      // of tile g and of the next one
+      auto logits = [&] {
+        first_next = il == 0;
+        if (first_next) {
+          wait_bar(bar(kdqQ), jl & 1, failed, &g_packed_error);
+          ahead = __shfl_sync(0xffffffffu, *failed ? 0 : tail->tiles[jl & 1], 0);
+          done = ahead == 0;
+        }
+        if (done) return;
+        ready(2 * g + 2);
+        if (g >= 0) { wait_bar(bar(kdqSRead), g & 1, failed, &g_packed_error); fence_after(); }
+        product_rows<M, TERMS, DW>(on, tmem, sq, slot(2 * g + 2), d);
+        commit(on, bar(kdqS));
+      };
+      auto dp = [&] {
+        if (done) return;
+        ready(2 * g + 3);
+        if (E && g >= 0) { wait_bar(bar(kdqDpRead), g & 1, failed, &g_packed_error); fence_after(); }
+        product_rows<M, TERMS, DW>(on, tmem + kTile, sg, slot(2 * g + 3), d);
+        commit(on, bar(kdqDp));
+        give(2 * g + 3);
+        last_next = ++il == ahead;
+        if (last_next) { commit(on, bar(kdqQFree)); ++jl; il = 0; }
+      };
+      for (int job = 0;; ++g) {
         if (!G::kShort) logits();
         if (E) dp();
-        wait_bar(bar(kdqDs), i & 1, failed, &g_packed_error);
-        fence_after();
-        const uint32_t at = tmem + kDs;
-        product_cols<M, TERMS, DW>(on, tmem + kOut, E ? Packed{{at, at + 64, at + 128}, {32, 32, 32}} : Packed{{at, at + 32, tmem + 256}, {64, 64, 32}},
-                                   slot(2 * i), d, i > 0);
-        if (E) commit(on, bar(kdqDsDone));
-        give(2 * i);
+        if (g >= 0) {
+          wait_bar(bar(kdqDs), g & 1, failed, &g_packed_error);
+          if (first && job > 0) wait_bar(bar(kdqOutRead), (job - 1) & 1, failed, &g_packed_error);
+          fence_after();
+          const uint32_t at = tmem + kDs;
+          product_cols<M, TERMS, DW>(on, tmem + kOut, E ? Packed{{at, at + 64, at + 128}, {32, 32, 32}} : Packed{{at, at + 32, tmem + 256}, {64, 64, 32}},
+                                     slot(2 * g), d, !first);
+          if (E) commit(on, bar(kdqDsDone));
+          if (last) { commit(on, bar(kdqOut)); ++job; }
+          give(2 * g);
+        }
         if (G::kShort) logits();
         if (!E) dp();
+        if (done) break;
+        first = first_next; last = last_next;
       }
-      commit(on, bar(kdqOut));
-    } else if (warp == kLoadWarp && n > 0) {
+    } else if (warp == kLoadWarp) {
       Loader<TERMS, DW> ld{lane, bar(kdqFix)};
-      if (lane == 0) {
-        expect(bar(kdqQ), 2 * tile_bytes);
-        ld.copies(sq, &maps.q, q0 + row0, h, bar(kdqQ));
-        ld.copies(sg, &maps.g, q0 + row0, h, bar(kdqQ));
+      int g = 0, job = 0;
+      for (int m = 0, index = blockIdx.x;; ++m) {
+        publish_job(tail, m, index, a.jobs, bar(kdqJob), bar(kdqJobFree), lane, failed);
+        if (__any_sync(0xffffffffu, index >= a.jobs || *failed)) break;
+        const DqJob j(a, index);
+        for (int i = 0; i < 2 * j.n; ++i, ++g) {
+          if (i == 1) {      // behind the first tile of keys, which finds room earlier
+            if (job > 0) wait_bar(bar(kdqQFree), (job - 1) & 1, failed, &g_packed_error);
+            if (lane == 0) {
+              tail->tiles[job & 1] = j.n;
+              expect(bar(kdqQ), 2 * tile_bytes);
+              ld.copies(sq, &maps.q, j.q0 + j.row0, j.h, bar(kdqQ));
+              ld.copies(sg, &maps.g, j.q0 + j.row0, j.h, bar(kdqQ));
+            }
+            __syncwarp();
+          }
+          if (g >= R) wait_bar(bar(kdqEmpty + g % R), (g / R - 1) & 1, failed, &g_packed_error);
+          const int r = j.k0 + (i >> 1) * kTile;
+          ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, j.h / a.group, bar(kdqFull + g % R), j.lk - r, !(i & 1), failed, &g_packed_error);
+        }
+        job += j.n > 0;
+        if (lane == 0) index = (int)gridDim.x + atomicAdd(a.queue, 1);
+        index = __shfl_sync(0xffffffffu, index, 0);
       }
+      // nothing is pending when the CTA ends
+      if (job > 0) wait_bar(bar(kdqQFree), (job - 1) & 1, failed, &g_packed_error);
+      if (lane == 0) { tail->tiles[job & 1] = 0; arrive(bar(kdqQ)); }      // no more jobs
       __syncwarp();
-      for (int j = 0; j < 2 * n; ++j) {
-        if (j >= R) wait_bar(bar(kdqEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
-        const int r = k0 + (j >> 1) * kTile;
-        ld.tile(ring + (j % R) * tile_bytes, (j & 1) ? &maps.v : &maps.k, c0 + r, kvh, bar(kdqFull + j % R), lk - r, !(j & 1), failed, &g_packed_error);
-      }
+      for (int t = max(0, g - R); t < g; ++t) wait_bar(bar(kdqEmpty + t % R), (t / R) & 1, failed, &g_packed_error);
     }
   } else {
     more_regs<kComputeRegs>();
-    const int half = warp >> 2, w = warp & 3, row = row0 + w * 32 + lane, first = row0 + w * 32, col = 64 * half;
-    const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16);
-    const int lim = min(a.causal ? row + off : lk - 1, lk - 1), lim_first = min(a.causal ? first + off : lk - 1, lk - 1);
-    const long long at = (long long)h * a.nq + q0 + row;
-    const bool there = row < lq;
-    const float e = there ? -a.lse[at] : -INFINITY, delta = there ? a.delta[at] : 0.f;
-    constexpr int kOwn = TERMS == 1 ? 1 : DW / 2;
-    float own[kOwn];                         // dq so far (float32), half of the row
-#pragma unroll
-    for (int c = 0; c < kOwn; ++c) own[c] = 0.f;
-    const uint32_t c2 = col / 2;
+    const int half = warp >> 2, w = warp & 3, col = 64 * half;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16), c2 = col / 2;
     const Packed to = E ? Packed{{kDs + c2, kDs + 64 + c2, kDs + 128 + c2}, {}} : Packed{{kDs + (uint32_t)col, kDs + 32 + (uint32_t)col, 256 + c2}, {}};
-    const float2 scale = make_float2(a.scale_log2, a.scale_log2), ref = make_float2(e, e);
-    for (int i = 0; i < n; ++i) {
-      uint32_t x[64], y[64];
-      wait_bar(bar(kdqS), i & 1, failed, &g_packed_error);
-      fence_after();
-      ld32(lanes + col, x);
-      ld32(lanes + col + 32, x + 32);
-      wait_ld(x);
-      fence_before();
-      arrive(bar(kdqSRead));
+    const float2 scale = make_float2(a.scale_log2, a.scale_log2);
+    // a row's statistics; rows that are not there: exp(-inf) = 0
+    auto stats = [&](const DqJob& j, float& e, float& delta) {
+      const int row = j.row0 + w * 32 + lane;
+      e = -INFINITY; delta = 0.f;
+      if (j.on && row < j.lq) { const long long at = (long long)j.h * a.nq + j.q0 + row; e = -a.lse[at]; delta = a.delta[at]; }
+    };
+    int g = 0, job = 0;
+    DqJob j(a, take_job(tail, 0, bar(kdqJob), bar(kdqJobFree), lane, failed));
+    float e, delta;
+    stats(j, e, delta);
+    for (int m = 1; j.on; ++m) {
+      const int row = j.row0 + w * 32 + lane, first = j.row0 + w * 32;
+      const int lim = min(a.causal ? row + j.off : j.lk - 1, j.lk - 1), lim_first = min(a.causal ? first + j.off : j.lk - 1, j.lk - 1);
+      const bool there = row < j.lq;
+      constexpr int kOwn = TERMS == 1 ? 1 : DW / 2;
+      float own[kOwn];                         // dq so far (float32), half of the row
 #pragma unroll
-      for (int c = 0; c < 64; c += 16) {
-        float v[16];
-        pow2_16<TERMS == 1>(x + c, scale, ref, v);
-#pragma unroll
-        for (int k = 0; k < 16; ++k) x[c + k] = __float_as_uint(v[k]);
-      }
-      const int kb = k0 + i * kTile + col;
-      wait_bar(bar(kdqDp), i & 1, failed, &g_packed_error);
-      fence_after();
-      ld32(lanes + kTile + col, y);
-      ld32(lanes + kTile + col + 32, y + 32);
-      wait_ld(y);
-      if (E) {
+      for (int c = 0; c < kOwn; ++c) own[c] = 0.f;
+      const float2 ref = make_float2(e, e);
+      for (int i = 0; i < j.n; ++i, ++g) {
+        uint32_t x[64], y[64];
+        wait_bar(bar(kdqS), g & 1, failed, &g_packed_error);
+        fence_after();
+        ld32(lanes + col, x);
+        ld32(lanes + col + 32, x + 32);
+        wait_ld(x);
         fence_before();
-        arrive(bar(kdqDpRead));
-        if (i > 0) { wait_bar(bar(kdqDsDone), (i - 1) & 1, failed, &g_packed_error); fence_after(); }
-      }
-      if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own); }
+        arrive(bar(kdqSRead));
 #pragma unroll
-      for (int c = 0; c < 64; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * (__uint_as_float(y[c]) - delta));
-      if (kb + 63 > lim_first) {
+        for (int c = 0; c < 64; c += 16) {
+          float v[16];
+          pow2_16<TERMS == 1>(x + c, scale, ref, v);
 #pragma unroll
-        for (int c = 0; c < 64; ++c) if (kb + c > lim) x[c] = 0;
-      }
+          for (int q = 0; q < 16; ++q) x[c + q] = __float_as_uint(v[q]);
+        }
+        const int kb = j.k0 + i * kTile + col;
+        wait_bar(bar(kdqDp), g & 1, failed, &g_packed_error);
+        fence_after();
+        ld32(lanes + kTile + col, y);
+        ld32(lanes + kTile + col + 32, y + 32);
+        wait_ld(y);
+        if (E) {
+          fence_before();
+          arrive(bar(kdqDpRead));
+          if (g > 0) { wait_bar(bar(kdqDsDone), (g - 1) & 1, failed, &g_packed_error); fence_after(); }
+        }
+        if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own); }
 #pragma unroll
-      for (int c = 0; c < 64; c += 16) {
-        float v[16];
+        for (int c = 0; c < 64; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * (__uint_as_float(y[c]) - delta));
+        if (kb + 63 > lim_first) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(x[c + k]);
-        put16<M, TERMS>(to, lanes, c, v);
-      }
-      wait_st();
-      fence_before();
-      arrive(bar(kdqDs));
-    }
-    if (n > 0) {
-      wait_bar(bar(kdqOut), 0, failed, &g_packed_error);
-      fence_after();
-    }
-    const float f = *failed ? NAN : a.scale;
-    const long long at_row = ((long long)(q0 + row) * a.hq + h) * d;
-    auto put = [&](auto* dst) {
-      if constexpr (TERMS == 3) {
-        if (n > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own);
+          for (int c = 0; c < 64; ++c) if (kb + c > lim) x[c] = 0;
+        }
 #pragma unroll
-        for (int c = 0; c < kOwn; ++c) own[c] *= f;
-#pragma unroll
-        for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own + c);
-      } else {
-        for (int c = 16 * half; c < d; c += 32) {
-          uint32_t o[16];
+        for (int c = 0; c < 64; c += 16) {
           float v[16];
 #pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = 0;
-          if (n > 0) { ld16(lanes + kOut + c, o); wait_ld(o); }
-#pragma unroll
-          for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(o[k]) * f;
-          if (there) store16(dst + c, v);
+          for (int q = 0; q < 16; ++q) v[q] = __uint_as_float(x[c + q]);
+          put16<M, TERMS>(to, lanes, c, v);
         }
+        wait_st();
+        fence_before();
+        arrive(bar(kdqDs));
       }
-    };
-    if (a.pieces > 1) put(a.share[0] + (long long)piece * a.nq * a.hq * d + at_row);
-    else put(static_cast<T*>(a.dq) + at_row);
+      const DqJob after(a, take_job(tail, m, bar(kdqJob), bar(kdqJobFree), lane, failed));
+      stats(after, e, delta);
+      if (j.n > 0) {
+        wait_bar(bar(kdqOut), job & 1, failed, &g_packed_error);
+        fence_after();
+      }
+      const float f = *failed ? NAN : a.scale;
+      const long long at_row = ((long long)(j.q0 + row) * a.hq + j.h) * d;
+      auto put = [&](auto* dst) {
+        if constexpr (TERMS == 3) {
+          if (j.n > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own);
+#pragma unroll
+          for (int c = 0; c < kOwn; ++c) own[c] *= f;
+#pragma unroll
+          for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own + c);
+        } else {
+          for (int c = 16 * half; c < d; c += 32) {
+            uint32_t o[16];
+            float v[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) o[q] = 0;
+            if (j.n > 0) { ld16(lanes + kOut + c, o); wait_ld(o); }
+#pragma unroll
+            for (int q = 0; q < 16; ++q) v[q] = __uint_as_float(o[q]) * f;
+            if (there) store16(dst + c, v);
+          }
+        }
+      };
+      if (a.pieces > 1) put(a.share[0] + (long long)j.piece * a.nq * a.hq * d + at_row);
+      else put(static_cast<T*>(a.dq) + at_row);
+      if (j.n > 0) { fence_before(); arrive(bar(kdqOutRead)); ++job; }
+      j = after;
+    }
     fence_before();
   }
   __syncthreads();
   if (warp == kMmaWarp) { fence_after(); free_tmem(tmem); }
 }
 
-// ---- reverse: dk and dv ---------------------------------------------------------------------------------------------
-// 128 keys of one key head: rows of the products are keys, columns the queries of all heads of the group, 128 at a time.  Tensor memory:
+// dk and dv: 128 keys of one key head.  Rows of the products are keys, columns the queries of all heads of the group, 128 at a time.  Tensor memory:
 // logits at 0 (P replaces them), dP at 128 (dS replaces it), dv at 256, dk at 384 (float32: the third terms of P and dS at 256 and 320, dv
 // at 384, dk at 448; up to 64 values a head in 16 bits: P at 256, dS at 320, dv at 384, dk at 448).  The tensor cores work in the order
 // dv(i), logits(i + 1), dk(i), dP(i + 1): each pair runs beside the other half of the elementwise work.
-enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvFix, kkvStat, kkvStatFree = kkvStat + 2,
-              kkvSRead = kkvStatFree + 2, kkvDpRead, kkvPDone, kkvDsDone, kDkvBars };
+enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvKFree, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvOutRead, kkvFix, kkvStat, kkvStatFree = kkvStat + 2,
+              kkvSRead = kkvStatFree + 2, kkvDpRead, kkvPDone, kkvDsDone, kkvJob, kkvJobFree = kkvJob + 2, kDkvBars = kkvJobFree + 2 };
+struct DkvJob {
+  bool on;
+  int q0, lq, c0, lk, kvh, row0, off, i0, per, j0, n, piece;      // `per` tiles of queries a head from query i0 on; n of all heads' from the j0-th on
+  __device__ __forceinline__ DkvJob(const PackedArgs& a, int index) {
+    on = index >= 0;
+    n = 0;
+    if (!on) return;
+    const int unit = index / a.pieces;
+    piece = index % a.pieces; kvh = unit % a.hk;
+    const int4 item = __ldg(a.items + unit / a.hk);
+    q0 = __ldg(a.start_q + item.x); lq = __ldg(a.start_q + item.x + 1) - q0; c0 = __ldg(a.start_kv + item.x); lk = __ldg(a.start_kv + item.x + 1) - c0;
+    row0 = item.y * kTile; off = lk - lq; i0 = item.z;
+    per = (max(lq - i0, 0) + kTile - 1) / kTile;
+    const int all = per * a.group, share = all / a.pieces, more = all % a.pieces;
+    j0 = piece * share + min(piece, more); n = share + (piece < more);
+  }
+};
 
 template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
@@ -551,18 +641,12 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   volatile int* failed = &tail->failed;
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int unit = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
-  const int4 item = a.items[unit / a.hk];
-  const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int kvh = unit % a.hk, row0 = item.y * kTile, off = lk - lq, i0 = item.z;
-  // tiles of queries of a head, of all heads of the group, and of this piece: from j0 on
-  const int per = (max(lq - i0, 0) + kTile - 1) / kTile, all = per * a.group, share = (all + a.pieces - 1) / a.pieces, j0 = piece * share;
-  const int n = min(share, max(0, all - j0));
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
     for (int i = 0; i < kDkvBars; ++i)
-      init_bar(bar(i), i == kkvP || i == kkvDs || i == kkvSRead || i == kkvDpRead ? 256 : i == kkvStat || i == kkvStat + 1 ? 64 : i == kkvStatFree || i == kkvStatFree + 1 ? 8 : 1);
+      init_bar(bar(i), i == kkvP || i == kkvDs || i == kkvSRead || i == kkvDpRead || i == kkvOutRead ? 256
+                       : i == kkvStat || i == kkvStat + 1 ? 64 : i == kkvStatFree || i == kkvStatFree + 1 ? 8 : i >= kkvJobFree ? 10 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
@@ -572,195 +656,234 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   constexpr bool E = G::kEarly;
   constexpr uint32_t kP = E ? 256 : 0, kDs = E ? 320 : kTile, kDv = E || TERMS == 3 ? 384 : 256, kDk = E || TERMS == 3 ? 448 : 384;
 
+  // tiles (queries 0, 2, .., cotangents 1, 3, ..) and jobs with any are counted as in dq_kernel
   if (warp >= kMmaWarp) {
     fewer_regs<kOtherRegs>();
-    if (warp == kMmaWarp && n > 0) {
+    if (warp == kMmaWarp) {
       const uint32_t on = elect_one();
-      auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };      // queries 0, 2, .., cotangents 1, 3, ..
+      auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
       auto ready = [&](int j) { wait_bar(bar(kkvFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
-      auto give = [&](int j) { if (j + R < 2 * n) commit(on, bar(kkvEmpty + j % R)); };
-      wait_bar(bar(kkvK), 0, failed, &g_packed_error);
-      ready(0);
-      product_rows<M, TERMS, DW>(on, tmem, sk, slot(0), d);
-      commit(on, bar(kkvS));
-      ready(1);
-      product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(1), d);
-      commit(on, bar(kkvDp));
-      for (int i = 0; i < n; ++i) {
-        const bool more = i + 1 < n;
-        auto logits = [&] {
-          if (!more) return;
-          ready(2 * i + 2);
-          if (E) { wait_bar(bar(kkvSRead), i & 1, failed, &g_packed_error); fence_after(); }
-          product_rows<M, TERMS, DW>(on, tmem, sk, slot(2 * i + 2), d);
-          commit(on, bar(kkvS));
-        };
-        auto dp = [&] {
-          if (!more) return;
-          ready(2 * i + 3);
-          if (E) { wait_bar(bar(kkvDpRead), i & 1, failed, &g_packed_error); fence_after(); }
-          product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(2 * i + 3), d);
-          commit(on, bar(kkvDp));
-        };
-        auto packed_at = [&](uint32_t at, uint32_t third) { return E ? Packed{{at}, {32}} : Packed{{at, at + 32, third}, {64, 64, 32}}; };
+      auto give = [&](int j) { commit(on, bar(kkvEmpty + j % R)); };
+      int g = -1, il = 0, jl = 0, ahead = 0;
+      bool done = false, first = false, last = false, first_next = false, last_next = false;      // of tile g and of the next one
+      auto logits = [&] {
+        first_next = il == 0;
+        if (first_next) {
+          wait_bar(bar(kkvK), jl & 1, failed, &g_packed_error);
+          ahead = __shfl_sync(0xffffffffu, *failed ? 0 : tail->tiles[jl & 1], 0);
+          done = ahead == 0;
+        }
+        if (done) return;
+        ready(2 * g + 2);
+        if (E && g >= 0) { wait_bar(bar(kkvSRead), g & 1, failed, &g_packed_error); fence_after(); }
+        product_rows<M, TERMS, DW>(on, tmem, sk, slot(2 * g + 2), d);
+        commit(on, bar(kkvS));
+      };
+      auto dp = [&] {
+        if (done) return;
+        ready(2 * g + 3);
+        if (E && g >= 0) { wait_bar(bar(kkvDpRead), g & 1, failed, &g_packed_error); fence_after(); }
+        product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(2 * g + 3), d);
+        commit(on, bar(kkvDp));
+        last_next = ++il == ahead;
+        if (last_next) { commit(on, bar(kkvKFree)); ++jl; il = 0; }
+      };
+      auto packed_at = [&](uint32_t at, uint32_t third) { return E ? Packed{{at}, {32}} : Packed{{at, at + 32, third}, {64, 64, 32}}; };
+      for (int job = 0;; ++g) {
         if (E) logits();
-        wait_bar(bar(kkvP), i & 1, failed, &g_packed_error);
-        fence_after();
-        product_cols<M, TERMS, DW>(on, tmem + kDv, packed_at(tmem + kP, tmem + 256), slot(2 * i + 1), d, i > 0);
-        if (E) commit(on, bar(kkvPDone));
-        give(2 * i + 1);
+        if (g >= 0) {
+          wait_bar(bar(kkvP), g & 1, failed, &g_packed_error);
+          if (first && job > 0) wait_bar(bar(kkvOutRead), (job - 1) & 1, failed, &g_packed_error);
+          fence_after();
+          product_cols<M, TERMS, DW>(on, tmem + kDv, packed_at(tmem + kP, tmem + 256), slot(2 * g + 1), d, !first);
+          if (E) commit(on, bar(kkvPDone));
+          give(2 * g + 1);
+        }
         if (!E && !G::kShort) logits();
         if (E) dp();
-        wait_bar(bar(kkvDs), i & 1, failed, &g_packed_error);
-        fence_after();
-        product_cols<M, TERMS, DW>(on, tmem + kDk, packed_at(tmem + kDs, tmem + 320), slot(2 * i), d, i > 0);
-        if (E) commit(on, bar(kkvDsDone));
-        give(2 * i);
+        if (g >= 0) {
+          wait_bar(bar(kkvDs), g & 1, failed, &g_packed_error);
+          fence_after();
+          product_cols<M, TERMS, DW>(on, tmem + kDk, packed_at(tmem + kDs, tmem + 320), slot(2 * g), d, !first);
+          if (E) commit(on, bar(kkvDsDone));
+          if (last) { commit(on, bar(kkvOut)); ++job; }
+          give(2 * g);
+        }
         if (G::kShort) logits();
         if (!E) dp();
+        if (done) break;
+        first = first_next; last = last_next;
       }
-      commit(on, bar(kkvOut));
-    } else if (warp == kLoadWarp && n > 0) {
+    } else if (warp == kLoadWarp) {
       Loader<TERMS, DW> ld{lane, bar(kkvFix)};
-      if (lane == 0) {
-        expect(bar(kkvK), 2 * tile_bytes);
-        ld.copies(sk, &maps.k, c0 + row0, kvh, bar(kkvK));
-        ld.copies(sv, &maps.v, c0 + row0, kvh, bar(kkvK));
-      }
-      __syncwarp();
-      for (int j = 0; j < 2 * n; ++j) {
-        if (j >= R) wait_bar(bar(kkvEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
-        const int i = j0 + (j >> 1), hq = kvh * a.group + i / per, b = i0 + (i % per) * kTile;
-        ld.tile(ring + (j % R) * tile_bytes, (j & 1) ? &maps.g : &maps.q, q0 + b, hq, bar(kkvFull + j % R), lq - b, true, failed, &g_packed_error);
-      }
-    } else if (warp > kLoadWarp) {
-      const int r0 = (warp - kLoadWarp - 1) * 32 + lane;
-      for (int i = 0; i < n; ++i) {
-        const int st = i & 1, hq = kvh * a.group + (j0 + i) / per, b = i0 + ((j0 + i) % per) * kTile;
-        if (i >= 2) wait_bar(bar(kkvStatFree + st), ((i >> 1) - 1) & 1, failed, &g_packed_error);
-        for (int r = r0; r < kTile; r += 64) {
-          const bool ok = b + r < lq;
-          const long long at = (long long)hq * a.nq + q0 + b + r;
-          stats[st * kTile + r] = ok ? packed::prob_shift<T>() - a.lse[at] : -INFINITY;
-          stats[(2 + st) * kTile + r] = ok ? -a.delta[at] * packed::prob_unscale<T>() : 0.f;
+      int g = 0, job = 0;
+      for (int m = 0, index = blockIdx.x;; ++m) {
+        publish_job(tail, m, index, a.jobs, bar(kkvJob), bar(kkvJobFree), lane, failed);
+        if (__any_sync(0xffffffffu, index >= a.jobs || *failed)) break;
+        const DkvJob j(a, index);
+        for (int i = 0; i < 2 * j.n; ++i, ++g) {
+          if (i == 1) {
+            if (job > 0) wait_bar(bar(kkvKFree), (job - 1) & 1, failed, &g_packed_error);
+            if (lane == 0) {
+              tail->tiles[job & 1] = j.n;
+              expect(bar(kkvK), 2 * tile_bytes);
+              ld.copies(sk, &maps.k, j.c0 + j.row0, j.kvh, bar(kkvK));
+              ld.copies(sv, &maps.v, j.c0 + j.row0, j.kvh, bar(kkvK));
+            }
+            __syncwarp();
+          }
+          if (g >= R) wait_bar(bar(kkvEmpty + g % R), (g / R - 1) & 1, failed, &g_packed_error);
+          const int t = j.j0 + (i >> 1), hq = j.kvh * a.group + t / j.per, b = j.i0 + (t % j.per) * kTile;
+          ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.g : &maps.q, j.q0 + b, hq, bar(kkvFull + g % R), j.lq - b, true, failed, &g_packed_error);
         }
-        arrive(bar(kkvStat + st));
+        job += j.n > 0;
+        if (lane == 0) index = (int)gridDim.x + atomicAdd(a.queue + 1, 1);
+        index = __shfl_sync(0xffffffffu, index, 0);
+      }
+      if (job > 0) wait_bar(bar(kkvKFree), (job - 1) & 1, failed, &g_packed_error);
+      if (lane == 0) { tail->tiles[job & 1] = 0; arrive(bar(kkvK)); }      // no more jobs
+      __syncwarp();
+      for (int t = max(0, g - R); t < g; ++t) wait_bar(bar(kkvEmpty + t % R), (t / R) & 1, failed, &g_packed_error);
+    } else {
+      const int r0 = (warp - kLoadWarp - 1) * 32 + lane;
+      int g = 0;
+      for (int m = 0;; ++m) {
+        const DkvJob j(a, take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, failed));
+        if (!j.on) break;
+        for (int i = 0; i < j.n; ++i, ++g) {
+          const int st = g & 1, hq = j.kvh * a.group + (j.j0 + i) / j.per, b = j.i0 + ((j.j0 + i) % j.per) * kTile;
+          if (g >= 2) wait_bar(bar(kkvStatFree + st), ((g >> 1) - 1) & 1, failed, &g_packed_error);
+          for (int r = r0; r < kTile; r += 64) {
+            const bool ok = b + r < j.lq;
+            const long long at = (long long)hq * a.nq + j.q0 + b + r;
+            stats[st * kTile + r] = ok ? packed::prob_shift<T>() - a.lse[at] : -INFINITY;
+            stats[(2 + st) * kTile + r] = ok ? -a.delta[at] * packed::prob_unscale<T>() : 0.f;
+          }
+          arrive(bar(kkvStat + st));
+        }
       }
     }
   } else {
     more_regs<kComputeRegs>();
-    const int half = warp >> 2, w = warp & 3, row = row0 + w * 32 + lane, last = row0 + w * 32 + 31, col = 64 * half;
-    const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16);
-    // first query that sees this key, and that sees the warp's last key
-    const int lim = a.causal ? row - off : 0, lim_last = a.causal ? last - off : 0;
-    constexpr int kOwn = TERMS == 1 ? 1 : DW / 2;
-    float own[2][kOwn];                      // dv, dk so far (float32), half of the row
-#pragma unroll
-    for (int c = 0; c < kOwn; ++c) own[0][c] = own[1][c] = 0.f;
-    const float2 scale = make_float2(a.scale_log2, a.scale_log2);
-    const uint32_t c2 = col / 2;
+    const int half = warp >> 2, w = warp & 3, col = 64 * half;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16), c2 = col / 2;
     const Packed to_p = E ? Packed{{kP + c2}, {}} : Packed{{kP + (uint32_t)col, kP + 32 + (uint32_t)col, 256 + c2}, {}};
     const Packed to_s = E ? Packed{{kDs + c2}, {}} : Packed{{kDs + (uint32_t)col, kDs + 32 + (uint32_t)col, 320 + c2}, {}};
-    for (int i = 0; i < n; ++i) {
-      const int st = i & 1, ib = i0 + ((j0 + i) % per) * kTile + col;
-      uint32_t x[64], y[64];
-      wait_bar(bar(kkvStat + st), (i >> 1) & 1, failed, &g_packed_error);
-      wait_bar(bar(kkvS), i & 1, failed, &g_packed_error);
-      fence_after();
-      ld32(lanes + col, x);
-      ld32(lanes + col + 32, x + 32);
-      wait_ld(x);
-      if (E) { fence_before(); arrive(bar(kkvSRead)); }
-      if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDv + half * (DW / 2), own[0]); }
-      const float4* e = reinterpret_cast<const float4*>(stats + st * kTile + col);
+    const float2 scale = make_float2(a.scale_log2, a.scale_log2);
+    int g = 0, job = 0;
+    DkvJob j(a, take_job(tail, 0, bar(kkvJob), bar(kkvJobFree), lane, failed));
+    for (int m = 1; j.on; ++m) {
+      const int row = j.row0 + w * 32 + lane, last = j.row0 + w * 32 + 31;
+      // first query that sees this key, and that sees the warp's last key
+      const int lim = a.causal ? row - j.off : 0, lim_last = a.causal ? last - j.off : 0;
+      constexpr int kOwn = TERMS == 1 ? 1 : DW / 2;
+      float own[2][kOwn];                      // dv, dk so far (float32), half of the row
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        const float4 v = e[c];
-        const float2 z0 = __ffma2_rn(make_float2(__uint_as_float(x[4 * c]), __uint_as_float(x[4 * c + 1])), scale, make_float2(v.x, v.y));
-        const float2 z1 = __ffma2_rn(make_float2(__uint_as_float(x[4 * c + 2]), __uint_as_float(x[4 * c + 3])), scale, make_float2(v.z, v.w));
-        const float2 r1 = TERMS == 1 ? pow2_poly(z1) : make_float2(pow2(z1.x), pow2(z1.y));
-        x[4 * c] = __float_as_uint(pow2(z0.x)); x[4 * c + 1] = __float_as_uint(pow2(z0.y));
-        x[4 * c + 2] = __float_as_uint(r1.x); x[4 * c + 3] = __float_as_uint(r1.y);
-      }
-      if (E && i > 0) { wait_bar(bar(kkvPDone), (i - 1) & 1, failed, &g_packed_error); fence_after(); }
-      if (a.causal && ib < lim_last) {
+      for (int c = 0; c < kOwn; ++c) own[0][c] = own[1][c] = 0.f;
+      for (int i = 0; i < j.n; ++i, ++g) {
+        const int st = g & 1, ib = j.i0 + ((j.j0 + i) % j.per) * kTile + col;
+        uint32_t x[64], y[64];
+        wait_bar(bar(kkvStat + st), (g >> 1) & 1, failed, &g_packed_error);
+        wait_bar(bar(kkvS), g & 1, failed, &g_packed_error);
+        fence_after();
+        ld32(lanes + col, x);
+        ld32(lanes + col + 32, x + 32);
+        wait_ld(x);
+        if (E) { fence_before(); arrive(bar(kkvSRead)); }
+        if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDv + half * (DW / 2), own[0]); }
+        const float4* e = reinterpret_cast<const float4*>(stats + st * kTile + col);
 #pragma unroll
-        for (int c = 0; c < 64; ++c) if (ib + c < lim) x[c] = 0;
-      }
+        for (int c = 0; c < 16; ++c) {
+          const float4 v = e[c];
+          const float2 z0 = __ffma2_rn(make_float2(__uint_as_float(x[4 * c]), __uint_as_float(x[4 * c + 1])), scale, make_float2(v.x, v.y));
+          const float2 z1 = __ffma2_rn(make_float2(__uint_as_float(x[4 * c + 2]), __uint_as_float(x[4 * c + 3])), scale, make_float2(v.z, v.w));
+          const float2 r1 = TERMS == 1 ? pow2_poly(z1) : make_float2(pow2(z1.x), pow2(z1.y));
+          x[4 * c] = __float_as_uint(pow2(z0.x)); x[4 * c + 1] = __float_as_uint(pow2(z0.y));
+          x[4 * c + 2] = __float_as_uint(r1.x); x[4 * c + 3] = __float_as_uint(r1.y);
+        }
+        if (E && g > 0) { wait_bar(bar(kkvPDone), (g - 1) & 1, failed, &g_packed_error); fence_after(); }
+        if (a.causal && ib < lim_last) {
 #pragma unroll
-      for (int c = 0; c < 64; c += 16) {
-        float v[16];
+          for (int c = 0; c < 64; ++c) if (ib + c < lim) x[c] = 0;
+        }
 #pragma unroll
-        for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(x[c + k]);
-        put16<M, TERMS>(to_p, lanes, c, v);
-      }
-      wait_st();
-      fence_before();
-      arrive(bar(kkvP));
-      wait_bar(bar(kkvDp), i & 1, failed, &g_packed_error);
-      fence_after();
-      ld32(lanes + kTile + col, y);
-      ld32(lanes + kTile + col + 32, y + 32);
-      wait_ld(y);
-      if (E) {
+        for (int c = 0; c < 64; c += 16) {
+          float v[16];
+#pragma unroll
+          for (int q = 0; q < 16; ++q) v[q] = __uint_as_float(x[c + q]);
+          put16<M, TERMS>(to_p, lanes, c, v);
+        }
+        wait_st();
         fence_before();
-        arrive(bar(kkvDpRead));
-        if (i > 0) { wait_bar(bar(kkvDsDone), (i - 1) & 1, failed, &g_packed_error); fence_after(); }
-      }
-      if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDk + half * (DW / 2), own[1]); }
-      const float4* dl = reinterpret_cast<const float4*>(stats + (2 + st) * kTile + col);
-      constexpr float un = packed::prob_unscale<T>();
-#pragma unroll
-      for (int c = 0; c < 64; c += 16) {
-        float v[16];
-#pragma unroll
-        for (int k = 0; k < 16; k += 4) {
-          const float4 z = dl[(c + k) / 4];
-          v[k] = __uint_as_float(x[c + k]) * fmaf(__uint_as_float(y[c + k]), un, z.x);
-          v[k + 1] = __uint_as_float(x[c + k + 1]) * fmaf(__uint_as_float(y[c + k + 1]), un, z.y);
-          v[k + 2] = __uint_as_float(x[c + k + 2]) * fmaf(__uint_as_float(y[c + k + 2]), un, z.z);
-          v[k + 3] = __uint_as_float(x[c + k + 3]) * fmaf(__uint_as_float(y[c + k + 3]), un, z.w);
+        arrive(bar(kkvP));
+        wait_bar(bar(kkvDp), g & 1, failed, &g_packed_error);
+        fence_after();
+        ld32(lanes + kTile + col, y);
+        ld32(lanes + kTile + col + 32, y + 32);
+        wait_ld(y);
+        if (E) {
+          fence_before();
+          arrive(bar(kkvDpRead));
+          if (g > 0) { wait_bar(bar(kkvDsDone), (g - 1) & 1, failed, &g_packed_error); fence_after(); }
         }
-        put16<M, TERMS>(to_s, lanes, c, v);
-      }
-      __syncwarp();
-      if (lane == 0) arrive(bar(kkvStatFree + st));
-      wait_st();
-      fence_before();
-      arrive(bar(kkvDs));
-    }
-    if (n > 0) {
-      wait_bar(bar(kkvOut), 0, failed, &g_packed_error);
-      fence_after();
-    }
-    const bool there = row < lk, bad = *failed;
-    const long long at = ((long long)(c0 + row) * a.hk + kvh) * d;
+        if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDk + half * (DW / 2), own[1]); }
+        const float4* dl = reinterpret_cast<const float4*>(stats + (2 + st) * kTile + col);
+        constexpr float un = packed::prob_unscale<T>();
 #pragma unroll
-    for (int which = 0; which < 2; ++which) {
-      const float f = bad ? NAN : which ? a.scale : packed::prob_unscale<T>();
-      const uint32_t from = lanes + (which ? kDk : kDv);
-      auto put = [&](auto* dst) {
-        if constexpr (TERMS == 3) {
-          if (n > 0) add_cols<DW, DW / 2>(from + half * (DW / 2), own[which]);
+        for (int c = 0; c < 64; c += 16) {
+          float v[16];
 #pragma unroll
-          for (int c = 0; c < kOwn; ++c) own[which][c] *= f;
-#pragma unroll
-          for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own[which] + c);
-        } else {
-          for (int c = 16 * half; c < d; c += 32) {
-            uint32_t o[16];
-            float v[16];
-#pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = 0;
-            if (n > 0) { ld16(from + c, o); wait_ld(o); }
-#pragma unroll
-            for (int k = 0; k < 16; ++k) v[k] = __uint_as_float(o[k]) * f;
-            if (there) store16(dst + c, v);
+          for (int q = 0; q < 16; q += 4) {
+            const float4 z = dl[(c + q) / 4];
+            v[q] = __uint_as_float(x[c + q]) * fmaf(__uint_as_float(y[c + q]), un, z.x);
+            v[q + 1] = __uint_as_float(x[c + q + 1]) * fmaf(__uint_as_float(y[c + q + 1]), un, z.y);
+            v[q + 2] = __uint_as_float(x[c + q + 2]) * fmaf(__uint_as_float(y[c + q + 2]), un, z.z);
+            v[q + 3] = __uint_as_float(x[c + q + 3]) * fmaf(__uint_as_float(y[c + q + 3]), un, z.w);
           }
+          put16<M, TERMS>(to_s, lanes, c, v);
         }
-      };
-      if (a.pieces > 1) put(a.share[which ? 1 : 2] + (long long)piece * a.nkv * a.hk * d + at);
-      else put(static_cast<T*>(which ? a.dk : a.dv) + at);
+        __syncwarp();
+        if (lane == 0) arrive(bar(kkvStatFree + st));
+        wait_st();
+        fence_before();
+        arrive(bar(kkvDs));
+      }
+      const DkvJob after(a, take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, failed));
+      if (j.n > 0) {
+        wait_bar(bar(kkvOut), job & 1, failed, &g_packed_error);
+        fence_after();
+      }
+      const bool there = row < j.lk, bad = *failed;
+      const long long at = ((long long)(j.c0 + row) * a.hk + j.kvh) * d;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const float f = bad ? NAN : which ? a.scale : packed::prob_unscale<T>();
+        const uint32_t from = lanes + (which ? kDk : kDv);
+        auto put = [&](auto* dst) {
+          if constexpr (TERMS == 3) {
+            if (j.n > 0) add_cols<DW, DW / 2>(from + half * (DW / 2), own[which]);
+#pragma unroll
+            for (int c = 0; c < kOwn; ++c) own[which][c] *= f;
+#pragma unroll
+            for (int c = 0; c < kOwn; c += 16) if (there && half * kOwn + c < d) store16(dst + half * kOwn + c, own[which] + c);
+          } else {
+            for (int c = 16 * half; c < d; c += 32) {
+              uint32_t o[16];
+              float v[16];
+#pragma unroll
+              for (int q = 0; q < 16; ++q) o[q] = 0;
+              if (j.n > 0) { ld16(from + c, o); wait_ld(o); }
+#pragma unroll
+              for (int q = 0; q < 16; ++q) v[q] = __uint_as_float(o[q]) * f;
+              if (there) store16(dst + c, v);
+            }
+          }
+        };
+        if (a.pieces > 1) put(a.share[which ? 1 : 2] + (long long)j.piece * a.nkv * a.hk * d + at);
+        else put(static_cast<T*>(which ? a.dk : a.dv) + at);
+      }
+      if (j.n > 0) { fence_before(); arrive(bar(kkvOutRead)); ++job; }
+      j = after;
     }
     fence_before();
   }
@@ -768,7 +891,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   if (warp == kMmaWarp) { fence_after(); free_tmem(tmem); }
 }
 
-static_assert(kFwdBars <= 32 && kDqBars <= 32 && kDkvBars <= 32, "barriers");
+static_assert(kFwdBars <= kBars && kDqBars <= kBars && kDkvBars <= kBars, "barriers");
 
 // float32 rows -> three bfloat16 terms, (rows, heads, 3, DW), zeros behind d; a thread per eight values, up to four operands
 struct SplitArgs { Rows src[4]; __nv_bfloat16* dst[4]; int rows[4], heads[4]; };
@@ -862,6 +985,12 @@ template <auto kernel> int launch(int64_t grid, int threads, int smem, cudaStrea
   count_launch();
   return kOk;
 }
+// a CTA per SM, which work through `jobs`
+template <auto kernel> int launch_jobs(int64_t jobs, int smem, cudaStream_t st, PackedArgs a, const Maps& m) {
+  if (jobs > 0x7fff0000) return kTooLarge;
+  a.jobs = (int)jobs;
+  return launch<kernel>(std::min<int64_t>(jobs, sm_count()), kThreads, smem, st, a, m);
+}
 template <typename T, int TERMS, int DW, int TILES> int forward_of(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace) {
   Maps m;
   int rc = maps_of<T, TERMS, DW>(&m, st, a, false, workspace);
@@ -887,11 +1016,11 @@ int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, cons
   if (pieces.dkv > 1) { a.share[1] = share; a.share[2] = share + pieces.dkv * stride_kv; }
   a.items = items_q;
   a.pieces = pieces.dq;
-  rc = launch<dq_kernel<T, TERMS, DW>>((int64_t)n_q * a.hq * a.pieces, kThreads, reverse_smem<TERMS, DW>(false), st, a, m);
+  rc = launch_jobs<dq_kernel<T, TERMS, DW>>((int64_t)n_q * a.hq * a.pieces, reverse_smem<TERMS, DW>(false), st, a, m);
   if (rc) return rc;
   a.items = items_kv;
   a.pieces = pieces.dkv;
-  rc = launch<dkv_kernel<T, TERMS, DW>>((int64_t)n_kv * a.hk * a.pieces, kThreads, reverse_smem<TERMS, DW>(true), st, a, m);
+  rc = launch_jobs<dkv_kernel<T, TERMS, DW>>((int64_t)n_kv * a.hk * a.pieces, reverse_smem<TERMS, DW>(true), st, a, m);
   if (rc || (pieces.dq == 1 && pieces.dkv == 1)) return rc;
   return packed_sum<T>(st, a, pieces.dq, pieces.dkv);
 }
