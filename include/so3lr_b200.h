@@ -444,8 +444,8 @@ SO3LR_B200_API int so3lr_b200_structure_attention_vjp(const int32_t* image, cons
                                                       const so3lr_b200_rows* k, const so3lr_b200_rows* v, const void* out, const void* out_rest,
                                                       const float* lse, const so3lr_b200_rows* g, float* delta, void* d_q, void* d_k, void* d_v,
                                                       void* workspace, int64_t workspace_bytes);
-/* 1 where a bounded wait of the tensor-core kernels has run out on the current device since the library was loaded (their rows are NaN
- * then); waits for the device */
+/* 1 where a bounded wait of the tensor-core kernels has run out on the current device since the library was loaded (the rows at hand are
+ * NaN, or not written, then); waits for the device */
 SO3LR_B200_API int so3lr_b200_structure_attention_error(int* out);
 
 /* Host-callable pieces of the device math, exported for the CPU tests (no GPU needed). */

@@ -27,11 +27,18 @@ using namespace tc;
 
 // barriers and scratch behind the tiles
 constexpr int kBars = 40;
+// What a CTA of a reverse kernel works on at a time: a tile of rows from row0 on of one head (or key head) h against n tiles of the other side, a
+// piece of an item's walk.  n < 0: there is no more.
+struct Job {
+  int q0, lq, c0, lk, h, row0, n, piece;
+  int k0;               // dq: first key
+  int i0, per, j0;      // dk and dv: first query; tiles of queries of a head from there on; the job's first one among those of all heads of the group
+};
 struct Tail {
   unsigned long long bars[kBars];
   uint32_t tmem;
   int failed;
-  int jobs[2];       // reverse kernels: indices of the jobs at hand, -1 behind the last one
+  Job jobs[2];       // reverse kernels: the jobs at hand
   int tiles[2];      // and tiles of those that have any, 0 behind the last one
 };
 template <typename T, int TERMS> struct Operand { using type = T; };
@@ -342,21 +349,24 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
 }
 
 // ---- reverse --------------------------------------------------------------------------------------------------------
-// A CTA stays on its SM and works through jobs (an item's piece of one head), so that a job's first tiles come in and its first products run
-// while the last results of the one before leave: with a CTA per job 6 of the 11 us of a job of 500 rows went by in its start and end (24 structures of
-// 150 to 900 rows, 16 heads x 64: dq @DQ0 -> @DQ1 us, dk and dv @KV0 -> @KV1).  The loading warp takes jobs from a queue, the
-// longest first (equal shares instead: SMs differ in their pace, @EQ), and passes them on through shared memory.
-__device__ __forceinline__ void publish_job(Tail* tail, int m, int index, int jobs, uint32_t full, uint32_t free, int lane, volatile int* failed) {
+// A CTA stays on its SM and works through jobs, so that a job's first tiles come in and its first products run while the last results of the
+// one before leave: with a CTA per job its start and end took 5 to 6 us, now 2.4 to 3.5.  dq / dk and dv, a CTA per job -> this, us: 24 structures of 150 to
+// 900 rows, 16 heads x 64, 124 / 147 -> 102 / 129; 64 of 64 to 128, 8 x 128, 28 / 32 -> 21 / 25; 8 causal ones of 2,000, 40 x 128, 613 / 588 ->
+// 549 / 594; one of 8,192, 9 x 64, 290 / 351 -> 303 / 366 (a job of 64 tiles has no start to hide).  The loading warp takes jobs from a queue, the
+// longest first, and passes them on through shared memory (equal shares instead: SMs differ in their pace by up to 15 %; 5,000 rows, 4 x 32
+// float32, dk and dv 184 us with the queue, 219 without).
+__device__ __forceinline__ void publish_job(Tail* tail, int m, const Job& j, uint32_t full, uint32_t free, int lane, volatile int* failed) {
   if (m >= 2) wait_bar(free + 8 * (m & 1), ((m >> 1) - 1) & 1, failed, &g_packed_error);
-  if (lane == 0) { tail->jobs[m & 1] = index < jobs ? index : -1; arrive(full + 8 * (m & 1)); }
+  if (lane == 0) { tail->jobs[m & 1] = j; arrive(full + 8 * (m & 1)); }
   __syncwarp();
 }
-// index of a warp's m-th job
-__device__ __forceinline__ int take_job(const Tail* tail, int m, uint32_t full, uint32_t free, int lane, volatile int* failed) {
+// a warp's m-th job
+__device__ __forceinline__ Job take_job(const Tail* tail, int m, uint32_t full, uint32_t free, int lane, volatile int* failed) {
   wait_bar(full + 8 * (m & 1), (m >> 1) & 1, failed, &g_packed_error);
-  const int index = __shfl_sync(0xffffffffu, *failed ? -1 : *const_cast<const volatile int*>(tail->jobs + (m & 1)), 0);
+  Job j = tail->jobs[m & 1];
+  if (__any_sync(0xffffffffu, *failed)) j.n = -1;
   if (lane == 0) arrive(free + 8 * (m & 1));
-  return index;
+  return j;
 }
 
 // dq: 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256 (float32: the third term of dS
@@ -364,22 +374,19 @@ __device__ __forceinline__ int take_job(const Tail* tail, int m, uint32_t full, 
 // next tile's logits are made as soon as these have been read, so that its exponentials run beside the products dS k and g v^T.
 enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqQFree, kdqS, kdqSRead, kdqDp, kdqDpRead, kdqDs, kdqDsDone, kdqOut, kdqOutRead, kdqFix, kdqJob,
              kdqJobFree = kdqJob + 2, kDqBars = kdqJobFree + 2 };
-struct DqJob {
-  bool on;
-  int q0, lq, c0, lk, h, row0, off, k0, n, piece;      // n tiles of keys from key k0 on
-  __device__ __forceinline__ DqJob(const PackedArgs& a, int index) {
-    on = index >= 0;
-    n = 0;
-    if (!on) return;
-    const int unit = index / a.pieces;
-    piece = index % a.pieces; h = unit % a.hq;
-    const int4 item = __ldg(a.items + unit / a.hq);
-    q0 = __ldg(a.start_q + item.x); lq = __ldg(a.start_q + item.x + 1) - q0; c0 = __ldg(a.start_kv + item.x); lk = __ldg(a.start_kv + item.x + 1) - c0;
-    row0 = item.y * kTile; off = lk - lq;
-    const int all = (item.w + kTile - 1) / kTile, share = all / a.pieces, more = all % a.pieces;
-    k0 = (piece * share + min(piece, more)) * kTile; n = share + (piece < more);
-  }
-};
+__device__ __forceinline__ Job dq_job(const PackedArgs& a, int index) {
+  Job j = {};
+  j.n = -1;
+  if (index >= a.jobs) return j;
+  const int unit = index / a.pieces;
+  const int4 item = __ldg(a.items + unit / a.hq);
+  j.piece = index % a.pieces; j.h = unit % a.hq;
+  j.q0 = __ldg(a.start_q + item.x); j.lq = __ldg(a.start_q + item.x + 1) - j.q0; j.c0 = __ldg(a.start_kv + item.x); j.lk = __ldg(a.start_kv + item.x + 1) - j.c0;
+  j.row0 = item.y * kTile;
+  const int all = (item.w + kTile - 1) / kTile, share = all / a.pieces, more = all % a.pieces;
+  j.k0 = (j.piece * share + min(j.piece, more)) * kTile; j.n = share + (j.piece < more);
+  return j;
+}
 
 template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
@@ -466,9 +473,9 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       Loader<TERMS, DW> ld{lane, bar(kdqFix)};
       int g = 0, job = 0;
       for (int m = 0, index = blockIdx.x;; ++m) {
-        publish_job(tail, m, index, a.jobs, bar(kdqJob), bar(kdqJobFree), lane, failed);
-        if (__any_sync(0xffffffffu, index >= a.jobs || *failed)) break;
-        const DqJob j(a, index);
+        const Job j = dq_job(a, index);
+        publish_job(tail, m, j, bar(kdqJob), bar(kdqJobFree), lane, failed);
+        if (__any_sync(0xffffffffu, j.n < 0 || *failed)) break;
         for (int i = 0; i < 2 * j.n; ++i, ++g) {
           if (i == 1) {      // behind the first tile of keys, which finds room earlier
             if (job > 0) wait_bar(bar(kdqQFree), (job - 1) & 1, failed, &g_packed_error);
@@ -501,18 +508,19 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
     const Packed to = E ? Packed{{kDs + c2, kDs + 64 + c2, kDs + 128 + c2}, {}} : Packed{{kDs + (uint32_t)col, kDs + 32 + (uint32_t)col, 256 + c2}, {}};
     const float2 scale = make_float2(a.scale_log2, a.scale_log2);
     // a row's statistics; rows that are not there: exp(-inf) = 0
-    auto stats = [&](const DqJob& j, float& e, float& delta) {
+    auto stats = [&](const Job& j, float& e, float& delta) {
       const int row = j.row0 + w * 32 + lane;
       e = -INFINITY; delta = 0.f;
-      if (j.on && row < j.lq) { const long long at = (long long)j.h * a.nq + j.q0 + row; e = -a.lse[at]; delta = a.delta[at]; }
+      if (j.n >= 0 && row < j.lq) { const long long at = (long long)j.h * a.nq + j.q0 + row; e = -a.lse[at]; delta = a.delta[at]; }
     };
     int g = 0, job = 0;
-    DqJob j(a, take_job(tail, 0, bar(kdqJob), bar(kdqJobFree), lane, failed));
+    Job j = take_job(tail, 0, bar(kdqJob), bar(kdqJobFree), lane, failed);
     float e, delta;
     stats(j, e, delta);
-    for (int m = 1; j.on; ++m) {
+    for (int m = 1; j.n >= 0; ++m) {
       const int row = j.row0 + w * 32 + lane, first = j.row0 + w * 32;
-      const int lim = min(a.causal ? row + j.off : j.lk - 1, j.lk - 1), lim_first = min(a.causal ? first + j.off : j.lk - 1, j.lk - 1);
+      const int off = j.lk - j.lq;
+      const int lim = min(a.causal ? row + off : j.lk - 1, j.lk - 1), lim_first = min(a.causal ? first + off : j.lk - 1, j.lk - 1);
       const bool there = row < j.lq;
       constexpr int kOwn = TERMS == 1 ? 1 : DW / 2;
       float own[kOwn];                         // dq so far (float32), half of the row
@@ -564,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
         fence_before();
         arrive(bar(kdqDs));
       }
-      const DqJob after(a, take_job(tail, m, bar(kdqJob), bar(kdqJobFree), lane, failed));
+      const Job after = take_job(tail, m, bar(kdqJob), bar(kdqJobFree), lane, failed);
       stats(after, e, delta);
       if (j.n > 0) {
         wait_bar(bar(kdqOut), job & 1, failed, &g_packed_error);
@@ -609,23 +617,20 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
 // dv(i), logits(i + 1), dk(i), dP(i + 1): each pair runs beside the other half of the elementwise work.
 enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvKFree, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvOutRead, kkvFix, kkvStat, kkvStatFree = kkvStat + 2,
               kkvSRead = kkvStatFree + 2, kkvDpRead, kkvPDone, kkvDsDone, kkvJob, kkvJobFree = kkvJob + 2, kDkvBars = kkvJobFree + 2 };
-struct DkvJob {
-  bool on;
-  int q0, lq, c0, lk, kvh, row0, off, i0, per, j0, n, piece;      // `per` tiles of queries a head from query i0 on; n of all heads' from the j0-th on
-  __device__ __forceinline__ DkvJob(const PackedArgs& a, int index) {
-    on = index >= 0;
-    n = 0;
-    if (!on) return;
-    const int unit = index / a.pieces;
-    piece = index % a.pieces; kvh = unit % a.hk;
-    const int4 item = __ldg(a.items + unit / a.hk);
-    q0 = __ldg(a.start_q + item.x); lq = __ldg(a.start_q + item.x + 1) - q0; c0 = __ldg(a.start_kv + item.x); lk = __ldg(a.start_kv + item.x + 1) - c0;
-    row0 = item.y * kTile; off = lk - lq; i0 = item.z;
-    per = (max(lq - i0, 0) + kTile - 1) / kTile;
-    const int all = per * a.group, share = all / a.pieces, more = all % a.pieces;
-    j0 = piece * share + min(piece, more); n = share + (piece < more);
-  }
-};
+__device__ __forceinline__ Job dkv_job(const PackedArgs& a, int index) {
+  Job j = {};
+  j.n = -1;
+  if (index >= a.jobs) return j;
+  const int unit = index / a.pieces;
+  const int4 item = __ldg(a.items + unit / a.hk);
+  j.piece = index % a.pieces; j.h = unit % a.hk;
+  j.q0 = __ldg(a.start_q + item.x); j.lq = __ldg(a.start_q + item.x + 1) - j.q0; j.c0 = __ldg(a.start_kv + item.x); j.lk = __ldg(a.start_kv + item.x + 1) - j.c0;
+  j.row0 = item.y * kTile; j.i0 = item.z;
+  j.per = (max(j.lq - j.i0, 0) + kTile - 1) / kTile;
+  const int all = j.per * a.group, share = all / a.pieces, more = all % a.pieces;
+  j.j0 = j.piece * share + min(j.piece, more); j.n = share + (j.piece < more);
+  return j;
+}
 
 template <typename T, int TERMS, int DW>
 __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
@@ -718,22 +723,22 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       Loader<TERMS, DW> ld{lane, bar(kkvFix)};
       int g = 0, job = 0;
       for (int m = 0, index = blockIdx.x;; ++m) {
-        publish_job(tail, m, index, a.jobs, bar(kkvJob), bar(kkvJobFree), lane, failed);
-        if (__any_sync(0xffffffffu, index >= a.jobs || *failed)) break;
-        const DkvJob j(a, index);
+        const Job j = dkv_job(a, index);
+        publish_job(tail, m, j, bar(kkvJob), bar(kkvJobFree), lane, failed);
+        if (__any_sync(0xffffffffu, j.n < 0 || *failed)) break;
         for (int i = 0; i < 2 * j.n; ++i, ++g) {
           if (i == 1) {
             if (job > 0) wait_bar(bar(kkvKFree), (job - 1) & 1, failed, &g_packed_error);
             if (lane == 0) {
               tail->tiles[job & 1] = j.n;
               expect(bar(kkvK), 2 * tile_bytes);
-              ld.copies(sk, &maps.k, j.c0 + j.row0, j.kvh, bar(kkvK));
-              ld.copies(sv, &maps.v, j.c0 + j.row0, j.kvh, bar(kkvK));
+              ld.copies(sk, &maps.k, j.c0 + j.row0, j.h, bar(kkvK));
+              ld.copies(sv, &maps.v, j.c0 + j.row0, j.h, bar(kkvK));
             }
             __syncwarp();
           }
           if (g >= R) wait_bar(bar(kkvEmpty + g % R), (g / R - 1) & 1, failed, &g_packed_error);
-          const int t = j.j0 + (i >> 1), hq = j.kvh * a.group + t / j.per, b = j.i0 + (t % j.per) * kTile;
+          const int t = j.j0 + (i >> 1), hq = j.h * a.group + t / j.per, b = j.i0 + (t % j.per) * kTile;
           ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.g : &maps.q, j.q0 + b, hq, bar(kkvFull + g % R), j.lq - b, true, failed, &g_packed_error);
         }
         job += j.n > 0;
@@ -748,10 +753,10 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       const int r0 = (warp - kLoadWarp - 1) * 32 + lane;
       int g = 0;
       for (int m = 0;; ++m) {
-        const DkvJob j(a, take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, failed));
-        if (!j.on) break;
+        const Job j = take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, failed);
+        if (j.n < 0) break;
         for (int i = 0; i < j.n; ++i, ++g) {
-          const int st = g & 1, hq = j.kvh * a.group + (j.j0 + i) / j.per, b = j.i0 + ((j.j0 + i) % j.per) * kTile;
+          const int st = g & 1, hq = j.h * a.group + (j.j0 + i) / j.per, b = j.i0 + ((j.j0 + i) % j.per) * kTile;
           if (g >= 2) wait_bar(bar(kkvStatFree + st), ((g >> 1) - 1) & 1, failed, &g_packed_error);
           for (int r = r0; r < kTile; r += 64) {
             const bool ok = b + r < j.lq;
@@ -771,11 +776,11 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
     const Packed to_s = E ? Packed{{kDs + c2}, {}} : Packed{{kDs + (uint32_t)col, kDs + 32 + (uint32_t)col, 320 + c2}, {}};
     const float2 scale = make_float2(a.scale_log2, a.scale_log2);
     int g = 0, job = 0;
-    DkvJob j(a, take_job(tail, 0, bar(kkvJob), bar(kkvJobFree), lane, failed));
-    for (int m = 1; j.on; ++m) {
+    Job j = take_job(tail, 0, bar(kkvJob), bar(kkvJobFree), lane, failed);
+    for (int m = 1; j.n >= 0; ++m) {
       const int row = j.row0 + w * 32 + lane, last = j.row0 + w * 32 + 31;
       // first query that sees this key, and that sees the warp's last key
-      const int lim = a.causal ? row - j.off : 0, lim_last = a.causal ? last - j.off : 0;
+      const int off = j.lk - j.lq, lim = a.causal ? row - off : 0, lim_last = a.causal ? last - off : 0;
       constexpr int kOwn = TERMS == 1 ? 1 : DW / 2;
       float own[2][kOwn];                      // dv, dk so far (float32), half of the row
 #pragma unroll
@@ -848,13 +853,13 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         fence_before();
         arrive(bar(kkvDs));
       }
-      const DkvJob after(a, take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, failed));
+      const Job after = take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, failed);
       if (j.n > 0) {
         wait_bar(bar(kkvOut), job & 1, failed, &g_packed_error);
         fence_after();
       }
       const bool there = row < j.lk, bad = *failed;
-      const long long at = ((long long)(j.c0 + row) * a.hk + j.kvh) * d;
+      const long long at = ((long long)(j.c0 + row) * a.hk + j.h) * d;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
         const float f = bad ? NAN : which ? a.scale : packed::prob_unscale<T>();

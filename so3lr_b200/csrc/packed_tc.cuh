@@ -35,7 +35,7 @@ __device__ __forceinline__ bool test_bar(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 // Every wait ends: after two seconds, or when another one of this CTA has run out, the kernel carries on to its end, reports through
-// *error, and writes NaN.
+// *error, and writes NaN to the rows at hand.
 __device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity, volatile int* failed, int* error) {
   if (test_bar(bar, parity)) return;
   unsigned long long t0 = 0;
