@@ -372,7 +372,7 @@ __device__ __forceinline__ Job take_job(const Tail* tail, int m, uint32_t full, 
 // dq: 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256 (float32: the third term of dS
 // at 256, dq at 320; where there is room dS at 256 and dq behind it).  The two groups of four warps have 64 columns each of every row.  The
 // next tile's logits are made as soon as these have been read, so that its exponentials run beside the products dS k and g v^T.
-enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqQFree, kdqS, kdqSRead, kdqDp, kdqDpRead, kdqDs, kdqDsDone, kdqOut, kdqOutRead, kdqFix, kdqJob,
+enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqQFree, kdqS, kdqSRead, kdqDp, kdqDpRead, kdqDs, kdqDsDone, kdqOut, kdqFix, kdqJob,
              kdqJobFree = kdqJob + 2, kDqBars = kdqJobFree + 2 };
 __device__ __forceinline__ Job dq_job(const PackedArgs& a, int index) {
   Job j = {};
@@ -404,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
   if (tid == 0) {
     tail->failed = 0;
-    for (int i = 0; i < kDqBars; ++i) init_bar(bar(i), i == kdqSRead || i == kdqDpRead || i == kdqDs || i == kdqOutRead ? 256 : i >= kdqJobFree ? 8 : 1);
+    for (int i = 0; i < kDqBars; ++i) init_bar(bar(i), i == kdqSRead || i == kdqDpRead || i == kdqDs ? 256 : i >= kdqJobFree ? 8 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   fence_before();
@@ -450,18 +450,17 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
         last_next = ++il == ahead;
         if (last_next) { commit(on, bar(kdqQFree)); ++jl; il = 0; }
       };
-      for (int job = 0;; ++g) {
+      for (;; ++g) {
         if (!G::kShort) logits();
         if (E) dp();
         if (g >= 0) {
           wait_bar(bar(kdqDs), g & 1, failed, &g_packed_error);
-          if (first && job > 0) wait_bar(bar(kdqOutRead), (job - 1) & 1, failed, &g_packed_error);
           fence_after();
           const uint32_t at = tmem + kDs;
           product_cols<M, TERMS, DW>(on, tmem + kOut, E ? Packed{{at, at + 64, at + 128}, {32, 32, 32}} : Packed{{at, at + 32, tmem + 256}, {64, 64, 32}},
                                      slot(2 * g), d, !first);
           if (E) commit(on, bar(kdqDsDone));
-          if (last) { commit(on, bar(kdqOut)); ++job; }
+          if (last) commit(on, bar(kdqOut));
           give(2 * g);
         }
         if (G::kShort) logits();
@@ -474,6 +473,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       int g = 0, job = 0;
       for (int m = 0, index = blockIdx.x;; ++m) {
         const Job j = dq_job(a, index);
+        const int kvh = j.h / a.group;
         publish_job(tail, m, j, bar(kdqJob), bar(kdqJobFree), lane, failed);
         if (__any_sync(0xffffffffu, j.n < 0 || *failed)) break;
         for (int i = 0; i < 2 * j.n; ++i, ++g) {
@@ -489,7 +489,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
           }
           if (g >= R) wait_bar(bar(kdqEmpty + g % R), (g / R - 1) & 1, failed, &g_packed_error);
           const int r = j.k0 + (i >> 1) * kTile;
-          ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, j.h / a.group, bar(kdqFull + g % R), j.lk - r, !(i & 1), failed, &g_packed_error);
+          ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kdqFull + g % R), j.lk - r, !(i & 1), failed, &g_packed_error);
         }
         job += j.n > 0;
         if (lane == 0) index = (int)gridDim.x + atomicAdd(a.queue, 1);
@@ -602,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       };
       if (a.pieces > 1) put(a.share[0] + (long long)j.piece * a.nq * a.hq * d + at_row);
       else put(static_cast<T*>(a.dq) + at_row);
-      if (j.n > 0) { fence_before(); arrive(bar(kdqOutRead)); ++job; }
+      if (j.n > 0) ++job;      // read before the next job's dS are handed over, and only then written again
       j = after;
     }
     fence_before();
@@ -615,7 +615,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
 // logits at 0 (P replaces them), dP at 128 (dS replaces it), dv at 256, dk at 384 (float32: the third terms of P and dS at 256 and 320, dv
 // at 384, dk at 448; up to 64 values a head in 16 bits: P at 256, dS at 320, dv at 384, dk at 448).  The tensor cores work in the order
 // dv(i), logits(i + 1), dk(i), dP(i + 1): each pair runs beside the other half of the elementwise work.
-enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvKFree, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvOutRead, kkvFix, kkvStat, kkvStatFree = kkvStat + 2,
+enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvKFree, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvFix, kkvStat, kkvStatFree = kkvStat + 2,
               kkvSRead = kkvStatFree + 2, kkvDpRead, kkvPDone, kkvDsDone, kkvJob, kkvJobFree = kkvJob + 2, kDkvBars = kkvJobFree + 2 };
 __device__ __forceinline__ Job dkv_job(const PackedArgs& a, int index) {
   Job j = {};
@@ -650,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   if (tid == 0) {
     tail->failed = 0;
     for (int i = 0; i < kDkvBars; ++i)
-      init_bar(bar(i), i == kkvP || i == kkvDs || i == kkvSRead || i == kkvDpRead || i == kkvOutRead ? 256
+      init_bar(bar(i), i == kkvP || i == kkvDs || i == kkvSRead || i == kkvDpRead ? 256
                        : i == kkvStat || i == kkvStat + 1 ? 64 : i == kkvStatFree || i == kkvStatFree + 1 ? 8 : i >= kkvJobFree ? 10 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -694,11 +694,10 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         if (last_next) { commit(on, bar(kkvKFree)); ++jl; il = 0; }
       };
       auto packed_at = [&](uint32_t at, uint32_t third) { return E ? Packed{{at}, {32}} : Packed{{at, at + 32, third}, {64, 64, 32}}; };
-      for (int job = 0;; ++g) {
+      for (;; ++g) {
         if (E) logits();
         if (g >= 0) {
           wait_bar(bar(kkvP), g & 1, failed, &g_packed_error);
-          if (first && job > 0) wait_bar(bar(kkvOutRead), (job - 1) & 1, failed, &g_packed_error);
           fence_after();
           product_cols<M, TERMS, DW>(on, tmem + kDv, packed_at(tmem + kP, tmem + 256), slot(2 * g + 1), d, !first);
           if (E) commit(on, bar(kkvPDone));
@@ -711,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
           fence_after();
           product_cols<M, TERMS, DW>(on, tmem + kDk, packed_at(tmem + kDs, tmem + 320), slot(2 * g), d, !first);
           if (E) commit(on, bar(kkvDsDone));
-          if (last) { commit(on, bar(kkvOut)); ++job; }
+          if (last) commit(on, bar(kkvOut));
           give(2 * g);
         }
         if (G::kShort) logits();
@@ -887,7 +886,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         if (a.pieces > 1) put(a.share[which ? 1 : 2] + (long long)j.piece * a.nkv * a.hk * d + at);
         else put(static_cast<T*>(which ? a.dk : a.dv) + at);
       }
-      if (j.n > 0) { fence_before(); arrive(bar(kkvOutRead)); ++job; }
+      if (j.n > 0) ++job;      // read before the next job's P are handed over, and only then written again
       j = after;
     }
     fence_before();
