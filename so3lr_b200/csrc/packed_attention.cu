@@ -154,18 +154,21 @@ int64_t part_floats(const int32_t* im, const so3lr_b200_attention_shape* a) {
   return (int64_t)im[kNItemsSplit] * a->heads_kv * im[kMaxQ] * (a->heads_q / a->heads_kv) * packed_padded(a->d);
 }
 
-// Batches whose longest structure has this many rows on both sides go to the tensor-core kernels, whose CTAs take 6 us to start and end and
-// whose tiles hold 128 rows.  Forward and backward together in us, tensor cores / warp-level, about 8,200 rows in structures between half
-// and all of the longest, which has L rows:
-//   16-bit, 4 heads x 32:   L = 512  69 / 65,    1,024  81 / 116     float32, 4 x 32:  L = 192  93 / 92,   256 101 / 117
-//   16-bit, 8 x 64:         L = 192 107 / 94,      256 102 / 107     float32, 8 x 64:  L = 96 263 / 245,   128 230 / 255
-//   16-bit, 8 x 128:        L = 96  150 / 155,     128 128 / 161     (float32 above 64 values has warp-level kernels only)
-int tensor_core_rows(int type, int d) {
-  if (type == kF32) return d <= 32 ? 200 : d <= 64 ? 128 : 0x7fffffff;
-  return d <= 32 ? 600 : d <= 64 ? 256 : 100;
+// Batches whose longest structure has this many rows on both sides go to the tensor-core kernels, whose tiles hold 128 rows and whose CTAs
+// take some us to start and end.  Tensor cores / warp-level, us, about 8,200 rows in structures between half and all of the longest, which
+// has L rows (float32 above 64 values has warp-level kernels only):
+//   forward   16-bit, 4 heads x 32:  L = 512 17.9 / 16.4,  640 19.8 / 18.5                  float32, 4 x 32:  192 24.8 / 22.3,  256 26.8 / 26.2
+//             16-bit, 8 x 64:        L = 192 23.0 / 22.3,  224 22.8 / 24.8                   float32, 8 x 64:  192 82 / 79,  224 80 / 92
+//             16-bit, 8 x 128:       L =  64 28.2 / 28.4,   80 30.5 / 40.0
+//   reverse   16-bit, 4 x 32:        L = 320 39 / 37,  384 37 / 40                           float32, 4 x 32:   80 60 / 51,  96 52 / 53
+//             16-bit, 8 x 64:        L =  80 65 / 57,   96 57 / 61                           float32, 8 x 64:   64 210 / 142,  80 177 / 190
+//             16-bit, 8 x 128:       L =  64 109 / 100,  80 96 / 121
+int tensor_core_rows(int type, int d, bool reverse) {
+  if (type == kF32) return d <= 32 ? (reverse ? 96 : 224) : d <= 64 ? (reverse ? 80 : 200) : 0x7fffffff;
+  return d <= 32 ? (reverse ? 360 : 600) : d <= 64 ? (reverse ? 90 : 200) : 72;
 }
-bool on_tensor_cores(const int32_t* im, const so3lr_b200_attention_shape* a) {
-  const int rows = tensor_core_rows(a->type, a->d);
+bool on_tensor_cores(const int32_t* im, const so3lr_b200_attention_shape* a, bool reverse) {
+  const int rows = tensor_core_rows(a->type, a->d, reverse);
   return im[kMaxQ] >= rows && im[kMaxKv] >= rows;
 }
 // Few queries: the heads of a group share one tile of rows with their token, and the keys are cut into stretches.  The keys are then
@@ -189,9 +192,10 @@ int pieces_of(int64_t items, int heads, int64_t walk, int longest, double tile, 
   }
   return at;
 }
-PackedPieces pieces(const int32_t* im, const so3lr_b200_attention_shape* a) {
+// of a forward call, or of its transpose
+PackedPieces pieces(const int32_t* im, const so3lr_b200_attention_shape* a, bool reverse) {
   PackedPieces p;
-  if (!on_tensor_cores(im, a)) {      // 64 x 64 tiles of the warp-level kernels, two CTAs on an SM
+  if (!on_tensor_cores(im, a, reverse)) {      // 64 x 64 tiles of the warp-level kernels, two CTAs on an SM
     const int long_q = (im[kMaxQ] + 63) / 64, long_kv = (im[kMaxKv] + 63) / 64, group = a->heads_q / a->heads_kv;
     const double bytes_q = 4.0 * im[kRowsQ] * a->heads_q * a->d, bytes_kv = 4.0 * im[kRowsKv] * a->heads_kv * a->d;
     const double tile = (a->type == kF32 ? 3.0 : 1.5) * (a->d <= 32 ? 0.4 : a->d <= 64 ? 0.7 : 1.3);
@@ -212,8 +216,8 @@ PackedPieces pieces(const int32_t* im, const so3lr_b200_attention_shape* a) {
   return p;
 }
 int64_t whole_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool reverse) {
-  return (a->type == kF32 && on_tensor_cores(im, a) ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0) +
-         packed_share_bytes(pieces(im, a), a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse);
+  return (a->type == kF32 && on_tensor_cores(im, a, reverse) ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0) +
+         packed_share_bytes(pieces(im, a, reverse), a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse);
 }
 constexpr int64_t kQueueBytes = 16;      // behind these: PackedArgs::queue
 
@@ -228,14 +232,14 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
     p.part_ml = reinterpret_cast<float2*>(p.part_o + part_floats(im, a));
     return packed_forward_split<T>(st, p, im[kNItemsSplit], im[kN], im[kCombine]);
   }
-  if (on_tensor_cores(im, a)) {
+  if (on_tensor_cores(im, a, false)) {
     const bool one = packed_one_tile(a->type == kF32, a->d, im[kMaxKv]);
     p.items = table(im, dev, one ? kItemsQ128 : kItemsQ256);
-    return packed_forward_tc<T>(st, p, im[one ? kNItemsQ128 : kNItemsQ256], pieces(im, a), workspace);
+    return packed_forward_tc<T>(st, p, im[one ? kNItemsQ128 : kNItemsQ256], pieces(im, a, false), workspace);
   }
   const bool small = p.tile_rows == 16;
   p.items = table(im, dev, small ? kItemsQ16 : kItemsQ);
-  p.pieces = pieces(im, a).forward;
+  p.pieces = pieces(im, a, false).forward;
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (int64_t)p.pieces * p.nq * p.hq * p.d);
   const int rc = packed_forward_mma<T>(st, p, im[small ? kNItemsQ16 : kNItemsQ]);
@@ -244,12 +248,12 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
 
 template <typename T>
 int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
-  if (on_tensor_cores(im, a)) p.queue = reinterpret_cast<int*>(static_cast<char*>(workspace) + whole_bytes(im, a, true));
+  if (on_tensor_cores(im, a, true)) p.queue = reinterpret_cast<int*>(static_cast<char*>(workspace) + whole_bytes(im, a, true));
   int rc = packed_delta<T>(st, p, im[kRowsQ]);
   if (rc) return rc;
-  if (on_tensor_cores(im, a))
-    return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128], pieces(im, a), workspace);
-  const PackedPieces n = pieces(im, a);
+  if (on_tensor_cores(im, a, true))
+    return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128], pieces(im, a, true), workspace);
+  const PackedPieces n = pieces(im, a, true);
   const int64_t stride_q = (int64_t)p.nq * p.hq * p.d, stride_kv = (int64_t)p.nkv * p.hk * p.d;
   float* share = static_cast<float*>(workspace);
   if (n.dq > 1) { p.share[0] = share; share += n.dq * stride_q; }
@@ -291,7 +295,7 @@ int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int
 
 int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* a, int vjp) {
   if (!shape_ok(image, a)) return -1;
-  if (vjp) return whole_bytes(image, a, true) + (on_tensor_cores(image, a) ? kQueueBytes : 0);
+  if (vjp) return whole_bytes(image, a, true) + (on_tensor_cores(image, a, true) ? kQueueBytes : 0);
   if (!few_rows(image, a)) return whole_bytes(image, a, false);
   if (!image[kCombine]) return 0;
   return part_floats(image, a) * (int64_t)sizeof(float) + part_floats(image, a) / packed_padded(a->d) * (int64_t)sizeof(float2);
