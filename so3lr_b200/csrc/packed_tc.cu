@@ -8,11 +8,11 @@
 // dS live in tensor memory: P and dS go back there packed to 16 bits, and are the A operand of the next product, so shared memory
 // carries q, k, v and g only.
 //
-// Bound by the tensor cores and the exponentials side by side.  Causal, 16,001 rows in 8 prompts, 40 heads of 128 bfloat16: forward 1.1, dq 1.27,
-// dk and dv 1.40 PFLOP/s of what each multiplies (cuBLAS 1.67), where the tensor cores are busy 58 % and the special function units 58
-// % of the forward kernel's time.  With 64 values a head a tile has half of the products and the same elementwise work (tensor 33 to 40 %
-// busy): what is left is the latency of two warps per scheduler.  The two reverse kernels form seven products where one with atomic sums
-// would form five; they give the same bits every time.
+// Bound by the tensor cores beside the elementwise work of eight warps.  8,192 rows, 9 heads x 128 bfloat16: forward 260 us (1.19 PFLOP/s), dq 386 (1.20),
+// dk and dv 447 (1.38; cuBLAS 1.67), the tensor cores busy 62, 59 and 71 % of the time and the schedulers 40 to 51 %.  With 64 values a head
+// a tile has half of the products, each of them no shorter for its 64 columns, and the same elementwise work (235, 303, 367 us; tensor 32, 36,
+// 40 % busy, schedulers 48 to 55 %): what is left is the latency of two warps per scheduler.  float32, 9 x 32: tensor 54 to 62 %.
+// The two reverse kernels form seven products where one with atomic sums would form five; they give the same bits every time.
 #include "packed_tc.cuh"
 
 #include <algorithm>
