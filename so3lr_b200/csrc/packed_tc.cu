@@ -8,9 +8,9 @@
 // dS live in tensor memory: P and dS go back there packed to 16 bits, and are the A operand of the next product, so shared memory
 // carries q, k, v and g only.
 //
-// Bound by the tensor cores beside the elementwise work of eight warps.  8,192 rows, 9 heads x 128 bfloat16: forward 260 us (1.19 PFLOP/s), dq 386 (1.20),
-// dk and dv 447 (1.38; cuBLAS 1.67), the tensor cores busy 62, 59 and 71 % of the time and the schedulers 40 to 51 %.  With 64 values a head
-// a tile has half of the products, each of them no shorter for its 64 columns, and the same elementwise work (235, 303, 367 us; tensor 32, 36,
+// Bound by the tensor cores beside the elementwise work of eight warps.  8,192 rows, 9 heads x 128 bfloat16: forward 260 us (1.19 PFLOP/s), dq 385 (1.20),
+// dk and dv 444 (1.39; cuBLAS 1.67), the tensor cores busy 62, 59 and 71 % of the time and the schedulers 40 to 51 %.  With 64 values a head
+// a tile has half of the products, each of them no shorter for its 64 columns, and the same elementwise work (235, 306, 366 us; tensor 32, 36,
 // 40 % busy, schedulers 48 to 55 %): what is left is the latency of two warps per scheduler.  float32, 9 x 32: tensor 54 to 62 %.
 // The two reverse kernels form seven products where one with atomic sums would form five; they give the same bits every time.
 #include "packed_tc.cuh"
@@ -350,11 +350,11 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
 
 // ---- reverse --------------------------------------------------------------------------------------------------------
 // A CTA stays on its SM and works through jobs, so that a job's first tiles come in and its first products run while the last results of the
-// one before leave: with a CTA per job its start and end took 5 to 6 us, now 2.4 to 3.5.  dq / dk and dv, a CTA per job -> this, us: 24 structures of 150 to
-// 900 rows, 16 heads x 64, 124 / 147 -> 102 / 129; 64 of 64 to 128, 8 x 128, 28 / 32 -> 21 / 25; 8 causal ones of 2,000, 40 x 128, 613 / 588 ->
-// 549 / 594; one of 8,192, 9 x 64, 290 / 351 -> 303 / 366 (a job of 64 tiles has no start to hide).  The loading warp takes jobs from a queue, the
+// one before leave: with a CTA per job its start and end took 5 to 6 us, now 2 to 3.  dq / dk and dv, a CTA per job -> this, us: 24 structures of 150 to
+// 900 rows, 16 heads x 64, 124 / 147 -> 100 / 121; 64 of 64 to 128, 8 x 128, 28 / 32 -> 20 / 26; 8 causal ones of 2,000, 40 x 128, 613 / 588 ->
+// 520 / 592; one of 8,192, 9 x 64, 290 / 351 -> 306 / 366 (a job of 64 tiles has no start to hide).  The loading warp takes jobs from a queue, the
 // longest first, and passes them on through shared memory (equal shares instead: SMs differ in their pace by up to 15 %; 5,000 rows, 4 x 32
-// float32, dk and dv 184 us with the queue, 219 without).
+// float32, dk and dv 187 us with the queue, 219 without).
 __device__ __forceinline__ void publish_job(Tail* tail, int m, const Job& j, uint32_t full, uint32_t free, int lane, volatile int* failed) {
   if (m >= 2) wait_bar(free + 8 * (m & 1), ((m >> 1) - 1) & 1, failed, &g_packed_error);
   if (lane == 0) { tail->jobs[m & 1] = j; arrive(full + 8 * (m & 1)); }
@@ -422,51 +422,49 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
       auto ready = [&](int j) { wait_bar(bar(kdqFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
       auto give = [&](int j) { commit(on, bar(kdqEmpty + j % R)); };
-      // Logits and dP run a tile ahead: tile g + 1 of all, the il-th of `ahead` of job jl.  The loop is as short as it can be (the loading warp says
-      // how many tiles a job has, every product stands in one place, so the walk starts a step early), and addresses come from g, which is
-      // the same in all lanes as the compiler sees it: what this warp does between two instructions keeps the tensor cores waiting.
-      int g = -1, il = 0, jl = 0, ahead = 0;
-      bool done = false, first = false, last = false, first_next = false, last_next = false;      // of tile g and of the next one
-      auto logits = [&] {
-        first_next = il == 0;
-        if (first_next) {
-          wait_bar(bar(kdqQ), jl & 1, failed, &g_packed_error);
-          ahead = __shfl_sync(0xffffffffu, *failed ? 0 : tail->tiles[jl & 1], 0);
-          done = ahead == 0;
+      // Logits and dP run a tile ahead: tile g + 1 of all, tile i + 1 of the job's n.  The loop is as short as it can be (the loading warp says how
+      // many tiles a job has, every product stands in one place, so that a job starts a step early): what this warp does between two
+      // instructions keeps the tensor cores waiting.  It waits for a job only behind the last product of the one before, without which the
+      // compute warps do not get to the jobs in between that have no tiles.
+      int g = -1;
+      for (int job = 0;; ++job) {
+        wait_bar(bar(kdqQ), job & 1, failed, &g_packed_error);
+        const int n = __shfl_sync(0xffffffffu, *failed ? 0 : tail->tiles[job & 1], 0);
+        if (n == 0) break;
+        for (int i = -1; i < n; ++i) {
+          const bool more = i + 1 < n;
+          auto logits = [&] {
+            if (!more) return;
+            ready(2 * g + 2);
+            if (g >= 0) { wait_bar(bar(kdqSRead), g & 1, failed, &g_packed_error); fence_after(); }
+            product_rows<M, TERMS, DW>(on, tmem, sq, slot(2 * g + 2), d);
+            commit(on, bar(kdqS));
+          };
+          auto dp = [&] {
+            if (!more) return;
+            ready(2 * g + 3);
+            if (E && g >= 0) { wait_bar(bar(kdqDpRead), g & 1, failed, &g_packed_error); fence_after(); }
+            product_rows<M, TERMS, DW>(on, tmem + kTile, sg, slot(2 * g + 3), d);
+            commit(on, bar(kdqDp));
+            give(2 * g + 3);
+            if (i + 2 == n) commit(on, bar(kdqQFree));
+          };
+          if (!G::kShort) logits();
+          if (E) dp();
+          if (i >= 0) {
+            wait_bar(bar(kdqDs), g & 1, failed, &g_packed_error);
+            fence_after();
+            const uint32_t at = tmem + kDs;
+            product_cols<M, TERMS, DW>(on, tmem + kOut, E ? Packed{{at, at + 64, at + 128}, {32, 32, 32}} : Packed{{at, at + 32, tmem + 256}, {64, 64, 32}},
+                                       slot(2 * g), d, i > 0);
+            if (E) commit(on, bar(kdqDsDone));
+            if (!more) commit(on, bar(kdqOut));
+            give(2 * g);
+          }
+          if (G::kShort) logits();
+          if (!E) dp();
+          if (more) ++g;
         }
-        if (done) return;
-        ready(2 * g + 2);
-        if (g >= 0) { wait_bar(bar(kdqSRead), g & 1, failed, &g_packed_error); fence_after(); }
-        product_rows<M, TERMS, DW>(on, tmem, sq, slot(2 * g + 2), d);
-        commit(on, bar(kdqS));
-      };
-      auto dp = [&] {
-        if (done) return;
-        ready(2 * g + 3);
-        if (E && g >= 0) { wait_bar(bar(kdqDpRead), g & 1, failed, &g_packed_error); fence_after(); }
-        product_rows<M, TERMS, DW>(on, tmem + kTile, sg, slot(2 * g + 3), d);
-        commit(on, bar(kdqDp));
-        give(2 * g + 3);
-        last_next = ++il == ahead;
-        if (last_next) { commit(on, bar(kdqQFree)); ++jl; il = 0; }
-      };
-      for (;; ++g) {
-        if (!G::kShort) logits();
-        if (E) dp();
-        if (g >= 0) {
-          wait_bar(bar(kdqDs), g & 1, failed, &g_packed_error);
-          fence_after();
-          const uint32_t at = tmem + kDs;
-          product_cols<M, TERMS, DW>(on, tmem + kOut, E ? Packed{{at, at + 64, at + 128}, {32, 32, 32}} : Packed{{at, at + 32, tmem + 256}, {64, 64, 32}},
-                                     slot(2 * g), d, !first);
-          if (E) commit(on, bar(kdqDsDone));
-          if (last) commit(on, bar(kdqOut));
-          give(2 * g);
-        }
-        if (G::kShort) logits();
-        if (!E) dp();
-        if (done) break;
-        first = first_next; last = last_next;
       }
     } else if (warp == kLoadWarp) {
       Loader<TERMS, DW> ld{lane, bar(kdqFix)};
@@ -669,54 +667,51 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
       auto ready = [&](int j) { wait_bar(bar(kkvFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
       auto give = [&](int j) { commit(on, bar(kkvEmpty + j % R)); };
-      int g = -1, il = 0, jl = 0, ahead = 0;
-      bool done = false, first = false, last = false, first_next = false, last_next = false;      // of tile g and of the next one
-      auto logits = [&] {
-        first_next = il == 0;
-        if (first_next) {
-          wait_bar(bar(kkvK), jl & 1, failed, &g_packed_error);
-          ahead = __shfl_sync(0xffffffffu, *failed ? 0 : tail->tiles[jl & 1], 0);
-          done = ahead == 0;
-        }
-        if (done) return;
-        ready(2 * g + 2);
-        if (E && g >= 0) { wait_bar(bar(kkvSRead), g & 1, failed, &g_packed_error); fence_after(); }
-        product_rows<M, TERMS, DW>(on, tmem, sk, slot(2 * g + 2), d);
-        commit(on, bar(kkvS));
-      };
-      auto dp = [&] {
-        if (done) return;
-        ready(2 * g + 3);
-        if (E && g >= 0) { wait_bar(bar(kkvDpRead), g & 1, failed, &g_packed_error); fence_after(); }
-        product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(2 * g + 3), d);
-        commit(on, bar(kkvDp));
-        last_next = ++il == ahead;
-        if (last_next) { commit(on, bar(kkvKFree)); ++jl; il = 0; }
-      };
       auto packed_at = [&](uint32_t at, uint32_t third) { return E ? Packed{{at}, {32}} : Packed{{at, at + 32, third}, {64, 64, 32}}; };
-      for (;; ++g) {
-        if (E) logits();
-        if (g >= 0) {
-          wait_bar(bar(kkvP), g & 1, failed, &g_packed_error);
-          fence_after();
-          product_cols<M, TERMS, DW>(on, tmem + kDv, packed_at(tmem + kP, tmem + 256), slot(2 * g + 1), d, !first);
-          if (E) commit(on, bar(kkvPDone));
-          give(2 * g + 1);
+      int g = -1;
+      for (int job = 0;; ++job) {
+        wait_bar(bar(kkvK), job & 1, failed, &g_packed_error);
+        const int n = __shfl_sync(0xffffffffu, *failed ? 0 : tail->tiles[job & 1], 0);
+        if (n == 0) break;
+        for (int i = -1; i < n; ++i) {
+          const bool more = i + 1 < n;
+          auto logits = [&] {
+            if (!more) return;
+            ready(2 * g + 2);
+            if (E && g >= 0) { wait_bar(bar(kkvSRead), g & 1, failed, &g_packed_error); fence_after(); }
+            product_rows<M, TERMS, DW>(on, tmem, sk, slot(2 * g + 2), d);
+            commit(on, bar(kkvS));
+          };
+          auto dp = [&] {
+            if (!more) return;
+            ready(2 * g + 3);
+            if (E && g >= 0) { wait_bar(bar(kkvDpRead), g & 1, failed, &g_packed_error); fence_after(); }
+            product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(2 * g + 3), d);
+            commit(on, bar(kkvDp));
+            if (i + 2 == n) commit(on, bar(kkvKFree));
+          };
+          if (E) logits();
+          if (i >= 0) {
+            wait_bar(bar(kkvP), g & 1, failed, &g_packed_error);
+            fence_after();
+            product_cols<M, TERMS, DW>(on, tmem + kDv, packed_at(tmem + kP, tmem + 256), slot(2 * g + 1), d, i > 0);
+            if (E) commit(on, bar(kkvPDone));
+            give(2 * g + 1);
+          }
+          if (!E && !G::kShort) logits();
+          if (E) dp();
+          if (i >= 0) {
+            wait_bar(bar(kkvDs), g & 1, failed, &g_packed_error);
+            fence_after();
+            product_cols<M, TERMS, DW>(on, tmem + kDk, packed_at(tmem + kDs, tmem + 320), slot(2 * g), d, i > 0);
+            if (E) commit(on, bar(kkvDsDone));
+            if (!more) commit(on, bar(kkvOut));
+            give(2 * g);
+          }
+          if (G::kShort) logits();
+          if (!E) dp();
+          if (more) ++g;
         }
-        if (!E && !G::kShort) logits();
-        if (E) dp();
-        if (g >= 0) {
-          wait_bar(bar(kkvDs), g & 1, failed, &g_packed_error);
-          fence_after();
-          product_cols<M, TERMS, DW>(on, tmem + kDk, packed_at(tmem + kDs, tmem + 320), slot(2 * g), d, !first);
-          if (E) commit(on, bar(kkvDsDone));
-          if (last) commit(on, bar(kkvOut));
-          give(2 * g);
-        }
-        if (G::kShort) logits();
-        if (!E) dp();
-        if (done) break;
-        first = first_next; last = last_next;
       }
     } else if (warp == kLoadWarp) {
       Loader<TERMS, DW> ld{lane, bar(kkvFix)};

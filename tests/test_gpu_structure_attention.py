@@ -485,3 +485,48 @@ def test_more_rows_than_an_index_holds_are_refused():
             structure_attention(q, k, k, packed)
     with pytest.raises(ValueError, match="rows"):
         norm_rotate(many, None, torch.zeros(1, 1, device="cuda").expand(2 ** 31, 1), torch.zeros(1, 8, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("hq,hk,d,causal,seed", [(16, 16, 32, False, 0), (12, 4, 64, True, 1), (14, 7, 128, True, 2), (16, 1, 48, False, 3)])
+def test_more_items_than_the_chip_takes_at_once(hq, hk, d, causal, seed, dtype):
+    # lengths of both sides from none to 500, in any order: every CTA works on many items, some of them without any row of the other side
+    rng = np.random.default_rng(seed)
+    lq, lk = (np.where(rng.random(30) < 0.15, 0, rng.integers(1, 500, 30)).tolist() for _ in range(2))
+    q, k, v, g = inputs(lq, lk, hq, hk, d, TYPES[dtype], seed=seed, extra=3)
+    packed = PackedStructures(starts(lq), starts(lk), causal=causal)
+    val, err = reference(q, k, v, g, lq, lk, causal, d ** -0.5, q.dtype)
+    got = train(q, k, v, g, packed)
+    within(got, val, err)
+    # beside another call of the same kind, and replayed: the same bits
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        beside = train(q, k, v, g, packed)
+    again = train(q, k, v, g, packed)
+    torch.cuda.synchronize()
+    for x, y, z in zip(got, again, beside):
+        assert torch.equal(x, y) and torch.equal(x, z)
+    no_wait_ran_out()
+
+
+def no_wait_ran_out():
+    import ctypes
+
+    from so3lr_b200._lib import check, lib
+    word = ctypes.c_int(-1)
+    check(lib.so3lr_b200_structure_attention_error(ctypes.byref(word)), "structure_attention_error")
+    assert word.value == 0
+
+
+@pytest.mark.parametrize("dtype,d", [("f32", 32), ("f32", 64), ("bf16", 64), ("f16", 128)])
+@pytest.mark.parametrize("side", ["queries", "keys"])
+def test_long_runs_of_items_that_meet_nothing(side, dtype, d):
+    # hundreds of structures without any key (any query) beside two that have both
+    full, none = [131] * 401, [0] * 200 + [250] + [0] * 199 + [140]
+    lq, lk = (full, none) if side == "queries" else (none, full)
+    q, k, v, g = inputs(lq, lk, 8, 4, d, TYPES[dtype], seed=11)
+    packed = PackedStructures(starts(lq), starts(lk))
+    val, err = reference(q, k, v, g, lq, lk, False, d ** -0.5, q.dtype)
+    within(train(q, k, v, g, packed), val, err)
+    no_wait_ran_out()
