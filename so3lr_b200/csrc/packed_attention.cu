@@ -235,6 +235,7 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
   if (on_tensor_cores(im, a, false)) {
     const bool one = packed_one_tile(a->type == kF32, a->d, im[kMaxKv]);
     p.items = table(im, dev, one ? kItemsQ128 : kItemsQ256);
+    p.queue = reinterpret_cast<int*>(static_cast<char*>(workspace) + whole_bytes(im, a, false));
     return packed_forward_tc<T>(st, p, im[one ? kNItemsQ128 : kNItemsQ256], pieces(im, a, false), workspace);
   }
   const bool small = p.tile_rows == 16;
@@ -295,8 +296,7 @@ int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int
 
 int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* a, int vjp) {
   if (!shape_ok(image, a)) return -1;
-  if (vjp) return whole_bytes(image, a, true) + (on_tensor_cores(image, a, true) ? kQueueBytes : 0);
-  if (!few_rows(image, a)) return whole_bytes(image, a, false);
+  if (vjp || !few_rows(image, a)) return whole_bytes(image, a, vjp) + (on_tensor_cores(image, a, vjp) ? kQueueBytes : 0);
   if (!image[kCombine]) return 0;
   return part_floats(image, a) * (int64_t)sizeof(float) + part_floats(image, a) / packed_padded(a->d) * (int64_t)sizeof(float2);
 }

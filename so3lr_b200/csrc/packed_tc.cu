@@ -27,19 +27,20 @@ using namespace tc;
 
 // barriers and scratch behind the tiles
 constexpr int kBars = 40;
-// What a CTA of a reverse kernel works on at a time: a tile of rows from row0 on of one head (or key head) h against n tiles of the other side, a
+// What a CTA works on at a time: a tile of rows from row0 on of one head (or key head) h against n tiles of the other side, a
 // piece of an item's walk.  n < 0: there is no more.
 struct Job {
   int q0, lq, c0, lk, h, row0, n, piece;
-  int k0;               // dq: first key
+  int k0;               // forward, dq: first key
+  int n0, n1;           // forward: tiles of keys that the two tiles of rows meet (n is the larger count)
   int i0, per, j0;      // dk and dv: first query; tiles of queries of a head from there on; the job's first one among those of all heads of the group
 };
 struct Tail {
   unsigned long long bars[kBars];
   uint32_t tmem;
   int failed;
-  Job jobs[2];       // reverse kernels: the jobs at hand
-  int tiles[2];      // and tiles of those that have any, 0 behind the last one
+  Job jobs[2];       // the jobs at hand
+  int tiles[2];      // reverse kernels: tiles of those that have any, 0 behind the last one
 };
 template <typename T, int TERMS> struct Operand { using type = T; };
 template <> struct Operand<float, 3> { using type = __nv_bfloat16; };
@@ -76,279 +77,7 @@ template <int DW, int W> __device__ __forceinline__ void add_cols(uint32_t at, f
 // sub-tiles need 1024-byte alignment
 __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* p) { return p + ((1024u - (smem_addr(p) & 1023u)) & 1023u); }
 
-// ---- forward --------------------------------------------------------------------------------------------------------
-// 256 queries of one head: two tiles of 128 rows take turns, so that the exponentials of one run beside the products of the other.
-// Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t; P of a tile replaces its logits.  (Up to 64 values a head: output at
-// 256 + 64 t, P at 384 + 64 t; one tile: logits at 0, output at 128, P at 192.  float32: logits at 256 t, the three terms of P from there on, its output at 256 t + 192.)
-// The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
-// the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
-enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kSFull = kQFull + 2, kPFull = kSFull + 2 /* tile + 2 half */, kOFull = kPFull + 4, kFix = kOFull + 2,
-              kSRead, kFwdBars = kSRead + 2 };
-
-// TILES = 1: a CTA has one tile and half of an SM, which two of them share: one's start and end pass beside the other's work.
-template <int TERMS, int DW, int TILES> struct Forward {
-  static constexpr int kMma = 4 * TILES, kLoad = kMma + 1, kThreads = 128 * TILES + 128;
-  // registers: 256 x 208 + 128 x 88 = 384 x 168; 128 x 200 + 128 x 56 = 256 x 128
-  static constexpr int kRegs = TILES == 2 ? 208 : 200, kOtherRegs = TILES == 2 ? 88 : 56;
-  static constexpr int kRing = TILES == 2 ? Geometry<TERMS, DW>::kRing : TERMS == 3 ? 3 : DW == 128 ? 2 : 4;
-  static constexpr int kSmem = 1024 + (TILES + kRing) * Geometry<TERMS, DW>::kSubs * (int)Geometry<TERMS, DW>::kSub + (int)sizeof(Tail);
-  static_assert(TILES == 2 || kSmem <= 232448 / 2, "two CTAs on an SM");
-};
-template <typename T, int TERMS, int DW, int TILES>
-__global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 2 ? 1 : 2) forward_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
-  using M = typename Operand<T, TERMS>::type;
-  using G = Geometry<TERMS, DW>;
-  using F = Forward<TERMS, DW, TILES>;
-  constexpr int kMmaWarp = F::kMma, kLoadWarp = F::kLoad;
-  extern __shared__ unsigned char raw[];
-  unsigned char* smem = aligned_smem(raw);
-  const int d = a.d;
-  constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = F::kRing;
-  Tail* tail = reinterpret_cast<Tail*>(smem + (TILES + R) * tile_bytes);
-  const uint32_t sq = smem_addr(smem), ring = sq + TILES * tile_bytes, bar0 = smem_addr(tail->bars);
-  volatile int* failed = &tail->failed;
-  auto bar = [&](int k) { return bar0 + 8 * k; };
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int unit = blockIdx.x / a.pieces, piece = blockIdx.x % a.pieces;
-  const int4 item = a.items[unit / a.hq];
-  const int s = item.x, q0 = a.start_q[s], lq = a.start_q[s + 1] - q0, c0 = a.start_kv[s], lk = a.start_kv[s + 1] - c0;
-  const int h = unit % a.hq, kvh = h / a.group, row0 = item.y * TILES * kTile, off = lk - lq;
-  // keys that a tile meets: [0, end[t]), and tiles of keys
-  const int end1 = item.w, end0 = TILES == 2 && a.causal ? min(end1, max(0, min(lq, row0 + kTile) + off)) : end1;
-  const int all0 = (end0 + kTile - 1) / kTile, all1 = TILES == 2 && row0 + kTile < lq ? (end1 + kTile - 1) / kTile : 0, per = (max(all0, all1) + a.pieces - 1) / a.pieces;
-  // this piece's: tiles from k0 / 128 on
-  const int k0 = piece * per * kTile, n0 = min(per, max(0, all0 - piece * per)), n1 = min(per, max(0, all1 - piece * per)), n = max(n0, n1);
-  if (warp == kMmaWarp) alloc_tmem(&tail->tmem, 256 * TILES);
-  if (tid == 0) {
-    tail->failed = 0;
-    for (int i = 0; i < kFwdBars; ++i) init_bar(bar(i), (i >= kPFull && i < kPFull + 4) || i >= kSRead ? kTile : 1);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  }
-  fence_before();
-  __syncthreads();
-  fence_after();
-  const uint32_t tmem = tail->tmem;
-  // columns from one tile's logits to the other's, output of a tile, columns from one output to the other, P
-  constexpr uint32_t kStride = TERMS == 1 ? kTile : 256, kOut = TERMS == 1 ? kTile * TILES : 192, kOutStride = TERMS == 1 ? DW : 256;
-  auto p_at = [](int t) { return G::kEarly ? kOut + 64 * TILES + 64 * t : kStride * t; };
-
-  if (warp >= kMmaWarp) {
-    fewer_regs<F::kOtherRegs>();
-    if (warp == kMmaWarp && n > 0) {
-      const uint32_t on = elect_one();
-      // keys are tiles 0, 2, .. of the ring, values 1, 3, ..; a slot is given back only where another tile waits for it, so that nothing is
-      // pending when the CTA ends
-      auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
-      auto ready = [&](int j) { wait_bar(bar(kFull + j % R), (j / R) & 1, failed, &g_packed_error); };
-      auto give = [&](int j) { if (j + R < 2 * n) commit(on, bar(kEmpty + j % R)); };
-      ready(0);
-#pragma unroll
-      for (int t = 0; t < TILES; ++t) {
-        if ((t ? n1 : n0) == 0) continue;
-        wait_bar(bar(kQFull + t), 0, failed, &g_packed_error);
-        fence_after();
-        product_rows<M, TERMS, DW>(on, tmem + kStride * t, sq + t * tile_bytes, slot(0), d);
-        commit(on, bar(kSFull + t));
-      }
-      give(0);
-      for (int i = 0; i < n; ++i) {
-        auto logits = [&](int t) {
-          if (i + 1 >= (t ? n1 : n0)) return;
-          product_rows<M, TERMS, DW>(on, tmem + kStride * t, sq + t * tile_bytes, slot(2 * i + 2), d);
-          commit(on, bar(kSFull + t));
-        };
-        if (i + 1 < n) ready(2 * i + 2);
-        if (G::kEarly) {
-#pragma unroll
-          for (int t = 0; t < TILES; ++t) {
-            if (i + 1 >= (t ? n1 : n0)) continue;
-            wait_bar(bar(kSRead + t), i & 1, failed, &g_packed_error);
-            fence_after();
-            logits(t);
-          }
-          if (i + 1 < n) give(2 * i + 2);
-        }
-        ready(2 * i + 1);
-#pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-          const int nt = t ? n1 : n0;
-          if (i >= nt) continue;
-          wait_bar(bar(kPFull + t), i & 1, failed, &g_packed_error);
-          fence_after();
-          const uint32_t at = tmem + p_at(t), out = tmem + kOut + kOutStride * t;
-          const Packed p{{at, at + 64, at + 128}, {32, 32, 32}};
-          if constexpr (TERMS == 1) {      // the first half of the keys while the exponentials of the second are formed
-            product_cols<M, TERMS, DW, 0, 4>(on, out, p, slot(2 * i + 1), d, i > 0);
-            wait_bar(bar(kPFull + 2 + t), i & 1, failed, &g_packed_error);
-            fence_after();
-            product_cols<M, TERMS, DW, 4, 8>(on, out, p, slot(2 * i + 1), d, 1);
-          } else {
-            product_cols<M, TERMS, DW>(on, out, p, slot(2 * i + 1), d, 0);
-          }
-          if (!G::kEarly) logits(t);
-          if (G::kEarly || i + 1 == nt) commit(on, bar(kOFull + t));
-        }
-        give(2 * i + 1);
-        if (!G::kEarly && i + 1 < n) give(2 * i + 2);
-      }
-    } else if (warp == kLoadWarp && n > 0) {
-      Loader<TERMS, DW> ld{lane, bar(kFix)};
-      for (int t = 0; t < TILES; ++t)
-        if ((t ? n1 : n0) > 0) ld.tile(sq + t * tile_bytes, &maps.q, q0 + row0 + t * kTile, h, bar(kQFull + t), kTile, false, failed, &g_packed_error);
-      for (int j = 0; j < 2 * n; ++j) {
-        if (j >= R) wait_bar(bar(kEmpty + j % R), (j / R - 1) & 1, failed, &g_packed_error);
-        const int r = k0 + (j >> 1) * kTile;
-        ld.tile(ring + (j % R) * tile_bytes, (j & 1) ? &maps.v : &maps.k, c0 + r, kvh, bar(kFull + j % R), lk - r, j & 1, failed, &g_packed_error);
-      }
-    }
-  } else {
-    more_regs<F::kRegs>();
-    const int t = warp >> 2, w = warp & 3, nt = t ? n1 : n0;
-    const int row = row0 + t * kTile + w * 32 + lane, first = row0 + t * kTile + w * 32;
-    const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16), ts = lanes + kStride * t, to = lanes + kOut + kOutStride * t;
-    constexpr int kOwn = TERMS == 1 ? 1 : DW;
-    float own[kOwn];                         // the output so far (float32)
-#pragma unroll
-    for (int c = 0; c < kOwn; ++c) own[c] = 0.f;
-    // last key that this row sees, and that the warp's first row sees
-    const int lim = min(a.causal ? row + off : lk - 1, lk - 1), lim_first = min(a.causal ? first + off : lk - 1, lk - 1);
-    float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < nt; ++i) {
-      wait_bar(bar(kSFull + t), i & 1, failed, &g_packed_error);
-      fence_after();
-      if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW>(to, own); }
-      uint32_t x[kTile];
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) ld32(ts + c, x + c);
-      wait_ld(x);
-      if (G::kEarly) { fence_before(); arrive(bar(kSRead + t)); }
-      const int kb = k0 + i * kTile;
-      const bool masked = kb + kTile - 1 > lim_first;
-      if (masked) {
-#pragma unroll
-        for (int c = 0; c < kTile; ++c) if (kb + c > lim) x[c] = 0xff800000u;
-      }
-      float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int c = 0; c < kTile; c += 8) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
-      }
-      const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2);
-      const bool raise = mn > m + 8.f;      // true where there was none yet
-      if (G::kEarly && i > 0) { wait_bar(bar(kOFull + t), (i - 1) & 1, failed, &g_packed_error); fence_after(); }      // the output and P are free
-      if (__any_sync(0xffffffffu, raise)) {
-        const float f = raise ? pow2(m - mn) : 1.f;
-        if (raise) m = mn;
-        l *= f;
-        if constexpr (TERMS == 3) {
-#pragma unroll
-          for (int c = 0; c < kOwn; ++c) own[c] *= f;
-        } else if (i > 0) {
-          for (int c = 0; c < d; c += 16) {
-            uint32_t o[16];
-            ld16(to + c, o);
-            wait_ld(o);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            st16(to + c, o);
-          }
-        }
-      }
-      const float u = m == -INFINITY ? 0.f : -m;
-      float2 sums[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) sums[e] = make_float2(0.f, 0.f);
-      const Packed at{{p_at(t), p_at(t) + 64, p_at(t) + 128}, {}};
-      const float2 scale = make_float2(a.scale_log2, a.scale_log2), ref = make_float2(u, u);
-#pragma unroll
-      for (int c = 0; c < kTile; c += 32) {
-        float y[32];
-        // a masked logit has to give zero, which the polynomial does not
-        if (TERMS == 1 && !masked) { pow2_16<true>(x + c, scale, ref, y); pow2_16<true>(x + c + 16, scale, ref, y + 16); }
-        else { pow2_16<false>(x + c, scale, ref, y); pow2_16<false>(x + c + 16, scale, ref, y + 16); }
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) sums[(e >> 1) & 3] = __fadd2_rn(sums[(e >> 1) & 3], make_float2(y[e], y[e + 1]));
-        put16<M, TERMS>(at, lanes, c, y);
-        put16<M, TERMS>(at, lanes, c + 16, y + 16);
-        if (TERMS == 1 && c == kTile / 2 - 32) {
-          wait_st();
-          fence_before();
-          arrive(bar(kPFull + t));
-        }
-      }
-      const float2 sum = __fadd2_rn(__fadd2_rn(sums[0], sums[1]), __fadd2_rn(sums[2], sums[3]));
-      l += sum.x + sum.y;
-      wait_st();
-      fence_before();
-      arrive(bar(kPFull + t + (TERMS == 1 ? 2 : 0)));
-    }
-    if (nt > 0) {
-      wait_bar(bar(kOFull + t), G::kEarly ? (nt - 1) & 1 : 0, failed, &g_packed_error);
-      fence_after();
-    }
-    if constexpr (TERMS == 3) { if (nt > 0) add_cols<DW, DW>(to, own); }
-    const bool there = row < lq, bad = *failed;
-    if (a.pieces > 1) {      // the share: o as it is, with its maximum and sum
-      const long long slot = ((long long)piece * a.hq + h) * a.nq + q0 + row;
-      if (there) a.part_ml[slot] = make_float2(m, bad ? NAN : l);
-      float* dst = a.part_o + slot * d;
-      if (nt > 0) {
-        if constexpr (TERMS == 3) {
-#pragma unroll
-          for (int c = 0; c < DW; c += 16) if (there && c < d) store16(dst + c, own + c);
-        } else {
-          for (int c = 0; c < d; c += 16) {
-            uint32_t o[16];
-            float y[16];
-            ld16(to + c, o);
-            wait_ld(o);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) y[k] = __uint_as_float(o[k]);
-            if (there) store16(dst + c, y);
-          }
-        }
-      }
-    } else {
-      const float inv = bad ? NAN : l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-      const long long at = ((long long)(q0 + row) * a.hq + h) * d;
-      T *dst = static_cast<T*>(a.out) + at, *rest = a.out_rest ? static_cast<T*>(a.out_rest) + at : nullptr;
-      if constexpr (TERMS == 3) {
-#pragma unroll
-        for (int c = 0; c < kOwn; ++c) own[c] *= inv;
-#pragma unroll
-        for (int c = 0; c < DW; c += 16) if (there && c < d) store16(dst + c, own + c);
-      } else {
-        for (int c = 0; c < d; c += 16) {
-          uint32_t o[16];
-          float y[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e) o[e] = 0;
-          if (nt > 0) { ld16(to + c, o); wait_ld(o); }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(o[e]) * inv;
-          if (there) {
-            store16(dst + c, y);
-            if (rest) {
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                const float2 r = packed::Half<T>::unpack(packed::Half<T>::pack(y[e], y[e + 1]));
-                y[e] -= r.x; y[e + 1] -= r.y;
-              }
-              store16(rest + c, y);
-            }
-          }
-        }
-      }
-      if (there && a.lse) a.lse[(long long)h * a.nq + q0 + row] = bad ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
-    }
-    fence_before();
-  }
-  __syncthreads();
-  if (warp == kMmaWarp) { fence_after(); free_tmem(tmem, 256 * TILES); }
-}
-
-// ---- reverse --------------------------------------------------------------------------------------------------------
+// ---- jobs -----------------------------------------------------------------------------------------------------------
 // A CTA stays on its SM and works through jobs, so that a job's first tiles come in and its first products run while the last results of the
 // one before leave: with a CTA per job its start and end took 5 to 6 us, now 2 to 3.  dq / dk and dv, a CTA per job -> this, us: 24 structures of 150 to
 // 900 rows, 16 heads x 64, 124 / 147 -> 100 / 121; 64 of 64 to 128, 8 x 128, 28 / 32 -> 20 / 26; 8 causal ones of 2,000, 40 x 128, 613 / 588 ->
@@ -369,6 +98,338 @@ __device__ __forceinline__ Job take_job(const Tail* tail, int m, uint32_t full, 
   return j;
 }
 
+// ---- forward --------------------------------------------------------------------------------------------------------
+// 256 queries of one head: two tiles of 128 rows take turns, so that the exponentials of one run beside the products of the other.
+// Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t; P of a tile replaces its logits.  (Up to 64 values a head: output at
+// 256 + 64 t, P at 384 + 64 t; one tile: logits at 0, output at 128, P at 192.  float32: logits at 256 t, the three terms of P from there on, its output at 256 t + 192.)
+// The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
+// the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
+enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kQFree = kQFull + 2, kSFull = kQFree + 2, kPFull = kSFull + 2 /* tile + 2 half */, kOFull = kPFull + 4,
+              kFix = kOFull + 2, kSRead, kJob = kSRead + 2, kJobFree = kJob + 2, kFwdBars = kJobFree + 2 };
+template <int TILES> __device__ __forceinline__ Job forward_job(const PackedArgs& a, int index) {
+  Job j = {};
+  j.n = -1;
+  if (index >= a.jobs) return j;
+  const int unit = index / a.pieces;
+  const int4 item = __ldg(a.items + unit / a.hq);
+  j.piece = index % a.pieces; j.h = unit % a.hq;
+  j.q0 = __ldg(a.start_q + item.x); j.lq = __ldg(a.start_q + item.x + 1) - j.q0; j.c0 = __ldg(a.start_kv + item.x); j.lk = __ldg(a.start_kv + item.x + 1) - j.c0;
+  j.row0 = item.y * TILES * kTile;
+  // keys that a tile of rows meets: [0, end), and tiles of keys
+  const int end1 = item.w, end0 = TILES == 2 && a.causal ? min(end1, max(0, min(j.lq, j.row0 + kTile) + j.lk - j.lq)) : end1;
+  const int all0 = (end0 + kTile - 1) / kTile, all1 = TILES == 2 && j.row0 + kTile < j.lq ? (end1 + kTile - 1) / kTile : 0;
+  const int all = max(all0, all1), share = all / a.pieces, more = all % a.pieces, first = j.piece * share + min(j.piece, more);
+  j.n = share + (j.piece < more); j.k0 = first * kTile;
+  j.n0 = min(j.n, max(0, all0 - first)); j.n1 = min(j.n, max(0, all1 - first));
+  return j;
+}
+
+// TILES = 1: a CTA has one tile and half of an SM, which two of them share: one's start and end pass beside the other's work.
+template <int TERMS, int DW, int TILES> struct Forward {
+  static constexpr int kMma = 4 * TILES, kLoad = kMma + 1, kThreads = 128 * TILES + 128;
+  // registers: 256 x 208 + 128 x 88 = 384 x 168; 128 x 200 + 128 x 56 = 256 x 128
+  static constexpr int kRegs = TILES == 2 ? 208 : 200, kOtherRegs = TILES == 2 ? 88 : 56;
+  static constexpr int kRing = TILES == 2 ? Geometry<TERMS, DW>::kRing : TERMS == 3 ? 3 : DW == 128 ? 2 : 4;
+  static constexpr int kSmem = 1024 + (TILES + kRing) * Geometry<TERMS, DW>::kSubs * (int)Geometry<TERMS, DW>::kSub + (int)sizeof(Tail);
+  static_assert(TILES == 2 || kSmem <= 232448 / 2, "two CTAs on an SM");
+  // Whether CTAs take jobs from a queue, or have one each.  us, one / queue: 8 causal prompts of 2,000, 40 heads x 128, 482 / 431; 24 structures of 150 to
+  // 900, 16 x 64, 94 / 87; one of 8,192, 9 x 64, 236 / 247; but float32, whose registers spill over what a job takes, 32 of 256, 4 x 32, 15.3 /
+  // 17.1, one of 5,000 100 / 117.
+  static constexpr bool kQueued = TERMS == 1;
+};
+template <typename T, int TERMS, int DW, int TILES>
+__global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 2 ? 1 : 2) forward_kernel(const PackedArgs a, const __grid_constant__ Maps maps) {
+  using M = typename Operand<T, TERMS>::type;
+  using G = Geometry<TERMS, DW>;
+  using F = Forward<TERMS, DW, TILES>;
+  constexpr int kMmaWarp = F::kMma, kLoadWarp = F::kLoad;
+  extern __shared__ unsigned char raw[];
+  unsigned char* smem = aligned_smem(raw);
+  const int d = a.d;
+  constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = F::kRing;
+  Tail* tail = reinterpret_cast<Tail*>(smem + (TILES + R) * tile_bytes);
+  const uint32_t sq = smem_addr(smem), ring = sq + TILES * tile_bytes, bar0 = smem_addr(tail->bars);
+  volatile int* failed = &tail->failed;
+  auto bar = [&](int k) { return bar0 + 8 * k; };
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (warp == kMmaWarp) alloc_tmem(&tail->tmem, 256 * TILES);
+  if (tid == 0) {
+    tail->failed = 0;
+    for (int i = 0; i < kFwdBars; ++i) init_bar(bar(i), (i >= kPFull && i < kPFull + 4) || (i >= kSRead && i < kSRead + 2) ? kTile : i >= kJobFree ? 4 * TILES + 1 : 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = tail->tmem;
+  // columns from one tile's logits to the other's, output of a tile, columns from one output to the other, P
+  constexpr uint32_t kStride = TERMS == 1 ? kTile : 256, kOut = TERMS == 1 ? kTile * TILES : 192, kOutStride = TERMS == 1 ? DW : 256;
+  auto p_at = [](int t) { return G::kEarly ? kOut + 64 * TILES + 64 * t : kStride * t; };
+
+  auto job_at = [&](int m) {
+    if constexpr (F::kQueued) return take_job(tail, m, bar(kJob), bar(kJobFree), lane, failed);
+    else return forward_job<TILES>(a, blockIdx.x);
+  };
+
+  if (warp >= kMmaWarp) {
+    fewer_regs<F::kOtherRegs>();
+    if (warp == kMmaWarp) {
+      const uint32_t on = elect_one();
+      // tiles are counted over all jobs: keys are tiles 0, 2, .. of the ring, values 1, 3, ..; g: the tile at hand, base: tiles of the two tiles of rows
+      // before the job
+      auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
+      auto ready = [&](int j) { wait_bar(bar(kFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
+      auto give = [&](int j) { commit(on, bar(kEmpty + j % R)); };
+      int g = 0, base[2] = {0, 0}, jobs_of[2] = {0, 0};
+      for (int m = 0; F::kQueued || m < 1; ++m) {
+        const Job j = job_at(m);
+        const int n = __shfl_sync(0xffffffffu, j.n, 0), n0 = __shfl_sync(0xffffffffu, j.n0, 0), n1 = __shfl_sync(0xffffffffu, j.n1, 0);
+        if (n < 0) break;
+        if (n == 0) continue;
+        ready(2 * g);
+#pragma unroll
+        for (int t = 0; t < TILES; ++t) {
+          const int nt = t ? n1 : n0;
+          if (nt == 0) continue;
+          wait_bar(bar(kQFull + t), jobs_of[t] & 1, failed, &g_packed_error);
+          ++jobs_of[t];
+          fence_after();
+          product_rows<M, TERMS, DW>(on, tmem + kStride * t, sq + t * tile_bytes, slot(2 * g), d);
+          commit(on, bar(kSFull + t));
+          if (nt == 1) commit(on, bar(kQFree + t));
+        }
+        give(2 * g);
+        for (int i = 0; i < n; ++i, ++g) {
+          auto logits = [&](int t) {
+            const int nt = t ? n1 : n0;
+            if (i + 1 >= nt) return;
+            product_rows<M, TERMS, DW>(on, tmem + kStride * t, sq + t * tile_bytes, slot(2 * g + 2), d);
+            commit(on, bar(kSFull + t));
+            if (i + 2 == nt) commit(on, bar(kQFree + t));
+          };
+          if (i + 1 < n) ready(2 * g + 2);
+          if (G::kEarly) {
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+              if (i + 1 >= (t ? n1 : n0)) continue;
+              wait_bar(bar(kSRead + t), (base[t] + i) & 1, failed, &g_packed_error);
+              fence_after();
+              logits(t);
+            }
+            if (i + 1 < n) give(2 * g + 2);
+          }
+          ready(2 * g + 1);
+#pragma unroll
+          for (int t = 0; t < TILES; ++t) {
+            const int nt = t ? n1 : n0;
+            if (i >= nt) continue;
+            wait_bar(bar(kPFull + t), (base[t] + i) & 1, failed, &g_packed_error);
+            fence_after();
+            const uint32_t at = tmem + p_at(t), out = tmem + kOut + kOutStride * t;
+            const Packed p{{at, at + 64, at + 128}, {32, 32, 32}};
+            if constexpr (TERMS == 1) {      // the first half of the keys while the exponentials of the second are formed
+              product_cols<M, TERMS, DW, 0, 4>(on, out, p, slot(2 * g + 1), d, i > 0);
+              wait_bar(bar(kPFull + 2 + t), (base[t] + i) & 1, failed, &g_packed_error);
+              fence_after();
+              product_cols<M, TERMS, DW, 4, 8>(on, out, p, slot(2 * g + 1), d, 1);
+            } else {
+              product_cols<M, TERMS, DW>(on, out, p, slot(2 * g + 1), d, 0);
+            }
+            if (!G::kEarly) logits(t);
+            if (G::kEarly || i + 1 == nt) commit(on, bar(kOFull + t));
+          }
+          give(2 * g + 1);
+          if (!G::kEarly && i + 1 < n) give(2 * g + 2);
+        }
+        base[0] += n0; base[1] += n1;
+      }
+    } else if (warp == kLoadWarp) {
+      Loader<TERMS, DW> ld{lane, bar(kFix)};
+      int g = 0, jobs_of[2] = {0, 0};
+      for (int m = 0, index = blockIdx.x; F::kQueued || m < 1; ++m) {
+        const Job j = forward_job<TILES>(a, index);
+        const int kvh = j.h / a.group;
+        if constexpr (F::kQueued) publish_job(tail, m, j, bar(kJob), bar(kJobFree), lane, failed);
+        if (__any_sync(0xffffffffu, j.n < 0 || *failed)) break;
+        for (int i = 0; i < 2 * j.n; ++i, ++g) {
+          if (i == 1) {      // behind the first tile of keys, which finds room earlier
+#pragma unroll
+            for (int t = 0; t < TILES; ++t) {
+              if ((t ? j.n1 : j.n0) == 0) continue;
+              if (jobs_of[t] > 0) wait_bar(bar(kQFree + t), (jobs_of[t] - 1) & 1, failed, &g_packed_error);
+              ++jobs_of[t];
+              ld.tile(sq + t * tile_bytes, &maps.q, j.q0 + j.row0 + t * kTile, j.h, bar(kQFull + t), kTile, false, failed, &g_packed_error);
+            }
+          }
+          if (g >= R) wait_bar(bar(kEmpty + g % R), (g / R - 1) & 1, failed, &g_packed_error);
+          const int r = j.k0 + (i >> 1) * kTile;
+          ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kFull + g % R), j.lk - r, i & 1, failed, &g_packed_error);
+        }
+        if (F::kQueued) {
+          if (lane == 0) index = a.queue ? (int)gridDim.x + atomicAdd(a.queue, 1) : a.jobs;
+          index = __shfl_sync(0xffffffffu, index, 0);
+        }
+      }
+      // nothing is pending when the CTA ends
+      for (int t = max(0, g - R); t < g; ++t) wait_bar(bar(kEmpty + t % R), (t / R) & 1, failed, &g_packed_error);
+#pragma unroll
+      for (int t = 0; t < TILES; ++t) if (jobs_of[t] > 0) wait_bar(bar(kQFree + t), (jobs_of[t] - 1) & 1, failed, &g_packed_error);
+    }
+  } else {
+    more_regs<F::kRegs>();
+    const int t = warp >> 2, w = warp & 3;
+    const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16), ts = lanes + kStride * t, to = lanes + kOut + kOutStride * t;
+    constexpr int kOwn = TERMS == 1 ? 1 : DW;
+    int g = 0, job = 0;                        // tiles, and jobs that had any
+    Job j = job_at(0);
+    for (int k = 1; j.n >= 0; ++k) {
+      const int nt = t ? j.n1 : j.n0, off = j.lk - j.lq, row = j.row0 + t * kTile + w * 32 + lane, first = j.row0 + t * kTile + w * 32;
+      float own[kOwn];                         // the output so far (float32)
+#pragma unroll
+      for (int c = 0; c < kOwn; ++c) own[c] = 0.f;
+      // last key that this row sees, and that the warp's first row sees
+      const int lim = min(a.causal ? row + off : j.lk - 1, j.lk - 1), lim_first = min(a.causal ? first + off : j.lk - 1, j.lk - 1);
+      float m = -INFINITY, l = 0.f;
+      for (int i = 0; i < nt; ++i, ++g) {
+        wait_bar(bar(kSFull + t), g & 1, failed, &g_packed_error);
+        fence_after();
+        if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW>(to, own); }
+        uint32_t x[kTile];
+#pragma unroll
+        for (int c = 0; c < kTile; c += 32) ld32(ts + c, x + c);
+        wait_ld(x);
+        if (G::kEarly) { fence_before(); arrive(bar(kSRead + t)); }
+        const int kb = j.k0 + i * kTile;
+        const bool masked = kb + kTile - 1 > lim_first;
+        if (masked) {
+#pragma unroll
+          for (int c = 0; c < kTile; ++c) if (kb + c > lim) x[c] = 0xff800000u;
+        }
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < kTile; c += 8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
+        }
+        const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2);
+        const bool raise = mn > m + 8.f;      // true where there was none yet
+        if (G::kEarly && i > 0) { wait_bar(bar(kOFull + t), (g - 1) & 1, failed, &g_packed_error); fence_after(); }      // the output and P are free
+        if (__any_sync(0xffffffffu, raise)) {
+          const float f = raise ? pow2(m - mn) : 1.f;
+          if (raise) m = mn;
+          l *= f;
+          if constexpr (TERMS == 3) {
+#pragma unroll
+            for (int c = 0; c < kOwn; ++c) own[c] *= f;
+          } else if (i > 0) {
+            for (int c = 0; c < d; c += 16) {
+              uint32_t o[16];
+              ld16(to + c, o);
+              wait_ld(o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+              st16(to + c, o);
+            }
+          }
+        }
+        const float u = m == -INFINITY ? 0.f : -m;
+        float2 sums[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) sums[e] = make_float2(0.f, 0.f);
+        const Packed at{{p_at(t), p_at(t) + 64, p_at(t) + 128}, {}};
+        const float2 scale = make_float2(a.scale_log2, a.scale_log2), ref = make_float2(u, u);
+#pragma unroll
+        for (int c = 0; c < kTile; c += 32) {
+          float y[32];
+          // a masked logit has to give zero, which the polynomial does not
+          if (TERMS == 1 && !masked) { pow2_16<true>(x + c, scale, ref, y); pow2_16<true>(x + c + 16, scale, ref, y + 16); }
+          else { pow2_16<false>(x + c, scale, ref, y); pow2_16<false>(x + c + 16, scale, ref, y + 16); }
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) sums[(e >> 1) & 3] = __fadd2_rn(sums[(e >> 1) & 3], make_float2(y[e], y[e + 1]));
+          put16<M, TERMS>(at, lanes, c, y);
+          put16<M, TERMS>(at, lanes, c + 16, y + 16);
+          if (TERMS == 1 && c == kTile / 2 - 32) {
+            wait_st();
+            fence_before();
+            arrive(bar(kPFull + t));
+          }
+        }
+        const float2 sum = __fadd2_rn(__fadd2_rn(sums[0], sums[1]), __fadd2_rn(sums[2], sums[3]));
+        l += sum.x + sum.y;
+        wait_st();
+        fence_before();
+        arrive(bar(kPFull + t + (TERMS == 1 ? 2 : 0)));
+      }
+      if (nt > 0) {
+        wait_bar(bar(kOFull + t), (G::kEarly ? g - 1 : job) & 1, failed, &g_packed_error);
+        ++job;
+        fence_after();
+      }
+      if constexpr (TERMS == 3) { if (nt > 0) add_cols<DW, DW>(to, own); }
+      const bool there = row < j.lq, bad = *failed;
+      if (a.pieces > 1) {      // the share: o as it is, with its maximum and sum
+        const long long slot = ((long long)j.piece * a.hq + j.h) * a.nq + j.q0 + row;
+        if (there) a.part_ml[slot] = make_float2(m, bad ? NAN : l);
+        float* dst = a.part_o + slot * d;
+        if (nt > 0) {
+          if constexpr (TERMS == 3) {
+#pragma unroll
+            for (int c = 0; c < DW; c += 16) if (there && c < d) store16(dst + c, own + c);
+          } else {
+            for (int c = 0; c < d; c += 16) {
+              uint32_t o[16];
+              float y[16];
+              ld16(to + c, o);
+              wait_ld(o);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(o[e]);
+              if (there) store16(dst + c, y);
+            }
+          }
+        }
+      } else {
+        const float inv = bad ? NAN : l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+        const long long at = ((long long)(j.q0 + row) * a.hq + j.h) * d;
+        T *dst = static_cast<T*>(a.out) + at, *rest = a.out_rest ? static_cast<T*>(a.out_rest) + at : nullptr;
+        if constexpr (TERMS == 3) {
+#pragma unroll
+          for (int c = 0; c < kOwn; ++c) own[c] *= inv;
+#pragma unroll
+          for (int c = 0; c < DW; c += 16) if (there && c < d) store16(dst + c, own + c);
+        } else {
+          for (int c = 0; c < d; c += 16) {
+            uint32_t o[16];
+            float y[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[e] = 0;
+            if (nt > 0) { ld16(to + c, o); wait_ld(o); }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) y[e] = __uint_as_float(o[e]) * inv;
+            if (there) {
+              store16(dst + c, y);
+              if (rest) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 2) {
+                  const float2 r = packed::Half<T>::unpack(packed::Half<T>::pack(y[e], y[e + 1]));
+                  y[e] -= r.x; y[e + 1] -= r.y;
+                }
+                store16(rest + c, y);
+              }
+            }
+          }
+        }
+        if (there && a.lse) a.lse[(long long)j.h * a.nq + j.q0 + row] = bad ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
+      }
+      if constexpr (!F::kQueued) break;
+      j = job_at(k);
+    }
+    fence_before();
+  }
+  __syncthreads();
+  if (warp == kMmaWarp) { fence_after(); free_tmem(tmem, 256 * TILES); }
+}
+
+// ---- reverse: dq ----------------------------------------------------------------------------------------------------
 // dq: 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256 (float32: the third term of dS
 // at 256, dq at 320; where there is room dS at 256 and dq behind it).  The two groups of four warps have 64 columns each of every row.  The
 // next tile's logits are made as soon as these have been read, so that its exponentials run beside the products dS k and g v^T.
@@ -984,11 +1045,11 @@ template <auto kernel> int launch(int64_t grid, int threads, int smem, cudaStrea
   count_launch();
   return kOk;
 }
-// a CTA per SM, which work through `jobs`
-template <auto kernel> int launch_jobs(int64_t jobs, int smem, cudaStream_t st, PackedArgs a, const Maps& m) {
+// up to `ctas` CTAs, which work through `jobs`
+template <auto kernel> int launch_jobs(int64_t jobs, int64_t ctas, int threads, int smem, cudaStream_t st, PackedArgs a, const Maps& m) {
   if (jobs > 0x7fff0000) return kTooLarge;
   a.jobs = (int)jobs;
-  return launch<kernel>(std::min<int64_t>(jobs, sm_count()), kThreads, smem, st, a, m);
+  return launch<kernel>(std::min(jobs, ctas), threads, smem, st, a, m);
 }
 template <typename T, int TERMS, int DW, int TILES> int forward_of(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace) {
   Maps m;
@@ -1000,7 +1061,10 @@ template <typename T, int TERMS, int DW, int TILES> int forward_of(cudaStream_t 
     a.part_ml = reinterpret_cast<float2*>(a.part_o + (long long)a.pieces * a.nq * a.hq * a.d);
   }
   using F = Forward<TERMS, DW, TILES>;
-  rc = launch<forward_kernel<T, TERMS, DW, TILES>>((int64_t)n_items * a.hq * a.pieces, F::kThreads, F::kSmem, st, a, m);
+  const int64_t jobs = (int64_t)n_items * a.hq * a.pieces, ctas = F::kQueued ? sm_count() * (TILES == 1 ? 2 : 1) : jobs;
+  if (jobs <= ctas) a.queue = nullptr;      // each CTA's first job is all
+  else SO3LR_CUDA_CHECK(cudaMemsetAsync(a.queue, 0, sizeof(int), st));
+  rc = launch_jobs<forward_kernel<T, TERMS, DW, TILES>>(jobs, ctas, F::kThreads, F::kSmem, st, a, m);
   if (rc || a.pieces == 1) return rc;
   return packed_join<T>(st, a);
 }
@@ -1015,11 +1079,11 @@ int reverse_of(cudaStream_t st, PackedArgs a, const int4* items_q, int n_q, cons
   if (pieces.dkv > 1) { a.share[1] = share; a.share[2] = share + pieces.dkv * stride_kv; }
   a.items = items_q;
   a.pieces = pieces.dq;
-  rc = launch_jobs<dq_kernel<T, TERMS, DW>>((int64_t)n_q * a.hq * a.pieces, reverse_smem<TERMS, DW>(false), st, a, m);
+  rc = launch_jobs<dq_kernel<T, TERMS, DW>>((int64_t)n_q * a.hq * a.pieces, sm_count(), kThreads, reverse_smem<TERMS, DW>(false), st, a, m);
   if (rc) return rc;
   a.items = items_kv;
   a.pieces = pieces.dkv;
-  rc = launch_jobs<dkv_kernel<T, TERMS, DW>>((int64_t)n_kv * a.hk * a.pieces, reverse_smem<TERMS, DW>(true), st, a, m);
+  rc = launch_jobs<dkv_kernel<T, TERMS, DW>>((int64_t)n_kv * a.hk * a.pieces, sm_count(), kThreads, reverse_smem<TERMS, DW>(true), st, a, m);
   if (rc || (pieces.dq == 1 && pieces.dkv == 1)) return rc;
   return packed_sum<T>(st, a, pieces.dq, pieces.dkv);
 }
