@@ -36,8 +36,8 @@ struct PackedArgs {
   int part_rows = 0;            // most rows of a structure: tokens times heads of a group
   int pieces = 1;               // into which an item's walk is cut; each leaves its share in part_o (pieces, hq, nq, d) and part_ml, or
   float* share[3] = {};         // (reverse) in share: (pieces, rows, heads, d) of dq, dk, dv
-  int jobs = 0;                 // of the tensor-core reverse kernels: items times heads times pieces
-  int* queue = nullptr;         // jobs of dq and of dk and dv that were handed out besides each CTA's first
+  int jobs = 0;                 // of the tensor-core kernels: items times heads times pieces
+  int* queue = nullptr;         // jobs that were handed out besides each CTA's first (forward; dq, and dk and dv)
   int rows = 0, rows_kv = 0;    // of the layout
   int longest_kv = 0;           // keys of its longest structure
   int stages = 2, rev_stages = 2;         // buffers for the walked side in the warp-level kernels: one where all of it fits into it
@@ -61,10 +61,10 @@ template <typename T> int packed_sum(cudaStream_t st, const PackedArgs& a, int p
 // Kernels on the tensor cores: tiles of 128 rows, two of them side by side in the forward kernel.  float32 (d <= 64) runs on operands that
 // are split into three bfloat16 terms ahead (packed_split_bytes of workspace).
 // Whether the forward kernel's CTAs have one tile of 128 rows and half of an SM, or two and all of it.  About 8,200 rows in structures of up to L, one
-// tile / two, us: 8 heads x 128, L = 128 22 / 32, 512 38 / 38, 1,024 46 / 53, but 16,001 rows to 8,192 697 / 666 (keys and values come in
-// twice as often, through half the buffers); 8 x 64 512 29 / 34, 1,024 36 / 47, 9 heads of 8,192 rows 231 / 234; float32 4 x 32, 256
-// 27 / 29, 1,024 41 / 47, 5,000 rows 105 / 100.
-inline bool packed_one_tile(bool f32, int d, int longest_kv) { return f32 ? d <= 32 && longest_kv < 2048 : d <= 64 || longest_kv < 2048; }
+// tile / two, us: 8 heads x 128, L = 128 23 / 29, 512 37 / 39, 1,024 54 / 51, 16,001 rows to 8,192 777 / 680 (keys and values come in
+// twice as often, through half the buffers); 8 x 64 512 29 / 34, 2,048 64 / 75, 9 heads of 8,192 rows 254 / 268; float32 4 x 32, 256
+// 31 / 34, 1,024 45 / 53, 5,000 rows 120 / 115.
+inline bool packed_one_tile(bool f32, int d, int longest_kv) { return f32 ? d <= 32 && longest_kv < 2048 : d <= 64 || longest_kv < 800; }
 struct PackedPieces { int forward = 1, dq = 1, dkv = 1; };
 template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n_items, const PackedPieces& pieces, void* workspace);
 template <typename T>

@@ -8,9 +8,9 @@
 // dS live in tensor memory: P and dS go back there packed to 16 bits, and are the A operand of the next product, so shared memory
 // carries q, k, v and g only.
 //
-// Bound by the tensor cores beside the elementwise work of eight warps.  8,192 rows, 9 heads x 128 bfloat16: forward 260 us (1.19 PFLOP/s), dq 385 (1.20),
+// Bound by the tensor cores beside the elementwise work of eight warps.  8,192 rows, 9 heads x 128 bfloat16: forward 275 us (1.12 PFLOP/s), dq 385 (1.20),
 // dk and dv 444 (1.39; cuBLAS 1.67), the tensor cores busy 62, 59 and 71 % of the time and the schedulers 40 to 51 %.  With 64 values a head
-// a tile has half of the products, each of them no shorter for its 64 columns, and the same elementwise work (235, 306, 366 us; tensor 32, 36,
+// a tile has half of the products, each of them no shorter for its 64 columns, and the same elementwise work (247, 300, 365 us; tensor 32, 36,
 // 40 % busy, schedulers 48 to 55 %): what is left is the latency of two warps per scheduler.  float32, 9 x 32: tensor 54 to 62 %.
 // The two reverse kernels form seven products where one with atomic sums would form five; they give the same bits every time.
 #include "packed_tc.cuh"
