@@ -527,8 +527,9 @@ def to_jax_md(potential, displacement_or_metric, box_size, species=None, dr_thre
 def make_so3lr(lr_cutoff=12.0, dispersion_energy_cutoff_lr_damping=2.0, calculate_forces=True, workdir=None, device=None, readout=None):
     """so3lr/base_calculator.py:8-124.  Returns so3lr_fn(inputs) -> outputs with keys energy (n_graph,),
     forces (n_node,3), dipole_vec (n_graph,3), hirshfeld_ratios (n_node,), partial_charges (n_node,).  With a `readout`
-    (so3lr_b200.StructureReadout, or anything called like it) also features (n_node,128), the network's last layer, and
-    readout (n_graph, ..) = readout(features, positions, graph_start), zero for masked graphs; gradients reach the readout's parameters.
+    (so3lr_b200.StructureReadout, or anything called like it) also features (n_node,128), the network's last layer, zero for masked
+    atoms, and readout (n_graph, ..) = readout(features, positions, graph_start), zero for masked graphs.  It is called with the rows of
+    the unmasked atoms of unmasked graphs alone; gradients reach the readout's parameters.
     `inputs` carries the same keys the reference passes to model.apply (positions, atomic_numbers, idx_i, idx_j,
     idx_i_lr, idx_j_lr, cell, total_charge, num_unpaired_electrons, batch_segments, node_mask, graph_mask);
     long-range lists hold both directions ('sparse', :31)."""
@@ -599,9 +600,17 @@ def make_so3lr(lr_cutoff=12.0, dispersion_energy_cutoff_lr_damping=2.0, calculat
             F = _displacements_vjp(n, torch.float32, dev, [(ii, jj, out["g_edges"]), (il, jl, out["g_edges_lr"])], sign=-1.0)
             res["forces"] = F
         if readout is not None:
-            res["features"] = s.features() * node_mask[:, None]
-            y = readout(res["features"], R, graph_start)
-            res["readout"] = y * gm_t.to(y.dtype).view(-1, *[1] * (y.ndim - 1))
+            res["features"] = s.features().masked_fill_(~node_mask[:, None], 0.0)
+            x, pos, starts = res["features"], R, graph_start
+            there = np.ones(n, bool) if bs is None else np.asarray(torch.as_tensor(gm).cpu(), dtype=bool)[bs_np]
+            if nm is not None:
+                there &= np.asarray(torch.as_tensor(nm).cpu(), dtype=bool)
+            if not there.all():      # a row of zeros would still be attended to
+                starts = np.concatenate([[0], np.cumsum(np.bincount(bs_np[there], minlength=n_graphs))]).astype(np.int32)
+                rows = torch.as_tensor(np.flatnonzero(there), device=dev)
+                x, pos = x[rows], pos[rows]
+            y = readout(x, pos, starts)
+            res["readout"] = torch.where(gm_t.view(-1, *[1] * (y.ndim - 1)), y, torch.zeros_like(y))
         return res
 
     return so3lr_fn
