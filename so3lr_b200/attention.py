@@ -225,7 +225,9 @@ def structure_attention(q, k, v, packed, scale=None):
     q (n, heads, d); k, v (n_kv, heads_kv, d) with heads a multiple of heads_kv (query head h reads key head h // (heads // heads_kv));
     float32, bfloat16 or float16 on one GPU, d a multiple of 16 up to 128, any strides.  scale: 1 / sqrt(d) unless given, positive.  Returns
     (n, heads, d); rows behind the layout's last structure are zero.  Values that are not finite spoil the rows of their own structure
-    only.  Sums and the softmax run in float32; 16-bit probabilities are rounded once to the inputs' type ahead of the product with v."""
+    only.  Sums and the softmax run in float32.  With 16-bit rows the probabilities, and in the backward pass their gradients dS = P (dP - delta),
+    are rounded to the inputs' type on the way into a second product.  float16's backward pass takes powers of two out of both first: cotangents
+    of any size keep their digits."""
     _first(q)
     if not isinstance(packed, PackedStructures):
         raise ValueError(f"packed must be a PackedStructures layout, not {type(packed).__name__}")

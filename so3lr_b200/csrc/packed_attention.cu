@@ -141,7 +141,7 @@ int short_rows(int d) { return d <= 32 ? kShortRows : d <= 64 ? 40 : 24; }
 PackedArgs common(const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a) {
   PackedArgs p;
   p.start_q = dev + im[kStartQ]; p.start_kv = dev + im[kStartKv]; p.split_first = dev + im[kSplitFirst];
-  p.rows = im[kRowsQ]; p.rows_kv = im[kRowsKv]; p.longest_kv = im[kMaxKv];
+  p.rows = im[kRowsQ]; p.rows_kv = im[kRowsKv]; p.longest_kv = im[kMaxKv]; p.structures = im[kN];
   if (std::max(im[kMaxQ], im[kMaxKv]) <= short_rows(a->d)) p.tile_rows = 16;
   p.stages = im[kMaxKv] <= (p.tile_rows == 16 || (a->type == kF32 && a->d > 64) ? 32 : 64) ? 1 : 2;
   p.rev_stages = im[kMaxKv] <= 32 && im[kMaxQ] <= 32 && a->heads_q == a->heads_kv ? 1 : 2;
@@ -219,7 +219,10 @@ int64_t whole_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool
   return (a->type == kF32 && on_tensor_cores(im, a, reverse) ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0) +
          packed_share_bytes(pieces(im, a, reverse), a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse);
 }
-constexpr int64_t kQueueBytes = 16;      // behind these: PackedArgs::queue
+constexpr int64_t kQueueBytes = 16;      // behind these: PackedArgs::queue, and in the reverse pass of float16 largest and size_g
+int64_t size_bytes(const int32_t* im, const so3lr_b200_attention_shape* a) {
+  return a->type == kF16 ? ((int64_t)im[kN] * a->heads_kv * 2 + a->rows_q * a->heads_q) * 4 : 0;
+}
 
 const int4* table(const int32_t* im, const int32_t* dev, int field) { return reinterpret_cast<const int4*>(dev + im[field]); }
 
@@ -249,8 +252,13 @@ int forward(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev
 
 template <typename T>
 int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
-  if (on_tensor_cores(im, a, true)) p.queue = reinterpret_cast<int*>(static_cast<char*>(workspace) + whole_bytes(im, a, true));
-  int rc = packed_delta<T>(st, p, im[kRowsQ]);
+  char* behind = static_cast<char*>(workspace) + whole_bytes(im, a, true);
+  if (on_tensor_cores(im, a, true)) { p.queue = reinterpret_cast<int*>(behind); behind += kQueueBytes; }
+  if (kShifted<T>) {
+    p.largest = reinterpret_cast<unsigned*>(behind);
+    p.size_g = reinterpret_cast<float*>(p.largest + (int64_t)im[kN] * p.hk * 2);
+  }
+  int rc = packed_delta<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128]);
   if (rc) return rc;
   if (on_tensor_cores(im, a, true))
     return packed_reverse_tc<T>(st, p, table(im, dev, kItemsQ128), im[kNItemsQ128], table(im, dev, kItemsKv128), im[kNItemsKv128], pieces(im, a, true), workspace);
@@ -296,7 +304,8 @@ int so3lr_b200_packing_build(int n_structures, const int32_t* start_q, const int
 
 int64_t so3lr_b200_structure_attention_workspace(const int32_t* image, const so3lr_b200_attention_shape* a, int vjp) {
   if (!shape_ok(image, a)) return -1;
-  if (vjp || !few_rows(image, a)) return whole_bytes(image, a, vjp) + (on_tensor_cores(image, a, vjp) ? kQueueBytes : 0);
+  if (vjp || !few_rows(image, a))
+    return whole_bytes(image, a, vjp) + (on_tensor_cores(image, a, vjp) ? kQueueBytes : 0) + (vjp ? size_bytes(image, a) : 0);
   if (!image[kCombine]) return 0;
   return part_floats(image, a) * (int64_t)sizeof(float) + part_floats(image, a) / packed_padded(a->d) * (int64_t)sizeof(float2);
 }

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 
@@ -36,6 +37,10 @@ struct PackedArgs {
   int part_rows = 0;            // most rows of a structure: tokens times heads of a group
   int pieces = 1;               // into which an item's walk is cut; each leaves its share in part_o (pieces, hq, nq, d) and part_ml, or
   float* share[3] = {};         // (reverse) in share: (pieces, rows, heads, d) of dq, dk, dv
+  // reverse pass of float16, else null: bits of the largest |g| and of sqrt(d) times the largest |v_jc| (structure, key head, 2), and |g| of every row (hq, nq)
+  unsigned* largest = nullptr;
+  float* size_g = nullptr;
+  int structures = 0;
   int jobs = 0;                 // of the tensor-core kernels: items times heads times pieces
   int* queue = nullptr;         // jobs that were handed out besides each CTA's first (forward; dq, and dk and dv)
   int rows = 0, rows_kv = 0;    // of the layout
@@ -48,12 +53,24 @@ struct PackedArgs {
 
 constexpr int kPackTile = 64;   // rows of a tile of the mma kernels
 
+// float16 keeps its 11 bits between 2^-14 and 2^16 only, and dS = P (dP - delta) is as small as the cotangents of a mean loss over thousands
+// of keys, or as large as those of a scaled one.  |dS| <= |g| |v| + |g| |o| <= 2 |g| sqrt(d) max |v_jc|: the exponent of two that puts this
+// bound into [2^14, 2^15).  dS goes into its products times that power, which leaves with the factor `scale` at their end: exact, and no instruction more.
+// A row of queries has its own ahead of dS k; ahead of dS^T q, which sums over queries, it is that of the structure and key head.
+template <typename T> constexpr bool kShifted = std::is_same<T, __half>::value;
+__device__ __forceinline__ int grad_shift(float g, float v) {
+  const float x = 2.f * g * v;
+  return x > 0.f ? 14 - ((int)(__float_as_uint(x) >> 23) - 127) : 0;
+}
+__device__ __forceinline__ float two_to(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
 // kernels on the warp-level matrix instructions, one translation unit per type
 template <typename T> int packed_forward_mma(cudaStream_t st, const PackedArgs& a, int n_items);
 template <typename T> int packed_forward_split(cudaStream_t st, const PackedArgs& a, int n_items, int n_structures, bool combine);
 template <typename T> int packed_dq_mma(cudaStream_t st, const PackedArgs& a, int n_items);
 template <typename T> int packed_dkv_mma(cudaStream_t st, const PackedArgs& a, int n_items);
-template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, int rows);
+// items: tiles of 128 rows of both sides
+template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, const int4* items_q, int n_q, const int4* items_kv, int n_kv);
 // joins of the pieces' shares (a.pieces of the forward kernel; of dq, of dk and dv)
 template <typename T> int packed_join(cudaStream_t st, const PackedArgs& a);
 template <typename T> int packed_sum(cudaStream_t st, const PackedArgs& a, int pieces_q, int pieces_kv);

@@ -13,11 +13,10 @@
 // CTAs hide each other's start); the tile of the other side is double-buffered by 16-byte asynchronous copies that fill rows and
 // columns that are not there with zeros.  The accumulator fragment of one product is the A fragment of the next, so P and dS never leave
 // the registers (and are rounded to the inputs' type on the way into the second product: their error then is that of one rounding of an
-// input).  float32 runs as three products of operands split into two tf32 numbers each (hi hi + hi lo + lo hi): 2^-21 of the
+// input; float16 takes a power of two out of both in the reverse pass, see prob_shift and grad_shift).  float32 runs as three products of operands split into two tf32 numbers each (hi hi + hi lo + lo hi): 2^-21 of the
 // product, where a single tf32 product has 2^-11.
 #pragma once
 #include <atomic>
-#include <type_traits>
 
 #include "packed_attention.h"
 
@@ -49,8 +48,9 @@ __device__ __forceinline__ void tf32_split(float x, uint32_t& hi, uint32_t& lo) 
 }
 
 template <typename T> struct Half;
-// float16 keeps its 11 bits down to 2^-14 only, and a normalised probability over thousands of keys lies there: the reverse kernels form
-// 2^15 P (at most 2^15 < 65504, exact, no instruction more) and take the factor out of dv at the end and out of dP - delta.
+// float16 keeps its 11 bits down to 2^-14 only, and a normalised probability over thousands of keys lies there: the kernels of dk and dv form
+// 2^15 P (at most 2^15 < 65504, exact, no instruction more) and take the factor out of dv at the end and out of dP - delta.  dS has a
+// power of two of its own (grad_shift).
 template <typename T> constexpr float prob_shift() { return std::is_same<T, __half>::value ? 15.f : 0.f; }
 template <typename T> constexpr float prob_unscale() { return std::is_same<T, __half>::value ? 1.f / 32768.f : 1.f; }
 template <> struct Half<__nv_bfloat16> {
@@ -613,6 +613,22 @@ __global__ void __launch_bounds__(256) sum_kernel(const PackedArgs a, int first,
 }
 
 // ---- reverse --------------------------------------------------------------------------------------------------------
+// g . o of 16 bytes with what rounding o left, and g . g of a 16-bit type
+template <typename T>
+__device__ __forceinline__ void dot16(const uint4 g, const uint4 o, const uint4 rest, float& sum, float& square) {
+  const uint32_t xs[4] = {g.x, g.y, g.z, g.w}, ys[4] = {o.x, o.y, o.z, o.w}, zs[4] = {rest.x, rest.y, rest.z, rest.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    if constexpr (sizeof(T) == 2) {
+      const float2 u = Half<T>::unpack(xs[e]), v = Half<T>::unpack(ys[e]), w = Half<T>::unpack(zs[e]);
+      sum = fmaf(u.x, v.x + w.x, fmaf(u.y, v.y + w.y, sum));
+      square = fmaf(u.x, u.x, fmaf(u.y, u.y, square));
+    } else {
+      sum = fmaf(__uint_as_float(xs[e]), __uint_as_float(ys[e]), sum);
+    }
+  }
+}
+template <typename T> __device__ __forceinline__ uint4 load16(const void* p, long long at) { return *reinterpret_cast<const uint4*>(static_cast<const T*>(p) + at); }
 // delta = sum over d of g * o, a thread per 16 bytes, rows of all heads; empties the queues of the kernels behind it
 template <typename T>
 __global__ void __launch_bounds__(256) delta_kernel(const PackedArgs a, int rows, int width) {
@@ -622,28 +638,86 @@ __global__ void __launch_bounds__(256) delta_kernel(const PackedArgs a, int rows
   const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) / width;
   const long long r = i / a.hq;
   const int h = (int)(i % a.hq);
-  float sum = 0.f;
+  float sum = 0.f, square = 0.f;
   if (r < rows && part * V < a.d) {
-    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.g.p) + r * a.g.row + h * a.g.head + part * V);
-    const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.o.p) + (r * a.hq + h) * a.d + part * V);
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-    uint32_t zs[4] = {0, 0, 0, 0};
-    if (sizeof(T) == 2 && a.out_rest) {
-      const uint4 z = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.out_rest) + (r * a.hq + h) * a.d + part * V);
-      zs[0] = z.x; zs[1] = z.y; zs[2] = z.z; zs[3] = z.w;
-    }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      if constexpr (sizeof(T) == 2) {
-        const float2 u = Half<T>::unpack(xs[e]), v = Half<T>::unpack(ys[e]), w = Half<T>::unpack(zs[e]);
-        sum = fmaf(u.x, v.x + w.x, fmaf(u.y, v.y + w.y, sum));
-      } else {
-        sum = fmaf(__uint_as_float(xs[e]), __uint_as_float(ys[e]), sum);
-      }
-    }
+    const long long at = (r * a.hq + h) * a.d + part * V;
+    dot16<T>(load16<T>(a.g.p, r * a.g.row + h * a.g.head + part * V), load16<T>(a.o.p, at),
+             sizeof(T) == 2 && a.out_rest ? load16<T>(a.out_rest, at) : make_uint4(0, 0, 0, 0), sum, square);
   }
   for (int x = width >> 1; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
   if (r < rows && part == 0) a.delta[(long long)h * a.nq + r] = sum;
+}
+// The same with the sizes of g and v (PackedArgs::largest, size_g): a CTA per 16 rows of a tile of 128 queries and up to 64 heads, and behind these
+// CTAs for the keys.  A warp takes two rows of 32 / width heads at a time, so that no thread divides and a head's largest stays in a
+// register.  The order of the atomics, one a CTA and head, does not matter.  |v| is bounded by sqrt(d) times its largest value, which
+// needs no sum.
+constexpr int kSizeRows = 16, kSizeHeads = 64;
+template <typename T>
+__global__ void __launch_bounds__(256) delta_sizes_kernel(const PackedArgs a, const int4* items_q, long long ctas_q, const int4* items_kv, int log_width) {
+  constexpr int V = 16 / (int)sizeof(T), kParts = 128 / kSizeRows;
+  __shared__ unsigned most[kSizeHeads];
+  if (a.queue && blockIdx.x == 0 && threadIdx.x < 2) a.queue[threadIdx.x] = 0;
+  const bool of_v = blockIdx.x >= ctas_q;
+  const int all = of_v ? a.hk : a.hq, blocks = (all + kSizeHeads - 1) / kSizeHeads, index = (int)(blockIdx.x - (of_v ? ctas_q : 0));
+  const int4 item = (of_v ? items_kv : items_q)[index / kParts / blocks];
+  const int* start = of_v ? a.start_kv : a.start_q;
+  const int row0 = item.y * 128 + index % kParts * kSizeRows, first = start[item.x] + row0, rows = min(kSizeRows, start[item.x + 1] - first);
+  if (rows <= 0) return;
+  const int h0 = index / kParts % blocks * kSizeHeads, heads = min(kSizeHeads, all - h0), width = 1 << log_width;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & (width - 1);
+  if (threadIdx.x < kSizeHeads) most[threadIdx.x] = 0;
+  __syncthreads();
+  const bool on = part * V < a.d;
+  for (int hb = 0; hb < heads; hb += 32 >> log_width) {      // the same trips for all lanes
+    const int hh = hb + (lane >> log_width), h = h0 + hh;
+    float size = 0.f;
+    uint4 g[2], o[2], rest[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const long long r = first + warp + 8 * u;
+      g[u] = o[u] = rest[u] = make_uint4(0, 0, 0, 0);
+      if (warp + 8 * u < rows && hh < heads && on) {
+        const Rows& x = of_v ? a.v : a.g;
+        g[u] = load16<T>(x.p, r * x.row + h * x.head + part * V);
+        if (!of_v) {
+          const long long at = (r * a.hq + h) * a.d + part * V;
+          o[u] = load16<T>(a.o.p, at);
+          if (a.out_rest) rest[u] = load16<T>(a.out_rest, at);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      // one that is not finite spoils its rows whatever their power of two: left out
+      if (of_v) {
+        const uint32_t xs[4] = {g[u].x, g[u].y, g[u].z, g[u].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 x = Half<T>::unpack(xs[e]);
+          if (isfinite(x.x)) size = fmaxf(size, fabsf(x.x));
+          if (isfinite(x.y)) size = fmaxf(size, fabsf(x.y));
+        }
+      } else {
+        float sum = 0.f, square = 0.f;
+        dot16<T>(g[u], o[u], rest[u], sum, square);
+        for (int x = width >> 1; x; x >>= 1) { sum += __shfl_xor_sync(0xffffffffu, sum, x); square += __shfl_xor_sync(0xffffffffu, square, x); }
+        const float norm = sqrtf(square);
+        if (warp + 8 * u < rows && hh < heads && part == 0) {
+          const long long at = (long long)h * a.nq + first + warp + 8 * u;
+          a.delta[at] = sum;
+          a.size_g[at] = norm;
+        }
+        if (isfinite(norm)) size = fmaxf(size, norm);
+      }
+    }
+    if (of_v) {
+      for (int x = width >> 1; x; x >>= 1) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, x));
+      size *= sqrtf((float)a.d);
+    }
+    if (hh < heads && part == 0) atomicMax(&most[hh], __float_as_uint(size));      // not negative: ordered as their bits are
+  }
+  __syncthreads();
+  if (threadIdx.x < heads) atomicMax(a.largest + ((long long)item.x * a.hk + (h0 + threadIdx.x) / (of_v ? 1 : a.group)) * 2 + of_v, most[threadIdx.x]);
 }
 
 // dq of a tile of 16 NW queries of one head
@@ -674,8 +748,14 @@ __global__ void __launch_bounds__(32 * NW) dq_kernel(const PackedArgs a) {
   const int wr = row0 + warp * 16, ra = wr + (lane >> 2), rb = ra + 8, off = lk - lq, big = 0x7fffffff;
   const int lim_a = a.causal ? ra + off : big, lim_b = a.causal ? rb + off : big, lim_lo = a.causal ? wr + off : big, lim_hi = a.causal ? wr + 15 + off : big;
   const long long at_row = (long long)h * a.nq + q0;
+  int shift_a = 0, shift_b = 0;      // of the rows' dS (grad_shift)
+  if constexpr (kShifted<T>) {
+    const float v = __uint_as_float(a.largest[((long long)s * a.hk + kvh) * 2 + 1]);
+    if (ra < lq) shift_a = grad_shift(a.size_g[at_row + ra], v);
+    if (rb < lq) shift_b = grad_shift(a.size_g[at_row + rb], v);
+  }
   // rows that are not there: exp(-inf) = 0
-  const float ea = ra < lq ? a.lse[at_row + ra] : INFINITY, eb = rb < lq ? a.lse[at_row + rb] : INFINITY;
+  const float ea = ra < lq ? a.lse[at_row + ra] - shift_a : INFINITY, eb = rb < lq ? a.lse[at_row + rb] - shift_b : INFINITY;
   const float da = ra < lq ? a.delta[at_row + ra] : 0.f, db = rb < lq ? a.delta[at_row + rb] : 0.f;
   float dq[DP / 8][4];
 #pragma unroll
@@ -712,11 +792,12 @@ __global__ void __launch_bounds__(32 * NW) dq_kernel(const PackedArgs a) {
     const int r = half ? rb : ra;
     if (r >= lq) continue;
     const long long at = ((long long)(q0 + r) * a.hq + h) * a.d;
+    const float f = kShifted<T> ? a.scale * two_to(-(half ? shift_b : shift_a)) : a.scale;
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n) {
       const int c = n * 8 + 2 * (lane & 3);
       if (c >= a.d) continue;
-      const float x = dq[n][2 * half] * a.scale, y = dq[n][2 * half + 1] * a.scale;
+      const float x = dq[n][2 * half] * f, y = dq[n][2 * half + 1] * f;
       if (a.pieces > 1) store2(a.share[0] + (long long)piece * a.nq * a.hq * a.d + at + c, x, y);
       else store2(static_cast<T*>(a.dq) + at + c, x, y);
     }
@@ -738,6 +819,12 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
   const int kvh = index % a.hk, row0 = item.y * kRows, i0 = item.z, i1 = item.w;
   const int per = (max(i1 - i0, 0) + BN - 1) / BN, all = per * a.group, share = (all + a.pieces - 1) / a.pieces, j0 = min(all, piece * share);
   const int nt = min(share, all - j0);      // from tile j0 on
+  int shift = 0;                            // of the structure's dS (grad_shift)
+  if constexpr (kShifted<T>) {
+    const unsigned* most = a.largest + ((long long)s * a.hk + kvh) * 2;
+    shift = grad_shift(__uint_as_float(most[0]), __uint_as_float(most[1]));
+  }
+  const float un = kShifted<T> ? prob_unscale<T>() * two_to(shift) : 1.f;      // from 2^15 P to P times the power of dS
   load_rows<T, DP, kRows, kThreads>(sk, a.k, kvh, c0, row0, lk, a.d, tid);
   load_rows<T, DP, kRows, kThreads>(sv, a.v, kvh, c0, row0, lk, a.d, tid);
   auto load = [&](int it) {
@@ -749,7 +836,7 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
         const bool ok = b + tid < i1;
         const long long at = (long long)h * a.nq + q0 + b + tid;
         se[buf * BN + tid] = ok ? a.lse[at] - prob_shift<T>() : INFINITY;
-        se[(2 + buf) * BN + tid] = ok ? a.delta[at] * prob_unscale<T>() : 0.f;
+        se[(2 + buf) * BN + tid] = ok ? a.delta[at] * un : 0.f;
       }
     }
     copy_commit();
@@ -780,7 +867,7 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
           const int i = ib + c + (x & 1), lim = x < 2 ? lim_a : lim_b;
           float w = exp2f(fmaf(p[n][x], a.scale_log2, -((x & 1) ? e.y : e.x)));
           if (mask && i < lim) w = 0.f;
-          ds[n][x] = w == 0.f ? 0.f : w * fmaf(ds[n][x], prob_unscale<T>(), -((x & 1) ? d.y : d.x));
+          ds[n][x] = w == 0.f ? 0.f : w * fmaf(ds[n][x], un, -((x & 1) ? d.y : d.x));
           p[n][x] = w;
         }
       }
@@ -790,6 +877,7 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
     __syncthreads();
   }
   copy_wait<0>();
+  const float f = kShifted<T> ? a.scale * two_to(-shift) : a.scale;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = half ? rb : ra;
@@ -799,7 +887,7 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
     for (int n = 0; n < DP / 8; ++n) {
       const int c = n * 8 + 2 * (lane & 3);
       if (c >= a.d) continue;
-      const float k0 = dk[n][2 * half] * a.scale, k1 = dk[n][2 * half + 1] * a.scale;
+      const float k0 = dk[n][2 * half] * f, k1 = dk[n][2 * half + 1] * f;
       const float v0 = dv[n][2 * half] * prob_unscale<T>(), v1 = dv[n][2 * half + 1] * prob_unscale<T>();
       if (a.pieces > 1) {
         const long long to = (long long)piece * a.nkv * a.hk * a.d + at + c;
@@ -893,13 +981,23 @@ template <typename T> int packed_sum(cudaStream_t st, const PackedArgs& a, int p
   count_launch();
   return kOk;
 }
-template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, int rows) {
+template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, const int4* items_q, int n_q, const int4* items_kv, int n_kv) {
   int width = 1;
   while (width * (16 / (int)sizeof(T)) < a.d) width <<= 1;
-  const int64_t ctas = ((int64_t)rows * a.hq * width + 255) / 256;
-  if (ctas > 0x7fffffff) return kTooLarge;
-  if (ctas == 0) return kOk;
-  packed::delta_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, rows, width);
+  if (a.rows == 0) return kOk;
+  if constexpr (kShifted<T>) {
+    auto per_item = [](int heads) { return 128 / packed::kSizeRows * (int64_t)((heads + packed::kSizeHeads - 1) / packed::kSizeHeads); };
+    const int64_t ctas_q = per_item(a.hq) * n_q, ctas = ctas_q + per_item(a.hk) * n_kv;
+    if (ctas > 0x7fffffff) return kTooLarge;
+    SO3LR_CUDA_CHECK(cudaMemsetAsync(a.largest, 0, (size_t)a.structures * a.hk * 2 * sizeof(unsigned), st));
+    int log_width = 0;
+    while (1 << log_width < width) ++log_width;
+    packed::delta_sizes_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, items_q, ctas_q, items_kv, log_width);
+  } else {
+    const int64_t ctas = ((int64_t)a.rows * a.hq * width + 255) / 256;
+    if (ctas > 0x7fffffff) return kTooLarge;
+    packed::delta_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, a.rows, width);
+  }
   count_launch();
   return kOk;
 }

@@ -34,6 +34,8 @@ struct Job {
   int k0;               // forward, dq: first key
   int n0, n1;           // forward: tiles of keys that the two tiles of rows meet (n is the larger count)
   int i0, per, j0;      // dk and dv: first query; tiles of queries of a head from there on; the job's first one among those of all heads of the group
+  float size_v;         // dq of float16: the largest |v|
+  int shift;            // dk and dv of float16: the power of two of dS (grad_shift)
 };
 struct Tail {
   unsigned long long bars[kBars];
@@ -444,6 +446,7 @@ __device__ __forceinline__ Job dq_job(const PackedArgs& a, int index) {
   j.piece = index % a.pieces; j.h = unit % a.hq;
   j.q0 = __ldg(a.start_q + item.x); j.lq = __ldg(a.start_q + item.x + 1) - j.q0; j.c0 = __ldg(a.start_kv + item.x); j.lk = __ldg(a.start_kv + item.x + 1) - j.c0;
   j.row0 = item.y * kTile;
+  if (a.largest) j.size_v = __uint_as_float(__ldg(a.largest + ((long long)item.x * a.hk + j.h / a.group) * 2 + 1));
   const int all = (item.w + kTile - 1) / kTile, share = all / a.pieces, more = all % a.pieces;
   j.k0 = (j.piece * share + min(j.piece, more)) * kTile; j.n = share + (j.piece < more);
   return j;
@@ -566,16 +569,21 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
     const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16), c2 = col / 2;
     const Packed to = E ? Packed{{kDs + c2, kDs + 64 + c2, kDs + 128 + c2}, {}} : Packed{{kDs + (uint32_t)col, kDs + 32 + (uint32_t)col, 256 + c2}, {}};
     const float2 scale = make_float2(a.scale_log2, a.scale_log2);
-    // a row's statistics; rows that are not there: exp(-inf) = 0
-    auto stats = [&](const Job& j, float& e, float& delta) {
+    // a row's statistics, and the power of two of its dS; rows that are not there: exp(-inf) = 0
+    auto stats = [&](const Job& j, float& e, float& delta, int& shift) {
       const int row = j.row0 + w * 32 + lane;
-      e = -INFINITY; delta = 0.f;
-      if (j.n >= 0 && row < j.lq) { const long long at = (long long)j.h * a.nq + j.q0 + row; e = -a.lse[at]; delta = a.delta[at]; }
+      e = -INFINITY; delta = 0.f; shift = 0;
+      if (j.n >= 0 && row < j.lq) {
+        const long long at = (long long)j.h * a.nq + j.q0 + row;
+        if constexpr (kShifted<T>) shift = grad_shift(a.size_g[at], j.size_v);
+        e = (float)shift - a.lse[at]; delta = a.delta[at];
+      }
     };
     int g = 0, job = 0;
     Job j = take_job(tail, 0, bar(kdqJob), bar(kdqJobFree), lane, failed);
     float e, delta;
-    stats(j, e, delta);
+    int shift;
+    stats(j, e, delta, shift);
     for (int m = 1; j.n >= 0; ++m) {
       const int row = j.row0 + w * 32 + lane, first = j.row0 + w * 32;
       const int off = j.lk - j.lq;
@@ -632,12 +640,13 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
         arrive(bar(kdqDs));
       }
       const Job after = take_job(tail, m, bar(kdqJob), bar(kdqJobFree), lane, failed);
-      stats(after, e, delta);
+      const float f0 = kShifted<T> ? a.scale * two_to(-shift) : a.scale;
+      stats(after, e, delta, shift);
       if (j.n > 0) {
         wait_bar(bar(kdqOut), job & 1, failed, &g_packed_error);
         fence_after();
       }
-      const float f = *failed ? NAN : a.scale;
+      const float f = *failed ? NAN : f0;
       const long long at_row = ((long long)(j.q0 + row) * a.hq + j.h) * d;
       auto put = [&](auto* dst) {
         if constexpr (TERMS == 3) {
@@ -686,6 +695,10 @@ __device__ __forceinline__ Job dkv_job(const PackedArgs& a, int index) {
   j.q0 = __ldg(a.start_q + item.x); j.lq = __ldg(a.start_q + item.x + 1) - j.q0; j.c0 = __ldg(a.start_kv + item.x); j.lk = __ldg(a.start_kv + item.x + 1) - j.c0;
   j.row0 = item.y * kTile; j.i0 = item.z;
   j.per = (max(j.lq - j.i0, 0) + kTile - 1) / kTile;
+  if (a.largest) {
+    const unsigned* most = a.largest + ((long long)item.x * a.hk + j.h) * 2;
+    j.shift = grad_shift(__uint_as_float(__ldg(most)), __uint_as_float(__ldg(most + 1)));
+  }
   const int all = j.per * a.group, share = all / a.pieces, more = all % a.pieces;
   j.j0 = j.piece * share + min(j.piece, more); j.n = share + (j.piece < more);
   return j;
@@ -810,6 +823,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       for (int m = 0;; ++m) {
         const Job j = take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, failed);
         if (j.n < 0) break;
+        const float un = kShifted<T> ? packed::prob_unscale<T>() * two_to(j.shift) : 1.f;
         for (int i = 0; i < j.n; ++i, ++g) {
           const int st = g & 1, hq = j.h * a.group + (j.j0 + i) / j.per, b = j.i0 + ((j.j0 + i) % j.per) * kTile;
           if (g >= 2) wait_bar(bar(kkvStatFree + st), ((g >> 1) - 1) & 1, failed, &g_packed_error);
@@ -817,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
             const bool ok = b + r < j.lq;
             const long long at = (long long)hq * a.nq + j.q0 + b + r;
             stats[st * kTile + r] = ok ? packed::prob_shift<T>() - a.lse[at] : -INFINITY;
-            stats[(2 + st) * kTile + r] = ok ? -a.delta[at] * packed::prob_unscale<T>() : 0.f;
+            stats[(2 + st) * kTile + r] = ok ? -a.delta[at] * un : 0.f;
           }
           arrive(bar(kkvStat + st));
         }
@@ -840,6 +854,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       float own[2][kOwn];                      // dv, dk so far (float32), half of the row
 #pragma unroll
       for (int c = 0; c < kOwn; ++c) own[0][c] = own[1][c] = 0.f;
+      const float un = kShifted<T> ? packed::prob_unscale<T>() * two_to(j.shift) : 1.f;      // from 2^15 P to P times the power of dS
       for (int i = 0; i < j.n; ++i, ++g) {
         const int st = g & 1, ib = j.i0 + ((j.j0 + i) % j.per) * kTile + col;
         uint32_t x[64], y[64];
@@ -888,7 +903,6 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         }
         if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDk + half * (DW / 2), own[1]); }
         const float4* dl = reinterpret_cast<const float4*>(stats + (2 + st) * kTile + col);
-        constexpr float un = packed::prob_unscale<T>();
 #pragma unroll
         for (int c = 0; c < 64; c += 16) {
           float v[16];
@@ -917,7 +931,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       const long long at = ((long long)(j.c0 + row) * a.hk + j.h) * d;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
-        const float f = bad ? NAN : which ? a.scale : packed::prob_unscale<T>();
+        const float f = bad ? NAN : !which ? packed::prob_unscale<T>() : kShifted<T> ? a.scale * two_to(-j.shift) : a.scale;
         const uint32_t from = lanes + (which ? kDk : kDv);
         auto put = [&](auto* dst) {
           if constexpr (TERMS == 3) {
