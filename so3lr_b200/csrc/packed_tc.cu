@@ -102,8 +102,8 @@ __device__ __forceinline__ Job take_job(const Tail* tail, int m, uint32_t full, 
 
 // ---- forward --------------------------------------------------------------------------------------------------------
 // 256 queries of one head: two tiles of 128 rows take turns, so that the exponentials of one run beside the products of the other.
-// Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t; P of a tile replaces its logits.  (Up to 64 values a head: output at
-// 256 + 64 t, P at 384 + 64 t; one tile: logits at 0, output at 128, P at 192.  float32: logits at 256 t, the three terms of P from there on, its output at 256 t + 192.)
+// Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t, one tile's at 128; P of a tile replaces its logits.  (Up to 64 values a head,
+// one tile: logits at 0, output at 128, P at 192.  float32: logits at 256 t, the three terms of P from there on, its output at 256 t + 192.)
 // The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
 // the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
 enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kQFree = kQFull + 2, kSFull = kQFree + 2, kPFull = kSFull + 2 /* tile + 2 half */, kOFull = kPFull + 4,
@@ -166,7 +166,8 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
   const uint32_t tmem = tail->tmem;
   // columns from one tile's logits to the other's, output of a tile, columns from one output to the other, P
   constexpr uint32_t kStride = TERMS == 1 ? kTile : 256, kOut = TERMS == 1 ? kTile * TILES : 192, kOutStride = TERMS == 1 ? DW : 256;
-  auto p_at = [](int t) { return G::kEarly ? kOut + 64 * TILES + 64 * t : kStride * t; };
+  static_assert(!G::kEarly || TILES == 1, "P beside the logits: room for one tile's");
+  auto p_at = [](int t) { return G::kEarly ? kOut + 64 : kStride * t; };
 
   auto job_at = [&](int m) {
     if constexpr (F::kQueued) return take_job(tail, m, bar(kJob), bar(kJobFree), lane, failed);
@@ -1108,7 +1109,7 @@ template <typename T> int packed_forward_tc(cudaStream_t st, PackedArgs a, int n
   const bool one = packed_one_tile(sizeof(T) == 4, a.d, a.longest_kv);
   if constexpr (sizeof(T) == 2) {
     if (a.d > 64) return one ? forward_of<T, 1, 128, 1>(st, a, n_items, pieces, workspace) : forward_of<T, 1, 128, 2>(st, a, n_items, pieces, workspace);
-    return one ? forward_of<T, 1, 64, 1>(st, a, n_items, pieces, workspace) : forward_of<T, 1, 64, 2>(st, a, n_items, pieces, workspace);
+    return forward_of<T, 1, 64, 1>(st, a, n_items, pieces, workspace);
   } else {
     if (a.d > 32) return forward_of<T, 3, 64, 2>(st, a, n_items, pieces, workspace);
     return one ? forward_of<T, 3, 32, 1>(st, a, n_items, pieces, workspace) : forward_of<T, 3, 32, 2>(st, a, n_items, pieces, workspace);
