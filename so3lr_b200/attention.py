@@ -7,8 +7,8 @@ The network's own attention stops at its 4.5 A cutoff.  These act on rows packed
     q, k = norm_rotate(q, k, positions, frequencies, q_weight=wq, k_weight=wk)
     out = structure_attention(q, k, v, packed)                    # every row attends to the rows of its structure
 
-Both run on the current stream of their inputs' device, support autograd once (not twice), and give the same bits every time.  No counterpart in
-the reference.  Memory comes from torch's allocator, so a call can be captured into a CUDA graph (capture the backward pass with leaves
+Both run on the current stream of their inputs' device, support autograd once (not twice, and not in forward mode), and give the same bits every time.
+No counterpart in the reference.  Memory comes from torch's allocator, so a call can be captured into a CUDA graph (capture the backward pass with leaves
 that no live eager graph holds: torch's own accumulation nodes remember the stream that they were made on).
 """
 from __future__ import annotations
@@ -18,6 +18,7 @@ import math
 
 import numpy as np
 import torch
+import torch.autograd.forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from ._lib import AttentionShape, NormRotateArgs, Rows, check, lib
@@ -62,6 +63,21 @@ def _first(q):
     if not isinstance(q, torch.Tensor) or q.device.type != "cuda" or q.dtype not in _TYPES or q.ndim != 3:
         got = f"{tuple(q.shape)} {q.dtype} on {q.device}" if isinstance(q, torch.Tensor) else type(q).__name__
         raise ValueError(f"rows must be (n, heads, d) float32, bfloat16 or float16 on a GPU, not {got}")
+
+
+def _no_tangents(name, *tensors):
+    """The kernels read a dual tensor's value through its pointer: its tangent would be dropped, which counts as zero."""
+    if _forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError(f"{name} is not differentiable in forward mode")
+
+
+def _constant(name, x):
+    """The number x; raises where a gradient is asked of it."""
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} is a constant: no gradient is formed for it")
+    return float(x)
 
 
 class _On:
@@ -139,7 +155,7 @@ class PackedStructures:
     def _call(self, q, k, scale):
         """What calls with rows of these shapes have in common: (shape, workspace of the forward call, of its transpose); raises where the
         shapes do not fit."""
-        scale = None if scale is None else float(scale)
+        scale = None if scale is None else _constant("scale", scale)
         key = (q.dtype, q.shape, k.shape, scale)
         call = self._calls.get(key)
         if call is None:
@@ -185,6 +201,7 @@ def _attention_forward(q, k, v, packed, call, train):
 def _attention_backward(ctx, g):
     q, k, v, out, rest, lse = ctx.saved_tensors
     packed, (shape, _, size) = ctx.packed, ctx.call
+    _no_tangents("structure_attention", g)
     with _On(packed._index):
         g = _cotangent(g, q)
         dq, dk, dv = torch.empty_like(q, memory_format=_CONTIGUOUS), torch.empty_like(k, memory_format=_CONTIGUOUS), torch.empty_like(k, memory_format=_CONTIGUOUS)
@@ -223,7 +240,7 @@ def structure_attention(q, k, v, packed, scale=None):
     """softmax(scale q k^T) v inside every structure of `packed`.
 
     q (n, heads, d); k, v (n_kv, heads_kv, d) with heads a multiple of heads_kv (query head h reads key head h // (heads // heads_kv));
-    float32, bfloat16 or float16 on one GPU, d a multiple of 16 up to 128, any strides.  scale: 1 / sqrt(d) unless given, positive.  Returns
+    float32, bfloat16 or float16 on one GPU, d a multiple of 16 up to 128, any strides.  scale: 1 / sqrt(d) unless given, positive, a constant.  Returns
     (n, heads, d); rows behind the layout's last structure are zero.  Values that are not finite spoil the rows of their own structure
     only.  Sums and the softmax run in float32.  With 16-bit rows the probabilities, and in the backward pass their gradients dS = P (dP - delta),
     are rounded to the inputs' type on the way into a second product.  float16's backward pass takes powers of two out of both first: cotangents
@@ -238,6 +255,7 @@ def structure_attention(q, k, v, packed, scale=None):
     _head_rows("v", v, dtype, device)
     if k.shape != v.shape:
         raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} differ")
+    _no_tangents("structure_attention", q, k, v, scale)
     call = packed._call(q, k, scale)
     unit = _UNIT[dtype]
     q, k, v = _aligned(q, unit), _aligned(k, unit), _aligned(v, unit)
@@ -272,6 +290,7 @@ def _norm_rotate_backward(ctx, gq, gk):
     q, k, positions, frequencies, wq, wk = ctx.saved_tensors
     if gq is None and gk is None:
         return (None,) * 8
+    _no_tangents("norm_rotate", gq, gk)
     index, need = q.device.index, ctx.needs_input_grad
     with _On(index):
         gq = _cotangent(torch.zeros_like(q) if gq is None else gq, q)
@@ -315,7 +334,7 @@ def norm_rotate(q, k=None, positions=None, frequencies=None, *, q_weight=None, k
     theta_p = sum_a positions[:, a] frequencies[a, p], formed in float64; pairs are (p, p + d / 2) ("halves") or (2p, 2p + 1)
     ("neighbors").  The product of two rotated rows then depends on the difference of their positions only.  q (n, heads, d) and
     k (n, heads_k, d), or None, float32, bfloat16 or float16 on one GPU, d a multiple of 16 up to 256, any strides.  Gradients: q, k, positions and the
-    weights (frequencies are constants).  Returns new (q, k), contiguous."""
+    weights (frequencies and eps are constants).  Returns new (q, k), contiguous."""
     _first(q)
     n, _, d = q.shape
     dtype, device = q.dtype, q.device
@@ -352,7 +371,8 @@ def norm_rotate(q, k=None, positions=None, frequencies=None, *, q_weight=None, k
             if w is not None and (w.shape != (d,) or w.device != device or w.dtype not in (torch.float32, dtype) or w.dtype != q_weight.dtype):
                 raise ValueError(f"{name} must be ({d},) float32 or {dtype} on {device}, both sides alike, not {tuple(w.shape)} {w.dtype} on {w.device}")
         q_weight, k_weight = q_weight.contiguous(), None if k_weight is None else k_weight.contiguous()
-    eps = float(eps)
+    _no_tangents("norm_rotate", q, k, positions, frequencies, q_weight, k_weight, eps)
+    eps = _constant("eps", eps)
     if not 0 <= eps < math.inf:
         raise ValueError(f"eps must not be negative, not {eps}")
     unit = _UNIT[dtype]
