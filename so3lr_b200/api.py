@@ -529,7 +529,8 @@ def make_so3lr(lr_cutoff=12.0, dispersion_energy_cutoff_lr_damping=2.0, calculat
     forces (n_node,3), dipole_vec (n_graph,3), hirshfeld_ratios (n_node,), partial_charges (n_node,).  With a `readout`
     (so3lr_b200.StructureReadout, or anything called like it) also features (n_node,128), the network's last layer, zero for masked
     atoms, and readout (n_graph, ..) = readout(features, positions, graph_start), zero for masked graphs.  It is called with the rows of
-    the unmasked atoms of unmasked graphs alone; gradients reach the readout's parameters.
+    the unmasked atoms of unmasked graphs alone; gradients reach the readout's parameters, and positions that ask for one are refused
+    then: the features carry no graph back to them, so it would lack most of itself.
     `inputs` carries the same keys the reference passes to model.apply (positions, atomic_numbers, idx_i, idx_j,
     idx_i_lr, idx_j_lr, cell, total_charge, num_unpaired_electrons, batch_segments, node_mask, graph_mask);
     long-range lists hold both directions ('sparse', :31)."""
@@ -543,6 +544,8 @@ def make_so3lr(lr_cutoff=12.0, dispersion_energy_cutoff_lr_damping=2.0, calculat
         n = R.shape[0]
         if tuple(R.shape) != (n, 3):
             raise ValueError(f"positions must be (n, 3), not {tuple(R.shape)}")
+        if readout is not None and ((R.requires_grad and torch.is_grad_enabled()) or torch.autograd.forward_ad.unpack_dual(R).tangent is not None):
+            raise ValueError("a readout has no derivative in the positions (the features carry none): pass positions.detach()")
         Z = np.asarray(torch.as_tensor(inputs["atomic_numbers"]).cpu(), dtype=np.int32)
         bs = inputs.get("batch_segments")
         gm = inputs.get("graph_mask")
