@@ -22,7 +22,8 @@ class StructureReadout(torch.nn.Module):
 
     heads x d: size of the attention (4 x 32, as the network's).  wavelengths: shortest and longest period of the rotation in Angstrom, over
     which the frequencies of each axis are spread geometrically.  Parameters are ordinary torch parameters on `device`, drawn from `seed`;
-    the last layer starts at zero, so an untrained readout gives zero."""
+    the last layer starts at zero, so an untrained readout gives zero.  With 16-bit parameters (`.to(torch.bfloat16)`) or under autocast the
+    products and the attention run in that type; the frequencies stay float32, as the angles of far positions need them."""
 
     MAX_CACHED_LAYOUTS = 8
 
@@ -51,6 +52,13 @@ class StructureReadout(torch.nn.Module):
         self.register_buffer("frequencies", f.float().to(dev))
         self._layouts, self._captured = {}, {}
 
+    def _apply(self, fn, *args, **kwargs):      # .to, .half, ..: the frequencies follow to another device, not to another type
+        frequencies = self.frequencies
+        super()._apply(fn, *args, **kwargs)
+        if self.frequencies.dtype != frequencies.dtype:
+            self.frequencies = frequencies.to(self.frequencies.device)
+        return self
+
     def __getstate__(self):      # layouts hold device tables: a copy makes its own
         return self.__dict__ | {"_layouts": {}, "_captured": {}}
 
@@ -73,9 +81,10 @@ class StructureReadout(torch.nn.Module):
             raise ValueError(f"features must be (n, {FEATURES}) and positions (n, 3), not {tuple(features.shape)} and {tuple(positions.shape)}")
         atoms, pool = self._layout(graph_start)
         heads, d = self.heads, self.d
+        features = features.to(self.qkv.dtype)
         q, k, v = (features @ self.qkv).unflatten(1, (3, heads, d)).unbind(1)
         q, k = norm_rotate(q, k, positions, self.frequencies, q_weight=self.norm_q, k_weight=self.norm_k)
         x = features + structure_attention(q, k, v, atoms).flatten(1) @ self.out
         k, v = (x @ self.pool_kv).unflatten(1, (2, heads, d)).unbind(1)
-        query = self.pool_query.expand(pool.rows_q, heads, d)
+        query = self.pool_query.to(k.dtype).expand(pool.rows_q, heads, d)      # autocast makes k and v 16-bit ones
         return structure_attention(query, k, v, pool).flatten(1) @ self.last
