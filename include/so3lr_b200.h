@@ -114,8 +114,8 @@ SO3LR_B200_API int so3lr_b200_system_aux(so3lr_b200_system* sys, const float** z
                           const float** dispersion_dev);
 
 /* Per-atom features of the network's last layer (n_atoms x 128 float32, caller's atom order) at the latest evaluation, copied to
- * out_dev on `stream`.  INVALID_ARGUMENT before the first evaluation and for decomposed contexts.  The reference keeps them inside its
- * network; here they are what a readout trained on top of it reads. */
+ * out_dev on `stream`.  INVALID_ARGUMENT before the first evaluation, after one that failed on its way, and for decomposed contexts.  The
+ * reference keeps them inside its network; here they are what a readout trained on top of it reads. */
 SO3LR_B200_API int so3lr_b200_system_features(so3lr_b200_system* sys, void* stream, float* out_dev);
 
 /* Counters: number of list rebuilds, short-range edges and long-range pairs of the latest build of each list (an export builds the

@@ -363,7 +363,7 @@ struct so3lr_b200_system {
     bool broken = false;        // a capture failed: the context stays on plain launches
   } step_graph;
   bool have_lists = false;
-  int features_order = 0;      // rows of x[kNumLayers]: 0 none yet, 1 in the caller's order, 2 in that of d_perm
+  int features_order = 0;      // rows of x[kNumLayers]: 0 none (none yet, or a call failed on its way), 1 in the caller's order, 2 in that of d_perm
   // graph-level row pointers
   int *d_rowptr_g = nullptr, *d_rowptr_lr_g = nullptr;
   // activations
@@ -436,6 +436,7 @@ int rebuild_lists(so3lr_b200_system* S, cudaStream_t st, const float* R_user, bo
   const int nb = (S->n + 255) / 256;
   S->sorted = allow_sort && S->cell.periodic && S->n_graphs == 1 && S->n >= kSortMinAtoms;
   if (S->sorted) {
+    S->features_order = 0;    // the order of the rows that an earlier evaluation left is written over
     int rc0 = spatial_order(S->nws, st, S->cell, S->n, R_user, r_sr, S->d_perm);
     if (rc0) return rc0;
     { launch_chained(gather_positions_kernel, nb, 256, 0, st, S->n, S->d_perm, R_user, S->d_Rs); count_launch(); }
@@ -638,6 +639,7 @@ int evaluate_graph(so3lr_b200_system* S, cudaStream_t st, const int* row_ptr, co
   // the reciprocal-space part needs the positions and returns its own gradient; its per-atom energies are not separable, so a
   // non-uniform upstream cotangent is not supported with it
   if (S->ks.mode && (!positions || !g_positions || ge)) return kInvalidArgument;
+  S->features_order = 0;
   float* dR = const_cast<float*>(dR_in);
   const bool tiled = graph_fast_path() && attention_mode() == kAttnTc && n_edges > 0;
   int* asym = S->d_flag + 2;      // 1: some entry has no reversed partner (or the tiled path is off)
@@ -794,6 +796,7 @@ int fused_forward(so3lr_b200_system* S, cudaStream_t st, const float* R, const S
   const int* row_ptr = S->sr.row_ptr; const int* nbr_j = S->sr.nbr_j; const int* edge_i = S->sr.edge_i;
   const int nrecv[kNumLayers] = {c.n2, c.n1, c.n0};   // receivers of layer l
   const int nsend[kNumLayers] = {c.n3, c.n2, c.n1};   // atoms whose q/k/v rows layer l reads
+  S->features_order = 0;
   {
     // everything the evaluation adds into, in one launch (small arrays: as many fills are as many gaps between launches)
     ClearArgs A;

@@ -155,7 +155,8 @@ class System:
         return out
 
     def features(self, stream=None):
-        """(n, 128) float32 features of the network's last layer, one row per atom, at the latest evaluation (a copy)."""
+        """(n, 128) float32 features of the network's last layer, one row per atom, at the latest evaluation (a copy).  Raises where there
+        was none, or where the latest failed on its way."""
         s = stream if stream is not None else torch.cuda.current_stream(self.device)
         with torch.cuda.stream(s):
             out = torch.empty(self.n, 128, device=self.device)
