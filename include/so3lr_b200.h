@@ -29,7 +29,8 @@ enum {
   SO3LR_B200_CUDA_ERROR = 2,
   SO3LR_B200_OVERFLOW = 3,      /* a neighbor list did not fit its fixed capacity */
   SO3LR_B200_NOT_FINITE = 4,    /* NaN / Inf positions */
-  SO3LR_B200_TOO_LARGE = 5
+  SO3LR_B200_TOO_LARGE = 5,
+  SO3LR_B200_INCOMPLETE = 6     /* a bounded wait of an earlier call ran out: that call's results are NaN */
 };
 
 typedef struct so3lr_b200_model so3lr_b200_model;     /* weights + derived tables on one device */
@@ -444,8 +445,9 @@ SO3LR_B200_API int so3lr_b200_structure_attention_vjp(const int32_t* image, cons
                                                       const so3lr_b200_rows* k, const so3lr_b200_rows* v, const void* out, const void* out_rest,
                                                       const float* lse, const so3lr_b200_rows* g, float* delta, void* d_q, void* d_k, void* d_v,
                                                       void* workspace, int64_t workspace_bytes);
-/* 1 where a bounded wait of the tensor-core kernels has run out on the current device since the library was loaded (the rows at hand are
- * NaN, or not written, then); waits for the device */
+/* The tensor-core kernels' waits are bounded (two seconds).  Where one has run out, the call's rows of that CTA and of the jobs that it has taken over
+ * are NaN, and the next structure_attention or _vjp call on that device returns INCOMPLETE, once, without running.  Here: 1 where one has run out
+ * and was not told yet (it is now); waits for the device. */
 SO3LR_B200_API int so3lr_b200_structure_attention_error(int* out);
 
 /* Host-callable pieces of the device math, exported for the CPU tests (no GPU needed). */
@@ -459,6 +461,10 @@ SO3LR_B200_API int so3lr_b200_list_row_total(void* stream, const int32_t* row_co
  * neither do those after it, until the next call.  Returns what is left of the count set before (0 when it ran out).  For tests of
  * what a context does when memory is short. */
 SO3LR_B200_API int64_t so3lr_b200_host_fail_allocation(int64_t nth, int persistent);
+/* How often a wait of the packed attention's tensor-core kernels is tried, for some 4 us each, in the calls to come (500,000 times as the library is
+ * loaded); negative: what the loading warps do not find over at once has run out.  Returns the count before.  For tests of what a call then leaves
+ * and tells. */
+SO3LR_B200_API int so3lr_b200_host_wait_tries(int tries);
 SO3LR_B200_API void so3lr_b200_host_sph_harm(float x, float y, float z, float* y24);
 SO3LR_B200_API void so3lr_b200_host_sph_harm_vjp(float x, float y, float z, const float* g24, float* g3);
 SO3LR_B200_API void so3lr_b200_host_pair_terms(float r, int zi, int zj, float qi, float qj, float hi, float hj, float cutoff_lr,

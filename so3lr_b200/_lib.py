@@ -10,7 +10,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "lib", "libso3lr_b200.so")
 
 STATUS = {0: "ok", 1: "invalid argument", 2: "CUDA error", 3: "neighbor list overflow", 4: "non-finite positions",
-          5: "system too large"}
+          5: "system too large", 6: "a bounded wait of an earlier call ran out, whose results are NaN"}
 
 
 class So3lrB200Error(RuntimeError):
@@ -108,6 +108,7 @@ def _load():
         "so3lr_b200_structure_attention_vjp": (i32, [p] * 16 + [i64]),
         "so3lr_b200_structure_attention_error": (i32, [C.POINTER(i32)]),
         "so3lr_b200_host_fail_allocation": (i64, [i64, i32]),
+        "so3lr_b200_host_wait_tries": (i32, [i32]),
         "so3lr_b200_host_sph_harm": (None, [f32, f32, f32, p]),
         "so3lr_b200_host_sph_harm_vjp": (None, [f32, f32, f32, p, p]),
         "so3lr_b200_host_pair_terms": (None, [f32, i32, i32, f32, f32, f32, f32, f32, f32, p]),

@@ -9,7 +9,8 @@ The network's own attention stops at its 4.5 A cutoff.  These act on rows packed
 
 Both run on the current stream of their inputs' device, support autograd once (not twice, and not in forward mode), and give the same bits every time.
 No counterpart in the reference.  Memory comes from torch's allocator, so a call can be captured into a CUDA graph (capture the backward pass with leaves
-that no live eager graph holds: torch's own accumulation nodes remember the stream that they were made on).
+that no live eager graph holds: torch's own accumulation nodes remember the stream that they were made on).  Every wait inside the kernels is bounded;
+should one run out, rows of that call are NaN and the next structure_attention on the device, forward or backward, raises So3lrB200Error, once.
 """
 from __future__ import annotations
 

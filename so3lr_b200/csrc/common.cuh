@@ -20,6 +20,7 @@ enum Status : int {
   kOverflow = 3,
   kNotFinite = 4,
   kTooLarge = 5,
+  kIncomplete = 6,
 };
 
 #define SO3LR_CUDA_CHECK(expr)                                                        \

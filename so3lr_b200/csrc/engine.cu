@@ -1035,6 +1035,7 @@ SO3LR_B200_API const char* so3lr_b200_status_string(int status) {
     case kOverflow: return "neighbor list overflow";
     case kNotFinite: return "non-finite positions";
     case kTooLarge: return "system too large";
+    case kIncomplete: return "a bounded wait of an earlier call ran out, whose results are NaN";
     default: return "unknown status";
   }
 }

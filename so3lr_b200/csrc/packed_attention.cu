@@ -4,6 +4,7 @@
 #include "../../include/so3lr_b200.h"
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <exception>
 #include <vector>
@@ -219,6 +220,14 @@ int64_t whole_bytes(const int32_t* im, const so3lr_b200_attention_shape* a, bool
   return (a->type == kF32 && on_tensor_cores(im, a, reverse) ? packed_split_bytes(a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse) : 0) +
          packed_share_bytes(pieces(im, a, reverse), a->rows_q, a->rows_kv, a->heads_q, a->heads_kv, a->d, reverse);
 }
+std::atomic<int> g_wait_tries{500000};      // some 4 us each: two seconds
+// The device's word, and kIncomplete where an earlier call's wait has run out: told once.
+int waits(PackedArgs* p) {
+  const int rc = packed_error_word(&p->error);
+  if (rc) return rc;
+  p->wait_tries = g_wait_tries.load(std::memory_order_relaxed);
+  return __atomic_load_n(p->error, __ATOMIC_RELAXED) && __atomic_exchange_n(p->error, 0, __ATOMIC_RELAXED) ? kIncomplete : kOk;
+}
 constexpr int64_t kQueueBytes = 16;      // behind these: PackedArgs::queue, and in the reverse pass of float16 largest and size_g
 int64_t size_bytes(const int32_t* im, const so3lr_b200_attention_shape* a) {
   return a->type == kF16 ? ((int64_t)im[kN] * a->heads_kv * 2 + a->rows_q * a->heads_q) * 4 : 0;
@@ -319,6 +328,8 @@ int so3lr_b200_structure_attention(const int32_t* image, const int32_t* image_de
   const int64_t need = so3lr_b200_structure_attention_workspace(image, a, 0);
   if (need > 0 && (!workspace || workspace_bytes < need)) return kInvalidArgument;
   PackedArgs p = common(image, image_dev, a);
+  const int told = waits(&p);
+  if (told) return told;
   p.q = rows_of(q);
   if (image[kRowsKv]) { p.k = rows_of(k); p.v = rows_of(v); } else { p.k = p.v = p.q; }   // never read: no structure has keys
   p.out = out; p.out_rest = a->type == kF32 ? nullptr : out_rest; p.lse = lse;
@@ -341,6 +352,8 @@ int so3lr_b200_structure_attention_vjp(const int32_t* image, const int32_t* imag
   const int64_t need = so3lr_b200_structure_attention_workspace(image, a, 1);
   if (need > 0 && (!workspace || workspace_bytes < need)) return kInvalidArgument;
   PackedArgs p = common(image, image_dev, a);
+  const int told = waits(&p);
+  if (told) return told;
   if (image[kRowsQ]) { p.q = rows_of(q); p.g = rows_of(g); }
   if (image[kRowsKv]) { p.k = rows_of(k); p.v = rows_of(v); }
   if (!image[kRowsQ]) p.q = p.g = p.k;      // never read: one side has no rows
@@ -353,6 +366,16 @@ int so3lr_b200_structure_attention_vjp(const int32_t* image, const int32_t* imag
   return rc;
 }
 
-int so3lr_b200_structure_attention_error(int* out) { return out ? packed_error(out) : kInvalidArgument; }
+int so3lr_b200_structure_attention_error(int* out) {
+  if (!out) return kInvalidArgument;
+  int* word = nullptr;
+  const int rc = packed_error_word(&word);
+  if (rc) return rc;
+  SO3LR_CUDA_CHECK(cudaDeviceSynchronize());
+  *out = __atomic_exchange_n(word, 0, __ATOMIC_RELAXED);
+  return kOk;
+}
+
+int so3lr_b200_host_wait_tries(int tries) { return g_wait_tries.exchange(tries); }
 
 }  // extern "C"

@@ -42,6 +42,8 @@ struct PackedArgs {
   float* size_g = nullptr;
   int structures = 0;
   int jobs = 0;                 // of the tensor-core kernels: items times heads times pieces
+  int* error = nullptr;         // of the tensor-core kernels: host memory that tells of a wait that has run out, and how often one is tried
+  int wait_tries = 0;
   int* queue = nullptr;         // jobs that were handed out besides each CTA's first (forward; dq, and dk and dv)
   int rows = 0, rows_kv = 0;    // of the layout
   int longest_kv = 0;           // keys of its longest structure
@@ -90,7 +92,7 @@ inline int packed_split_width(int d) { return d <= 32 ? 32 : 64; }
 inline int64_t packed_split_bytes(int64_t rows_q, int64_t rows_kv, int hq, int hk, int d, bool reverse) {
   return ((reverse ? 2 : 1) * rows_q * hq + 2 * rows_kv * hk) * 3 * packed_split_width(d) * 2;
 }
-int packed_error(int* out);
+int packed_error_word(int** word);
 
 // shares of the pieces, behind the split operands
 inline int64_t packed_share_bytes(const PackedPieces& p, int64_t rows_q, int64_t rows_kv, int hq, int hk, int d, bool reverse) {

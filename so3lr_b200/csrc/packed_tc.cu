@@ -16,10 +16,9 @@
 #include "packed_tc.cuh"
 
 #include <algorithm>
+#include <mutex>
 
 namespace so3lr {
-
-__device__ int g_packed_error;      // a bounded wait ran out (so3lr_b200_structure_attention_error)
 
 namespace {
 
@@ -86,16 +85,19 @@ __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* p) { retur
 // 520 / 592; one of 8,192, 9 x 64, 290 / 351 -> 306 / 366 (a job of 64 tiles has no start to hide).  The loading warp takes jobs from a queue, the
 // longest first, and passes them on through shared memory (equal shares instead: SMs differ in their pace by up to 15 %; 5,000 rows, 4 x 32
 // float32, dk and dv 187 us with the queue, 219 without).
-__device__ __forceinline__ void publish_job(Tail* tail, int m, const Job& j, uint32_t full, uint32_t free, int lane, volatile int* failed) {
-  if (m >= 2) wait_bar(free + 8 * (m & 1), ((m >> 1) - 1) & 1, failed, &g_packed_error);
+// Jobs are passed on after a failure too, so that the rows of all of them are written; false where that is at an end as well.
+__device__ __forceinline__ bool publish_job(Tail* tail, int m, const Job& j, uint32_t full, uint32_t free, int lane, const Wait& wait) {
+  const bool ok = m < 2 || wait.end(free + 8 * (m & 1), ((m >> 1) - 1) & 1);
+  if (!__all_sync(0xffffffffu, ok)) return false;
   if (lane == 0) { tail->jobs[m & 1] = j; arrive(full + 8 * (m & 1)); }
   __syncwarp();
+  return true;
 }
 // a warp's m-th job
-__device__ __forceinline__ Job take_job(const Tail* tail, int m, uint32_t full, uint32_t free, int lane, volatile int* failed) {
-  wait_bar(full + 8 * (m & 1), (m >> 1) & 1, failed, &g_packed_error);
+__device__ __forceinline__ Job take_job(const Tail* tail, int m, uint32_t full, uint32_t free, int lane, const Wait& wait) {
+  const bool ok = wait.end(full + 8 * (m & 1), (m >> 1) & 1);
   Job j = tail->jobs[m & 1];
-  if (__any_sync(0xffffffffu, *failed)) j.n = -1;
+  if (!__all_sync(0xffffffffu, ok)) j.n = -1;
   if (lane == 0) arrive(free + 8 * (m & 1));
   return j;
 }
@@ -107,7 +109,7 @@ __device__ __forceinline__ Job take_job(const Tail* tail, int m, uint32_t full, 
 // The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
 // the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
 enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kQFree = kQFull + 2, kSFull = kQFree + 2, kPFull = kSFull + 2 /* tile + 2 half */, kOFull = kPFull + 4,
-              kFix = kOFull + 2, kSRead, kJob = kSRead + 2, kJobFree = kJob + 2, kFwdBars = kJobFree + 2 };
+              kFix = kOFull + 2, kDone, kSRead, kJob = kSRead + 2, kJobFree = kJob + 2, kFwdBars = kJobFree + 2 };
 template <int TILES> __device__ __forceinline__ Job forward_job(const PackedArgs& a, int index) {
   Job j = {};
   j.n = -1;
@@ -151,7 +153,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
   constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = F::kRing;
   Tail* tail = reinterpret_cast<Tail*>(smem + (TILES + R) * tile_bytes);
   const uint32_t sq = smem_addr(smem), ring = sq + TILES * tile_bytes, bar0 = smem_addr(tail->bars);
-  volatile int* failed = &tail->failed;
+  const Wait wait{&tail->failed, a.wait_tries};
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem, 256 * TILES);
@@ -170,7 +172,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
   auto p_at = [](int t) { return G::kEarly ? kOut + 64 : kStride * t; };
 
   auto job_at = [&](int m) {
-    if constexpr (F::kQueued) return take_job(tail, m, bar(kJob), bar(kJobFree), lane, failed);
+    if constexpr (F::kQueued) return take_job(tail, m, bar(kJob), bar(kJobFree), lane, wait);
     else return forward_job<TILES>(a, blockIdx.x);
   };
 
@@ -178,10 +180,11 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
     fewer_regs<F::kOtherRegs>();
     if (warp == kMmaWarp) {
       const uint32_t on = elect_one();
+      auto need = [&](uint32_t b, uint32_t parity) { wait(b, parity); fence_after(); };
       // tiles are counted over all jobs: keys are tiles 0, 2, .. of the ring, values 1, 3, ..; g: the tile at hand, base: tiles of the two tiles of rows
       // before the job
       auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
-      auto ready = [&](int j) { wait_bar(bar(kFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
+      auto ready = [&](int j) { need(bar(kFull + j % R), (j / R) & 1); };
       auto give = [&](int j) { commit(on, bar(kEmpty + j % R)); };
       int g = 0, base[2] = {0, 0}, jobs_of[2] = {0, 0};
       for (int m = 0; F::kQueued || m < 1; ++m) {
@@ -194,9 +197,8 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
         for (int t = 0; t < TILES; ++t) {
           const int nt = t ? n1 : n0;
           if (nt == 0) continue;
-          wait_bar(bar(kQFull + t), jobs_of[t] & 1, failed, &g_packed_error);
+          need(bar(kQFull + t), jobs_of[t] & 1);
           ++jobs_of[t];
-          fence_after();
           product_rows<M, TERMS, DW>(on, tmem + kStride * t, sq + t * tile_bytes, slot(2 * g), d);
           commit(on, bar(kSFull + t));
           if (nt == 1) commit(on, bar(kQFree + t));
@@ -215,8 +217,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
               if (i + 1 >= (t ? n1 : n0)) continue;
-              wait_bar(bar(kSRead + t), (base[t] + i) & 1, failed, &g_packed_error);
-              fence_after();
+              need(bar(kSRead + t), (base[t] + i) & 1);
               logits(t);
             }
             if (i + 1 < n) give(2 * g + 2);
@@ -226,14 +227,12 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
           for (int t = 0; t < TILES; ++t) {
             const int nt = t ? n1 : n0;
             if (i >= nt) continue;
-            wait_bar(bar(kPFull + t), (base[t] + i) & 1, failed, &g_packed_error);
-            fence_after();
+            need(bar(kPFull + t), (base[t] + i) & 1);
             const uint32_t at = tmem + p_at(t), out = tmem + kOut + kOutStride * t;
             const Packed p{{at, at + 64, at + 128}, {32, 32, 32}};
             if constexpr (TERMS == 1) {      // the first half of the keys while the exponentials of the second are formed
               product_cols<M, TERMS, DW, 0, 4>(on, out, p, slot(2 * g + 1), d, i > 0);
-              wait_bar(bar(kPFull + 2 + t), (base[t] + i) & 1, failed, &g_packed_error);
-              fence_after();
+              need(bar(kPFull + 2 + t), (base[t] + i) & 1);
               product_cols<M, TERMS, DW, 4, 8>(on, out, p, slot(2 * g + 1), d, 1);
             } else {
               product_cols<M, TERMS, DW>(on, out, p, slot(2 * g + 1), d, 0);
@@ -246,37 +245,49 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
         }
         base[0] += n0; base[1] += n1;
       }
+      commit(on, bar(kDone));      // no matrix instruction is under way when the CTA ends
+      wait.end(bar(kDone), 0);
     } else if (warp == kLoadWarp) {
       Loader<TERMS, DW> ld{lane, bar(kFix)};
       int g = 0, jobs_of[2] = {0, 0};
+      bool ok = true;             // the same for all lanes
+      auto need = [&](uint32_t b, uint32_t parity) { ok = wait.whole_warp(b, parity) && ok; };
+      auto pass = [&](Job& j) {      // after a failure: the job's rows, without any tile
+        ok = ok && !__any_sync(0xffffffffu, *wait.failed);
+        if (!ok) { j.n = min(j.n, 0); j.n0 = j.n1 = 0; }
+      };
       for (int m = 0, index = blockIdx.x; F::kQueued || m < 1; ++m) {
-        const Job j = forward_job<TILES>(a, index);
+        Job j = forward_job<TILES>(a, index);
+        pass(j);
         const int kvh = j.h / a.group;
-        if constexpr (F::kQueued) publish_job(tail, m, j, bar(kJob), bar(kJobFree), lane, failed);
-        if (__any_sync(0xffffffffu, j.n < 0 || *failed)) break;
-        for (int i = 0; i < 2 * j.n; ++i, ++g) {
+        if constexpr (F::kQueued) { if (!publish_job(tail, m, j, bar(kJob), bar(kJobFree), lane, wait)) break; }
+        if (j.n < 0) break;
+        for (int i = 0; ok && i < 2 * j.n; ++i) {
           if (i == 1) {      // behind the first tile of keys, which finds room earlier
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
               if ((t ? j.n1 : j.n0) == 0) continue;
-              if (jobs_of[t] > 0) wait_bar(bar(kQFree + t), (jobs_of[t] - 1) & 1, failed, &g_packed_error);
+              if (jobs_of[t] > 0) need(bar(kQFree + t), (jobs_of[t] - 1) & 1);
+              if (!ok) continue;
               ++jobs_of[t];
-              ld.tile(sq + t * tile_bytes, &maps.q, j.q0 + j.row0 + t * kTile, j.h, bar(kQFull + t), kTile, false, failed, &g_packed_error);
+              ld.tile(sq + t * tile_bytes, &maps.q, j.q0 + j.row0 + t * kTile, j.h, bar(kQFull + t), kTile, false, wait);
             }
           }
-          if (g >= R) wait_bar(bar(kEmpty + g % R), (g / R - 1) & 1, failed, &g_packed_error);
+          if (ok && g >= R) need(bar(kEmpty + g % R), (g / R - 1) & 1);
+          if (!ok) break;
           const int r = j.k0 + (i >> 1) * kTile;
-          ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kFull + g % R), j.lk - r, i & 1, failed, &g_packed_error);
+          ok = ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kFull + g % R), j.lk - r, i & 1, wait);
+          g += ok;
         }
         if (F::kQueued) {
           if (lane == 0) index = a.queue ? (int)gridDim.x + atomicAdd(a.queue, 1) : a.jobs;
           index = __shfl_sync(0xffffffffu, index, 0);
         }
       }
-      // nothing is pending when the CTA ends
-      for (int t = max(0, g - R); t < g; ++t) wait_bar(bar(kEmpty + t % R), (t / R) & 1, failed, &g_packed_error);
+      // no copy is under way when the CTA ends
+      for (int t = max(0, g - R); t < g; ++t) wait.end(bar(kFull + t % R), (t / R) & 1);
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) if (jobs_of[t] > 0) wait_bar(bar(kQFree + t), (jobs_of[t] - 1) & 1, failed, &g_packed_error);
+      for (int t = 0; t < TILES; ++t) if (jobs_of[t] > 0) wait.end(bar(kQFull + t), (jobs_of[t] - 1) & 1);
     }
   } else {
     more_regs<F::kRegs>();
@@ -294,7 +305,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
       const int lim = min(a.causal ? row + off : j.lk - 1, j.lk - 1), lim_first = min(a.causal ? first + off : j.lk - 1, j.lk - 1);
       float m = -INFINITY, l = 0.f;
       for (int i = 0; i < nt; ++i, ++g) {
-        wait_bar(bar(kSFull + t), g & 1, failed, &g_packed_error);
+        wait(bar(kSFull + t), g & 1);
         fence_after();
         if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW>(to, own); }
         uint32_t x[kTile];
@@ -316,7 +327,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
         }
         const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2);
         const bool raise = mn > m + 8.f;      // true where there was none yet
-        if (G::kEarly && i > 0) { wait_bar(bar(kOFull + t), (g - 1) & 1, failed, &g_packed_error); fence_after(); }      // the output and P are free
+        if (G::kEarly && i > 0) { wait(bar(kOFull + t), (g - 1) & 1); fence_after(); }      // the output and P are free
         if (__any_sync(0xffffffffu, raise)) {
           const float f = raise ? pow2(m - mn) : 1.f;
           if (raise) m = mn;
@@ -364,12 +375,12 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
         arrive(bar(kPFull + t + (TERMS == 1 ? 2 : 0)));
       }
       if (nt > 0) {
-        wait_bar(bar(kOFull + t), (G::kEarly ? g - 1 : job) & 1, failed, &g_packed_error);
+        wait(bar(kOFull + t), (G::kEarly ? g - 1 : job) & 1);
         ++job;
         fence_after();
       }
       if constexpr (TERMS == 3) { if (nt > 0) add_cols<DW, DW>(to, own); }
-      const bool there = row < j.lq, bad = *failed;
+      const bool there = row < j.lq, bad = *wait.failed;
       if (a.pieces > 1) {      // the share: o as it is, with its maximum and sum
         const long long slot = ((long long)j.piece * a.hq + j.h) * a.nq + j.q0 + row;
         if (there) a.part_ml[slot] = make_float2(m, bad ? NAN : l);
@@ -429,6 +440,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
     fence_before();
   }
   __syncthreads();
+  if (tid == 0) wait.report(a.error);
   if (warp == kMmaWarp) { fence_after(); free_tmem(tmem, 256 * TILES); }
 }
 
@@ -436,7 +448,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
 // dq: 128 queries of one head.  Tensor memory: logits at 0, dP at 128 (dS replaces it, in two halves), dq at 256 (float32: the third term of dS
 // at 256, dq at 320; where there is room dS at 256 and dq behind it).  The two groups of four warps have 64 columns each of every row.  The
 // next tile's logits are made as soon as these have been read, so that its exponentials run beside the products dS k and g v^T.
-enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqQFree, kdqS, kdqSRead, kdqDp, kdqDpRead, kdqDs, kdqDsDone, kdqOut, kdqFix, kdqJob,
+enum DqBar { kdqFull, kdqEmpty = kdqFull + 8, kdqQ = kdqEmpty + 8, kdqQFree, kdqS, kdqSRead, kdqDp, kdqDpRead, kdqDs, kdqDsDone, kdqOut, kdqFix, kdqDone, kdqJob,
              kdqJobFree = kdqJob + 2, kDqBars = kdqJobFree + 2 };
 __device__ __forceinline__ Job dq_job(const PackedArgs& a, int index) {
   Job j = {};
@@ -463,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = G::kRing;
   Tail* tail = reinterpret_cast<Tail*>(smem + (2 + R) * tile_bytes);
   const uint32_t sq = smem_addr(smem), sg = sq + tile_bytes, ring = sg + tile_bytes, bar0 = smem_addr(tail->bars);
-  volatile int* failed = &tail->failed;
+  const Wait wait{&tail->failed, a.wait_tries};
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
@@ -484,8 +496,9 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
     fewer_regs<kOtherRegs>();
     if (warp == kMmaWarp) {
       const uint32_t on = elect_one();
+      auto need = [&](uint32_t b, uint32_t parity) { wait(b, parity); fence_after(); };
       auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
-      auto ready = [&](int j) { wait_bar(bar(kdqFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
+      auto ready = [&](int j) { need(bar(kdqFull + j % R), (j / R) & 1); };
       auto give = [&](int j) { commit(on, bar(kdqEmpty + j % R)); };
       // Logits and dP run a tile ahead: tile g + 1 of all, tile i + 1 of the job's n.  The loop is as short as it can be (the loading warp says how
       // many tiles a job has, every product stands in one place, so that a job starts a step early): what this warp does between two
@@ -493,22 +506,22 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       // compute warps do not get to the jobs in between that have no tiles.
       int g = -1;
       for (int job = 0;; ++job) {
-        wait_bar(bar(kdqQ), job & 1, failed, &g_packed_error);
-        const int n = __shfl_sync(0xffffffffu, *failed ? 0 : tail->tiles[job & 1], 0);
+        need(bar(kdqQ), job & 1);
+        const int n = __shfl_sync(0xffffffffu, *wait.failed ? 0 : tail->tiles[job & 1], 0);
         if (n == 0) break;
         for (int i = -1; i < n; ++i) {
           const bool more = i + 1 < n;
           auto logits = [&] {
             if (!more) return;
             ready(2 * g + 2);
-            if (g >= 0) { wait_bar(bar(kdqSRead), g & 1, failed, &g_packed_error); fence_after(); }
+            if (g >= 0) need(bar(kdqSRead), g & 1);
             product_rows<M, TERMS, DW>(on, tmem, sq, slot(2 * g + 2), d);
             commit(on, bar(kdqS));
           };
           auto dp = [&] {
             if (!more) return;
             ready(2 * g + 3);
-            if (E && g >= 0) { wait_bar(bar(kdqDpRead), g & 1, failed, &g_packed_error); fence_after(); }
+            if (E && g >= 0) need(bar(kdqDpRead), g & 1);
             product_rows<M, TERMS, DW>(on, tmem + kTile, sg, slot(2 * g + 3), d);
             commit(on, bar(kdqDp));
             give(2 * g + 3);
@@ -517,8 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
           if (!G::kShort) logits();
           if (E) dp();
           if (i >= 0) {
-            wait_bar(bar(kdqDs), g & 1, failed, &g_packed_error);
-            fence_after();
+            need(bar(kdqDs), g & 1);
             const uint32_t at = tmem + kDs;
             product_cols<M, TERMS, DW>(on, tmem + kOut, E ? Packed{{at, at + 64, at + 128}, {32, 32, 32}} : Packed{{at, at + 32, tmem + 256}, {64, 64, 32}},
                                        slot(2 * g), d, i > 0);
@@ -531,17 +543,27 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
           if (more) ++g;
         }
       }
+      commit(on, bar(kdqDone));      // no matrix instruction is under way when the CTA ends
+      wait.end(bar(kdqDone), 0);
     } else if (warp == kLoadWarp) {
       Loader<TERMS, DW> ld{lane, bar(kdqFix)};
-      int g = 0, job = 0;
+      int g = 0, job = 0;         // tiles, and jobs with any, whose copies were issued
+      bool ok = true;             // the same for all lanes
+      auto need = [&](uint32_t b, uint32_t parity) { ok = wait.whole_warp(b, parity) && ok; };
+      auto pass = [&](Job& j) {      // after a failure: the job's rows, without any tile
+        ok = ok && !__any_sync(0xffffffffu, *wait.failed);
+        if (!ok) { j.n = min(j.n, 0); j.n0 = j.n1 = 0; }
+      };
       for (int m = 0, index = blockIdx.x;; ++m) {
-        const Job j = dq_job(a, index);
+        Job j = dq_job(a, index);
+        pass(j);
         const int kvh = j.h / a.group;
-        publish_job(tail, m, j, bar(kdqJob), bar(kdqJobFree), lane, failed);
-        if (__any_sync(0xffffffffu, j.n < 0 || *failed)) break;
-        for (int i = 0; i < 2 * j.n; ++i, ++g) {
+        if (!publish_job(tail, m, j, bar(kdqJob), bar(kdqJobFree), lane, wait)) break;
+        if (j.n < 0) break;
+        for (int i = 0; ok && i < 2 * j.n; ++i) {
           if (i == 1) {      // behind the first tile of keys, which finds room earlier
-            if (job > 0) wait_bar(bar(kdqQFree), (job - 1) & 1, failed, &g_packed_error);
+            if (job > 0) need(bar(kdqQFree), (job - 1) & 1);
+            if (!ok) break;
             if (lane == 0) {
               tail->tiles[job & 1] = j.n;
               expect(bar(kdqQ), 2 * tile_bytes);
@@ -549,20 +571,23 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
               ld.copies(sg, &maps.g, j.q0 + j.row0, j.h, bar(kdqQ));
             }
             __syncwarp();
+            ++job;
           }
-          if (g >= R) wait_bar(bar(kdqEmpty + g % R), (g / R - 1) & 1, failed, &g_packed_error);
+          if (g >= R) need(bar(kdqEmpty + g % R), (g / R - 1) & 1);
+          if (!ok) break;
           const int r = j.k0 + (i >> 1) * kTile;
-          ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kdqFull + g % R), j.lk - r, !(i & 1), failed, &g_packed_error);
+          ok = ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kdqFull + g % R), j.lk - r, !(i & 1), wait);
+          g += ok;
         }
-        job += j.n > 0;
         if (lane == 0) index = (int)gridDim.x + atomicAdd(a.queue, 1);
         index = __shfl_sync(0xffffffffu, index, 0);
       }
-      // nothing is pending when the CTA ends
-      if (job > 0) wait_bar(bar(kdqQFree), (job - 1) & 1, failed, &g_packed_error);
-      if (lane == 0) { tail->tiles[job & 1] = 0; arrive(bar(kdqQ)); }      // no more jobs
+      // no copy is under way when the CTA ends
+      if (ok && job > 0) need(bar(kdqQFree), (job - 1) & 1);
+      for (int t = max(0, g - R); t < g; ++t) wait.end(bar(kdqFull + t % R), (t / R) & 1);
+      if (job > 0) wait.end(bar(kdqQ), (job - 1) & 1);
+      if (ok && lane == 0) { tail->tiles[job & 1] = 0; arrive(bar(kdqQ)); }      // no more jobs
       __syncwarp();
-      for (int t = max(0, g - R); t < g; ++t) wait_bar(bar(kdqEmpty + t % R), (t / R) & 1, failed, &g_packed_error);
     }
   } else {
     more_regs<kComputeRegs>();
@@ -581,7 +606,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       }
     };
     int g = 0, job = 0;
-    Job j = take_job(tail, 0, bar(kdqJob), bar(kdqJobFree), lane, failed);
+    Job j = take_job(tail, 0, bar(kdqJob), bar(kdqJobFree), lane, wait);
     float e, delta;
     int shift;
     stats(j, e, delta, shift);
@@ -597,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       const float2 ref = make_float2(e, e);
       for (int i = 0; i < j.n; ++i, ++g) {
         uint32_t x[64], y[64];
-        wait_bar(bar(kdqS), g & 1, failed, &g_packed_error);
+        wait(bar(kdqS), g & 1);
         fence_after();
         ld32(lanes + col, x);
         ld32(lanes + col + 32, x + 32);
@@ -612,7 +637,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
           for (int q = 0; q < 16; ++q) x[c + q] = __float_as_uint(v[q]);
         }
         const int kb = j.k0 + i * kTile + col;
-        wait_bar(bar(kdqDp), g & 1, failed, &g_packed_error);
+        wait(bar(kdqDp), g & 1);
         fence_after();
         ld32(lanes + kTile + col, y);
         ld32(lanes + kTile + col + 32, y + 32);
@@ -620,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
         if (E) {
           fence_before();
           arrive(bar(kdqDpRead));
-          if (g > 0) { wait_bar(bar(kdqDsDone), (g - 1) & 1, failed, &g_packed_error); fence_after(); }
+          if (g > 0) { wait(bar(kdqDsDone), (g - 1) & 1); fence_after(); }
         }
         if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kOut + half * (DW / 2), own); }
 #pragma unroll
@@ -640,14 +665,14 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
         fence_before();
         arrive(bar(kdqDs));
       }
-      const Job after = take_job(tail, m, bar(kdqJob), bar(kdqJobFree), lane, failed);
+      const Job after = take_job(tail, m, bar(kdqJob), bar(kdqJobFree), lane, wait);
       const float f0 = kShifted<T> ? a.scale * two_to(-shift) : a.scale;
       stats(after, e, delta, shift);
       if (j.n > 0) {
-        wait_bar(bar(kdqOut), job & 1, failed, &g_packed_error);
+        wait(bar(kdqOut), job & 1);
         fence_after();
       }
-      const float f = *failed ? NAN : f0;
+      const float f = *wait.failed ? NAN : f0;
       const long long at_row = ((long long)(j.q0 + row) * a.hq + j.h) * d;
       auto put = [&](auto* dst) {
         if constexpr (TERMS == 3) {
@@ -677,6 +702,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
     fence_before();
   }
   __syncthreads();
+  if (tid == 0) wait.report(a.error);
   if (warp == kMmaWarp) { fence_after(); free_tmem(tmem); }
 }
 
@@ -684,7 +710,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
 // logits at 0 (P replaces them), dP at 128 (dS replaces it), dv at 256, dk at 384 (float32: the third terms of P and dS at 256 and 320, dv
 // at 384, dk at 448; up to 64 values a head in 16 bits: P at 256, dS at 320, dv at 384, dk at 448).  The tensor cores work in the order
 // dv(i), logits(i + 1), dk(i), dP(i + 1): each pair runs beside the other half of the elementwise work.
-enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvKFree, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvFix, kkvStat, kkvStatFree = kkvStat + 2,
+enum DkvBar { kkvFull, kkvEmpty = kkvFull + 8, kkvK = kkvEmpty + 8, kkvKFree, kkvS, kkvP, kkvDp, kkvDs, kkvOut, kkvFix, kkvDone, kkvStat, kkvStatFree = kkvStat + 2,
               kkvSRead = kkvStatFree + 2, kkvDpRead, kkvPDone, kkvDsDone, kkvJob, kkvJobFree = kkvJob + 2, kDkvBars = kkvJobFree + 2 };
 __device__ __forceinline__ Job dkv_job(const PackedArgs& a, int index) {
   Job j = {};
@@ -716,7 +742,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   float* stats = reinterpret_cast<float*>(smem + (2 + R) * tile_bytes);      // [2][128] -lse in log2, [2][128] -delta
   Tail* tail = reinterpret_cast<Tail*>(stats + 4 * kTile);
   const uint32_t sk = smem_addr(smem), sv = sk + tile_bytes, ring = sv + tile_bytes, bar0 = smem_addr(tail->bars);
-  volatile int* failed = &tail->failed;
+  const Wait wait{&tail->failed, a.wait_tries};
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
@@ -739,36 +765,36 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
     fewer_regs<kOtherRegs>();
     if (warp == kMmaWarp) {
       const uint32_t on = elect_one();
+      auto need = [&](uint32_t b, uint32_t parity) { wait(b, parity); fence_after(); };
       auto slot = [&](int j) { return ring + (j % R) * tile_bytes; };
-      auto ready = [&](int j) { wait_bar(bar(kkvFull + j % R), (j / R) & 1, failed, &g_packed_error); fence_after(); };
+      auto ready = [&](int j) { need(bar(kkvFull + j % R), (j / R) & 1); };
       auto give = [&](int j) { commit(on, bar(kkvEmpty + j % R)); };
       auto packed_at = [&](uint32_t at, uint32_t third) { return E ? Packed{{at}, {32}} : Packed{{at, at + 32, third}, {64, 64, 32}}; };
       int g = -1;
       for (int job = 0;; ++job) {
-        wait_bar(bar(kkvK), job & 1, failed, &g_packed_error);
-        const int n = __shfl_sync(0xffffffffu, *failed ? 0 : tail->tiles[job & 1], 0);
+        need(bar(kkvK), job & 1);
+        const int n = __shfl_sync(0xffffffffu, *wait.failed ? 0 : tail->tiles[job & 1], 0);
         if (n == 0) break;
         for (int i = -1; i < n; ++i) {
           const bool more = i + 1 < n;
           auto logits = [&] {
             if (!more) return;
             ready(2 * g + 2);
-            if (E && g >= 0) { wait_bar(bar(kkvSRead), g & 1, failed, &g_packed_error); fence_after(); }
+            if (E && g >= 0) need(bar(kkvSRead), g & 1);
             product_rows<M, TERMS, DW>(on, tmem, sk, slot(2 * g + 2), d);
             commit(on, bar(kkvS));
           };
           auto dp = [&] {
             if (!more) return;
             ready(2 * g + 3);
-            if (E && g >= 0) { wait_bar(bar(kkvDpRead), g & 1, failed, &g_packed_error); fence_after(); }
+            if (E && g >= 0) need(bar(kkvDpRead), g & 1);
             product_rows<M, TERMS, DW>(on, tmem + kTile, sv, slot(2 * g + 3), d);
             commit(on, bar(kkvDp));
             if (i + 2 == n) commit(on, bar(kkvKFree));
           };
           if (E) logits();
           if (i >= 0) {
-            wait_bar(bar(kkvP), g & 1, failed, &g_packed_error);
-            fence_after();
+            need(bar(kkvP), g & 1);
             product_cols<M, TERMS, DW>(on, tmem + kDv, packed_at(tmem + kP, tmem + 256), slot(2 * g + 1), d, i > 0);
             if (E) commit(on, bar(kkvPDone));
             give(2 * g + 1);
@@ -776,8 +802,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
           if (!E && !G::kShort) logits();
           if (E) dp();
           if (i >= 0) {
-            wait_bar(bar(kkvDs), g & 1, failed, &g_packed_error);
-            fence_after();
+            need(bar(kkvDs), g & 1);
             product_cols<M, TERMS, DW>(on, tmem + kDk, packed_at(tmem + kDs, tmem + 320), slot(2 * g), d, i > 0);
             if (E) commit(on, bar(kkvDsDone));
             if (!more) commit(on, bar(kkvOut));
@@ -788,16 +813,26 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
           if (more) ++g;
         }
       }
+      commit(on, bar(kkvDone));      // no matrix instruction is under way when the CTA ends
+      wait.end(bar(kkvDone), 0);
     } else if (warp == kLoadWarp) {
       Loader<TERMS, DW> ld{lane, bar(kkvFix)};
-      int g = 0, job = 0;
+      int g = 0, job = 0;         // as in dq_kernel
+      bool ok = true;
+      auto need = [&](uint32_t b, uint32_t parity) { ok = wait.whole_warp(b, parity) && ok; };
+      auto pass = [&](Job& j) {      // after a failure: the job's rows, without any tile
+        ok = ok && !__any_sync(0xffffffffu, *wait.failed);
+        if (!ok) { j.n = min(j.n, 0); j.n0 = j.n1 = 0; }
+      };
       for (int m = 0, index = blockIdx.x;; ++m) {
-        const Job j = dkv_job(a, index);
-        publish_job(tail, m, j, bar(kkvJob), bar(kkvJobFree), lane, failed);
-        if (__any_sync(0xffffffffu, j.n < 0 || *failed)) break;
-        for (int i = 0; i < 2 * j.n; ++i, ++g) {
+        Job j = dkv_job(a, index);
+        pass(j);
+        if (!publish_job(tail, m, j, bar(kkvJob), bar(kkvJobFree), lane, wait)) break;
+        if (j.n < 0) break;
+        for (int i = 0; ok && i < 2 * j.n; ++i) {
           if (i == 1) {
-            if (job > 0) wait_bar(bar(kkvKFree), (job - 1) & 1, failed, &g_packed_error);
+            if (job > 0) need(bar(kkvKFree), (job - 1) & 1);
+            if (!ok) break;
             if (lane == 0) {
               tail->tiles[job & 1] = j.n;
               expect(bar(kkvK), 2 * tile_bytes);
@@ -805,29 +840,32 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
               ld.copies(sv, &maps.v, j.c0 + j.row0, j.h, bar(kkvK));
             }
             __syncwarp();
+            ++job;
           }
-          if (g >= R) wait_bar(bar(kkvEmpty + g % R), (g / R - 1) & 1, failed, &g_packed_error);
+          if (g >= R) need(bar(kkvEmpty + g % R), (g / R - 1) & 1);
+          if (!ok) break;
           const int t = j.j0 + (i >> 1), hq = j.h * a.group + t / j.per, b = j.i0 + (t % j.per) * kTile;
-          ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.g : &maps.q, j.q0 + b, hq, bar(kkvFull + g % R), j.lq - b, true, failed, &g_packed_error);
+          ok = ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.g : &maps.q, j.q0 + b, hq, bar(kkvFull + g % R), j.lq - b, true, wait);
+          g += ok;
         }
-        job += j.n > 0;
         if (lane == 0) index = (int)gridDim.x + atomicAdd(a.queue + 1, 1);
         index = __shfl_sync(0xffffffffu, index, 0);
       }
-      if (job > 0) wait_bar(bar(kkvKFree), (job - 1) & 1, failed, &g_packed_error);
-      if (lane == 0) { tail->tiles[job & 1] = 0; arrive(bar(kkvK)); }      // no more jobs
+      if (ok && job > 0) need(bar(kkvKFree), (job - 1) & 1);
+      for (int t = max(0, g - R); t < g; ++t) wait.end(bar(kkvFull + t % R), (t / R) & 1);
+      if (job > 0) wait.end(bar(kkvK), (job - 1) & 1);
+      if (ok && lane == 0) { tail->tiles[job & 1] = 0; arrive(bar(kkvK)); }      // no more jobs
       __syncwarp();
-      for (int t = max(0, g - R); t < g; ++t) wait_bar(bar(kkvEmpty + t % R), (t / R) & 1, failed, &g_packed_error);
     } else {
       const int r0 = (warp - kLoadWarp - 1) * 32 + lane;
       int g = 0;
       for (int m = 0;; ++m) {
-        const Job j = take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, failed);
+        const Job j = take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, wait);
         if (j.n < 0) break;
         const float un = kShifted<T> ? packed::prob_unscale<T>() * two_to(j.shift) : 1.f;
         for (int i = 0; i < j.n; ++i, ++g) {
           const int st = g & 1, hq = j.h * a.group + (j.j0 + i) / j.per, b = j.i0 + ((j.j0 + i) % j.per) * kTile;
-          if (g >= 2) wait_bar(bar(kkvStatFree + st), ((g >> 1) - 1) & 1, failed, &g_packed_error);
+          if (g >= 2) wait(bar(kkvStatFree + st), ((g >> 1) - 1) & 1);
           for (int r = r0; r < kTile; r += 64) {
             const bool ok = b + r < j.lq;
             const long long at = (long long)hq * a.nq + j.q0 + b + r;
@@ -846,7 +884,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
     const Packed to_s = E ? Packed{{kDs + c2}, {}} : Packed{{kDs + (uint32_t)col, kDs + 32 + (uint32_t)col, 320 + c2}, {}};
     const float2 scale = make_float2(a.scale_log2, a.scale_log2);
     int g = 0, job = 0;
-    Job j = take_job(tail, 0, bar(kkvJob), bar(kkvJobFree), lane, failed);
+    Job j = take_job(tail, 0, bar(kkvJob), bar(kkvJobFree), lane, wait);
     for (int m = 1; j.n >= 0; ++m) {
       const int row = j.row0 + w * 32 + lane, last = j.row0 + w * 32 + 31;
       // first query that sees this key, and that sees the warp's last key
@@ -859,8 +897,8 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       for (int i = 0; i < j.n; ++i, ++g) {
         const int st = g & 1, ib = j.i0 + ((j.j0 + i) % j.per) * kTile + col;
         uint32_t x[64], y[64];
-        wait_bar(bar(kkvStat + st), (g >> 1) & 1, failed, &g_packed_error);
-        wait_bar(bar(kkvS), g & 1, failed, &g_packed_error);
+        wait(bar(kkvStat + st), (g >> 1) & 1);
+        wait(bar(kkvS), g & 1);
         fence_after();
         ld32(lanes + col, x);
         ld32(lanes + col + 32, x + 32);
@@ -877,7 +915,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
           x[4 * c] = __float_as_uint(pow2(z0.x)); x[4 * c + 1] = __float_as_uint(pow2(z0.y));
           x[4 * c + 2] = __float_as_uint(r1.x); x[4 * c + 3] = __float_as_uint(r1.y);
         }
-        if (E && g > 0) { wait_bar(bar(kkvPDone), (g - 1) & 1, failed, &g_packed_error); fence_after(); }
+        if (E && g > 0) { wait(bar(kkvPDone), (g - 1) & 1); fence_after(); }
         if (a.causal && ib < lim_last) {
 #pragma unroll
           for (int c = 0; c < 64; ++c) if (ib + c < lim) x[c] = 0;
@@ -892,7 +930,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         wait_st();
         fence_before();
         arrive(bar(kkvP));
-        wait_bar(bar(kkvDp), g & 1, failed, &g_packed_error);
+        wait(bar(kkvDp), g & 1);
         fence_after();
         ld32(lanes + kTile + col, y);
         ld32(lanes + kTile + col + 32, y + 32);
@@ -900,7 +938,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         if (E) {
           fence_before();
           arrive(bar(kkvDpRead));
-          if (g > 0) { wait_bar(bar(kkvDsDone), (g - 1) & 1, failed, &g_packed_error); fence_after(); }
+          if (g > 0) { wait(bar(kkvDsDone), (g - 1) & 1); fence_after(); }
         }
         if constexpr (TERMS == 3) { if (i > 0) add_cols<DW, DW / 2>(lanes + kDk + half * (DW / 2), own[1]); }
         const float4* dl = reinterpret_cast<const float4*>(stats + (2 + st) * kTile + col);
@@ -923,12 +961,12 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         fence_before();
         arrive(bar(kkvDs));
       }
-      const Job after = take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, failed);
+      const Job after = take_job(tail, m, bar(kkvJob), bar(kkvJobFree), lane, wait);
       if (j.n > 0) {
-        wait_bar(bar(kkvOut), job & 1, failed, &g_packed_error);
+        wait(bar(kkvOut), job & 1);
         fence_after();
       }
-      const bool there = row < j.lk, bad = *failed;
+      const bool there = row < j.lk, bad = *wait.failed;
       const long long at = ((long long)(j.c0 + row) * a.hk + j.h) * d;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {
@@ -963,6 +1001,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
     fence_before();
   }
   __syncthreads();
+  if (tid == 0) wait.report(a.error);
   if (warp == kMmaWarp) { fence_after(); free_tmem(tmem); }
 }
 
@@ -1122,9 +1161,27 @@ int packed_reverse_tc(cudaStream_t st, PackedArgs a, const int4* items_q, int n_
   else return a.d <= 32 ? reverse_of<T, 3, 32>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace)
                         : reverse_of<T, 3, 64>(st, a, items_q, n_q, items_kv, n_kv, pieces, workspace);
 }
-int packed_error(int* out) {
-  const cudaError_t e = cudaMemcpyFromSymbol(out, g_packed_error, sizeof(int));
-  return e == cudaSuccess ? kOk : kCudaError;
+// A word of host memory for every device, which a kernel sets when a wait has run out: the next call finds it without waiting for the device.
+int packed_error_word(int** word) {
+  static std::mutex lock;
+  static int* words[64] = {};
+  int dev = 0;
+  SO3LR_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 0 || dev >= 64) return kInvalidArgument;
+  const std::lock_guard<std::mutex> held(lock);
+  if (!words[dev]) {
+    // the first call of all may come while its stream is being captured
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    SO3LR_CUDA_CHECK(cudaThreadExchangeStreamCaptureMode(&mode));
+    void* p = nullptr;
+    const cudaError_t e = cudaHostAlloc(&p, sizeof(int), cudaHostAllocMapped | cudaHostAllocPortable);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    SO3LR_CUDA_CHECK(e);
+    words[dev] = static_cast<int*>(p);
+    __atomic_store_n(words[dev], 0, __ATOMIC_RELAXED);
+  }
+  *word = words[dev];
+  return kOk;
 }
 
 template int packed_forward_tc<__nv_bfloat16>(cudaStream_t, PackedArgs, int, const PackedPieces&, void*);

@@ -19,13 +19,9 @@ constexpr int kMmaWarp = 8, kLoadWarp = 9;      // 0 .. 7 compute, 10 and 11 fet
 constexpr int kThreads = 384;
 // registers a thread of the compute and of the other warps after the split: 256 x 208 + 128 x 88 = 384 x 168, the launch's total
 constexpr int kComputeRegs = 208, kOtherRegs = 88;
-constexpr long long kWaitNs = 2000000000LL;
+constexpr int kEndTries = 2000000;      // 8 s
 
-__device__ __forceinline__ unsigned long long now_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
+// holds the thread for up to some 4 us
 __device__ __forceinline__ bool test_bar(uint32_t bar, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -34,21 +30,45 @@ __device__ __forceinline__ bool test_bar(uint32_t bar, uint32_t parity) {
       "selp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
   return ok != 0;
 }
-// Every wait ends: after two seconds, or when another one of this CTA has run out, the kernel carries on to its end, reports through
-// *error, and writes NaN to the rows at hand.
-__device__ __forceinline__ void wait_bar(uint32_t bar, uint32_t parity, volatile int* failed, int* error) {
-  if (test_bar(bar, parity)) return;
-  unsigned long long t0 = 0;
-  for (unsigned it = 1;; ++it) {
-    if (test_bar(bar, parity)) return;
-    if ((it & 63) == 0) {
-      if (*failed) return;
-      const unsigned long long t = now_ns();
-      if (t0 == 0) t0 = t;
-      if (t - t0 > kWaitNs) { *failed = 1; atomicExch(error, 1); return; }
-    }
+// Every wait ends: after `tries` tries, or when another one of this CTA has run out.  From then on no copy is issued, jobs are passed on without
+// tiles and their rows written as NaN, and the CTA ends behind what is under way (end), where it tells the host (report).  The code of a wait
+// is as short as this: with a clock in it the kernels took up to a tenth longer.
+struct Wait {
+  volatile int* failed;      // in shared memory
+  int tries;
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
+    for (int left = tries; !test_bar(bar, parity);)
+      if (--left < 0 || *failed) { *failed = 1; return false; }
+    return true;
   }
-}
+  // The loading warp's, which issues nothing behind a failure: a slot may have been given back by products that did not wait for its tile, and its
+  // copy may still be under way.  With negative tries, for tests, what is not over at once has run out.
+  __device__ __forceinline__ bool whole_warp(uint32_t bar, uint32_t parity) const {
+    bool ok;
+    if (tries < 0) {
+      uint32_t now;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(now) : "r"(bar), "r"(parity) : "memory");
+      ok = now != 0;
+      if (!ok) *failed = 1;
+    } else {
+      ok = (*this)(bar, parity);
+    }
+    return __all_sync(0xffffffffu, ok && !*failed);
+  }
+  // The waits that hold after a failure too: for what is under way, and for the next job.  What they wait for comes once the waits above have
+  // ended; kEndTries is the bound for what should not be.
+  __device__ __forceinline__ bool end(uint32_t bar, uint32_t parity) const {
+    for (int left = kEndTries; !test_bar(bar, parity);)
+      if (--left < 0) { *failed = 1; return false; }
+    return true;
+  }
+  __device__ __forceinline__ void report(int* error) const {
+    if (*failed) { *const_cast<volatile int*>(error) = 1; __threadfence_system(); }
+  }
+};
 __device__ __forceinline__ void init_bar(uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
 __device__ __forceinline__ void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void fence_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -263,7 +283,7 @@ __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // The whole loading warp calls it.  rows: how many of the tile's 128 rows belong to the structure; where `clear`, the others are cleared
-// (through `fix`, a barrier of this warp's own, and its parity).
+// (through `fix`, a barrier of this warp's own, and its parity).  False where that wait has run out: the tile is not handed over then.
 template <int TERMS, int DW> struct Loader {
   static constexpr uint32_t kSub = Geometry<TERMS, DW>::kSub;
   static constexpr int subs = Geometry<TERMS, DW>::kSubs;
@@ -272,16 +292,18 @@ template <int TERMS, int DW> struct Loader {
   __device__ __forceinline__ void copies(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t bar) const {
     for (int x = 0; x < subs; ++x) tma(dst + x * kSub, map, TERMS == 1 ? 64 * x : 0, row, TERMS == 1 ? head : 3 * head + x, bar);
   }
-  __device__ __forceinline__ void tile(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t full, int rows, bool clear, volatile int* failed,
-                                       int* error) {
+  __device__ __forceinline__ bool tile(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t full, int rows, bool clear, const Wait& wait) {
     if (!clear || rows >= kTile) {
       if (lane == 0) { expect(full, subs * kSub); copies(dst, map, row, head, full); }
       __syncwarp();
-      return;
+      return true;
     }
     if (lane == 0) { expect(fix, subs * kSub); copies(dst, map, row, head, fix); }
     __syncwarp();
-    wait_bar(fix, parity, failed, error);
+    if (!wait.whole_warp(fix, parity)) {
+      wait.end(fix, parity);
+      return false;
+    }
     parity ^= 1;
     for (int x = 0; x < subs; ++x)
       for (int b = rows * Geometry<TERMS, DW>::kRow + lane * 16; b < (int)kSub; b += 512)
@@ -290,6 +312,7 @@ template <int TERMS, int DW> struct Loader {
     __syncwarp();
     if (lane == 0) arrive(full);
     __syncwarp();
+    return true;
   }
 };
 
