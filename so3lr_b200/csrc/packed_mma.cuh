@@ -984,12 +984,13 @@ template <typename T> int packed_sum(cudaStream_t st, const PackedArgs& a, int p
 template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, const int4* items_q, int n_q, const int4* items_kv, int n_kv) {
   int width = 1;
   while (width * (16 / (int)sizeof(T)) < a.d) width <<= 1;
+  // ahead of all else: the kernel of dk and dv reads it where there are no queries too
+  if (kShifted<T> && a.structures > 0) SO3LR_CUDA_CHECK(cudaMemsetAsync(a.largest, 0, (size_t)a.structures * a.hk * 2 * sizeof(unsigned), st));
   if (a.rows == 0) return kOk;
   if constexpr (kShifted<T>) {
     auto per_item = [](int heads) { return 128 / packed::kSizeRows * (int64_t)((heads + packed::kSizeHeads - 1) / packed::kSizeHeads); };
     const int64_t ctas_q = per_item(a.hq) * n_q, ctas = ctas_q + per_item(a.hk) * n_kv;
     if (ctas > 0x7fffffff) return kTooLarge;
-    SO3LR_CUDA_CHECK(cudaMemsetAsync(a.largest, 0, (size_t)a.structures * a.hk * 2 * sizeof(unsigned), st));
     int log_width = 0;
     while (1 << log_width < width) ++log_width;
     packed::delta_sizes_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, items_q, ctas_q, items_kv, log_width);
