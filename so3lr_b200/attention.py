@@ -244,8 +244,8 @@ def structure_attention(q, k, v, packed, scale=None):
     float32, bfloat16 or float16 on one GPU, d a multiple of 16 up to 128, any strides.  scale: 1 / sqrt(d) unless given, positive, a constant.  Returns
     (n, heads, d); rows behind the layout's last structure are zero.  Values that are not finite spoil the rows of their own structure
     only.  Sums and the softmax run in float32.  With 16-bit rows the probabilities, and in the backward pass their gradients dS = P (dP - delta),
-    are rounded to the inputs' type on the way into a second product.  float16's backward pass takes powers of two out of both first: cotangents
-    of any size keep their digits."""
+    are rounded to the inputs' type on the way into a second product.  float16 takes powers of two out of both first: neither the tails of
+    a softmax nor cotangents of any size are lost in its last steps."""
     _first(q)
     if not isinstance(packed, PackedStructures):
         raise ValueError(f"packed must be a PackedStructures layout, not {type(packed).__name__}")

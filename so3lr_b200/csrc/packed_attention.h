@@ -60,6 +60,11 @@ constexpr int kPackTile = 64;   // rows of a tile of the mma kernels
 // bound into [2^14, 2^15).  dS goes into its products times that power, which leaves with the factor `scale` at their end: exact, and no instruction more.
 // A row of queries has its own ahead of dS k; ahead of dS^T q, which sums over queries, it is that of the structure and key head.
 template <typename T> constexpr bool kShifted = std::is_same<T, __half>::value;
+// The forward kernels' probabilities relative to a row's largest take a power of two as well, so that what many keys far below the largest add up to
+// is not lost in the last steps of float16: its largest number, 65504, leaves room for 2^15.  On the tensor cores the reference may lag behind
+// the largest by a factor 2^kLag, for which room has to be left too.
+template <typename T> constexpr float kLag = kShifted<T> ? 4.f : 8.f;
+template <typename T, bool LAGS> constexpr float kHead = !kShifted<T> ? 0.f : LAGS ? 15.f - kLag<T> : 15.f;
 __device__ __forceinline__ int grad_shift(float g, float v) {
   const float x = 2.f * g * v;
   return x > 0.f ? 14 - ((int)(__float_as_uint(x) >> 23) - 127) : 0;

@@ -13,7 +13,7 @@
 // CTAs hide each other's start); the tile of the other side is double-buffered by 16-byte asynchronous copies that fill rows and
 // columns that are not there with zeros.  The accumulator fragment of one product is the A fragment of the next, so P and dS never leave
 // the registers (and are rounded to the inputs' type on the way into the second product: their error then is that of one rounding of an
-// input; float16 takes a power of two out of both in the reverse pass, see prob_shift and grad_shift).  float32 runs as three products of operands split into two tf32 numbers each (hi hi + hi lo + lo hi): 2^-21 of the
+// input; float16 takes a power of two out of both, see kHead, prob_shift and grad_shift).  float32 runs as three products of operands split into two tf32 numbers each (hi hi + hi lo + lo hi): 2^-21 of the
 // product, where a single tf32 product has 2^-11.
 #pragma once
 #include <atomic>
@@ -301,6 +301,7 @@ __global__ void __launch_bounds__(32 * NW) forward_kernel(const PackedArgs a) {
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+  constexpr float head = kHead<T, false>;
   for (int it = 0; it < nt; ++it) {
     if (stages == 2) { load(it + 1); copy_wait<1>(); } else { if (it > 0) load(it); copy_wait<0>(); }
     __syncthreads();
@@ -332,8 +333,8 @@ __global__ void __launch_bounds__(32 * NW) forward_kernel(const PackedArgs a) {
       float ta = 0.f, tb = 0.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        p[n][0] = exp2f(fmaf(p[n][0], a.scale_log2, -ua)); p[n][1] = exp2f(fmaf(p[n][1], a.scale_log2, -ua));
-        p[n][2] = exp2f(fmaf(p[n][2], a.scale_log2, -ub)); p[n][3] = exp2f(fmaf(p[n][3], a.scale_log2, -ub));
+        p[n][0] = exp2f(fmaf(p[n][0], a.scale_log2, head - ua)); p[n][1] = exp2f(fmaf(p[n][1], a.scale_log2, head - ua));
+        p[n][2] = exp2f(fmaf(p[n][2], a.scale_log2, head - ub)); p[n][3] = exp2f(fmaf(p[n][3], a.scale_log2, head - ub));
         ta += p[n][0] + p[n][1]; tb += p[n][2] + p[n][3];
       }
       la = fmaf(la, fa, ta); lb = fmaf(lb, fb, tb);
@@ -351,7 +352,7 @@ __global__ void __launch_bounds__(32 * NW) forward_kernel(const PackedArgs a) {
   for (int half = 0; half < 2; ++half) {
     const int pr = half ? rb : ra;
     if (pr >= rows) continue;
-    const float m = half ? mb : ma, l = half ? lb : la;
+    const float m = (half ? mb : ma) - head, l = half ? lb : la;
     if (SPLIT && item.y > 1) {
       const size_t slot = ((size_t)unit * a.hk + hy) * a.part_rows + pr;
       float* dst = a.part_o + slot * DP + 2 * (lane & 3);
@@ -433,6 +434,7 @@ __global__ void __launch_bounds__(128) narrow_kernel(const PackedArgs a) {
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
   float ma = -INFINITY, mb = -INFINITY, la = 0.f, lb = 0.f;
+  constexpr float head = kHead<T, false>;
   for (int it = 0; it < nt; ++it) {
     load(it + ST - 1);
     copy_wait<ST - 1>();
@@ -461,8 +463,8 @@ __global__ void __launch_bounds__(128) narrow_kernel(const PackedArgs a) {
     ma = na; mb = nb;
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
-      p[n][0] = exp2f(fmaf(p[n][0], a.scale_log2, -ua)); p[n][1] = exp2f(fmaf(p[n][1], a.scale_log2, -ua));
-      p[n][2] = exp2f(fmaf(p[n][2], a.scale_log2, -ub)); p[n][3] = exp2f(fmaf(p[n][3], a.scale_log2, -ub));
+      p[n][0] = exp2f(fmaf(p[n][0], a.scale_log2, head - ua)); p[n][1] = exp2f(fmaf(p[n][1], a.scale_log2, head - ua));
+      p[n][2] = exp2f(fmaf(p[n][2], a.scale_log2, head - ub)); p[n][3] = exp2f(fmaf(p[n][3], a.scale_log2, head - ub));
     }
     la = fmaf(la, fa, p[0][0] + p[0][1] + p[1][0] + p[1][1]);
     lb = fmaf(lb, fb, p[0][2] + p[0][3] + p[1][2] + p[1][3]);
@@ -493,6 +495,7 @@ __global__ void __launch_bounds__(128) narrow_kernel(const PackedArgs a) {
 #pragma unroll
     for (int w = 0; w < 4; ++w) m = fmaxf(m, so[(w * kNarrowRows + r) * W + DP]);
     const float u = m == -INFINITY ? 0.f : m;
+    m -= head;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
       f[w] = exp2f(so[(w * kNarrowRows + r) * W + DP] - u);

@@ -106,8 +106,8 @@ __device__ __forceinline__ Job take_job(const Tail* tail, int m, uint32_t full, 
 // 256 queries of one head: two tiles of 128 rows take turns, so that the exponentials of one run beside the products of the other.
 // Tensor memory: logits of tile t at 128 t, its output at 256 + 128 t, one tile's at 128; P of a tile replaces its logits.  (Up to 64 values a head,
 // one tile: logits at 0, output at 128, P at 192.  float32: logits at 256 t, the three terms of P from there on, its output at 256 t + 192.)
-// The running maximum that the exponentials refer to is raised only where it would grow by more than 8 (in log2): P stays below 2^8, and
-// the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
+// The running maximum that the exponentials refer to is raised only where it would grow by more than kLag (in log2): P stays below
+// 2^(kHead + kLag), and the output, which the tensor cores add to, is rescaled a few times per row instead of once per tile of keys.
 enum FwdBar { kFull, kEmpty = kFull + 8, kQFull = kEmpty + 8, kQFree = kQFull + 2, kSFull = kQFree + 2, kPFull = kSFull + 2 /* tile + 2 half */, kOFull = kPFull + 4,
               kFix = kOFull + 2, kDone, kSRead, kJob = kSRead + 2, kJobFree = kJob + 2, kFwdBars = kJobFree + 2 };
 template <int TILES> __device__ __forceinline__ Job forward_job(const PackedArgs& a, int index) {
@@ -294,6 +294,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
     const int t = warp >> 2, w = warp & 3;
     const uint32_t lanes = tmem + ((uint32_t)(32 * w) << 16), ts = lanes + kStride * t, to = lanes + kOut + kOutStride * t;
     constexpr int kOwn = TERMS == 1 ? 1 : DW;
+    constexpr float head = kHead<T, true>;
     int g = 0, job = 0;                        // tiles, and jobs that had any
     Job j = job_at(0);
     for (int k = 1; j.n >= 0; ++k) {
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
           for (int e = 0; e < 4; ++e) top[e] = max3(top[e], __uint_as_float(x[c + 2 * e]), __uint_as_float(x[c + 2 * e + 1]));
         }
         const float mn = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.scale_log2);
-        const bool raise = mn > m + 8.f;      // true where there was none yet
+        const bool raise = mn > m + kLag<T>;      // true where there was none yet
         if (G::kEarly && i > 0) { wait(bar(kOFull + t), (g - 1) & 1); fence_after(); }      // the output and P are free
         if (__any_sync(0xffffffffu, raise)) {
           const float f = raise ? pow2(m - mn) : 1.f;
@@ -346,7 +347,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
             }
           }
         }
-        const float u = m == -INFINITY ? 0.f : -m;
+        const float u = m == -INFINITY ? 0.f : head - m;
         float2 sums[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) sums[e] = make_float2(0.f, 0.f);
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
       const bool there = row < j.lq, bad = *wait.failed;
       if (a.pieces > 1) {      // the share: o as it is, with its maximum and sum
         const long long slot = ((long long)j.piece * a.hq + j.h) * a.nq + j.q0 + row;
-        if (there) a.part_ml[slot] = make_float2(m, bad ? NAN : l);
+        if (there) a.part_ml[slot] = make_float2(m - head, bad ? NAN : l);
         float* dst = a.part_o + slot * d;
         if (nt > 0) {
           if constexpr (TERMS == 3) {
@@ -432,7 +433,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
             }
           }
         }
-        if (there && a.lse) a.lse[(long long)j.h * a.nq + j.q0 + row] = bad ? NAN : l == 0.f ? -INFINITY : m + log2f(l);
+        if (there && a.lse) a.lse[(long long)j.h * a.nq + j.q0 + row] = bad ? NAN : l == 0.f ? -INFINITY : m - head + log2f(l);
       }
       if constexpr (!F::kQueued) break;
       j = job_at(k);
