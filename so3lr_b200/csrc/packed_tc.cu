@@ -87,8 +87,7 @@ __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* p) { retur
 // float32, dk and dv 187 us with the queue, 219 without).
 // Jobs are passed on after a failure too, so that the rows of all of them are written; false where that is at an end as well.
 __device__ __forceinline__ bool publish_job(Tail* tail, int m, const Job& j, uint32_t full, uint32_t free, int lane, const Wait& wait) {
-  const bool ok = m < 2 || wait.end(free + 8 * (m & 1), ((m >> 1) - 1) & 1);
-  if (!__all_sync(0xffffffffu, ok)) return false;
+  if (m >= 2 && !__all_sync(0xffffffffu, wait.end(free + 8 * (m & 1), ((m >> 1) - 1) & 1))) return false;
   if (lane == 0) { tail->jobs[m & 1] = j; arrive(full + 8 * (m & 1)); }
   __syncwarp();
   return true;
@@ -100,6 +99,12 @@ __device__ __forceinline__ Job take_job(const Tail* tail, int m, uint32_t full, 
   if (!__all_sync(0xffffffffu, ok)) j.n = -1;
   if (lane == 0) arrive(free + 8 * (m & 1));
   return j;
+}
+// the next job's index
+__device__ __forceinline__ int next_index(int* queue, int at, int last, int lane) {
+  int index = 0;
+  if (lane == 0) index = queue ? at + atomicAdd(queue, 1) : last;
+  return __shfl_sync(0xffffffffu, index, 0);
 }
 
 // ---- forward --------------------------------------------------------------------------------------------------------
@@ -153,7 +158,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
   constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = F::kRing;
   Tail* tail = reinterpret_cast<Tail*>(smem + (TILES + R) * tile_bytes);
   const uint32_t sq = smem_addr(smem), ring = sq + TILES * tile_bytes, bar0 = smem_addr(tail->bars);
-  const Wait wait{&tail->failed, a.wait_tries};
+  const Wait wait{smem_addr(&tail->failed), a.wait_tries};
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem, 256 * TILES);
@@ -248,46 +253,36 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
       commit(on, bar(kDone));      // no matrix instruction is under way when the CTA ends
       wait.end(bar(kDone), 0);
     } else if (warp == kLoadWarp) {
-      Loader<TERMS, DW> ld{lane, bar(kFix)};
-      int g = 0, jobs_of[2] = {0, 0};
-      bool ok = true;             // the same for all lanes
-      auto need = [&](uint32_t b, uint32_t parity) { ok = wait.whole_warp(b, parity) && ok; };
-      auto pass = [&](Job& j) {      // after a failure: the job's rows, without any tile
-        ok = ok && !__any_sync(0xffffffffu, *wait.failed);
-        if (!ok) { j.n = min(j.n, 0); j.n0 = j.n1 = 0; }
-      };
+      Loader<TERMS, DW> ld{lane, bar(kFix), wait};
+      int g = 0, issued = 0, jobs_of[2] = {0, 0}, issued_of[2] = {0, 0};      // tiles; those whose copies the first lane has issued
+      bool stop = false;          // after a failure: jobs without any tile
       for (int m = 0, index = blockIdx.x; F::kQueued || m < 1; ++m) {
         Job j = forward_job<TILES>(a, index);
-        pass(j);
+        if (stop) { j.n = min(j.n, 0); j.n0 = j.n1 = 0; }
         const int kvh = j.h / a.group;
         if constexpr (F::kQueued) { if (!publish_job(tail, m, j, bar(kJob), bar(kJobFree), lane, wait)) break; }
         if (j.n < 0) break;
-        for (int i = 0; ok && i < 2 * j.n; ++i) {
+        for (int i = 0; i < 2 * j.n; ++i, ++g) {
           if (i == 1) {      // behind the first tile of keys, which finds room earlier
 #pragma unroll
             for (int t = 0; t < TILES; ++t) {
               if ((t ? j.n1 : j.n0) == 0) continue;
-              if (jobs_of[t] > 0) need(bar(kQFree + t), (jobs_of[t] - 1) & 1);
-              if (!ok) continue;
+              if (jobs_of[t] > 0) ld.need(bar(kQFree + t), (jobs_of[t] - 1) & 1);
               ++jobs_of[t];
-              ld.tile(sq + t * tile_bytes, &maps.q, j.q0 + j.row0 + t * kTile, j.h, bar(kQFull + t), kTile, false, wait);
+              issued_of[t] += ld.tile(sq + t * tile_bytes, &maps.q, j.q0 + j.row0 + t * kTile, j.h, bar(kQFull + t), kTile, false);
             }
           }
-          if (ok && g >= R) need(bar(kEmpty + g % R), (g / R - 1) & 1);
-          if (!ok) break;
+          if (g >= R) ld.need(bar(kEmpty + g % R), (g / R - 1) & 1);
           const int r = j.k0 + (i >> 1) * kTile;
-          ok = ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kFull + g % R), j.lk - r, i & 1, wait);
-          g += ok;
+          issued += ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kFull + g % R), j.lk - r, i & 1);
         }
-        if (F::kQueued) {
-          if (lane == 0) index = a.queue ? (int)gridDim.x + atomicAdd(a.queue, 1) : a.jobs;
-          index = __shfl_sync(0xffffffffu, index, 0);
-        }
+        if (F::kQueued) { index = next_index(a.queue, gridDim.x, a.jobs, lane); stop = __any_sync(0xffffffffu, wait.failed()); }
       }
       // no copy is under way when the CTA ends
-      for (int t = max(0, g - R); t < g; ++t) wait.end(bar(kFull + t % R), (t / R) & 1);
+      for (int t = max(0, issued - R); t < issued; ++t) wait.end(bar(kFull + t % R), (t / R) & 1);
 #pragma unroll
-      for (int t = 0; t < TILES; ++t) if (jobs_of[t] > 0) wait.end(bar(kQFull + t), (jobs_of[t] - 1) & 1);
+      for (int t = 0; t < TILES; ++t) if (issued_of[t] > 0) wait.end(bar(kQFull + t), (issued_of[t] - 1) & 1);
+      __syncwarp();
     }
   } else {
     more_regs<F::kRegs>();
@@ -381,7 +376,7 @@ __global__ void __launch_bounds__(Forward<TERMS, DW, TILES>::kThreads, TILES == 
         fence_after();
       }
       if constexpr (TERMS == 3) { if (nt > 0) add_cols<DW, DW>(to, own); }
-      const bool there = row < j.lq, bad = *wait.failed;
+      const bool there = row < j.lq, bad = wait.failed();
       if (a.pieces > 1) {      // the share: o as it is, with its maximum and sum
         const long long slot = ((long long)j.piece * a.hq + j.h) * a.nq + j.q0 + row;
         if (there) a.part_ml[slot] = make_float2(m - head, bad ? NAN : l);
@@ -476,7 +471,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
   constexpr int tile_bytes = G::kSubs * (int)G::kSub, R = G::kRing;
   Tail* tail = reinterpret_cast<Tail*>(smem + (2 + R) * tile_bytes);
   const uint32_t sq = smem_addr(smem), sg = sq + tile_bytes, ring = sg + tile_bytes, bar0 = smem_addr(tail->bars);
-  const Wait wait{&tail->failed, a.wait_tries};
+  const Wait wait{smem_addr(&tail->failed), a.wait_tries};
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
@@ -508,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       int g = -1;
       for (int job = 0;; ++job) {
         need(bar(kdqQ), job & 1);
-        const int n = __shfl_sync(0xffffffffu, *wait.failed ? 0 : tail->tiles[job & 1], 0);
+        const int n = __shfl_sync(0xffffffffu, wait.failed() ? 0 : tail->tiles[job & 1], 0);
         if (n == 0) break;
         for (int i = -1; i < n; ++i) {
           const bool more = i + 1 < n;
@@ -547,47 +542,40 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
       commit(on, bar(kdqDone));      // no matrix instruction is under way when the CTA ends
       wait.end(bar(kdqDone), 0);
     } else if (warp == kLoadWarp) {
-      Loader<TERMS, DW> ld{lane, bar(kdqFix)};
-      int g = 0, job = 0;         // tiles, and jobs with any, whose copies were issued
-      bool ok = true;             // the same for all lanes
-      auto need = [&](uint32_t b, uint32_t parity) { ok = wait.whole_warp(b, parity) && ok; };
-      auto pass = [&](Job& j) {      // after a failure: the job's rows, without any tile
-        ok = ok && !__any_sync(0xffffffffu, *wait.failed);
-        if (!ok) { j.n = min(j.n, 0); j.n0 = j.n1 = 0; }
-      };
+      Loader<TERMS, DW> ld{lane, bar(kdqFix), wait};
+      int g = 0, job = 0, issued = 0, issued_q = 0;         // tiles, and jobs with any; those whose copies the first lane has issued
+      bool stop = false;          // after a failure: jobs without any tile
       for (int m = 0, index = blockIdx.x;; ++m) {
         Job j = dq_job(a, index);
-        pass(j);
+        if (stop) { j.n = min(j.n, 0); j.n0 = j.n1 = 0; }
         const int kvh = j.h / a.group;
         if (!publish_job(tail, m, j, bar(kdqJob), bar(kdqJobFree), lane, wait)) break;
         if (j.n < 0) break;
-        for (int i = 0; ok && i < 2 * j.n; ++i) {
+        for (int i = 0; i < 2 * j.n; ++i, ++g) {
           if (i == 1) {      // behind the first tile of keys, which finds room earlier
-            if (job > 0) need(bar(kdqQFree), (job - 1) & 1);
-            if (!ok) break;
-            if (lane == 0) {
+            if (job > 0) ld.need(bar(kdqQFree), (job - 1) & 1);
+            if (ld.go()) {
               tail->tiles[job & 1] = j.n;
               expect(bar(kdqQ), 2 * tile_bytes);
               ld.copies(sq, &maps.q, j.q0 + j.row0, j.h, bar(kdqQ));
               ld.copies(sg, &maps.g, j.q0 + j.row0, j.h, bar(kdqQ));
+              ++issued_q;
             }
             __syncwarp();
-            ++job;
           }
-          if (g >= R) need(bar(kdqEmpty + g % R), (g / R - 1) & 1);
-          if (!ok) break;
+          if (g >= R) ld.need(bar(kdqEmpty + g % R), (g / R - 1) & 1);
           const int r = j.k0 + (i >> 1) * kTile;
-          ok = ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kdqFull + g % R), j.lk - r, !(i & 1), wait);
-          g += ok;
+          issued += ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.v : &maps.k, j.c0 + r, kvh, bar(kdqFull + g % R), j.lk - r, !(i & 1));
         }
-        if (lane == 0) index = (int)gridDim.x + atomicAdd(a.queue, 1);
-        index = __shfl_sync(0xffffffffu, index, 0);
+        job += j.n > 0;
+        index = next_index(a.queue, gridDim.x, a.jobs, lane);
+        stop = __any_sync(0xffffffffu, wait.failed());
       }
       // no copy is under way when the CTA ends
-      if (ok && job > 0) need(bar(kdqQFree), (job - 1) & 1);
-      for (int t = max(0, g - R); t < g; ++t) wait.end(bar(kdqFull + t % R), (t / R) & 1);
-      if (job > 0) wait.end(bar(kdqQ), (job - 1) & 1);
-      if (ok && lane == 0) { tail->tiles[job & 1] = 0; arrive(bar(kdqQ)); }      // no more jobs
+      if (job > 0) ld.need(bar(kdqQFree), (job - 1) & 1);
+      for (int t = max(0, issued - R); t < issued; ++t) wait.end(bar(kdqFull + t % R), (t / R) & 1);
+      if (issued_q > 0) wait.end(bar(kdqQ), (issued_q - 1) & 1);
+      if (ld.go()) { tail->tiles[job & 1] = 0; arrive(bar(kdqQ)); }      // no more jobs
       __syncwarp();
     }
   } else {
@@ -673,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, 1) dq_kernel(const PackedArgs a, con
         wait(bar(kdqOut), job & 1);
         fence_after();
       }
-      const float f = *wait.failed ? NAN : f0;
+      const float f = wait.failed() ? NAN : f0;
       const long long at_row = ((long long)(j.q0 + row) * a.hq + j.h) * d;
       auto put = [&](auto* dst) {
         if constexpr (TERMS == 3) {
@@ -743,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
   float* stats = reinterpret_cast<float*>(smem + (2 + R) * tile_bytes);      // [2][128] -lse in log2, [2][128] -delta
   Tail* tail = reinterpret_cast<Tail*>(stats + 4 * kTile);
   const uint32_t sk = smem_addr(smem), sv = sk + tile_bytes, ring = sv + tile_bytes, bar0 = smem_addr(tail->bars);
-  const Wait wait{&tail->failed, a.wait_tries};
+  const Wait wait{smem_addr(&tail->failed), a.wait_tries};
   auto bar = [&](int k) { return bar0 + 8 * k; };
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (warp == kMmaWarp) alloc_tmem(&tail->tmem);
@@ -774,7 +762,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       int g = -1;
       for (int job = 0;; ++job) {
         need(bar(kkvK), job & 1);
-        const int n = __shfl_sync(0xffffffffu, *wait.failed ? 0 : tail->tiles[job & 1], 0);
+        const int n = __shfl_sync(0xffffffffu, wait.failed() ? 0 : tail->tiles[job & 1], 0);
         if (n == 0) break;
         for (int i = -1; i < n; ++i) {
           const bool more = i + 1 < n;
@@ -817,45 +805,38 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
       commit(on, bar(kkvDone));      // no matrix instruction is under way when the CTA ends
       wait.end(bar(kkvDone), 0);
     } else if (warp == kLoadWarp) {
-      Loader<TERMS, DW> ld{lane, bar(kkvFix)};
-      int g = 0, job = 0;         // as in dq_kernel
-      bool ok = true;
-      auto need = [&](uint32_t b, uint32_t parity) { ok = wait.whole_warp(b, parity) && ok; };
-      auto pass = [&](Job& j) {      // after a failure: the job's rows, without any tile
-        ok = ok && !__any_sync(0xffffffffu, *wait.failed);
-        if (!ok) { j.n = min(j.n, 0); j.n0 = j.n1 = 0; }
-      };
+      Loader<TERMS, DW> ld{lane, bar(kkvFix), wait};
+      int g = 0, job = 0, issued = 0, issued_k = 0;         // as in dq_kernel
+      bool stop = false;
       for (int m = 0, index = blockIdx.x;; ++m) {
         Job j = dkv_job(a, index);
-        pass(j);
+        if (stop) { j.n = min(j.n, 0); j.n0 = j.n1 = 0; }
         if (!publish_job(tail, m, j, bar(kkvJob), bar(kkvJobFree), lane, wait)) break;
         if (j.n < 0) break;
-        for (int i = 0; ok && i < 2 * j.n; ++i) {
+        for (int i = 0; i < 2 * j.n; ++i, ++g) {
           if (i == 1) {
-            if (job > 0) need(bar(kkvKFree), (job - 1) & 1);
-            if (!ok) break;
-            if (lane == 0) {
+            if (job > 0) ld.need(bar(kkvKFree), (job - 1) & 1);
+            if (ld.go()) {
               tail->tiles[job & 1] = j.n;
               expect(bar(kkvK), 2 * tile_bytes);
               ld.copies(sk, &maps.k, j.c0 + j.row0, j.h, bar(kkvK));
               ld.copies(sv, &maps.v, j.c0 + j.row0, j.h, bar(kkvK));
+              ++issued_k;
             }
             __syncwarp();
-            ++job;
           }
-          if (g >= R) need(bar(kkvEmpty + g % R), (g / R - 1) & 1);
-          if (!ok) break;
+          if (g >= R) ld.need(bar(kkvEmpty + g % R), (g / R - 1) & 1);
           const int t = j.j0 + (i >> 1), hq = j.h * a.group + t / j.per, b = j.i0 + (t % j.per) * kTile;
-          ok = ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.g : &maps.q, j.q0 + b, hq, bar(kkvFull + g % R), j.lq - b, true, wait);
-          g += ok;
+          issued += ld.tile(ring + (g % R) * tile_bytes, (i & 1) ? &maps.g : &maps.q, j.q0 + b, hq, bar(kkvFull + g % R), j.lq - b, true);
         }
-        if (lane == 0) index = (int)gridDim.x + atomicAdd(a.queue + 1, 1);
-        index = __shfl_sync(0xffffffffu, index, 0);
+        job += j.n > 0;
+        index = next_index(a.queue + 1, gridDim.x, a.jobs, lane);
+        stop = __any_sync(0xffffffffu, wait.failed());
       }
-      if (ok && job > 0) need(bar(kkvKFree), (job - 1) & 1);
-      for (int t = max(0, g - R); t < g; ++t) wait.end(bar(kkvFull + t % R), (t / R) & 1);
-      if (job > 0) wait.end(bar(kkvK), (job - 1) & 1);
-      if (ok && lane == 0) { tail->tiles[job & 1] = 0; arrive(bar(kkvK)); }      // no more jobs
+      if (job > 0) ld.need(bar(kkvKFree), (job - 1) & 1);
+      for (int t = max(0, issued - R); t < issued; ++t) wait.end(bar(kkvFull + t % R), (t / R) & 1);
+      if (issued_k > 0) wait.end(bar(kkvK), (issued_k - 1) & 1);
+      if (ld.go()) { tail->tiles[job & 1] = 0; arrive(bar(kkvK)); }      // no more jobs
       __syncwarp();
     } else {
       const int r0 = (warp - kLoadWarp - 1) * 32 + lane;
@@ -967,7 +948,7 @@ __global__ void __launch_bounds__(kThreads, 1) dkv_kernel(const PackedArgs a, co
         wait(bar(kkvOut), job & 1);
         fence_after();
       }
-      const bool there = row < j.lk, bad = *wait.failed;
+      const bool there = row < j.lk, bad = wait.failed();
       const long long at = ((long long)(j.c0 + row) * a.hk + j.h) * d;
 #pragma unroll
       for (int which = 0; which < 2; ++which) {

@@ -31,42 +31,47 @@ __device__ __forceinline__ bool test_bar(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 // Every wait ends: after `tries` tries, or when another one of this CTA has run out.  From then on no copy is issued, jobs are passed on without
-// tiles and their rows written as NaN, and the CTA ends behind what is under way (end), where it tells the host (report).  The code of a wait
-// is as short as this: with a clock in it the kernels took up to a tenth longer.
+// tiles and their rows written as NaN, and the CTA ends behind what is under way (end), where it tells the host (report).  What stands in a wait
+// shows: with the first try as one of the loop's dk and dv of 8,192 rows, 9 x 64, take 364 us instead of 351, with a clock in the loop the forward
+// kernel of 24 structures of 150 to 900 rows 99 instead of 92.
 struct Wait {
-  volatile int* failed;      // in shared memory
+  uint32_t failed_at;        // the word of shared memory that says so
   int tries;
-  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
-    for (int left = tries; !test_bar(bar, parity);)
-      if (--left < 0 || *failed) { *failed = 1; return false; }
-    return true;
+  __device__ __forceinline__ bool failed() const {
+    uint32_t x;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(x) : "r"(failed_at) : "memory");
+    return x != 0;
   }
-  // The loading warp's, which issues nothing behind a failure: a slot may have been given back by products that did not wait for its tile, and its
-  // copy may still be under way.  With negative tries, for tests, what is not over at once has run out.
-  __device__ __forceinline__ bool whole_warp(uint32_t bar, uint32_t parity) const {
-    bool ok;
-    if (tries < 0) {
-      uint32_t now;
-      asm volatile(
-          "{\n\t.reg .pred p;\n\t"
-          "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-          "selp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(now) : "r"(bar), "r"(parity) : "memory");
-      ok = now != 0;
-      if (!ok) *failed = 1;
-    } else {
-      ok = (*this)(bar, parity);
-    }
-    return __all_sync(0xffffffffu, ok && !*failed);
+  __device__ __forceinline__ void fail() const { asm volatile("st.volatile.shared.u32 [%0], 1;" ::"r"(failed_at) : "memory"); }
+  __device__ __forceinline__ bool operator()(uint32_t bar, uint32_t parity) const {
+    if (test_bar(bar, parity)) return true;
+    for (int left = tries; --left >= 0 && !failed();)
+      if (test_bar(bar, parity)) return true;
+    fail();
+    return false;
+  }
+  // The loading warp's.  With negative tries, for tests, what is not over at once has run out.
+  __device__ __forceinline__ bool of_loader(uint32_t bar, uint32_t parity) const {
+    if (tries >= 0) return (*this)(bar, parity);
+    uint32_t now;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(now) : "r"(bar), "r"(parity) : "memory");
+    if (!now) fail();
+    return now != 0;
   }
   // The waits that hold after a failure too: for what is under way, and for the next job.  What they wait for comes once the waits above have
   // ended; kEndTries is the bound for what should not be.
   __device__ __forceinline__ bool end(uint32_t bar, uint32_t parity) const {
-    for (int left = kEndTries; !test_bar(bar, parity);)
-      if (--left < 0) { *failed = 1; return false; }
-    return true;
+    if (test_bar(bar, parity)) return true;
+    for (int left = kEndTries; --left >= 0;)
+      if (test_bar(bar, parity)) return true;
+    fail();
+    return false;
   }
   __device__ __forceinline__ void report(int* error) const {
-    if (*failed) { *const_cast<volatile int*>(error) = 1; __threadfence_system(); }
+    if (failed()) { *const_cast<volatile int*>(error) = 1; __threadfence_system(); }
   }
 };
 __device__ __forceinline__ void init_bar(uint32_t bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
@@ -283,36 +288,42 @@ __device__ __forceinline__ void expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 // The whole loading warp calls it.  rows: how many of the tile's 128 rows belong to the structure; where `clear`, the others are cleared
-// (through `fix`, a barrier of this warp's own, and its parity).  False where that wait has run out: the tile is not handed over then.
+// (through `fix`, a barrier of this warp's own, and its parity).  Behind a failure nothing is issued any more: a slot may have been given back by
+// products that did not wait for its tile, and its copy may still be under way.
 template <int TERMS, int DW> struct Loader {
   static constexpr uint32_t kSub = Geometry<TERMS, DW>::kSub;
   static constexpr int subs = Geometry<TERMS, DW>::kSubs;
   int lane;
-  uint32_t fix, parity = 0;
+  uint32_t fix;
+  Wait wait;
+  uint32_t parity = 0;
+  bool ok = true;            // no wait has run out
+  __device__ __forceinline__ void need(uint32_t bar, uint32_t phase) { ok = wait.of_loader(bar, phase) && !wait.failed() && ok; }
+  __device__ __forceinline__ bool go() const { return lane == 0 && ok; }      // whether this lane issues
   __device__ __forceinline__ void copies(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t bar) const {
     for (int x = 0; x < subs; ++x) tma(dst + x * kSub, map, TERMS == 1 ? 64 * x : 0, row, TERMS == 1 ? head : 3 * head + x, bar);
   }
-  __device__ __forceinline__ bool tile(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t full, int rows, bool clear, const Wait& wait) {
+  // returns 1 in the first lane where the tile was handed over or is on its way
+  __device__ __forceinline__ int tile(uint32_t dst, const CUtensorMap* map, int row, int head, uint32_t full, int rows, bool clear) {
+    const bool issue = go();
     if (!clear || rows >= kTile) {
-      if (lane == 0) { expect(full, subs * kSub); copies(dst, map, row, head, full); }
+      if (issue) { expect(full, subs * kSub); copies(dst, map, row, head, full); }
       __syncwarp();
-      return true;
+      return issue;
     }
-    if (lane == 0) { expect(fix, subs * kSub); copies(dst, map, row, head, fix); }
+    if (issue) { expect(fix, subs * kSub); copies(dst, map, row, head, fix); }
     __syncwarp();
-    if (!wait.whole_warp(fix, parity)) {
-      wait.end(fix, parity);
-      return false;
-    }
+    need(fix, parity);
+    if (issue && !ok) wait.end(fix, parity);
     parity ^= 1;
     for (int x = 0; x < subs; ++x)
       for (int b = rows * Geometry<TERMS, DW>::kRow + lane * 16; b < (int)kSub; b += 512)
         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + x * kSub + b), "r"(0) : "memory");
     fence_smem();
     __syncwarp();
-    if (lane == 0) arrive(full);
+    if (issue && ok) arrive(full);
     __syncwarp();
-    return true;
+    return issue && ok;
   }
 };
 
