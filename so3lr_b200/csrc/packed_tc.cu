@@ -8,10 +8,10 @@
 // dS live in tensor memory: P and dS go back there packed to 16 bits, and are the A operand of the next product, so shared memory
 // carries q, k, v and g only.
 //
-// Bound by the tensor cores beside the elementwise work of eight warps.  8,192 rows, 9 heads x 128 bfloat16: forward 275 us (1.12 PFLOP/s), dq 385 (1.20),
-// dk and dv 444 (1.39; cuBLAS 1.67), the tensor cores busy 62, 59 and 71 % of the time and the schedulers 40 to 51 %.  With 64 values a head
-// a tile has half of the products, each of them no shorter for its 64 columns, and the same elementwise work (247, 300, 365 us; tensor 32, 36,
-// 40 % busy, schedulers 48 to 55 %): what is left is the latency of two warps per scheduler.  float32, 9 x 32: tensor 54 to 62 %.
+// Bound by the tensor cores beside the elementwise work of eight warps.  8,192 rows, 9 heads x 128 bfloat16: forward 261 us (1.18 PFLOP/s), dq 382 (1.21),
+// dk and dv 444 (1.39; cuBLAS 1.67), the tensor cores busy 61, 59 and 73 % of the time and the schedulers 40 to 53 %.  With 64 values a head
+// a tile has half of the products, each of them no shorter for its 64 columns, and the same elementwise work (237, 297, 351 us; tensor 31, 37,
+// 42 % busy, schedulers 49 to 56 %): what is left is the latency of two warps per scheduler.  float32, 9 x 32: 425, 517, 796 us, tensor 55 to 66 %.
 // The two reverse kernels form seven products where one with atomic sums would form five; they give the same bits every time.
 #include "packed_tc.cuh"
 
@@ -82,7 +82,7 @@ __device__ __forceinline__ unsigned char* aligned_smem(unsigned char* p) { retur
 // A CTA stays on its SM and works through jobs, so that a job's first tiles come in and its first products run while the last results of the
 // one before leave: with a CTA per job its start and end took 5 to 6 us, now 2 to 3.  dq / dk and dv, a CTA per job -> this, us: 24 structures of 150 to
 // 900 rows, 16 heads x 64, 124 / 147 -> 100 / 121; 64 of 64 to 128, 8 x 128, 28 / 32 -> 20 / 26; 8 causal ones of 2,000, 40 x 128, 613 / 588 ->
-// 520 / 592; one of 8,192, 9 x 64, 290 / 351 -> 306 / 366 (a job of 64 tiles has no start to hide).  The loading warp takes jobs from a queue, the
+// 520 / 592; one of 8,192, 9 x 64, 290 / 351 -> 297 / 351 (a job of 64 tiles has no start to hide).  The loading warp takes jobs from a queue, the
 // longest first, and passes them on through shared memory (equal shares instead: SMs differ in their pace by up to 15 %; 5,000 rows, 4 x 32
 // float32, dk and dv 187 us with the queue, 219 without).
 // Jobs are passed on after a failure too, so that the rows of all of them are written; false where that is at an end as well.
@@ -141,9 +141,9 @@ template <int TERMS, int DW, int TILES> struct Forward {
   static constexpr int kRing = TILES == 2 ? Geometry<TERMS, DW>::kRing : TERMS == 3 ? 3 : DW == 128 ? 2 : 4;
   static constexpr int kSmem = 1024 + (TILES + kRing) * Geometry<TERMS, DW>::kSubs * (int)Geometry<TERMS, DW>::kSub + (int)sizeof(Tail);
   static_assert(TILES == 2 || kSmem <= 232448 / 2, "two CTAs on an SM");
-  // Whether CTAs take jobs from a queue, or have one each.  us, one / queue: 8 causal prompts of 2,000, 40 heads x 128, 482 / 431; 24 structures of 150 to
-  // 900, 16 x 64, 94 / 87; one of 8,192, 9 x 64, 236 / 247; but float32, whose registers spill over what a job takes, 32 of 256, 4 x 32, 15.3 /
-  // 17.1, one of 5,000 100 / 117.
+  // Whether CTAs take jobs from a queue, or have one each.  us, one / queue: 8 causal prompts of 2,000, 40 heads x 128, 509 / 452; 24 structures of 150 to
+  // 900, 16 x 64, 104 / 96; one of 8,192, 9 x 128 260 / 261, 9 x 64 234 / 237; but float32, whose registers spill over what a job takes, 32 of 256,
+  // 4 x 32, 15.1 / 16.8, one of 5,000 101 / 113, one of 8,192, 9 x 32, 425 / 486.
   static constexpr bool kQueued = TERMS == 1;
 };
 template <typename T, int TERMS, int DW, int TILES>
