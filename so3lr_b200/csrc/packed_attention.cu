@@ -233,7 +233,7 @@ int waits(PackedArgs* p) {
 }
 constexpr int64_t kQueueBytes = 16;      // behind these: PackedArgs::queue, and in the reverse pass of float16 largest and size_g
 int64_t size_bytes(const int32_t* im, const so3lr_b200_attention_shape* a) {
-  return a->type == kF16 ? ((int64_t)im[kN] * a->heads_kv * 2 + a->rows_q * a->heads_q) * 4 : 0;
+  return a->type == kF16 && on_tensor_cores(im, a, true) ? ((int64_t)im[kN] * a->heads_kv * 2 + a->rows_q * a->heads_q) * 4 : 0;
 }
 
 const int4* table(const int32_t* im, const int32_t* dev, int field) { return reinterpret_cast<const int4*>(dev + im[field]); }
@@ -266,7 +266,7 @@ template <typename T>
 int reverse(cudaStream_t st, PackedArgs p, const int32_t* im, const int32_t* dev, const so3lr_b200_attention_shape* a, void* workspace) {
   char* behind = static_cast<char*>(workspace) + whole_bytes(im, a, true);
   if (on_tensor_cores(im, a, true)) { p.queue = reinterpret_cast<int*>(behind); behind += kQueueBytes; }
-  if (kShifted<T>) {
+  if (size_bytes(im, a)) {
     p.largest = reinterpret_cast<unsigned*>(behind);
     p.size_g = reinterpret_cast<float*>(p.largest + (int64_t)im[kN] * p.hk * 2);
   }

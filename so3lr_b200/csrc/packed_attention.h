@@ -37,7 +37,7 @@ struct PackedArgs {
   int part_rows = 0;            // most rows of a structure: tokens times heads of a group
   int pieces = 1;               // into which an item's walk is cut; each leaves its share in part_o (pieces, hq, nq, d) and part_ml, or
   float* share[3] = {};         // (reverse) in share: (pieces, rows, heads, d) of dq, dk, dv
-  // reverse pass of float16, else null: bits of the largest |g| and of sqrt(d) times the largest |v_jc| (structure, key head, 2), and |g| of every row (hq, nq)
+  // reverse pass of float16 on the tensor cores, else null: bits of the largest |g| and of sqrt(d) times the largest |v_jc| (structure, key head, 2), and |g| of every row (hq, nq)
   unsigned* largest = nullptr;
   float* size_g = nullptr;
   int structures = 0;
@@ -56,9 +56,10 @@ struct PackedArgs {
 constexpr int kPackTile = 64;   // rows of a tile of the mma kernels
 
 // float16 keeps its 11 bits between 2^-14 and 2^16 only, and dS = P (dP - delta) is as small as the cotangents of a mean loss over thousands
-// of keys, or as large as those of a scaled one.  |dS| <= |g| |v| + |g| |o| <= 2 |g| sqrt(d) max |v_jc|: the exponent of two that puts this
-// bound into [2^14, 2^15).  dS goes into its products times that power, which leaves with the factor `scale` at their end: exact, and no instruction more.
-// A row of queries has its own ahead of dS k; ahead of dS^T q, which sums over queries, it is that of the structure and key head.
+// of keys, or as large as those of a scaled one.  It goes into its products times a power of two, which leaves with the factor `scale` at their
+// end: exact.  The warp-level kernels, whose sums are in registers, take it from the values (shift_rows).  On the tensor cores it is known ahead and
+// costs no instruction: |dS| <= |g| |v| + |g| |o| <= 2 |g| sqrt(d) max |v_jc|, and the exponent that puts this bound into [2^14, 2^15) is a query
+// row's own ahead of dS k, and one of a structure and key head ahead of dS^T q, which sums over queries.
 template <typename T> constexpr bool kShifted = std::is_same<T, __half>::value;
 // The forward kernels' probabilities relative to a row's largest take a power of two as well, so that what many keys far below the largest add up to
 // is not lost in the last steps of float16: its largest number, 65504, leaves room for 2^15.  On the tensor cores the reference may lag behind

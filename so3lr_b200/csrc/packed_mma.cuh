@@ -650,23 +650,23 @@ __global__ void __launch_bounds__(256) delta_kernel(const PackedArgs a, int rows
   for (int x = width >> 1; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
   if (r < rows && part == 0) a.delta[(long long)h * a.nq + r] = sum;
 }
-// The same with the sizes of g and v (PackedArgs::largest, size_g): a CTA per 16 rows of a tile of 128 queries and up to 64 heads, and behind these
-// CTAs for the keys.  A warp takes two rows of 32 / width heads at a time, so that no thread divides and a head's largest stays in a
-// register.  The order of the atomics, one a CTA and head, does not matter.  |v| is bounded by sqrt(d) times its largest value, which
-// needs no sum.
-constexpr int kSizeRows = 16, kSizeHeads = 64;
+// The same with the sizes of g and v (PackedArgs::largest, size_g), for the tensor-core kernels of float16: a CTA per 128 / parts rows of a tile of 128
+// queries and up to 64 heads, and behind these CTAs for the keys.  A warp takes two rows of 32 / width heads at a time, so that no thread divides
+// and a head's largest stays in a register.  The order of the atomics, one a CTA and head, does not matter.  |v| is bounded by sqrt(d) times
+// its largest value, which needs no sum.  (24 structures of 150 to 900 rows, 16 heads x 64: 26 us, where delta alone takes 16.)
+constexpr int kSizeHeads = 64;
 template <typename T>
-__global__ void __launch_bounds__(256) delta_sizes_kernel(const PackedArgs a, const int4* items_q, long long ctas_q, const int4* items_kv, int log_width) {
-  constexpr int V = 16 / (int)sizeof(T), kParts = 128 / kSizeRows;
+__global__ void __launch_bounds__(256) delta_sizes_kernel(const PackedArgs a, const int4* items_q, long long ctas_q, const int4* items_kv, int log_width, int parts) {
+  constexpr int V = 16 / (int)sizeof(T);
   __shared__ unsigned most[kSizeHeads];
   if (a.queue && blockIdx.x == 0 && threadIdx.x < 2) a.queue[threadIdx.x] = 0;
   const bool of_v = blockIdx.x >= ctas_q;
   const int all = of_v ? a.hk : a.hq, blocks = (all + kSizeHeads - 1) / kSizeHeads, index = (int)(blockIdx.x - (of_v ? ctas_q : 0));
-  const int4 item = (of_v ? items_kv : items_q)[index / kParts / blocks];
+  const int4 item = (of_v ? items_kv : items_q)[index / parts / blocks];
   const int* start = of_v ? a.start_kv : a.start_q;
-  const int row0 = item.y * 128 + index % kParts * kSizeRows, first = start[item.x] + row0, rows = min(kSizeRows, start[item.x + 1] - first);
+  const int per = 128 / parts, row0 = item.y * 128 + index % parts * per, first = start[item.x] + row0, rows = min(per, start[item.x + 1] - first);
   if (rows <= 0) return;
-  const int h0 = index / kParts % blocks * kSizeHeads, heads = min(kSizeHeads, all - h0), width = 1 << log_width;
+  const int h0 = index / parts % blocks * kSizeHeads, heads = min(kSizeHeads, all - h0), width = 1 << log_width;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = lane & (width - 1);
   if (threadIdx.x < kSizeHeads) most[threadIdx.x] = 0;
   __syncthreads();
@@ -674,43 +674,45 @@ __global__ void __launch_bounds__(256) delta_sizes_kernel(const PackedArgs a, co
   for (int hb = 0; hb < heads; hb += 32 >> log_width) {      // the same trips for all lanes
     const int hh = hb + (lane >> log_width), h = h0 + hh;
     float size = 0.f;
-    uint4 g[2], o[2], rest[2];
+    for (int row = warp; row < rows + warp; row += 16) {
+      uint4 g[2], o[2], rest[2];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const long long r = first + warp + 8 * u;
-      g[u] = o[u] = rest[u] = make_uint4(0, 0, 0, 0);
-      if (warp + 8 * u < rows && hh < heads && on) {
-        const Rows& x = of_v ? a.v : a.g;
-        g[u] = load16<T>(x.p, r * x.row + h * x.head + part * V);
-        if (!of_v) {
-          const long long at = (r * a.hq + h) * a.d + part * V;
-          o[u] = load16<T>(a.o.p, at);
-          if (a.out_rest) rest[u] = load16<T>(a.out_rest, at);
+      for (int u = 0; u < 2; ++u) {
+        const long long r = first + row + 8 * u;
+        g[u] = o[u] = rest[u] = make_uint4(0, 0, 0, 0);
+        if (row + 8 * u < rows && hh < heads && on) {
+          const Rows& x = of_v ? a.v : a.g;
+          g[u] = load16<T>(x.p, r * x.row + h * x.head + part * V);
+          if (!of_v) {
+            const long long at = (r * a.hq + h) * a.d + part * V;
+            o[u] = load16<T>(a.o.p, at);
+            if (a.out_rest) rest[u] = load16<T>(a.out_rest, at);
+          }
         }
       }
-    }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      // one that is not finite spoils its rows whatever their power of two: left out
-      if (of_v) {
-        const uint32_t xs[4] = {g[u].x, g[u].y, g[u].z, g[u].w};
+      for (int u = 0; u < 2; ++u) {
+        // one that is not finite spoils its rows whatever their power of two: left out
+        if (of_v) {
+          const uint32_t xs[4] = {g[u].x, g[u].y, g[u].z, g[u].w};
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 x = Half<T>::unpack(xs[e]);
-          if (isfinite(x.x)) size = fmaxf(size, fabsf(x.x));
-          if (isfinite(x.y)) size = fmaxf(size, fabsf(x.y));
+          for (int e = 0; e < 4; ++e) {
+            const float2 x = Half<T>::unpack(xs[e]);
+            if (isfinite(x.x)) size = fmaxf(size, fabsf(x.x));
+            if (isfinite(x.y)) size = fmaxf(size, fabsf(x.y));
+          }
+        } else {
+          float sum = 0.f, square = 0.f;
+          dot16<T>(g[u], o[u], rest[u], sum, square);
+          for (int x = width >> 1; x; x >>= 1) { sum += __shfl_xor_sync(0xffffffffu, sum, x); square += __shfl_xor_sync(0xffffffffu, square, x); }
+          const float norm = sqrtf(square);
+          if (row + 8 * u < rows && hh < heads && part == 0) {
+            const long long at = (long long)h * a.nq + first + row + 8 * u;
+            a.delta[at] = sum;
+            a.size_g[at] = norm;
+          }
+          if (isfinite(norm)) size = fmaxf(size, norm);
         }
-      } else {
-        float sum = 0.f, square = 0.f;
-        dot16<T>(g[u], o[u], rest[u], sum, square);
-        for (int x = width >> 1; x; x >>= 1) { sum += __shfl_xor_sync(0xffffffffu, sum, x); square += __shfl_xor_sync(0xffffffffu, square, x); }
-        const float norm = sqrtf(square);
-        if (warp + 8 * u < rows && hh < heads && part == 0) {
-          const long long at = (long long)h * a.nq + first + warp + 8 * u;
-          a.delta[at] = sum;
-          a.size_g[at] = norm;
-        }
-        if (isfinite(norm)) size = fmaxf(size, norm);
       }
     }
     if (of_v) {
@@ -721,6 +723,34 @@ __global__ void __launch_bounds__(256) delta_sizes_kernel(const PackedArgs a, co
   }
   __syncthreads();
   if (threadIdx.x < heads) atomicMax(a.largest + ((long long)item.x * a.hk + (h0 + threadIdx.x) / (of_v ? 1 : a.group)) * 2 + of_v, most[threadIdx.x]);
+}
+
+// float16: the power of two of dS (grad_shift) from the values themselves, of every row of the product.  A row's first value that is not zero sets it, and
+// it falls where a value would pass 2^15; what was summed so far is scaled along, exactly.  `v`: rows a and b of this thread, shared by four
+// lanes, times the present powers.  Not above 2^80, with which float32 holds any |dS| of float16 rows (2^39).  (With sizes found ahead as for
+// the tensor cores: 512 structures of 10 to 40, 4 x 32, 48 us a training step instead of 35, 50,000 of two rows 2,550 instead of 1,240.)
+struct RowShift {
+  int shift = 0;
+  float top = 0.f;
+};
+template <int NT, int DP> __device__ __forceinline__ void shift_rows(float (&v)[NT][4], float (&acc)[DP / 8][4], RowShift& a, RowShift& b) {
+  float xa = 0.f, xb = 0.f;
+#pragma unroll
+  for (int n = 0; n < NT; ++n) { xa = fmaxf(xa, fmaxf(fabsf(v[n][0]), fabsf(v[n][1]))); xb = fmaxf(xb, fmaxf(fabsf(v[n][2]), fabsf(v[n][3]))); }
+  if (!__any_sync(0xffffffffu, xa > a.top || xb > b.top)) return;
+#pragma unroll
+  for (int x = 1; x < 4; x <<= 1) { xa = fmaxf(xa, __shfl_xor_sync(0xffffffffu, xa, x)); xb = fmaxf(xb, __shfl_xor_sync(0xffffffffu, xb, x)); }
+  auto factor = [](float x, RowShift& r) {
+    if (!(x > r.top)) return 1.f;
+    const int by = min(14 - ((int)(__float_as_uint(x) >> 23) - 127), 80 - r.shift);
+    r.shift += by; r.top = 32768.f;
+    return two_to(max(by, -126));
+  };
+  const float fa = factor(xa, a), fb = factor(xb, b);
+#pragma unroll
+  for (int n = 0; n < NT; ++n) { v[n][0] *= fa; v[n][1] *= fa; v[n][2] *= fb; v[n][3] *= fb; }
+#pragma unroll
+  for (int n = 0; n < DP / 8; ++n) { acc[n][0] *= fa; acc[n][1] *= fa; acc[n][2] *= fb; acc[n][3] *= fb; }
 }
 
 // dq of a tile of 16 NW queries of one head
@@ -751,18 +781,13 @@ __global__ void __launch_bounds__(32 * NW) dq_kernel(const PackedArgs a) {
   const int wr = row0 + warp * 16, ra = wr + (lane >> 2), rb = ra + 8, off = lk - lq, big = 0x7fffffff;
   const int lim_a = a.causal ? ra + off : big, lim_b = a.causal ? rb + off : big, lim_lo = a.causal ? wr + off : big, lim_hi = a.causal ? wr + 15 + off : big;
   const long long at_row = (long long)h * a.nq + q0;
-  int shift_a = 0, shift_b = 0;      // of the rows' dS (grad_shift)
-  if constexpr (kShifted<T>) {
-    const float v = __uint_as_float(a.largest[((long long)s * a.hk + kvh) * 2 + 1]);
-    if (ra < lq) shift_a = grad_shift(a.size_g[at_row + ra], v);
-    if (rb < lq) shift_b = grad_shift(a.size_g[at_row + rb], v);
-  }
   // rows that are not there: exp(-inf) = 0
-  const float ea = ra < lq ? a.lse[at_row + ra] - shift_a : INFINITY, eb = rb < lq ? a.lse[at_row + rb] - shift_b : INFINITY;
+  const float ea = ra < lq ? a.lse[at_row + ra] : INFINITY, eb = rb < lq ? a.lse[at_row + rb] : INFINITY;
   const float da = ra < lq ? a.delta[at_row + ra] : 0.f, db = rb < lq ? a.delta[at_row + rb] : 0.f;
   float dq[DP / 8][4];
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) dq[n][0] = dq[n][1] = dq[n][2] = dq[n][3] = 0.f;
+  RowShift sh_a, sh_b;      // of the rows' dS and what was summed of them
   for (int it = 0; it < nt; ++it) {
     if (a.rev_stages == 2) { load(it + 1); copy_wait<1>(); } else { if (it > 0) load(it); copy_wait<0>(); }
     __syncthreads();
@@ -773,18 +798,20 @@ __global__ void __launch_bounds__(32 * NW) dq_kernel(const PackedArgs a) {
       product_nt<T, DP, NT>(p, sq + warp * 16 * L::kStride, sk + buf * BN * L::kStride, lane, cols);
       product_nt<T, DP, NT>(dp, sg + warp * 16 * L::kStride, sv + buf * BN * L::kStride, lane, cols);
       const bool mask = kb + BN > k1 || kb + BN - 1 > lim_lo;
+      const float ua = kShifted<T> ? sh_a.shift - ea : -ea, ub = kShifted<T> ? sh_b.shift - eb : -eb;      // P times the power of dS
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int j = kb + n * 8 + 2 * (lane & 3) + e;
-          float x = exp2f(fmaf(p[n][e], a.scale_log2, -ea)) * (dp[n][e] - da);
-          float y = exp2f(fmaf(p[n][2 + e], a.scale_log2, -eb)) * (dp[n][2 + e] - db);
+          float x = exp2f(fmaf(p[n][e], a.scale_log2, ua)) * (dp[n][e] - da);
+          float y = exp2f(fmaf(p[n][2 + e], a.scale_log2, ub)) * (dp[n][2 + e] - db);
           if (mask && (j >= k1 || j > lim_a)) x = 0.f;
           if (mask && (j >= k1 || j > lim_b)) y = 0.f;
           p[n][e] = x; p[n][2 + e] = y;
         }
       }
+      if constexpr (kShifted<T>) shift_rows<NT, DP>(p, dq, sh_a, sh_b);
       product_nn<T, DP, NT>(dq, p, sk + buf * BN * L::kStride, lane, cols);
     }
     __syncthreads();
@@ -795,7 +822,7 @@ __global__ void __launch_bounds__(32 * NW) dq_kernel(const PackedArgs a) {
     const int r = half ? rb : ra;
     if (r >= lq) continue;
     const long long at = ((long long)(q0 + r) * a.hq + h) * a.d;
-    const float f = kShifted<T> ? a.scale * two_to(-(half ? shift_b : shift_a)) : a.scale;
+    const float f = kShifted<T> ? a.scale * two_to(-(half ? sh_b.shift : sh_a.shift)) : a.scale;
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n) {
       const int c = n * 8 + 2 * (lane & 3);
@@ -822,12 +849,6 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
   const int kvh = index % a.hk, row0 = item.y * kRows, i0 = item.z, i1 = item.w;
   const int per = (max(i1 - i0, 0) + BN - 1) / BN, all = per * a.group, share = (all + a.pieces - 1) / a.pieces, j0 = min(all, piece * share);
   const int nt = min(share, all - j0);      // from tile j0 on
-  int shift = 0;                            // of the structure's dS (grad_shift)
-  if constexpr (kShifted<T>) {
-    const unsigned* most = a.largest + ((long long)s * a.hk + kvh) * 2;
-    shift = grad_shift(__uint_as_float(most[0]), __uint_as_float(most[1]));
-  }
-  const float un = kShifted<T> ? prob_unscale<T>() * two_to(shift) : 1.f;      // from 2^15 P to P times the power of dS
   load_rows<T, DP, kRows, kThreads>(sk, a.k, kvh, c0, row0, lk, a.d, tid);
   load_rows<T, DP, kRows, kThreads>(sv, a.v, kvh, c0, row0, lk, a.d, tid);
   auto load = [&](int it) {
@@ -839,7 +860,7 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
         const bool ok = b + tid < i1;
         const long long at = (long long)h * a.nq + q0 + b + tid;
         se[buf * BN + tid] = ok ? a.lse[at] - prob_shift<T>() : INFINITY;
-        se[(2 + buf) * BN + tid] = ok ? a.delta[at] * un : 0.f;
+        se[(2 + buf) * BN + tid] = ok ? a.delta[at] * prob_unscale<T>() : 0.f;
       }
     }
     copy_commit();
@@ -851,6 +872,7 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
   float dk[DP / 8][4], dv[DP / 8][4];
 #pragma unroll
   for (int n = 0; n < DP / 8; ++n) { dk[n][0] = dk[n][1] = dk[n][2] = dk[n][3] = 0.f; dv[n][0] = dv[n][1] = dv[n][2] = dv[n][3] = 0.f; }
+  RowShift sh_a, sh_b;
   for (int it = 0; it < nt; ++it) {
     if (a.rev_stages == 2) { load(it + 1); copy_wait<1>(); } else { if (it > 0) load(it); copy_wait<0>(); }
     __syncthreads();
@@ -861,6 +883,7 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
       product_nt<T, DP, NT>(p, sk + warp * 16 * L::kStride, sq + buf * BN * L::kStride, lane, cols);
       product_nt<T, DP, NT>(ds, sv + warp * 16 * L::kStride, sg + buf * BN * L::kStride, lane, cols);
       const bool mask = a.causal && ib < lim_hi;
+      const float pa = kShifted<T> ? two_to(sh_a.shift) : 1.f, pb = kShifted<T> ? two_to(sh_b.shift) : 1.f;
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int c = n * 8 + 2 * (lane & 3);
@@ -870,21 +893,22 @@ __global__ void __launch_bounds__(32 * NW) dkv_kernel(const PackedArgs a) {
           const int i = ib + c + (x & 1), lim = x < 2 ? lim_a : lim_b;
           float w = exp2f(fmaf(p[n][x], a.scale_log2, -((x & 1) ? e.y : e.x)));
           if (mask && i < lim) w = 0.f;
-          ds[n][x] = w == 0.f ? 0.f : w * fmaf(ds[n][x], un, -((x & 1) ? d.y : d.x));
+          ds[n][x] = w == 0.f ? 0.f : w * fmaf(ds[n][x], prob_unscale<T>(), -((x & 1) ? d.y : d.x)) * (x < 2 ? pa : pb);
           p[n][x] = w;
         }
       }
       product_nn<T, DP, NT>(dv, p, sg + buf * BN * L::kStride, lane, cols);
+      if constexpr (kShifted<T>) shift_rows<NT, DP>(ds, dk, sh_a, sh_b);
       product_nn<T, DP, NT>(dk, ds, sq + buf * BN * L::kStride, lane, cols);
     }
     __syncthreads();
   }
   copy_wait<0>();
-  const float f = kShifted<T> ? a.scale * two_to(-shift) : a.scale;
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
     const int r = half ? rb : ra;
     if (r >= lk) continue;
+    const float f = kShifted<T> ? a.scale * two_to(-(half ? sh_b.shift : sh_a.shift)) : a.scale;
     const long long at = ((long long)(c0 + r) * a.hk + kvh) * a.d;
 #pragma unroll
     for (int n = 0; n < DP / 8; ++n) {
@@ -987,21 +1011,24 @@ template <typename T> int packed_sum(cudaStream_t st, const PackedArgs& a, int p
 template <typename T> int packed_delta(cudaStream_t st, const PackedArgs& a, const int4* items_q, int n_q, const int4* items_kv, int n_kv) {
   int width = 1;
   while (width * (16 / (int)sizeof(T)) < a.d) width <<= 1;
-  // ahead of all else: the kernel of dk and dv reads it where there are no queries too
-  if (kShifted<T> && a.structures > 0) SO3LR_CUDA_CHECK(cudaMemsetAsync(a.largest, 0, (size_t)a.structures * a.hk * 2 * sizeof(unsigned), st));
   if (a.rows == 0) return kOk;
   if constexpr (kShifted<T>) {
-    auto per_item = [](int heads) { return 128 / packed::kSizeRows * (int64_t)((heads + packed::kSizeHeads - 1) / packed::kSizeHeads); };
-    const int64_t ctas_q = per_item(a.hq) * n_q, ctas = ctas_q + per_item(a.hk) * n_kv;
-    if (ctas > 0x7fffffff) return kTooLarge;
-    int log_width = 0;
-    while (1 << log_width < width) ++log_width;
-    packed::delta_sizes_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, items_q, ctas_q, items_kv, log_width);
-  } else {
-    const int64_t ctas = ((int64_t)a.rows * a.hq * width + 255) / 256;
-    if (ctas > 0x7fffffff) return kTooLarge;
-    packed::delta_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, a.rows, width);
+    if (a.largest) {
+      auto blocks = [](int heads) { return (int64_t)((heads + packed::kSizeHeads - 1) / packed::kSizeHeads); };
+      const int64_t whole = blocks(a.hq) * n_q + blocks(a.hk) * n_kv;
+      int parts = 8, log_width = 0;
+      while (parts > 1 && whole * parts > 16384) parts >>= 1;      // many structures, most of them short: CTAs without a row cost some 10 ns each
+      while (1 << log_width < width) ++log_width;
+      if (whole * parts > 0x7fffffff) return kTooLarge;
+      SO3LR_CUDA_CHECK(cudaMemsetAsync(a.largest, 0, (size_t)a.structures * a.hk * 2 * sizeof(unsigned), st));
+      packed::delta_sizes_kernel<T><<<(unsigned)(whole * parts), 256, 0, st>>>(a, items_q, blocks(a.hq) * n_q * parts, items_kv, log_width, parts);
+      count_launch();
+      return kOk;
+    }
   }
+  const int64_t ctas = ((int64_t)a.rows * a.hq * width + 255) / 256;
+  if (ctas > 0x7fffffff) return kTooLarge;
+  packed::delta_kernel<T><<<(unsigned)ctas, 256, 0, st>>>(a, a.rows, width);
   count_launch();
   return kOk;
 }

@@ -1,8 +1,8 @@
 """Gradients of structure_attention in float16 for cotangents of any size, against the formula in 64 bits.
 
 float16 has 11 bits down to 2^-14 and steps of 2^-24 below; a mean loss has cotangents of 1e-3 and less, a scaled one of 1e3 and more.  The kernels
-form dS times a power of two (a query row's own ahead of dS k, one of a structure and key head ahead of dS^T q) that brings
-2 |g| sqrt(d) max |v_jc|, which no |dS| passes, between 2^14 and 2^15.  So dS is off by 2^-11 of itself and by 2^-25 of that scale: 2^-38 of
+form dS times a power of two (on the tensor cores a query row's own ahead of dS k, one of a structure and key head ahead of dS^T q) that brings
+2 |g| sqrt(d) max |v_jc|, which no |dS| passes, between 2^14 and 2^15 (the warp-level ones: the largest |dS| so far).  So dS is off by 2^-11 of itself and by 2^-25 of that scale: 2^-38 of
 |g| sqrt(d) max |v_jc|.
 Bounds otherwise, with u = 2^-11: logits are off by (d + 4) 2^-24 of sum |q||k| (times scale: e), probabilities by 3 max e + 2^-20 + L 2^-24, o by a
 rounding of P (u, and 2^-25 of the row's largest one) and of the result with its rest (2^-22 |o|, or half a step of 2^-24), delta by that times

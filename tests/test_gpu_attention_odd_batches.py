@@ -54,3 +54,15 @@ def test_a_side_without_rows_whatever_memory_holds(lq, lk, dtype):
         assert all((x == 0).all() for x in d_), hex(word)
     assert all((x == 0).all() for x in train(q, k, v, g, packed))
     assert (structure_attention(q, k, v, packed) == 0).all()
+
+
+@pytest.mark.parametrize("d,lengths", [(64, [85, 40]), (32, [300]), (128, [60, 71]), (64, [150]), (128, [400])])
+@pytest.mark.parametrize("rising", [True, False])
+def test_gradients_that_grow_along_the_walk(d, lengths, rising):
+    """float16: cotangents and values over five powers of ten from the first row to the last, or the other way; some rows without any."""
+    n = sum(lengths)
+    t = torch.linspace(0, 1, n, device="cuda") if rising else torch.linspace(1, 0, n, device="cuda")
+    sizes = (10.0 ** (5 * t - 3))[:, None, None].clone()
+    sizes[:7] = 0.0
+    check(lengths, 2, 1, d, False, sizes, v_size=(10.0 ** (3 * t - 2))[:, None, None], qk_size=0.3)
+    check(lengths, 2, 2, d, True, sizes, v_size=(10.0 ** (3 * t - 2))[:, None, None], qk_size=0.3)
