@@ -37,7 +37,8 @@ struct PackedArgs {
   int part_rows = 0;            // most rows of a structure: tokens times heads of a group
   int pieces = 1;               // into which an item's walk is cut; each leaves its share in part_o (pieces, hq, nq, d) and part_ml, or
   float* share[3] = {};         // (reverse) in share: (pieces, rows, heads, d) of dq, dk, dv
-  // reverse pass of float16 on the tensor cores, else null: bits of the largest |g| and of sqrt(d) times the largest |v_jc| (structure, key head, 2), and |g| of every row (hq, nq)
+  // reverse pass of float16 on the tensor cores, else null: bits of the largest |g| and of sqrt(d) times the largest |v_jc| (structure, key head, 2),
+  // and |g| of every row (hq, nq)
   unsigned* largest = nullptr;
   float* size_g = nullptr;
   int structures = 0;

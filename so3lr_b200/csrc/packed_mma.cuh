@@ -13,8 +13,8 @@
 // CTAs hide each other's start); the tile of the other side is double-buffered by 16-byte asynchronous copies that fill rows and
 // columns that are not there with zeros.  The accumulator fragment of one product is the A fragment of the next, so P and dS never leave
 // the registers (and are rounded to the inputs' type on the way into the second product: their error then is that of one rounding of an
-// input; float16 takes a power of two out of both, see kHead, prob_shift and grad_shift).  float32 runs as three products of operands split into two tf32 numbers each (hi hi + hi lo + lo hi): 2^-21 of the
-// product, where a single tf32 product has 2^-11.
+// input; float16 takes a power of two out of both, see kHead, prob_shift and grad_shift).  float32 runs as three products of operands split into
+// two tf32 numbers each (hi hi + hi lo + lo hi): 2^-21 of the product, where a single tf32 product has 2^-11.
 #pragma once
 #include <atomic>
 

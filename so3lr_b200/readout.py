@@ -23,7 +23,8 @@ class StructureReadout(torch.nn.Module):
     heads x d: size of the attention (4 x 32, as the network's).  wavelengths: shortest and longest period of the rotation in Angstrom, over
     which the frequencies of each axis are spread geometrically.  Parameters are ordinary torch parameters on `device`, drawn from `seed`;
     the last layer starts at zero, so an untrained readout gives zero.  With 16-bit parameters (`.to(torch.bfloat16)`) or under autocast the
-    products and the attention run in that type; the frequencies stay float32, as the angles of far positions need them."""
+    products and the attention run in that type; the frequencies stay float32, as the angles of far positions need them.
+    The layouts of captured calls are kept as long as the readout lives: a graph reads their tables."""
 
     MAX_CACHED_LAYOUTS = 8
 
