@@ -559,6 +559,8 @@ def make_so3lr(lr_cutoff=12.0, dispersion_energy_cutoff_lr_damping=2.0, calculat
             n_graphs = int(gm_t.shape[0])
         if np.any(np.diff(bs_np) < 0):
             raise ValueError("batch_segments must be non-decreasing (atoms of one graph contiguous)")
+        if len(bs_np) != n or (n and not 0 <= bs_np[0] <= bs_np[-1] < n_graphs):      # they index arrays of n_graphs on the device
+            raise ValueError(f"batch_segments must hold the graphs (0 to {n_graphs - 1}) of {n} atoms, not {len(bs_np)} from {bs_np[:1]} to {bs_np[-1:]}")
         graph_start = np.searchsorted(bs_np, np.arange(n_graphs + 1)).astype(np.int32)
         s = pot.system_for(Z, graph_start=graph_start if n_graphs > 1 else None, total_charge=inputs.get("total_charge"),
                            num_unpaired=inputs.get("num_unpaired_electrons"))
